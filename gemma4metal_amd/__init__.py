@@ -4,6 +4,6 @@ of svv232/gemma4metal rebuilt as hand-written HIP behind a C ABI.
     from gemma4metal_amd import turboquant as tq
     out = tq.sdpa_int4(q, kq, ks, kb, vq, vs, vb, gqa_factor=2)
 """
-from . import turboquant  # noqa: F401
+from . import paged, turboquant  # noqa: F401
 
-__all__ = ["turboquant"]
+__all__ = ["paged", "turboquant"]

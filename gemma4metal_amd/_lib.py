@@ -50,6 +50,20 @@ SIGNATURES = {
     "tq_quantize_int4": (I, [P, I, I64, I, I, I, I, P, P, P, I, P]),
     "tq_kv_append_int4": (I, [P, P, I, P, P, P, P, P, P, I, I, I, I, I, P, I, I, P]),
     "tq_kv_append_int4_ring": (I, [P, P, I, P, P, P, P, P, P, I, I, I, I, I, P, I, I, P]),
+    "tq_kv_append_int4_paged": (I, [P, P, I, P, P, P, P, P, P, I, I, I, I, I, I, P, I, P, I, I, P]),
+    "tq_sdpa_int4_paged_workspace_size": (SZ, [I, I, I, I, I, I]),
+    "tq_sdpa_int4_paged": (I, [P, I, P, P, P, P, P, P, I, P, I, I, I, I, I, I, P, I, P, P, I, I, F, I,
+                               I, I, P, SZ, P]),
+    "tq_sdpa_int4_paged_prefill_workspace_size": (SZ, [I, I, I, I, I]),
+    "tq_sdpa_int4_paged_prefill": (I, [P, I, P, P, P, P, P, P, I, P, I, I, I, I, I, P, I, I, I, I, F,
+                                       I, I, P, SZ, P]),
+    "tq_kv_pages_workspace_size": (SZ, [I, I]),
+    "tq_kv_pages_reserve": (I, [P, P, P, P, P, I, I, I, I, P, SZ, P]),
+    "tq_kv_pages_fork": (I, [P, I, I, I, I, P, P, P, P, P, I, I, I, I, P, SZ, P]),
+    "tq_kv_pages_free": (I, [P, P, P, P, I, I, I, P]),
+    "tq_kv_pages_evict": (I, [P, P, P, P, I, I, I, I, I, I, P]),
+    "tq_kv_pages_compact": (I, [P, I, I, I, I, P, P, P, P, P, I, I, I, I, P, SZ, P]),
+    "tq_kv_pages_copy": (I, [P, I, I, I, I, I, I, P, P, I, P]),
     "tq_dequantize_int4": (I, [P, P, P, I, I64, I, P, P]),
     "tq_polar_quantize": (I, [P, P, P, P, I64, I, I, P, P, P, P, P, P]),
     "tq_polar_quantize_levels": (I, [P, P, P, P, I64, I, I, P, P, P, P, P, P]),

@@ -45,6 +45,20 @@ void clear_error();
 inline bool valid_dtype(int d) { return d == TQ_F32 || d == TQ_F16 || d == TQ_BF16; }
 inline size_t dtype_size(int d) { return d == TQ_F32 ? 4 : 2; }
 
+// Page geometry of the paged cache's entry points: page_size a power of two from
+// 32 (the attention kernels' block) to 1024, rows of a sequence below 2^31.
+inline int check_paging(int page_size, int num_pages, int max_pages, const char* fn) {
+  if (page_size < 32 || page_size > 1024 || (page_size & (page_size - 1)) != 0) {
+    set_error("%s: page_size must be a power of two from 32 to 1024 (got %d)", fn, page_size);
+    return TQ_ERR_UNSUPPORTED;
+  }
+  TQ_CHECK_ARG(num_pages >= 1 && num_pages <= (1 << 28) && max_pages >= 1,
+               "%s: need 1 <= num_pages <= 2^28 and max_pages >= 1", fn);
+  TQ_CHECK_ARG(static_cast<int64_t>(max_pages) * page_size < (int64_t{1} << 31),
+               "%s: max_pages * page_size must be below 2^31", fn);
+  return TQ_OK;
+}
+
 // ---- device-side helpers ---------------------------------------------------
 __device__ __forceinline__ float bf16_to_f32(uint16_t b) {
   return __uint_as_float(static_cast<uint32_t>(b) << 16);

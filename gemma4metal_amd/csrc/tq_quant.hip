@@ -30,6 +30,10 @@ struct QuantParams {
   int n_new;            // append: rows per (sequence, head)
   int cap;              // append: cache capacity (row stride per head)
   int ring;             // append: rows (pos[b] + t) mod cap, last cap rows of n_new only
+  // paged append: row r of sequence b is row r % 2^page_shift of page
+  // tables[b * max_pages + r / 2^page_shift] (cap = max_pages << page_shift)
+  const int32_t* tables;
+  int max_pages, num_pages, page_shift;
 };
 
 __device__ __forceinline__ void load8(const void* x, int dtype, int64_t off, float v[8]) {
@@ -58,7 +62,7 @@ __device__ __forceinline__ void load8(const void* x, int dtype, int64_t off, flo
 // What bounds it: HBM, once the VALU is out of the way -- eight correctly
 // rounded divisions a word and 64-bit index divisions made 65,536 rows of 256
 // fp32 values 19.0 us (4.0 TB/s).
-template <typename SB>
+template <typename SB, bool PAGED>
 __global__ __launch_bounds__(256) void quantize_int4_kernel(QuantParams p) {
   // every argument in one batch of scalar loads (one memory round trip),
   // the job picked by a select rather than a load indexed by blockIdx.y
@@ -66,6 +70,7 @@ __global__ __launch_bounds__(256) void quantize_int4_kernel(QuantParams p) {
                "s"(p.job[1].x), "s"(p.job[1].wq), "s"(p.job[1].s), "s"(p.job[1].b),
                "s"(p.x_dtype), "s"(p.words), "s"(p.dim), "s"(p.mode), "s"(p.pos), "s"(p.heads),
                "s"(p.n_new), "s"(p.cap), "s"(p.ring));
+  if constexpr (PAGED) asm volatile("" ::"s"(p.tables), "s"(p.max_pages), "s"(p.num_pages), "s"(p.page_shift));
   const QuantJob J = blockIdx.y ? p.job[1] : p.job[0];
   const int64_t gid = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;  // word of the input
   if (gid >= p.words) return;  // whole 8-lane groups leave together (words % 8 == 0)
@@ -145,15 +150,24 @@ __global__ __launch_bounds__(256) void quantize_int4_kernel(QuantParams p) {
       b = bh / p.heads;
     }
     const int t = static_cast<int>(row - bh * p.n_new);
-    int dst = p.pos[b] + t;
-    if (p.ring) {
-      // a ring keeps the newest cap rows: older rows of this append would
-      // land on the same slots, so they are not written at all
-      if (p.pos[b] < 0 || t < p.n_new - p.cap) return;
-      dst %= p.cap;
+    if constexpr (PAGED) {
+      const int64_t r = static_cast<int64_t>(p.pos[b]) + t;
+      if (r < 0 || r >= p.cap) return;
+      const int page = p.tables[b * p.max_pages + (r >> p.page_shift)];
+      if (static_cast<unsigned>(page) >= static_cast<unsigned>(p.num_pages)) return;
+      const int64_t first = (static_cast<int64_t>(page) * p.heads + (bh - b * p.heads)) << p.page_shift;
+      dw = gid + (first + (r & ((int64_t{1} << p.page_shift) - 1)) - row) * wpr;
+    } else {
+      int dst = p.pos[b] + t;
+      if (p.ring) {
+        // a ring keeps the newest cap rows: older rows of this append would
+        // land on the same slots, so they are not written at all
+        if (p.pos[b] < 0 || t < p.n_new - p.cap) return;
+        dst %= p.cap;
+      }
+      if (dst < 0 || dst >= p.cap) return;
+      dw = gid + (bh * p.cap + dst - row) * wpr;
     }
-    if (dst < 0 || dst >= p.cap) return;
-    dw = gid + (bh * p.cap + dst - row) * wpr;
   }
   J.wq[dw] = word;
   if ((gid & 7) == 0) {  // a row is a whole number of groups
@@ -202,10 +216,16 @@ int launch_quantize(const QuantParams& p, int jobs, int sb_dtype, hipStream_t st
     return TQ_ERR_INVALID;
   }
   dim3 grid(static_cast<unsigned>(blocks), jobs);
-  if (sb_dtype == TQ_F16)
-    quantize_int4_kernel<__half><<<grid, 256, 0, stream>>>(p);
-  else
-    quantize_int4_kernel<float><<<grid, 256, 0, stream>>>(p);
+  if (p.tables) {
+    if (sb_dtype == TQ_F16)
+      quantize_int4_kernel<__half, true><<<grid, 256, 0, stream>>>(p);
+    else
+      quantize_int4_kernel<float, true><<<grid, 256, 0, stream>>>(p);
+  } else if (sb_dtype == TQ_F16) {
+    quantize_int4_kernel<__half, false><<<grid, 256, 0, stream>>>(p);
+  } else {
+    quantize_int4_kernel<float, false><<<grid, 256, 0, stream>>>(p);
+  }
   TQ_CHECK_LAUNCH("quantize_int4_kernel");
   return TQ_OK;
 }
@@ -297,6 +317,50 @@ extern "C" int tq_kv_append_int4_ring(const void* k_new, const void* v_new, tq_d
   return kv_append(k_new, v_new, x_dtype, k_quant, k_scales, k_biases, v_quant, v_scales,
                    v_biases, sb_dtype, batch, num_kv_heads, head_dim, kv_capacity, positions,
                    n_new, mode, 1, stream, "tq_kv_append_int4_ring");
+}
+
+extern "C" int tq_kv_append_int4_paged(const void* k_new, const void* v_new, tq_dtype x_dtype,
+                                       uint32_t* k_quant, void* k_scales, void* k_biases,
+                                       uint32_t* v_quant, void* v_scales, void* v_biases,
+                                       tq_dtype sb_dtype, int batch, int num_kv_heads, int head_dim,
+                                       int page_size, int num_pages, const int32_t* block_tables,
+                                       int max_pages, const int32_t* positions, int n_new,
+                                       tq_quant_mode mode, void* stream) {
+  clear_error();
+  const char* fn = "tq_kv_append_int4_paged";
+  TQ_CHECK_ARG(valid_dtype(x_dtype), "%s: bad x_dtype", fn);
+  TQ_CHECK_ARG(sb_dtype == TQ_F16 || sb_dtype == TQ_F32, "%s: sb_dtype must be f16 or f32", fn);
+  TQ_CHECK_ARG(mode == TQ_QUANT_MLX || mode == TQ_QUANT_MINMAX, "%s: bad mode", fn);
+  TQ_CHECK_ARG(head_dim > 0 && head_dim % 64 == 0 && head_dim <= 4096,
+               "%s: head_dim must be a multiple of 64 <= 4096", fn);
+  TQ_CHECK_ARG(batch >= 0 && num_kv_heads > 0 && n_new >= 0, "%s: bad sizes", fn);
+  if (int r = check_paging(page_size, num_pages, max_pages, fn)) return r;
+  if (batch == 0 || n_new == 0) return TQ_OK;
+  TQ_CHECK_ARG(k_new && v_new && k_quant && k_scales && k_biases && v_quant && v_scales &&
+                   v_biases && positions && block_tables,
+               "%s: null pointer", fn);
+  if (int r = check_align(k_new, 16, "k_new")) return r;
+  if (int r = check_align(v_new, 16, "v_new")) return r;
+  for (const void* t : {static_cast<const void*>(k_quant), static_cast<const void*>(k_scales),
+                        static_cast<const void*>(k_biases), static_cast<const void*>(v_quant),
+                        static_cast<const void*>(v_scales), static_cast<const void*>(v_biases)})
+    if (int r = check_align(t, 16, "page tensors")) return r;
+  QuantParams p{};
+  p.job[0] = {k_new, k_quant, k_scales, k_biases};
+  p.job[1] = {v_new, v_quant, v_scales, v_biases};
+  p.x_dtype = x_dtype;
+  p.words = static_cast<int64_t>(batch) * num_kv_heads * n_new * (head_dim / 8);
+  p.dim = head_dim;
+  p.mode = mode;
+  p.pos = positions;
+  p.heads = num_kv_heads;
+  p.n_new = n_new;
+  p.cap = max_pages * page_size;
+  p.tables = block_tables;
+  p.max_pages = max_pages;
+  p.num_pages = num_pages;
+  p.page_shift = __builtin_ctz(static_cast<unsigned>(page_size));
+  return launch_quantize(p, 2, sb_dtype, static_cast<hipStream_t>(stream));
 }
 
 extern "C" int tq_dequantize_int4(const uint32_t* w_q, const void* scales, const void* biases,

@@ -75,6 +75,15 @@ struct SdpaParams {
   // ints between the split counters of consecutive (sequence, head) rows
   // (counter_stride of the launch's counter count, set on the host)
   int cnt_stride;
+  // Paged cache (tables != nullptr): row t of sequence b is row t % 2^page_shift
+  // of page tables[b * max_pages + (t >> page_shift)], and key t < n is attended
+  // iff it lies in the window or t < sinks.  Entries outside [0, num_pages) name
+  // no page.  Rows below `shared` are those of sequence 0's pages for every
+  // sequence.
+  const int* tables;
+  int max_pages, num_pages, page_shift;
+  int sinks;
+  int shared;
 };
 
 // Counter `c` of a launch with n counters in use sits at ws_cnt[c * stride]:

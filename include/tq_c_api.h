@@ -215,6 +215,149 @@ int tq_kv_append_int4_ring(const void* k_new, const void* v_new, tq_dtype x_dtyp
                            const int32_t* positions, int n_new, tq_quant_mode mode,
                            void* stream);
 
+/* ---- paged cache -----------------------------------------------------------
+ * No counterpart in the reference, whose cache is one growing array per layer
+ * (engine/gemma4_multilayer.cpp:230-249).  A pool of num_pages pages holds the
+ * rows of many sequences; each page is page_size rows (a power of two, 32 to
+ * 1024) of every kv head:
+ *   quant   uint32  [num_pages, num_kv_heads, page_size, D/8]
+ *   scales  f16|f32 [num_pages, num_kv_heads, page_size, D/64] (and biases)
+ * all six tensors 16-byte aligned.  Row t of sequence s lies in row t %
+ * page_size of page block_tables[s * max_pages + t / page_size]; the tables
+ * are DEVICE int32 arrays.  A table entry outside [0, num_pages) names no page:
+ * rows appended there are dropped, and keys there are not attended.
+ *
+ * tq_kv_append_int4_paged: tq_kv_append_int4 into pages: k_new / v_new [batch,
+ * num_kv_heads, n_new, head_dim] to rows positions[b] .. positions[b]+n_new-1
+ * of sequence b; rows outside [0, max_pages * page_size) are not written.
+ * Sequences must not share the pages they append to (tq_kv_pages_fork keeps
+ * it so). */
+int tq_kv_append_int4_paged(const void* k_new, const void* v_new, tq_dtype x_dtype,
+                            uint32_t* k_quant, void* k_scales, void* k_biases,
+                            uint32_t* v_quant, void* v_scales, void* v_biases, tq_dtype sb_dtype,
+                            int batch, int num_kv_heads, int head_dim, int page_size,
+                            int num_pages, const int32_t* block_tables, int max_pages,
+                            const int32_t* positions, int n_new, tq_quant_mode mode,
+                            void* stream);
+
+/* Batched decode attention over pages.  The query of sequence b stands at
+ * position n - 1, n = min(seq_lens[b], max_kv_len), and attends key t < n iff
+ *   W == 0  or  t >= n - W  or  t < num_sinks,
+ * W = windows[b] (windows == NULL: sliding_window): a sliding window with the
+ * first num_sinks tokens of the sequence kept visible.  A sequence with no
+ * attended key gives 0.
+ *   q [batch, num_heads, head_dim]; out [batch, num_heads, head_dim] f32, both
+ *   16-byte aligned; head_dim in {128, 256, 512}; num_heads == num_kv_heads *
+ *   gqa_factor; max_kv_len <= max_pages * page_size.
+ * shared_prefix (a multiple of page_size, <= max_kv_len): the first
+ * shared_prefix rows of every sequence lie in the same pages, those of
+ * sequence 0's table (the other tables' entries there are not read); they are
+ * attended once for the whole batch instead of once per sequence.  Sequences
+ * may be shorter than it.  It changes no result beyond rounding.
+ * Workspace as for tq_sdpa_int4_ragged: at least
+ * tq_sdpa_int4_paged_workspace_size(...) bytes, zero-filled once, left with its
+ * counters zeroed; calls that may overlap (two streams, or two captured graphs
+ * replayed at once) need one each. */
+size_t tq_sdpa_int4_paged_workspace_size(int batch, int num_heads, int num_kv_heads,
+                                         int head_dim, int max_kv_len, int shared_prefix);
+int tq_sdpa_int4_paged(const void* q, tq_dtype q_dtype,
+                       const uint32_t* k_quant, const void* k_scales, const void* k_biases,
+                       const uint32_t* v_quant, const void* v_scales, const void* v_biases,
+                       tq_dtype sb_dtype, float* out,
+                       int batch, int num_heads, int num_kv_heads, int head_dim,
+                       int page_size, int num_pages, const int32_t* block_tables, int max_pages,
+                       const int32_t* seq_lens, const int32_t* windows, int max_kv_len,
+                       int gqa_factor, float scale, int sliding_window, int num_sinks,
+                       int shared_prefix, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Prompt (multi-query) attention of one sequence over pages: tq_sdpa_int4_prefill
+ * with block_table [max_pages] of that sequence and num_sinks.  Query i at
+ * position n_prior + i attends key t <= n_prior + i iff sliding_window == 0 or
+ * n_prior + i - t < sliding_window or t < num_sinks; the new rows must already
+ * be appended.  n_prior + n_new <= max_pages * page_size.  Workspace:
+ * tq_sdpa_int4_paged_prefill_workspace_size(...) bytes, zero-filled once. */
+size_t tq_sdpa_int4_paged_prefill_workspace_size(int num_heads, int num_kv_heads, int head_dim,
+                                                 int n_prior, int n_new);
+int tq_sdpa_int4_paged_prefill(const void* q, tq_dtype q_dtype,
+                               const uint32_t* k_quant, const void* k_scales, const void* k_biases,
+                               const uint32_t* v_quant, const void* v_scales, const void* v_biases,
+                               tq_dtype sb_dtype, float* out,
+                               int num_heads, int num_kv_heads, int head_dim,
+                               int page_size, int num_pages, const int32_t* block_table,
+                               int max_pages, int n_prior, int n_new, int gqa_factor, float scale,
+                               int sliding_window, int num_sinks,
+                               void* workspace, size_t workspace_bytes, void* stream);
+
+/* Page management.  All state is on the device, so that these calls can be
+ * captured into a HIP graph: block_tables int32 [num_seqs, max_pages] (-1 = no
+ * page), lengths int32 [num_seqs], refs int32 [num_pages] = the number of table
+ * entries that name a page (<= 0: free).  granted int32 [num_seqs] is written:
+ * 1 where the sequence's request was carried out, 0 where there was none or
+ * it was refused (its state is then left as it was).  Requests are served in
+ * sequence order; once the free pages do not suffice for one, no later request
+ * that needs a page is granted.  Free pages are taken lowest first, so results do not depend
+ * on timing.
+ *
+ * The six page tensors of num_layers layers that share the tables are passed
+ * as a HOST array pages[6] (k_quant, k_scales, k_biases, v_quant, v_scales,
+ * v_biases), each [num_layers, num_pages, num_kv_heads, page_size, .].
+ *
+ * workspace: tq_kv_pages_workspace_size(...) bytes, 16-byte aligned; need not
+ * be zeroed; calls that may overlap need one each. */
+size_t tq_kv_pages_workspace_size(int num_seqs, int num_pages);
+
+/* Gives sequence s (n_new[s] > 0; n_new DEVICE int32 [num_seqs]) the pages that
+ * rows lengths[s] .. lengths[s] + n_new[s] - 1 need and it lacks.  Refused too
+ * when they exceed max_pages. */
+int tq_kv_pages_reserve(int32_t* block_tables, int32_t* refs, const int32_t* lengths,
+                        const int32_t* n_new, int32_t* granted, int num_seqs, int max_pages,
+                        int num_pages, int page_size, void* workspace, size_t workspace_bytes,
+                        void* stream);
+
+/* Makes sequence s a continuation of sequence parents[s] (DEVICE int32
+ * [num_seqs]; negative = none): the parent's full pages are shared, and its
+ * last page, where partly filled, is copied to a page of s's own, so that both
+ * can append.  lengths[s] = the parent's.  Refused when s is not empty (a
+ * length or a page), when parents[s] is s, >= num_seqs or itself being forked
+ * into.  pages, num_layers, num_kv_heads, head_dim, sb_dtype as above. */
+int tq_kv_pages_fork(void* const* pages, tq_dtype sb_dtype, int num_layers, int num_kv_heads,
+                     int head_dim, int32_t* block_tables, int32_t* refs, int32_t* lengths,
+                     const int32_t* parents, int32_t* granted, int num_seqs, int max_pages,
+                     int num_pages, int page_size, void* workspace, size_t workspace_bytes,
+                     void* stream);
+
+/* Ends the sequences with which[s] != 0 (DEVICE int32 [num_seqs]): their pages
+ * lose a reference, their table rows become -1 and their lengths 0. */
+int tq_kv_pages_free(int32_t* block_tables, int32_t* refs, int32_t* lengths, const int32_t* which,
+                     int num_seqs, int max_pages, int num_pages, void* stream);
+
+/* Gives up the pages of which no row is visible any more under sliding_window
+ * (> 0) and num_sinks: those wholly in rows [num_sinks, lengths[s] -
+ * sliding_window) of the sequences with which[s] != 0 (which == NULL: all).
+ * Their entries become -1; lengths stay. */
+int tq_kv_pages_evict(int32_t* block_tables, int32_t* refs, const int32_t* lengths,
+                      const int32_t* which, int num_seqs, int max_pages, int num_pages,
+                      int page_size, int sliding_window, int num_sinks, void* stream);
+
+/* Moves the pages in use to the front of the pool: of n pages in use, the k-th
+ * free place below n takes the k-th page at or above it.  Tables and reference
+ * counts are written to tables_out / refs_out (either may be its input) and n
+ * to live_out [1]; entries that name a page not in use become -1, negative ones
+ * and those >= num_pages stay. */
+int tq_kv_pages_compact(void* const* pages, tq_dtype sb_dtype, int num_layers, int num_kv_heads,
+                        int head_dim, const int32_t* block_tables, const int32_t* refs,
+                        int32_t* tables_out, int32_t* refs_out, int32_t* live_out, int num_seqs,
+                        int max_pages, int num_pages, int page_size, void* workspace,
+                        size_t workspace_bytes, void* stream);
+
+/* Copies page src[i] to page dst[i] (DEVICE int32 [n]) in every tensor and
+ * layer; pairs with a page outside [0, num_pages) or src[i] == dst[i] are
+ * skipped.  No page may be the destination of two pairs, or of one and the
+ * source of another. */
+int tq_kv_pages_copy(void* const* pages, tq_dtype sb_dtype, int num_layers, int num_kv_heads,
+                     int head_dim, int num_pages, int page_size, const int32_t* src,
+                     const int32_t* dst, int n, void* stream);
+
 /* Dequantize rows (for the engine's prefill fallback,
  * engine/gemma4_multilayer.cpp:307-308): out[r, d] = s*nibble + b as f32. */
 int tq_dequantize_int4(const uint32_t* w_q, const void* scales, const void* biases,
