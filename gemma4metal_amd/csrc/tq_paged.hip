@@ -12,7 +12,7 @@ namespace {
 // A wave per (query, head) row: lane i holds dims i E .. i E + E - 1, E = D / 64,
 // and walks the row's keys one by one with a running maximum and sum.
 template <int D, typename SB>
-__global__ __launch_bounds__(256) void paged_rows_kernel(SdpaParams p, int64_t rows) {
+__global__ __launch_bounds__(256) void paged_rows_kernel(PagedParams p, int64_t rows) {
   constexpr int E = D / 64;
   const int lane = threadIdx.x & 63;
   const int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
@@ -54,7 +54,7 @@ __global__ __launch_bounds__(256) void paged_rows_kernel(SdpaParams p, int64_t r
 }
 
 template <int D>
-int launch_rows(const SdpaParams& p, int sb_dtype, int64_t rows, hipStream_t s) {
+int launch_rows(const PagedParams& p, int sb_dtype, int64_t rows, hipStream_t s) {
   const unsigned grid = static_cast<unsigned>((rows + 3) / 4);
   if (sb_dtype == TQ_F16) paged_rows_kernel<D, __half><<<grid, 256, 0, s>>>(p, rows);
   else paged_rows_kernel<D, float><<<grid, 256, 0, s>>>(p, rows);
@@ -63,7 +63,7 @@ int launch_rows(const SdpaParams& p, int sb_dtype, int64_t rows, hipStream_t s) 
 }
 
 // What both calls refuse; fills the parameters that they share.
-int paged_params(SdpaParams& p, const void* q, int q_dtype, const uint32_t* kq, const void* ks, const void* kb,
+int paged_params(PagedParams& p, const void* q, int q_dtype, const uint32_t* kq, const void* ks, const void* kb,
                  const uint32_t* vq, const void* vs, const void* vb, int sb_dtype, float* out, int batch, int Hq,
                  int Hkv, int D, int page_size, int num_pages, const int32_t* tables, int max_pages, int gqa,
                  float scale, int window, int sinks, const char* fn) {
@@ -103,7 +103,46 @@ int paged_params(SdpaParams& p, const void* q, int q_dtype, const uint32_t* kq, 
   return TQ_OK;
 }
 
-int launch_any(const SdpaParams& p, int D, int sb_dtype, int64_t rows, hipStream_t s) {
+// Kernel and split plan of a decode call: sdpa_int4_hc2_kernel for D 512 with
+// GQA a multiple of 8, else sdpa_int4_mfma_kernel, on blocks of 32 keys.
+struct PagedPlan {
+  bool hc;
+  int G, n_sub, chunk, max_splits;
+  bool lpt;
+  WsLayout wl;
+};
+
+// max_len: what any sequence attends beside the shared rows, at most.
+PagedPlan plan_paged(int batch, int Hq, int Hkv, int D, int sb_dtype, int max_len) {
+  PagedPlan pl{};
+  const int gqa = Hq / Hkv;
+  pl.hc = D == 512 && gqa % 8 == 0;
+  pl.G = head_subgroup(gqa);
+  while (!pl.hc && pl.G > 1 && !mfma_serves(D, pl.G, sb_dtype)) pl.G /= 2;
+  pl.n_sub = gqa / pl.G;
+  const int64_t groups = static_cast<int64_t>(batch) * Hkv * pl.n_sub;
+  const int len = static_cast<int>(std::min<int64_t>((static_cast<int64_t>(max_len) + 31) / 32 * 32, 0x7FFFFFE0));
+  const int min_splits = min_splits_for(batch);
+  pl.chunk = (plan_chunk(len, groups, min_splits) + 31) / 32 * 32;
+  pl.max_splits = max_splits_bound(len, groups, min_splits);
+  // the device chooses the chunk (see plan_sdpa)
+  pl.lpt = batch <= 64 && !pl.hc;
+  if (pl.lpt && groups >= 2 * static_cast<int64_t>(target_wgs()) && pl.max_splits > 2) {
+    pl.max_splits = 2;
+    pl.chunk = std::max(pl.chunk, ((len + 1) / 2 + 127) / 128 * 128);
+  }
+  pl.wl = ws_layout(batch, Hq, D, pl.max_splits);
+  return pl;
+}
+
+// Keys a sequence attends at most, in whole blocks.
+int attended_bound(int max_kv_len, int window, bool windows, int sinks) {
+  if (windows || window == 0) return max_kv_len;
+  const int64_t most = static_cast<int64_t>(window) + 62 + (static_cast<int64_t>(sinks) + 31) / 32 * 32;
+  return static_cast<int>(std::min<int64_t>(most, max_kv_len));
+}
+
+int launch_any(const PagedParams& p, int D, int sb_dtype, int64_t rows, hipStream_t s) {
   if (D == 128) return launch_rows<128>(p, sb_dtype, rows, s);
   if (D == 256) return launch_rows<256>(p, sb_dtype, rows, s);
   return launch_rows<512>(p, sb_dtype, rows, s);
@@ -116,7 +155,11 @@ using namespace tq;
 
 extern "C" size_t tq_sdpa_int4_paged_workspace_size(int batch, int num_heads, int num_kv_heads, int head_dim,
                                                     int max_kv_len, int shared_prefix) {
-  return 0;
+  if (batch < 1 || num_kv_heads < 1 || num_heads < num_kv_heads || max_kv_len < 0 || shared_prefix < 0) return 0;
+  // (every plan of a call with these sizes: a window only shortens the splits)
+  const int gqa = num_heads / num_kv_heads;
+  const int64_t groups = static_cast<int64_t>(batch) * num_kv_heads * (gqa / head_subgroup(gqa));
+  return ws_layout(batch, num_heads, head_dim, max_splits_bound(max_kv_len, groups, min_splits_for(batch))).total;
 }
 
 extern "C" int tq_sdpa_int4_paged(const void* q, tq_dtype q_dtype, const uint32_t* k_quant, const void* k_scales,
@@ -131,7 +174,7 @@ extern "C" int tq_sdpa_int4_paged(const void* q, tq_dtype q_dtype, const uint32_
   const char* fn = "tq_sdpa_int4_paged";
   TQ_CHECK_ARG(batch >= 0 && batch <= 65535, "%s: batch must be 0 to 65535", fn);
   if (batch == 0) return TQ_OK;
-  SdpaParams p{};
+  PagedParams p{};
   if (int r = paged_params(p, q, q_dtype, k_quant, k_scales, k_biases, v_quant, v_scales, v_biases, sb_dtype, out,
                            batch, num_heads, num_kv_heads, head_dim, page_size, num_pages, block_tables, max_pages,
                            gqa_factor, scale, sliding_window, num_sinks, fn))
@@ -146,7 +189,37 @@ extern "C" int tq_sdpa_int4_paged(const void* q, tq_dtype q_dtype, const uint32_
   p.windows = windows;
   p.n_clamp = max_kv_len;
   p.shared = shared_prefix;
-  return launch_any(p, head_dim, sb_dtype, static_cast<int64_t>(batch) * num_heads, static_cast<hipStream_t>(stream));
+  if (shared_prefix > 0)
+    return launch_any(p, head_dim, sb_dtype, static_cast<int64_t>(batch) * num_heads, static_cast<hipStream_t>(stream));
+  const PagedPlan pl = plan_paged(batch, num_heads, num_kv_heads, head_dim, sb_dtype,
+                                  attended_bound(max_kv_len, sliding_window, windows != nullptr, num_sinks));
+  TQ_CHECK_ARG(num_kv_heads * static_cast<int64_t>(pl.n_sub) <= 65535, "%s: grid too large", fn);
+  TQ_CHECK_ARG(static_cast<int64_t>(batch) * num_heads <= kMaxCounters, "%s: batch * num_heads must be <= %lld", fn,
+               static_cast<long long>(kMaxCounters));
+  p.n_sub = pl.n_sub;
+  p.chunk = pl.chunk;
+  p.max_splits = pl.max_splits;
+  p.lpt = pl.lpt ? 1 : 0;
+  if (pl.max_splits > 1) {
+    if (!workspace || workspace_bytes < pl.wl.total) {
+      set_error("%s: workspace of %zu bytes needed (got %zu)", fn, pl.wl.total, workspace_bytes);
+      return TQ_ERR_WORKSPACE;
+    }
+    TQ_CHECK_ARG(reinterpret_cast<uintptr_t>(workspace) % 16 == 0, "%s: workspace must be 16-byte aligned", fn);
+    // the split partials are addressed with 32-bit byte offsets
+    TQ_CHECK_ARG(pl.wl.total - pl.wl.o_off < (size_t{1} << 31), "%s: split-K partials exceed 2 GiB", fn);
+    char* ws = static_cast<char*>(workspace);
+    p.ws_cnt = reinterpret_cast<int*>(ws + pl.wl.cnt_off);
+    p.ws_ml = reinterpret_cast<float*>(ws + pl.wl.ml_off);
+    p.ws_o = reinterpret_cast<float*>(ws + pl.wl.o_off);
+  }
+  const dim3 grid(pl.max_splits, num_kv_heads * pl.n_sub, batch);
+  p.cnt_stride = counter_stride(static_cast<int64_t>(batch) * num_heads);
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (!pl.hc) return launch_sdpa_mfma(p, head_dim, pl.G, sb_dtype, grid, s);
+  p.ext_merge = pl.max_splits > 1 ? 1 : 0;
+  const int r = launch_sdpa_hc(p, sb_dtype, grid, s);
+  return r != TQ_OK || !p.ext_merge ? r : launch_merge_splits(p, head_dim, batch, s);
 }
 
 extern "C" size_t tq_sdpa_int4_paged_prefill_workspace_size(int num_heads, int num_kv_heads, int head_dim,
@@ -165,7 +238,7 @@ extern "C" int tq_sdpa_int4_paged_prefill(const void* q, tq_dtype q_dtype, const
   const char* fn = "tq_sdpa_int4_paged_prefill";
   TQ_CHECK_ARG(n_prior >= 0 && n_new >= 0, "%s: n_prior and n_new must be >= 0", fn);
   if (n_new == 0) return TQ_OK;
-  SdpaParams p{};
+  PagedParams p{};
   if (int r = paged_params(p, q, q_dtype, k_quant, k_scales, k_biases, v_quant, v_scales, v_biases, sb_dtype, out,
                            n_new, num_heads, num_kv_heads, head_dim, page_size, num_pages, block_table, max_pages,
                            gqa_factor, scale, sliding_window, num_sinks, fn))

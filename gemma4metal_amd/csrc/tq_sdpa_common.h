@@ -8,6 +8,7 @@
 #include <math.h>
 
 #include <algorithm>
+#include <type_traits>
 
 // The split-K completion protocol below (Finalize::run: relaxed agent-scope
 // partial stores and loads, one relaxed counter atomic, no L2 write-back or
@@ -75,16 +76,22 @@ struct SdpaParams {
   // ints between the split counters of consecutive (sequence, head) rows
   // (counter_stride of the launch's counter count, set on the host)
   int cnt_stride;
-  // Paged cache (tables != nullptr): row t of sequence b is row t % 2^page_shift
-  // of page tables[b * max_pages + (t >> page_shift)], and key t < n is attended
-  // iff it lies in the window or t < sinks.  Entries outside [0, num_pages) name
-  // no page.  Rows below `shared` are those of sequence 0's pages for every
-  // sequence.
+};
+
+// Paged cache: row t of sequence b is row t % 2^page_shift of page tables[b *
+// max_pages + (t >> page_shift)], and key t < n is attended iff it lies in the
+// window or t < sinks.  Entries outside [0, num_pages) name no page.
+struct PagedParams : SdpaParams {
   const int* tables;
   int max_pages, num_pages, page_shift;
   int sinks;
-  int shared;
+  int shared;  // rows of every sequence that lie in sequence 0's pages
+  // Partials of every row that lie before a launch's own splits (those of the
+  // shared rows), joined with them.
+  int pre;
 };
+template <bool PG>
+using ParamsOf = typename std::conditional<PG, PagedParams, SdpaParams>::type;
 
 // Counter `c` of a launch with n counters in use sits at ws_cnt[c * stride]:
 // up to 32 ints (one 128 B line) from its neighbours, as far as the counter
@@ -133,6 +140,42 @@ __device__ __forceinline__ SplitRange split_range(const SdpaParams& p, int b, in
   return r;
 }
 
+// A paged sequence's keys as blocks of 32 (a page is a whole number of them),
+// without those of which no key is attended: the blocks that hold sinks, then
+// those of the window.  Splits are ranges of this list; block v of it is block
+// `block(v)` of the sequence.
+struct PagedKeys {
+  int n;      // keys are attended below n ...
+  int lo;     // ... from lo on, or below p.sinks
+  int first;  // first block (of the rows behind the shared ones)
+  int ns;     // blocks in front of the gap
+  int skip;   // blocks in the gap
+  int nb;     // blocks of the list
+  __device__ __forceinline__ int block(int v) const { return first + v + (v < ns ? 0 : skip); }
+};
+
+__device__ __forceinline__ PagedKeys paged_keys(const PagedParams& p, int seq_len, int W, int shared) {
+  PagedKeys k;
+  k.n = max(min(seq_len, p.n_clamp), 0);
+  k.lo = W > 0 ? max(0, k.n - W) : 0;
+  k.first = shared >> 5;
+  const int end = (k.n + 31) >> 5;
+  // (a key count near 2^31: no + 31)
+  k.ns = max(min((p.sinks >> 5) + ((p.sinks & 31) != 0), end) - k.first, 0);
+  k.skip = max((k.lo >> 5) - k.first - k.ns, 0);
+  k.nb = max(end - k.first - k.skip, 0);
+  return k;
+}
+
+// The split of a paged sequence, in keys of its list.
+__device__ __forceinline__ SplitRange paged_range(const SdpaParams& p, const PagedKeys& k, int split) {
+  SplitRange r;
+  r.S = k.nb > 0 ? (32 * k.nb + p.chunk - 1) / p.chunk : 1;
+  r.t_begin = split * p.chunk;
+  r.t_end = min(r.t_begin + p.chunk, 32 * k.nb);
+  return r;
+}
+
 // Job of a workgroup in a ragged launch with p.lpt set (at most 64
 // sequences).
 // - The chunk is chosen here, from the actual lengths (the host knows only
@@ -161,7 +204,8 @@ __device__ __forceinline__ int wave_max_i(int v) {
   return v;
 }
 
-__device__ __forceinline__ bool ragged_job(const SdpaParams& p, int& b, int& hy, int& split, int& chunk) {
+template <bool PG = false>
+__device__ __forceinline__ bool ragged_job(const ParamsOf<PG>& p, int& b, int& hy, int& split, int& chunk) {
   const int lane = threadIdx.x & 63;
   const int H = static_cast<int>(gridDim.y);
   const int64_t wg = blockIdx.x + static_cast<int64_t>(gridDim.x) * (blockIdx.y + static_cast<int64_t>(gridDim.y) * blockIdx.z);
@@ -169,7 +213,8 @@ __device__ __forceinline__ bool ragged_job(const SdpaParams& p, int& b, int& hy,
   const int n_b = mine ? min(p.seq_lens[lane], p.n_clamp) : 0;
   const int W = mine ? (p.windows ? p.windows[lane] : p.window) : 0;
   const int lo = W > 0 ? max(0, n_b - W) : 0;
-  const int len = max(n_b - lo, 0);
+  int len = max(n_b - lo, 0);
+  if constexpr (PG) len = 32 * paged_keys(p, n_b, W, p.shared).nb;
   // ---- chunk: candidates k = 1 .. max_splits, one wave-wide job count each
   const int lmax = wave_max_i(len);
   const float keys = static_cast<float>(wave_sum_dpp(len)) * H;
@@ -412,9 +457,15 @@ struct Finalize {
   // exp2 per lane, not one per output and partial), the denominator is a
   // lane reduction, and each output then takes one FMA per partial with f_k
   // read back as a scalar.
-  __device__ static void run(const SdpaParams& p, float* arena, int64_t head_base, int S,
+  //
+  // PRE: p.pre partials of every row lie in its first slots, written by an
+  // earlier launch; this one's follow them and are merged together with them.
+  template <bool PRE = false>
+  __device__ static void run(const ParamsOf<PRE>& p, float* arena, int64_t head_base, int S,
                              int split, int counter, int gh = G, int64_t qstride = 0,
                              int nvalid = G) {
+    int pre = 0;
+    if constexpr (PRE) pre = p.pre;
     static_assert(D % 64 == 0, "one head per wave");
     static_assert(NW <= 16, "per-wave partials fit one row of 16 lanes");
     // A thread takes VEC consecutive dims of one head: the arena rows are
@@ -492,16 +543,16 @@ struct Finalize {
           for (int e = 0; e < VEC; ++e) O[e] = fmaf(v[e], fk, O[e]);
         }
       }
-      if (S == 1) {
+      if (S == 1 && pre == 0) {
 #pragma unroll
         for (int e = 0; e < VEC; ++e) p.out[row(h) * D + d + e] = normalise(O[e], Ls, p.denom_eps);
       } else {
-        const int64_t slot = row(h) * p.max_splits + split;
+        const int64_t slot = row(h) * p.max_splits + split + pre;
         CV::store(wso, static_cast<uint32_t>((slot * D + d) * 4), O);
         if (d == 0) store_coherent_pair(p.ws_ml + slot * 2, M, Ls);
       }
     }
-    if (S == 1 || p.ext_merge) return;
+    if ((S == 1 && pre == 0) || p.ext_merge) return;
 
     // The last workgroup of this (sequence, kv head, subgroup) to finish merges
     // the splits.  Partials are written with agent-scope stores (write-through
@@ -526,6 +577,7 @@ struct Finalize {
     }
     __syncthreads();
     if (!s_last) return;
+    S += pre;
 
     // Merge, KC splits at a time: lane k (mod 16) loads split s0 + k's
     // (m, l), and every thread the KC partial vectors of its units.  All
@@ -665,9 +717,12 @@ bool prefill_tiles_serve(int D, int sb_dtype, int gqa);
 // a tq_status error, or -1 when (D, G) is not served by that kernel.
 int launch_sdpa_mfma(const SdpaParams& p, int D, int G, int sb_dtype, dim3 grid,
                      hipStream_t stream);
+int launch_sdpa_mfma(const PagedParams& p, int D, int G, int sb_dtype, dim3 grid,
+                     hipStream_t stream);
 // D = 512, 8 query heads per workgroup (heads as matrix-core columns), fp16
 // scale/bias: tq_sdpa_hc.hip.
 int launch_sdpa_hc(const SdpaParams& p, int sb_dtype, dim3 grid, hipStream_t stream);
+int launch_sdpa_hc(const PagedParams& p, int sb_dtype, dim3 grid, hipStream_t stream);
 // Prefill with K/V tiles shared by 32 or 64 (query, head) rows (tq_prefill.hip);
 // -1 when the shape is not served (D other than 128 / 256 / 512, gqa not
 // dividing 64).
@@ -677,5 +732,6 @@ int launch_prefill_tiles_f32(const SdpaParams& p, int D, int sb_dtype, hipStream
 // Merge of the split partials of a launch with ext_merge = 1 (batch b of
 // grid.y): tq_sdpa_hc.hip.
 int launch_merge_splits(const SdpaParams& p, int D, int batch, hipStream_t stream);
+int launch_merge_splits(const PagedParams& p, int D, int batch, hipStream_t stream);
 
 }  // namespace tq

@@ -36,6 +36,8 @@
 //   V A-operand row m of block blk: word 16 blk + m.
 // Four waves, one per SIMD (the P.V accumulators of 8 heads x 512 dims take
 // 128 registers); loads double-buffered one 32-key iteration ahead.
+#include <type_traits>
+
 #include "tq_sdpa_common.h"
 
 namespace tq {
@@ -60,13 +62,15 @@ struct HcBuf {
   u32x4 sc[2][1];      // scales of array c for keys 2m, 2m+1 (8 fp16 each)
 };
 
+// (R: int, or int64_t for rows of a page pool.)
 // Loads of the 32 keys at t0 (rows clamped to `last`, the uniform limit
 // `lim` = last - t0 >= 0), non-temporal, uniform base + 32-bit lane offset:
 // K words, the scale arrays and the V words, as separate parts.
 // K words: one 16-byte load per (tile, pair P): lane group c takes words
 // 16 P + 4c .. + 3 of its key (group 2P + c / 2, half c % 2 of it), so the 4
 // lane groups of a row read its 64 bytes of the pair contiguously.
-__device__ __forceinline__ void hc_load_kw_pair(uint32_t (&kw)[2][16], const char* kq, int t0, int lim, int m,
+template <typename R>
+__device__ __forceinline__ void hc_load_kw_pair(uint32_t (&kw)[2][16], const char* kq, R t0, int lim, int m,
                                                 int c, int P) {
   const char* kb = kq + static_cast<int64_t>(t0) * kHcRB;
 #pragma unroll
@@ -80,15 +84,16 @@ __device__ __forceinline__ void hc_load_kw_pair(uint32_t (&kw)[2][16], const cha
   }
 }
 
-__device__ __forceinline__ void hc_load_kw(uint32_t (&kw)[2][16], const char* kq, int t0, int lim, int m, int c) {
+template <typename R>
+__device__ __forceinline__ void hc_load_kw(uint32_t (&kw)[2][16], const char* kq, R t0, int lim, int m, int c) {
 #pragma unroll
   for (int P = 0; P < 4; ++P) hc_load_kw_pair(kw, kq, t0, lim, m, c, P);
 }
 
 // Scale array of lane group c (k scale, k bias, v scale, v bias) for keys
 // 2m, 2m + 1: 8 groups per key, fp16 (4 words per key) or fp32 (8 words).
-template <bool F32>
-__device__ __forceinline__ void hc_load_sc(u32x4 (&scw)[2][F32 ? 2 : 1], const char* sc, int t0, int lim,
+template <bool F32, typename R>
+__device__ __forceinline__ void hc_load_sc(u32x4 (&scw)[2][F32 ? 2 : 1], const char* sc, R t0, int lim,
                                            int m) {
   constexpr int RB = F32 ? 32 : 16;  // scale bytes per key
   const char* sb = sc + static_cast<int64_t>(t0) * RB;
@@ -124,7 +129,8 @@ __device__ __forceinline__ void hc_load_v(uint32_t (&vw)[8][4], const char* vq, 
 // 16 T + 4c + i, so a quad of lanes reads 4 keys x 16 contiguous bytes.
 // hc_quad_transpose then gives lane i of the quad word 16 blk + 4 qd + i of
 // keys 16 T + 4c + 0 .. 3: the slots 4T .. 4T + 3 of hc_load_v's layout.
-__device__ __forceinline__ void hc_load_v4_blk(u32x4 (&vr)[2][4], const char* vq, int t0, int lim, int m, int c,
+template <typename R>
+__device__ __forceinline__ void hc_load_v4_blk(u32x4 (&vr)[2][4], const char* vq, R t0, int lim, int m, int c,
                                                int blk) {
   const char* vb = vq + static_cast<int64_t>(t0) * kHcRB;
 #pragma unroll
@@ -134,7 +140,8 @@ __device__ __forceinline__ void hc_load_v4_blk(u32x4 (&vr)[2][4], const char* vq
   }
 }
 
-__device__ __forceinline__ void hc_load_v4(u32x4 (&vr)[2][4], const char* vq, int t0, int lim, int m, int c) {
+template <typename R>
+__device__ __forceinline__ void hc_load_v4(u32x4 (&vr)[2][4], const char* vq, R t0, int lim, int m, int c) {
 #pragma unroll
   for (int blk = 0; blk < 4; ++blk) hc_load_v4_blk(vr, vq, t0, lim, m, c, blk);
 }
@@ -587,9 +594,11 @@ constexpr int kHs = 4;  // key streams (producer / consumer pairs)
 
 // F32: fp32 scale/bias (8 words per key in each array instead of 4); the
 // producer's scale registers and LDS stage double, nothing else changes.
-template <bool F32>
+// PG: paged cache, as in sdpa_int4_mfma_kernel: steps are blocks of the
+// sequence's PagedKeys list, their page numbers held 64 steps ahead in the lanes.
+template <bool F32, bool PG = false>
 __global__ __launch_bounds__(2 * kHs * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
-void sdpa_int4_hc2_kernel(SdpaParams p) {
+void sdpa_int4_hc2_kernel(ParamsOf<PG> p) {
   pin_args(p);
   constexpr int NS = kHs, NWV = 2 * kHs, D = kHcD, G = kHcG, NG = kHcNG;
   constexpr int kNT = NWV * 64;
@@ -602,7 +611,9 @@ void sdpa_int4_hc2_kernel(SdpaParams p) {
   const int kvh = hy / p.n_sub, sub = hy - kvh * p.n_sub;
   const int h0 = kvh * p.gqa + sub * G;
 
-  const SplitRange rg = split_range(p, b, split);
+  PagedKeys pk{};
+  if constexpr (PG) pk = paged_keys(p, p.seq_lens[b], p.windows ? p.windows[b] : p.window, p.shared);
+  const SplitRange rg = PG ? paged_range(p, pk, split) : split_range(p, b, split);
   if (split >= rg.S) return;
   const int t_end = rg.t_end;
 
@@ -625,7 +636,7 @@ void sdpa_int4_hc2_kernel(SdpaParams p) {
   __shared__ float sh_qhat[G][NG];
   __shared__ int sh_F[G];
 
-  const int64_t row0 = (static_cast<int64_t>(cache_batch(p, b)) * p.Hkv + kvh) * p.cap;
+  const int64_t row0 = PG ? 0 : (static_cast<int64_t>(cache_batch(p, b)) * p.Hkv + kvh) * p.cap;
   const char* kq_rows = reinterpret_cast<const char*>(p.kq + row0 * (D / 8));
   const char* vq_rows = reinterpret_cast<const char*>(p.vq + row0 * (D / 8));
   const void* sc_base = c == 0 ? p.ks : (c == 1 ? p.kb : (c == 2 ? p.vs : p.vb));
@@ -642,6 +653,44 @@ void sdpa_int4_hc2_kernel(SdpaParams p) {
   const int last = t_end - 1;
   const int safe_last = max(last, 0);
   auto tclamp = [&](int t0) { return min(t0, safe_last); };
+  // PG: page numbers of steps st .. st + 63 in the lanes (past the list's end the
+  // last one's, -1 where the list is empty), and a step's block.
+  int pages = -1;
+  auto load_pages = [&](int st) {
+    if constexpr (PG) {
+      if (pk.nb > 0) {
+        const int v = min(((base0 + st * kIter) >> 5) + (lane * kIter >> 5), pk.nb - 1);
+        pages = p.tables[static_cast<int64_t>(b) * p.max_pages + (pk.block(v) >> (p.page_shift - 5))];
+      }
+    }
+  };
+  struct Block {
+    typename std::conditional<PG, int64_t, int>::type row;  // first row: of the head, or of the pool
+    int lim;      // last row to read, from there
+    int key;      // PG: its first key
+    bool has;     // PG: it lies in the split, and its page exists
+  };
+  auto block_at = [&](int st) {
+    const int t0 = base0 + st * kIter;
+    Block r{};
+    if constexpr (PG) {
+      if (st != 0 && (st & 63) == 0) {  // waited for in here: the steady loop waits for nothing
+        load_pages(st);
+        asm volatile("" : "+v"(pages));
+      }
+      const int e = __builtin_amdgcn_readlane(pages, st & 63);
+      const bool in = static_cast<unsigned>(e) < static_cast<unsigned>(p.num_pages);
+      const int v = min(t0 >> 5, max(pk.nb - 1, 0));
+      r.has = in && t0 < t_end;
+      r.key = 32 * pk.block(v);
+      r.row = ((static_cast<int64_t>(in ? e : 0) * p.Hkv + kvh) << p.page_shift) + (r.key & ((1 << p.page_shift) - 1));
+      r.lim = 31;
+    } else {
+      r.row = tclamp(t0);
+      r.lim = safe_last - tclamp(t0);
+    }
+    return r;
+  };
 
   const int64_t qbase = (static_cast<int64_t>(b) * p.Hq + h0) * D;
   const v4i zero4 = v4i{0, 0, 0, 0};
@@ -649,17 +698,15 @@ void sdpa_int4_hc2_kernel(SdpaParams p) {
   if (producer) {
     // ======================= producer: K . q, softmax, B operands ===========
     HcQ<kNT> Q;
+    if constexpr (PG) load_pages(0);
     hc_q_load<kNT>(Q, p, qbase);
     __builtin_amdgcn_sched_barrier(0);
     constexpr int SW = F32 ? 2 : 1;  // 16-byte scale vectors per key
     uint32_t kA[2][16], kB[2][16];
     u32x4 sA[2][SW], sB[2][SW];
-    auto load_k = [&](uint32_t (&kw)[2][16], u32x4 (&scw)[2][SW], int t0) {
-      const int tc = tclamp(t0);
-      hc_load_kw(kw, kq_rows, tc, safe_last - tc, m, c);
-      hc_load_sc<F32>(scw, sc_rows, tc, safe_last - tc, m);
-    };
-    load_k(kA, sA, base0);
+    Block cur = block_at(0);
+    hc_load_kw(kA, kq_rows, cur.row, cur.lim, m, c);
+    hc_load_sc<F32>(sA, sc_rows, cur.row, cur.lim, m);
     __builtin_amdgcn_sched_barrier(0);
     hc_q_build<kNT>(Q, p, bq_lds, sh_qhat, sh_F, lane);
     const float sf = ldexpf(1.0f, -sh_F[hh]);
@@ -679,14 +726,37 @@ void sdpa_int4_hc2_kernel(SdpaParams p) {
     auto produce = [&](const uint32_t (&kw)[2][16], const u32x4 (&scw)[2][SW], int st, uint32_t (&nk)[2][16],
                        u32x4 (&ns)[2][SW]) {
       const int t0 = base0 + st * kIter, slot = st & 1;
-      const int tn = tclamp(t0 + kIter);
+      const Block nx = block_at(st + 1);
+      // PG: whether key t is attended, and whether all of the block's are; the
+      // others lose their scales and biases
+      int sinks = 0;
+      if constexpr (PG) sinks = p.sinks;
+      auto keeps = [&](int t) { return cur.has && t < pk.n && (t >= pk.lo || t < sinks); };
+      const bool full = cur.has && cur.key <= pk.n - 32 && (cur.key >= pk.lo || cur.key <= sinks - 32);
+      u32x4 scv[2][SW];
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+#pragma unroll
+        for (int h = 0; h < SW; ++h) scv[e][h] = scw[e][h];
+      if constexpr (PG) {
+        if (!full) {  // uniform
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const bool keep = keeps(cur.key + 2 * m + e);
+#pragma unroll
+            for (int h = 0; h < SW; ++h)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) scv[e][h][i] = keep ? scv[e][h][i] : 0u;
+          }
+        }
+      }
       // scales -> LDS [array][group][key pair] (fp16) or [..][key] (fp32)
 #pragma unroll
       for (int g = 0; g < NG; ++g) {
         if constexpr (F32) {
-          *reinterpret_cast<u32x2*>(&sc_lds[s][c][g][2 * m]) = u32x2{scw[0][g >> 2][g & 3], scw[1][g >> 2][g & 3]};
+          *reinterpret_cast<u32x2*>(&sc_lds[s][c][g][2 * m]) = u32x2{scv[0][g >> 2][g & 3], scv[1][g >> 2][g & 3]};
         } else {
-          const uint32_t a0 = scw[0][0][g >> 1], a1 = scw[1][0][g >> 1];
+          const uint32_t a0 = scv[0][0][g >> 1], a1 = scv[1][0][g >> 1];
           sc_lds[s][c][g][m] = (g & 1) ? ((a0 >> 16) | (a1 & 0xFFFF0000u)) : ((a0 & 0xFFFFu) | (a1 << 16));
         }
       }
@@ -704,7 +774,7 @@ void sdpa_int4_hc2_kernel(SdpaParams p) {
       __builtin_amdgcn_wave_barrier();
       __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
       __builtin_amdgcn_sched_barrier(0);
-      hc_load_sc<F32>(ns, sc_rows, tn, safe_last - tn, m);
+      hc_load_sc<F32>(ns, sc_rows, nx.row, nx.lim, m);
       __builtin_amdgcn_sched_barrier(0);
 
       // K . q per pair of quant groups (as in the kernel above)
@@ -752,8 +822,8 @@ void sdpa_int4_hc2_kernel(SdpaParams p) {
         // was fetched twice: 1.16x the algorithmic bytes)
         if ((P & 1) == 0) {
           __builtin_amdgcn_sched_barrier(0);
-          hc_load_kw_pair(nk, kq_rows, tn, safe_last - tn, m, c, P);
-          hc_load_kw_pair(nk, kq_rows, tn, safe_last - tn, m, c, P + 1);
+          hc_load_kw_pair(nk, kq_rows, nx.row, nx.lim, m, c, P);
+          hc_load_kw_pair(nk, kq_rows, nx.row, nx.lim, m, c, P + 1);
           __builtin_amdgcn_sched_barrier(0);
         }
       }
@@ -764,7 +834,15 @@ void sdpa_int4_hc2_kernel(SdpaParams p) {
           sc[tile][i] = sf * (sc[tile][i] + __int_as_float(__builtin_amdgcn_mov_dpp(
                                                  __float_as_int(sc[tile][i]), 0x128, 0xF, 0xF, false)));
       // keys from t_end on: only the last step of a stream reaches them
-      if (t0 + 32 > t_end) {  // uniform
+      if constexpr (PG) {
+        if (!full) {  // uniform
+#pragma unroll
+          for (int tile = 0; tile < 2; ++tile)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (!keeps(cur.key + 16 * tile + 4 * c + i)) sc[tile][i] = -INFINITY;
+        }
+      } else if (t0 + 32 > t_end) {  // uniform
 #pragma unroll
         for (int tile = 0; tile < 2; ++tile)
 #pragma unroll
@@ -837,6 +915,7 @@ void sdpa_int4_hc2_kernel(SdpaParams p) {
         dst[0] = uint4{bh[0], bh[1], bh[2], bh[3]};
         dst[64] = uint4{bl[0], bl[1], bl[2], bl[3]};
       }
+      cur = nx;
     };
 
     for (int st = 0; st < NI; st += 2) {
@@ -868,9 +947,13 @@ void sdpa_int4_hc2_kernel(SdpaParams p) {
     // V stream started ~2 us late: global layer 24.8 -> 24.2 us)
     u32x4 vA[2][4], vB[2][4];
     HcQ<kNT> Q;
+    if constexpr (PG) load_pages(0);
     hc_q_load<kNT>(Q, p, qbase);
     __builtin_amdgcn_sched_barrier(0);
-    hc_load_v4(vA, vq_rows, tclamp(base0), safe_last - tclamp(base0), m, c);
+    {
+      const Block b0 = block_at(0);
+      hc_load_v4(vA, vq_rows, b0.row, b0.lim, m, c);
+    }
     __builtin_amdgcn_sched_barrier(0);
     hc_q_build<kNT>(Q, p, bq_lds, sh_qhat, sh_F, lane);
 
@@ -885,7 +968,7 @@ void sdpa_int4_hc2_kernel(SdpaParams p) {
     // One step: this step's products, with the next step's V loads issued
     // among them (four after each even block).
     auto consume = [&](const u32x4 (&vr)[2][4], int st, u32x4 (&nx)[2][4]) {
-      const int tn = tclamp(base0 + (st + 1) * kIter);
+      const Block bn = block_at(st + 1);
       const int slot = st & 1;
       const float f = f_lds[slot][s][m];
       if (__any(f != 1.0f)) {
@@ -906,8 +989,8 @@ void sdpa_int4_hc2_kernel(SdpaParams p) {
         }
         if ((blk & 1) == 0) {  // both halves of each 128-byte line at once
           __builtin_amdgcn_sched_barrier(0);
-          hc_load_v4_blk(nx, vq_rows, tn, safe_last - tn, m, c, blk);
-          hc_load_v4_blk(nx, vq_rows, tn, safe_last - tn, m, c, blk + 1);
+          hc_load_v4_blk(nx, vq_rows, bn.row, bn.lim, m, c, blk);
+          hc_load_v4_blk(nx, vq_rows, bn.row, bn.lim, m, c, blk + 1);
           __builtin_amdgcn_sched_barrier(0);
         }
         const uint4* src = pv_lds + (((slot * NS + s) * 4 + blk) * 2) * 64 + lane;
@@ -980,7 +1063,9 @@ void sdpa_int4_hc2_kernel(SdpaParams p) {
       L = fmaf(ml_lds[1][w][h], f, L);
     }
     const int64_t row = static_cast<int64_t>(b) * p.Hq + h0 + h;
-    if (rg.S == 1) {
+    int pre = 0;
+    if constexpr (PG) pre = p.pre;
+    if (rg.S == 1 && pre == 0) {
       const v4f r = v4f{normalise(O[0], L, p.denom_eps), normalise(O[1], L, p.denom_eps),
                         normalise(O[2], L, p.denom_eps), normalise(O[3], L, p.denom_eps)};
       float* dst = p.out + row * D + 4 * d4;
@@ -991,7 +1076,7 @@ void sdpa_int4_hc2_kernel(SdpaParams p) {
       }
     } else {
       // read once, by the merge kernel: streaming (non-temporal) stores
-      const int64_t slot = row * p.max_splits + split;
+      const int64_t slot = row * p.max_splits + split + pre;
       __builtin_nontemporal_store(O, reinterpret_cast<v4f*>(p.ws_o + slot * D + 4 * d4));
       if (d4 == 0) {
         __builtin_nontemporal_store(M, p.ws_ml + slot * 2);
@@ -1008,7 +1093,9 @@ void sdpa_int4_hc2_kernel(SdpaParams p) {
 // lane's running (m, l, O), then the 16 lanes merge by shuffles.  The
 // partials come from an earlier kernel, so plain loads see them.  Grid
 // (ceil(Hq * D / 4 / 16), batch).
-__global__ __launch_bounds__(256) void merge_splits_kernel(SdpaParams p, int D) {
+// PG: a paged sequence's splits, behind the p.pre partials of the shared rows.
+template <bool PG = false>
+__global__ __launch_bounds__(256) void merge_splits_kernel(ParamsOf<PG> p, int D) {
   pin_args(p);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int sl = lane & 15;
@@ -1016,8 +1103,9 @@ __global__ __launch_bounds__(256) void merge_splits_kernel(SdpaParams p, int D) 
   const int o0 = (blockIdx.x * 4 + wave) * 4;  // first output of this wave
   const int b = blockIdx.y;
   if (o0 >= p.Hq * D4) return;                 // whole waves (Hq * D4 % 4 == 0)
-  const SplitRange rg = split_range(p, b, 0);
-  const int S = rg.S;
+  int S;
+  if constexpr (PG) S = paged_range(p, paged_keys(p, p.seq_lens[b], p.windows ? p.windows[b] : p.window, p.shared), 0).S + p.pre;
+  else S = split_range(p, b, 0).S;
   if (S == 1) return;                          // written by the attention kernel
   const int o = o0 + (lane >> 4);
   const int h = o / D4, d4 = o - h * D4;
@@ -1075,9 +1163,16 @@ __global__ __launch_bounds__(256) void merge_splits_kernel(SdpaParams p, int D) 
 
 }  // namespace
 
+int launch_merge_splits(const PagedParams& p, int D, int batch, hipStream_t s) {
+  const int outs = p.Hq * D / 4;
+  merge_splits_kernel<true><<<dim3((outs + 15) / 16, batch), 256, 0, s>>>(p, D);
+  TQ_CHECK_LAUNCH("merge_splits_kernel");
+  return TQ_OK;
+}
+
 int launch_merge_splits(const SdpaParams& p, int D, int batch, hipStream_t s) {
   const int outs = p.Hq * D / 4;
-  merge_splits_kernel<<<dim3((outs + 15) / 16, batch), 256, 0, s>>>(p, D);
+  merge_splits_kernel<false><<<dim3((outs + 15) / 16, batch), 256, 0, s>>>(p, D);
   TQ_CHECK_LAUNCH("merge_splits_kernel");
   return TQ_OK;
 }
@@ -1085,6 +1180,13 @@ int launch_merge_splits(const SdpaParams& p, int D, int batch, hipStream_t s) {
 // fp16 scale/bias on either kernel; fp32 on the wave-specialised one
 bool hc_serves(int sb_dtype) {
   return sb_dtype == TQ_F16 || (sb_dtype == TQ_F32 && !options().hc_one);
+}
+
+int launch_sdpa_hc(const PagedParams& p, int sb_dtype, dim3 grid, hipStream_t s) {
+  if (sb_dtype == TQ_F32) sdpa_int4_hc2_kernel<true, true><<<grid, 2 * kHs * 64, 0, s>>>(p);
+  else sdpa_int4_hc2_kernel<false, true><<<grid, 2 * kHs * 64, 0, s>>>(p);
+  TQ_CHECK_LAUNCH("sdpa_int4_hc2_kernel");
+  return TQ_OK;
 }
 
 int launch_sdpa_hc(const SdpaParams& p, int sb_dtype, dim3 grid, hipStream_t s) {

@@ -102,10 +102,11 @@ __device__ __forceinline__ T stream_load(const T* p) {
 // addresses.  The caller keeps rows r0 .. r0 + 31 inside the cache
 // (block_row).  In three parts, in the order the products consume them:
 // 0 = scales and K, 1 = V slots 0-3, 2 = V slots 4-7.
-template <int PART, int D, int G, bool F32, bool kNT>
+// (R: int, or int64_t for rows of a page pool)
+template <int PART, int D, int G, bool F32, bool kNT, typename R>
 __device__ __forceinline__ void load_part(IterBuf<D, F32>& B, const uint32_t* kq_row0,
                                           const uint32_t* vq_row0, const uint32_t* sc_arr,
-                                          const LaneOffs& lo, int r0) {
+                                          const LaneOffs& lo, R r0) {
   using Gm = MGeom<D, G, F32>;
   constexpr uint32_t RB = D / 2;  // bytes per packed row
   // (uniform base + zero-extended lane offset, then the constant row offset
@@ -157,10 +158,10 @@ __device__ __forceinline__ void load_part(IterBuf<D, F32>& B, const uint32_t* kq
   }
 }
 
-template <int D, int G, bool F32, bool kNT>
+template <int D, int G, bool F32, bool kNT, typename R>
 __device__ __forceinline__ void load_iter(IterBuf<D, F32>& B, const uint32_t* kq_row0,
                                           const uint32_t* vq_row0, const uint32_t* sc_arr,
-                                          const LaneOffs& lo, int r0) {
+                                          const LaneOffs& lo, R r0) {
   load_part<0, D, G, F32, kNT>(B, kq_row0, vq_row0, sc_arr, lo, r0);
   load_part<1, D, G, F32, kNT>(B, kq_row0, vq_row0, sc_arr, lo, r0);
   load_part<2, D, G, F32, kNT>(B, kq_row0, vq_row0, sc_arr, lo, r0);
@@ -180,10 +181,15 @@ __device__ __forceinline__ float half_hi(uint32_t w) {
 // Decode and single-query prefill use kQG = false.
 // kStreamNT: non-temporal K/V loads (see stream_load).
 // F32: fp32 scale/bias (the reference's cache dtype); fp16 otherwise.
-template <int D, int G, int NW, bool kQG, bool kStreamNT, bool F32>
+// PG: paged cache.  Keys are the blocks of the sequence's PagedKeys list, each
+// inside one page; a wave's lanes hold the page numbers of its next 64 blocks
+// (lane i: iteration i), so that a block's rows cost a v_readlane and scalar
+// arithmetic.  Blocks with masked keys (the sequence's end, the edges of window
+// and sinks, missing pages) lose those keys' scales and biases too.
+template <int D, int G, int NW, bool kQG, bool kStreamNT, bool F32, bool PG = false>
 __global__ __launch_bounds__(NW * 64)
 __attribute__((amdgpu_waves_per_eu(D == 512 ? 1 : 2, D == 512 ? 1 : 2)))
-void sdpa_int4_mfma_kernel(SdpaParams p) {
+void sdpa_int4_mfma_kernel(ParamsOf<PG> p) {
   constexpr int kNT = NW * 64;       // threads per workgroup
   using Gm = MGeom<D, G, F32>;
   constexpr int kIter = 32 * (NW / Gm::VS);  // keys per workgroup iteration
@@ -219,7 +225,7 @@ void sdpa_int4_mfma_kernel(SdpaParams p) {
   if constexpr (!kQG && !kStreamNT) {
     if (p.lpt) {
       int chunk = p.chunk;
-      const bool job = ragged_job(p, b, hy, split, chunk);
+      const bool job = ragged_job<PG>(p, b, hy, split, chunk);
       // Every lane computes the same job; read back as wave-uniform values
       // so that the split range, the key offsets and the load addresses
       // derived from them stay in scalar registers.
@@ -239,7 +245,11 @@ void sdpa_int4_mfma_kernel(SdpaParams p) {
   const int b0 = b * pq;
   const int b_last = kQG ? min(b0 + pq - 1, p.nq - 1) : b;
 
-  const SplitRange rg = kQG ? prefill_range(p, b0, b_last, split) : split_range(p, b, split);
+  PagedKeys pk{};
+  if constexpr (PG) pk = paged_keys(p, p.seq_lens[b], p.windows ? p.windows[b] : p.window, p.shared);
+  const SplitRange rg = PG    ? paged_range(p, pk, split)
+                        : kQG ? prefill_range(p, b0, b_last, split)
+                              : split_range(p, b, split);
   if (split >= rg.S) return;
   const int t_begin = rg.t_begin, t_end = rg.t_end;
   // this column's causal / window limits (the queries of a group differ)
@@ -267,7 +277,7 @@ void sdpa_int4_mfma_kernel(SdpaParams p) {
   if ((threadIdx.x & 63) == 0) s_done[threadIdx.x >> 6] = 0;
 
   // ---- first loads, issued before the prologue to overlap its latency ------
-  const int64_t row0 = (static_cast<int64_t>(cache_batch(p, b)) * p.Hkv + kvh) * p.cap;
+  const int64_t row0 = PG ? 0 : (static_cast<int64_t>(cache_batch(p, b)) * p.Hkv + kvh) * p.cap;
   const uint32_t* kq_row0 = p.kq + row0 * RW;
   const uint32_t* vq_row0 = p.vq + row0 * RW;
   // (a select chain over kernel-argument pointers keeps the global address
@@ -293,6 +303,38 @@ void sdpa_int4_mfma_kernel(SdpaParams p) {
   // in [0, max(t_end, 32)), inside the cache: the planner gives this kernel
   // capacities of at least 32 rows.  Wave-uniform (scalar).
   auto block_row = [&](int t0) { return max(0, min(t0, t_end - 32)); };
+  // PG: the page numbers of iterations it .. it + 63 in the lanes (-1 where the
+  // list is empty; past its end the last one), and the block of iteration `it`.
+  int pages = -1;
+  auto load_pages = [&](int it) {
+    if constexpr (PG) {
+      if (pk.nb > 0) {
+        const int v = min(((base0 + it * kIter) >> 5) + (lane * kIter >> 5), pk.nb - 1);
+        pages = p.tables[static_cast<int64_t>(b) * p.max_pages + (pk.block(v) >> (p.page_shift - 5))];
+      }
+    }
+  };
+  struct PgBlock {
+    int64_t row;  // its first row in the pool
+    int key;      // its first key
+    bool has;     // its page exists
+  };
+  auto pg_block = [&](int it) {
+    PgBlock r{};
+    if constexpr (PG) {
+      const int e = __builtin_amdgcn_readlane(pages, it & 63);
+      r.has = static_cast<unsigned>(e) < static_cast<unsigned>(p.num_pages);
+      r.key = 32 * pk.block((base0 + it * kIter) >> 5);
+      r.row = ((static_cast<int64_t>(r.has ? e : 0) * p.Hkv + kvh) << p.page_shift) + (r.key & ((1 << p.page_shift) - 1));
+    }
+    return r;
+  };
+  // first row of the block at key t0 (PG: of pb)
+  auto first_row = [&](int t0, const PgBlock& pb) {
+    if constexpr (PG) return pb.row;
+    else return block_row(t0);
+  };
+  if constexpr (PG) load_pages(0);
 
   // q is loaded first, then the first block's K/V, which stay in flight
   // while the prologue runs.  Every wave loads all G * D q elements of its
@@ -314,6 +356,7 @@ void sdpa_int4_mfma_kernel(SdpaParams p) {
     qb[s] = *reinterpret_cast<const uint4*>(qp + (q32 ? 16 : 0));
   }
   __builtin_amdgcn_sched_barrier(0);
+  PgBlock pbA = pg_block(0), pbB;
   // Issued unconditionally (a load under a branch makes the compiler drain
   // every outstanding load at the join): block_row keeps the rows of a wave
   // or split with no keys inside the cache.
@@ -324,9 +367,9 @@ void sdpa_int4_mfma_kernel(SdpaParams p) {
   constexpr bool kLateV = NW == 4 && VS == 1;
   IterBuf<D, F32> bufA, bufB;
   if constexpr (kLateV)
-    load_part<0, D, G, F32, kStreamNT>(bufA, kq_row0, vq_row0, sc_arr, lo, block_row(base0));
+    load_part<0, D, G, F32, kStreamNT>(bufA, kq_row0, vq_row0, sc_arr, lo, first_row(base0, pbA));
   else
-    load_iter<D, G, F32, kStreamNT>(bufA, kq_row0, vq_row0, sc_arr, lo, block_row(base0));
+    load_iter<D, G, F32, kStreamNT>(bufA, kq_row0, vq_row0, sc_arr, lo, first_row(base0, pbA));
   __builtin_amdgcn_sched_barrier(0);
 
   // ---- prologue: q as 22-bit fixed point per column set, B image per wave ---
@@ -453,8 +496,8 @@ void sdpa_int4_mfma_kernel(SdpaParams p) {
 
   if constexpr (kLateV) {
     __builtin_amdgcn_sched_barrier(0);
-    load_part<1, D, G, F32, kStreamNT>(bufA, kq_row0, vq_row0, sc_arr, lo, block_row(base0));
-    load_part<2, D, G, F32, kStreamNT>(bufA, kq_row0, vq_row0, sc_arr, lo, block_row(base0));
+    load_part<1, D, G, F32, kStreamNT>(bufA, kq_row0, vq_row0, sc_arr, lo, first_row(base0, pbA));
+    load_part<2, D, G, F32, kStreamNT>(bufA, kq_row0, vq_row0, sc_arr, lo, first_row(base0, pbA));
     __builtin_amdgcn_sched_barrier(0);
   }
 
@@ -483,10 +526,15 @@ void sdpa_int4_mfma_kernel(SdpaParams p) {
   // before the V products): a wave's loads go out in three smaller bursts,
   // so the waves of a CU stay closer together than with one burst of all
   // thirteen loads per iteration.
-  auto process = [&](const IterBuf<D, F32>& B, int t0, auto&& issue) {
+  auto process = [&](const IterBuf<D, F32>& B, int t0, const PgBlock& pb, auto&& issue) {
     // B holds the block of rows r0 .. r0 + 31 (r0 <= t0); its keys below t0
     // or from t_end on are masked
-    const int r0 = block_row(t0);
+    const int r0 = PG ? pb.key : block_row(t0);
+    // PG: whether key t is attended, and whether all of the block's are
+    int sinks = 0;
+    if constexpr (PG) sinks = p.sinks;
+    auto keeps = [&](int t) { return pb.has && t < pk.n && (t >= pk.lo || t < sinks); };
+    const bool pg_full = pb.has && pb.key <= pk.n - 32 && (pb.key >= pk.lo || pb.key <= sinks - 32);
     issue(std::integral_constant<int, 0>{});
     __builtin_amdgcn_sched_barrier(0);
     const uint32_t n_keep = static_cast<uint32_t>(t_end - t0);  // > 0 for a processed iteration
@@ -500,7 +548,16 @@ void sdpa_int4_mfma_kernel(SdpaParams p) {
     for (int e = 0; e < 2; ++e)
 #pragma unroll
       for (int w = 0; w < Gm::SCW; ++w) scv[e][w] = B.sc[e][w];
-    if (t_end < 32) {  // uniform, and rare: only then can a block row pass t_end
+    if constexpr (PG) {
+      if (!pg_full) {  // uniform
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const bool keep = keeps(r0 + 2 * k16 + e);
+#pragma unroll
+          for (int w = 0; w < Gm::SCW; ++w) scv[e][w] = keep ? scv[e][w] : 0u;
+        }
+      }
+    } else if (t_end < 32) {  // uniform, and rare: only then can a block row pass t_end
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const bool in_seq = r0 + 2 * k16 + e < t_end;
@@ -563,8 +620,8 @@ void sdpa_int4_mfma_kernel(SdpaParams p) {
     };
     // With packed columns (every lane's column used) and no per-column
     // limits, a block whose 32 rows all lie in [t0, t_end) needs no mask.
-    constexpr bool kMaskAll = !PACK || kQG;
-    const bool full = r0 == t0 && n_keep >= 32;  // uniform
+    constexpr bool kMaskAll = !PG && (!PACK || kQG);
+    const bool full = PG ? pg_full : r0 == t0 && n_keep >= 32;  // uniform
     auto scores = [&](const v4i (&acc)[3], int u, int tile) {
       const v4f ks = scale4(0, gn, tile), kb = scale4(1, gn, tile);
 #pragma unroll
@@ -582,6 +639,8 @@ void sdpa_int4_mfma_kernel(SdpaParams p) {
           bool keep = static_cast<uint32_t>(t - t0) < n_keep && col_used;
           if constexpr (kQG) keep = keep && t <= col_hi && t >= col_lo;
           sc[4 * u + i] = keep ? part : -INFINITY;
+        } else if constexpr (PG && COLS < 16 && !PACK) {
+          sc[4 * u + i] = col_used ? part : -INFINITY;
         } else {
           sc[4 * u + i] = part;
         }
@@ -591,7 +650,7 @@ void sdpa_int4_mfma_kernel(SdpaParams p) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const int t = r0 + 16 * tile + 4 * c + i;
-            if (static_cast<uint32_t>(t - t0) >= n_keep) sc[4 * u + i] = -INFINITY;
+            if (PG ? !keeps(t) : static_cast<uint32_t>(t - t0) >= n_keep) sc[4 * u + i] = -INFINITY;
           }
         }
       }
@@ -644,6 +703,8 @@ void sdpa_int4_mfma_kernel(SdpaParams p) {
     // weights of this lane's own scores; the denominator and the V bias
     // term count each key once (the lane of its score)
     float pw[4 * NU];
+    // PG: a block without any key may come first; -inf - -inf would be NaN
+    const float m_sub = PG && m_run == -INFINITY ? 0.0f : m_run;
 #pragma unroll
     for (int u = 0; u < NU; ++u) {
       const v4f vb = scale4(3, gn, PACK ? T : u);
@@ -652,7 +713,7 @@ void sdpa_int4_mfma_kernel(SdpaParams p) {
         // (a masked score gives 2^-inf = 0 as long as m_run is finite: with
         // packed columns every column scores every key, and a processed
         // iteration holds at least one key, so only the other forms test)
-        const float pj = (PACK && !kQG) || sc[4 * u + i] != -INFINITY ? fast_exp2(sc[4 * u + i] - m_run) : 0.0f;
+        const float pj = PG || (PACK && !kQG) || sc[4 * u + i] != -INFINITY ? fast_exp2(sc[4 * u + i] - m_sub) : 0.0f;
         pw[4 * u + i] = pj;
         l_run += pj;
         bacc = fmaf(pj, vb[i], bacc);
@@ -737,8 +798,8 @@ void sdpa_int4_mfma_kernel(SdpaParams p) {
   };
 
   // the next block's loads (into B, rows from key t0), issued in parts by process
-  auto next_of = [&](IterBuf<D, F32>& B, int t0) {
-    const int r0 = block_row(t0);
+  auto next_of = [&](IterBuf<D, F32>& B, int t0, const PgBlock& pb) {
+    const auto r0 = first_row(t0, pb);
     return [&B, r0, &kq_row0, &vq_row0, &sc_arr, &lo](auto part) {
       load_part<decltype(part)::value, D, G, F32, kStreamNT>(B, kq_row0, vq_row0, sc_arr, lo, r0);
     };
@@ -746,6 +807,18 @@ void sdpa_int4_mfma_kernel(SdpaParams p) {
   auto no_loads = [](auto) {};
 
   auto pace = [&](int done) { pace_waves<NW>(s_done, wv, lane, done); };
+  // PG: the block of iteration `it`, with the next 64 pages before it where
+  // they are due.  Waited for inside the branch, so that the steady loop waits
+  // for nothing here.
+  auto block_at = [&](int it) {
+    if constexpr (PG) {
+      if ((it & 63) == 0) {
+        load_pages(it);
+        asm volatile("" : "+v"(pages));
+      }
+    }
+    return pg_block(it);
+  };
   pace(0);
   // Steady state: every load in the body is for an iteration of this wave.
   // The last one or two iterations are peeled, so no load is issued past
@@ -753,19 +826,22 @@ void sdpa_int4_mfma_kernel(SdpaParams p) {
   // before their reuse after the loop, a full memory round trip per wave.
   int it = 0;
   for (; it + 2 < nit; it += 2) {
-    process(bufA, base0 + it * kIter, next_of(bufB, base0 + (it + 1) * kIter));
+    pbB = block_at(it + 1);
+    process(bufA, base0 + it * kIter, pbA, next_of(bufB, base0 + (it + 1) * kIter, pbB));
     pace(it + 1);
     __builtin_amdgcn_sched_barrier(0);
-    process(bufB, base0 + (it + 1) * kIter, next_of(bufA, base0 + (it + 2) * kIter));
+    pbA = block_at(it + 2);
+    process(bufB, base0 + (it + 1) * kIter, pbB, next_of(bufA, base0 + (it + 2) * kIter, pbA));
     pace(it + 2);
     __builtin_amdgcn_sched_barrier(0);
   }
   if (it + 1 < nit) {
-    process(bufA, base0 + it * kIter, next_of(bufB, base0 + (it + 1) * kIter));
+    pbB = block_at(it + 1);
+    process(bufA, base0 + it * kIter, pbA, next_of(bufB, base0 + (it + 1) * kIter, pbB));
     __builtin_amdgcn_sched_barrier(0);
-    process(bufB, base0 + (it + 1) * kIter, no_loads);
+    process(bufB, base0 + (it + 1) * kIter, pbB, no_loads);
   } else if (it < nit) {
-    process(bufA, base0 + it * kIter, no_loads);
+    process(bufA, base0 + it * kIter, pbA, no_loads);
   }
 
   // ---- per-wave result into the finalisation arena --------------------------
@@ -831,7 +907,15 @@ void sdpa_int4_mfma_kernel(SdpaParams p) {
     Fin::run(p, arena, static_cast<int64_t>(b0) * p.Hq + h0, rg.S, split, b * p.Hq + hy, GH,
              p.Hq, (b_last - b0 + 1) * GH);
   else
-    Fin::run(p, arena, static_cast<int64_t>(b) * p.Hq + h0, rg.S, split, b * p.Hq + hy);
+    Fin::template run<PG>(p, arena, static_cast<int64_t>(b) * p.Hq + h0, rg.S, split, b * p.Hq + hy);
+}
+
+template <int D, int G, bool F32>
+int launch_dgs(const PagedParams& p, dim3 grid, hipStream_t s) {
+  constexpr int NW = D == 512 ? 4 : kMfmaWaves;
+  sdpa_int4_mfma_kernel<D, G, NW, false, false, F32, true><<<grid, NW * 64, 0, s>>>(p);
+  TQ_CHECK_LAUNCH("sdpa_int4_mfma_kernel");
+  return TQ_OK;
 }
 
 template <int D, int G, bool F32>
@@ -853,23 +937,13 @@ int launch_dgs(const SdpaParams& p, dim3 grid, hipStream_t s) {
   return TQ_OK;
 }
 
-template <int D, int G>
-int launch_dg(const SdpaParams& p, int sb_dtype, dim3 grid, hipStream_t s) {
+template <int D, int G, typename P>
+int launch_dg(const P& p, int sb_dtype, dim3 grid, hipStream_t s) {
   return sb_dtype == TQ_F32 ? launch_dgs<D, G, true>(p, grid, s) : launch_dgs<D, G, false>(p, grid, s);
 }
 
-}  // namespace
-
-bool mfma_serves(int D, int cols, int sb_dtype) {
-  if (sb_dtype != TQ_F16 && sb_dtype != TQ_F32) return false;
-  if (D == 256) return cols == 1 || cols == 2 || cols == 4;
-  if (D == 512) return cols == 1 || cols == 2;
-  if (D == 128) return cols == 1 || cols == 2 || cols == 4 || cols == 8;
-  return false;
-}
-
-int launch_sdpa_mfma(const SdpaParams& p, int D, int G, int sb_dtype, dim3 grid,
-                     hipStream_t stream) {
+template <typename P>
+int launch_any(const P& p, int D, int G, int sb_dtype, dim3 grid, hipStream_t stream) {
   if (!mfma_serves(D, G, sb_dtype)) return -1;
   if (D == 256) {
     if (G == 1) return launch_dg<256, 1>(p, sb_dtype, grid, stream);
@@ -885,6 +959,26 @@ int launch_sdpa_mfma(const SdpaParams& p, int D, int G, int sb_dtype, dim3 grid,
     if (G == 8) return launch_dg<128, 8>(p, sb_dtype, grid, stream);
   }
   return -1;
+}
+
+}  // namespace
+
+bool mfma_serves(int D, int cols, int sb_dtype) {
+  if (sb_dtype != TQ_F16 && sb_dtype != TQ_F32) return false;
+  if (D == 256) return cols == 1 || cols == 2 || cols == 4;
+  if (D == 512) return cols == 1 || cols == 2;
+  if (D == 128) return cols == 1 || cols == 2 || cols == 4 || cols == 8;
+  return false;
+}
+
+int launch_sdpa_mfma(const SdpaParams& p, int D, int G, int sb_dtype, dim3 grid,
+                     hipStream_t stream) {
+  return launch_any(p, D, G, sb_dtype, grid, stream);
+}
+
+int launch_sdpa_mfma(const PagedParams& p, int D, int G, int sb_dtype, dim3 grid,
+                     hipStream_t stream) {
+  return launch_any(p, D, G, sb_dtype, grid, stream);
 }
 
 }  // namespace tq
