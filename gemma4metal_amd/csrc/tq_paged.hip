@@ -1,5 +1,10 @@
 // Attention over the paged int4 cache (single tokens, batches that share a
-// prefix, prompts), with a sliding window and first tokens that stay visible.
+// prefix, prompts), with a sliding window and first tokens that stay visible:
+// argument checks, split plans and launches.  Single tokens run the decode
+// kernels in their paged form (tq_sdpa_mfma.hip, tq_sdpa_hc.hip); prompts, and
+// the part of a batch's keys that all its sequences share, run the K/V-tile
+// kernel (tq_paged_tiles.hip), whose partials the decode kernel joins with those
+// of each sequence's own keys.
 #include <math.h>
 
 #include <algorithm>
@@ -8,59 +13,6 @@
 
 namespace tq {
 namespace {
-
-// A wave per (query, head) row: lane i holds dims i E .. i E + E - 1, E = D / 64,
-// and walks the row's keys one by one with a running maximum and sum.
-template <int D, typename SB>
-__global__ __launch_bounds__(256) void paged_rows_kernel(PagedParams p, int64_t rows) {
-  constexpr int E = D / 64;
-  const int lane = threadIdx.x & 63;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
-  if (row >= rows) return;
-  const int b = static_cast<int>(row / p.Hq), h = static_cast<int>(row - static_cast<int64_t>(b) * p.Hq);
-  const int kvh = h / p.gqa;
-  const int n = p.prefill ? p.n + b + 1 : min(p.seq_lens[b], p.n_clamp);
-  const int W = p.windows ? p.windows[b] : p.window;
-  const int lo = W > 0 ? max(0, n - W) : 0;
-  const int64_t mine = p.prefill ? 0 : static_cast<int64_t>(b) * p.max_pages;
-  float q[E], o[E];
-#pragma unroll
-  for (int e = 0; e < E; ++e) {
-    q[e] = load_any(p.q, p.q_dtype, row * D + lane * E + e) * p.scale_log2;
-    o[e] = 0.0f;
-  }
-  float m = -INFINITY, l = 0.0f;
-  for (int t = 0; t < n; ++t) {
-    if (t < lo && t >= p.sinks) t = lo;
-    const int page = p.tables[(t < p.shared ? 0 : mine) + (t >> p.page_shift)];
-    if (static_cast<unsigned>(page) >= static_cast<unsigned>(p.num_pages)) continue;
-    const int64_t r = ((static_cast<int64_t>(page) * p.Hkv + kvh) << p.page_shift) + (t & ((1 << p.page_shift) - 1));
-    const int64_t g = r * (D / 64) + lane * E / 64, w = r * (D / 8) + lane * E / 8;
-    const int sh = 4 * (lane * E % 8);
-    const float ks = sb_to_f32(static_cast<const SB*>(p.ks)[g]), kb = sb_to_f32(static_cast<const SB*>(p.kb)[g]);
-    const float vs = sb_to_f32(static_cast<const SB*>(p.vs)[g]), vb = sb_to_f32(static_cast<const SB*>(p.vb)[g]);
-    float s = 0.0f;
-#pragma unroll
-    for (int e = 0; e < E; ++e) s = fmaf(q[e], fmaf(ks, static_cast<float>(p.kq[w] >> (sh + 4 * e) & 15u), kb), s);
-    s = group_sum<64>(s);
-    const float mn = fmaxf(m, s), f = merge_factor(m, mn), x = fast_exp2(s - mn);
-    l = fmaf(l, f, x);
-#pragma unroll
-    for (int e = 0; e < E; ++e) o[e] = fmaf(o[e], f, x * fmaf(vs, static_cast<float>(p.vq[w] >> (sh + 4 * e) & 15u), vb));
-    m = mn;
-  }
-#pragma unroll
-  for (int e = 0; e < E; ++e) p.out[row * D + lane * E + e] = normalise(o[e], l, 0.0f);
-}
-
-template <int D>
-int launch_rows(const PagedParams& p, int sb_dtype, int64_t rows, hipStream_t s) {
-  const unsigned grid = static_cast<unsigned>((rows + 3) / 4);
-  if (sb_dtype == TQ_F16) paged_rows_kernel<D, __half><<<grid, 256, 0, s>>>(p, rows);
-  else paged_rows_kernel<D, float><<<grid, 256, 0, s>>>(p, rows);
-  TQ_CHECK_LAUNCH("paged_rows_kernel");
-  return TQ_OK;
-}
 
 // What both calls refuse; fills the parameters that they share.
 int paged_params(PagedParams& p, const void* q, int q_dtype, const uint32_t* kq, const void* ks, const void* kb,
@@ -109,7 +61,6 @@ struct PagedPlan {
   bool hc;
   int G, n_sub, chunk, max_splits;
   bool lpt;
-  WsLayout wl;
 };
 
 // max_len: what any sequence attends beside the shared rows, at most.
@@ -131,7 +82,6 @@ PagedPlan plan_paged(int batch, int Hq, int Hkv, int D, int sb_dtype, int max_le
     pl.max_splits = 2;
     pl.chunk = std::max(pl.chunk, ((len + 1) / 2 + 127) / 128 * 128);
   }
-  pl.wl = ws_layout(batch, Hq, D, pl.max_splits);
   return pl;
 }
 
@@ -142,10 +92,26 @@ int attended_bound(int max_kv_len, int window, bool windows, int sinks) {
   return static_cast<int>(std::min<int64_t>(most, max_kv_len));
 }
 
-int launch_any(const PagedParams& p, int D, int sb_dtype, int64_t rows, hipStream_t s) {
-  if (D == 128) return launch_rows<128>(p, sb_dtype, rows, s);
-  if (D == 256) return launch_rows<256>(p, sb_dtype, rows, s);
-  return launch_rows<512>(p, sb_dtype, rows, s);
+// The split partials of a call in its workspace.
+int set_workspace(PagedParams& p, void* workspace, size_t bytes, const WsLayout& wl, const char* fn) {
+  if (!workspace || bytes < wl.total) {
+    set_error("%s: workspace of %zu bytes needed (got %zu)", fn, wl.total, workspace ? bytes : size_t{0});
+    return TQ_ERR_WORKSPACE;
+  }
+  TQ_CHECK_ARG(reinterpret_cast<uintptr_t>(workspace) % 16 == 0, "%s: workspace must be 16-byte aligned", fn);
+  // the split partials are addressed with 32-bit byte offsets
+  TQ_CHECK_ARG(wl.total - wl.o_off < (size_t{1} << 31), "%s: split partials exceed 2 GiB", fn);
+  char* ws = static_cast<char*>(workspace);
+  p.ws_cnt = reinterpret_cast<int*>(ws + wl.cnt_off);
+  p.ws_ml = reinterpret_cast<float*>(ws + wl.ml_off);
+  p.ws_o = reinterpret_cast<float*>(ws + wl.o_off);
+  return TQ_OK;
+}
+
+// Keys that the rows of a prompt's workgroup attend, about.
+int64_t prompt_keys(int n_prior, int n_new, int window, int sinks) {
+  const int64_t n = static_cast<int64_t>(n_prior) + (n_new + 1) / 2;
+  return window > 0 ? std::min<int64_t>(n, static_cast<int64_t>(window) + sinks + 64) : n;
 }
 
 }  // namespace
@@ -159,7 +125,10 @@ extern "C" size_t tq_sdpa_int4_paged_workspace_size(int batch, int num_heads, in
   // (every plan of a call with these sizes: a window only shortens the splits)
   const int gqa = num_heads / num_kv_heads;
   const int64_t groups = static_cast<int64_t>(batch) * num_kv_heads * (gqa / head_subgroup(gqa));
-  return ws_layout(batch, num_heads, head_dim, max_splits_bound(max_kv_len, groups, min_splits_for(batch))).total;
+  int splits = max_splits_bound(max_kv_len, groups, min_splits_for(batch));
+  if (shared_prefix > 0)
+    splits += paged_tiles_splits(static_cast<int64_t>(batch) * gqa, num_kv_heads, head_dim, shared_prefix);
+  return ws_layout(batch, num_heads, head_dim, splits).total;
 }
 
 extern "C" int tq_sdpa_int4_paged(const void* q, tq_dtype q_dtype, const uint32_t* k_quant, const void* k_scales,
@@ -189,42 +158,41 @@ extern "C" int tq_sdpa_int4_paged(const void* q, tq_dtype q_dtype, const uint32_
   p.windows = windows;
   p.n_clamp = max_kv_len;
   p.shared = shared_prefix;
-  if (shared_prefix > 0)
-    return launch_any(p, head_dim, sb_dtype, static_cast<int64_t>(batch) * num_heads, static_cast<hipStream_t>(stream));
+  // of the rows behind the shared ones
   const PagedPlan pl = plan_paged(batch, num_heads, num_kv_heads, head_dim, sb_dtype,
-                                  attended_bound(max_kv_len, sliding_window, windows != nullptr, num_sinks));
+                                  std::min(attended_bound(max_kv_len, sliding_window, windows != nullptr, num_sinks),
+                                           max_kv_len - shared_prefix));
   TQ_CHECK_ARG(num_kv_heads * static_cast<int64_t>(pl.n_sub) <= 65535, "%s: grid too large", fn);
   TQ_CHECK_ARG(static_cast<int64_t>(batch) * num_heads <= kMaxCounters, "%s: batch * num_heads must be <= %lld", fn,
                static_cast<long long>(kMaxCounters));
   p.n_sub = pl.n_sub;
   p.chunk = pl.chunk;
-  p.max_splits = pl.max_splits;
   p.lpt = pl.lpt ? 1 : 0;
-  if (pl.max_splits > 1) {
-    if (!workspace || workspace_bytes < pl.wl.total) {
-      set_error("%s: workspace of %zu bytes needed (got %zu)", fn, pl.wl.total, workspace_bytes);
-      return TQ_ERR_WORKSPACE;
-    }
-    TQ_CHECK_ARG(reinterpret_cast<uintptr_t>(workspace) % 16 == 0, "%s: workspace must be 16-byte aligned", fn);
-    // the split partials are addressed with 32-bit byte offsets
-    TQ_CHECK_ARG(pl.wl.total - pl.wl.o_off < (size_t{1} << 31), "%s: split-K partials exceed 2 GiB", fn);
-    char* ws = static_cast<char*>(workspace);
-    p.ws_cnt = reinterpret_cast<int*>(ws + pl.wl.cnt_off);
-    p.ws_ml = reinterpret_cast<float*>(ws + pl.wl.ml_off);
-    p.ws_o = reinterpret_cast<float*>(ws + pl.wl.o_off);
+  if (shared_prefix > 0)
+    p.pre = paged_tiles_splits(static_cast<int64_t>(batch) * gqa_factor, num_kv_heads, head_dim, shared_prefix);
+  const int own = pl.max_splits;
+  p.max_splits = own + p.pre;
+  if (p.max_splits > 1) {
+    if (int r = set_workspace(p, workspace, workspace_bytes, ws_layout(batch, num_heads, head_dim, p.max_splits), fn)) return r;
   }
-  const dim3 grid(pl.max_splits, num_kv_heads * pl.n_sub, batch);
+  const dim3 grid(own, num_kv_heads * pl.n_sub, batch);
   p.cnt_stride = counter_stride(static_cast<int64_t>(batch) * num_heads);
   hipStream_t s = static_cast<hipStream_t>(stream);
+  if (p.pre > 0)
+    if (int r = launch_paged_tiles(p, head_dim, sb_dtype, p.pre, true, s)) return r;
   if (!pl.hc) return launch_sdpa_mfma(p, head_dim, pl.G, sb_dtype, grid, s);
-  p.ext_merge = pl.max_splits > 1 ? 1 : 0;
+  p.ext_merge = p.max_splits > 1 ? 1 : 0;
   const int r = launch_sdpa_hc(p, sb_dtype, grid, s);
   return r != TQ_OK || !p.ext_merge ? r : launch_merge_splits(p, head_dim, batch, s);
 }
 
 extern "C" size_t tq_sdpa_int4_paged_prefill_workspace_size(int num_heads, int num_kv_heads, int head_dim,
                                                             int n_prior, int n_new) {
-  return 0;
+  if (num_kv_heads < 1 || num_heads < num_kv_heads || n_prior < 0 || n_new < 1) return 0;
+  // (a window only shortens the splits)
+  const int splits = paged_tiles_max_splits(static_cast<int64_t>(n_new) * (num_heads / num_kv_heads), num_kv_heads,
+                                            head_dim, prompt_keys(n_prior, n_new, 0, 0));
+  return splits > 1 ? ws_layout(n_new, num_heads, head_dim, splits).total : 0;
 }
 
 extern "C" int tq_sdpa_int4_paged_prefill(const void* q, tq_dtype q_dtype, const uint32_t* k_quant,
@@ -249,5 +217,11 @@ extern "C" int tq_sdpa_int4_paged_prefill(const void* q, tq_dtype q_dtype, const
   TQ_CHECK_ARG(n_new <= 65535, "%s: at most 65535 queries per call", fn);
   p.prefill = 1;
   p.n = n_prior;
-  return launch_any(p, head_dim, sb_dtype, static_cast<int64_t>(n_new) * num_heads, static_cast<hipStream_t>(stream));
+  const int64_t rows = static_cast<int64_t>(n_new) * gqa_factor;
+  TQ_CHECK_ARG((rows + 63) / 64 * num_kv_heads < (int64_t{1} << 31), "%s: grid too large", fn);
+  const int splits = paged_tiles_splits(rows, num_kv_heads, head_dim, prompt_keys(n_prior, n_new, sliding_window, num_sinks));
+  p.max_splits = splits;
+  if (splits > 1)
+    if (int r = set_workspace(p, workspace, workspace_bytes, ws_layout(n_new, num_heads, head_dim, splits), fn)) return r;
+  return launch_paged_tiles(p, head_dim, sb_dtype, splits, false, static_cast<hipStream_t>(stream));
 }

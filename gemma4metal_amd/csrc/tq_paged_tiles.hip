@@ -1,0 +1,642 @@
+// Multi-query attention over pages with K/V tiles shared by a workgroup's 64
+// (query, head) rows of one kv head: prompts (rows of consecutive queries of one
+// sequence), and the shared prefix of a batch (rows of all its sequences).
+//
+// The mathematics, operand layouts and staging are those of tq_prefill.hip, and
+// so is what bounds it (VALU).  What differs:
+// - A tile is TK keys at a multiple of TK, one or two 32-row parts of pages;
+//   the page numbers of the next 64 parts are held in a wave's lanes.  Tiles
+//   between the sinks and the window that no row attends are left out.
+// - Rows have limits of their own, [lo, hi) or below the sinks.  In a part of a
+//   tile that some row does not attend wholly, V scales and biases of weight 0
+//   are taken as 0 (a key that other rows attend may be infinite or NaN); rows
+//   that nobody attends are staged with scales and biases of 0.
+// - The tiles of a workgroup's rows may be split over workgroups (grid y), which
+//   then leave partials (m, l, O).
+// - fp32 queries are two fp16 parts, 22 bits, and take two products a k-step.
+//   fp32 biases are applied in fp32.
+#include "tq_prefill_tile.h"
+
+namespace tq {
+namespace {
+
+constexpr int kRs = 4;           // 16-row sets of a workgroup
+constexpr int kRows = 16 * kRs;
+
+template <int KH>
+struct PgTile {
+  int key;           // its first key
+  int64_t row[KH];   // first pool row of each 32-row part
+  bool has[KH];      // whether that part's page exists
+};
+
+__device__ __forceinline__ int wave_min_i(int v) { return -wave_max_i(-v); }
+
+template <class Gm>
+__device__ __forceinline__ void pg_load(PfRaw<Gm>& R, const PagedParams& p, const PgTile<Gm::KH>& t, int hi) {
+  constexpr int KH = Gm::KH;
+  // the part of a tile row; the same for a wave's 64 units where those span at
+  // most one part
+  const auto part = [](int r) { return KH == 1 ? 0 : __builtin_amdgcn_readfirstlane(r >> 5); };
+#pragma unroll
+  for (int i = 0; i < Gm::NU; ++i) {
+    const int e = threadIdx.x + i * Gm::NT;
+    const int role = __builtin_amdgcn_readfirstlane(e / Gm::UNITS);
+    const int u = e % Gm::UNITS;
+    if (role == 0) {
+      const int r = u / Gm::NG;
+      const int64_t base = KH == 2 && part(r) ? t.row[KH - 1] : t.row[0];
+      const u32x4* src = reinterpret_cast<const u32x4*>(p.kq + base * Gm::W) + ((r & 31) * (Gm::W / 4) + 2 * (u % Gm::NG));
+      const u32x4 a = src[0], b = src[1];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        R.w[i][k] = a[k];
+        R.w[i][4 + k] = b[k];
+      }
+    } else {  // (threads past the units load one again and do not store it)
+      const int w = u % Gm::W, kc = u / Gm::W;  // kc = 4 part + c
+      const int64_t base = KH == 2 && part(8 * kc) ? t.row[KH - 1] : t.row[0];
+      const uint32_t* src = p.vq + base * Gm::W;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) R.w[i][j] = src[(4 * (kc & 3) + 16 * (j >> 2) + (j & 3)) * Gm::W + w];
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < Gm::NSD; ++i) {
+    const int e = threadIdx.x + i * Gm::NT;
+    // (threads past the tensors load one again and do not store it)
+    const int a = min(__builtin_amdgcn_readfirstlane(e / Gm::SDW), 3), d = e % Gm::SDW;
+    constexpr int DPR = Gm::SDW / Gm::TK;  // dwords a row
+    const void* src = a == 0 ? p.ks : a == 1 ? p.kb : a == 2 ? p.vs : p.vb;
+    const int r = d / DPR;
+    const uint32_t* s32 = static_cast<const uint32_t*>(src);
+    uint32_t v;
+    bool has;
+    if constexpr (KH == 2 && DPR == 1) {  // a wave spans both parts
+      const bool second = r >= 32;
+      has = second ? t.has[KH - 1] : t.has[0];
+      v = s32[(second ? t.row[KH - 1] : t.row[0]) + (r & 31)];
+    } else {
+      const int q = part(r);
+      has = KH == 2 && q ? t.has[KH - 1] : t.has[0];
+      v = (s32 + (KH == 2 && q ? t.row[KH - 1] : t.row[0]) * DPR)[(r & 31) * DPR + d % DPR];
+    }
+    // rows past every limit, and those of missing pages, may hold anything
+    R.s[i] = has && t.key + r < hi ? v : 0u;
+  }
+}
+
+struct TileParams : PagedParams {
+  int splits;  // workgroups along the tiles (grid y); 1: write p.out
+};
+
+template <int D, bool F32, bool Q32>
+__global__ __launch_bounds__(128 * kRs) __attribute__((amdgpu_waves_per_eu(2, 2)))
+void paged_tiles_kernel(TileParams p) {
+  using Gm = PfGeom<D, F32, kRs>;
+  using SB = typename Gm::SB;
+  constexpr int NG = Gm::NG, NWG = Gm::NW_, TK = Gm::TK, KH = Gm::KH, DH = Gm::DH, RS = kRs;
+  __shared__ __attribute__((aligned(16))) typename Gm::Lds L;
+  __shared__ uint32_t vmx;                  // bits of the first tile's largest |V scale|
+  __shared__ int alike[2][Gm::NSW];         // a buffer's V scales are alike (all of them set)
+  __shared__ float ml[Gm::NW][16], ll[Gm::NW][16];
+
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
+  const int rs = wave % RS, kh = wave / RS % KH, dh = wave / (RS * KH);
+  const int m = lane & 15, c = lane >> 4;
+  // heads vary fastest, the longest key ranges (last queries) start first
+  const int nblk = gridDim.x / p.Hkv;
+  const int kvh = blockIdx.x % p.Hkv, blk = nblk - 1 - static_cast<int>(blockIdx.x / p.Hkv);
+  const int total = p.nq * p.gqa;           // rows of this kv head
+  const int r0 = blk * kRows;               // first row of this workgroup
+
+  // ---- the rows' limits, and the workgroup's tiles ----------------------------
+  // row r attends key t iff t < hi and (t >= lo or t < sinks)
+  const auto limits = [&](int r, int& hi, int& lo) {
+    const int q = r / p.gqa;
+    if (p.prefill) {
+      hi = p.n + q + 1;
+      lo = p.window > 0 ? max(0, hi - p.window) : 0;
+    } else {
+      const int n = max(min(p.seq_lens[q], p.n_clamp), 0);
+      const int W = p.windows ? p.windows[q] : p.window;
+      hi = min(n, p.shared);
+      lo = W > 0 ? max(0, n - W) : 0;
+    }
+  };
+  int hi_w, lo_w;
+  {
+    int h, l;
+    limits(min(r0 + lane, total - 1), h, l);  // lane: row (kRows of them)
+    hi_w = __builtin_amdgcn_readfirstlane(wave_max_i(h));
+    lo_w = __builtin_amdgcn_readfirstlane(wave_min_i(l));
+  }
+  const int end = (hi_w + TK - 1) / TK;
+  const int ns = min(p.sinks / TK + (p.sinks % TK != 0), end);  // tiles that hold sinks
+  const int skip = max(0, min(lo_w / TK, end) - ns);            // tiles between those and the window's
+  const int nt = end - skip;
+  const int per = (nt + p.splits - 1) / p.splits;
+  const int it0 = min(static_cast<int>(blockIdx.y) * per, nt), it1 = min(it0 + per, nt);
+  int pages = -1;  // lane i: page of part i % KH of tile it + i / KH
+  const auto load_pages = [&](int it) {
+    if (nt > 0) {
+      const int v = min(it + lane / KH, nt - 1);
+      const int key = TK * (v + (v < ns ? 0 : skip)) + 32 * (lane % KH);
+      pages = p.tables[min(key >> p.page_shift, p.max_pages - 1)];
+    }
+  };
+  const auto tile_at = [&](int it) {
+    const int i = (it - it0) % (64 / KH);
+    if (it != it0 && i == 0) {  // waited for in here: the steady loop waits for nothing
+      load_pages(it);
+      asm volatile("" : "+v"(pages));
+    }
+    PgTile<KH> t;
+    t.key = TK * (it + (it < ns ? 0 : skip));
+#pragma unroll
+    for (int h = 0; h < KH; ++h) {
+      const int e = __builtin_amdgcn_readlane(pages, i * KH + h);
+      t.has[h] = static_cast<unsigned>(e) < static_cast<unsigned>(p.num_pages);
+      t.row[h] = ((static_cast<int64_t>(t.has[h] ? e : 0) * p.Hkv + kvh) << p.page_shift) +
+                 ((t.key + 32 * h) & ((1 << p.page_shift) - 1));
+    }
+    return t;
+  };
+  load_pages(it0);
+
+  const int rw = r0 + 16 * rs;              // the wave's first row
+  const int R = min(rw + m, total - 1);     // this lane's row (column m)
+  const int qi = R / p.gqa;
+  int hi, lo;
+  limits(R, hi, lo);
+  // over the wave's rows
+  const int hi_max = __builtin_amdgcn_readfirstlane(wave_max_i(hi)), hi_min = __builtin_amdgcn_readfirstlane(wave_min_i(hi));
+  const int lo_max = __builtin_amdgcn_readfirstlane(wave_max_i(lo)), lo_min = __builtin_amdgcn_readfirstlane(wave_min_i(lo));
+
+  PgTile<KH> cur = tile_at(it0), nxt = cur;
+  PfRaw<Gm> raw;
+  pg_load<Gm>(raw, p, cur, hi_w);
+
+  // ---- q: B operands of k-step s of group g are dims 64 g + 16 c + 8 s + {0, 4,
+  // 1, 5, 2, 6, 3, 7}, times 2^(15 - ex) (the row's largest below 2^15), the odd
+  // ones over 16; fp32 queries in two fp16 parts.  The sign of a negative scale
+  // goes into q.
+  v8h qf[2 * NWG], ql[Q32 ? 2 * NWG : 1], qb;
+  const int64_t qrow = static_cast<int64_t>(qi) * p.Hq + kvh * p.gqa + (R - qi * p.gqa);
+  float f[2 * NWG][8];
+  float mx = 0.0f;
+#pragma unroll
+  for (int j = 0; j < 2 * NWG; ++j) {
+    const int64_t e0 = qrow * D + Gm::OW * dh + 64 * (j >> 1) + 16 * c + 8 * (j & 1);
+    if constexpr (Q32) {
+      const v4f* src = reinterpret_cast<const v4f*>(static_cast<const float*>(p.q) + e0);
+      const v4f a = src[0], b = src[1];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        f[j][i] = a[i];
+        f[j][4 + i] = b[i];
+      }
+    } else {
+      const uint4 u = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.q) + e0);
+      const uint32_t wd[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (p.q_dtype == TQ_F16) {
+          const v2h h = __builtin_bit_cast(v2h, wd[i]);
+          f[j][2 * i] = static_cast<float>(h[0]);
+          f[j][2 * i + 1] = static_cast<float>(h[1]);
+        } else {
+          f[j][2 * i] = __uint_as_float(wd[i] << 16);
+          f[j][2 * i + 1] = __uint_as_float(wd[i] & 0xFFFF0000u);
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) mx = fmaxf(mx, fabsf(f[j][i]));
+  }
+  mx = xor32_max(xor16_max(mx));
+  const int ex = __builtin_amdgcn_frexp_expf(mx);
+  const float rf = ldexpf(fabsf(p.scale_log2), ex - 15);  // score = rf * products
+  const bool neg = p.scale_log2 < 0.0f;
+  float qs[NWG];
+#pragma unroll
+  for (int g = 0; g < NWG; ++g) qs[g] = 0.0f;
+#pragma unroll
+  for (int j = 0; j < 2 * NWG; ++j) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      float x = ldexpf(f[j][i], 15 - ex);
+      x = neg ? -x : x;
+      qs[j >> 1] += x;
+      const int slot = (i & 2) ? 4 + 2 * (i & 1) + (i >> 2) : 2 * (i & 1) + (i >> 2);
+      const float y = (i & 1) ? x * 0.0625f : x;
+      if constexpr (Q32) {
+        // one rounding for both parts: the remainder is of the part that is stored
+        uint32_t hb = __builtin_bit_cast(uint16_t, static_cast<_Float16>(y));
+        asm("" : "+v"(hb));
+        const _Float16 h = __builtin_bit_cast(_Float16, static_cast<uint16_t>(hb));
+        qf[j][slot] = h;
+        ql[j][slot] = static_cast<_Float16>(y - static_cast<float>(h));
+      } else {
+        qf[j][slot] = static_cast<_Float16>(y);
+      }
+    }
+  }
+  // group sums over 512 (|.| < 2^12).  fp16 scale/bias: part c of three fp16
+  // parts in lane group c for the biases, 8 times it for the scales; fp32: kept
+  // in fp32.
+#pragma unroll
+  for (int g = 0; g < NWG; ++g) qs[g] = xor32_sum(xor16_sum(qs[g])) * 0x1p-9f;
+#pragma unroll
+  for (int g = 0; g < 4; ++g) {
+    _Float16 pt = static_cast<_Float16>(0.0f);
+    if (!F32 && g < NWG) {
+      float x = qs[g < NWG ? g : 0];
+      const _Float16 h0 = static_cast<_Float16>(x);
+      x -= static_cast<float>(h0);
+      const _Float16 h1 = static_cast<_Float16>(x);
+      x -= static_cast<float>(h1);
+      const _Float16 h2 = static_cast<_Float16>(x);
+      pt = c == 0 ? h0 : c == 1 ? h1 : c == 2 ? h2 : pt;
+    }
+    qb[g] = pt;
+    qb[4 + g] = pt * static_cast<_Float16>(8.0f);
+  }
+
+  if (threadIdx.x == 0) vmx = 0;
+  __syncthreads();
+  const float wm = pf_vmax<Gm>(raw);
+  if (lane == 0) atomicMax(&vmx, __float_as_uint(wm));
+  pf_store<Gm>(L.st, raw, 0);
+  __syncthreads();
+  // (a first tile outside these bounds, like an infinity, is not alike)
+  const int e0 = min(max(__builtin_amdgcn_frexp_expf(__uint_as_float(__builtin_amdgcn_readfirstlane(vmx))), -20), 24);
+  pf_alike<Gm>(raw, e0, alike[0]);
+  __syncthreads();
+
+  // p = 2^(x - m_ref), m_ref = a score of the row + e0 - kPfHead, the largest so
+  // far up to kPfLazy
+  float m_ref = -INFINITY, l_run = 0.0f, bsum[NWG];
+  v4f o[4 * NWG];
+#pragma unroll
+  for (int b = 0; b < 4 * NWG; ++b) o[b] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+  for (int g = 0; g < NWG; ++g) bsum[g] = 0.0f;
+  const v4f z = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+
+#pragma unroll 1
+  for (int it = it0; it < it1; ++it) {
+    const int buf = (it - it0) & 1;
+    if (it + 1 < it1) {
+      nxt = tile_at(it + 1);
+      pg_load<Gm>(raw, p, nxt, hi_w);
+    }
+    const int t0 = cur.key + 32 * kh;  // this wave's keys t0 .. t0 + 31
+    const bool has = KH == 2 && kh ? cur.has[KH - 1] : cur.has[0];
+    const bool any = has && rw < total && t0 < hi_max && (t0 + 31 >= lo_min || t0 < p.sinks);  // wave-uniform
+    // this wave's groups
+    const u32x4* ku = L.st.k[buf] + 2 * kh * Gm::KU + 128 * NWG * dh + 16 * c;
+    const u32x4* vu = L.st.v[buf] + kh * Gm::VU + 256 * NWG * dh + 16 * c;
+    const SB* sks = L.st.sb[buf][0] + 32 * kh * NG + NWG * dh;
+    const SB* skb = L.st.sb[buf][1] + 32 * kh * NG + NWG * dh;
+    const SB* svs = L.st.sb[buf][2] + 32 * kh * NG + NWG * dh;
+    const SB* svb = L.st.sb[buf][3] + 32 * kh * NG + NWG * dh;
+
+    float sc[8];
+    if (any) {
+      // ---- S^T: two 16-key halves ------------------------------------------
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        v4f bt = z;
+        if constexpr (!F32) {
+          v8h kb;
+          const SB* br = skb + (16 * h + m) * NG;
+          const SB* sr = sks + (16 * h + m) * NG;
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            const _Float16 zero = static_cast<_Float16>(0.0f);
+            kb[g] = g < NWG ? br[g < NWG ? g : 0] : zero;
+            kb[4 + g] = g < NWG ? sr[g < NWG ? g : 0] : zero;
+          }
+          bt = __builtin_amdgcn_mfma_f32_16x16x32_f16(kb, qb, z, 0, 0, 0);
+        }
+        v4f acc[NWG];
+#pragma unroll
+        for (int g = 0; g < NWG; ++g) {
+          const u32x4* kr = ku + h * Gm::KU + 128 * g + (m ^ Gm::kswz(NWG * dh + g));
+          const v8h a0 = __builtin_bit_cast(v8h, kr[0]), a1 = __builtin_bit_cast(v8h, kr[64]);
+          v4f a = __builtin_amdgcn_mfma_f32_16x16x32_f16(a0, qf[2 * g], z, 0, 0, 0);
+          a = __builtin_amdgcn_mfma_f32_16x16x32_f16(a1, qf[2 * g + 1], a, 0, 0, 0);
+          if constexpr (Q32) {
+            a = __builtin_amdgcn_mfma_f32_16x16x32_f16(a0, ql[2 * g], a, 0, 0, 0);
+            a = __builtin_amdgcn_mfma_f32_16x16x32_f16(a1, ql[2 * g + 1], a, 0, 0, 0);
+          }
+          acc[g] = a;
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int key = (16 * h + 4 * c + i) * NG;
+          float s = bt[i] * 512.0f;
+#pragma unroll
+          for (int g = 0; g < NWG; ++g) {
+            if constexpr (F32) {
+              // b' = b + 8 s
+              const float ks = sks[key + g];
+              s = fmaf(fmaf(ks, 8.0f, skb[key + g]) * 512.0f, qs[g], s);
+              s = fmaf(ks, acc[g][i], s);
+            } else {
+              s = fmaf(static_cast<float>(sks[key + g]), acc[g][i], s);
+            }
+          }
+          sc[4 * h + i] = s * rf;
+        }
+      }
+    }
+    if constexpr (DH == 2) {
+      // the other wave's groups: its parts of the same scores
+      if (any) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          L.st.xch[wave][h][lane] = v4f{sc[4 * h], sc[4 * h + 1], sc[4 * h + 2], sc[4 * h + 3]};
+      }
+      __syncthreads();
+      if (any) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const v4f x = L.st.xch[wave ^ RS][h][lane];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) sc[4 * h + i] += x[i];
+        }
+      }
+    }
+    if (any) {
+      // whether all of these keys are attended by all rows; wave-uniform
+      const bool inside = t0 <= hi_min - 32 && (t0 >= lo_max || t0 <= p.sinks - 32);
+      if (!inside) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const int t = t0 + 16 * (j >> 2) + 4 * c + (j & 3);
+          sc[j] = t < hi && (t >= lo || t < p.sinks) ? sc[j] : -INFINITY;
+        }
+      }
+
+      // ---- online softmax (log2 domain) of rows m ------------------------------
+      const float up = static_cast<float>(e0 - kPfHead);
+      float mt = sc[0];
+#pragma unroll
+      for (int j = 1; j < 8; ++j) mt = fmaxf(mt, sc[j]);
+      const float need = xor32_max(xor16_max(mt)) + up;
+      // (a row with nothing attended yet and nothing here keeps -inf)
+      if (__any(need > m_ref + kPfLazy)) {
+        const float m_new = need > m_ref ? need : m_ref;
+        const float fr = m_new == m_ref ? 1.0f : merge_factor(m_ref, m_new);
+        l_run *= fr;
+#pragma unroll
+        for (int b = 0; b < 4 * NWG; ++b) o[b] *= fr;
+#pragma unroll
+        for (int g = 0; g < NWG; ++g) bsum[g] *= fr;
+        m_ref = m_new;
+      }
+      float pw[8];
+      // (with nothing attended so far, -inf - -inf would be NaN)
+      const float ms = m_ref == -INFINITY ? 0.0f : m_ref;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        pw[j] = fast_exp2(sc[j] - ms);
+        l_run += pw[j];
+      }
+
+      // ---- O^T += V^T P^T ----------------------------------------------------
+      // B operands of eight weights, and O^T's 16 dims x of group g
+      const auto split = [&](const float (&y)[8], v8h& bh, v8h& bl) {
+        u32x4 hw, lw;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          hw[q] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(y[2 * q], y[2 * q + 1]));
+          lw[q] = pf_rem_pair(hw[q], y[2 * q], y[2 * q + 1]);
+        }
+        bh = __builtin_bit_cast(v8h, hw);
+        bl = __builtin_bit_cast(v8h, lw);
+      };
+      float pz[8];  // the weights of the common products
+#pragma unroll
+      for (int j = 0; j < 8; ++j) pz[j] = pw[j];
+      int al = 1;
+#pragma unroll
+      for (int i = 0; i < Gm::NSW; ++i) al &= alike[buf][i];
+      if (!__builtin_amdgcn_readfirstlane(al)) {
+        // V scales apart: the largest weight of every row and group to 2^13 .. 2^14
+        // (an infinity, of exponent 0, stays one), the products on their own, added
+        // in fp32
+#pragma unroll
+        for (int g = 0; g < NWG; ++g) {
+          float y[8], big = 0.0f;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const float s = static_cast<float>(svs[(16 * (j >> 2) + 4 * c + (j & 3)) * NG + g]);
+            y[j] = pw[j] > 0.0f || pw[j] != pw[j] ? s * pw[j] : 0.0f;
+            big = fmaxf(big, fabsf(y[j]));
+          }
+          const int k = min(14 - __builtin_amdgcn_frexp_expf(xor32_max(xor16_max(big))), 120);
+          const float un = ldexpf(1.0f, -k);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) y[j] = ldexpf(y[j], k);
+          v8h bh, bl;
+          split(y, bh, bl);
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            const v8h a = __builtin_bit_cast(v8h, vu[(4 * g + x) * 64 + (m ^ Gm::vswz(g))]);
+            v4f t = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, bh, z, 0, 0, 0);
+            t = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, bl, t, 0, 0, 0);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[4 * g + x][i] = fmaf(t[i], un, o[4 * g + x][i]);
+          }
+        }
+        // (nothing is left for the products below: a branch around them costs registers)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) pz[j] = 0.0f;
+      }
+      SB s[8][NWG], bb[8][NWG];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int key = 16 * (j >> 2) + 4 * c + (j & 3);
+#pragma unroll
+        for (int g = 0; g < NWG; ++g) {
+          s[j][g] = svs[key * NG + g];
+          bb[j][g] = svb[key * NG + g];
+        }
+      }
+      if (!inside) {
+        // keys that this row does not attend (or with a weight of 0)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const bool none = pw[j] == 0.0f;
+#pragma unroll
+          for (int g = 0; g < NWG; ++g) {
+            s[j][g] = none ? static_cast<SB>(0.0f) : s[j][g];
+            bb[j][g] = none ? static_cast<SB>(0.0f) : bb[j][g];
+          }
+        }
+      }
+#pragma unroll
+      for (int g = 0; g < NWG; ++g) {
+        v8h bh, bl;
+        float y[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          y[j] = fmaf(static_cast<float>(s[j][g]), pz[j], 0.0f);
+          // b' = b + 8 s
+          bsum[g] = fmaf(fmaf(static_cast<float>(s[j][g]), 8.0f, static_cast<float>(bb[j][g])), pw[j], bsum[g]);
+        }
+        split(y, bh, bl);
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          const v8h a = __builtin_bit_cast(v8h, vu[(4 * g + x) * 64 + (m ^ Gm::vswz(g))]);
+          v4f& acc = o[4 * g + x];
+          acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, bh, acc, 0, 0, 0);
+          acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, bl, acc, 0, 0, 0);
+        }
+      }
+    }
+    if (it + 1 < it1) {
+      pf_store<Gm>(L.st, raw, buf ^ 1);
+      pf_alike<Gm>(raw, e0, alike[buf ^ 1]);
+    }
+    cur = nxt;
+    __syncthreads();
+  }
+
+  // ---- merge of the KH partials of every row, and the output ------------------
+  const float un = c < 2 ? 1.0f : 0.0625f;  // odd nibbles (rows 8-15) were 16 times as large
+  const float lt = xor32_sum(xor16_sum(l_run));
+  if (c == 0) {
+    ml[wave][m] = m_ref;
+    ll[wave][m] = lt;
+  }
+  float* orow = L.o[wave] + m * Gm::OSTR;
+#pragma unroll
+  for (int g = 0; g < NWG; ++g) {
+    const float bg = xor32_sum(xor16_sum(bsum[g]));
+#pragma unroll
+    for (int x = 0; x < 4; ++x)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        orow[64 * g + 8 * (4 * (c & 1) + i) + 2 * x + (c >> 1)] = fmaf(o[4 * g + x][i], un, bg);
+  }
+  __syncthreads();
+  for (int u = threadIdx.x; u < kRows * (D / 2); u += Gm::NT) {
+    // a wave's 64 units lie in one row and in one wave's dims
+    const int r = __builtin_amdgcn_readfirstlane(u / (D / 2)), d = 2 * (u % (D / 2));
+    const int Ro = r0 + r;
+    if (Ro >= total) break;
+    const int rm = r % 16, w0 = r / 16 + RS * KH * (d / Gm::OW);
+    float M = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < KH; ++k) M = fmaxf(M, ml[w0 + RS * k][rm]);
+    float l = 0.0f, x0 = 0.0f, x1 = 0.0f;
+#pragma unroll
+    for (int k = 0; k < KH; ++k) {
+      const int wv = w0 + RS * k;
+      const float fk = merge_factor(ml[wv][rm], M);
+      const float2 v = *reinterpret_cast<const float2*>(&L.o[wv][rm * Gm::OSTR + d % Gm::OW]);
+      l = fmaf(ll[wv][rm], fk, l);
+      x0 = fmaf(v.x, fk, x0);
+      x1 = fmaf(v.y, fk, x1);
+    }
+    const int qo = Ro / p.gqa;
+    const int64_t row = static_cast<int64_t>(qo) * p.Hq + kvh * p.gqa + (Ro - qo * p.gqa);
+    if (p.ext_merge == 0) {
+      *reinterpret_cast<float2*>(p.out + row * D + d) = make_float2(normalise(x0, l, 0.0f), normalise(x1, l, 0.0f));
+    } else {
+      const int64_t slot = row * p.max_splits + blockIdx.y;
+      *reinterpret_cast<float2*>(p.ws_o + slot * D + d) = make_float2(x0, x1);
+      if (d == 0) *reinterpret_cast<float2*>(p.ws_ml + slot * 2) = make_float2(M, l);
+    }
+  }
+}
+
+// The output of a row from its S partials: a thread takes four dims.
+__global__ __launch_bounds__(256) void merge_tiles_kernel(const float* ws_ml, const float* ws_o, float* out,
+                                                          int64_t rows, int S, int stride, int D4) {
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  if (i >= rows * D4) return;
+  const int64_t row = i / D4;
+  const int d4 = static_cast<int>(i - row * D4);
+  const float2* ml = reinterpret_cast<const float2*>(ws_ml) + row * stride;
+  const v4f* po = reinterpret_cast<const v4f*>(ws_o) + row * stride * D4 + d4;
+  float M = -INFINITY, L = 0.0f;
+  for (int k = 0; k < S; ++k) M = fmaxf(M, ml[k].x);
+  v4f O = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+  for (int k = 0; k < S; ++k) {
+    const float fk = merge_factor(ml[k].x, M);
+    L = fmaf(ml[k].y, fk, L);
+    O += fk * po[static_cast<int64_t>(k) * D4];
+  }
+  v4f r;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) r[e] = normalise(O[e], L, 0.0f);
+  reinterpret_cast<v4f*>(out)[i] = r;
+}
+
+template <int D, bool F32>
+void launch_q(const TileParams& p, dim3 grid, hipStream_t s) {
+  if (p.q_dtype == TQ_F32) paged_tiles_kernel<D, F32, true><<<grid, 128 * kRs, 0, s>>>(p);
+  else paged_tiles_kernel<D, F32, false><<<grid, 128 * kRs, 0, s>>>(p);
+}
+
+template <bool F32>
+void launch_dim(const TileParams& p, int D, dim3 grid, hipStream_t s) {
+  if (D == 128) launch_q<128, F32>(p, grid, s);
+  else if (D == 256) launch_q<256, F32>(p, grid, s);
+  else launch_q<512, F32>(p, grid, s);
+}
+
+}  // namespace
+
+int paged_tiles_max_splits(int64_t rows, int Hkv, int D, int64_t keys) {
+  const int TK = D == 512 ? 32 : 64;
+  const int64_t wgs = (rows + kRows - 1) / kRows * Hkv, tiles = (keys + TK - 1) / TK;
+  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({64, tiles / 2, (target_wgs() + wgs - 1) / wgs})));
+}
+
+int paged_tiles_splits(int64_t rows, int Hkv, int D, int64_t keys) {
+  const int TK = D == 512 ? 32 : 64;
+  const int64_t wgs = (rows + kRows - 1) / kRows * Hkv, tiles = (keys + TK - 1) / TK;
+  const int64_t cus = target_wgs();
+  // A workgroup fills a CU, and costs its prologue, epilogue and part of the
+  // merge beside its tiles, about kFixed of them: the split of least estimated
+  // time.
+  constexpr int64_t kFixed = 6;
+  int best = 1;
+  int64_t least = INT64_MAX;
+  for (int s = 1; s <= paged_tiles_max_splits(rows, Hkv, D, keys); ++s) {
+    const int64_t cost = (wgs * s + cus - 1) / cus * ((tiles + s - 1) / s + kFixed);
+    if (cost < least) {
+      least = cost;
+      best = s;
+    }
+  }
+  return best;
+}
+
+int launch_paged_tiles(const PagedParams& p0, int D, int sb_dtype, int splits, bool partials, hipStream_t s) {
+  TileParams p;
+  static_cast<PagedParams&>(p) = p0;
+  p.splits = splits;
+  p.ext_merge = partials || splits > 1;
+  const int64_t rows = static_cast<int64_t>(p.nq) * p.gqa;
+  const dim3 grid(static_cast<unsigned>((rows + kRows - 1) / kRows * p.Hkv), splits);
+  if (sb_dtype == TQ_F32) launch_dim<true>(p, D, grid, s);
+  else launch_dim<false>(p, D, grid, s);
+  TQ_CHECK_LAUNCH("paged_tiles_kernel");
+  if (partials || splits == 1) return TQ_OK;
+  const int64_t out_rows = static_cast<int64_t>(p.nq) * p.Hq;
+  merge_tiles_kernel<<<static_cast<unsigned>((out_rows * (D / 4) + 255) / 256), 256, 0, s>>>(
+      p.ws_ml, p.ws_o, p.out, out_rows, splits, p.max_splits, D / 4);
+  TQ_CHECK_LAUNCH("merge_tiles_kernel");
+  return TQ_OK;
+}
+
+}  // namespace tq

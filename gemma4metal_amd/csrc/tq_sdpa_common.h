@@ -221,7 +221,9 @@ __device__ __forceinline__ bool ragged_job(const ParamsOf<PG>& p, int& b, int& h
   const float cus = static_cast<float>(max(p.cus, 1));
   float best = INFINITY;
   chunk = p.chunk;
-  for (int k = 1; k <= p.max_splits; ++k) {  // uniform loop
+  int most = p.max_splits;
+  if constexpr (PG) most -= p.pre;
+  for (int k = 1; k <= most; ++k) {  // uniform loop
     const int cand = max(128, ((lmax + k - 1) / k + 127) / 128 * 128);
     const int jobs = wave_sum_dpp(mine ? (len > 0 ? (len + cand - 1) / cand : 1) : 0);
     const float est = fmaxf(static_cast<float>(kLptFixedKeys + cand),
@@ -729,6 +731,13 @@ int launch_sdpa_hc(const PagedParams& p, int sb_dtype, dim3 grid, hipStream_t st
 int launch_prefill_tiles(const SdpaParams& p, int D, int sb_dtype, hipStream_t stream);
 // The same for fp32 queries, 64 rows (tq_prefill_f32.hip).
 int launch_prefill_tiles_f32(const SdpaParams& p, int D, int sb_dtype, hipStream_t stream);
+// Rows of a paged sequence (prefill) or of a batch's shared prefix on K/V tiles
+// (tq_paged_tiles.hip): the workgroups that share a row's tiles, at most and by
+// plan, and the launch; `partials`: leave (m, l, O) in slots 0 .. splits - 1 of
+// the rows' partials, else write the output.
+int paged_tiles_max_splits(int64_t rows, int Hkv, int D, int64_t keys);
+int paged_tiles_splits(int64_t rows, int Hkv, int D, int64_t keys);
+int launch_paged_tiles(const PagedParams& p, int D, int sb_dtype, int splits, bool partials, hipStream_t stream);
 // Merge of the split partials of a launch with ext_merge = 1 (batch b of
 // grid.y): tq_sdpa_hc.hip.
 int launch_merge_splits(const SdpaParams& p, int D, int batch, hipStream_t stream);
