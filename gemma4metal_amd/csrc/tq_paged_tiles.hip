@@ -32,8 +32,11 @@ struct PgTile {
 
 __device__ __forceinline__ int wave_min_i(int v) { return -wave_max_i(-v); }
 
+// A tile's words and scales into registers.  Every address is a scalar base, a
+// 32-bit lane offset and an immediate; no load is conditional (the wait for one
+// would drain all of them).
 template <class Gm>
-__device__ __forceinline__ void pg_load(PfRaw<Gm>& R, const PagedParams& p, const PgTile<Gm::KH>& t, int hi) {
+__device__ __forceinline__ void pg_load(PfRaw<Gm>& R, const PagedParams& p, const PgTile<Gm::KH>& t) {
   constexpr int KH = Gm::KH;
   // the part of a tile row; the same for a wave's 64 units where those span at
   // most one part
@@ -46,8 +49,9 @@ __device__ __forceinline__ void pg_load(PfRaw<Gm>& R, const PagedParams& p, cons
     if (role == 0) {
       const int r = u / Gm::NG;
       const int64_t base = KH == 2 && part(r) ? t.row[KH - 1] : t.row[0];
-      const u32x4* src = reinterpret_cast<const u32x4*>(p.kq + base * Gm::W) + ((r & 31) * (Gm::W / 4) + 2 * (u % Gm::NG));
-      const u32x4 a = src[0], b = src[1];
+      const uint32_t off = (r & 31) * (4 * Gm::W) + 32 * (u % Gm::NG);
+      const char* src = reinterpret_cast<const char*>(p.kq + base * Gm::W) + off;
+      const u32x4 a = *reinterpret_cast<const u32x4*>(src), b = *reinterpret_cast<const u32x4*>(src + 16);
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         R.w[i][k] = a[k];
@@ -56,9 +60,11 @@ __device__ __forceinline__ void pg_load(PfRaw<Gm>& R, const PagedParams& p, cons
     } else {  // (threads past the units load one again and do not store it)
       const int w = u % Gm::W, kc = u / Gm::W;  // kc = 4 part + c
       const int64_t base = KH == 2 && part(8 * kc) ? t.row[KH - 1] : t.row[0];
-      const uint32_t* src = p.vq + base * Gm::W;
+      const uint32_t off = 4 * (kc & 3) * (4 * Gm::W) + 4 * w;
+      const char* src = reinterpret_cast<const char*>(p.vq + base * Gm::W) + off;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) R.w[i][j] = src[(4 * (kc & 3) + 16 * (j >> 2) + (j & 3)) * Gm::W + w];
+      for (int j = 0; j < 8; ++j)
+        R.w[i][j] = *reinterpret_cast<const uint32_t*>(src + (16 * (j >> 2) + (j & 3)) * (4 * Gm::W));
     }
   }
 #pragma unroll
@@ -69,20 +75,26 @@ __device__ __forceinline__ void pg_load(PfRaw<Gm>& R, const PagedParams& p, cons
     constexpr int DPR = Gm::SDW / Gm::TK;  // dwords a row
     const void* src = a == 0 ? p.ks : a == 1 ? p.kb : a == 2 ? p.vs : p.vb;
     const int r = d / DPR;
-    const uint32_t* s32 = static_cast<const uint32_t*>(src);
-    uint32_t v;
-    bool has;
-    if constexpr (KH == 2 && DPR == 1) {  // a wave spans both parts
-      const bool second = r >= 32;
-      has = second ? t.has[KH - 1] : t.has[0];
-      v = s32[(second ? t.row[KH - 1] : t.row[0]) + (r & 31)];
-    } else {
-      const int q = part(r);
-      has = KH == 2 && q ? t.has[KH - 1] : t.has[0];
-      v = (s32 + (KH == 2 && q ? t.row[KH - 1] : t.row[0]) * DPR)[(r & 31) * DPR + d % DPR];
-    }
-    // rows past every limit, and those of missing pages, may hold anything
-    R.s[i] = has && t.key + r < hi ? v : 0u;
+    const uint32_t off = (r & 31) * (4 * DPR) + 4 * (d % DPR);
+    int64_t base;
+    if constexpr (KH == 2 && DPR == 1) base = r >= 32 ? t.row[KH - 1] : t.row[0];  // a wave spans both parts
+    else base = KH == 2 && part(r) ? t.row[KH - 1] : t.row[0];
+    R.s[i] = *reinterpret_cast<const uint32_t*>(static_cast<const char*>(src) + base * (4 * DPR) + off);
+  }
+}
+
+// Zeroes the scales and biases of rows past every limit and of missing pages,
+// which may hold anything.
+template <class Gm>
+__device__ __forceinline__ void pg_mask(PfRaw<Gm>& R, const PgTile<Gm::KH>& t, int hi) {
+  constexpr int KH = Gm::KH;
+  if (t.key <= hi - Gm::TK && t.has[0] && t.has[KH - 1]) return;  // uniform, most tiles
+#pragma unroll
+  for (int i = 0; i < Gm::NSD; ++i) {
+    constexpr int DPR = Gm::SDW / Gm::TK;
+    const int r = (threadIdx.x + i * Gm::NT) % Gm::SDW / DPR;
+    const bool has = KH == 2 && r >= 32 ? t.has[KH - 1] : t.has[0];
+    R.s[i] = has && t.key + r < hi ? R.s[i] : 0u;
   }
 }
 
@@ -147,7 +159,7 @@ void paged_tiles_kernel(TileParams p) {
     }
   };
   const auto tile_at = [&](int it) {
-    const int i = (it - it0) % (64 / KH);
+    const int i = (it - it0) & (64 / KH - 1);
     if (it != it0 && i == 0) {  // waited for in here: the steady loop waits for nothing
       load_pages(it);
       asm volatile("" : "+v"(pages));
@@ -176,7 +188,7 @@ void paged_tiles_kernel(TileParams p) {
 
   PgTile<KH> cur = tile_at(it0), nxt = cur;
   PfRaw<Gm> raw;
-  pg_load<Gm>(raw, p, cur, hi_w);
+  pg_load<Gm>(raw, p, cur);
 
   // ---- q: B operands of k-step s of group g are dims 64 g + 16 c + 8 s + {0, 4,
   // 1, 5, 2, 6, 3, 7}, times 2^(15 - ex) (the row's largest below 2^15), the odd
@@ -266,6 +278,7 @@ void paged_tiles_kernel(TileParams p) {
 
   if (threadIdx.x == 0) vmx = 0;
   __syncthreads();
+  pg_mask<Gm>(raw, cur, hi_w);
   const float wm = pf_vmax<Gm>(raw);
   if (lane == 0) atomicMax(&vmx, __float_as_uint(wm));
   pf_store<Gm>(L.st, raw, 0);
@@ -290,7 +303,7 @@ void paged_tiles_kernel(TileParams p) {
     const int buf = (it - it0) & 1;
     if (it + 1 < it1) {
       nxt = tile_at(it + 1);
-      pg_load<Gm>(raw, p, nxt, hi_w);
+      pg_load<Gm>(raw, p, nxt);
     }
     const int t0 = cur.key + 32 * kh;  // this wave's keys t0 .. t0 + 31
     const bool has = KH == 2 && kh ? cur.has[KH - 1] : cur.has[0];
@@ -500,6 +513,7 @@ void paged_tiles_kernel(TileParams p) {
       }
     }
     if (it + 1 < it1) {
+      pg_mask<Gm>(raw, nxt, hi_w);
       pf_store<Gm>(L.st, raw, buf ^ 1);
       pf_alike<Gm>(raw, e0, alike[buf ^ 1]);
     }
