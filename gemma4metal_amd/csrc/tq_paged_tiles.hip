@@ -32,11 +32,39 @@ struct PgTile {
 
 __device__ __forceinline__ int wave_min_i(int v) { return -wave_max_i(-v); }
 
-// A tile's words and scales into registers.  Every address is a scalar base, a
-// 32-bit lane offset and an immediate; no load is conditional (the wait for one
-// would drain all of them).
+// Raw loads behind a uniform address: a 32-bit lane offset beside the scalar base,
+// where global loads of this kernel took 64-bit addresses in vector registers.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t pg_rsrc(const void* base) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, 0x7FFFFFFF, 0x00020000);
+}
+
+// The tensors a wave stages from: of its words (K or V) per unit, and of its
+// scales or biases.
 template <class Gm>
-__device__ __forceinline__ void pg_load(PfRaw<Gm>& R, const PagedParams& p, const PgTile<Gm::KH>& t) {
+struct PgSource {
+  const char* w[Gm::NU];
+  const char* s[Gm::NSD];
+};
+
+template <class Gm>
+__device__ __forceinline__ PgSource<Gm> pg_source(const PagedParams& p) {
+  PgSource<Gm> r;
+#pragma unroll
+  for (int i = 0; i < Gm::NU; ++i)
+    r.w[i] = reinterpret_cast<const char*>(
+        __builtin_amdgcn_readfirstlane((threadIdx.x + i * Gm::NT) / Gm::UNITS) == 0 ? p.kq : p.vq);
+#pragma unroll
+  for (int i = 0; i < Gm::NSD; ++i) {
+    const int a = __builtin_amdgcn_readfirstlane((threadIdx.x + i * Gm::NT) / Gm::SDW);
+    r.s[i] = static_cast<const char*>(a == 0 ? p.ks : a == 1 ? p.kb : a == 2 ? p.vs : p.vb);
+  }
+  return r;
+}
+
+// A tile's words and scales into registers.  No load is conditional (the wait for
+// one would drain all of them).
+template <class Gm>
+__device__ __forceinline__ void pg_load(PfRaw<Gm>& R, const PgSource<Gm>& from, const PgTile<Gm::KH>& t) {
   constexpr int KH = Gm::KH;
   // the part of a tile row; the same for a wave's 64 units where those span at
   // most one part
@@ -50,8 +78,9 @@ __device__ __forceinline__ void pg_load(PfRaw<Gm>& R, const PagedParams& p, cons
       const int r = u / Gm::NG;
       const int64_t base = KH == 2 && part(r) ? t.row[KH - 1] : t.row[0];
       const uint32_t off = (r & 31) * (4 * Gm::W) + 32 * (u % Gm::NG);
-      const char* src = reinterpret_cast<const char*>(p.kq + base * Gm::W) + off;
-      const u32x4 a = *reinterpret_cast<const u32x4*>(src), b = *reinterpret_cast<const u32x4*>(src + 16);
+      const auto src = pg_rsrc(from.w[i] + base * (4 * Gm::W));
+      const u32x4 a = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(src, off, 0, 0));
+      const u32x4 b = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(src, off, 16, 0));
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         R.w[i][k] = a[k];
@@ -61,25 +90,27 @@ __device__ __forceinline__ void pg_load(PfRaw<Gm>& R, const PagedParams& p, cons
       const int w = u % Gm::W, kc = u / Gm::W;  // kc = 4 part + c
       const int64_t base = KH == 2 && part(8 * kc) ? t.row[KH - 1] : t.row[0];
       const uint32_t off = 4 * (kc & 3) * (4 * Gm::W) + 4 * w;
-      const char* src = reinterpret_cast<const char*>(p.vq + base * Gm::W) + off;
+      const auto src = pg_rsrc(from.w[i] + base * (4 * Gm::W));
 #pragma unroll
       for (int j = 0; j < 8; ++j)
-        R.w[i][j] = *reinterpret_cast<const uint32_t*>(src + (16 * (j >> 2) + (j & 3)) * (4 * Gm::W));
+        R.w[i][j] = __builtin_amdgcn_raw_buffer_load_b32(src, off, (16 * (j >> 2) + (j & 3)) * (4 * Gm::W), 0);
     }
   }
 #pragma unroll
   for (int i = 0; i < Gm::NSD; ++i) {
     const int e = threadIdx.x + i * Gm::NT;
     // (threads past the tensors load one again and do not store it)
-    const int a = min(__builtin_amdgcn_readfirstlane(e / Gm::SDW), 3), d = e % Gm::SDW;
+    const int d = e % Gm::SDW;
     constexpr int DPR = Gm::SDW / Gm::TK;  // dwords a row
-    const void* src = a == 0 ? p.ks : a == 1 ? p.kb : a == 2 ? p.vs : p.vb;
     const int r = d / DPR;
     const uint32_t off = (r & 31) * (4 * DPR) + 4 * (d % DPR);
-    int64_t base;
-    if constexpr (KH == 2 && DPR == 1) base = r >= 32 ? t.row[KH - 1] : t.row[0];  // a wave spans both parts
-    else base = KH == 2 && part(r) ? t.row[KH - 1] : t.row[0];
-    R.s[i] = *reinterpret_cast<const uint32_t*>(static_cast<const char*>(src) + base * (4 * DPR) + off);
+    if constexpr (KH == 2 && DPR == 1) {  // a wave spans both parts
+      const int64_t base = r >= 32 ? t.row[KH - 1] : t.row[0];
+      R.s[i] = *reinterpret_cast<const uint32_t*>(from.s[i] + base * (4 * DPR) + off);
+    } else {
+      const int64_t base = KH == 2 && part(r) ? t.row[KH - 1] : t.row[0];
+      R.s[i] = __builtin_amdgcn_raw_buffer_load_b32(pg_rsrc(from.s[i] + base * (4 * DPR)), off, 0, 0);
+    }
   }
 }
 
@@ -98,6 +129,87 @@ __device__ __forceinline__ void pg_mask(PfRaw<Gm>& R, const PgTile<Gm::KH>& t, i
   }
 }
 
+// LDS of a workgroup: the operand images of PfGeom, K scales and biases by key,
+// and what the V products take by group: scales and biases (fp32 caches), and the
+// rows of the bias products' A operand in fp16 -- bias and scale of a group (fp16
+// caches), or high and low parts of both, over 2^e0 (fp32).
+template <int D, bool F32>
+struct PgStage {
+  using Gm = PfGeom<D, F32, kRs>;
+  using SB = typename Gm::SB;
+  static constexpr int NP = F32 ? 4 : 2;       // fp16 rows of a group
+  static constexpr int TKP = Gm::TK + 8;       // (rows apart in the banks)
+  u32x4 k[2][2 * Gm::KH * Gm::KU];
+  u32x4 v[2][Gm::KH * Gm::VU];
+  SB ksb[2][2][Gm::TK * Gm::NG];               // k scale, k bias: [key][group]
+  _Float16 vp[2][NP][Gm::NG][TKP];
+  float vsb[F32 ? 2 : 1][2][F32 ? Gm::NG : 1][F32 ? Gm::TK + 4 : 4];  // fp32 scale, bias
+  _Float16 one[TKP], zero[TKP];
+  v4f xch[Gm::DH == 2 ? Gm::NW : 1][2][64];    // score parts of a row set's waves
+};
+
+// Scales and biases from registers into LDS buffer b.
+template <int D, bool F32>
+__device__ __forceinline__ void pg_store_sb(PgStage<D, F32>& S, const PfRaw<PfGeom<D, F32, kRs>>& R, int b, int e0) {
+  using St = PgStage<D, F32>;
+  using Gm = typename St::Gm;
+  constexpr int DPR = Gm::SDW / Gm::TK;
+#pragma unroll
+  for (int i = 0; i < Gm::NSD; ++i) {
+    const int e = threadIdx.x + i * Gm::NT;
+    const int t = __builtin_amdgcn_readfirstlane(e / Gm::SDW), d = e % Gm::SDW;
+    const uint32_t a = R.s[i];
+    if (t < 2) {
+      reinterpret_cast<uint32_t*>(S.ksb[b][t])[d] = a;
+    } else if (t < 4) {
+      const int key = d / DPR;
+      if constexpr (F32) {
+        const int g = d % DPR;
+        const float x = ldexpf(__uint_as_float(a), -e0);
+        uint32_t hb = __builtin_bit_cast(uint16_t, static_cast<_Float16>(x));
+        asm("" : "+v"(hb));  // one rounding: the remainder is of the stored part
+        const _Float16 h = __builtin_bit_cast(_Float16, static_cast<uint16_t>(hb));
+        const int part = t == 2 ? 2 : 0;
+        S.vp[b][part][g][key] = h;
+        S.vp[b][part + 1][g][key] = static_cast<_Float16>(x - static_cast<float>(h));
+        S.vsb[b][t - 2][g][key] = __uint_as_float(a);
+      } else {
+        const int g = 2 * (d % DPR);
+        const v2h h = __builtin_bit_cast(v2h, a);
+        S.vp[b][t == 2 ? 1 : 0][g][key] = h[0];
+        S.vp[b][t == 2 ? 1 : 0][g + 1][key] = h[1];
+      }
+    }
+  }
+}
+
+// Whether a tile's V scales are alike (0, or within 2^-kPfDown .. 2^kPfUp of 2^e0) and
+// its V biases of fp16's range (fp32: over 2^e0), per wave that stages some, into
+// ok[2 NSW].
+template <class Gm>
+__device__ __forceinline__ void pg_alike(const PfRaw<Gm>& R, int e0, int* ok) {
+  constexpr bool kHalf = sizeof(typename Gm::SB) == 2;
+  // the bounds' bit patterns (magnitudes order as these do), of 2^k
+  const auto bits = [](int k) -> uint32_t {
+    if constexpr (kHalf) return k > 15 ? 0x7C00u : k >= -14 ? (k + 15) << 10 : k >= -24 ? 1u << (k + 24) : 0u;
+    else return (k + 127) << 23;
+  };
+  const uint32_t lo = bits(e0 - kPfDown), n = bits(e0 + kPfUp) - lo;
+  const uint32_t big = kHalf ? 0x7C00u : bits(e0 + 15);
+#pragma unroll
+  for (int i = 0; i < Gm::NSD; ++i) {
+    const int e = threadIdx.x + i * Gm::NT;
+    const int t = __builtin_amdgcn_readfirstlane(e / Gm::SDW);
+    if (t != 2 && t != 3) continue;
+    const auto fine = [&](uint32_t a) { return t == 2 ? a - lo < n || a == 0 : a < big; };
+    const uint32_t a = R.s[i];
+    bool in;
+    if constexpr (kHalf) in = fine(a & 0x7FFFu) && fine(a >> 16 & 0x7FFFu);
+    else in = fine(a & 0x7FFFFFFFu);
+    ok[(t - 2) * Gm::NSW + e % Gm::SDW / 64] = __all(in);  // (one value from every lane)
+  }
+}
+
 struct TileParams : PagedParams {
   int splits;  // workgroups along the tiles (grid y); 1: write p.out
 };
@@ -108,9 +220,14 @@ void paged_tiles_kernel(TileParams p) {
   using Gm = PfGeom<D, F32, kRs>;
   using SB = typename Gm::SB;
   constexpr int NG = Gm::NG, NWG = Gm::NW_, TK = Gm::TK, KH = Gm::KH, DH = Gm::DH, RS = kRs;
-  __shared__ __attribute__((aligned(16))) typename Gm::Lds L;
+  using St = PgStage<D, F32>;
+  __shared__ __attribute__((aligned(16))) union Lds {
+    St st;
+    float o[Gm::NW][16 * Gm::OSTR];
+    __device__ Lds() {}
+  } L;
   __shared__ uint32_t vmx;                  // bits of the first tile's largest |V scale|
-  __shared__ int alike[2][Gm::NSW];         // a buffer's V scales are alike (all of them set)
+  __shared__ int alike[2][2 * Gm::NSW];     // see pg_alike (all of them set)
   __shared__ float ml[Gm::NW][16], ll[Gm::NW][16];
 
   const int lane = threadIdx.x & 63;
@@ -187,8 +304,9 @@ void paged_tiles_kernel(TileParams p) {
   const int lo_max = __builtin_amdgcn_readfirstlane(wave_max_i(lo)), lo_min = __builtin_amdgcn_readfirstlane(wave_min_i(lo));
 
   PgTile<KH> cur = tile_at(it0), nxt = cur;
+  const PgSource<Gm> from = pg_source<Gm>(p);
   PfRaw<Gm> raw;
-  pg_load<Gm>(raw, p, cur);
+  pg_load<Gm>(raw, from, cur);
 
   // ---- q: B operands of k-step s of group g are dims 64 g + 16 c + 8 s + {0, 4,
   // 1, 5, 2, 6, 3, 7}, times 2^(15 - ex) (the row's largest below 2^15), the odd
@@ -277,33 +395,54 @@ void paged_tiles_kernel(TileParams p) {
   }
 
   if (threadIdx.x == 0) vmx = 0;
+  if (threadIdx.x < St::TKP) {
+    L.st.one[threadIdx.x] = static_cast<_Float16>(1.0f);
+    L.st.zero[threadIdx.x] = static_cast<_Float16>(0.0f);
+  }
   __syncthreads();
   pg_mask<Gm>(raw, cur, hi_w);
   const float wm = pf_vmax<Gm>(raw);
   if (lane == 0) atomicMax(&vmx, __float_as_uint(wm));
-  pf_store<Gm>(L.st, raw, 0);
   __syncthreads();
   // (a first tile outside these bounds, like an infinity, is not alike)
   const int e0 = min(max(__builtin_amdgcn_frexp_expf(__uint_as_float(__builtin_amdgcn_readfirstlane(vmx))), -20), 24);
-  pf_alike<Gm>(raw, e0, alike[0]);
+  const auto stage = [&](int b) {
+    pf_store_words<Gm>(L.st, raw, b);
+    pg_store_sb<D, F32>(L.st, raw, b, e0);
+    pg_alike<Gm>(raw, e0, alike[b]);
+  };
+  stage(0);
   __syncthreads();
+
+  // Rows of the bias products' A operand: lane group c's keys of row m = 4 part +
+  // group of this wave's groups; row 8 is 1 (fp16 caches: the sum of the weights).
+  // Weights go in times 2^(e0 + 2), below 2^14; sums come out times 1 / bun.
+  const _Float16* brow = L.st.zero;
+  int bstep = 0;
+  if (m / 4 < St::NP && m % 4 < NWG) {
+    brow = &L.st.vp[0][m / 4][NWG * dh + m % 4][0];
+    bstep = sizeof(L.st.vp[0]) / sizeof(_Float16);
+  } else if (!F32 && m == 8) {
+    brow = L.st.one;
+  }
+  brow += 4 * c + (bstep ? 32 * kh : 0);
+  const float pscale = __uint_as_float((e0 + 2 + 127) << 23);
+  const float bun = F32 ? 0.25f : __uint_as_float((127 - e0 - 2) << 23), bup = F32 ? 4.0f : pscale;
 
   // p = 2^(x - m_ref), m_ref = a score of the row + e0 - kPfHead, the largest so
   // far up to kPfLazy
-  float m_ref = -INFINITY, l_run = 0.0f, bsum[NWG];
-  v4f o[4 * NWG];
-#pragma unroll
-  for (int b = 0; b < 4 * NWG; ++b) o[b] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-  for (int g = 0; g < NWG; ++g) bsum[g] = 0.0f;
+  float m_ref = -INFINITY, l_run = 0.0f;
   const v4f z = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+  v4f o[4 * NWG], ob = z;
+#pragma unroll
+  for (int b = 0; b < 4 * NWG; ++b) o[b] = z;
 
 #pragma unroll 1
   for (int it = it0; it < it1; ++it) {
     const int buf = (it - it0) & 1;
     if (it + 1 < it1) {
       nxt = tile_at(it + 1);
-      pg_load<Gm>(raw, p, nxt);
+      pg_load<Gm>(raw, from, nxt);
     }
     const int t0 = cur.key + 32 * kh;  // this wave's keys t0 .. t0 + 31
     const bool has = KH == 2 && kh ? cur.has[KH - 1] : cur.has[0];
@@ -311,14 +450,39 @@ void paged_tiles_kernel(TileParams p) {
     // this wave's groups
     const u32x4* ku = L.st.k[buf] + 2 * kh * Gm::KU + 128 * NWG * dh + 16 * c;
     const u32x4* vu = L.st.v[buf] + kh * Gm::VU + 256 * NWG * dh + 16 * c;
-    const SB* sks = L.st.sb[buf][0] + 32 * kh * NG + NWG * dh;
-    const SB* skb = L.st.sb[buf][1] + 32 * kh * NG + NWG * dh;
-    const SB* svs = L.st.sb[buf][2] + 32 * kh * NG + NWG * dh;
-    const SB* svb = L.st.sb[buf][3] + 32 * kh * NG + NWG * dh;
+    const SB* sks = L.st.ksb[buf][0] + 32 * kh * NG + NWG * dh;
+    const SB* skb = L.st.ksb[buf][1] + 32 * kh * NG + NWG * dh;
+    // V operands of group g, and its scales of this lane's 8 keys
+    const auto v_read = [&](int g, u32x4 (&a)[4]) {
+#pragma unroll
+      for (int x = 0; x < 4; ++x) a[x] = vu[(4 * g + x) * 64 + (m ^ Gm::vswz(g))];
+    };
+    typedef typename std::conditional<F32, v4f, v4h>::type s4;
+    const auto s_read = [&](int g, s4 (&s)[2]) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int at = 32 * kh + 16 * h + 4 * c;
+        if constexpr (F32) s[h] = *reinterpret_cast<const s4*>(&L.st.vsb[buf][0][NWG * dh + g][at]);
+        else s[h] = *reinterpret_cast<const s4*>(&L.st.vp[buf][1][NWG * dh + g][at]);
+      }
+    };
 
     float sc[8];
     if (any) {
-      // ---- S^T: two 16-key halves ------------------------------------------
+      // ---- S^T: two 16-key halves.  The operands of GB groups are read at once,
+      // the next ones under the products and scores of these.
+      constexpr int GB = Q32 && NWG > 1 ? NWG / 2 : NWG;
+      u32x4 ka[2 * GB];
+      const auto k_read = [&](int h, int g0) {
+#pragma unroll
+        for (int g = 0; g < GB; ++g) {
+          const u32x4* kr = ku + h * Gm::KU + 128 * (g0 + g) + (m ^ Gm::kswz(NWG * dh + g0 + g));
+          ka[2 * g] = kr[0];
+          ka[2 * g + 1] = kr[64];
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      };
+      k_read(0, 0);
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         v4f bt = z;
@@ -336,16 +500,22 @@ void paged_tiles_kernel(TileParams p) {
         }
         v4f acc[NWG];
 #pragma unroll
-        for (int g = 0; g < NWG; ++g) {
-          const u32x4* kr = ku + h * Gm::KU + 128 * g + (m ^ Gm::kswz(NWG * dh + g));
-          const v8h a0 = __builtin_bit_cast(v8h, kr[0]), a1 = __builtin_bit_cast(v8h, kr[64]);
-          v4f a = __builtin_amdgcn_mfma_f32_16x16x32_f16(a0, qf[2 * g], z, 0, 0, 0);
-          a = __builtin_amdgcn_mfma_f32_16x16x32_f16(a1, qf[2 * g + 1], a, 0, 0, 0);
-          if constexpr (Q32) {
-            a = __builtin_amdgcn_mfma_f32_16x16x32_f16(a0, ql[2 * g], a, 0, 0, 0);
-            a = __builtin_amdgcn_mfma_f32_16x16x32_f16(a1, ql[2 * g + 1], a, 0, 0, 0);
+        for (int g0 = 0; g0 < NWG; g0 += GB) {
+#pragma unroll
+          for (int gi = 0; gi < GB; ++gi) {
+            const int g = g0 + gi;
+            const v8h a0 = __builtin_bit_cast(v8h, ka[2 * gi]), a1 = __builtin_bit_cast(v8h, ka[2 * gi + 1]);
+            v4f a = __builtin_amdgcn_mfma_f32_16x16x32_f16(a0, qf[2 * g], z, 0, 0, 0);
+            a = __builtin_amdgcn_mfma_f32_16x16x32_f16(a1, qf[2 * g + 1], a, 0, 0, 0);
+            if constexpr (Q32) {
+              a = __builtin_amdgcn_mfma_f32_16x16x32_f16(a0, ql[2 * g], a, 0, 0, 0);
+              a = __builtin_amdgcn_mfma_f32_16x16x32_f16(a1, ql[2 * g + 1], a, 0, 0, 0);
+            }
+            acc[g] = a;
           }
-          acc[g] = a;
+          __builtin_amdgcn_sched_barrier(0);
+          if (g0 + GB < NWG) k_read(h, g0 + GB);
+          else if (h == 0) k_read(1, 0);
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -354,10 +524,9 @@ void paged_tiles_kernel(TileParams p) {
 #pragma unroll
           for (int g = 0; g < NWG; ++g) {
             if constexpr (F32) {
-              // b' = b + 8 s
-              const float ks = sks[key + g];
-              s = fmaf(fmaf(ks, 8.0f, skb[key + g]) * 512.0f, qs[g], s);
-              s = fmaf(ks, acc[g][i], s);
+              // s (. + 8 sum q) + b sum q
+              s = fmaf(skb[key + g], qs[g] * 512.0f, s);
+              s = fmaf(sks[key + g], fmaf(qs[g], 4096.0f, acc[g][i]), s);
             } else {
               s = fmaf(static_cast<float>(sks[key + g]), acc[g][i], s);
             }
@@ -387,10 +556,11 @@ void paged_tiles_kernel(TileParams p) {
       // whether all of these keys are attended by all rows; wave-uniform
       const bool inside = t0 <= hi_min - 32 && (t0 >= lo_max || t0 <= p.sinks - 32);
       if (!inside) {
+        const int at = t0 + 4 * c;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          const int t = t0 + 16 * (j >> 2) + 4 * c + (j & 3);
-          sc[j] = t < hi && (t >= lo || t < p.sinks) ? sc[j] : -INFINITY;
+          const int k = 16 * (j >> 2) + (j & 3);
+          sc[j] = k < hi - at && (k >= lo - at || k < p.sinks - at) ? sc[j] : -INFINITY;
         }
       }
 
@@ -405,23 +575,33 @@ void paged_tiles_kernel(TileParams p) {
         const float m_new = need > m_ref ? need : m_ref;
         const float fr = m_new == m_ref ? 1.0f : merge_factor(m_ref, m_new);
         l_run *= fr;
+        ob *= fr;
 #pragma unroll
         for (int b = 0; b < 4 * NWG; ++b) o[b] *= fr;
-#pragma unroll
-        for (int g = 0; g < NWG; ++g) bsum[g] *= fr;
         m_ref = m_new;
       }
+      u32x4 va[4];
+      s4 vs[2][2];
+      v_read(0, va);
+      s_read(0, vs[0]);
+      const u32x2 b0 = *reinterpret_cast<const u32x2*>(brow + buf * bstep);
+      const u32x2 b1 = *reinterpret_cast<const u32x2*>(brow + buf * bstep + 16);
+      int al = 1;
+#pragma unroll
+      for (int i = 0; i < 2 * Gm::NSW; ++i) al &= alike[buf][i];
+      __builtin_amdgcn_sched_barrier(0);
       float pw[8];
       // (with nothing attended so far, -inf - -inf would be NaN)
       const float ms = m_ref == -INFINITY ? 0.0f : m_ref;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        pw[j] = fast_exp2(sc[j] - ms);
-        l_run += pw[j];
+      for (int j = 0; j < 8; ++j) pw[j] = fast_exp2(sc[j] - ms);
+      if constexpr (F32) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) l_run += pw[j];
       }
 
       // ---- O^T += V^T P^T ----------------------------------------------------
-      // B operands of eight weights, and O^T's 16 dims x of group g
+      // B operands of eight weights
       const auto split = [&](const float (&y)[8], v8h& bh, v8h& bl) {
         u32x4 hw, lw;
 #pragma unroll
@@ -432,25 +612,35 @@ void paged_tiles_kernel(TileParams p) {
         bh = __builtin_bit_cast(v8h, hw);
         bl = __builtin_bit_cast(v8h, lw);
       };
-      float pz[8];  // the weights of the common products
-#pragma unroll
-      for (int j = 0; j < 8; ++j) pz[j] = pw[j];
-      int al = 1;
-#pragma unroll
-      for (int i = 0; i < Gm::NSW; ++i) al &= alike[buf][i];
       if (!__builtin_amdgcn_readfirstlane(al)) {
-        // V scales apart: the largest weight of every row and group to 2^13 .. 2^14
-        // (an infinity, of exponent 0, stays one), the products on their own, added
-        // in fp32
-#pragma unroll
+        // V scales apart, or scales and biases out of range or not finite: the
+        // largest weight of every row and group to 2^13 .. 2^14 (an infinity, of
+        // exponent 0, stays one), the products on their own, added in fp32, and
+        // bias terms in fp32 -- without those of weight 0, whose keys the row may
+        // not attend at all
+        const auto times = [](float w, float x) { return w > 0.0f || w != w ? w * x : 0.0f; };
+        float add[4] = {0.0f, 0.0f, 0.0f, 0.0f}, lw = 0.0f;
+#pragma unroll 1
         for (int g = 0; g < NWG; ++g) {
-          float y[8], big = 0.0f;
+          float y[8], big = 0.0f, sb = 0.0f;
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
-            const float s = static_cast<float>(svs[(16 * (j >> 2) + 4 * c + (j & 3)) * NG + g]);
-            y[j] = pw[j] > 0.0f || pw[j] != pw[j] ? s * pw[j] : 0.0f;
+            const int at = 32 * kh + 16 * (j >> 2) + 4 * c + (j & 3);
+            float s, b;
+            if constexpr (F32) {
+              s = L.st.vsb[buf][0][NWG * dh + g][at];
+              b = L.st.vsb[buf][1][NWG * dh + g][at];
+            } else {
+              s = static_cast<float>(L.st.vp[buf][1][NWG * dh + g][at]);
+              b = static_cast<float>(L.st.vp[buf][0][NWG * dh + g][at]);
+            }
+            y[j] = times(pw[j], s);
+            sb += times(pw[j], fmaf(s, 8.0f, b));
             big = fmaxf(big, fabsf(y[j]));
           }
+          sb = xor32_sum(xor16_sum(sb)) * bup;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) add[i] = i == g ? sb : add[i];
           const int k = min(14 - __builtin_amdgcn_frexp_expf(xor32_max(xor16_max(big))), 120);
           const float un = ldexpf(1.0f, -k);
 #pragma unroll
@@ -458,64 +648,60 @@ void paged_tiles_kernel(TileParams p) {
           v8h bh, bl;
           split(y, bh, bl);
 #pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            const v8h a = __builtin_bit_cast(v8h, vu[(4 * g + x) * 64 + (m ^ Gm::vswz(g))]);
-            v4f t = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, bh, z, 0, 0, 0);
-            t = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, bl, t, 0, 0, 0);
+          for (int gg = 0; gg < NWG; ++gg) {
+            if (gg != g) continue;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) o[4 * g + x][i] = fmaf(t[i], un, o[4 * g + x][i]);
+            for (int x = 0; x < 4; ++x) {
+              const v8h a = __builtin_bit_cast(v8h, vu[(4 * gg + x) * 64 + (m ^ Gm::vswz(gg))]);
+              v4f t = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, bh, z, 0, 0, 0);
+              t = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, bl, t, 0, 0, 0);
+#pragma unroll
+              for (int i = 0; i < 4; ++i) o[4 * gg + x][i] = fmaf(t[i], un, o[4 * gg + x][i]);
+            }
           }
         }
-        // (nothing is left for the products below: a branch around them costs registers)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) pz[j] = 0.0f;
-      }
-      SB s[8][NWG], bb[8][NWG];
+        for (int j = 0; j < 8; ++j) lw += pw[j];
+        lw = xor32_sum(xor16_sum(lw)) * bup;
+        // into the rows that hold biases and, for fp16 caches, the weights' sum
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int key = 16 * (j >> 2) + 4 * c + (j & 3);
+        for (int i = 0; i < 4; ++i) ob[i] += c == 0 ? add[i] : 0.0f;
+        if (!F32 && c == 2) ob[0] += lw;
+      } else {
+        const v8h ba = __builtin_bit_cast(v8h, u32x4{b0[0], b0[1], b1[0], b1[1]});
+        {
+          v8h bh, bl;
+          float y[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) y[j] = pw[j] * pscale;
+          split(y, bh, bl);
+          ob = __builtin_amdgcn_mfma_f32_16x16x32_f16(ba, bh, ob, 0, 0, 0);
+          ob = __builtin_amdgcn_mfma_f32_16x16x32_f16(ba, bl, ob, 0, 0, 0);
+        }
 #pragma unroll
         for (int g = 0; g < NWG; ++g) {
-          s[j][g] = svs[key * NG + g];
-          bb[j][g] = svb[key * NG + g];
-        }
-      }
-      if (!inside) {
-        // keys that this row does not attend (or with a weight of 0)
+          if (g + 1 < NWG) s_read(g + 1, vs[(g + 1) & 1]);
+          __builtin_amdgcn_sched_barrier(0);
+          v8h bh, bl;
+          float y[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const bool none = pw[j] == 0.0f;
+          for (int j = 0; j < 8; ++j) y[j] = fmaf(static_cast<float>(vs[g & 1][j >> 2][j & 3]), pw[j], 0.0f);
+          split(y, bh, bl);
 #pragma unroll
-          for (int g = 0; g < NWG; ++g) {
-            s[j][g] = none ? static_cast<SB>(0.0f) : s[j][g];
-            bb[j][g] = none ? static_cast<SB>(0.0f) : bb[j][g];
+          for (int x = 0; x < 4; ++x) {
+            const v8h a = __builtin_bit_cast(v8h, va[x]);
+            v4f& acc = o[4 * g + x];
+            acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, bh, acc, 0, 0, 0);
+            acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, bl, acc, 0, 0, 0);
           }
-        }
-      }
-#pragma unroll
-      for (int g = 0; g < NWG; ++g) {
-        v8h bh, bl;
-        float y[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          y[j] = fmaf(static_cast<float>(s[j][g]), pz[j], 0.0f);
-          // b' = b + 8 s
-          bsum[g] = fmaf(fmaf(static_cast<float>(s[j][g]), 8.0f, static_cast<float>(bb[j][g])), pw[j], bsum[g]);
-        }
-        split(y, bh, bl);
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          const v8h a = __builtin_bit_cast(v8h, vu[(4 * g + x) * 64 + (m ^ Gm::vswz(g))]);
-          v4f& acc = o[4 * g + x];
-          acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, bh, acc, 0, 0, 0);
-          acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, bl, acc, 0, 0, 0);
+          __builtin_amdgcn_sched_barrier(0);
+          if (g + 1 < NWG) v_read(g + 1, va);  // under the next group's weights
         }
       }
     }
     if (it + 1 < it1) {
       pg_mask<Gm>(raw, nxt, hi_w);
-      pf_store<Gm>(L.st, raw, buf ^ 1);
-      pf_alike<Gm>(raw, e0, alike[buf ^ 1]);
+      stage(buf ^ 1);
     }
     cur = nxt;
     __syncthreads();
@@ -523,7 +709,7 @@ void paged_tiles_kernel(TileParams p) {
 
   // ---- merge of the KH partials of every row, and the output ------------------
   const float un = c < 2 ? 1.0f : 0.0625f;  // odd nibbles (rows 8-15) were 16 times as large
-  const float lt = xor32_sum(xor16_sum(l_run));
+  const float lt = F32 ? xor32_sum(xor16_sum(l_run)) : xor32_sum(xor16_sum(c == 2 ? ob[0] : 0.0f)) * bun;
   if (c == 0) {
     ml[wave][m] = m_ref;
     ll[wave][m] = lt;
@@ -531,7 +717,10 @@ void paged_tiles_kernel(TileParams p) {
   float* orow = L.o[wave] + m * Gm::OSTR;
 #pragma unroll
   for (int g = 0; g < NWG; ++g) {
-    const float bg = xor32_sum(xor16_sum(bsum[g]));
+    // b' = b + 8 s: biases in the rows of lane group 0 (fp32 caches: and 1), scales
+    // in those of 1 (2 and 3)
+    const float bs = c < (F32 ? 2 : 1) ? ob[g] : c < (F32 ? 4 : 2) ? 8.0f * ob[g] : 0.0f;
+    const float bg = xor32_sum(xor16_sum(bs)) * bun;
 #pragma unroll
     for (int x = 0; x < 4; ++x)
 #pragma unroll

@@ -12,6 +12,7 @@ namespace tq {
 namespace {
 
 typedef _Float16 v8h __attribute__((ext_vector_type(8)));
+typedef _Float16 v4h __attribute__((ext_vector_type(4)));
 typedef _Float16 v2h __attribute__((ext_vector_type(2)));
 typedef float v4f __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
@@ -107,9 +108,9 @@ __device__ __forceinline__ void pf_alike(const PfRaw<Gm>& R, int e0, int* ok) {
   }
 }
 
-// Into LDS buffer b.
-template <class Gm>
-__device__ __forceinline__ void pf_store(typename Gm::Stage& S, const PfRaw<Gm>& R, int b) {
+// Words into LDS buffer b.
+template <class Gm, class Stage>
+__device__ __forceinline__ void pf_store_words(Stage& S, const PfRaw<Gm>& R, int b) {
   const uint32_t mlo = 0x000F000Fu, mhi = 0x00F000F0u;
 #pragma unroll
   for (int i = 0; i < Gm::NU; ++i) {
@@ -145,6 +146,12 @@ __device__ __forceinline__ void pf_store(typename Gm::Stage& S, const PfRaw<Gm>&
       }
     }
   }
+}
+
+// Words, scales and biases into LDS buffer b.
+template <class Gm>
+__device__ __forceinline__ void pf_store(typename Gm::Stage& S, const PfRaw<Gm>& R, int b) {
+  pf_store_words<Gm>(S, R, b);
 #pragma unroll
   for (int i = 0; i < Gm::NSD; ++i) {
     const int e = threadIdx.x + i * Gm::NT;
