@@ -467,6 +467,8 @@ void paged_tiles_kernel(TileParams p) {
       }
     };
 
+    u32x2 b0{}, b1{};  // the bias products' operand
+    int al = 1;
     float sc[8];
     if (any) {
       // ---- S^T: two 16-key halves.  The operands of GB groups are read at once,
@@ -483,18 +485,39 @@ void paged_tiles_kernel(TileParams p) {
         __builtin_amdgcn_sched_barrier(0);
       };
       k_read(0, 0);
+      // and the scales and biases: of key m for the bias product, of this lane's
+      // scores (keys 4 c + i); of both halves, or (fp32: registers) of one
+      typedef SB row_t __attribute__((ext_vector_type(NWG)));
+      constexpr int HA = F32 ? 1 : 2;
+      row_t kbr[HA], ksr[HA], sk[HA][4], bk[4];
+      const auto sb_read = [&](int h) {
+        if constexpr (!F32) {
+          kbr[h % HA] = *reinterpret_cast<const row_t*>(skb + (16 * h + m) * NG);
+          ksr[h % HA] = *reinterpret_cast<const row_t*>(sks + (16 * h + m) * NG);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          sk[h % HA][i] = *reinterpret_cast<const row_t*>(sks + (16 * h + 4 * c + i) * NG);
+          if constexpr (F32) bk[i] = *reinterpret_cast<const row_t*>(skb + (16 * h + 4 * c + i) * NG);
+        }
+      };
+#pragma unroll
+      for (int h = 0; h < HA; ++h) sb_read(h);
+      b0 = *reinterpret_cast<const u32x2*>(brow + buf * bstep);
+      b1 = *reinterpret_cast<const u32x2*>(brow + buf * bstep + 16);
+#pragma unroll
+      for (int i = 0; i < 2 * Gm::NSW; ++i) al &= alike[buf][i];
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         v4f bt = z;
         if constexpr (!F32) {
           v8h kb;
-          const SB* br = skb + (16 * h + m) * NG;
-          const SB* sr = sks + (16 * h + m) * NG;
 #pragma unroll
           for (int g = 0; g < 4; ++g) {
             const _Float16 zero = static_cast<_Float16>(0.0f);
-            kb[g] = g < NWG ? br[g < NWG ? g : 0] : zero;
-            kb[4 + g] = g < NWG ? sr[g < NWG ? g : 0] : zero;
+            kb[g] = g < NWG ? kbr[h % HA][g < NWG ? g : 0] : zero;
+            kb[4 + g] = g < NWG ? ksr[h % HA][g < NWG ? g : 0] : zero;
           }
           bt = __builtin_amdgcn_mfma_f32_16x16x32_f16(kb, qb, z, 0, 0, 0);
         }
@@ -517,18 +540,18 @@ void paged_tiles_kernel(TileParams p) {
           if (g0 + GB < NWG) k_read(h, g0 + GB);
           else if (h == 0) k_read(1, 0);
         }
+        if (F32 && h == 1) sb_read(1);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const int key = (16 * h + 4 * c + i) * NG;
           float s = bt[i] * 512.0f;
 #pragma unroll
           for (int g = 0; g < NWG; ++g) {
             if constexpr (F32) {
               // s (. + 8 sum q) + b sum q
-              s = fmaf(skb[key + g], qs[g] * 512.0f, s);
-              s = fmaf(sks[key + g], fmaf(qs[g], 4096.0f, acc[g][i]), s);
+              s = fmaf(bk[i][g], qs[g] * 512.0f, s);
+              s = fmaf(sk[h % HA][i][g], fmaf(qs[g], 4096.0f, acc[g][i]), s);
             } else {
-              s = fmaf(static_cast<float>(sks[key + g]), acc[g][i], s);
+              s = fmaf(static_cast<float>(sk[h % HA][i][g]), acc[g][i], s);
             }
           }
           sc[4 * h + i] = s * rf;
@@ -584,11 +607,6 @@ void paged_tiles_kernel(TileParams p) {
       s4 vs[2][2];
       v_read(0, va);
       s_read(0, vs[0]);
-      const u32x2 b0 = *reinterpret_cast<const u32x2*>(brow + buf * bstep);
-      const u32x2 b1 = *reinterpret_cast<const u32x2*>(brow + buf * bstep + 16);
-      int al = 1;
-#pragma unroll
-      for (int i = 0; i < 2 * Gm::NSW; ++i) al &= alike[buf][i];
       __builtin_amdgcn_sched_barrier(0);
       float pw[8];
       // (with nothing attended so far, -inf - -inf would be NaN)
