@@ -8,6 +8,7 @@
 #include <math.h>
 
 #include <algorithm>
+#include <cstdio>
 
 #include "tq_sdpa_common.h"
 
@@ -59,9 +60,20 @@ int paged_params(PagedParams& p, const void* q, int q_dtype, const uint32_t* kq,
 // GQA a multiple of 8, else sdpa_int4_mfma_kernel, on blocks of 32 keys.
 struct PagedPlan {
   bool hc;
-  int G, n_sub, chunk, max_splits;
-  bool lpt;
+  int G, n_sub, chunk;
+  int max_splits;  // of any sequence
+  int grid_x;      // workgroups per (sequence, head) of the grid, on average
+  bool lpt;        // the device chooses the chunk and orders the jobs (paged_job)
+  int waves;       // of a workgroup
+  int slots;       // workgroups that the chip runs at once
 };
+
+// Splits of a sequence that the device may choose (see plan_paged), from those of
+// equal sequences.
+int lpt_splits(int splits, int len, int64_t groups, int64_t slots) {
+  return static_cast<int>(std::min<int64_t>({2 * static_cast<int64_t>(splits), std::max((static_cast<int64_t>(len) + 127) / 128, int64_t{1}),
+                                             kMaxSplits, 1 + (2 * slots + groups - 1) / groups}));
+}
 
 // max_len: what any sequence attends beside the shared rows, at most.
 PagedPlan plan_paged(int batch, int Hq, int Hkv, int D, int sb_dtype, int max_len) {
@@ -71,18 +83,39 @@ PagedPlan plan_paged(int batch, int Hq, int Hkv, int D, int sb_dtype, int max_le
   pl.G = head_subgroup(gqa);
   while (!pl.hc && pl.G > 1 && !mfma_serves(D, pl.G, sb_dtype)) pl.G /= 2;
   pl.n_sub = gqa / pl.G;
-  const int64_t groups = static_cast<int64_t>(batch) * Hkv * pl.n_sub;
+  const int64_t groups = static_cast<int64_t>(batch) * Hkv * pl.n_sub, cus = target_wgs();
   const int len = static_cast<int>(std::min<int64_t>((static_cast<int64_t>(max_len) + 31) / 32 * 32, 0x7FFFFFE0));
   const int min_splits = min_splits_for(batch);
   pl.chunk = (plan_chunk(len, groups, min_splits) + 31) / 32 * 32;
-  pl.max_splits = max_splits_bound(len, groups, min_splits);
-  // the device chooses the chunk (see plan_sdpa)
-  pl.lpt = batch <= 64 && !pl.hc;
-  if (pl.lpt && groups >= 2 * static_cast<int64_t>(target_wgs()) && pl.max_splits > 2) {
-    pl.max_splits = 2;
-    pl.chunk = std::max(pl.chunk, ((len + 1) / 2 + 127) / 128 * 128);
+  pl.grid_x = pl.max_splits = max_splits_bound(len, groups, min_splits);
+  // Four waves a workgroup, two workgroups a CU: one streams under the other's
+  // prologue and merge.  64 sequences of 256 .. 1,024 keys (Hq 32 Hkv 16 D 256) 38
+  // against 52 us, 32 with a window of 1,024 33 against 42; eight waves once every CU
+  // has 24,576 keys to stream: 64 of 4,096 .. 16,384 keys (Hq 16 Hkv 8 D 128) 136
+  // against 150 us, 16 such sequences of D 256 140 both.
+  pl.waves = D != 512 && !(len >= 12288 && groups * len >= cus * 24576) ? 4 : 8;
+  pl.slots = static_cast<int>(pl.waves == 4 ? 2 * cus : cus);
+  // Batches of up to 64 sequences, where there is something to choose or to order.
+  // The longest sequences may then be split twice as far as equal ones would be;
+  // the grid holds a job per sequence and one per slot beside (workgroups without
+  // a job cost 2 to 3 us of a slot each round).
+  pl.lpt = batch > 1 && batch <= 64 && (pl.max_splits > 1 || groups > pl.slots);
+  if (pl.lpt) {
+    pl.max_splits = lpt_splits(pl.max_splits, len, groups, pl.slots);
+    pl.grid_x = static_cast<int>(std::min<int64_t>(pl.max_splits, 1 + (pl.slots + groups - 1) / groups));
   }
+  // every sequence's keys fit its splits
+  const int64_t least = (static_cast<int64_t>(len) + pl.max_splits - 1) / pl.max_splits;
+  pl.chunk = static_cast<int>(std::max<int64_t>(pl.chunk, (least + 31) / 32 * 32));
   return pl;
+}
+
+// Splits of any plan of these sizes, whatever its window.
+int max_paged_splits(int batch, int Hq, int Hkv, int D, int max_len) {
+  const PagedPlan pl = plan_paged(batch, Hq, Hkv, D, TQ_F16, max_len);
+  const int64_t groups = static_cast<int64_t>(batch) * Hkv * pl.n_sub;
+  const int s = max_splits_bound(max_len, groups, min_splits_for(batch));
+  return std::max({pl.max_splits, s, lpt_splits(s, max_len, groups, 2 * target_wgs())});
 }
 
 // Keys a sequence attends at most, in whole blocks.
@@ -92,10 +125,14 @@ int attended_bound(int max_kv_len, int window, bool windows, int sinks) {
   return static_cast<int>(std::min<int64_t>(most, max_kv_len));
 }
 
-// The split partials of a call in its workspace.
+// The split partials of a call in its workspace, and behind them the chunk that a
+// launch chose.
+constexpr size_t kWsTail = 256;
+
 int set_workspace(PagedParams& p, void* workspace, size_t bytes, const WsLayout& wl, const char* fn) {
-  if (!workspace || bytes < wl.total) {
-    set_error("%s: workspace of %zu bytes needed (got %zu)", fn, wl.total, workspace ? bytes : size_t{0});
+  const size_t need = wl.total + kWsTail;
+  if (!workspace || bytes < need) {
+    set_error("%s: workspace of %zu bytes needed (got %zu)", fn, need, workspace ? bytes : size_t{0});
     return TQ_ERR_WORKSPACE;
   }
   TQ_CHECK_ARG(reinterpret_cast<uintptr_t>(workspace) % 16 == 0, "%s: workspace must be 16-byte aligned", fn);
@@ -105,6 +142,7 @@ int set_workspace(PagedParams& p, void* workspace, size_t bytes, const WsLayout&
   p.ws_cnt = reinterpret_cast<int*>(ws + wl.cnt_off);
   p.ws_ml = reinterpret_cast<float*>(ws + wl.ml_off);
   p.ws_o = reinterpret_cast<float*>(ws + wl.o_off);
+  p.lpt_chunk = reinterpret_cast<int*>(ws + wl.total);
   return TQ_OK;
 }
 
@@ -123,12 +161,12 @@ extern "C" size_t tq_sdpa_int4_paged_workspace_size(int batch, int num_heads, in
                                                     int max_kv_len, int shared_prefix) {
   if (batch < 1 || num_kv_heads < 1 || num_heads < num_kv_heads || max_kv_len < 0 || shared_prefix < 0) return 0;
   // (every plan of a call with these sizes: a window only shortens the splits)
+  if (num_heads % num_kv_heads != 0) return 0;
   const int gqa = num_heads / num_kv_heads;
-  const int64_t groups = static_cast<int64_t>(batch) * num_kv_heads * (gqa / head_subgroup(gqa));
-  int splits = max_splits_bound(max_kv_len, groups, min_splits_for(batch));
+  int splits = max_paged_splits(batch, num_heads, num_kv_heads, head_dim, max_kv_len);
   if (shared_prefix > 0)
     splits += paged_tiles_splits(static_cast<int64_t>(batch) * gqa, num_kv_heads, head_dim, shared_prefix);
-  return ws_layout(batch, num_heads, head_dim, splits).total;
+  return ws_layout(batch, num_heads, head_dim, splits).total + kWsTail;
 }
 
 extern "C" int tq_sdpa_int4_paged(const void* q, tq_dtype q_dtype, const uint32_t* k_quant, const void* k_scales,
@@ -168,14 +206,16 @@ extern "C" int tq_sdpa_int4_paged(const void* q, tq_dtype q_dtype, const uint32_
   p.n_sub = pl.n_sub;
   p.chunk = pl.chunk;
   p.lpt = pl.lpt ? 1 : 0;
+  p.lpt_jobs = pl.grid_x * batch;
+  p.waves = pl.waves;
+  p.cus = pl.slots;
   if (shared_prefix > 0)
     p.pre = paged_tiles_splits(static_cast<int64_t>(batch) * gqa_factor, num_kv_heads, head_dim, shared_prefix);
-  const int own = pl.max_splits;
-  p.max_splits = own + p.pre;
+  p.max_splits = pl.max_splits + p.pre;
   if (p.max_splits > 1) {
     if (int r = set_workspace(p, workspace, workspace_bytes, ws_layout(batch, num_heads, head_dim, p.max_splits), fn)) return r;
   }
-  const dim3 grid(own, num_kv_heads * pl.n_sub, batch);
+  const dim3 grid(pl.grid_x, num_kv_heads * pl.n_sub, batch);
   p.cnt_stride = counter_stride(static_cast<int64_t>(batch) * num_heads);
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (p.pre > 0)
@@ -186,13 +226,39 @@ extern "C" int tq_sdpa_int4_paged(const void* q, tq_dtype q_dtype, const uint32_
   return r != TQ_OK || !p.ext_merge ? r : launch_merge_splits(p, head_dim, batch, s);
 }
 
+extern "C" int tq_sdpa_int4_paged_plan(int batch, int num_heads, int num_kv_heads, int head_dim, int max_kv_len,
+                                       int sliding_window, int num_sinks, int shared_prefix, int* splits,
+                                       int* chunk_keys, int* shared_splits, int* on_device, char* kernel,
+                                       size_t kernel_bytes) {
+  clear_error();
+  const char* fn = "tq_sdpa_int4_paged_plan";
+  TQ_CHECK_ARG(head_dim == 128 || head_dim == 256 || head_dim == 512, "%s: bad head_dim %d", fn, head_dim);
+  TQ_CHECK_ARG(batch >= 1 && num_kv_heads >= 1 && num_heads >= num_kv_heads && num_heads % num_kv_heads == 0 &&
+                   max_kv_len >= 0 && sliding_window >= 0 && num_sinks >= 0 && shared_prefix >= 0 &&
+                   shared_prefix <= max_kv_len,
+               "%s: bad shape", fn);
+  const PagedPlan pl = plan_paged(batch, num_heads, num_kv_heads, head_dim, TQ_F16,
+                                  std::min(attended_bound(max_kv_len, sliding_window, false, num_sinks),
+                                           max_kv_len - shared_prefix));
+  if (splits) *splits = pl.max_splits;
+  if (chunk_keys) *chunk_keys = pl.chunk;
+  if (shared_splits)
+    *shared_splits = shared_prefix > 0 ? paged_tiles_splits(static_cast<int64_t>(batch) * (num_heads / num_kv_heads),
+                                                            num_kv_heads, head_dim, shared_prefix)
+                                       : 0;
+  if (on_device) *on_device = pl.lpt ? 1 : 0;
+  if (kernel && kernel_bytes > 0)
+    std::snprintf(kernel, kernel_bytes, "%s", pl.hc ? "sdpa_int4_hc2_kernel" : "sdpa_int4_mfma_kernel");
+  return TQ_OK;
+}
+
 extern "C" size_t tq_sdpa_int4_paged_prefill_workspace_size(int num_heads, int num_kv_heads, int head_dim,
                                                             int n_prior, int n_new) {
   if (num_kv_heads < 1 || num_heads < num_kv_heads || n_prior < 0 || n_new < 1) return 0;
   // (a window only shortens the splits)
   const int splits = paged_tiles_max_splits(static_cast<int64_t>(n_new) * (num_heads / num_kv_heads), num_kv_heads,
                                             head_dim, prompt_keys(n_prior, n_new, 0, 0));
-  return splits > 1 ? ws_layout(n_new, num_heads, head_dim, splits).total : 0;
+  return splits > 1 ? ws_layout(n_new, num_heads, head_dim, splits).total + kWsTail : 0;
 }
 
 extern "C" int tq_sdpa_int4_paged_prefill(const void* q, tq_dtype q_dtype, const uint32_t* k_quant,

@@ -89,6 +89,9 @@ struct PagedParams : SdpaParams {
   // Partials of every row that lie before a launch's own splits (those of the
   // shared rows), joined with them.
   int pre;
+  int waves;      // of a workgroup of sdpa_int4_mfma_kernel, D 128 / 256: 8 or 4
+  int lpt_jobs;   // (sequence, split) jobs that the launch's grid holds (paged_chunk)
+  int* lpt_chunk; // where the chunk goes for the merge launch (ext_merge)
 };
 template <bool PG>
 using ParamsOf = typename std::conditional<PG, PagedParams, SdpaParams>::type;
@@ -204,8 +207,7 @@ __device__ __forceinline__ int wave_max_i(int v) {
   return v;
 }
 
-template <bool PG = false>
-__device__ __forceinline__ bool ragged_job(const ParamsOf<PG>& p, int& b, int& hy, int& split, int& chunk) {
+__device__ __forceinline__ bool ragged_job(const SdpaParams& p, int& b, int& hy, int& split, int& chunk) {
   const int lane = threadIdx.x & 63;
   const int H = static_cast<int>(gridDim.y);
   const int64_t wg = blockIdx.x + static_cast<int64_t>(gridDim.x) * (blockIdx.y + static_cast<int64_t>(gridDim.y) * blockIdx.z);
@@ -213,17 +215,14 @@ __device__ __forceinline__ bool ragged_job(const ParamsOf<PG>& p, int& b, int& h
   const int n_b = mine ? min(p.seq_lens[lane], p.n_clamp) : 0;
   const int W = mine ? (p.windows ? p.windows[lane] : p.window) : 0;
   const int lo = W > 0 ? max(0, n_b - W) : 0;
-  int len = max(n_b - lo, 0);
-  if constexpr (PG) len = 32 * paged_keys(p, n_b, W, p.shared).nb;
+  const int len = max(n_b - lo, 0);
   // ---- chunk: candidates k = 1 .. max_splits, one wave-wide job count each
   const int lmax = wave_max_i(len);
   const float keys = static_cast<float>(wave_sum_dpp(len)) * H;
   const float cus = static_cast<float>(max(p.cus, 1));
   float best = INFINITY;
   chunk = p.chunk;
-  int most = p.max_splits;
-  if constexpr (PG) most -= p.pre;
-  for (int k = 1; k <= most; ++k) {  // uniform loop
+  for (int k = 1; k <= p.max_splits; ++k) {  // uniform loop
     const int cand = max(128, ((lmax + k - 1) / k + 127) / 128 * 128);
     const int jobs = wave_sum_dpp(mine ? (len > 0 ? (len + cand - 1) / cand : 1) : 0);
     const float est = fmaxf(static_cast<float>(kLptFixedKeys + cand),
@@ -264,6 +263,125 @@ __device__ __forceinline__ bool ragged_job(const ParamsOf<PG>& p, int& b, int& h
   const uint64_t m = __ballot(part && rank == static_cast<int>(r - F));
   b = __builtin_ffsll(static_cast<long long>(m)) - 1;
   split = __builtin_amdgcn_readlane(full, b);
+  return true;
+}
+
+// ragged_job for paged sequences (keys of their lists as lengths), in a few hundred
+// cycles: the loop over candidates above, with two divisions each, and the rank by
+// 64 comparisons were 3 to 6 us of a short launch.
+
+// This lane's sequence (lane < p.nq): its length, window, and keys of its list.
+struct PagedLane {
+  int n, W, len;
+};
+
+__device__ __forceinline__ PagedLane paged_lane(const PagedParams& p) {
+  const int lane = threadIdx.x & 63;
+  PagedLane r{0, 0, 0};
+  if (lane < p.nq) {
+    r.n = p.seq_lens[lane];
+    r.W = p.windows ? p.windows[lane] : p.window;
+    r.len = 32 * paged_keys(p, r.n, r.W, p.shared).nb;
+  }
+  return r;
+}
+
+// The chunk of least estimated makespan, as in ragged_job, among those whose jobs
+// the grid holds (p.lpt_jobs; one chunk a sequence always fits); p.cus = workgroups
+// that the chip runs at once.
+__device__ __forceinline__ int paged_chunk(const PagedParams& p, int len, int H) {
+  const int lane = threadIdx.x & 63;
+  const int lmax = wave_max_i(len);
+  const float fixed = static_cast<float>(kLptFixedKeys), slots = static_cast<float>(p.cus);
+  const float room = static_cast<float>(p.lpt_jobs);
+  const float keys = static_cast<float>(wave_sum_dpp(len)) * H;
+  const int most = min(p.max_splits - p.pre, max((lmax + 127) >> 7, 1));
+  const auto cand_of = [&](int k) {
+    // (within a granule of ceil(lmax / k), never below it)
+    const int c = static_cast<int>(static_cast<float>(lmax) * __builtin_amdgcn_rcpf(static_cast<float>(k)) * 1.000001f) + 1;
+    return k == 1 ? max(128, (lmax + 127) & ~127) : max(128, (c + 127) & ~127);
+  };
+  // ceil(l / cand), at least 1: by the reciprocal, then made exact
+  const auto splits_of = [&](int l, int cand, float r) {
+    int j = static_cast<int>(static_cast<float>(l) * r);
+    j += static_cast<uint32_t>(j) * static_cast<uint32_t>(cand) < static_cast<uint32_t>(l);
+    j += static_cast<uint32_t>(j) * static_cast<uint32_t>(cand) < static_cast<uint32_t>(l);
+    return max(j, 1);
+  };
+  const auto cost = [&](float jobs, int cand) {
+    return jobs > room ? INFINITY : fmaxf(fixed + static_cast<float>(cand), (fixed * jobs * H + keys) / slots);
+  };
+  float best = INFINITY;
+  int chunk = cand_of(1);
+  if (most * 4 <= p.nq) {  // a lane a sequence
+    for (int k = 1; k <= most; ++k) {
+      const int cand = cand_of(k);
+      const int j = lane < p.nq ? splits_of(len, cand, __builtin_amdgcn_rcpf(static_cast<float>(cand))) : 0;
+      const float c = cost(static_cast<float>(wave_sum_dpp(j)), cand);
+      if (c < best) {
+        best = c;
+        chunk = cand;
+      }
+    }
+  } else {                 // a lane a candidate
+    for (int k0 = 0; k0 < most; k0 += 64) {
+      const int cand = cand_of(min(k0 + lane + 1, most));
+      const float r = __builtin_amdgcn_rcpf(static_cast<float>(cand));
+      int jobs = 0;
+      for (int b = 0; b < p.nq; ++b) jobs += splits_of(__builtin_amdgcn_readlane(len, b), cand, r);
+      const float c = cost(static_cast<float>(jobs), cand);
+      const float least = -wave_max_dpp(-c);
+      if (least < best) {  // uniform; ties keep the fewest splits
+        best = least;
+        chunk = __builtin_amdgcn_readlane(cand, __builtin_ffsll(static_cast<long long>(__ballot(c == least))) - 1);
+      }
+    }
+  }
+  return __builtin_amdgcn_readfirstlane(chunk);
+}
+
+// Job of this workgroup; `me`: its sequence's length, window and list.  The
+// partial chunk of rank r is found by bisection over their sizes.
+__device__ __forceinline__ bool paged_job(const PagedParams& p, int& b, int& hy, int& split, int& chunk, PagedLane& me) {
+  const int lane = threadIdx.x & 63;
+  const int H = static_cast<int>(gridDim.y);
+  const uint32_t wg = blockIdx.x + gridDim.x * (blockIdx.y + gridDim.y * blockIdx.z);
+  const bool mine = lane < p.nq;
+  const PagedLane l = paged_lane(p);
+  chunk = p.max_splits - p.pre == 1 ? p.chunk : paged_chunk(p, l.len, H);
+  const int full = l.len / chunk;
+  const int rem = l.len - full * chunk;
+  const bool part = mine && (rem > 0 || l.len == 0);  // one partial (or empty) chunk
+  const int F = wave_sum_dpp(full);                   // full chunks in all
+  int r = static_cast<int>(wg / H);
+  hy = static_cast<int>(wg - static_cast<uint32_t>(r) * H);
+  if (r >= F + static_cast<int>(__builtin_popcountll(__ballot(part)))) return false;  // no job
+  if (r < F) {
+    int pre = full;  // inclusive prefix over the lanes
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int v = __shfl_up(pre, d, 64);
+      if (lane >= d) pre += v;
+    }
+    b = __builtin_ffsll(static_cast<long long>(__ballot(pre > r))) - 1;
+    split = r - (__builtin_amdgcn_readlane(pre, b) - __builtin_amdgcn_readlane(full, b));
+  } else {
+    // longest first, then by sequence; sizes are whole blocks of 32
+    r -= F;
+    const int key = part ? rem >> 5 : -1;
+    int lo = 0, hi = (chunk >> 5) + 1;  // more than r keys >= lo, at most r >= hi
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (static_cast<int>(__builtin_popcountll(__ballot(key >= mid))) > r) lo = mid;
+      else hi = mid;
+    }
+    r -= static_cast<int>(__builtin_popcountll(__ballot(key > lo)));
+    uint64_t m = __ballot(key == lo);
+    for (; r > 0; --r) m &= m - 1;  // the r-th of the equal ones
+    b = __builtin_ffsll(static_cast<long long>(m)) - 1;
+    split = __builtin_amdgcn_readlane(full, b);
+  }
+  me = PagedLane{__builtin_amdgcn_readlane(l.n, b), __builtin_amdgcn_readlane(l.W, b), __builtin_amdgcn_readlane(l.len, b)};
   return true;
 }
 

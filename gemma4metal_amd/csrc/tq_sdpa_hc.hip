@@ -607,12 +607,28 @@ void sdpa_int4_hc2_kernel(ParamsOf<PG> p) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int m = lane & 15, c = lane >> 4;
   const int hh = m & 7;  // this lane's head (column m)
-  const int b = blockIdx.z, hy = blockIdx.y, split = blockIdx.x;
+  int b = blockIdx.z, hy = blockIdx.y, split = blockIdx.x;
+  PagedLane me{};
+  if constexpr (PG) {
+    if (p.lpt) {
+      int chunk;
+      if (!__builtin_amdgcn_readfirstlane(paged_job(p, b, hy, split, chunk, me))) return;
+      b = __builtin_amdgcn_readfirstlane(b);
+      hy = __builtin_amdgcn_readfirstlane(hy);
+      split = __builtin_amdgcn_readfirstlane(split);
+      p.chunk = __builtin_amdgcn_readfirstlane(chunk);
+      // every workgroup's is the same
+      if (p.ext_merge && threadIdx.x == 0) *p.lpt_chunk = p.chunk;
+    }
+  }
   const int kvh = hy / p.n_sub, sub = hy - kvh * p.n_sub;
   const int h0 = kvh * p.gqa + sub * G;
 
   PagedKeys pk{};
-  if constexpr (PG) pk = paged_keys(p, p.seq_lens[b], p.windows ? p.windows[b] : p.window, p.shared);
+  if constexpr (PG) {
+    if (!p.lpt) me = PagedLane{p.seq_lens[b], p.windows ? p.windows[b] : p.window, 0};
+    pk = paged_keys(p, me.n, me.W, p.shared);
+  }
   const SplitRange rg = PG ? paged_range(p, pk, split) : split_range(p, b, split);
   if (split >= rg.S) return;
   const int t_end = rg.t_end;
@@ -1104,6 +1120,9 @@ __global__ __launch_bounds__(256) void merge_splits_kernel(ParamsOf<PG> p, int D
   const int b = blockIdx.y;
   if (o0 >= p.Hq * D4) return;                 // whole waves (Hq * D4 % 4 == 0)
   int S;
+  if constexpr (PG) {
+    if (p.lpt) p.chunk = *p.lpt_chunk;
+  }
   if constexpr (PG) S = paged_range(p, paged_keys(p, p.seq_lens[b], p.windows ? p.windows[b] : p.window, p.shared), 0).S + p.pre;
   else S = split_range(p, b, 0).S;
   if (S == 1) return;                          // written by the attention kernel

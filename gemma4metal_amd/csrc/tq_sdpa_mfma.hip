@@ -220,12 +220,15 @@ void sdpa_int4_mfma_kernel(ParamsOf<PG> p) {
   const int hn = n / NG, gn = n - (n / NG) * NG;
   const bool col_used = n < COLS;
   int b = blockIdx.z, hy = blockIdx.y, split = blockIdx.x;
+  PagedLane me{};
   // Longest-first ragged order: batched launches only (single-sequence and
   // grouped-prefill launches never set lpt).
   if constexpr (!kQG && !kStreamNT) {
     if (p.lpt) {
       int chunk = p.chunk;
-      const bool job = ragged_job<PG>(p, b, hy, split, chunk);
+      bool job;
+      if constexpr (PG) job = paged_job(p, b, hy, split, chunk, me);
+      else job = ragged_job(p, b, hy, split, chunk);
       // Every lane computes the same job; read back as wave-uniform values
       // so that the split range, the key offsets and the load addresses
       // derived from them stay in scalar registers.
@@ -246,7 +249,10 @@ void sdpa_int4_mfma_kernel(ParamsOf<PG> p) {
   const int b_last = kQG ? min(b0 + pq - 1, p.nq - 1) : b;
 
   PagedKeys pk{};
-  if constexpr (PG) pk = paged_keys(p, p.seq_lens[b], p.windows ? p.windows[b] : p.window, p.shared);
+  if constexpr (PG) {
+    if (!p.lpt) me = PagedLane{p.seq_lens[b], p.windows ? p.windows[b] : p.window, 0};
+    pk = paged_keys(p, me.n, me.W, p.shared);
+  }
   const SplitRange rg = PG    ? paged_range(p, pk, split)
                         : kQG ? prefill_range(p, b0, b_last, split)
                               : split_range(p, b, split);
@@ -912,8 +918,10 @@ void sdpa_int4_mfma_kernel(ParamsOf<PG> p) {
 
 template <int D, int G, bool F32>
 int launch_dgs(const PagedParams& p, dim3 grid, hipStream_t s) {
-  constexpr int NW = D == 512 ? 4 : kMfmaWaves;
-  sdpa_int4_mfma_kernel<D, G, NW, false, false, F32, true><<<grid, NW * 64, 0, s>>>(p);
+  if (D == 512 || p.waves == 4)
+    sdpa_int4_mfma_kernel<D, G, 4, false, false, F32, true><<<grid, 4 * 64, 0, s>>>(p);
+  else
+    sdpa_int4_mfma_kernel<D, G, kMfmaWaves, false, false, F32, true><<<grid, kMfmaWaves * 64, 0, s>>>(p);
   TQ_CHECK_LAUNCH("sdpa_int4_mfma_kernel");
   return TQ_OK;
 }

@@ -70,6 +70,36 @@ def test_nothing_to_do_is_no_error():
     assert prompt(new=0, q=NULL)[0] == 0
 
 
+def plan(B, Hq, Hkv, D, n, W=0, sinks=0, P=0):
+    lib = _lib.load()
+    out = [ctypes.c_int(-1) for _ in range(4)]
+    name = ctypes.create_string_buffer(64)
+    assert lib.tq_sdpa_int4_paged_plan(B, Hq, Hkv, D, n, W, sinks, P, *map(ctypes.byref, out), name, 64) == 0
+    return [x.value for x in out] + [name.value.decode()]
+
+
+@pytest.mark.parametrize("Hq,Hkv,D", [(8, 4, 128), (2, 1, 128), (32, 16, 256), (8, 1, 256), (32, 4, 512), (4, 2, 512)])
+def test_every_plan_has_room(Hq, Hkv, D):
+    """A split for every key that a sequence may attend, and a workspace that
+    holds the splits of any window."""
+    lib = _lib.load()
+    for B in (1, 2, 7, 16, 64, 65, 300):
+        for n in (0, 1, 33, 127, 128, 129, 192, 500, 1000, 4097, 20000, 131072, 1 << 20):
+            for P in (0, 64, 4096):
+                if P > n:
+                    continue
+                room = lib.tq_sdpa_int4_paged_workspace_size(B, Hq, Hkv, D, n, P)
+                for W, sinks in ((0, 0), (1, 0), (64, 33), (100, 64), (1000, 4), (4000, 3000)):
+                    splits, chunk, pre, device, _ = plan(B, Hq, Hkv, D, n, W, sinks, P)
+                    most = n if W == 0 else min(n, W + 62 + -(-sinks // 32) * 32)
+                    keys = -(-min(most, n - P) // 32) * 32
+                    assert splits >= 1 and chunk >= 1 and chunk % 32 == 0
+                    assert splits * chunk >= keys, (B, n, W, sinks, P)
+                    assert (pre > 0) == (P > 0)
+                    need = (1 << 18) + B * Hq * (splits + pre) * (D + 2) * 4
+                    assert room >= need, (B, n, W, sinks, P, room, need)
+
+
 def append(**over):
     a = dict(k=FAKE, v=FAKE, xd=_lib.TQ_F32, kq=FAKE, ks=FAKE, kb=FAKE, vq=FAKE, vs=FAKE, vb=FAKE, sb=_lib.TQ_F16, B=2,
              Hkv=16, D=256, page=64, N=10, tab=FAKE, P=4, pos=FAKE, T=1, mode=0)
