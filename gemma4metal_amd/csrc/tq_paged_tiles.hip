@@ -30,7 +30,19 @@ struct PgTile {
   bool has[KH];      // whether that part's page exists
 };
 
-__device__ __forceinline__ int wave_min_i(int v) { return -wave_max_i(-v); }
+// Largest of 64 lanes, by the steps of wave_max_dpp (wave_max_i goes through the
+// LDS: six of them were 1.5 us of a launch's start).
+__device__ __forceinline__ int max_of_wave(int v) {
+  v = max(v, __builtin_amdgcn_update_dpp(0, v, 0xB1, 0xF, 0xF, false));
+  v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x4E, 0xF, 0xF, false));
+  v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x141, 0xF, 0xF, false));
+  v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x140, 0xF, 0xF, false));
+  const auto a = __builtin_amdgcn_permlane16_swap(static_cast<unsigned>(v), static_cast<unsigned>(v), false, false);
+  v = max(static_cast<int>(a[0]), static_cast<int>(a[1]));
+  const auto b = __builtin_amdgcn_permlane32_swap(static_cast<unsigned>(v), static_cast<unsigned>(v), false, false);
+  return __builtin_amdgcn_readfirstlane(max(static_cast<int>(b[0]), static_cast<int>(b[1])));
+}
+__device__ __forceinline__ int min_of_wave(int v) { return -max_of_wave(-v); }
 
 // Raw loads behind a uniform address: a 32-bit lane offset beside the scalar base,
 // where global loads of this kernel took 64-bit addresses in vector registers.
@@ -258,8 +270,8 @@ void paged_tiles_kernel(TileParams p) {
   {
     int h, l;
     limits(min(r0 + lane, total - 1), h, l);  // lane: row (kRows of them)
-    hi_w = __builtin_amdgcn_readfirstlane(wave_max_i(h));
-    lo_w = __builtin_amdgcn_readfirstlane(wave_min_i(l));
+    hi_w = max_of_wave(h);
+    lo_w = min_of_wave(l);
   }
   const int end = (hi_w + TK - 1) / TK;
   const int ns = min(p.sinks / TK + (p.sinks % TK != 0), end);  // tiles that hold sinks
@@ -300,8 +312,8 @@ void paged_tiles_kernel(TileParams p) {
   int hi, lo;
   limits(R, hi, lo);
   // over the wave's rows
-  const int hi_max = __builtin_amdgcn_readfirstlane(wave_max_i(hi)), hi_min = __builtin_amdgcn_readfirstlane(wave_min_i(hi));
-  const int lo_max = __builtin_amdgcn_readfirstlane(wave_max_i(lo)), lo_min = __builtin_amdgcn_readfirstlane(wave_min_i(lo));
+  const int hi_max = max_of_wave(hi), hi_min = min_of_wave(hi);
+  const int lo_max = max_of_wave(lo), lo_min = min_of_wave(lo);
 
   PgTile<KH> cur = tile_at(it0), nxt = cur;
   const PgSource<Gm> from = pg_source<Gm>(p);

@@ -25,7 +25,7 @@ import torch
 
 from . import _lib
 from ._lib import call
-from .turboquant import _DT, _MODES, _QUANT_DT, _check_cuda, _ptr, _sb_dtype, _stream
+from .turboquant import _DT, _MODES, _QUANT_DT, _check_cuda, _ptr, _sb_dtype, _size_caches, _stream
 from .turboquant import workspace as _cached_workspace
 
 # Buffers that a captured graph points to: kept for good, since the cached one
@@ -90,6 +90,31 @@ def _check_pages(pages, D: int, device, lead: int = 0):
     return shape[lead], shape[lead + 1], shape[lead + 2], sbt
 
 
+def _pages_fine(pages, D: int, di: int) -> bool:
+    """What _check_pages checks of pages without leading axes, as one expression:
+    a decode call's host time is part of a short layer's."""
+    kq, ks, kb, vq, vs, vb = pages
+    try:
+        shape, dt = kq.shape, ks.dtype
+        rows = shape[:3] + (D // 64,)
+        return (len(shape) == 4 and shape[3] == D // 8 and D % 64 == 0 and vq.shape == shape
+                and ks.shape == rows and kb.shape == rows and vs.shape == rows and vb.shape == rows
+                and dt is kb.dtype and dt is vs.dtype and dt is vb.dtype
+                and (dt is torch.float16 or dt is torch.float32)
+                and kq.dtype in _QUANT_DT and vq.dtype in _QUANT_DT
+                and kq.get_device() == di and ks.get_device() == di and kb.get_device() == di
+                and vq.get_device() == di and vs.get_device() == di and vb.get_device() == di
+                and kq.is_contiguous() and ks.is_contiguous() and kb.is_contiguous()
+                and vq.is_contiguous() and vs.is_contiguous() and vb.is_contiguous())
+    except (AttributeError, IndexError):
+        return False
+
+
+def _ints_fine(t, shape, di: int) -> bool:
+    return (isinstance(t, torch.Tensor) and t.dtype is torch.int32 and t.shape == shape and t.get_device() == di
+            and t.is_contiguous())
+
+
 def _check_ints(name: str, t: torch.Tensor, shape, device):
     _check_cuda(name, t)
     if t.dtype != torch.int32 or tuple(t.shape) != tuple(shape) or t.device != device:
@@ -134,8 +159,16 @@ def kv_append_int4_paged(k_new: torch.Tensor, v_new: torch.Tensor,
 
 
 @functools.lru_cache(maxsize=256)
+def _prefill_ws_size(*shape) -> int:
+    return _lib.load().tq_sdpa_int4_paged_prefill_workspace_size(*shape)
+
+
+@functools.lru_cache(maxsize=256)
 def _paged_ws_size(*shape) -> int:
     return _lib.load().tq_sdpa_int4_paged_workspace_size(*shape)
+
+
+_size_caches += [_paged_ws_size, _prefill_ws_size]
 
 
 @_placed
@@ -160,16 +193,25 @@ def sdpa_int4_paged(queries: torch.Tensor,
     _need(queries.dim() == 3 and queries.dtype in _DT, "queries must be (B, Hq, D) float32, float16 or bfloat16")
     B, Hq, D = queries.shape
     dev = queries.device
+    di = dev.index
     pages = (k_quant, k_scales, k_biases, v_quant, v_scales, v_biases)
-    N, Hkv, page, sbt = _check_pages(pages, D, dev)
+    if not _pages_fine(pages, D, di):
+        _check_pages(pages, D, dev)
+    N, Hkv, page, _ = k_quant.shape
+    sbt = _DT[k_scales.dtype]
     _need(block_tables.dim() == 2, "block_tables must be (B, max_pages)")
     P = block_tables.shape[1]
-    _check_ints("block_tables", block_tables, (B, P), dev)
-    _check_ints("seq_lens", seq_lens, (B,), dev)
+    if not _ints_fine(block_tables, (B, P), di):
+        _check_ints("block_tables", block_tables, (B, P), dev)
+    if not _ints_fine(seq_lens, (B,), di):
+        _check_ints("seq_lens", seq_lens, (B,), dev)
     if windows is not None:
         _check_ints("windows", windows, (B,), dev)
     mx = P * page if max_kv_len is None else int(max_kv_len)
-    out = _out(out, (B, Hq, D), dev)
+    if out is None:
+        out = torch.empty((B, Hq, D), dtype=torch.float32, device=dev)
+    else:
+        out = _out(out, (B, Hq, D), dev)
     sh = _stream(None)
     ws = _workspace(workspace, _paged_ws_size(B, Hq, Hkv, D, mx, int(shared_prefix)), dev, sh)
     call("tq_sdpa_int4_paged", queries.data_ptr(), _DT[queries.dtype], *[t.data_ptr() for t in pages], sbt,
@@ -196,13 +238,15 @@ def sdpa_int4_paged_prefill(queries: torch.Tensor,
     S, Hq, D = queries.shape
     dev = queries.device
     pages = (k_quant, k_scales, k_biases, v_quant, v_scales, v_biases)
-    N, Hkv, page, sbt = _check_pages(pages, D, dev)
+    if not _pages_fine(pages, D, dev.index):
+        _check_pages(pages, D, dev)
+    N, Hkv, page, _ = k_quant.shape
+    sbt = _DT[k_scales.dtype]
     _need(block_table.dim() == 1, "block_table must be (max_pages,)")
     _check_ints("block_table", block_table, block_table.shape, dev)
     out = _out(out, (S, Hq, D), dev)
     sh = _stream(None)
-    nbytes = _lib.load().tq_sdpa_int4_paged_prefill_workspace_size(Hq, Hkv, D, int(n_prior), S)
-    ws = _workspace(workspace, nbytes, dev, sh)
+    ws = _workspace(workspace, _prefill_ws_size(Hq, Hkv, D, int(n_prior), S), dev, sh)
     call("tq_sdpa_int4_paged_prefill", queries.data_ptr(), _DT[queries.dtype], *[t.data_ptr() for t in pages], sbt,
          out.data_ptr(), Hq, Hkv, D, page, N, block_table.data_ptr(), block_table.shape[0], int(n_prior), S,
          int(gqa_factor), float(scale), int(sliding_window), int(num_sinks), ws.data_ptr(), ws.numel(), sh)
@@ -240,8 +284,13 @@ def _six(pages, refs, device):
     return arr, sbt, (kq.shape[0] if lead else 1), Hkv, kq.shape[-1] * 8, N, page
 
 
+@functools.lru_cache(maxsize=64)
+def _pages_ws_size(S: int, N: int) -> int:
+    return _lib.load().tq_kv_pages_workspace_size(S, N)
+
+
 def _pages_ws(ws, S, N, device):
-    nbytes = _lib.load().tq_kv_pages_workspace_size(S, N)
+    nbytes = _pages_ws_size(S, N)
     if ws is None:
         # a buffer of the call's own: plans overwrite what attention keeps zeroed
         return torch.empty(nbytes, dtype=torch.uint8, device=device)

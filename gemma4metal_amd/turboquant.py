@@ -174,7 +174,8 @@ def reload_options() -> None:
     """Re-read the TQ_* kernel-choice switches from the environment (they
     are read once per process otherwise)."""
     call("tq_reload_options")
-    _decode_ws_size.cache_clear()
+    for cache in _size_caches:
+        cache.cache_clear()
 
 
 @functools.lru_cache(maxsize=256)
@@ -182,6 +183,10 @@ def _decode_ws_size(Hq: int, Hkv: int, D: int, n: int) -> int:
     """Workspace bytes of one single-sequence decode call (a pure function
     of the shape, cached: the C query costs a call per layer otherwise)."""
     return _lib.load().tq_sdpa_int4_workspace_size(1, Hq, Hkv, D, n)
+
+
+# workspace sizes that depend on the switches
+_size_caches = [_decode_ws_size]
 
 
 def sdpa_int4_prefill(queries: torch.Tensor,
