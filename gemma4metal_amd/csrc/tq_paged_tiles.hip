@@ -157,6 +157,7 @@ struct PgStage {
   _Float16 vp[2][NP][Gm::NG][TKP];
   float vsb[F32 ? 2 : 1][2][F32 ? Gm::NG : 1][F32 ? Gm::TK + 4 : 4];  // fp32 scale, bias
   _Float16 one[TKP], zero[TKP];
+  float zero32[F32 ? Gm::TK : 1];
   v4f xch[Gm::DH == 2 ? Gm::NW : 1][2][64];    // score parts of a row set's waves
 };
 
@@ -411,6 +412,7 @@ void paged_tiles_kernel(TileParams p) {
     L.st.one[threadIdx.x] = static_cast<_Float16>(1.0f);
     L.st.zero[threadIdx.x] = static_cast<_Float16>(0.0f);
   }
+  if (F32 && threadIdx.x < Gm::TK) L.st.zero32[threadIdx.x] = 0.0f;
   __syncthreads();
   pg_mask<Gm>(raw, cur, hi_w);
   const float wm = pf_vmax<Gm>(raw);
@@ -470,13 +472,10 @@ void paged_tiles_kernel(TileParams p) {
       for (int x = 0; x < 4; ++x) a[x] = vu[(4 * g + x) * 64 + (m ^ Gm::vswz(g))];
     };
     typedef typename std::conditional<F32, v4f, v4h>::type s4;
-    const auto s_read = [&](int g, s4 (&s)[2]) {
+    // (from, by bytes a group: the staged scales, or zeros)
+    const auto s_read = [&](const char* from, int step, int g, s4 (&s)[2]) {
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int at = 32 * kh + 16 * h + 4 * c;
-        if constexpr (F32) s[h] = *reinterpret_cast<const s4*>(&L.st.vsb[buf][0][NWG * dh + g][at]);
-        else s[h] = *reinterpret_cast<const s4*>(&L.st.vp[buf][1][NWG * dh + g][at]);
-      }
+      for (int h = 0; h < 2; ++h) s[h] = *reinterpret_cast<const s4*>(from + g * step + 16 * h * (F32 ? 4 : 2));
     };
 
     u32x2 b0{}, b1{};  // the bias products' operand
@@ -497,24 +496,23 @@ void paged_tiles_kernel(TileParams p) {
         __builtin_amdgcn_sched_barrier(0);
       };
       k_read(0, 0);
-      // and the scales and biases: of key m for the bias product, of this lane's
-      // scores (keys 4 c + i); of both halves, or (fp32: registers) of one
+      // and a half's scales and biases: of key m for the bias product, of this lane's
+      // scores (keys 4 c + i)
       typedef SB row_t __attribute__((ext_vector_type(NWG)));
-      constexpr int HA = F32 ? 1 : 2;
-      row_t kbr[HA], ksr[HA], sk[HA][4], bk[4];
+      row_t kbr, ksr, sk[4], bk[4];
       const auto sb_read = [&](int h) {
         if constexpr (!F32) {
-          kbr[h % HA] = *reinterpret_cast<const row_t*>(skb + (16 * h + m) * NG);
-          ksr[h % HA] = *reinterpret_cast<const row_t*>(sks + (16 * h + m) * NG);
+          kbr = *reinterpret_cast<const row_t*>(skb + (16 * h + m) * NG);
+          ksr = *reinterpret_cast<const row_t*>(sks + (16 * h + m) * NG);
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          sk[h % HA][i] = *reinterpret_cast<const row_t*>(sks + (16 * h + 4 * c + i) * NG);
+          sk[i] = *reinterpret_cast<const row_t*>(sks + (16 * h + 4 * c + i) * NG);
           if constexpr (F32) bk[i] = *reinterpret_cast<const row_t*>(skb + (16 * h + 4 * c + i) * NG);
         }
+        __builtin_amdgcn_sched_barrier(0);
       };
-#pragma unroll
-      for (int h = 0; h < HA; ++h) sb_read(h);
+      sb_read(0);
       b0 = *reinterpret_cast<const u32x2*>(brow + buf * bstep);
       b1 = *reinterpret_cast<const u32x2*>(brow + buf * bstep + 16);
 #pragma unroll
@@ -522,17 +520,6 @@ void paged_tiles_kernel(TileParams p) {
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        v4f bt = z;
-        if constexpr (!F32) {
-          v8h kb;
-#pragma unroll
-          for (int g = 0; g < 4; ++g) {
-            const _Float16 zero = static_cast<_Float16>(0.0f);
-            kb[g] = g < NWG ? kbr[h % HA][g < NWG ? g : 0] : zero;
-            kb[4 + g] = g < NWG ? ksr[h % HA][g < NWG ? g : 0] : zero;
-          }
-          bt = __builtin_amdgcn_mfma_f32_16x16x32_f16(kb, qb, z, 0, 0, 0);
-        }
         v4f acc[NWG];
 #pragma unroll
         for (int g0 = 0; g0 < NWG; g0 += GB) {
@@ -552,7 +539,17 @@ void paged_tiles_kernel(TileParams p) {
           if (g0 + GB < NWG) k_read(h, g0 + GB);
           else if (h == 0) k_read(1, 0);
         }
-        if (F32 && h == 1) sb_read(1);
+        v4f bt = z;
+        if constexpr (!F32) {
+          v8h kb;
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            const _Float16 zero = static_cast<_Float16>(0.0f);
+            kb[g] = g < NWG ? kbr[g < NWG ? g : 0] : zero;
+            kb[4 + g] = g < NWG ? ksr[g < NWG ? g : 0] : zero;
+          }
+          bt = __builtin_amdgcn_mfma_f32_16x16x32_f16(kb, qb, z, 0, 0, 0);
+        }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           float s = bt[i] * 512.0f;
@@ -561,12 +558,16 @@ void paged_tiles_kernel(TileParams p) {
             if constexpr (F32) {
               // s (. + 8 sum q) + b sum q
               s = fmaf(bk[i][g], qs[g] * 512.0f, s);
-              s = fmaf(sk[h % HA][i][g], fmaf(qs[g], 4096.0f, acc[g][i]), s);
+              s = fmaf(sk[i][g], fmaf(qs[g], 4096.0f, acc[g][i]), s);
             } else {
-              s = fmaf(static_cast<float>(sk[h % HA][i][g]), acc[g][i], s);
+              s = fmaf(static_cast<float>(sk[i][g]), acc[g][i], s);
             }
           }
           sc[4 * h + i] = s * rf;
+        }
+        if (h == 0) {
+          __builtin_amdgcn_sched_barrier(0);
+          sb_read(1);
         }
       }
     }
@@ -615,10 +616,26 @@ void paged_tiles_kernel(TileParams p) {
         for (int b = 0; b < 4 * NWG; ++b) o[b] *= fr;
         m_ref = m_new;
       }
+      // In a tile that is not plain the products below take weights and biases of 0
+      // (a branch around them would cost a second set of accumulators).
+      const bool plain = __builtin_amdgcn_readfirstlane(al) != 0;
+      const char* sfrom;
+      int sstep = 0;
+      if constexpr (F32) {
+        sfrom = reinterpret_cast<const char*>(plain ? &L.st.vsb[buf][0][NWG * dh][32 * kh] : &L.st.zero32[0]);
+        if (plain) sstep = sizeof(L.st.vsb[0][0][0]);
+        sfrom += 16 * c;
+      } else {
+        sfrom = reinterpret_cast<const char*>(plain ? &L.st.vp[buf][1][NWG * dh][32 * kh] : &L.st.zero[0]);
+        if (plain) sstep = sizeof(L.st.vp[0][0][0]);
+        sfrom += 8 * c;
+      }
       u32x4 va[4];
       s4 vs[2][2];
       v_read(0, va);
-      s_read(0, vs[0]);
+      s_read(sfrom, sstep, 0, vs[0]);
+      const uint32_t bm = plain ? ~0u : 0u;
+      const v8h ba = __builtin_bit_cast(v8h, u32x4{b0[0] & bm, b0[1] & bm, b1[0] & bm, b1[1] & bm});
       __builtin_amdgcn_sched_barrier(0);
       float pw[8];
       // (with nothing attended so far, -inf - -inf would be NaN)
@@ -642,7 +659,7 @@ void paged_tiles_kernel(TileParams p) {
         bh = __builtin_bit_cast(v8h, hw);
         bl = __builtin_bit_cast(v8h, lw);
       };
-      if (!__builtin_amdgcn_readfirstlane(al)) {
+      if (!plain) {
         // V scales apart, or scales and biases out of range or not finite: the
         // largest weight of every row and group to 2^13 .. 2^14 (an infinity, of
         // exponent 0, stays one), the products on their own, added in fp32, and
@@ -697,36 +714,36 @@ void paged_tiles_kernel(TileParams p) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) ob[i] += c == 0 ? add[i] : 0.0f;
         if (!F32 && c == 2) ob[0] += lw;
-      } else {
-        const v8h ba = __builtin_bit_cast(v8h, u32x4{b0[0], b0[1], b1[0], b1[1]});
-        {
-          v8h bh, bl;
-          float y[8];
 #pragma unroll
-          for (int j = 0; j < 8; ++j) y[j] = pw[j] * pscale;
-          split(y, bh, bl);
-          ob = __builtin_amdgcn_mfma_f32_16x16x32_f16(ba, bh, ob, 0, 0, 0);
-          ob = __builtin_amdgcn_mfma_f32_16x16x32_f16(ba, bl, ob, 0, 0, 0);
+        for (int j = 0; j < 8; ++j) pw[j] = 0.0f;
+      }
+      {
+        v8h bh, bl;
+        float y[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) y[j] = pw[j] * pscale;
+        split(y, bh, bl);
+        ob = __builtin_amdgcn_mfma_f32_16x16x32_f16(ba, bh, ob, 0, 0, 0);
+        ob = __builtin_amdgcn_mfma_f32_16x16x32_f16(ba, bl, ob, 0, 0, 0);
+      }
+#pragma unroll
+      for (int g = 0; g < NWG; ++g) {
+        if (g + 1 < NWG) s_read(sfrom, sstep, g + 1, vs[(g + 1) & 1]);
+        __builtin_amdgcn_sched_barrier(0);
+        v8h bh, bl;
+        float y[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) y[j] = fmaf(static_cast<float>(vs[g & 1][j >> 2][j & 3]), pw[j], 0.0f);
+        split(y, bh, bl);
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          const v8h a = __builtin_bit_cast(v8h, va[x]);
+          v4f& acc = o[4 * g + x];
+          acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, bh, acc, 0, 0, 0);
+          acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, bl, acc, 0, 0, 0);
         }
-#pragma unroll
-        for (int g = 0; g < NWG; ++g) {
-          if (g + 1 < NWG) s_read(g + 1, vs[(g + 1) & 1]);
-          __builtin_amdgcn_sched_barrier(0);
-          v8h bh, bl;
-          float y[8];
-#pragma unroll
-          for (int j = 0; j < 8; ++j) y[j] = fmaf(static_cast<float>(vs[g & 1][j >> 2][j & 3]), pw[j], 0.0f);
-          split(y, bh, bl);
-#pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            const v8h a = __builtin_bit_cast(v8h, va[x]);
-            v4f& acc = o[4 * g + x];
-            acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, bh, acc, 0, 0, 0);
-            acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, bl, acc, 0, 0, 0);
-          }
-          __builtin_amdgcn_sched_barrier(0);
-          if (g + 1 < NWG) v_read(g + 1, va);  // under the next group's weights
-        }
+        __builtin_amdgcn_sched_barrier(0);
+        if (g + 1 < NWG) v_read(g + 1, va);  // under the next group's weights
       }
     }
     if (it + 1 < it1) {
