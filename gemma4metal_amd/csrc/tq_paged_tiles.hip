@@ -496,23 +496,24 @@ void paged_tiles_kernel(TileParams p) {
         __builtin_amdgcn_sched_barrier(0);
       };
       k_read(0, 0);
-      // and a half's scales and biases: of key m for the bias product, of this lane's
-      // scores (keys 4 c + i)
+      // and the scales and biases: of key m for the bias product, of this lane's
+      // scores (keys 4 c + i); of both halves, or (fp32: registers) of one
       typedef SB row_t __attribute__((ext_vector_type(NWG)));
-      row_t kbr, ksr, sk[4], bk[4];
+      constexpr int HA = F32 ? 1 : 2;
+      row_t kbr[HA], ksr[HA], sk[HA][4], bk[4];
       const auto sb_read = [&](int h) {
         if constexpr (!F32) {
-          kbr = *reinterpret_cast<const row_t*>(skb + (16 * h + m) * NG);
-          ksr = *reinterpret_cast<const row_t*>(sks + (16 * h + m) * NG);
+          kbr[h % HA] = *reinterpret_cast<const row_t*>(skb + (16 * h + m) * NG);
+          ksr[h % HA] = *reinterpret_cast<const row_t*>(sks + (16 * h + m) * NG);
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          sk[i] = *reinterpret_cast<const row_t*>(sks + (16 * h + 4 * c + i) * NG);
+          sk[h % HA][i] = *reinterpret_cast<const row_t*>(sks + (16 * h + 4 * c + i) * NG);
           if constexpr (F32) bk[i] = *reinterpret_cast<const row_t*>(skb + (16 * h + 4 * c + i) * NG);
         }
-        __builtin_amdgcn_sched_barrier(0);
       };
-      sb_read(0);
+#pragma unroll
+      for (int h = 0; h < HA; ++h) sb_read(h);
       b0 = *reinterpret_cast<const u32x2*>(brow + buf * bstep);
       b1 = *reinterpret_cast<const u32x2*>(brow + buf * bstep + 16);
 #pragma unroll
@@ -520,6 +521,17 @@ void paged_tiles_kernel(TileParams p) {
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
+        v4f bt = z;
+        if constexpr (!F32) {
+          v8h kb;
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            const _Float16 zero = static_cast<_Float16>(0.0f);
+            kb[g] = g < NWG ? kbr[h % HA][g < NWG ? g : 0] : zero;
+            kb[4 + g] = g < NWG ? ksr[h % HA][g < NWG ? g : 0] : zero;
+          }
+          bt = __builtin_amdgcn_mfma_f32_16x16x32_f16(kb, qb, z, 0, 0, 0);
+        }
         v4f acc[NWG];
 #pragma unroll
         for (int g0 = 0; g0 < NWG; g0 += GB) {
@@ -539,17 +551,7 @@ void paged_tiles_kernel(TileParams p) {
           if (g0 + GB < NWG) k_read(h, g0 + GB);
           else if (h == 0) k_read(1, 0);
         }
-        v4f bt = z;
-        if constexpr (!F32) {
-          v8h kb;
-#pragma unroll
-          for (int g = 0; g < 4; ++g) {
-            const _Float16 zero = static_cast<_Float16>(0.0f);
-            kb[g] = g < NWG ? kbr[g < NWG ? g : 0] : zero;
-            kb[4 + g] = g < NWG ? ksr[g < NWG ? g : 0] : zero;
-          }
-          bt = __builtin_amdgcn_mfma_f32_16x16x32_f16(kb, qb, z, 0, 0, 0);
-        }
+        if (F32 && h == 1) sb_read(1);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           float s = bt[i] * 512.0f;
@@ -558,16 +560,12 @@ void paged_tiles_kernel(TileParams p) {
             if constexpr (F32) {
               // s (. + 8 sum q) + b sum q
               s = fmaf(bk[i][g], qs[g] * 512.0f, s);
-              s = fmaf(sk[i][g], fmaf(qs[g], 4096.0f, acc[g][i]), s);
+              s = fmaf(sk[h % HA][i][g], fmaf(qs[g], 4096.0f, acc[g][i]), s);
             } else {
-              s = fmaf(static_cast<float>(sk[i][g]), acc[g][i], s);
+              s = fmaf(static_cast<float>(sk[h % HA][i][g]), acc[g][i], s);
             }
           }
           sc[4 * h + i] = s * rf;
-        }
-        if (h == 0) {
-          __builtin_amdgcn_sched_barrier(0);
-          sb_read(1);
         }
       }
     }
