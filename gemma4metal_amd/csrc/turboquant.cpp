@@ -61,14 +61,17 @@ struct Workspace {
   size_t bytes = 0;
 };
 std::mutex g_ws_mutex;
-std::map<std::pair<int, hipStream_t>, Workspace> g_ws;
+using Workspaces = std::map<std::pair<int, hipStream_t>, Workspace>;
+Workspaces g_ws;
+// Of the page plans, which leave other values in theirs.
+Workspaces g_plan_ws;
 
-void* workspace(size_t bytes, size_t* have, StreamOrDevice s) {
+void* workspace(size_t bytes, size_t* have, StreamOrDevice s, Workspaces& all = g_ws) {
   int dev = 0;
   check_hip(hipGetDevice(&dev), "hipGetDevice");
   const hipStream_t stream = static_cast<hipStream_t>(s);
   std::lock_guard<std::mutex> lock(g_ws_mutex);
-  Workspace& w = g_ws[{dev, stream}];
+  Workspace& w = all[{dev, stream}];
   if (w.bytes < bytes) {
     // Growing records an allocation, a fill and a free: under stream capture
     // they would become graph nodes, and the graph would own the buffer this
@@ -77,9 +80,9 @@ void* workspace(size_t bytes, size_t* have, StreamOrDevice s) {
     check_hip(hipStreamIsCapturing(stream, &cap), "hipStreamIsCapturing");
     if (cap != hipStreamCaptureStatusNone)
       throw std::runtime_error(
-          "turboquant: the split-K workspace of this (device, stream) must grow, but the stream "
+          "turboquant: the workspace of this (device, stream) must grow, but the stream "
           "is being captured; make one eager call of the largest shape on this stream before "
-          "capture, pass a workspace (sdpa_int4_into with workspace), or use "
+          "capture, pass a workspace (sdpa_int4_into with workspace, or the C calls), or use "
           "tq_sdpa_int4_noalloc");
     const size_t nb = std::max<size_t>(bytes, size_t{1} << 20);
     void* p = nullptr;
@@ -343,6 +346,221 @@ void kv_append_int4_ring(const array& k_new, const array& v_new, array& k_quant,
                          array& v_biases, const array& positions, StreamOrDevice s) {
   append_common(tq_kv_append_int4_ring, "kv_append_int4_ring", k_new, v_new, k_quant, k_scales,
                 k_biases, v_quant, v_scales, v_biases, positions, s);
+}
+
+// ---------------------------------------------------------------------------
+// Paged cache
+
+namespace {
+// Sizes of a pool, checked: all six tensors of one pool, with `lead` axes in front of
+// (num_pages, Hkv, page, .).
+struct PoolDims {
+  int layers = 1, pages = 0, Hkv = 0, page = 0, D = 0;
+  tq_dtype sb = TQ_F16;
+};
+
+PoolDims pool_dims(const kv_pages& p, bool layered) {
+  const std::vector<int64_t>& sh = p.k_quant.shape();
+  const size_t nd = sh.size();
+  need(nd == 4 || (layered && nd == 5),
+       "pages must be ([layers,] num_pages, num_kv_heads, page_size, .)");
+  std::vector<int64_t> sb = sh;
+  need(sb.back() % 8 == 0, "quant last dim must be a multiple of 8 (head_dim / 8)");
+  sb.back() /= 8;
+  for (const array* a : {&p.k_quant, &p.v_quant})
+    need(a->dtype() == Dtype::uint32 && a->shape() == sh, "k_quant / v_quant must be uint32 of one shape");
+  for (const array* a : {&p.k_scales, &p.k_biases, &p.v_scales, &p.v_biases})
+    need(is_sb(a->dtype()) && a->dtype() == p.k_scales.dtype() && a->shape() == sb,
+         "scales / biases must be (num_pages, num_kv_heads, page_size, head_dim/64) of one dtype");
+  for (int64_t d : sh) need(d >= 0 && d <= INT32_MAX, "pages: a size does not fit 32 bits");
+  PoolDims d;
+  d.layers = nd == 5 ? static_cast<int>(sh[0]) : 1;
+  d.pages = static_cast<int>(sh[nd - 4]);
+  d.Hkv = static_cast<int>(sh[nd - 3]);
+  d.page = static_cast<int>(sh[nd - 2]);
+  need(sh[nd - 1] <= INT32_MAX / 8, "pages: head_dim does not fit 32 bits");
+  d.D = static_cast<int>(sh[nd - 1] * 8);
+  d.sb = c_dtype(p.k_scales.dtype());
+  return d;
+}
+
+const int32_t* ints(const array& a, std::vector<int64_t> shape, const char* name) {
+  need(a.dtype() == Dtype::int32 && a.shape() == shape, std::string(name) + ": int32 of another shape needed");
+  return static_cast<const int32_t*>(a.data());
+}
+int32_t* ints(array& a, std::vector<int64_t> shape, const char* name) {
+  return const_cast<int32_t*>(ints(static_cast<const array&>(a), std::move(shape), name));
+}
+
+// Block tables (num_seqs, max_pages).
+struct Tables {
+  int32_t* p;
+  int seqs, width;
+};
+Tables tables_of(const array& t) {
+  need(t.ndim() == 2 && t.dtype() == Dtype::int32, "block_tables must be int32 (num_seqs, max_pages)");
+  need(t.shape(0) <= INT32_MAX && t.shape(1) <= INT32_MAX, "block_tables: a size does not fit 32 bits");
+  return {static_cast<int32_t*>(const_cast<void*>(t.data())), static_cast<int>(t.shape(0)),
+          static_cast<int>(t.shape(1))};
+}
+
+int page_count(const array& refs) {
+  need(refs.ndim() == 1 && refs.dtype() == Dtype::int32 && refs.shape(0) <= INT32_MAX,
+       "refs must be int32 (num_pages)");
+  return static_cast<int>(refs.shape(0));
+}
+
+const uint32_t* words(const array& a) { return static_cast<const uint32_t*>(a.data()); }
+
+struct SixPages {
+  void* p[6];
+  explicit SixPages(kv_pages& k)
+      : p{k.k_quant.data(), k.k_scales.data(), k.k_biases.data(),
+          k.v_quant.data(), k.v_scales.data(), k.v_biases.data()} {}
+};
+}  // namespace
+
+void kv_append_int4_paged(const array& k_new, const array& v_new, kv_pages& pages,
+                          const array& block_tables, const array& positions, StreamOrDevice s) {
+  const PoolDims d = pool_dims(pages, false);
+  const Tables t = tables_of(block_tables);
+  need(k_new.ndim() == 4 && v_new.shape() == k_new.shape() && v_new.dtype() == k_new.dtype(),
+       "k_new / v_new must be (B, Hkv, T, D) of one dtype");
+  need(k_new.shape(0) == t.seqs && k_new.shape(1) == d.Hkv && k_new.shape(3) == d.D,
+       "k_new / v_new do not fit the pages or block_tables");
+  need(k_new.shape(2) <= INT32_MAX, "k_new: a size does not fit 32 bits");
+  check(tq_kv_append_int4_paged(
+            k_new.data(), v_new.data(), c_dtype(k_new.dtype()),
+            static_cast<uint32_t*>(pages.k_quant.data()), pages.k_scales.data(),
+            pages.k_biases.data(), static_cast<uint32_t*>(pages.v_quant.data()),
+            pages.v_scales.data(), pages.v_biases.data(), d.sb, t.seqs, d.Hkv, d.D, d.page,
+            d.pages, t.p, t.width, ints(positions, {t.seqs}, "positions"),
+            static_cast<int>(k_new.shape(2)), TQ_QUANT_MLX, s),
+        "kv_append_int4_paged");
+}
+
+array sdpa_int4_paged(const array& queries, const kv_pages& pages, const array& block_tables,
+                      const array& seq_lens, int gqa_factor, float scale, int sliding_window,
+                      int num_sinks, int shared_prefix, const array& windows, int max_kv_len,
+                      StreamOrDevice s) {
+  const PoolDims d = pool_dims(pages, false);
+  const Tables t = tables_of(block_tables);
+  need(queries.ndim() == 3 && queries.shape(0) == t.seqs && queries.shape(2) == d.D &&
+           queries.shape(1) <= INT32_MAX,
+       "queries must be (B, num_heads, head_dim) for these pages and block_tables");
+  const int Hq = static_cast<int>(queries.shape(1));
+  const int64_t reach = static_cast<int64_t>(t.width) * d.page;
+  need(max_kv_len >= 0 || reach <= INT32_MAX, "block_tables reach past 32 bits");
+  const int n = max_kv_len < 0 ? static_cast<int>(reach) : max_kv_len;
+  array out = array::empty({t.seqs, Hq, d.D}, Dtype::float32);
+  size_t have = 0;
+  void* ws = workspace(tq_sdpa_int4_paged_workspace_size(t.seqs, Hq, d.Hkv, d.D, n, shared_prefix), &have, s);
+  check(tq_sdpa_int4_paged(queries.data(), c_dtype(queries.dtype()), words(pages.k_quant),
+                           pages.k_scales.data(), pages.k_biases.data(), words(pages.v_quant),
+                           pages.v_scales.data(), pages.v_biases.data(), d.sb,
+                           static_cast<float*>(out.data()), t.seqs, Hq, d.Hkv, d.D, d.page,
+                           d.pages, t.p, t.width, ints(seq_lens, {t.seqs}, "seq_lens"),
+                           windows.ndim() > 0 ? ints(windows, {t.seqs}, "windows") : nullptr, n,
+                           gqa_factor, scale, sliding_window, num_sinks, shared_prefix, ws, have, s),
+        "sdpa_int4_paged");
+  return out;
+}
+
+array sdpa_int4_paged_prefill(const array& queries, const kv_pages& pages,
+                              const array& block_table, int n_prior, int gqa_factor, float scale,
+                              int sliding_window, int num_sinks, StreamOrDevice s) {
+  const PoolDims d = pool_dims(pages, false);
+  need(queries.ndim() == 3 && queries.shape(2) == d.D && queries.shape(0) <= INT32_MAX &&
+           queries.shape(1) <= INT32_MAX,
+       "queries must be (n_new, num_heads, head_dim) for these pages");
+  need(block_table.ndim() == 1 && block_table.dtype() == Dtype::int32 &&
+           block_table.shape(0) <= INT32_MAX,
+       "block_table must be int32 (max_pages)");
+  const int S = static_cast<int>(queries.shape(0)), Hq = static_cast<int>(queries.shape(1));
+  array out = array::empty({S, Hq, d.D}, Dtype::float32);
+  size_t have = 0;
+  void* ws = workspace(tq_sdpa_int4_paged_prefill_workspace_size(Hq, d.Hkv, d.D, n_prior, S), &have, s);
+  check(tq_sdpa_int4_paged_prefill(queries.data(), c_dtype(queries.dtype()), words(pages.k_quant),
+                                   pages.k_scales.data(), pages.k_biases.data(),
+                                   words(pages.v_quant), pages.v_scales.data(),
+                                   pages.v_biases.data(), d.sb, static_cast<float*>(out.data()),
+                                   Hq, d.Hkv, d.D, d.page, d.pages,
+                                   static_cast<const int32_t*>(block_table.data()),
+                                   static_cast<int>(block_table.shape(0)), n_prior, S, gqa_factor,
+                                   scale, sliding_window, num_sinks, ws, have, s),
+        "sdpa_int4_paged_prefill");
+  return out;
+}
+
+array kv_pages_reserve(array& block_tables, array& refs, const array& lengths, const array& n_new,
+                       int page_size, StreamOrDevice s) {
+  const Tables t = tables_of(block_tables);
+  const int pages = page_count(refs);
+  array granted = array::empty({t.seqs}, Dtype::int32);
+  size_t have = 0;
+  void* ws = workspace(tq_kv_pages_workspace_size(t.seqs, pages), &have, s, g_plan_ws);
+  check(tq_kv_pages_reserve(t.p, static_cast<int32_t*>(refs.data()), ints(lengths, {t.seqs}, "lengths"),
+                            ints(n_new, {t.seqs}, "n_new"), static_cast<int32_t*>(granted.data()),
+                            t.seqs, t.width, pages, page_size, ws, have, s),
+        "kv_pages_reserve");
+  return granted;
+}
+
+array kv_pages_fork(kv_pages& pages, array& block_tables, array& refs, array& lengths,
+                    const array& parents, StreamOrDevice s) {
+  const PoolDims d = pool_dims(pages, true);
+  const Tables t = tables_of(block_tables);
+  array granted = array::empty({t.seqs}, Dtype::int32);
+  size_t have = 0;
+  void* ws = workspace(tq_kv_pages_workspace_size(t.seqs, d.pages), &have, s, g_plan_ws);
+  check(tq_kv_pages_fork(SixPages(pages).p, d.sb, d.layers, d.Hkv, d.D, t.p,
+                         ints(refs, {d.pages}, "refs"), ints(lengths, {t.seqs}, "lengths"),
+                         ints(parents, {t.seqs}, "parents"), static_cast<int32_t*>(granted.data()),
+                         t.seqs, t.width, d.pages, d.page, ws, have, s),
+        "kv_pages_fork");
+  return granted;
+}
+
+void kv_pages_free(array& block_tables, array& refs, array& lengths, const array& which,
+                   StreamOrDevice s) {
+  const Tables t = tables_of(block_tables);
+  const int pages = page_count(refs);
+  check(tq_kv_pages_free(t.p, static_cast<int32_t*>(refs.data()), ints(lengths, {t.seqs}, "lengths"),
+                         ints(which, {t.seqs}, "which"), t.seqs, t.width, pages, s),
+        "kv_pages_free");
+}
+
+void kv_pages_evict(array& block_tables, array& refs, const array& lengths, int page_size,
+                    int sliding_window, int num_sinks, const array& which, StreamOrDevice s) {
+  const Tables t = tables_of(block_tables);
+  const int pages = page_count(refs);
+  check(tq_kv_pages_evict(t.p, static_cast<int32_t*>(refs.data()), ints(lengths, {t.seqs}, "lengths"),
+                          which.ndim() > 0 ? ints(which, {t.seqs}, "which") : nullptr, t.seqs,
+                          t.width, pages, page_size, sliding_window, num_sinks, s),
+        "kv_pages_evict");
+}
+
+array kv_pages_compact(kv_pages& pages, array& block_tables, array& refs, StreamOrDevice s) {
+  const PoolDims d = pool_dims(pages, true);
+  const Tables t = tables_of(block_tables);
+  int32_t* r = ints(refs, {d.pages}, "refs");
+  array live = array::empty({1}, Dtype::int32);
+  size_t have = 0;
+  void* ws = workspace(tq_kv_pages_workspace_size(t.seqs, d.pages), &have, s, g_plan_ws);
+  check(tq_kv_pages_compact(SixPages(pages).p, d.sb, d.layers, d.Hkv, d.D, t.p, r, t.p, r,
+                            static_cast<int32_t*>(live.data()), t.seqs, t.width, d.pages, d.page,
+                            ws, have, s),
+        "kv_pages_compact");
+  return live;
+}
+
+void kv_pages_copy(kv_pages& pages, const array& src, const array& dst, StreamOrDevice s) {
+  const PoolDims d = pool_dims(pages, true);
+  need(src.ndim() == 1 && src.shape(0) <= INT32_MAX, "src must be int32 (n)");
+  check(tq_kv_pages_copy(SixPages(pages).p, d.sb, d.layers, d.Hkv, d.D, d.pages, d.page,
+                         ints(src, {src.shape(0)}, "src"), ints(dst, {src.shape(0)}, "dst"),
+                         static_cast<int>(src.shape(0)), s),
+        "kv_pages_copy");
 }
 
 // ---------------------------------------------------------------------------

@@ -140,6 +140,58 @@ void kv_append_int4_ring(const array& k_new, const array& v_new, array& k_quant,
                          array& k_scales, array& k_biases, array& v_quant, array& v_scales,
                          array& v_biases, const array& positions, StreamOrDevice s = {});
 
+// ---- paged int4 cache (no counterpart in the reference) ----------------------
+// The six tensors of a pool of pages: quant uint32 (num_pages, num_kv_heads,
+// page_size, head_dim/8), scales / biases float16 | float32 (num_pages,
+// num_kv_heads, page_size, head_dim/64); page_size a power of two, 32 to 1024.
+// The calls that move pages take a leading axis of layers as well.  Block tables
+// (num_seqs, max_pages), lengths and reference counts are int32 device arrays; an
+// entry outside [0, num_pages) names no page.  Their semantics are those of the
+// tq_kv_pages_* and *_paged calls of tq_c_api.h.  Workspaces are the library's, per
+// (device, stream), as for sdpa_int4_into.
+struct kv_pages {
+  array k_quant, k_scales, k_biases, v_quant, v_scales, v_biases;
+};
+
+// k_new / v_new (B, Hkv, T, D) at rows positions[b] .. positions[b]+T-1 of sequence b.
+void kv_append_int4_paged(const array& k_new, const array& v_new, kv_pages& pages,
+                          const array& block_tables, const array& positions,
+                          StreamOrDevice s = {});
+// Decode: queries (B, num_heads, head_dim); key t < seq_lens[b] is attended iff
+// sliding_window (windows[b], if given) is 0, or t is among the last that many, or
+// t < num_sinks.  The first shared_prefix rows of all sequences lie in the pages of
+// sequence 0.  max_kv_len < 0: what the tables reach.  Returns (B, num_heads,
+// head_dim) f32.
+array sdpa_int4_paged(const array& queries, const kv_pages& pages, const array& block_tables,
+                      const array& seq_lens, int gqa_factor, float scale = 1.0f,
+                      int sliding_window = 0, int num_sinks = 0, int shared_prefix = 0,
+                      const array& windows = {}, int max_kv_len = -1, StreamOrDevice s = {});
+// Prompt: queries (n_new, num_heads, head_dim) at positions n_prior ... over the
+// pages of one sequence, block_table (max_pages), which hold the new rows already.
+array sdpa_int4_paged_prefill(const array& queries, const kv_pages& pages,
+                              const array& block_table, int n_prior, int gqa_factor,
+                              float scale = 1.0f, int sliding_window = 0, int num_sinks = 0,
+                              StreamOrDevice s = {});
+
+// Pages for rows lengths[s] .. lengths[s] + n_new[s] - 1.  Returns int32
+// (num_seqs): 1 where the request was granted (as kv_pages_fork does).
+array kv_pages_reserve(array& block_tables, array& refs, const array& lengths, const array& n_new,
+                       int page_size, StreamOrDevice s = {});
+// Sequence s continues parents[s] (negative: none).
+array kv_pages_fork(kv_pages& pages, array& block_tables, array& refs, array& lengths,
+                    const array& parents, StreamOrDevice s = {});
+// Ends the sequences with which[s] != 0.
+void kv_pages_free(array& block_tables, array& refs, array& lengths, const array& which,
+                   StreamOrDevice s = {});
+// Gives up the pages that a window and sinks no longer see (which empty: of all).
+void kv_pages_evict(array& block_tables, array& refs, const array& lengths, int page_size,
+                    int sliding_window, int num_sinks = 0, const array& which = {},
+                    StreamOrDevice s = {});
+// Moves the pages in use to the front, in place.  Returns int32 (1): how many.
+array kv_pages_compact(kv_pages& pages, array& block_tables, array& refs, StreamOrDevice s = {});
+// Copies page src[i] to page dst[i].
+void kv_pages_copy(kv_pages& pages, const array& src, const array& dst, StreamOrDevice s = {});
+
 // ---- PolarQuant (lib/turboquant.h:52-165) -----------------------------------
 // Reference layouts: 16-value blocks, 4 levels, codebooks per level.
 std::vector<array> polar_quantize(const array& vectors, const array& precondition,
