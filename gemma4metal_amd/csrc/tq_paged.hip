@@ -165,7 +165,7 @@ extern "C" size_t tq_sdpa_int4_paged_workspace_size(int batch, int num_heads, in
   const int gqa = num_heads / num_kv_heads;
   int splits = max_paged_splits(batch, num_heads, num_kv_heads, head_dim, max_kv_len);
   if (shared_prefix > 0)
-    splits += paged_tiles_splits(static_cast<int64_t>(batch) * gqa, num_kv_heads, head_dim, shared_prefix);
+    splits += plan_paged_tiles(static_cast<int64_t>(batch) * gqa, num_kv_heads, head_dim, shared_prefix).splits;
   return ws_layout(batch, num_heads, head_dim, splits).total + kWsTail;
 }
 
@@ -209,8 +209,10 @@ extern "C" int tq_sdpa_int4_paged(const void* q, tq_dtype q_dtype, const uint32_
   p.lpt_jobs = pl.grid_x * batch;
   p.waves = pl.waves;
   p.cus = pl.slots;
+  TilesPlan tiles{0, 0};
   if (shared_prefix > 0)
-    p.pre = paged_tiles_splits(static_cast<int64_t>(batch) * gqa_factor, num_kv_heads, head_dim, shared_prefix);
+    tiles = plan_paged_tiles(static_cast<int64_t>(batch) * gqa_factor, num_kv_heads, head_dim, shared_prefix);
+  p.pre = tiles.splits;
   p.max_splits = pl.max_splits + p.pre;
   if (p.max_splits > 1) {
     if (int r = set_workspace(p, workspace, workspace_bytes, ws_layout(batch, num_heads, head_dim, p.max_splits), fn)) return r;
@@ -219,7 +221,7 @@ extern "C" int tq_sdpa_int4_paged(const void* q, tq_dtype q_dtype, const uint32_
   p.cnt_stride = counter_stride(static_cast<int64_t>(batch) * num_heads);
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (p.pre > 0)
-    if (int r = launch_paged_tiles(p, head_dim, sb_dtype, p.pre, true, s)) return r;
+    if (int r = launch_paged_tiles(p, head_dim, sb_dtype, tiles, true, s)) return r;
   if (!pl.hc) return launch_sdpa_mfma(p, head_dim, pl.G, sb_dtype, grid, s);
   p.ext_merge = p.max_splits > 1 ? 1 : 0;
   const int r = launch_sdpa_hc(p, sb_dtype, grid, s);
@@ -243,8 +245,8 @@ extern "C" int tq_sdpa_int4_paged_plan(int batch, int num_heads, int num_kv_head
   if (splits) *splits = pl.max_splits;
   if (chunk_keys) *chunk_keys = pl.chunk;
   if (shared_splits)
-    *shared_splits = shared_prefix > 0 ? paged_tiles_splits(static_cast<int64_t>(batch) * (num_heads / num_kv_heads),
-                                                            num_kv_heads, head_dim, shared_prefix)
+    *shared_splits = shared_prefix > 0 ? plan_paged_tiles(static_cast<int64_t>(batch) * (num_heads / num_kv_heads),
+                                                          num_kv_heads, head_dim, shared_prefix).splits
                                        : 0;
   if (on_device) *on_device = pl.lpt ? 1 : 0;
   if (kernel && kernel_bytes > 0)
@@ -285,9 +287,9 @@ extern "C" int tq_sdpa_int4_paged_prefill(const void* q, tq_dtype q_dtype, const
   p.n = n_prior;
   const int64_t rows = static_cast<int64_t>(n_new) * gqa_factor;
   TQ_CHECK_ARG((rows + 63) / 64 * num_kv_heads < (int64_t{1} << 31), "%s: grid too large", fn);
-  const int splits = paged_tiles_splits(rows, num_kv_heads, head_dim, prompt_keys(n_prior, n_new, sliding_window, num_sinks));
-  p.max_splits = splits;
-  if (splits > 1)
-    if (int r = set_workspace(p, workspace, workspace_bytes, ws_layout(n_new, num_heads, head_dim, splits), fn)) return r;
-  return launch_paged_tiles(p, head_dim, sb_dtype, splits, false, static_cast<hipStream_t>(stream));
+  const TilesPlan tiles = plan_paged_tiles(rows, num_kv_heads, head_dim, prompt_keys(n_prior, n_new, sliding_window, num_sinks));
+  p.max_splits = tiles.splits;
+  if (tiles.splits > 1)
+    if (int r = set_workspace(p, workspace, workspace_bytes, ws_layout(n_new, num_heads, head_dim, tiles.splits), fn)) return r;
+  return launch_paged_tiles(p, head_dim, sb_dtype, tiles, false, static_cast<hipStream_t>(stream));
 }

@@ -20,8 +20,7 @@
 namespace tq {
 namespace {
 
-constexpr int kRs = 4;           // 16-row sets of a workgroup
-constexpr int kRows = 16 * kRs;
+constexpr int kRs = 4;  // 16-row sets of a tile's geometry (PfGeom): 8 waves
 
 template <int KH>
 struct PgTile {
@@ -227,12 +226,17 @@ struct TileParams : PagedParams {
   int splits;  // workgroups along the tiles (grid y); 1: write p.out
 };
 
-template <int D, bool F32, bool Q32>
+// RS: 16-row sets of a workgroup.  4: a wave takes 32 keys of a tile (of 64 keys, D
+// 512 of 32); 8 (D < 512): all 64, one half after the other.
+template <int D, bool F32, bool Q32, int RS>
 __global__ __launch_bounds__(128 * kRs) __attribute__((amdgpu_waves_per_eu(2, 2)))
 void paged_tiles_kernel(TileParams p) {
   using Gm = PfGeom<D, F32, kRs>;
   using SB = typename Gm::SB;
-  constexpr int NG = Gm::NG, NWG = Gm::NW_, TK = Gm::TK, KH = Gm::KH, DH = Gm::DH, RS = kRs;
+  constexpr int NG = Gm::NG, NWG = Gm::NW_, TK = Gm::TK, KH = Gm::KH, DH = Gm::DH;
+  constexpr int KW = Gm::NW / (RS * DH), HB = KH / KW;  // waves that share a row set's keys; parts of each
+  constexpr int kRows = 16 * RS;
+  static_assert(KW >= 1 && HB >= 1, "waves");
   using St = PgStage<D, F32>;
   __shared__ __attribute__((aligned(16))) union Lds {
     St st;
@@ -245,7 +249,7 @@ void paged_tiles_kernel(TileParams p) {
 
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
-  const int rs = wave % RS, kh = wave / RS % KH, dh = wave / (RS * KH);
+  const int rs = wave % RS, kw = wave / RS % KW, dh = wave / (RS * KW);
   const int m = lane & 15, c = lane >> 4;
   // heads vary fastest, the longest key ranges (last queries) start first
   const int nblk = gridDim.x / p.Hkv;
@@ -270,7 +274,13 @@ void paged_tiles_kernel(TileParams p) {
   int hi_w, lo_w;
   {
     int h, l;
-    limits(min(r0 + lane, total - 1), h, l);  // lane: row (kRows of them)
+    limits(min(r0 + lane, total - 1), h, l);
+    if constexpr (kRows > 64) {
+      int h1, l1;
+      limits(min(r0 + 64 + lane, total - 1), h1, l1);
+      h = max(h, h1);
+      l = min(l, l1);
+    }
     hi_w = max_of_wave(h);
     lo_w = min_of_wave(l);
   }
@@ -439,7 +449,7 @@ void paged_tiles_kernel(TileParams p) {
   } else if (!F32 && m == 8) {
     brow = L.st.one;
   }
-  brow += 4 * c + (bstep ? 32 * kh : 0);
+  brow += 4 * c;
   const float pscale = __uint_as_float((e0 + 2 + 127) << 23);
   const float bun = F32 ? 0.25f : __uint_as_float((127 - e0 - 2) << 23), bup = F32 ? 4.0f : pscale;
 
@@ -458,290 +468,294 @@ void paged_tiles_kernel(TileParams p) {
       nxt = tile_at(it + 1);
       pg_load<Gm>(raw, from, nxt);
     }
-    const int t0 = cur.key + 32 * kh;  // this wave's keys t0 .. t0 + 31
-    const bool has = KH == 2 && kh ? cur.has[KH - 1] : cur.has[0];
-    const bool any = has && rw < total && t0 < hi_max && (t0 + 31 >= lo_min || t0 < p.sinks);  // wave-uniform
-    // this wave's groups
-    const u32x4* ku = L.st.k[buf] + 2 * kh * Gm::KU + 128 * NWG * dh + 16 * c;
-    const u32x4* vu = L.st.v[buf] + kh * Gm::VU + 256 * NWG * dh + 16 * c;
-    const SB* sks = L.st.ksb[buf][0] + 32 * kh * NG + NWG * dh;
-    const SB* skb = L.st.ksb[buf][1] + 32 * kh * NG + NWG * dh;
-    // V operands of group g, and its scales of this lane's 8 keys
-    const auto v_read = [&](int g, u32x4 (&a)[4]) {
+#pragma unroll 1
+    for (int part = 0; part < HB; ++part) {
+      const int kh = KW == 1 ? part : kw;
+      const int t0 = cur.key + 32 * kh;  // this wave's keys t0 .. t0 + 31
+      const bool has = KH == 2 && kh ? cur.has[KH - 1] : cur.has[0];
+      const bool any = has && rw < total && t0 < hi_max && (t0 + 31 >= lo_min || t0 < p.sinks);  // wave-uniform
+      // this wave's groups
+      const u32x4* ku = L.st.k[buf] + 2 * kh * Gm::KU + 128 * NWG * dh + 16 * c;
+      const u32x4* vu = L.st.v[buf] + kh * Gm::VU + 256 * NWG * dh + 16 * c;
+      const SB* sks = L.st.ksb[buf][0] + 32 * kh * NG + NWG * dh;
+      const SB* skb = L.st.ksb[buf][1] + 32 * kh * NG + NWG * dh;
+      // V operands of group g, and its scales of this lane's 8 keys
+      const auto v_read = [&](int g, u32x4 (&a)[4]) {
 #pragma unroll
-      for (int x = 0; x < 4; ++x) a[x] = vu[(4 * g + x) * 64 + (m ^ Gm::vswz(g))];
-    };
-    typedef typename std::conditional<F32, v4f, v4h>::type s4;
-    // (from, by bytes a group: the staged scales, or zeros)
-    const auto s_read = [&](const char* from, int step, int g, s4 (&s)[2]) {
+        for (int x = 0; x < 4; ++x) a[x] = vu[(4 * g + x) * 64 + (m ^ Gm::vswz(g))];
+      };
+      typedef typename std::conditional<F32, v4f, v4h>::type s4;
+      // (from, by bytes a group: the staged scales, or zeros)
+      const auto s_read = [&](const char* from, int step, int g, s4 (&s)[2]) {
 #pragma unroll
-      for (int h = 0; h < 2; ++h) s[h] = *reinterpret_cast<const s4*>(from + g * step + 16 * h * (F32 ? 4 : 2));
-    };
+        for (int h = 0; h < 2; ++h) s[h] = *reinterpret_cast<const s4*>(from + g * step + 16 * h * (F32 ? 4 : 2));
+      };
 
-    u32x2 b0{}, b1{};  // the bias products' operand
-    int al = 1;
-    float sc[8];
-    if (any) {
-      // ---- S^T: two 16-key halves.  The operands of GB groups are read at once,
-      // the next ones under the products and scores of these.
-      constexpr int GB = Q32 && NWG > 1 ? NWG / 2 : NWG;
-      u32x4 ka[2 * GB];
-      const auto k_read = [&](int h, int g0) {
+      u32x2 b0{}, b1{};  // the bias products' operand
+      int al = 1;
+      float sc[8];
+      if (any) {
+        // ---- S^T: two 16-key halves.  The operands of GB groups are read at once,
+        // the next ones under the products and scores of these.
+        constexpr int GB = Q32 && NWG > 1 ? NWG / 2 : NWG;
+        u32x4 ka[2 * GB];
+        const auto k_read = [&](int h, int g0) {
 #pragma unroll
-        for (int g = 0; g < GB; ++g) {
-          const u32x4* kr = ku + h * Gm::KU + 128 * (g0 + g) + (m ^ Gm::kswz(NWG * dh + g0 + g));
-          ka[2 * g] = kr[0];
-          ka[2 * g + 1] = kr[64];
-        }
-        __builtin_amdgcn_sched_barrier(0);
-      };
-      k_read(0, 0);
-      // and the scales and biases: of key m for the bias product, of this lane's
-      // scores (keys 4 c + i); of both halves, or (fp32: registers) of one
-      typedef SB row_t __attribute__((ext_vector_type(NWG)));
-      constexpr int HA = F32 ? 1 : 2;
-      row_t kbr[HA], ksr[HA], sk[HA][4], bk[4];
-      const auto sb_read = [&](int h) {
-        if constexpr (!F32) {
-          kbr[h % HA] = *reinterpret_cast<const row_t*>(skb + (16 * h + m) * NG);
-          ksr[h % HA] = *reinterpret_cast<const row_t*>(sks + (16 * h + m) * NG);
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          sk[h % HA][i] = *reinterpret_cast<const row_t*>(sks + (16 * h + 4 * c + i) * NG);
-          if constexpr (F32) bk[i] = *reinterpret_cast<const row_t*>(skb + (16 * h + 4 * c + i) * NG);
-        }
-      };
-#pragma unroll
-      for (int h = 0; h < HA; ++h) sb_read(h);
-      b0 = *reinterpret_cast<const u32x2*>(brow + buf * bstep);
-      b1 = *reinterpret_cast<const u32x2*>(brow + buf * bstep + 16);
-#pragma unroll
-      for (int i = 0; i < 2 * Gm::NSW; ++i) al &= alike[buf][i];
-      __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        v4f bt = z;
-        if constexpr (!F32) {
-          v8h kb;
-#pragma unroll
-          for (int g = 0; g < 4; ++g) {
-            const _Float16 zero = static_cast<_Float16>(0.0f);
-            kb[g] = g < NWG ? kbr[h % HA][g < NWG ? g : 0] : zero;
-            kb[4 + g] = g < NWG ? ksr[h % HA][g < NWG ? g : 0] : zero;
-          }
-          bt = __builtin_amdgcn_mfma_f32_16x16x32_f16(kb, qb, z, 0, 0, 0);
-        }
-        v4f acc[NWG];
-#pragma unroll
-        for (int g0 = 0; g0 < NWG; g0 += GB) {
-#pragma unroll
-          for (int gi = 0; gi < GB; ++gi) {
-            const int g = g0 + gi;
-            const v8h a0 = __builtin_bit_cast(v8h, ka[2 * gi]), a1 = __builtin_bit_cast(v8h, ka[2 * gi + 1]);
-            v4f a = __builtin_amdgcn_mfma_f32_16x16x32_f16(a0, qf[2 * g], z, 0, 0, 0);
-            a = __builtin_amdgcn_mfma_f32_16x16x32_f16(a1, qf[2 * g + 1], a, 0, 0, 0);
-            if constexpr (Q32) {
-              a = __builtin_amdgcn_mfma_f32_16x16x32_f16(a0, ql[2 * g], a, 0, 0, 0);
-              a = __builtin_amdgcn_mfma_f32_16x16x32_f16(a1, ql[2 * g + 1], a, 0, 0, 0);
-            }
-            acc[g] = a;
+          for (int g = 0; g < GB; ++g) {
+            const u32x4* kr = ku + h * Gm::KU + 128 * (g0 + g) + (m ^ Gm::kswz(NWG * dh + g0 + g));
+            ka[2 * g] = kr[0];
+            ka[2 * g + 1] = kr[64];
           }
           __builtin_amdgcn_sched_barrier(0);
-          if (g0 + GB < NWG) k_read(h, g0 + GB);
-          else if (h == 0) k_read(1, 0);
-        }
-        if (F32 && h == 1) sb_read(1);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          float s = bt[i] * 512.0f;
-#pragma unroll
-          for (int g = 0; g < NWG; ++g) {
-            if constexpr (F32) {
-              // s (. + 8 sum q) + b sum q
-              s = fmaf(bk[i][g], qs[g] * 512.0f, s);
-              s = fmaf(sk[h % HA][i][g], fmaf(qs[g], 4096.0f, acc[g][i]), s);
-            } else {
-              s = fmaf(static_cast<float>(sk[h % HA][i][g]), acc[g][i], s);
-            }
+        };
+        k_read(0, 0);
+        // and the scales and biases: of key m for the bias product, of this lane's
+        // scores (keys 4 c + i); of both halves, or (fp32: registers) of one
+        typedef SB row_t __attribute__((ext_vector_type(NWG)));
+        constexpr int HA = F32 ? 1 : 2;
+        row_t kbr[HA], ksr[HA], sk[HA][4], bk[4];
+        const auto sb_read = [&](int h) {
+          if constexpr (!F32) {
+            kbr[h % HA] = *reinterpret_cast<const row_t*>(skb + (16 * h + m) * NG);
+            ksr[h % HA] = *reinterpret_cast<const row_t*>(sks + (16 * h + m) * NG);
           }
-          sc[4 * h + i] = s * rf;
-        }
-      }
-    }
-    if constexpr (DH == 2) {
-      // the other wave's groups: its parts of the same scores
-      if (any) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
-          L.st.xch[wave][h][lane] = v4f{sc[4 * h], sc[4 * h + 1], sc[4 * h + 2], sc[4 * h + 3]};
-      }
-      __syncthreads();
-      if (any) {
+          for (int i = 0; i < 4; ++i) {
+            sk[h % HA][i] = *reinterpret_cast<const row_t*>(sks + (16 * h + 4 * c + i) * NG);
+            if constexpr (F32) bk[i] = *reinterpret_cast<const row_t*>(skb + (16 * h + 4 * c + i) * NG);
+          }
+        };
+#pragma unroll
+        for (int h = 0; h < HA; ++h) sb_read(h);
+        b0 = *reinterpret_cast<const u32x2*>(brow + buf * bstep + 32 * kh);
+        b1 = *reinterpret_cast<const u32x2*>(brow + buf * bstep + 32 * kh + 16);
+#pragma unroll
+        for (int i = 0; i < 2 * Gm::NSW; ++i) al &= alike[buf][i];
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const v4f x = L.st.xch[wave ^ RS][h][lane];
+          v4f bt = z;
+          if constexpr (!F32) {
+            v8h kb;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) sc[4 * h + i] += x[i];
+            for (int g = 0; g < 4; ++g) {
+              const _Float16 zero = static_cast<_Float16>(0.0f);
+              kb[g] = g < NWG ? kbr[h % HA][g < NWG ? g : 0] : zero;
+              kb[4 + g] = g < NWG ? ksr[h % HA][g < NWG ? g : 0] : zero;
+            }
+            bt = __builtin_amdgcn_mfma_f32_16x16x32_f16(kb, qb, z, 0, 0, 0);
+          }
+          v4f acc[NWG];
+#pragma unroll
+          for (int g0 = 0; g0 < NWG; g0 += GB) {
+#pragma unroll
+            for (int gi = 0; gi < GB; ++gi) {
+              const int g = g0 + gi;
+              const v8h a0 = __builtin_bit_cast(v8h, ka[2 * gi]), a1 = __builtin_bit_cast(v8h, ka[2 * gi + 1]);
+              v4f a = __builtin_amdgcn_mfma_f32_16x16x32_f16(a0, qf[2 * g], z, 0, 0, 0);
+              a = __builtin_amdgcn_mfma_f32_16x16x32_f16(a1, qf[2 * g + 1], a, 0, 0, 0);
+              if constexpr (Q32) {
+                a = __builtin_amdgcn_mfma_f32_16x16x32_f16(a0, ql[2 * g], a, 0, 0, 0);
+                a = __builtin_amdgcn_mfma_f32_16x16x32_f16(a1, ql[2 * g + 1], a, 0, 0, 0);
+              }
+              acc[g] = a;
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            if (g0 + GB < NWG) k_read(h, g0 + GB);
+            else if (h == 0) k_read(1, 0);
+          }
+          if (F32 && h == 1) sb_read(1);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            float s = bt[i] * 512.0f;
+#pragma unroll
+            for (int g = 0; g < NWG; ++g) {
+              if constexpr (F32) {
+                // s (. + 8 sum q) + b sum q
+                s = fmaf(bk[i][g], qs[g] * 512.0f, s);
+                s = fmaf(sk[h % HA][i][g], fmaf(qs[g], 4096.0f, acc[g][i]), s);
+              } else {
+                s = fmaf(static_cast<float>(sk[h % HA][i][g]), acc[g][i], s);
+              }
+            }
+            sc[4 * h + i] = s * rf;
+          }
         }
       }
-    }
-    if (any) {
-      // whether all of these keys are attended by all rows; wave-uniform
-      const bool inside = t0 <= hi_min - 32 && (t0 >= lo_max || t0 <= p.sinks - 32);
-      if (!inside) {
-        const int at = t0 + 4 * c;
+      if constexpr (DH == 2) {
+        // the other wave's groups: its parts of the same scores
+        if (any) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const int k = 16 * (j >> 2) + (j & 3);
-          sc[j] = k < hi - at && (k >= lo - at || k < p.sinks - at) ? sc[j] : -INFINITY;
+          for (int h = 0; h < 2; ++h)
+            L.st.xch[wave][h][lane] = v4f{sc[4 * h], sc[4 * h + 1], sc[4 * h + 2], sc[4 * h + 3]};
+        }
+        __syncthreads();
+        if (any) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const v4f x = L.st.xch[wave ^ RS][h][lane];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sc[4 * h + i] += x[i];
+          }
         }
       }
-
-      // ---- online softmax (log2 domain) of rows m ------------------------------
-      const float up = static_cast<float>(e0 - kPfHead);
-      float mt = sc[0];
-#pragma unroll
-      for (int j = 1; j < 8; ++j) mt = fmaxf(mt, sc[j]);
-      const float need = xor32_max(xor16_max(mt)) + up;
-      // (a row with nothing attended yet and nothing here keeps -inf)
-      if (__any(need > m_ref + kPfLazy)) {
-        const float m_new = need > m_ref ? need : m_ref;
-        const float fr = m_new == m_ref ? 1.0f : merge_factor(m_ref, m_new);
-        l_run *= fr;
-        ob *= fr;
-#pragma unroll
-        for (int b = 0; b < 4 * NWG; ++b) o[b] *= fr;
-        m_ref = m_new;
-      }
-      // In a tile that is not plain the products below take weights and biases of 0
-      // (a branch around them would cost a second set of accumulators).
-      const bool plain = __builtin_amdgcn_readfirstlane(al) != 0;
-      const char* sfrom;
-      int sstep = 0;
-      if constexpr (F32) {
-        sfrom = reinterpret_cast<const char*>(plain ? &L.st.vsb[buf][0][NWG * dh][32 * kh] : &L.st.zero32[0]);
-        if (plain) sstep = sizeof(L.st.vsb[0][0][0]);
-        sfrom += 16 * c;
-      } else {
-        sfrom = reinterpret_cast<const char*>(plain ? &L.st.vp[buf][1][NWG * dh][32 * kh] : &L.st.zero[0]);
-        if (plain) sstep = sizeof(L.st.vp[0][0][0]);
-        sfrom += 8 * c;
-      }
-      u32x4 va[4];
-      s4 vs[2][2];
-      v_read(0, va);
-      s_read(sfrom, sstep, 0, vs[0]);
-      const uint32_t bm = plain ? ~0u : 0u;
-      const v8h ba = __builtin_bit_cast(v8h, u32x4{b0[0] & bm, b0[1] & bm, b1[0] & bm, b1[1] & bm});
-      __builtin_amdgcn_sched_barrier(0);
-      float pw[8];
-      // (with nothing attended so far, -inf - -inf would be NaN)
-      const float ms = m_ref == -INFINITY ? 0.0f : m_ref;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) pw[j] = fast_exp2(sc[j] - ms);
-      if constexpr (F32) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) l_run += pw[j];
-      }
-
-      // ---- O^T += V^T P^T ----------------------------------------------------
-      // B operands of eight weights
-      const auto split = [&](const float (&y)[8], v8h& bh, v8h& bl) {
-        u32x4 hw, lw;
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          hw[q] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(y[2 * q], y[2 * q + 1]));
-          lw[q] = pf_rem_pair(hw[q], y[2 * q], y[2 * q + 1]);
-        }
-        bh = __builtin_bit_cast(v8h, hw);
-        bl = __builtin_bit_cast(v8h, lw);
-      };
-      if (!plain) {
-        // V scales apart, or scales and biases out of range or not finite: the
-        // largest weight of every row and group to 2^13 .. 2^14 (an infinity, of
-        // exponent 0, stays one), the products on their own, added in fp32, and
-        // bias terms in fp32 -- without those of weight 0, whose keys the row may
-        // not attend at all
-        const auto times = [](float w, float x) { return w > 0.0f || w != w ? w * x : 0.0f; };
-        float add[4] = {0.0f, 0.0f, 0.0f, 0.0f}, lw = 0.0f;
-#pragma unroll 1
-        for (int g = 0; g < NWG; ++g) {
-          float y[8], big = 0.0f, sb = 0.0f;
+      if (any) {
+        // whether all of these keys are attended by all rows; wave-uniform
+        const bool inside = t0 <= hi_min - 32 && (t0 >= lo_max || t0 <= p.sinks - 32);
+        if (!inside) {
+          const int at = t0 + 4 * c;
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
-            const int at = 32 * kh + 16 * (j >> 2) + 4 * c + (j & 3);
-            float s, b;
-            if constexpr (F32) {
-              s = L.st.vsb[buf][0][NWG * dh + g][at];
-              b = L.st.vsb[buf][1][NWG * dh + g][at];
-            } else {
-              s = static_cast<float>(L.st.vp[buf][1][NWG * dh + g][at]);
-              b = static_cast<float>(L.st.vp[buf][0][NWG * dh + g][at]);
-            }
-            y[j] = times(pw[j], s);
-            sb += times(pw[j], fmaf(s, 8.0f, b));
-            big = fmaxf(big, fabsf(y[j]));
+            const int k = 16 * (j >> 2) + (j & 3);
+            sc[j] = k < hi - at && (k >= lo - at || k < p.sinks - at) ? sc[j] : -INFINITY;
           }
-          sb = xor32_sum(xor16_sum(sb)) * bup;
+        }
+
+        // ---- online softmax (log2 domain) of rows m ------------------------------
+        const float up = static_cast<float>(e0 - kPfHead);
+        float mt = sc[0];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) add[i] = i == g ? sb : add[i];
-          const int k = min(14 - __builtin_amdgcn_frexp_expf(xor32_max(xor16_max(big))), 120);
-          const float un = ldexpf(1.0f, -k);
+        for (int j = 1; j < 8; ++j) mt = fmaxf(mt, sc[j]);
+        const float need = xor32_max(xor16_max(mt)) + up;
+        // (a row with nothing attended yet and nothing here keeps -inf)
+        if (__any(need > m_ref + kPfLazy)) {
+          const float m_new = need > m_ref ? need : m_ref;
+          const float fr = m_new == m_ref ? 1.0f : merge_factor(m_ref, m_new);
+          l_run *= fr;
+          ob *= fr;
 #pragma unroll
-          for (int j = 0; j < 8; ++j) y[j] = ldexpf(y[j], k);
+          for (int b = 0; b < 4 * NWG; ++b) o[b] *= fr;
+          m_ref = m_new;
+        }
+        // In a tile that is not plain the products below take weights and biases of 0
+        // (a branch around them would cost a second set of accumulators).
+        const bool plain = __builtin_amdgcn_readfirstlane(al) != 0;
+        const char* sfrom;
+        int sstep = 0;
+        if constexpr (F32) {
+          sfrom = reinterpret_cast<const char*>(plain ? &L.st.vsb[buf][0][NWG * dh][32 * kh] : &L.st.zero32[0]);
+          if (plain) sstep = sizeof(L.st.vsb[0][0][0]);
+          sfrom += 16 * c;
+        } else {
+          sfrom = reinterpret_cast<const char*>(plain ? &L.st.vp[buf][1][NWG * dh][32 * kh] : &L.st.zero[0]);
+          if (plain) sstep = sizeof(L.st.vp[0][0][0]);
+          sfrom += 8 * c;
+        }
+        u32x4 va[4];
+        s4 vs[2][2];
+        v_read(0, va);
+        s_read(sfrom, sstep, 0, vs[0]);
+        const uint32_t bm = plain ? ~0u : 0u;
+        const v8h ba = __builtin_bit_cast(v8h, u32x4{b0[0] & bm, b0[1] & bm, b1[0] & bm, b1[1] & bm});
+        __builtin_amdgcn_sched_barrier(0);
+        float pw[8];
+        // (with nothing attended so far, -inf - -inf would be NaN)
+        const float ms = m_ref == -INFINITY ? 0.0f : m_ref;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) pw[j] = fast_exp2(sc[j] - ms);
+        if constexpr (F32) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) l_run += pw[j];
+        }
+
+        // ---- O^T += V^T P^T ----------------------------------------------------
+        // B operands of eight weights
+        const auto split = [&](const float (&y)[8], v8h& bh, v8h& bl) {
+          u32x4 hw, lw;
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            hw[q] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(y[2 * q], y[2 * q + 1]));
+            lw[q] = pf_rem_pair(hw[q], y[2 * q], y[2 * q + 1]);
+          }
+          bh = __builtin_bit_cast(v8h, hw);
+          bl = __builtin_bit_cast(v8h, lw);
+        };
+        if (!plain) {
+          // V scales apart, or scales and biases out of range or not finite: the
+          // largest weight of every row and group to 2^13 .. 2^14 (an infinity, of
+          // exponent 0, stays one), the products on their own, added in fp32, and
+          // bias terms in fp32 -- without those of weight 0, whose keys the row may
+          // not attend at all
+          const auto times = [](float w, float x) { return w > 0.0f || w != w ? w * x : 0.0f; };
+          float add[4] = {0.0f, 0.0f, 0.0f, 0.0f}, lw = 0.0f;
+#pragma unroll 1
+          for (int g = 0; g < NWG; ++g) {
+            float y[8], big = 0.0f, sb = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              const int at = 32 * kh + 16 * (j >> 2) + 4 * c + (j & 3);
+              float s, b;
+              if constexpr (F32) {
+                s = L.st.vsb[buf][0][NWG * dh + g][at];
+                b = L.st.vsb[buf][1][NWG * dh + g][at];
+              } else {
+                s = static_cast<float>(L.st.vp[buf][1][NWG * dh + g][at]);
+                b = static_cast<float>(L.st.vp[buf][0][NWG * dh + g][at]);
+              }
+              y[j] = times(pw[j], s);
+              sb += times(pw[j], fmaf(s, 8.0f, b));
+              big = fmaxf(big, fabsf(y[j]));
+            }
+            sb = xor32_sum(xor16_sum(sb)) * bup;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) add[i] = i == g ? sb : add[i];
+            const int k = min(14 - __builtin_amdgcn_frexp_expf(xor32_max(xor16_max(big))), 120);
+            const float un = ldexpf(1.0f, -k);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) y[j] = ldexpf(y[j], k);
+            v8h bh, bl;
+            split(y, bh, bl);
+#pragma unroll
+            for (int gg = 0; gg < NWG; ++gg) {
+              if (gg != g) continue;
+#pragma unroll
+              for (int x = 0; x < 4; ++x) {
+                const v8h a = __builtin_bit_cast(v8h, vu[(4 * gg + x) * 64 + (m ^ Gm::vswz(gg))]);
+                v4f t = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, bh, z, 0, 0, 0);
+                t = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, bl, t, 0, 0, 0);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) o[4 * gg + x][i] = fmaf(t[i], un, o[4 * gg + x][i]);
+              }
+            }
+          }
+#pragma unroll
+          for (int j = 0; j < 8; ++j) lw += pw[j];
+          lw = xor32_sum(xor16_sum(lw)) * bup;
+          // into the rows that hold biases and, for fp16 caches, the weights' sum
+#pragma unroll
+          for (int i = 0; i < 4; ++i) ob[i] += c == 0 ? add[i] : 0.0f;
+          if (!F32 && c == 2) ob[0] += lw;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) pw[j] = 0.0f;
+        }
+        {
           v8h bh, bl;
+          float y[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) y[j] = pw[j] * pscale;
+          split(y, bh, bl);
+          ob = __builtin_amdgcn_mfma_f32_16x16x32_f16(ba, bh, ob, 0, 0, 0);
+          ob = __builtin_amdgcn_mfma_f32_16x16x32_f16(ba, bl, ob, 0, 0, 0);
+        }
+#pragma unroll
+        for (int g = 0; g < NWG; ++g) {
+          if (g + 1 < NWG) s_read(sfrom, sstep, g + 1, vs[(g + 1) & 1]);
+          __builtin_amdgcn_sched_barrier(0);
+          v8h bh, bl;
+          float y[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) y[j] = fmaf(static_cast<float>(vs[g & 1][j >> 2][j & 3]), pw[j], 0.0f);
           split(y, bh, bl);
 #pragma unroll
-          for (int gg = 0; gg < NWG; ++gg) {
-            if (gg != g) continue;
-#pragma unroll
-            for (int x = 0; x < 4; ++x) {
-              const v8h a = __builtin_bit_cast(v8h, vu[(4 * gg + x) * 64 + (m ^ Gm::vswz(gg))]);
-              v4f t = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, bh, z, 0, 0, 0);
-              t = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, bl, t, 0, 0, 0);
-#pragma unroll
-              for (int i = 0; i < 4; ++i) o[4 * gg + x][i] = fmaf(t[i], un, o[4 * gg + x][i]);
-            }
+          for (int x = 0; x < 4; ++x) {
+            const v8h a = __builtin_bit_cast(v8h, va[x]);
+            v4f& acc = o[4 * g + x];
+            acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, bh, acc, 0, 0, 0);
+            acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, bl, acc, 0, 0, 0);
           }
+          __builtin_amdgcn_sched_barrier(0);
+          if (g + 1 < NWG) v_read(g + 1, va);  // under the next group's weights
         }
-#pragma unroll
-        for (int j = 0; j < 8; ++j) lw += pw[j];
-        lw = xor32_sum(xor16_sum(lw)) * bup;
-        // into the rows that hold biases and, for fp16 caches, the weights' sum
-#pragma unroll
-        for (int i = 0; i < 4; ++i) ob[i] += c == 0 ? add[i] : 0.0f;
-        if (!F32 && c == 2) ob[0] += lw;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) pw[j] = 0.0f;
-      }
-      {
-        v8h bh, bl;
-        float y[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) y[j] = pw[j] * pscale;
-        split(y, bh, bl);
-        ob = __builtin_amdgcn_mfma_f32_16x16x32_f16(ba, bh, ob, 0, 0, 0);
-        ob = __builtin_amdgcn_mfma_f32_16x16x32_f16(ba, bl, ob, 0, 0, 0);
-      }
-#pragma unroll
-      for (int g = 0; g < NWG; ++g) {
-        if (g + 1 < NWG) s_read(sfrom, sstep, g + 1, vs[(g + 1) & 1]);
-        __builtin_amdgcn_sched_barrier(0);
-        v8h bh, bl;
-        float y[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) y[j] = fmaf(static_cast<float>(vs[g & 1][j >> 2][j & 3]), pw[j], 0.0f);
-        split(y, bh, bl);
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          const v8h a = __builtin_bit_cast(v8h, va[x]);
-          v4f& acc = o[4 * g + x];
-          acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, bh, acc, 0, 0, 0);
-          acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, bl, acc, 0, 0, 0);
-        }
-        __builtin_amdgcn_sched_barrier(0);
-        if (g + 1 < NWG) v_read(g + 1, va);  // under the next group's weights
       }
     }
     if (it + 1 < it1) {
@@ -752,7 +766,7 @@ void paged_tiles_kernel(TileParams p) {
     __syncthreads();
   }
 
-  // ---- merge of the KH partials of every row, and the output ------------------
+  // ---- merge of the KW partials of every row, and the output ------------------
   const float un = c < 2 ? 1.0f : 0.0625f;  // odd nibbles (rows 8-15) were 16 times as large
   const float lt = F32 ? xor32_sum(xor16_sum(l_run)) : xor32_sum(xor16_sum(c == 2 ? ob[0] : 0.0f)) * bun;
   if (c == 0) {
@@ -778,13 +792,13 @@ void paged_tiles_kernel(TileParams p) {
     const int r = __builtin_amdgcn_readfirstlane(u / (D / 2)), d = 2 * (u % (D / 2));
     const int Ro = r0 + r;
     if (Ro >= total) break;
-    const int rm = r % 16, w0 = r / 16 + RS * KH * (d / Gm::OW);
+    const int rm = r % 16, w0 = r / 16 + RS * KW * (d / Gm::OW);
     float M = -INFINITY;
 #pragma unroll
-    for (int k = 0; k < KH; ++k) M = fmaxf(M, ml[w0 + RS * k][rm]);
+    for (int k = 0; k < KW; ++k) M = fmaxf(M, ml[w0 + RS * k][rm]);
     float l = 0.0f, x0 = 0.0f, x1 = 0.0f;
 #pragma unroll
-    for (int k = 0; k < KH; ++k) {
+    for (int k = 0; k < KW; ++k) {
       const int wv = w0 + RS * k;
       const float fk = merge_factor(ml[wv][rm], M);
       const float2 v = *reinterpret_cast<const float2*>(&L.o[wv][rm * Gm::OSTR + d % Gm::OW]);
@@ -828,61 +842,68 @@ __global__ __launch_bounds__(256) void merge_tiles_kernel(const float* ws_ml, co
   reinterpret_cast<v4f*>(out)[i] = r;
 }
 
-template <int D, bool F32>
+template <int D, bool F32, int RS>
 void launch_q(const TileParams& p, dim3 grid, hipStream_t s) {
-  if (p.q_dtype == TQ_F32) paged_tiles_kernel<D, F32, true><<<grid, 128 * kRs, 0, s>>>(p);
-  else paged_tiles_kernel<D, F32, false><<<grid, 128 * kRs, 0, s>>>(p);
+  if (p.q_dtype == TQ_F32) paged_tiles_kernel<D, F32, true, RS><<<grid, 128 * kRs, 0, s>>>(p);
+  else paged_tiles_kernel<D, F32, false, RS><<<grid, 128 * kRs, 0, s>>>(p);
 }
 
 template <bool F32>
-void launch_dim(const TileParams& p, int D, dim3 grid, hipStream_t s) {
-  if (D == 128) launch_q<128, F32>(p, grid, s);
-  else if (D == 256) launch_q<256, F32>(p, grid, s);
-  else launch_q<512, F32>(p, grid, s);
+void launch_dim(const TileParams& p, int D, int rs, dim3 grid, hipStream_t s) {
+  if (D == 512) launch_q<512, F32, 4>(p, grid, s);
+  else if (D == 256) rs == 8 ? launch_q<256, F32, 8>(p, grid, s) : launch_q<256, F32, 4>(p, grid, s);
+  else rs == 8 ? launch_q<128, F32, 8>(p, grid, s) : launch_q<128, F32, 4>(p, grid, s);
+}
+
+int tile_keys(int D) { return D == 512 ? 32 : 64; }
+int64_t tile_wgs(int64_t rows, int Hkv, int rs) { return (rows + 16 * rs - 1) / (16 * rs) * Hkv; }
+
+// Splits of a grid of wgs workgroups that could be of use.
+int most_splits(int64_t wgs, int64_t tiles) {
+  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({64, tiles / 2, (target_wgs() + wgs - 1) / wgs})));
 }
 
 }  // namespace
 
 int paged_tiles_max_splits(int64_t rows, int Hkv, int D, int64_t keys) {
-  const int TK = D == 512 ? 32 : 64;
-  const int64_t wgs = (rows + kRows - 1) / kRows * Hkv, tiles = (keys + TK - 1) / TK;
-  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({64, tiles / 2, (target_wgs() + wgs - 1) / wgs})));
+  return most_splits(tile_wgs(rows, Hkv, D == 512 ? 4 : 8), (keys + tile_keys(D) - 1) / tile_keys(D));
 }
 
-int paged_tiles_splits(int64_t rows, int Hkv, int D, int64_t keys) {
-  const int TK = D == 512 ? 32 : 64;
-  const int64_t wgs = (rows + kRows - 1) / kRows * Hkv, tiles = (keys + TK - 1) / TK;
-  const int64_t cus = target_wgs();
-  // A workgroup fills a CU, and costs its prologue, epilogue and part of the
-  // merge beside its tiles, about kFixed of them: the split of least estimated
-  // time.
-  constexpr int64_t kFixed = 6;
-  int best = 1;
+TilesPlan plan_paged_tiles(int64_t rows, int Hkv, int D, int64_t keys) {
+  const int64_t tiles = (keys + tile_keys(D) - 1) / tile_keys(D), cus = target_wgs();
+  // A workgroup fills a CU, and costs its prologue, epilogue and part of the merge
+  // beside its tiles, about kFixed of them; a tile of 128 rows costs kTile8 eighths
+  // of one of 64: the plan of least estimated time.
+  constexpr int64_t kFixed = 6, kTile8 = 12;
+  TilesPlan best{4, 1};
   int64_t least = INT64_MAX;
-  for (int s = 1; s <= paged_tiles_max_splits(rows, Hkv, D, keys); ++s) {
-    const int64_t cost = (wgs * s + cus - 1) / cus * ((tiles + s - 1) / s + kFixed);
-    if (cost < least) {
-      least = cost;
-      best = s;
+  for (int rs = 4; rs <= (D == 512 ? 4 : 8); rs += 4) {
+    const int64_t wgs = tile_wgs(rows, Hkv, rs);
+    for (int s = 1; s <= most_splits(wgs, tiles); ++s) {
+      const int64_t cost = (wgs * s + cus - 1) / cus * ((tiles + s - 1) / s * (rs == 8 ? kTile8 : 8) + 8 * kFixed);
+      if (cost < least) {
+        least = cost;
+        best = {rs, s};
+      }
     }
   }
   return best;
 }
 
-int launch_paged_tiles(const PagedParams& p0, int D, int sb_dtype, int splits, bool partials, hipStream_t s) {
+int launch_paged_tiles(const PagedParams& p0, int D, int sb_dtype, TilesPlan plan, bool partials, hipStream_t s) {
   TileParams p;
   static_cast<PagedParams&>(p) = p0;
-  p.splits = splits;
-  p.ext_merge = partials || splits > 1;
+  p.splits = plan.splits;
+  p.ext_merge = partials || plan.splits > 1;
   const int64_t rows = static_cast<int64_t>(p.nq) * p.gqa;
-  const dim3 grid(static_cast<unsigned>((rows + kRows - 1) / kRows * p.Hkv), splits);
-  if (sb_dtype == TQ_F32) launch_dim<true>(p, D, grid, s);
-  else launch_dim<false>(p, D, grid, s);
+  const dim3 grid(static_cast<unsigned>(tile_wgs(rows, p.Hkv, plan.rs)), plan.splits);
+  if (sb_dtype == TQ_F32) launch_dim<true>(p, D, plan.rs, grid, s);
+  else launch_dim<false>(p, D, plan.rs, grid, s);
   TQ_CHECK_LAUNCH("paged_tiles_kernel");
-  if (partials || splits == 1) return TQ_OK;
+  if (partials || plan.splits == 1) return TQ_OK;
   const int64_t out_rows = static_cast<int64_t>(p.nq) * p.Hq;
   merge_tiles_kernel<<<static_cast<unsigned>((out_rows * (D / 4) + 255) / 256), 256, 0, s>>>(
-      p.ws_ml, p.ws_o, p.out, out_rows, splits, p.max_splits, D / 4);
+      p.ws_ml, p.ws_o, p.out, out_rows, plan.splits, p.max_splits, D / 4);
   TQ_CHECK_LAUNCH("merge_tiles_kernel");
   return TQ_OK;
 }

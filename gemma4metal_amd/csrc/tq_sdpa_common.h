@@ -850,12 +850,16 @@ int launch_prefill_tiles(const SdpaParams& p, int D, int sb_dtype, hipStream_t s
 // The same for fp32 queries, 64 rows (tq_prefill_f32.hip).
 int launch_prefill_tiles_f32(const SdpaParams& p, int D, int sb_dtype, hipStream_t stream);
 // Rows of a paged sequence (prefill) or of a batch's shared prefix on K/V tiles
-// (tq_paged_tiles.hip): the workgroups that share a row's tiles, at most and by
-// plan, and the launch; `partials`: leave (m, l, O) in slots 0 .. splits - 1 of
-// the rows' partials, else write the output.
+// (tq_paged_tiles.hip): the most workgroups that share a row's tiles, the plan, and
+// the launch; `partials`: leave (m, l, O) in slots 0 .. splits - 1 of the rows'
+// partials, else write the output.
 int paged_tiles_max_splits(int64_t rows, int Hkv, int D, int64_t keys);
-int paged_tiles_splits(int64_t rows, int Hkv, int D, int64_t keys);
-int launch_paged_tiles(const PagedParams& p, int D, int sb_dtype, int splits, bool partials, hipStream_t stream);
+struct TilesPlan {
+  int rs;      // 16-row sets of a workgroup
+  int splits;  // workgroups along the tiles
+};
+TilesPlan plan_paged_tiles(int64_t rows, int Hkv, int D, int64_t keys);
+int launch_paged_tiles(const PagedParams& p, int D, int sb_dtype, TilesPlan plan, bool partials, hipStream_t stream);
 // Merge of the split partials of a launch with ext_merge = 1 (batch b of
 // grid.y): tq_sdpa_hc.hip.
 int launch_merge_splits(const SdpaParams& p, int D, int batch, hipStream_t stream);
