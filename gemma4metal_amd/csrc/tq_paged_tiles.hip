@@ -22,11 +22,11 @@ namespace {
 
 constexpr int kRs = 4;  // 16-row sets of a tile's geometry (PfGeom): 8 waves
 
-template <int KH>
-struct PgTile {
-  int key;           // its first key
-  int64_t row[KH];   // first pool row of each 32-row part
-  bool has[KH];      // whether that part's page exists
+// Pool rows at which the 32-row parts of a run of tiles begin: part h of the run's
+// tile i in lane KH i + h, and whether its page exists in that bit of has.
+struct PgRun {
+  int lo, hi;
+  uint64_t has;
 };
 
 // Largest of 64 lanes, by the steps of wave_max_dpp (wave_max_i goes through the
@@ -75,8 +75,13 @@ __device__ __forceinline__ PgSource<Gm> pg_source(const PagedParams& p) {
 // A tile's words and scales into registers.  No load is conditional (the wait for
 // one would drain all of them).
 template <class Gm>
-__device__ __forceinline__ void pg_load(PfRaw<Gm>& R, const PgSource<Gm>& from, const PgTile<Gm::KH>& t) {
+__device__ __forceinline__ void pg_load(PfRaw<Gm>& R, const PgSource<Gm>& from, const PgRun& run, int i0) {
   constexpr int KH = Gm::KH;
+  // (i0: lane of the tile's first part)
+  const auto base_of = [&](int part) {
+    return static_cast<int64_t>(static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(run.hi, i0 + part))) << 32 |
+                                static_cast<uint32_t>(__builtin_amdgcn_readlane(run.lo, i0 + part)));
+  };
   // the part of a tile row; the same for a wave's 64 units where those span at
   // most one part
   const auto part = [](int r) { return KH == 1 ? 0 : __builtin_amdgcn_readfirstlane(r >> 5); };
@@ -87,7 +92,7 @@ __device__ __forceinline__ void pg_load(PfRaw<Gm>& R, const PgSource<Gm>& from, 
     const int u = e % Gm::UNITS;
     if (role == 0) {
       const int r = u / Gm::NG;
-      const int64_t base = KH == 2 && part(r) ? t.row[KH - 1] : t.row[0];
+      const int64_t base = base_of(part(r));
       const uint32_t off = (r & 31) * (4 * Gm::W) + 32 * (u % Gm::NG);
       const auto src = pg_rsrc(from.w[i] + base * (4 * Gm::W));
       const u32x4 a = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(src, off, 0, 0));
@@ -99,7 +104,7 @@ __device__ __forceinline__ void pg_load(PfRaw<Gm>& R, const PgSource<Gm>& from, 
       }
     } else {  // (threads past the units load one again and do not store it)
       const int w = u % Gm::W, kc = u / Gm::W;  // kc = 4 part + c
-      const int64_t base = KH == 2 && part(8 * kc) ? t.row[KH - 1] : t.row[0];
+      const int64_t base = base_of(part(8 * kc));
       const uint32_t off = 4 * (kc & 3) * (4 * Gm::W) + 4 * w;
       const auto src = pg_rsrc(from.w[i] + base * (4 * Gm::W));
 #pragma unroll
@@ -116,10 +121,10 @@ __device__ __forceinline__ void pg_load(PfRaw<Gm>& R, const PgSource<Gm>& from, 
     const int r = d / DPR;
     const uint32_t off = (r & 31) * (4 * DPR) + 4 * (d % DPR);
     if constexpr (KH == 2 && DPR == 1) {  // a wave spans both parts
-      const int64_t base = r >= 32 ? t.row[KH - 1] : t.row[0];
+      const int64_t base = r >= 32 ? base_of(KH - 1) : base_of(0);
       R.s[i] = *reinterpret_cast<const uint32_t*>(from.s[i] + base * (4 * DPR) + off);
     } else {
-      const int64_t base = KH == 2 && part(r) ? t.row[KH - 1] : t.row[0];
+      const int64_t base = base_of(part(r));
       R.s[i] = __builtin_amdgcn_raw_buffer_load_b32(pg_rsrc(from.s[i] + base * (4 * DPR)), off, 0, 0);
     }
   }
@@ -128,15 +133,13 @@ __device__ __forceinline__ void pg_load(PfRaw<Gm>& R, const PgSource<Gm>& from, 
 // Zeroes the scales and biases of rows past every limit and of missing pages,
 // which may hold anything.
 template <class Gm>
-__device__ __forceinline__ void pg_mask(PfRaw<Gm>& R, const PgTile<Gm::KH>& t, int hi) {
-  constexpr int KH = Gm::KH;
-  if (t.key <= hi - Gm::TK && t.has[0] && t.has[KH - 1]) return;  // uniform, most tiles
+__device__ __forceinline__ void pg_mask(PfRaw<Gm>& R, int key, int has, int hi) {
+  if (key <= hi - Gm::TK && has == (1 << Gm::KH) - 1) return;  // uniform, most tiles
 #pragma unroll
   for (int i = 0; i < Gm::NSD; ++i) {
     constexpr int DPR = Gm::SDW / Gm::TK;
     const int r = (threadIdx.x + i * Gm::NT) % Gm::SDW / DPR;
-    const bool has = KH == 2 && r >= 32 ? t.has[KH - 1] : t.has[0];
-    R.s[i] = has && t.key + r < hi ? R.s[i] : 0u;
+    R.s[i] = (has >> (r >> 5) & 1) && key + r < hi ? R.s[i] : 0u;
   }
 }
 
@@ -290,32 +293,29 @@ void paged_tiles_kernel(TileParams p) {
   const int nt = end - skip;
   const int per = (nt + p.splits - 1) / p.splits;
   const int it0 = min(static_cast<int>(blockIdx.y) * per, nt), it1 = min(it0 + per, nt);
-  int pages = -1;  // lane i: page of part i % KH of tile it + i / KH
-  const auto load_pages = [&](int it) {
-    if (nt > 0) {
-      const int v = min(it + lane / KH, nt - 1);
-      const int key = TK * (v + (v < ns ? 0 : skip)) + 32 * (lane % KH);
-      pages = p.tables[min(key >> p.page_shift, p.max_pages - 1)];
-    }
+  PgRun run;
+  const auto load_run = [&](int it) {  // of tiles it ...
+    const int v = min(it + lane / KH, nt - 1);
+    const int key = max(TK * (v + (v < ns ? 0 : skip)) + 32 * (lane % KH), 0);
+    const int e = nt > 0 ? p.tables[min(key >> p.page_shift, p.max_pages - 1)] : -1;
+    const bool has = static_cast<unsigned>(e) < static_cast<unsigned>(p.num_pages);
+    const int64_t row = ((static_cast<int64_t>(has ? e : 0) * p.Hkv + kvh) << p.page_shift) + (key & ((1 << p.page_shift) - 1));
+    run.lo = static_cast<int>(row);
+    run.hi = static_cast<int>(row >> 32);
+    run.has = __ballot(has);
   };
-  const auto tile_at = [&](int it) {
+  // Tile it: its lane in the run, first key, and bits of the parts that exist.
+  const auto tile_at = [&](int it, int& key, int& has) {
     const int i = (it - it0) & (64 / KH - 1);
     if (it != it0 && i == 0) {  // waited for in here: the steady loop waits for nothing
-      load_pages(it);
-      asm volatile("" : "+v"(pages));
+      load_run(it);
+      asm volatile("" : "+v"(run.lo), "+v"(run.hi));
     }
-    PgTile<KH> t;
-    t.key = TK * (it + (it < ns ? 0 : skip));
-#pragma unroll
-    for (int h = 0; h < KH; ++h) {
-      const int e = __builtin_amdgcn_readlane(pages, i * KH + h);
-      t.has[h] = static_cast<unsigned>(e) < static_cast<unsigned>(p.num_pages);
-      t.row[h] = ((static_cast<int64_t>(t.has[h] ? e : 0) * p.Hkv + kvh) << p.page_shift) +
-                 ((t.key + 32 * h) & ((1 << p.page_shift) - 1));
-    }
-    return t;
+    key = TK * (it + (it < ns ? 0 : skip));
+    has = static_cast<int>(run.has >> (i * KH)) & ((1 << KH) - 1);
+    return i * KH;
   };
-  load_pages(it0);
+  load_run(it0);
 
   const int rw = r0 + 16 * rs;              // the wave's first row
   const int R = min(rw + m, total - 1);     // this lane's row (column m)
@@ -326,10 +326,11 @@ void paged_tiles_kernel(TileParams p) {
   const int hi_max = max_of_wave(hi), hi_min = min_of_wave(hi);
   const int lo_max = max_of_wave(lo), lo_min = min_of_wave(lo);
 
-  PgTile<KH> cur = tile_at(it0), nxt = cur;
+  int key, has;  // of the tile in LDS
+  const int i0 = tile_at(it0, key, has);
   const PgSource<Gm> from = pg_source<Gm>(p);
   PfRaw<Gm> raw;
-  pg_load<Gm>(raw, from, cur);
+  pg_load<Gm>(raw, from, run, i0);
 
   // ---- q: B operands of k-step s of group g are dims 64 g + 16 c + 8 s + {0, 4,
   // 1, 5, 2, 6, 3, 7}, times 2^(15 - ex) (the row's largest below 2^15), the odd
@@ -424,7 +425,7 @@ void paged_tiles_kernel(TileParams p) {
   }
   if (F32 && threadIdx.x < Gm::TK) L.st.zero32[threadIdx.x] = 0.0f;
   __syncthreads();
-  pg_mask<Gm>(raw, cur, hi_w);
+  pg_mask<Gm>(raw, key, has, hi_w);
   const float wm = pf_vmax<Gm>(raw);
   if (lane == 0) atomicMax(&vmx, __float_as_uint(wm));
   __syncthreads();
@@ -464,16 +465,16 @@ void paged_tiles_kernel(TileParams p) {
 #pragma unroll 1
   for (int it = it0; it < it1; ++it) {
     const int buf = (it - it0) & 1;
+    int nkey = key, nhas = has;
     if (it + 1 < it1) {
-      nxt = tile_at(it + 1);
-      pg_load<Gm>(raw, from, nxt);
+      const int i = tile_at(it + 1, nkey, nhas);
+      pg_load<Gm>(raw, from, run, i);
     }
 #pragma unroll 1
     for (int part = 0; part < HB; ++part) {
       const int kh = KW == 1 ? part : kw;
-      const int t0 = cur.key + 32 * kh;  // this wave's keys t0 .. t0 + 31
-      const bool has = KH == 2 && kh ? cur.has[KH - 1] : cur.has[0];
-      const bool any = has && rw < total && t0 < hi_max && (t0 + 31 >= lo_min || t0 < p.sinks);  // wave-uniform
+      const int t0 = key + 32 * kh;  // this wave's keys t0 .. t0 + 31
+      const bool any = (has >> kh & 1) && rw < total && t0 < hi_max && (t0 + 31 >= lo_min || t0 < p.sinks);  // wave-uniform
       // this wave's groups
       const u32x4* ku = L.st.k[buf] + 2 * kh * Gm::KU + 128 * NWG * dh + 16 * c;
       const u32x4* vu = L.st.v[buf] + kh * Gm::VU + 256 * NWG * dh + 16 * c;
@@ -565,21 +566,26 @@ void paged_tiles_kernel(TileParams p) {
             else if (h == 0) k_read(1, 0);
           }
           if (F32 && h == 1) sb_read(1);
+          // (four sums side by side: one after the other, each step waits for the last)
+          float s[4];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            float s = bt[i] * 512.0f;
+          for (int i = 0; i < 4; ++i) s[i] = bt[i] * 512.0f;
 #pragma unroll
-            for (int g = 0; g < NWG; ++g) {
+          for (int g = 0; g < NWG; ++g) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
               if constexpr (F32) {
                 // s (. + 8 sum q) + b sum q
-                s = fmaf(bk[i][g], qs[g] * 512.0f, s);
-                s = fmaf(sk[h % HA][i][g], fmaf(qs[g], 4096.0f, acc[g][i]), s);
+                s[i] = fmaf(bk[i][g], qs[g] * 512.0f, s[i]);
+                s[i] = fmaf(sk[h % HA][i][g], fmaf(qs[g], 4096.0f, acc[g][i]), s[i]);
               } else {
-                s = fmaf(static_cast<float>(sk[h % HA][i][g]), acc[g][i], s);
+                s[i] = fmaf(static_cast<float>(sk[h % HA][i][g]), acc[g][i], s[i]);
               }
             }
-            sc[4 * h + i] = s * rf;
+            __builtin_amdgcn_sched_barrier(0);
           }
+#pragma unroll
+          for (int i = 0; i < 4; ++i) sc[4 * h + i] = s[i] * rf;
         }
       }
       if constexpr (DH == 2) {
@@ -759,10 +765,11 @@ void paged_tiles_kernel(TileParams p) {
       }
     }
     if (it + 1 < it1) {
-      pg_mask<Gm>(raw, nxt, hi_w);
+      pg_mask<Gm>(raw, nkey, nhas, hi_w);
       stage(buf ^ 1);
     }
-    cur = nxt;
+    key = nkey;
+    has = nhas;
     __syncthreads();
   }
 
