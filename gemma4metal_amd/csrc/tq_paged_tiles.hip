@@ -78,10 +78,12 @@ template <class Gm>
 __device__ __forceinline__ void pg_load(PfRaw<Gm>& R, const PgSource<Gm>& from, const PgRun& run, int i0) {
   constexpr int KH = Gm::KH;
   // (i0: lane of the tile's first part)
-  const auto base_of = [&](int part) {
-    return static_cast<int64_t>(static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(run.hi, i0 + part))) << 32 |
-                                static_cast<uint32_t>(__builtin_amdgcn_readlane(run.lo, i0 + part)));
+  const auto lane_row = [&](int i) {
+    return static_cast<int64_t>(static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(run.hi, i))) << 32 |
+                                static_cast<uint32_t>(__builtin_amdgcn_readlane(run.lo, i)));
   };
+  const int64_t only = KH == 1 ? lane_row(i0) : 0;  // (once, not on every branch)
+  const auto base_of = [&](int part) { return KH == 1 ? only : lane_row(i0 + part); };
   // the part of a tile row; the same for a wave's 64 units where those span at
   // most one part
   const auto part = [](int r) { return KH == 1 ? 0 : __builtin_amdgcn_readfirstlane(r >> 5); };
