@@ -309,7 +309,11 @@ __device__ __forceinline__ int paged_chunk(const PagedParams& p, int len, int H)
     return max(j, 1);
   };
   const auto cost = [&](float jobs, int cand) {
-    return jobs > room ? INFINITY : fmaxf(fixed + static_cast<float>(cand), (fixed * jobs * H + keys) / slots);
+    // (jobs past the slots start when the shortest others end: half a fixed cost
+    // more than an even share.  8 sequences of 1,024 to 28,137 keys, 4 kv heads:
+    // 268 jobs of 1,792 keys on 256 CUs 77.7 us, 252 of 1,920 keys 63.6)
+    const float late = jobs * H > slots ? 0.5f * fixed : 0.0f;
+    return jobs > room ? INFINITY : fmaxf(fixed + static_cast<float>(cand), (fixed * jobs * H + keys) / slots + late);
   };
   float best = INFINITY;
   int chunk = cand_of(1);
