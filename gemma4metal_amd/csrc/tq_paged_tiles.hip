@@ -17,6 +17,8 @@
 //   fp32 biases are applied in fp32.
 #include "tq_prefill_tile.h"
 
+#include <cfloat>
+
 namespace tq {
 namespace {
 
@@ -335,7 +337,8 @@ void paged_tiles_kernel(TileParams p) {
   pg_load<Gm>(raw, from, run, i0);
 
   // ---- q: B operands of k-step s of group g are dims 64 g + 16 c + 8 s + {0, 4,
-  // 1, 5, 2, 6, 3, 7}, times 2^(15 - ex) (the row's largest below 2^15), the odd
+  // 1, 5, 2, 6, 3, 7}, times 2^(6 - ex) (the row's largest below 2^6, so that group
+  // sums fit fp16; what is below fp16's 2^-24 is 2^-26 of it and less), the odd
   // ones over 16; fp32 queries in two fp16 parts.  The sign of a negative scale
   // goes into q.
   v8h qf[2 * NWG], ql[Q32 ? 2 * NWG : 1], qb;
@@ -373,7 +376,9 @@ void paged_tiles_kernel(TileParams p) {
   }
   mx = xor32_max(xor16_max(mx));
   const int ex = __builtin_amdgcn_frexp_expf(mx);
-  const float rf = ldexpf(fabsf(p.scale_log2), ex - 15);  // score = rf * products
+  // score = rf * products (of a scale of 0 not 0: -inf stays one)
+  const float rf0 = ldexpf(fabsf(p.scale_log2), ex - 6);
+  const float rf = rf0 < FLT_MIN ? FLT_MIN : rf0 > FLT_MAX ? FLT_MAX : rf0;
   const bool neg = p.scale_log2 < 0.0f;
   float qs[NWG];
 #pragma unroll
@@ -382,7 +387,7 @@ void paged_tiles_kernel(TileParams p) {
   for (int j = 0; j < 2 * NWG; ++j) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      float x = ldexpf(f[j][i], 15 - ex);
+      float x = ldexpf(f[j][i], 6 - ex);
       x = neg ? -x : x;
       qs[j >> 1] += x;
       const int slot = (i & 2) ? 4 + 2 * (i & 1) + (i >> 2) : 2 * (i & 1) + (i >> 2);
@@ -399,11 +404,11 @@ void paged_tiles_kernel(TileParams p) {
       }
     }
   }
-  // group sums over 512 (|.| < 2^12).  fp16 scale/bias: part c of three fp16
+  // group sums (|.| < 2^12).  fp16 scale/bias: part c of three fp16
   // parts in lane group c for the biases, 8 times it for the scales; fp32: kept
   // in fp32.
 #pragma unroll
-  for (int g = 0; g < NWG; ++g) qs[g] = xor32_sum(xor16_sum(qs[g])) * 0x1p-9f;
+  for (int g = 0; g < NWG; ++g) qs[g] = xor32_sum(xor16_sum(qs[g]));
 #pragma unroll
   for (int g = 0; g < 4; ++g) {
     _Float16 pt = static_cast<_Float16>(0.0f);
@@ -571,15 +576,15 @@ void paged_tiles_kernel(TileParams p) {
           // (four sums side by side: one after the other, each step waits for the last)
           float s[4];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) s[i] = bt[i] * 512.0f;
+          for (int i = 0; i < 4; ++i) s[i] = bt[i];
 #pragma unroll
           for (int g = 0; g < NWG; ++g) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
               if constexpr (F32) {
                 // s (. + 8 sum q) + b sum q
-                s[i] = fmaf(bk[i][g], qs[g] * 512.0f, s[i]);
-                s[i] = fmaf(sk[h % HA][i][g], fmaf(qs[g], 4096.0f, acc[g][i]), s[i]);
+                s[i] = fmaf(bk[i][g], qs[g], s[i]);
+                s[i] = fmaf(sk[h % HA][i][g], fmaf(qs[g], 8.0f, acc[g][i]), s[i]);
               } else {
                 s[i] = fmaf(static_cast<float>(sk[h % HA][i][g]), acc[g][i], s[i]);
               }
@@ -587,7 +592,7 @@ void paged_tiles_kernel(TileParams p) {
             __builtin_amdgcn_sched_barrier(0);
           }
 #pragma unroll
-          for (int i = 0; i < 4; ++i) sc[4 * h + i] = s[i] * rf;
+          for (int i = 0; i < 4; ++i) sc[4 * h + i] = DH == 2 ? s[i] * rf : s[i];  // (a wave's dims have an rf of their own)
         }
       }
       if constexpr (DH == 2) {
@@ -624,7 +629,7 @@ void paged_tiles_kernel(TileParams p) {
         float mt = sc[0];
 #pragma unroll
         for (int j = 1; j < 8; ++j) mt = fmaxf(mt, sc[j]);
-        const float need = xor32_max(xor16_max(mt)) + up;
+        const float need = fmaf(xor32_max(xor16_max(mt)), DH == 2 ? 1.0f : rf, up);
         // (a row with nothing attended yet and nothing here keeps -inf)
         if (__any(need > m_ref + kPfLazy)) {
           const float m_new = need > m_ref ? need : m_ref;
@@ -660,7 +665,7 @@ void paged_tiles_kernel(TileParams p) {
         // (with nothing attended so far, -inf - -inf would be NaN)
         const float ms = m_ref == -INFINITY ? 0.0f : m_ref;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) pw[j] = fast_exp2(sc[j] - ms);
+        for (int j = 0; j < 8; ++j) pw[j] = fast_exp2(DH == 2 ? sc[j] - ms : fmaf(sc[j], rf, -ms));
         if constexpr (F32) {
 #pragma unroll
           for (int j = 0; j < 8; ++j) l_run += pw[j];
