@@ -305,6 +305,60 @@ def test_prompt_long(pg, Hq, Hkv, D, page, prior, new, W, sinks):
     assert torch.equal(got, pg.sdpa_int4_paged_prefill(*args))
 
 
+def of_heads(pages, heads, gqa):
+    """The pages of the kv heads of some query heads, one each."""
+    return [x[:, [h // gqa for h in heads]] for x in pages]
+
+
+# More workgroups of 64 rows than compute units: workgroups of 128 rows are taken.
+MANY = [(66, 33, 256, 32), (33, 33, 256, 64), (66, 33, 128, 32)]
+
+
+@pytest.mark.parametrize("sb,qt", [("f16", "bf16"), ("f32", "f32"), ("f16", "f32"), ("f32", "f16")])
+@pytest.mark.parametrize("Hq,Hkv,D,page", MANY)
+@pytest.mark.parametrize("prior,window,sinks", [(0, 0, 0), (37, 70, 6), (130, 31, 100)])
+def test_prompt_of_many_heads(pg, Hq, Hkv, D, page, prior, window, sinks, sb, qt):
+    rng = np.random.default_rng(prior + Hq + D)
+    new = 301 if Hq > Hkv else 650
+    n = prior + new
+    N = -(-n // page)
+    table = random_tables(rng, [n], page, N, N + 1)
+    pages = make_pool(rng, N, Hkv, page, D, sb)
+    if window:  # keys that some rows do not attend: of one key each NaN, infinite
+        pages[4][table[0, 120 // page], :, 120 % page] = np.nan
+        pages[5][table[0, (n - 1) // page], :, (n - 1) % page] = np.inf
+        table[0, 5] = -1
+    spoil(pages, table, [n], page)
+    q, qf = queries(rng, (new, Hq, D), qt)
+    got = host(pg.sdpa_int4_paged_prefill(q, *map(dev, pages), dev(table[0]), prior, Hq // Hkv, 0.9, window, sinks))
+    heads = [0, 1, Hq // 2, Hq - 1]
+    with np.errstate(all="ignore"):
+        ref = OP.sdpa_int4_paged_prefill(qf[:, heads], of_heads(pages, heads, Hq // Hkv), table[0], prior, page, 1, 0.9,
+                                         window, sinks)
+    keep = np.isfinite(ref).all((1, 2))
+    assert keep.sum() >= (new // 2 if window else new)
+    close(got[:, heads][keep], ref[keep])
+
+
+@pytest.mark.parametrize("sb,qt", [("f16", "bf16"), ("f32", "f32")])
+@pytest.mark.parametrize("D", [128, 256])
+def test_shared_prefix_of_many_heads(pg, D, sb, qt):
+    rng = np.random.default_rng(D)
+    Hkv, Hq, page, B = 66, 132, 32, 130
+    P = 5 * page
+    lens = [P + int(x) for x in rng.integers(0, 2 * page, B)]
+    lens[7], lens[99] = P - page - 5, 0
+    N = P // page + sum(max(-(-n // page) - P // page, 0) for n in lens)
+    tables = random_tables(rng, lens, page, N, P // page + 2, P // page)
+    pages = make_pool(rng, N, Hkv, page, D, sb)
+    spoil(pages, tables, lens, page)
+    q, qf = queries(rng, (B, Hq, D), qt)
+    got = pg.sdpa_int4_paged(q, *map(dev, pages), dev(tables), ints(lens), 2, 0.9, 100, 3, shared_prefix=P)
+    heads = [0, 67, 131]
+    ref = OP.sdpa_int4_paged(qf[:, heads], of_heads(pages, heads, 2), tables, lens, page, 1, 0.9, 100, 3, shared_prefix=P)
+    close(host(got)[:, heads], ref)
+
+
 @pytest.mark.parametrize("scale", [0.0, -0.7])
 def test_scale_zero_and_negative(pg, scale):
     rng = np.random.default_rng(3)
