@@ -731,6 +731,8 @@ void sdpa_int4_hc2_kernel(ParamsOf<PG> p) {
     for (int P = 0; P < NG / 2; ++P) qh[P] = sh_qhat[hh][2 * P + (m >> 3)] * ldexpf(1.0f, sh_F[hh]);
 
     float m_run = -INFINITY, l_run = 0.0f;
+    // the mean nibble of a weight whole, as in sdpa_int4_mfma_kernel
+    constexpr bool kMean = PG && F32;
     float wsum[4], bacc[4];
 #pragma unroll
     for (int blk = 0; blk < 4; ++blk) wsum[blk] = bacc[blk] = 0.0f;
@@ -926,6 +928,10 @@ void sdpa_int4_hc2_kernel(ParamsOf<PG> p) {
           wsum[blk] = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(v2bf, lb), ones, wsum[blk], false);
           bacc[blk] = fmaf(pw[j], vb[j >> 2][j & 3], bacc[blk]);
           bacc[blk] = fmaf(pw[j + 1], vb[(j + 1) >> 2][(j + 1) & 3], bacc[blk]);
+          if constexpr (kMean) {
+            bacc[blk] = fmaf(7.5f, w0, bacc[blk]);
+            bacc[blk] = fmaf(7.5f, w1, bacc[blk]);
+          }
         }
         uint4* dst = pv_lds + (((slot * NS + s) * 4 + blk) * 2) * 64 + lane;
         dst[0] = uint4{bh[0], bh[1], bh[2], bh[3]};
@@ -950,7 +956,7 @@ void sdpa_int4_hc2_kernel(ParamsOf<PG> p) {
       wsum[blk] = xor32_sum(wsum[blk]);
       bacc[blk] = xor16_sum(bacc[blk]);
       bacc[blk] = xor32_sum(bacc[blk]);
-      if (c == 0) off_lds[s][blk][m] = bacc[blk] - 128.0f * wsum[blk];
+      if (c == 0) off_lds[s][blk][m] = bacc[blk] - (kMean ? 135.5f : 128.0f) * wsum[blk];
     }
     if (c == 0 && m < 8) {
       ml_lds[0][s][hh] = m_run;

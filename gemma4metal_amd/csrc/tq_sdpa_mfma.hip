@@ -509,6 +509,7 @@ void sdpa_int4_mfma_kernel(ParamsOf<PG> p) {
 
   // ---- main loop ----------------------------------------------------------
   float m_run = -INFINITY, l_run = 0.0f, wsum = 0.0f, bacc = 0.0f;
+  constexpr bool kMean = PG && F32;  // see the weights' parts below
   v4f cv[VM];
 #pragma unroll
   for (int f = 0; f < VM; ++f) cv[f] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
@@ -744,6 +745,11 @@ void sdpa_int4_mfma_kernel(ParamsOf<PG> p) {
     // weight sum of the 128 offset takes a word per v_dot2 with (1, 1).
     uint32_t bh[4], bl[4];
     const v2bf ones = __builtin_bit_cast(v2bf, 0x3F803F80u);
+    // 7.5, the mean nibble, of a weight whole: what its parts leave out (2^-18 of it)
+    // then only counts for nibbles' distances from that.  Paged fp32 scales: a
+    // weight of 1 is not exact in its parts, as it is with an fp16 scale (outputs off
+    // by 8e-6 of themselves without, 4e-6 with it).
+    const float mean = PACK && T ? 0.0f : 7.5f;
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       const int j = 2 * k;
@@ -755,6 +761,10 @@ void sdpa_int4_mfma_kernel(ParamsOf<PG> p) {
       const float h0 = __uint_as_float(hb << 16), h1 = __uint_as_float(hb & 0xFFFF0000u);
       const uint32_t lb =
           __builtin_bit_cast(uint32_t, v2bf{static_cast<__bf16>(w0 - h0), static_cast<__bf16>(w1 - h1)});
+      if constexpr (kMean) {
+        bacc = fmaf(mean, w0, bacc);
+        bacc = fmaf(mean, w1, bacc);
+      }
       if constexpr (PACK) {
         // column n + 8T takes part T of the weight
         bh[k] = T ? lb : hb;
@@ -870,7 +880,7 @@ void sdpa_int4_mfma_kernel(ParamsOf<PG> p) {
   }
   // packed: slot 2 * wave + T holds column n's part T (hi / lo)
   const int slot = PACK ? 2 * wave + T : wave;
-  const float corr = bacc - 128.0f * wsum;  // bias term and the 128 offset
+  const float corr = bacc - (kMean ? 135.5f : 128.0f) * wsum;  // bias term and the 128 offset
   if (col_used) {
     // Accumulator element (s, j) of C row 4c + i is dim 8 * (VW * (4c + i) +
     // s) + j: for one (c, i) the 8 * VW dims are contiguous and lie in one
