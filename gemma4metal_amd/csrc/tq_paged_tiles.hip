@@ -234,7 +234,12 @@ struct TileParams : PagedParams {
 };
 
 // RS: 16-row sets of a workgroup.  4: a wave takes 32 keys of a tile (of 64 keys, D
-// 512 of 32); 8 (D < 512): all 64, one half after the other.
+// 512 of 32); 8 (D < 512): all 64, one half after the other, so that twice as many
+// rows share the staging of a tile (64 sequences with 2 query heads a kv head over
+// 32,768 shared keys, D 256: 233 us with 4, 212 with 8, 199 with the steps after).
+// Two waves fill a SIMD (registers).  VALU takes 54% of its cycles and the matrix
+// cores 27% there, 49% and 23% at D 512 (2,048 queries after 6,144 keys: 2.75 ms, 350
+// TFLOP/s); a wave runs the two one after the other.
 template <int D, bool F32, bool Q32, int RS>
 __global__ __launch_bounds__(128 * kRs) __attribute__((amdgpu_waves_per_eu(2, 2)))
 void paged_tiles_kernel(TileParams p) {
@@ -887,8 +892,8 @@ TilesPlan plan_paged_tiles(int64_t rows, int Hkv, int D, int64_t keys) {
   const int64_t tiles = (keys + tile_keys(D) - 1) / tile_keys(D), cus = target_wgs();
   // A workgroup fills a CU, and costs its prologue, epilogue and part of the merge
   // beside its tiles, about kFixed of them; a tile of 128 rows costs kTile8 eighths
-  // of one of 64: the plan of least estimated time.
-  constexpr int64_t kFixed = 6, kTile8 = 12;
+  // of one of 64 (5.9 us and 3.3 at D 256): the plan of least estimated time.
+  constexpr int64_t kFixed = 6, kTile8 = 14;
   TilesPlan best{4, 1};
   int64_t least = INT64_MAX;
   for (int rs = 4; rs <= (D == 512 ? 4 : 8); rs += 4) {

@@ -12,6 +12,24 @@
 namespace tq {
 namespace {
 
+// Division of n < 2^31 by d: the high half of n m, shifted, with m = ceil(2^(31 + l) /
+// d), l = ceil(log2 d).  m d exceeds 2^(31 + l) by less than d <= 2^l, so that n m /
+// 2^(31 + l) exceeds n / d by less than 1 / d and rounds down as it does.
+struct FastDiv {
+  uint32_t d, m;
+  int shift;  // l - 1; -1: d = 1
+};
+
+FastDiv fast_div(uint32_t d) {
+  int l = 0;
+  while ((uint64_t{1} << l) < d) ++l;
+  return {d, l == 0 ? 0u : static_cast<uint32_t>(((uint64_t{1} << (31 + l)) + d - 1) / d), l - 1};
+}
+
+__device__ __forceinline__ uint32_t fast_div(uint32_t n, const FastDiv& f) {
+  return f.shift < 0 ? n : __umulhi(n, f.m) >> f.shift;
+}
+
 struct QuantJob {
   const void* x;
   uint32_t* wq;
@@ -34,6 +52,7 @@ struct QuantParams {
   // tables[b * max_pages + r / 2^page_shift] (cap = max_pages << page_shift)
   const int32_t* tables;
   int max_pages, num_pages, page_shift;
+  FastDiv by_row, by_new, by_heads;  // append: words of a row, n_new, heads
 };
 
 __device__ __forceinline__ void load8(const void* x, int dtype, int64_t off, float v[8]) {
@@ -61,7 +80,8 @@ __device__ __forceinline__ void load8(const void* x, int dtype, int64_t off, flo
 
 // What bounds it: HBM, once the VALU is out of the way -- eight correctly
 // rounded divisions a word and 64-bit index divisions made 65,536 rows of 256
-// fp32 values 19.0 us (4.0 TB/s).
+// fp32 values 19.0 us (4.0 TB/s).  PAGED: a row's page is looked up at its store; two
+// prompts of 2,048 rows, 16 heads of D 256 (bf16, K and V): 38 us (4.5 TB/s).
 template <typename SB, bool PAGED>
 __global__ __launch_bounds__(256) void quantize_int4_kernel(QuantParams p) {
   // every argument in one batch of scalar loads (one memory round trip),
@@ -112,25 +132,20 @@ __global__ __launch_bounds__(256) void quantize_int4_kernel(QuantParams p) {
   // where that is certain: x r is within 2^-22 of the quotient (one ulp of r,
   // half an ulp of the product) and the rounded quotient within 2^-24, so
   // 1e-5 and 2^-20 of the quotient away from a half-integer all round alike.
-  // A lane with a value closer to one (about 2 values in 10^5), a NaN or an
-  // infinity divides.
+  // A value closer to one (2 in 10^5 of fp32 values, but most waves have one of 16
+  // bits), a NaN or an infinity divides, each by itself.
   const float r = fabsf(scale) < 0x1p100f ? __builtin_amdgcn_rcpf(scale) : NAN;  // 1 / scale stays normal
   float q[8];
-  bool sure = true;
 #pragma unroll
   for (int k = 0; k < 8; ++k) {
     const float x = (v[k] - bias) * r;
     q[k] = __builtin_rintf(x);
-    sure &= fabsf(x - q[k]) < 0.5f - 1e-5f - fabsf(x) * 0x1p-20f;
-  }
-  if (!sure) {
-#pragma unroll
-    for (int k = 0; k < 8; ++k) q[k] = __builtin_rintf((v[k] - bias) / scale);
+    if (!(fabsf(x - q[k]) < 0.5f - 1e-5f - fabsf(x) * 0x1p-20f)) q[k] = __builtin_rintf((v[k] - bias) / scale);
   }
   uint32_t word = 0;
 #pragma unroll
   for (int k = 0; k < 8; ++k) {
-    const float n = q[k] < 0.0f ? 0.0f : (q[k] > n_bins ? n_bins : q[k]);
+    const float n = fminf(fmaxf(q[k], 0.0f), n_bins);  // a NaN: 0
     word |= static_cast<uint32_t>(n) << (4 * k);
   }
 
@@ -139,11 +154,11 @@ __global__ __launch_bounds__(256) void quantize_int4_kernel(QuantParams p) {
     // input row = ((b * heads + h) * n_new + t) -> cache row (b*heads+h)*cap + pos[b] + t
     const uint32_t wpr = static_cast<uint32_t>(p.dim) >> 3;  // words per row
     int64_t row, bh, b;
-    if (p.words <= 0xFFFFFFFFll) {  // uniform; 32-bit divisions
-      const uint32_t r = static_cast<uint32_t>(gid) / wpr, h = r / static_cast<uint32_t>(p.n_new);
+    if (p.words <= 0x7FFFFFFFll) {  // uniform
+      const uint32_t r = fast_div(static_cast<uint32_t>(gid), p.by_row), h = fast_div(r, p.by_new);
       row = r;
       bh = h;
-      b = h / static_cast<uint32_t>(p.heads);
+      b = fast_div(h, p.by_heads);
     } else {
       row = gid / wpr;
       bh = row / p.n_new;
@@ -208,8 +223,13 @@ int check_align(const void* p, size_t a, const char* what) {
   return TQ_OK;
 }
 
-int launch_quantize(const QuantParams& p, int jobs, int sb_dtype, hipStream_t stream) {
+int launch_quantize(QuantParams p, int jobs, int sb_dtype, hipStream_t stream) {
   if (p.words == 0) return TQ_OK;
+  if (p.pos != nullptr) {
+    p.by_row = fast_div(static_cast<uint32_t>(p.dim) >> 3);
+    p.by_new = fast_div(static_cast<uint32_t>(p.n_new));
+    p.by_heads = fast_div(static_cast<uint32_t>(p.heads));
+  }
   const int64_t blocks = (p.words + 255) / 256;
   if (blocks > 0x7FFFFFFF) {
     set_error("quantize: too many rows");
