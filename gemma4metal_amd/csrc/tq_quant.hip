@@ -9,6 +9,8 @@
 // quantize(x, 64, 4) (engine/gemma4_multilayer.cpp:228-229).
 #include "tq_internal.h"
 
+#include <type_traits>
+
 namespace tq {
 namespace {
 
@@ -55,15 +57,22 @@ struct QuantParams {
   FastDiv by_row, by_new, by_heads;  // append: words of a row, n_new, heads
 };
 
-__device__ __forceinline__ void load8(const void* x, int dtype, int64_t off, float v[8]) {
+__device__ __forceinline__ void load8(const void* x, int dtype, int64_t off, uint4 (&u)[2]) {
   if (dtype == TQ_F32) {
-    const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(x) + off);
-    float4 a = p[0], b = p[1];
-    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-    v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+    const uint4* p = reinterpret_cast<const uint4*>(static_cast<const float*>(x) + off);
+    u[0] = p[0];
+    u[1] = p[1];
   } else {
-    const uint4 u = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(x) + off);
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+    u[0] = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(x) + off);
+  }
+}
+
+__device__ __forceinline__ void floats8(const uint4 (&u)[2], int dtype, float v[8]) {
+  const uint32_t w[8] = {u[0].x, u[0].y, u[0].z, u[0].w, u[1].x, u[1].y, u[1].z, u[1].w};
+  if (dtype == TQ_F32) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(w[i]);
+  } else {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const uint16_t lo = w[i] & 0xFFFFu, hi = w[i] >> 16;
@@ -78,10 +87,23 @@ __device__ __forceinline__ void load8(const void* x, int dtype, int64_t off, flo
   }
 }
 
+// Of the 8 lanes of a group.
+template <class F>
+__device__ __forceinline__ float of_group(float x, F f) {
+  const auto other = [](float y, auto ctl) {
+    return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(y), decltype(ctl)::value, 0xF, 0xF, false));
+  };
+  x = f(x, other(x, std::integral_constant<int, 0xB1>{}));     // lane ^ 1
+  x = f(x, other(x, std::integral_constant<int, 0x4E>{}));     // lane ^ 2
+  return f(x, other(x, std::integral_constant<int, 0x141>{})); // the other four lanes (mirrored)
+}
+
 // What bounds it: HBM, once the VALU is out of the way -- eight correctly
 // rounded divisions a word and 64-bit index divisions made 65,536 rows of 256
-// fp32 values 19.0 us (4.0 TB/s).  PAGED: a row's page is looked up at its store; two
-// prompts of 2,048 rows, 16 heads of D 256 (bf16, K and V): 38 us (4.5 TB/s).
+// fp32 values 19.0 us (4.0 TB/s); 13.1 us now.  16-bit inputs, half the bytes a value,
+// are still bound by VALU and the chain of a wave's loads: two prompts of 2,048 rows,
+// 16 heads of D 256 (bf16, K and V) append in 23.8 us (3.6 TB/s), into pages (PAGED:
+// one more dependent load, the page) in 27 us.
 template <typename SB, bool PAGED>
 __global__ __launch_bounds__(256) void quantize_int4_kernel(QuantParams p) {
   // every argument in one batch of scalar loads (one memory round trip),
@@ -95,20 +117,56 @@ __global__ __launch_bounds__(256) void quantize_int4_kernel(QuantParams p) {
   const int64_t gid = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;  // word of the input
   if (gid >= p.words) return;  // whole 8-lane groups leave together (words % 8 == 0)
 
-  float v[8];
-  load8(J.x, p.x_dtype, gid * 8, v);
+  // (the place is looked up while the values are on their way)
+  uint4 raw[2];
+  load8(J.x, p.x_dtype, gid * 8, raw);
 
+  int64_t dw = gid;  // destination word
+  if (p.pos != nullptr) {
+    // input row = ((b * heads + h) * n_new + t) -> cache row (b*heads+h)*cap + pos[b] + t
+    const uint32_t wpr = static_cast<uint32_t>(p.dim) >> 3;  // words per row
+    int64_t row, bh, b;
+    if (p.words <= 0x7FFFFFFFll) {  // uniform
+      const uint32_t r = fast_div(static_cast<uint32_t>(gid), p.by_row), h = fast_div(r, p.by_new);
+      row = r;
+      bh = h;
+      b = fast_div(h, p.by_heads);
+    } else {
+      row = gid / wpr;
+      bh = row / p.n_new;
+      b = bh / p.heads;
+    }
+    const int t = static_cast<int>(row - bh * p.n_new);
+    if constexpr (PAGED) {
+      const int64_t r = static_cast<int64_t>(p.pos[b]) + t;
+      if (r < 0 || r >= p.cap) return;
+      const int page = p.tables[b * p.max_pages + (r >> p.page_shift)];
+      if (static_cast<unsigned>(page) >= static_cast<unsigned>(p.num_pages)) return;
+      const int64_t first = (static_cast<int64_t>(page) * p.heads + (bh - b * p.heads)) << p.page_shift;
+      dw = gid + (first + (r & ((int64_t{1} << p.page_shift) - 1)) - row) * wpr;
+    } else {
+      int dst = p.pos[b] + t;
+      if (p.ring) {
+        // a ring keeps the newest cap rows: older rows of this append would
+        // land on the same slots, so they are not written at all
+        if (p.pos[b] < 0 || t < p.n_new - p.cap) return;
+        dst %= p.cap;
+      }
+      if (dst < 0 || dst >= p.cap) return;
+      dw = gid + (bh * p.cap + dst - row) * wpr;
+    }
+  }
+
+  float v[8];
+  floats8(raw, p.x_dtype, v);
   float mx = v[0], mn = v[0];
 #pragma unroll
   for (int i = 1; i < 8; ++i) {
     mx = fmaxf(mx, v[i]);
     mn = fminf(mn, v[i]);
   }
-#pragma unroll
-  for (int off = 1; off < 8; off <<= 1) {
-    mx = fmaxf(mx, shfl_xor_f(mx, off));
-    mn = fminf(mn, shfl_xor_f(mn, off));
-  }
+  mx = of_group(mx, [](float a, float b) { return fmaxf(a, b); });
+  mn = of_group(mn, [](float a, float b) { return fminf(a, b); });
 
   const float n_bins = 15.0f, eps = 1e-7f;
   float d = (mx - mn) / n_bins;
@@ -149,41 +207,6 @@ __global__ __launch_bounds__(256) void quantize_int4_kernel(QuantParams p) {
     word |= static_cast<uint32_t>(n) << (4 * k);
   }
 
-  int64_t dw = gid;  // destination word
-  if (p.pos != nullptr) {
-    // input row = ((b * heads + h) * n_new + t) -> cache row (b*heads+h)*cap + pos[b] + t
-    const uint32_t wpr = static_cast<uint32_t>(p.dim) >> 3;  // words per row
-    int64_t row, bh, b;
-    if (p.words <= 0x7FFFFFFFll) {  // uniform
-      const uint32_t r = fast_div(static_cast<uint32_t>(gid), p.by_row), h = fast_div(r, p.by_new);
-      row = r;
-      bh = h;
-      b = fast_div(h, p.by_heads);
-    } else {
-      row = gid / wpr;
-      bh = row / p.n_new;
-      b = bh / p.heads;
-    }
-    const int t = static_cast<int>(row - bh * p.n_new);
-    if constexpr (PAGED) {
-      const int64_t r = static_cast<int64_t>(p.pos[b]) + t;
-      if (r < 0 || r >= p.cap) return;
-      const int page = p.tables[b * p.max_pages + (r >> p.page_shift)];
-      if (static_cast<unsigned>(page) >= static_cast<unsigned>(p.num_pages)) return;
-      const int64_t first = (static_cast<int64_t>(page) * p.heads + (bh - b * p.heads)) << p.page_shift;
-      dw = gid + (first + (r & ((int64_t{1} << p.page_shift) - 1)) - row) * wpr;
-    } else {
-      int dst = p.pos[b] + t;
-      if (p.ring) {
-        // a ring keeps the newest cap rows: older rows of this append would
-        // land on the same slots, so they are not written at all
-        if (p.pos[b] < 0 || t < p.n_new - p.cap) return;
-        dst %= p.cap;
-      }
-      if (dst < 0 || dst >= p.cap) return;
-      dw = gid + (bh * p.cap + dst - row) * wpr;
-    }
-  }
   J.wq[dw] = word;
   if ((gid & 7) == 0) {  // a row is a whole number of groups
     static_cast<SB*>(J.s)[dw >> 3] = f32_to_sb<SB>(scale);
