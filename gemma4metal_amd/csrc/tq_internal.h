@@ -54,8 +54,9 @@ inline int check_paging(int page_size, int num_pages, int max_pages, const char*
   }
   TQ_CHECK_ARG(num_pages >= 1 && num_pages <= (1 << 28) && max_pages >= 1,
                "%s: need 1 <= num_pages <= 2^28 and max_pages >= 1", fn);
-  TQ_CHECK_ARG(static_cast<int64_t>(max_pages) * page_size < (int64_t{1} << 31),
-               "%s: max_pages * page_size must be below 2^31", fn);
+  // (key positions are rounded up to whole tiles and splits in 32 bits)
+  TQ_CHECK_ARG(static_cast<int64_t>(max_pages) * page_size <= (int64_t{1} << 31) - (1 << 16),
+               "%s: max_pages * page_size must be at most 2^31 - 2^16", fn);
   return TQ_OK;
 }
 

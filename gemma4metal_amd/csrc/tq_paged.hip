@@ -286,7 +286,7 @@ extern "C" int tq_sdpa_int4_paged_prefill(const void* q, tq_dtype q_dtype, const
   p.prefill = 1;
   p.n = n_prior;
   const int64_t rows = static_cast<int64_t>(n_new) * gqa_factor;
-  TQ_CHECK_ARG((rows + 63) / 64 * num_kv_heads < (int64_t{1} << 31), "%s: grid too large", fn);
+  TQ_CHECK_ARG(rows < (int64_t{1} << 31) && (rows + 63) / 64 * num_kv_heads < (int64_t{1} << 31), "%s: grid too large", fn);
   const TilesPlan tiles = plan_paged_tiles(rows, num_kv_heads, head_dim, prompt_keys(n_prior, n_new, sliding_window, num_sinks));
   p.max_splits = tiles.splits;
   if (tiles.splits > 1)

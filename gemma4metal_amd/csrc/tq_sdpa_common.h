@@ -173,9 +173,11 @@ __device__ __forceinline__ PagedKeys paged_keys(const PagedParams& p, int seq_le
 // The split of a paged sequence, in keys of its list.
 __device__ __forceinline__ SplitRange paged_range(const SdpaParams& p, const PagedKeys& k, int split) {
   SplitRange r;
-  r.S = k.nb > 0 ? (32 * k.nb + p.chunk - 1) / p.chunk : 1;
+  // (unsigned: the sum of two lengths near 2^31)
+  const uint32_t len = 32u * static_cast<uint32_t>(k.nb), chunk = static_cast<uint32_t>(p.chunk);
+  r.S = k.nb > 0 ? static_cast<int>((len + chunk - 1) / chunk) : 1;
   r.t_begin = split * p.chunk;
-  r.t_end = min(r.t_begin + p.chunk, 32 * k.nb);
+  r.t_end = r.t_begin + min(p.chunk, 32 * k.nb - r.t_begin);
   return r;
 }
 

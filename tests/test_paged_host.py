@@ -65,6 +65,18 @@ def test_prompt_attention_refuses_bad_arguments_on_the_host(over, status, needle
     assert st == status and needle in msg, (st, msg)
 
 
+@pytest.mark.parametrize("call", ["attend", "prompt"])
+def test_refuses_tables_that_reach_past_whole_splits_in_32_bits(call):
+    """Positions are rounded up in 32 bits: 2^31 - 2^16 rows are the most."""
+    st, msg = {"attend": attend, "prompt": prompt}[call](P=(1 << 31) // 1024 - 63, page=1024)
+    assert st == 1 and "2^31" in msg
+
+
+def test_refuses_prompt_rows_past_32_bits():
+    st, msg = prompt(Hq=65535, Hkv=1, gqa=65535, new=65535, prior=0, P=4096, page=64)
+    assert st == 1 and "grid" in msg, msg
+
+
 def test_nothing_to_do_is_no_error():
     assert attend(B=0, q=NULL, lens=NULL)[0] == 0
     assert prompt(new=0, q=NULL)[0] == 0
