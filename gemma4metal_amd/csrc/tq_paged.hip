@@ -165,7 +165,8 @@ extern "C" size_t tq_sdpa_int4_paged_workspace_size(int batch, int num_heads, in
   const int gqa = num_heads / num_kv_heads;
   int splits = max_paged_splits(batch, num_heads, num_kv_heads, head_dim, max_kv_len);
   if (shared_prefix > 0)
-    splits += plan_paged_tiles(static_cast<int64_t>(batch) * gqa, num_kv_heads, head_dim, shared_prefix).splits;
+    splits += std::max(plan_paged_tiles(static_cast<int64_t>(batch) * gqa, num_kv_heads, head_dim, shared_prefix, false).splits,
+                       plan_paged_tiles(static_cast<int64_t>(batch) * gqa, num_kv_heads, head_dim, shared_prefix, true).splits);
   return ws_layout(batch, num_heads, head_dim, splits).total + kWsTail;
 }
 
@@ -211,7 +212,8 @@ extern "C" int tq_sdpa_int4_paged(const void* q, tq_dtype q_dtype, const uint32_
   p.cus = pl.slots;
   TilesPlan tiles{0, 0};
   if (shared_prefix > 0)
-    tiles = plan_paged_tiles(static_cast<int64_t>(batch) * gqa_factor, num_kv_heads, head_dim, shared_prefix);
+    tiles = plan_paged_tiles(static_cast<int64_t>(batch) * gqa_factor, num_kv_heads, head_dim, shared_prefix,
+                             q_dtype == TQ_F32 && sb_dtype == TQ_F32);
   p.pre = tiles.splits;
   p.max_splits = pl.max_splits + p.pre;
   if (p.max_splits > 1) {
@@ -246,7 +248,7 @@ extern "C" int tq_sdpa_int4_paged_plan(int batch, int num_heads, int num_kv_head
   if (chunk_keys) *chunk_keys = pl.chunk;
   if (shared_splits)
     *shared_splits = shared_prefix > 0 ? plan_paged_tiles(static_cast<int64_t>(batch) * (num_heads / num_kv_heads),
-                                                          num_kv_heads, head_dim, shared_prefix).splits
+                                                          num_kv_heads, head_dim, shared_prefix, false).splits
                                        : 0;
   if (on_device) *on_device = pl.lpt ? 1 : 0;
   if (kernel && kernel_bytes > 0)
@@ -287,7 +289,8 @@ extern "C" int tq_sdpa_int4_paged_prefill(const void* q, tq_dtype q_dtype, const
   p.n = n_prior;
   const int64_t rows = static_cast<int64_t>(n_new) * gqa_factor;
   TQ_CHECK_ARG(rows < (int64_t{1} << 31) && (rows + 63) / 64 * num_kv_heads < (int64_t{1} << 31), "%s: grid too large", fn);
-  const TilesPlan tiles = plan_paged_tiles(rows, num_kv_heads, head_dim, prompt_keys(n_prior, n_new, sliding_window, num_sinks));
+  const TilesPlan tiles = plan_paged_tiles(rows, num_kv_heads, head_dim, prompt_keys(n_prior, n_new, sliding_window, num_sinks),
+                                           q_dtype == TQ_F32 && sb_dtype == TQ_F32);
   p.max_splits = tiles.splits;
   if (tiles.splits > 1)
     if (int r = set_workspace(p, workspace, workspace_bytes, ws_layout(n_new, num_heads, head_dim, tiles.splits), fn)) return r;

@@ -274,8 +274,8 @@ int tq_sdpa_int4_paged(const void* q, tq_dtype q_dtype,
  * the rows behind the shared ones, at most how many splits of a sequence it makes,
  * the keys of a split (*on_device = 1: the device chooses them from the lengths,
  * within that many splits; the number given is the least that would do for equal
- * ones), and the splits of the shared rows.  Pass the length that windows on the
- * device leave as max_kv_len with sliding_window 0. */
+ * ones), and the splits of the shared rows (queries or scales of 16 bits).  Pass the
+ * length that windows on the device leave as max_kv_len with sliding_window 0. */
 int tq_sdpa_int4_paged_plan(int batch, int num_heads, int num_kv_heads, int head_dim,
                             int max_kv_len, int sliding_window, int num_sinks, int shared_prefix,
                             int* splits, int* chunk_keys, int* shared_splits, int* on_device,
