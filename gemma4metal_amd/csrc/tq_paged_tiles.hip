@@ -1,11 +1,11 @@
-// Multi-query attention over pages with K/V tiles shared by a workgroup's 64
-// (query, head) rows of one kv head: prompts (rows of consecutive queries of one
+// Multi-query attention over pages with K/V tiles shared by a workgroup's 64 or
+// 128 (query, head) rows of one kv head: prompts (rows of consecutive queries of one
 // sequence), and the shared prefix of a batch (rows of all its sequences).
 //
 // The mathematics, operand layouts and staging are those of tq_prefill.hip, and
 // so is what bounds it (VALU).  What differs:
 // - A tile is TK keys at a multiple of TK, one or two 32-row parts of pages;
-//   the page numbers of the next 64 parts are held in a wave's lanes.  Tiles
+//   the pool rows of the next 64 parts are held in a wave's lanes.  Tiles
 //   between the sinks and the window that no row attends are left out.
 // - Rows have limits of their own, [lo, hi) or below the sinks.  In a part of a
 //   tile that some row does not attend wholly, V scales and biases of weight 0
