@@ -149,13 +149,21 @@ def kv_append_int4_paged(k_new: torch.Tensor, v_new: torch.Tensor,
     _need(k_new.dtype in _DT, "k_new must be float32, float16 or bfloat16")
     B, Hkv, T, D = k_new.shape
     pages = (k_quant, k_scales, k_biases, v_quant, v_scales, v_biases)
-    N, H, page, sbt = _check_pages(pages, D, k_new.device)
+    dev = k_new.device
+    di = dev.index
+    if not _pages_fine(pages, D, di):
+        _check_pages(pages, D, dev)
+    N, H, page, _ = k_quant.shape
     _need(H == Hkv, "k_new and the pages must have the same kv heads")
     _need(block_tables.dim() == 2, "block_tables must be (B, max_pages)")
-    _check_ints("block_tables", block_tables, (B, block_tables.shape[1]), k_new.device)
-    _check_ints("positions", positions, (B,), k_new.device)
-    call("tq_kv_append_int4_paged", _ptr(k_new), _ptr(v_new), _DT[k_new.dtype], *map(_ptr, pages), sbt, B, Hkv, D,
-         page, N, _ptr(block_tables), block_tables.shape[1], _ptr(positions), T, _MODES[mode], _stream(None))
+    P = block_tables.shape[1]
+    if not _ints_fine(block_tables, (B, P), di):
+        _check_ints("block_tables", block_tables, (B, P), dev)
+    if not _ints_fine(positions, (B,), di):
+        _check_ints("positions", positions, (B,), dev)
+    call("tq_kv_append_int4_paged", k_new.data_ptr(), v_new.data_ptr(), _DT[k_new.dtype],
+         *[t.data_ptr() for t in pages], _DT[k_scales.dtype], B, Hkv, D, page, N, block_tables.data_ptr(), P,
+         positions.data_ptr(), T, _MODES[mode], _stream(None))
 
 
 @functools.lru_cache(maxsize=256)
