@@ -148,7 +148,8 @@ void kv_append_int4_ring(const array& k_new, const array& v_new, array& k_quant,
 // (num_seqs, max_pages), lengths and reference counts are int32 device arrays; an
 // entry outside [0, num_pages) names no page.  Their semantics are those of the
 // tq_kv_pages_* and *_paged calls of tq_c_api.h.  Workspaces are the library's, per
-// (device, stream), as for sdpa_int4_into.
+// (device, stream), as for sdpa_int4_into; outputs are allocated, so a step that is to
+// be captured into a graph makes the C calls.
 struct kv_pages {
   array k_quant, k_scales, k_biases, v_quant, v_scales, v_biases;
 };
