@@ -60,6 +60,7 @@ SIGNATURES = {
                                        I, I, P, SZ, P]),
     "tq_kv_pages_workspace_size": (SZ, [I, I]),
     "tq_kv_pages_reserve": (I, [P, P, P, P, P, I, I, I, I, P, SZ, P]),
+    "tq_kv_pages_advance": (I, [P, P, P, P, I, I, I, I, P]),
     "tq_kv_pages_fork": (I, [P, I, I, I, I, P, P, P, P, P, I, I, I, I, P, SZ, P]),
     "tq_kv_pages_free": (I, [P, P, P, P, I, I, I, P]),
     "tq_kv_pages_evict": (I, [P, P, P, P, I, I, I, I, I, I, P]),

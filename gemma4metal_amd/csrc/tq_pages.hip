@@ -387,6 +387,31 @@ __global__ __launch_bounds__(256) void pages_free_kernel(int32_t* tables, int32_
   }
 }
 
+// Lengths of sequences whose new rows have pages, a group of lanes a sequence.  One
+// chain of loads (length, entry) bounds it.
+__global__ __launch_bounds__(256) void pages_advance_kernel(const int32_t* tables, int32_t* lengths, const int32_t* n_new,
+                                                            int32_t* advanced, int seqs, int max_pages, int num_pages,
+                                                            int page_size) {
+  const int lane = threadIdx.x % kPlanGroup;
+  const int s = static_cast<int>((static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) / kPlanGroup);
+  if (s >= seqs) return;  // whole groups
+  const int64_t own = lengths[s], k = n_new[s];
+  const int64_t n = max(own, int64_t{0}), e1 = (n + k + page_size - 1) / page_size;
+  bool ok = k > 0 && e1 <= max_pages;
+  if (ok) {
+    const int32_t* row = tables + static_cast<int64_t>(s) * max_pages;
+    bool lacks = false;
+#pragma unroll 4
+    for (int64_t e = n / page_size + lane; e < e1; e += kPlanGroup) lacks |= !is_page(row[e], num_pages);
+    ok = group_ballot(lacks) == 0;
+  }
+  if (lane == 0) {
+    if (ok) lengths[s] = static_cast<int>(n + k);
+    else if (k < 0) lengths[s] = static_cast<int>(max(own + k, int64_t{0}));
+    advanced[s] = ok;
+  }
+}
+
 int check_tables(int num_seqs, int max_pages, int num_pages, int page_size, const char* fn) {
   if (int r = check_paging(page_size, num_pages, max_pages, fn)) return r;
   TQ_CHECK_ARG(num_seqs >= 0 && num_seqs <= (1 << 20), "%s: num_seqs must be 0 to 2^20", fn);
@@ -525,6 +550,21 @@ extern "C" int tq_kv_pages_evict(int32_t* block_tables, int32_t* refs, const int
       block_tables, refs, const_cast<int32_t*>(lengths), which, n, max_pages, num_pages, page_size, sliding_window,
       num_sinks);
   TQ_CHECK_LAUNCH("pages_free_kernel");
+  return TQ_OK;
+}
+
+extern "C" int tq_kv_pages_advance(const int32_t* block_tables, int32_t* lengths, const int32_t* n_new,
+                                   int32_t* advanced, int num_seqs, int max_pages, int num_pages, int page_size,
+                                   void* stream) {
+  clear_error();
+  const char* fn = "tq_kv_pages_advance";
+  if (int r = check_tables(num_seqs, max_pages, num_pages, page_size, fn)) return r;
+  if (num_seqs == 0) return TQ_OK;
+  TQ_CHECK_ARG(block_tables && lengths && n_new && advanced, "%s: null pointer", fn);
+  constexpr int kSeqs = 256 / kPlanGroup;
+  pages_advance_kernel<<<static_cast<unsigned>((num_seqs + kSeqs - 1) / kSeqs), 256, 0, static_cast<hipStream_t>(stream)>>>(
+      block_tables, lengths, n_new, advanced, num_seqs, max_pages, num_pages, page_size);
+  TQ_CHECK_LAUNCH("pages_advance_kernel");
   return TQ_OK;
 }
 

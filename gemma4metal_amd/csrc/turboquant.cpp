@@ -506,6 +506,17 @@ array kv_pages_reserve(array& block_tables, array& refs, const array& lengths, c
   return granted;
 }
 
+array kv_pages_advance(const array& block_tables, const array& refs, array& lengths,
+                       const array& n_new, int page_size, StreamOrDevice s) {
+  const Tables t = tables_of(block_tables);
+  const int pages = page_count(refs);
+  array advanced = array::empty({t.seqs}, Dtype::int32);
+  check(tq_kv_pages_advance(t.p, ints(lengths, {t.seqs}, "lengths"), ints(n_new, {t.seqs}, "n_new"),
+                            static_cast<int32_t*>(advanced.data()), t.seqs, t.width, pages, page_size, s),
+        "kv_pages_advance");
+  return advanced;
+}
+
 array kv_pages_fork(kv_pages& pages, array& block_tables, array& refs, array& lengths,
                     const array& parents, StreamOrDevice s) {
   const PoolDims d = pool_dims(pages, true);

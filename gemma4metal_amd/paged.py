@@ -323,6 +323,23 @@ def kv_pages_reserve(block_tables: torch.Tensor, refs: torch.Tensor, lengths: to
 
 
 @_placed
+def kv_pages_advance(block_tables: torch.Tensor, refs: torch.Tensor, lengths: torch.Tensor, n_new: torch.Tensor,
+                     page_size: int) -> torch.Tensor:
+    """Counts appended rows: lengths[s] += n_new[s] where every one of those rows
+    has a page, as after a granted :func:`kv_pages_reserve`.  Elsewhere the length
+    stays: the append dropped rows, and a page that the sequence gets later holds
+    what its last owner left there.  A negative n_new takes rows back (not into
+    pages that other sequences share).  Returns int32 (sequences,): 1 where rows
+    were counted."""
+    S, P, N, dev = _check_state(block_tables, refs, lengths)
+    _check_ints("n_new", n_new, (S,), dev)
+    advanced = torch.empty(S, dtype=torch.int32, device=dev)
+    call("tq_kv_pages_advance", _ptr(block_tables), _ptr(lengths), _ptr(n_new), _ptr(advanced), S, P, N,
+         int(page_size), _stream(None))
+    return advanced
+
+
+@_placed
 def kv_pages_fork(pages, block_tables: torch.Tensor, refs: torch.Tensor, lengths: torch.Tensor,
                   parents: torch.Tensor, *, workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Makes every sequence s with parents[s] >= 0 a continuation of that
@@ -405,7 +422,10 @@ class PagedInt4KVCache:
 
     One step of a batch is ``reserve(n_new)``, ``append(layer, k, v)`` and
     ``attend(layer, q, ...)`` per layer, then ``advance(n_new)``; attention
-    covers the rows appended since the last ``advance`` too."""
+    covers the rows appended since the last ``advance`` too.  A sequence that
+    ``reserve`` refused (0 in what it returns) is left behind by the step: its
+    rows are dropped, ``advance`` does not count them, and its attention is not
+    that of the new token.  It asks for the same rows again."""
 
     def __init__(self, num_pages: int, page_size: int, sequences: int, max_pages: int, num_kv_heads: int,
                  head_dim: int, device, *, num_layers: int = 1, scale_dtype: torch.dtype = torch.float16):
@@ -438,8 +458,13 @@ class PagedInt4KVCache:
         kv_append_int4_paged(k_new[None], v_new[None], *self.layer(layer), self.block_tables[s], self.lengths[s],
                              mode=mode)
 
-    def advance(self, n_new: torch.Tensor) -> None:
-        self.lengths += n_new
+    def advance(self, n_new: torch.Tensor) -> torch.Tensor:
+        """Counts the rows appended in this step, of the sequences that have pages
+        for them: a sequence that ``reserve`` refused keeps its length.  Returns
+        int32 (sequences,): 1 where rows were counted."""
+        if not _ints_fine(n_new, self.lengths.shape, self.lengths.get_device()):
+            n_new = torch.zeros_like(self.lengths).add_(n_new)
+        return kv_pages_advance(self.block_tables, self.refs, self.lengths, n_new, self.page_size)
 
     def attend(self, layer: int, queries: torch.Tensor, gqa_factor: int, scale: float = 1.0, sliding_window: int = 0,
                num_sinks: int = 0, *, new: int = 1, windows: Optional[torch.Tensor] = None, shared_prefix: int = 0,

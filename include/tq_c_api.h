@@ -325,6 +325,16 @@ int tq_kv_pages_reserve(int32_t* block_tables, int32_t* refs, const int32_t* len
                         int num_pages, int page_size, void* workspace, size_t workspace_bytes,
                         void* stream);
 
+/* Counts the rows appended to sequence s: lengths[s] += n_new[s] (> 0) where every
+ * one of rows lengths[s] .. lengths[s] + n_new[s] - 1 has a page, as after a granted
+ * tq_kv_pages_reserve; else the length stays, since tq_kv_append_int4_paged dropped
+ * rows, and a page that the sequence gets later holds what its last owner left there.
+ * advanced [num_seqs] is written: 1 where rows were counted.  A negative n_new takes
+ * rows back (to 0 at the least), not into pages that other sequences share. */
+int tq_kv_pages_advance(const int32_t* block_tables, int32_t* lengths, const int32_t* n_new,
+                        int32_t* advanced, int num_seqs, int max_pages, int num_pages,
+                        int page_size, void* stream);
+
 /* Makes sequence s a continuation of sequence parents[s] (DEVICE int32
  * [num_seqs]; negative = none): the parent's full pages are shared, and its
  * last page, where partly filled, is copied to a page of s's own, so that both

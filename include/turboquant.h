@@ -178,6 +178,10 @@ array sdpa_int4_paged_prefill(const array& queries, const kv_pages& pages,
 // (num_seqs): 1 where the request was granted (as kv_pages_fork does).
 array kv_pages_reserve(array& block_tables, array& refs, const array& lengths, const array& n_new,
                        int page_size, StreamOrDevice s = {});
+// lengths[s] += n_new[s] where all of those rows have pages.  Returns int32 (num_seqs):
+// 1 where they were counted.
+array kv_pages_advance(const array& block_tables, const array& refs, array& lengths,
+                       const array& n_new, int page_size, StreamOrDevice s = {});
 // Sequence s continues parents[s] (negative: none).
 array kv_pages_fork(kv_pages& pages, array& block_tables, array& refs, array& lengths,
                     const array& parents, StreamOrDevice s = {});

@@ -115,6 +115,18 @@ class Pool:
             granted[s] = 1
         return granted
 
+    def advance(self, n_new):
+        advanced = np.zeros(len(n_new), np.int32)
+        for s, new in enumerate(n_new):
+            n, new = max(int(self.lengths[s]), 0), int(new)
+            e1 = -(-(n + new) // self.page)
+            if new < 0:
+                self.lengths[s] = max(int(self.lengths[s]) + new, 0)
+            elif new and e1 <= self.tables.shape[1] and all(
+                    self._is_page(e) for e in self.tables[s, n // self.page:e1]):
+                self.lengths[s], advanced[s] = n + new, 1
+        return advanced
+
     def fork(self, parents):
         granted = np.zeros(len(parents), np.int32)
         free = [p for p, r in enumerate(self.refs) if r <= 0]
