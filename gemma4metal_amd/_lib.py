@@ -54,6 +54,8 @@ SIGNATURES = {
     "tq_sdpa_int4_paged_workspace_size": (SZ, [I, I, I, I, I, I]),
     "tq_sdpa_int4_paged": (I, [P, I, P, P, P, P, P, P, I, P, I, I, I, I, I, I, P, I, P, P, I, I, F, I,
                                I, I, P, SZ, P]),
+    "tq_sdpa_int4_paged_prefix": (I, [P, I, P, P, P, P, P, P, I, P, I, I, I, I, I, I, P, I, P, P, I, I, F, I,
+                                      I, P, I, P, SZ, P]),
     "tq_sdpa_int4_paged_plan": (I, [I, I, I, I, I, I, I, I, P, P, P, P, P, SZ]),
     "tq_sdpa_int4_paged_prefill_workspace_size": (SZ, [I, I, I, I, I]),
     "tq_sdpa_int4_paged_prefill": (I, [P, I, P, P, P, P, P, P, I, P, I, I, I, I, I, P, I, I, I, I, F,

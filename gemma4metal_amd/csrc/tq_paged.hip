@@ -170,16 +170,16 @@ extern "C" size_t tq_sdpa_int4_paged_workspace_size(int batch, int num_heads, in
   return ws_layout(batch, num_heads, head_dim, splits).total + kWsTail;
 }
 
-extern "C" int tq_sdpa_int4_paged(const void* q, tq_dtype q_dtype, const uint32_t* k_quant, const void* k_scales,
-                                  const void* k_biases, const uint32_t* v_quant, const void* v_scales,
-                                  const void* v_biases, tq_dtype sb_dtype, float* out, int batch, int num_heads,
-                                  int num_kv_heads, int head_dim, int page_size, int num_pages,
-                                  const int32_t* block_tables, int max_pages, const int32_t* seq_lens,
-                                  const int32_t* windows, int max_kv_len, int gqa_factor, float scale,
-                                  int sliding_window, int num_sinks, int shared_prefix, void* workspace,
-                                  size_t workspace_bytes, void* stream) {
+namespace {
+
+// prefix_table: the pages of the shared rows; NULL: sequence 0's.
+int paged_decode(const void* q, int q_dtype, const uint32_t* k_quant, const void* k_scales, const void* k_biases,
+                 const uint32_t* v_quant, const void* v_scales, const void* v_biases, int sb_dtype, float* out, int batch,
+                 int num_heads, int num_kv_heads, int head_dim, int page_size, int num_pages, const int32_t* block_tables,
+                 int max_pages, const int32_t* seq_lens, const int32_t* windows, int max_kv_len, int gqa_factor,
+                 float scale, int sliding_window, int num_sinks, const int32_t* prefix_table, int shared_prefix,
+                 void* workspace, size_t workspace_bytes, void* stream, const char* fn) {
   clear_error();
-  const char* fn = "tq_sdpa_int4_paged";
   TQ_CHECK_ARG(batch >= 0 && batch <= 65535, "%s: batch must be 0 to 65535", fn);
   if (batch == 0) return TQ_OK;
   PagedParams p{};
@@ -222,12 +222,47 @@ extern "C" int tq_sdpa_int4_paged(const void* q, tq_dtype q_dtype, const uint32_
   const dim3 grid(pl.grid_x, num_kv_heads * pl.n_sub, batch);
   p.cnt_stride = counter_stride(static_cast<int64_t>(batch) * num_heads);
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (p.pre > 0)
-    if (int r = launch_paged_tiles(p, head_dim, sb_dtype, tiles, true, s)) return r;
+  if (p.pre > 0) {
+    PagedParams t = p;
+    if (prefix_table) t.tables = prefix_table;
+    t.max_pages = shared_prefix / page_size;
+    if (int r = launch_paged_tiles(t, head_dim, sb_dtype, tiles, true, s)) return r;
+  }
   if (!pl.hc) return launch_sdpa_mfma(p, head_dim, pl.G, sb_dtype, grid, s);
   p.ext_merge = p.max_splits > 1 ? 1 : 0;
   const int r = launch_sdpa_hc(p, sb_dtype, grid, s);
   return r != TQ_OK || !p.ext_merge ? r : launch_merge_splits(p, head_dim, batch, s);
+}
+
+}  // namespace
+
+extern "C" int tq_sdpa_int4_paged(const void* q, tq_dtype q_dtype, const uint32_t* k_quant, const void* k_scales,
+                                  const void* k_biases, const uint32_t* v_quant, const void* v_scales,
+                                  const void* v_biases, tq_dtype sb_dtype, float* out, int batch, int num_heads,
+                                  int num_kv_heads, int head_dim, int page_size, int num_pages,
+                                  const int32_t* block_tables, int max_pages, const int32_t* seq_lens,
+                                  const int32_t* windows, int max_kv_len, int gqa_factor, float scale,
+                                  int sliding_window, int num_sinks, int shared_prefix, void* workspace,
+                                  size_t workspace_bytes, void* stream) {
+  return paged_decode(q, q_dtype, k_quant, k_scales, k_biases, v_quant, v_scales, v_biases, sb_dtype, out, batch, num_heads,
+                      num_kv_heads, head_dim, page_size, num_pages, block_tables, max_pages, seq_lens, windows,
+                      max_kv_len, gqa_factor, scale, sliding_window, num_sinks, nullptr, shared_prefix, workspace,
+                      workspace_bytes, stream, "tq_sdpa_int4_paged");
+}
+
+extern "C" int tq_sdpa_int4_paged_prefix(const void* q, tq_dtype q_dtype, const uint32_t* k_quant,
+                                         const void* k_scales, const void* k_biases, const uint32_t* v_quant,
+                                         const void* v_scales, const void* v_biases, tq_dtype sb_dtype, float* out,
+                                         int batch, int num_heads, int num_kv_heads, int head_dim, int page_size,
+                                         int num_pages, const int32_t* block_tables, int max_pages,
+                                         const int32_t* seq_lens, const int32_t* windows, int max_kv_len,
+                                         int gqa_factor, float scale, int sliding_window, int num_sinks,
+                                         const int32_t* prefix_table, int shared_prefix, void* workspace,
+                                         size_t workspace_bytes, void* stream) {
+  return paged_decode(q, q_dtype, k_quant, k_scales, k_biases, v_quant, v_scales, v_biases, sb_dtype, out, batch, num_heads,
+                      num_kv_heads, head_dim, page_size, num_pages, block_tables, max_pages, seq_lens, windows,
+                      max_kv_len, gqa_factor, scale, sliding_window, num_sinks, prefix_table, shared_prefix, workspace,
+                      workspace_bytes, stream, "tq_sdpa_int4_paged_prefix");
 }
 
 extern "C" int tq_sdpa_int4_paged_plan(int batch, int num_heads, int num_kv_heads, int head_dim, int max_kv_len,

@@ -85,7 +85,7 @@ struct PagedParams : SdpaParams {
   const int* tables;
   int max_pages, num_pages, page_shift;
   int sinks;
-  int shared;  // rows of every sequence that lie in sequence 0's pages
+  int shared;  // rows of every sequence that lie in the same pages
   // Partials of every row that lie before a launch's own splits (those of the
   // shared rows), joined with them.
   int pre;

@@ -442,7 +442,7 @@ void kv_append_int4_paged(const array& k_new, const array& v_new, kv_pages& page
 array sdpa_int4_paged(const array& queries, const kv_pages& pages, const array& block_tables,
                       const array& seq_lens, int gqa_factor, float scale, int sliding_window,
                       int num_sinks, int shared_prefix, const array& windows, int max_kv_len,
-                      StreamOrDevice s) {
+                      StreamOrDevice s, const array& prefix_table) {
   const PoolDims d = pool_dims(pages, false);
   const Tables t = tables_of(block_tables);
   need(queries.ndim() == 3 && queries.shape(0) == t.seqs && queries.shape(2) == d.D &&
@@ -455,13 +455,16 @@ array sdpa_int4_paged(const array& queries, const kv_pages& pages, const array& 
   array out = array::empty({t.seqs, Hq, d.D}, Dtype::float32);
   size_t have = 0;
   void* ws = workspace(tq_sdpa_int4_paged_workspace_size(t.seqs, Hq, d.Hkv, d.D, n, shared_prefix), &have, s);
-  check(tq_sdpa_int4_paged(queries.data(), c_dtype(queries.dtype()), words(pages.k_quant),
-                           pages.k_scales.data(), pages.k_biases.data(), words(pages.v_quant),
-                           pages.v_scales.data(), pages.v_biases.data(), d.sb,
-                           static_cast<float*>(out.data()), t.seqs, Hq, d.Hkv, d.D, d.page,
-                           d.pages, t.p, t.width, ints(seq_lens, {t.seqs}, "seq_lens"),
-                           windows.ndim() > 0 ? ints(windows, {t.seqs}, "windows") : nullptr, n,
-                           gqa_factor, scale, sliding_window, num_sinks, shared_prefix, ws, have, s),
+  need(shared_prefix >= 0 && d.page > 0, "sdpa_int4_paged: bad shared_prefix or page_size");
+  check(tq_sdpa_int4_paged_prefix(
+            queries.data(), c_dtype(queries.dtype()), words(pages.k_quant), pages.k_scales.data(),
+            pages.k_biases.data(), words(pages.v_quant), pages.v_scales.data(), pages.v_biases.data(),
+            d.sb, static_cast<float*>(out.data()), t.seqs, Hq, d.Hkv, d.D, d.page, d.pages, t.p,
+            t.width, ints(seq_lens, {t.seqs}, "seq_lens"),
+            windows.ndim() > 0 ? ints(windows, {t.seqs}, "windows") : nullptr, n, gqa_factor, scale,
+            sliding_window, num_sinks,
+            prefix_table.ndim() > 0 ? ints(prefix_table, {shared_prefix / d.page}, "prefix_table") : nullptr,
+            shared_prefix, ws, have, s),
         "sdpa_int4_paged");
   return out;
 }

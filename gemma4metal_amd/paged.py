@@ -185,7 +185,8 @@ def sdpa_int4_paged(queries: torch.Tensor,
                     v_quant: torch.Tensor, v_scales: torch.Tensor, v_biases: torch.Tensor,
                     block_tables: torch.Tensor, seq_lens: torch.Tensor, gqa_factor: int, scale: float = 1.0,
                     sliding_window: int = 0, num_sinks: int = 0, *, windows: Optional[torch.Tensor] = None,
-                    shared_prefix: int = 0, max_kv_len: Optional[int] = None, out: Optional[torch.Tensor] = None,
+                    shared_prefix: int = 0, prefix_table: Optional[torch.Tensor] = None,
+                    max_kv_len: Optional[int] = None, out: Optional[torch.Tensor] = None,
                     workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Batched decode attention over pages.  queries (B, Hq, D) f32|f16|bf16;
     block_tables int32 (B, max_pages); seq_lens / windows int32 (B).  The query
@@ -193,10 +194,13 @@ def sdpa_int4_paged(queries: torch.Tensor,
     seq_lens[b] - W, or t < num_sinks (the first tokens stay visible); none: 0.
 
     ``shared_prefix`` (a multiple of the page size): the first rows of every
-    sequence lie in sequence 0's pages, as after :func:`kv_pages_fork`, and are
-    attended once for the whole batch.  ``max_kv_len`` bounds the lengths
-    (longer ones are cut to it); the table's reach by default.  Returns
-    (B, Hq, D) float32."""
+    sequence lie in the same pages, as after :func:`kv_pages_fork`, and are
+    attended once for the whole batch.  They are those of sequence 0's table or,
+    where it has been freed or evicted from, of ``prefix_table`` (int32
+    (shared_prefix / page size,)), which must name every prefix page that a
+    sequence attends (:meth:`PagedInt4KVCache.prefix_table`).
+    ``max_kv_len`` bounds the lengths (longer ones are cut to it); the table's
+    reach by default.  Returns (B, Hq, D) float32."""
     _check_cuda("queries", queries)
     _need(queries.dim() == 3 and queries.dtype in _DT, "queries must be (B, Hq, D) float32, float16 or bfloat16")
     B, Hq, D = queries.shape
@@ -222,10 +226,15 @@ def sdpa_int4_paged(queries: torch.Tensor,
         out = _out(out, (B, Hq, D), dev)
     sh = _stream(None)
     ws = _workspace(workspace, _paged_ws_size(B, Hq, Hkv, D, mx, int(shared_prefix)), dev, sh)
-    call("tq_sdpa_int4_paged", queries.data_ptr(), _DT[queries.dtype], *[t.data_ptr() for t in pages], sbt,
-         out.data_ptr(), B, Hq, Hkv, D, page, N, block_tables.data_ptr(), P, seq_lens.data_ptr(), _ptr(windows), mx,
-         int(gqa_factor), float(scale), int(sliding_window), int(num_sinks), int(shared_prefix), ws.data_ptr(),
-         ws.numel(), sh)
+    if prefix_table is None:
+        name, prefix = "tq_sdpa_int4_paged", ()
+    else:
+        _need(page > 0, "k_quant must have rows")
+        _check_ints("prefix_table", prefix_table, (int(shared_prefix) // page,), dev)
+        name, prefix = "tq_sdpa_int4_paged_prefix", (prefix_table.data_ptr(),)
+    call(name, queries.data_ptr(), _DT[queries.dtype], *[t.data_ptr() for t in pages], sbt, out.data_ptr(), B, Hq, Hkv,
+         D, page, N, block_tables.data_ptr(), P, seq_lens.data_ptr(), _ptr(windows), mx, int(gqa_factor), float(scale),
+         int(sliding_window), int(num_sinks), *prefix, int(shared_prefix), ws.data_ptr(), ws.numel(), sh)
     return out
 
 
@@ -361,7 +370,8 @@ def kv_pages_fork(pages, block_tables: torch.Tensor, refs: torch.Tensor, lengths
 @_placed
 def kv_pages_free(block_tables: torch.Tensor, refs: torch.Tensor, lengths: torch.Tensor, which: torch.Tensor) -> None:
     """Ends the sequences with which[s] != 0: pages lose a reference, table rows
-    become -1 and lengths 0."""
+    become -1 and lengths 0.  See ``prefix_table`` of :func:`sdpa_int4_paged` where
+    sequences share a prefix."""
     S, P, N, dev = _check_state(block_tables, refs, lengths)
     _check_ints("which", which, (S,), dev)
     call("tq_kv_pages_free", _ptr(block_tables), _ptr(refs), _ptr(lengths), _ptr(which), S, P, N, _stream(None))
@@ -372,7 +382,9 @@ def kv_pages_evict(block_tables: torch.Tensor, refs: torch.Tensor, lengths: torc
                    sliding_window: int, num_sinks: int = 0, which: Optional[torch.Tensor] = None) -> None:
     """Gives up the pages that lie wholly between the first num_sinks rows and
     the window's last ``sliding_window`` ones, of the sequences with which[s]
-    != 0 (all by default); their entries become -1."""
+    != 0 (all by default); their entries become -1.  The tables are every layer's:
+    layers that see further back lose those keys too.  See ``prefix_table`` of
+    :func:`sdpa_int4_paged` where sequences share a prefix."""
     S, P, N, dev = _check_state(block_tables, refs, lengths)
     if which is not None:
         _check_ints("which", which, (S,), dev)
@@ -419,6 +431,9 @@ class PagedInt4KVCache:
     it: ``block_tables``, ``lengths`` and page reference counts on the device, so
     that a decode step with its bookkeeping can be captured into a HIP graph.
     Methods run on the current stream.
+
+    The layers share the tables: those with a window and those that see everything
+    need a cache each where ``evict`` is used.
 
     One step of a batch is ``reserve(n_new)``, ``append(layer, k, v)`` and
     ``attend(layer, q, ...)`` per layer, then ``advance(n_new)``; attention
@@ -467,14 +482,22 @@ class PagedInt4KVCache:
         return kv_pages_advance(self.block_tables, self.refs, self.lengths, n_new, self.page_size)
 
     def attend(self, layer: int, queries: torch.Tensor, gqa_factor: int, scale: float = 1.0, sliding_window: int = 0,
-               num_sinks: int = 0, *, new: int = 1, windows: Optional[torch.Tensor] = None, shared_prefix: int = 0,
-               max_kv_len: Optional[int] = None, out: Optional[torch.Tensor] = None,
-               workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
+               num_sinks: int = 0, *, new: int = 1, windows: Optional[torch.Tensor] = None,
+               shared_prefix: int = 0, prefix_table: Optional[torch.Tensor] = None, max_kv_len: Optional[int] = None,
+               out: Optional[torch.Tensor] = None, workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
         """Decode attention of (sequences, Hq, D) queries over the lengths plus
         the ``new`` rows appended in this step."""
         return sdpa_int4_paged(queries, *self.layer(layer), self.block_tables, self.lengths + new, gqa_factor, scale,
                                sliding_window, num_sinks, windows=windows, shared_prefix=shared_prefix,
-                               max_kv_len=max_kv_len, out=out, workspace=workspace)
+                               prefix_table=prefix_table, max_kv_len=max_kv_len, out=out, workspace=workspace)
+
+    def prefix_table(self, shared_prefix: int, sequences: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """The pages of the first ``shared_prefix`` rows, which these sequences (an
+        index tensor; all by default) share as far as they have not given them up:
+        int32 (shared_prefix / page size,), for :meth:`attend`.  Good until pages
+        move or are given up."""
+        t = self.block_tables if sequences is None else self.block_tables[sequences]
+        return t[:, :shared_prefix // self.page_size].amax(0)
 
     def prefill(self, layer: int, sequence: int, queries: torch.Tensor, n_prior: int, gqa_factor: int,
                 scale: float = 1.0, sliding_window: int = 0, num_sinks: int = 0, *,

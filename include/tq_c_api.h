@@ -250,10 +250,18 @@ int tq_kv_append_int4_paged(const void* k_new, const void* v_new, tq_dtype x_dty
  *   16-byte aligned; head_dim in {128, 256, 512}; num_heads == num_kv_heads *
  *   gqa_factor; max_kv_len <= max_pages * page_size.
  * shared_prefix (a multiple of page_size, <= max_kv_len): the first
- * shared_prefix rows of every sequence lie in the same pages, those of
- * sequence 0's table (the other tables' entries there are not read); they are
- * attended once for the whole batch instead of once per sequence.  Sequences
- * may be shorter than it.  It changes no result beyond rounding.
+ * shared_prefix rows of every sequence lie in the same pages; they are attended
+ * once for the whole batch instead of once per sequence.  Sequences may be
+ * shorter than it.  The pages are those of sequence 0's table, or
+ * (tq_sdpa_int4_paged_prefix) of prefix_table, DEVICE int32 [shared_prefix /
+ * page_size], e.g. another sequence's row of the tables; NULL there is sequence
+ * 0's.  No other entry of the tables is read for those rows, so that a page which
+ * the table in use lacks is attended by no sequence: it has to name every prefix
+ * page that any of them attends.  Sequence 0's no longer does after
+ * tq_kv_pages_free of it, nor after tq_kv_pages_evict of pages outside its own
+ * window that shorter sequences (or layers without the window) still attend; the
+ * elementwise maximum of the sequences' rows then does.  Given that, it changes no
+ * result beyond rounding.
  * Workspace as for tq_sdpa_int4_ragged: at least
  * tq_sdpa_int4_paged_workspace_size(...) bytes, zero-filled once, left with its
  * counters zeroed; calls that may overlap (two streams, or two captured graphs
@@ -269,6 +277,17 @@ int tq_sdpa_int4_paged(const void* q, tq_dtype q_dtype,
                        const int32_t* seq_lens, const int32_t* windows, int max_kv_len,
                        int gqa_factor, float scale, int sliding_window, int num_sinks,
                        int shared_prefix, void* workspace, size_t workspace_bytes, void* stream);
+
+int tq_sdpa_int4_paged_prefix(const void* q, tq_dtype q_dtype,
+                              const uint32_t* k_quant, const void* k_scales, const void* k_biases,
+                              const uint32_t* v_quant, const void* v_scales, const void* v_biases,
+                              tq_dtype sb_dtype, float* out,
+                              int batch, int num_heads, int num_kv_heads, int head_dim,
+                              int page_size, int num_pages, const int32_t* block_tables,
+                              int max_pages, const int32_t* seq_lens, const int32_t* windows,
+                              int max_kv_len, int gqa_factor, float scale, int sliding_window,
+                              int num_sinks, const int32_t* prefix_table, int shared_prefix,
+                              void* workspace, size_t workspace_bytes, void* stream);
 
 /* Planning query, with no GPU work: the kernel that tq_sdpa_int4_paged launches for
  * the rows behind the shared ones, at most how many splits of a sequence it makes,
@@ -348,14 +367,20 @@ int tq_kv_pages_fork(void* const* pages, tq_dtype sb_dtype, int num_layers, int 
                      void* stream);
 
 /* Ends the sequences with which[s] != 0 (DEVICE int32 [num_seqs]): their pages
- * lose a reference, their table rows become -1 and their lengths 0. */
+ * lose a reference, their table rows become -1 and their lengths 0.  A batch that
+ * attends a shared prefix by an ended sequence's row needs another prefix_table
+ * (tq_sdpa_int4_paged_prefix). */
 int tq_kv_pages_free(int32_t* block_tables, int32_t* refs, int32_t* lengths, const int32_t* which,
                      int num_seqs, int max_pages, int num_pages, void* stream);
 
 /* Gives up the pages of which no row is visible any more under sliding_window
  * (> 0) and num_sinks: those wholly in rows [num_sinks, lengths[s] -
  * sliding_window) of the sequences with which[s] != 0 (which == NULL: all).
- * Their entries become -1; lengths stay. */
+ * Their entries become -1; lengths stay.  The tables are those of every layer of the
+ * pool: layers whose attention sees further back than this window and these sinks
+ * lose those keys as well, so they need a pool of their own.  A batch that attends a
+ * shared prefix by the row of a longer sequence needs another prefix_table
+ * (tq_sdpa_int4_paged_prefix). */
 int tq_kv_pages_evict(int32_t* block_tables, int32_t* refs, const int32_t* lengths,
                       const int32_t* which, int num_seqs, int max_pages, int num_pages,
                       int page_size, int sliding_window, int num_sinks, void* stream);

@@ -161,12 +161,14 @@ void kv_append_int4_paged(const array& k_new, const array& v_new, kv_pages& page
 // Decode: queries (B, num_heads, head_dim); key t < seq_lens[b] is attended iff
 // sliding_window (windows[b], if given) is 0, or t is among the last that many, or
 // t < num_sinks.  The first shared_prefix rows of all sequences lie in the pages of
-// sequence 0.  max_kv_len < 0: what the tables reach.  Returns (B, num_heads,
-// head_dim) f32.
+// sequence 0, or of prefix_table (shared_prefix / page_size), which name every one of
+// them that a sequence attends.  max_kv_len < 0: what the tables reach.  Returns (B,
+// num_heads, head_dim) f32.
 array sdpa_int4_paged(const array& queries, const kv_pages& pages, const array& block_tables,
                       const array& seq_lens, int gqa_factor, float scale = 1.0f,
                       int sliding_window = 0, int num_sinks = 0, int shared_prefix = 0,
-                      const array& windows = {}, int max_kv_len = -1, StreamOrDevice s = {});
+                      const array& windows = {}, int max_kv_len = -1, StreamOrDevice s = {},
+                      const array& prefix_table = {});
 // Prompt: queries (n_new, num_heads, head_dim) at positions n_prior ... over the
 // pages of one sequence, block_table (max_pages), which hold the new rows already.
 array sdpa_int4_paged_prefill(const array& queries, const kv_pages& pages,

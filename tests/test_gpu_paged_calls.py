@@ -78,3 +78,79 @@ def test_advance_random(pg, S, width, N, page):
     pool = OP.Pool(tables, np.zeros(N, np.int32), lens, page)
     assert np.array_equal(host(pg.kv_pages_advance(t, r, n, dev(ask), page)), pool.advance(ask))
     assert np.array_equal(host(n), pool.lengths) and np.array_equal(host(t), tables)
+
+
+# ---------------------------------------------------------------------------
+# prefixes whose sequences give pages up
+# ---------------------------------------------------------------------------
+
+def shared_run(pg, rng, Hq, Hkv, D, page, P, tails):
+    """A prompt of P rows, forked, each sequence with rows of its own; the cache and
+    its state on the host."""
+    S, width = len(tails), P // page + 4
+    N = P // page + 4 * S
+    c = pg.PagedInt4KVCache(N, page, S, width, Hkv, D, "cuda")
+    ask = np.zeros(S, np.int32)
+    ask[0] = P
+    assert host(c.reserve(ints(ask)))[0] == 1
+    c.append_one(0, 0, *(queries(rng, (Hkv, P, D), "bf16")[0] for _ in range(2)))
+    c.advance(ints(ask))
+    par = np.zeros(S, np.int32)
+    par[0] = -1
+    assert host(c.fork(ints(par))).tolist() == [0] + [1] * (S - 1)
+    assert host(c.reserve(ints(tails))).all()
+    for s, T in enumerate(tails):
+        c.append_one(0, s, *(queries(rng, (Hkv, T, D), "bf16")[0] for _ in range(2)))
+    assert host(c.advance(ints(tails))).all()
+    return c
+
+
+def attention_of(c, qf, gqa, W, sinks):
+    return OP.sdpa_int4_paged(qf, [host(x[0]) for x in c.tensors()], host(c.block_tables), host(c.lengths), c.page_size,
+                              gqa, 1.0, W, sinks)
+
+
+CASES = [(4, 2, 128, 32, 5), (8, 1, 256, 64, 4), (8, 1, 512, 32, 9), (4, 2, 512, 128, 2)]
+
+
+@pytest.mark.parametrize("Hq,Hkv,D,page,blocks", CASES)
+def test_a_prefix_outlives_the_sequence_it_came_with(pg, Hq, Hkv, D, page, blocks):
+    rng = np.random.default_rng(D + page)
+    P, none = blocks * page, ints([0] * 4)
+    c = shared_run(pg, rng, Hq, Hkv, D, page, P, [9, 40, 1, 2 * page])
+    q, qf = queries(rng, (4, Hq, D), "bf16")
+    whole = attention_of(c, qf, Hq // Hkv, 0, 0)
+    close(host(c.attend(0, q, Hq // Hkv, new=none, shared_prefix=P)), whole)
+    c.free(ints([1, 0, 0, 0]))
+    for table in (c.block_tables[2, :blocks], c.prefix_table(P), c.prefix_table(P, torch.tensor([1, 3], device="cuda"))):
+        got = host(c.attend(0, q, Hq // Hkv, new=none, shared_prefix=P, prefix_table=table))
+        close(got[1:], whole[1:])
+        assert not got[0].any()
+
+
+@pytest.mark.parametrize("Hq,Hkv,D,page,blocks", CASES)
+@pytest.mark.parametrize("sinks", [0, 5])
+def test_a_prefix_after_evictions(pg, Hq, Hkv, D, page, blocks, sinks):
+    """The longest sequence comes first and gives up what the others attend."""
+    rng = np.random.default_rng(D + sinks)
+    P, W, none = blocks * page, blocks * page - page // 2, ints([0] * 4)
+    c = shared_run(pg, rng, Hq, Hkv, D, page, P, [3 * page, 40, 1, page])
+    q, qf = queries(rng, (4, Hq, D), "bf16")
+    whole = attention_of(c, qf, Hq // Hkv, W, sinks)
+    c.evict(W, sinks)
+    tables = host(c.block_tables)[:, :blocks]
+    assert (tables[0] < 0).sum() > (tables[2] < 0).sum()
+    close(attention_of(c, qf, Hq // Hkv, W, sinks), whole)  # nothing attended was given up
+    got = c.attend(0, q, Hq // Hkv, 1.0, W, sinks, new=none, shared_prefix=P, prefix_table=c.prefix_table(P))
+    close(host(got), whole)
+
+
+def test_prefix_table_refusals(pg):
+    rng = np.random.default_rng(0)
+    d = [dev(p) for p in make_pool(rng, 4, 2, 32, 128, "f16")]
+    q = torch.zeros((1, 4, 128), device="cuda")
+    t, n = ints([[0, 1]]), ints([40])
+    pg.sdpa_int4_paged(q, *d, t, n, 2, shared_prefix=32, prefix_table=t[0, :1])
+    for bad in (t[0], t[0, :0], t[0, :1].long(), t[0, :1].cpu(), t[:, :1]):
+        with pytest.raises(ValueError, match="prefix_table"):
+            pg.sdpa_int4_paged(q, *d, t, n, 2, shared_prefix=32, prefix_table=bad)

@@ -43,3 +43,31 @@ def test_oracle_advances_only_rows_that_have_pages():
     assert p.lengths.tolist() == [64, 32, 0, 96, 30]
     assert list(p.advance([0, 1, -5, 1, -7])) == [0, 0, 0, 0, 0]  # row 96 is past the table
     assert p.lengths.tolist() == [64, 32, 0, 96, 23]
+
+
+# ---------------------------------------------------------------------------
+# a prefix by a table of its own
+# ---------------------------------------------------------------------------
+
+def prefix(**over):
+    a = dict(q=FAKE, qd=_lib.TQ_BF16, kq=FAKE, ks=FAKE, kb=FAKE, vq=FAKE, vs=FAKE, vb=FAKE, sb=_lib.TQ_F16, out=FAKE,
+             B=2, Hq=32, Hkv=16, D=256, page=64, N=10, tab=FAKE, P=4, lens=FAKE, win=NULL, mx=256, gqa=2, scale=1.0,
+             W=0, sinks=0, table=FAKE, pre=64, ws=NULL, wsb=0)
+    assert set(over) <= set(a)
+    a.update(over)
+    lib = _lib.load()
+    return lib.tq_sdpa_int4_paged_prefix(*a.values(), NULL), lib.tq_last_error().decode()
+
+
+@pytest.mark.parametrize("over,status,needle", [
+    (dict(pre=32), 1, "shared_prefix"), (dict(pre=320), 1, "shared_prefix"), (dict(pre=-64), 1, "shared_prefix"),
+    (dict(lens=NULL), 1, "seq_lens"), (dict(tab=NULL), 1, "null"), (dict(D=64), 2, "head_dim"), (dict(mx=257), 1, "max_kv_len"),
+    (dict(), 4, "workspace"),
+])
+def test_prefix_call_refuses_bad_arguments_on_the_host(over, status, needle):
+    st, msg = prefix(**over)
+    assert st == status and needle in msg and "tq_sdpa_int4_paged_prefix" in msg, (st, msg)
+
+
+def test_prefix_call_with_nothing_to_do_is_no_error():
+    assert prefix(B=0, q=NULL, table=NULL)[0] == 0
