@@ -19,7 +19,7 @@ from __future__ import annotations
 
 import ctypes
 import functools
-from typing import Optional
+from typing import Optional, Union
 
 import torch
 
@@ -482,11 +482,13 @@ class PagedInt4KVCache:
         return kv_pages_advance(self.block_tables, self.refs, self.lengths, n_new, self.page_size)
 
     def attend(self, layer: int, queries: torch.Tensor, gqa_factor: int, scale: float = 1.0, sliding_window: int = 0,
-               num_sinks: int = 0, *, new: int = 1, windows: Optional[torch.Tensor] = None,
+               num_sinks: int = 0, *, new: Union[int, torch.Tensor] = 1, windows: Optional[torch.Tensor] = None,
                shared_prefix: int = 0, prefix_table: Optional[torch.Tensor] = None, max_kv_len: Optional[int] = None,
                out: Optional[torch.Tensor] = None, workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
         """Decode attention of (sequences, Hq, D) queries over the lengths plus
-        the ``new`` rows appended in this step."""
+        the ``new`` rows appended in this step: one count for all, or int32
+        (sequences,).  A sequence that appended fewer rows than that attends
+        whatever its pages hold behind them; its result means nothing."""
         return sdpa_int4_paged(queries, *self.layer(layer), self.block_tables, self.lengths + new, gqa_factor, scale,
                                sliding_window, num_sinks, windows=windows, shared_prefix=shared_prefix,
                                prefix_table=prefix_table, max_kv_len=max_kv_len, out=out, workspace=workspace)

@@ -80,6 +80,25 @@ def test_advance_random(pg, S, width, N, page):
     assert np.array_equal(host(n), pool.lengths) and np.array_equal(host(t), tables)
 
 
+def test_sequences_that_append_nothing(pg):
+    """With a count per sequence the others attend just their own rows, whatever
+    lies behind those."""
+    rng = np.random.default_rng(12)
+    Hq, Hkv, D, page = 4, 2, 128, 32
+    c = pg.PagedInt4KVCache(6, page, 3, 2, Hkv, D, "cuda")
+    first = ints([40, 33, 7])
+    c.reserve(first)
+    for s, T in enumerate((40, 33, 7)):
+        k, v = (queries(rng, (Hkv, 64, D), "bf16")[0] for _ in range(2))
+        c.append_one(0, s, k, v)  # rows behind the length too
+    c.advance(first)
+    q, qf = queries(rng, (3, Hq, D), "bf16")
+    n = ints([0, 1, 0])
+    got = host(c.attend(0, q, 2, new=n))
+    ref = OP.sdpa_int4_paged(qf, [host(x[0]) for x in c.tensors()], host(c.block_tables), [40, 34, 7], page, 2)
+    close(got, ref)
+
+
 # ---------------------------------------------------------------------------
 # prefixes whose sequences give pages up
 # ---------------------------------------------------------------------------
