@@ -6,6 +6,7 @@
 // the page a request gets does not depend on timing); the application copies
 // pages with every CU and rewrites table rows.
 #include "tq_internal.h"
+#include "tq_page_plan.h"
 
 #include <algorithm>
 
@@ -48,22 +49,23 @@ PlanWs plan_ws(void* ws, int64_t seqs, int64_t pages) {
 }
 
 // Exclusive prefix of v over the workgroup's threads, and their total.
-__device__ __forceinline__ int wg_scan(int v, int* lds, int& total) {
+template <typename T>
+__device__ __forceinline__ T wg_scan(T v, T* lds, T& total) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  int x = v;
+  T x = v;
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) {
-    const int y = __shfl_up(x, d, 64);
+    const T y = __shfl_up(x, d, 64);
     if (lane >= d) x += y;
   }
   __syncthreads();  // the last call's readers are done
   if (lane == 63) lds[wave] = x;
   __syncthreads();
-  int before = 0;
+  T before = 0;
   total = 0;
 #pragma unroll
   for (int w = 0; w < kPlanWaves; ++w) {
-    const int t = lds[w];
+    const T t = lds[w];
     before += w < wave ? t : 0;
     total += t;
   }
@@ -119,6 +121,7 @@ __device__ __forceinline__ unsigned group_ballot(bool c) {
 template <bool FORK>
 __global__ __launch_bounds__(kPlanThreads) void pages_plan_kernel(PlanParams p) {
   __shared__ int lds[kPlanWaves];
+  __shared__ PlanSum sums[kPlanWaves];
   constexpr int kGroups = kPlanThreads / kPlanGroup;
   const int lane = threadIdx.x % kPlanGroup, group = threadIdx.x / kPlanGroup;
   const int64_t rows = static_cast<int64_t>(p.max_pages) * p.page_size;
@@ -148,21 +151,19 @@ __global__ __launch_bounds__(kPlanThreads) void pages_plan_kernel(PlanParams p) 
     if (lane == 0) p.w.need[s] = need;
   }
   __syncthreads();
-  // (64 bits: the needs of many requests may exceed what any pool has)
-  int64_t want = 0;
+  PlanSum want = 0;
   for (int s0 = 0; s0 < p.seqs; s0 += kPlanThreads) {
     const int s = s0 + threadIdx.x;
-    const int need = s < p.seqs ? max(p.w.need[s], 0) : 0;
-    int total;
-    const int b = wg_scan(need, lds, total);
-    if (s < p.seqs) p.w.before[s] = static_cast<int>(min(want + b, static_cast<int64_t>(p.num_pages) + 1));
+    PlanSum total;
+    const PlanSum b = wg_scan<PlanSum>(s < p.seqs ? max(p.w.need[s], 0) : 0, sums, total);
+    if (s < p.seqs) p.w.before[s] = plan_before(want + b, p.num_pages);
     want += total;
   }
-  const int found = free_pages(p.refs, p.num_pages, static_cast<int>(min(want, static_cast<int64_t>(p.num_pages))), p.w.list, lds);
+  const int found = free_pages(p.refs, p.num_pages, static_cast<int>(min(want, static_cast<PlanSum>(p.num_pages))), p.w.list, lds);
   __syncthreads();
   for (int s = FORK ? threadIdx.x : group; s < p.seqs; s += FORK ? kPlanThreads : kGroups) {
     const int need = p.w.need[s], before = p.w.before[s], ask = p.ask[s];
-    const bool ok = need == 0 || (need > 0 && need <= found - before);
+    const bool ok = plan_grants(need, before, found);
     if (FORK || lane == 0) p.granted[s] = ok;
     if (!ok) continue;
     if constexpr (FORK) {
@@ -191,7 +192,7 @@ __global__ __launch_bounds__(kPlanThreads) void pages_plan_kernel(PlanParams p) 
   }
   if constexpr (FORK) {
     // granted requests for a page are the first `found` in order, all or none
-    if (threadIdx.x == 0) *p.w.n_jobs = static_cast<int>(min(want, static_cast<int64_t>(found)));
+    if (threadIdx.x == 0) *p.w.n_jobs = static_cast<int>(min(want, static_cast<PlanSum>(found)));
   }
 }
 

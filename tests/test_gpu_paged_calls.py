@@ -173,3 +173,22 @@ def test_prefix_table_refusals(pg):
     for bad in (t[0], t[0, :0], t[0, :1].long(), t[0, :1].cpu(), t[:, :1]):
         with pytest.raises(ValueError, match="prefix_table"):
             pg.sdpa_int4_paged(q, *d, t, n, 2, shared_prefix=32, prefix_table=bad)
+
+
+# ---------------------------------------------------------------------------
+# page plans
+# ---------------------------------------------------------------------------
+
+def test_reserve_of_more_pages_than_32_bits_count(pg):
+    """1,024 neighbours that need 2^31 pages together (tables of 8 GiB, all empty): the
+    first request is small and granted, the others are refused, and nothing else
+    changes."""
+    S, width, page, N = 1024, (1 << 21) + 2, 32, 9
+    t = torch.full((S, width), -1, dtype=torch.int32, device="cuda")
+    r, n = ints([1, 0, 1] + [0] * 6), ints([0] * S)
+    ask = torch.full((S,), width * page, dtype=torch.int32, device="cuda")
+    ask[0], ask[1] = 33, 0
+    got = host(pg.kv_pages_reserve(t, r, n, ask, page))
+    assert got[0] == 1 and not got[1:].any()
+    assert host(r).tolist() == [1, 1, 1, 1] + [0] * 5 and host(t[0, :3]).tolist() == [1, 3, -1]
+    assert int(t[0, 2:].max()) == -1 and int(t[1:].amax(1).max()) == -1

@@ -1,6 +1,8 @@
 """CPU: calls of the paged cache beside those of ``test_paged_host.py``: refusals
 before any GPU work, the arithmetic of the page plans, the Python layer."""
 import ctypes
+import os
+import subprocess
 
 import numpy as np
 import pytest
@@ -71,3 +73,13 @@ def test_prefix_call_refuses_bad_arguments_on_the_host(over, status, needle):
 
 def test_prefix_call_with_nothing_to_do_is_no_error():
     assert prefix(B=0, q=NULL, table=NULL)[0] == 0
+
+
+# ---------------------------------------------------------------------------
+# page plans
+# ---------------------------------------------------------------------------
+
+def test_plans_of_more_pages_than_32_bits_count():
+    r = subprocess.run([os.path.join(os.path.dirname(__file__), "cpp", "test_page_plan")], capture_output=True, text=True,
+                       timeout=60)
+    assert r.returncode == 0 and r.stdout.count("PASS") == 6, r.stdout + r.stderr
