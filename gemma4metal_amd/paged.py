@@ -9,7 +9,8 @@ is one growing array per layer (``engine/gemma4_multilayer.cpp:230-249``).
 
 As in ``turboquant.py``, torch holds device memory and streams; every
 computation runs in ``libturboquant_hip.so``.  Tensors of one call lie on one
-device, which need not be the current one.
+device, which need not be the current one.  Every function also takes
+``stream=`` (a ``torch.cuda.Stream`` of that device; the current one by default).
 
 Workspaces are cached per (device, stream).  Calls captured into HIP graphs
 that may be replayed at the same time need a ``workspace=`` each (uint8,
@@ -19,6 +20,7 @@ from __future__ import annotations
 
 import ctypes
 import functools
+import inspect
 from typing import Optional, Union
 
 import torch
@@ -53,18 +55,24 @@ def _workspace(ws: Optional[torch.Tensor], nbytes: int, device: torch.device, st
 def _placed(fn):
     """Runs fn with its first tensor's device, and ``stream=`` where given,
     current: launches, allocations and the capture state all go by those."""
+    sig = inspect.signature(fn)
+    name = next(iter(sig.parameters))
+
     @functools.wraps(fn)
-    def run(first, *args, stream=None, **kw):
+    def run(*args, stream=None, **kw):
+        first = args[0] if args else kw.get(name)
         t = first[0] if isinstance(first, (list, tuple)) and first else first
         if isinstance(t, torch.Tensor) and t.is_cuda:
             if stream is not None:
                 _need(stream.device == t.device, "stream must be on the tensors' device")
                 with torch.cuda.stream(stream):
-                    return fn(first, *args, **kw)
+                    return fn(*args, **kw)
             if t.device.index != torch.cuda.current_device():
                 with torch.cuda.device(t.device):
-                    return fn(first, *args, **kw)
-        return fn(first, *args, **kw)
+                    return fn(*args, **kw)
+        return fn(*args, **kw)
+    extra = inspect.Parameter("stream", inspect.Parameter.KEYWORD_ONLY, default=None, annotation=Optional[torch.cuda.Stream])
+    run.__signature__ = sig.replace(parameters=[*sig.parameters.values(), extra])
     return run
 
 

@@ -192,3 +192,22 @@ def test_reserve_of_more_pages_than_32_bits_count(pg):
     assert got[0] == 1 and not got[1:].any()
     assert host(r).tolist() == [1, 1, 1, 1] + [0] * 5 and host(t[0, :3]).tolist() == [1, 3, -1]
     assert int(t[0, 2:].max()) == -1 and int(t[1:].amax(1).max()) == -1
+
+
+def test_named_arguments_and_a_stream(pg):
+    rng = np.random.default_rng(3)
+    Hq, Hkv, D, page = 4, 2, 128, 32
+    names = ("k_quant", "k_scales", "k_biases", "v_quant", "v_scales", "v_biases")
+    d = dict(zip(names, map(dev, make_pool(rng, 4, Hkv, page, D, "f16"))))
+    q = queries(rng, (1, Hq, D), "bf16")[0]
+    t, n = ints([[2, 0, 3]]), ints([80])
+    want = pg.sdpa_int4_paged(q, *d.values(), t, n, 2)
+    s = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for stream in (None, s):
+        got = pg.sdpa_int4_paged(queries=q, **d, block_tables=t, seq_lens=n, gqa_factor=2, stream=stream)
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)
+    pg.kv_pages_free(block_tables=t, refs=ints([1] * 4), lengths=n, which=ints([1]), stream=s)
+    s.synchronize()
+    assert host(t).tolist() == [[-1] * 3] and host(n).tolist() == [0]

@@ -1,6 +1,7 @@
 """CPU: calls of the paged cache beside those of ``test_paged_host.py``: refusals
 before any GPU work, the arithmetic of the page plans, the Python layer."""
 import ctypes
+import inspect
 import os
 import subprocess
 
@@ -83,3 +84,31 @@ def test_plans_of_more_pages_than_32_bits_count():
     r = subprocess.run([os.path.join(os.path.dirname(__file__), "cpp", "test_page_plan")], capture_output=True, text=True,
                        timeout=60)
     assert r.returncode == 0 and r.stdout.count("PASS") == 6, r.stdout + r.stderr
+
+
+# ---------------------------------------------------------------------------
+# the Python layer
+# ---------------------------------------------------------------------------
+
+FUNCTIONS = ["kv_append_int4_paged", "sdpa_int4_paged", "sdpa_int4_paged_prefill", "kv_pages_reserve",
+             "kv_pages_advance", "kv_pages_fork", "kv_pages_free", "kv_pages_evict", "kv_pages_compact", "kv_pages_copy"]
+
+
+@pytest.mark.parametrize("name", FUNCTIONS)
+def test_every_argument_can_be_named(name):
+    """Also the first: the call reaches the function's own checks (of host tensors)."""
+    import torch
+    from gemma4metal_amd import paged
+    fn = getattr(paged, name)
+    params = inspect.signature(fn).parameters
+    assert params["stream"].kind is inspect.Parameter.KEYWORD_ONLY
+    t = torch.zeros(1, dtype=torch.int32)
+    args = {n: 32 if n in ("page_size", "sliding_window", "gqa_factor", "n_prior") else [t] * 6 if n == "pages" else t
+            for n, p in params.items() if p.default is inspect.Parameter.empty}
+    assert list(args) == list(params)[:len(args)]
+    for call in (lambda: fn(**args), lambda: fn(*args.values()),
+                 lambda: fn(*list(args.values())[:1], **dict(list(args.items())[1:]))):
+        with pytest.raises(ValueError, match="must be on a GPU device"):
+            call()
+    with pytest.raises(TypeError, match=list(args)[0]):
+        fn()
