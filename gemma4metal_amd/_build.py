@@ -58,7 +58,7 @@ def _compile(src: str) -> str:
     return obj
 
 
-CPP_TESTS = ["test_sdpa_int4", "test_paged", "test_page_plan"]
+CPP_TESTS = ["test_sdpa_int4", "test_paged", "test_page_plan", "test_paged_calls"]
 CPP_TEST_DIR = os.path.join(os.path.dirname(HERE), "tests", "cpp")
 
 

@@ -452,18 +452,19 @@ array sdpa_int4_paged(const array& queries, const kv_pages& pages, const array& 
   const int64_t reach = static_cast<int64_t>(t.width) * d.page;
   need(max_kv_len >= 0 || reach <= INT32_MAX, "block_tables reach past 32 bits");
   const int n = max_kv_len < 0 ? static_cast<int>(reach) : max_kv_len;
+  need(shared_prefix >= 0 && d.page > 0, "sdpa_int4_paged: bad shared_prefix or page_size");
+  const int32_t* lens = ints(seq_lens, {t.seqs}, "seq_lens");
+  const int32_t* wins = windows.ndim() > 0 ? ints(windows, {t.seqs}, "windows") : nullptr;
+  const int32_t* prefix =
+      prefix_table.ndim() > 0 ? ints(prefix_table, {shared_prefix / d.page}, "prefix_table") : nullptr;
   array out = array::empty({t.seqs, Hq, d.D}, Dtype::float32);
   size_t have = 0;
   void* ws = workspace(tq_sdpa_int4_paged_workspace_size(t.seqs, Hq, d.Hkv, d.D, n, shared_prefix), &have, s);
-  need(shared_prefix >= 0 && d.page > 0, "sdpa_int4_paged: bad shared_prefix or page_size");
   check(tq_sdpa_int4_paged_prefix(
             queries.data(), c_dtype(queries.dtype()), words(pages.k_quant), pages.k_scales.data(),
             pages.k_biases.data(), words(pages.v_quant), pages.v_scales.data(), pages.v_biases.data(),
             d.sb, static_cast<float*>(out.data()), t.seqs, Hq, d.Hkv, d.D, d.page, d.pages, t.p,
-            t.width, ints(seq_lens, {t.seqs}, "seq_lens"),
-            windows.ndim() > 0 ? ints(windows, {t.seqs}, "windows") : nullptr, n, gqa_factor, scale,
-            sliding_window, num_sinks,
-            prefix_table.ndim() > 0 ? ints(prefix_table, {shared_prefix / d.page}, "prefix_table") : nullptr,
+            t.width, lens, wins, n, gqa_factor, scale, sliding_window, num_sinks, prefix,
             shared_prefix, ws, have, s),
         "sdpa_int4_paged");
   return out;
@@ -499,12 +500,13 @@ array kv_pages_reserve(array& block_tables, array& refs, const array& lengths, c
                        int page_size, StreamOrDevice s) {
   const Tables t = tables_of(block_tables);
   const int pages = page_count(refs);
+  const int32_t *n = ints(lengths, {t.seqs}, "lengths"), *ask = ints(n_new, {t.seqs}, "n_new");
   array granted = array::empty({t.seqs}, Dtype::int32);
   size_t have = 0;
   void* ws = workspace(tq_kv_pages_workspace_size(t.seqs, pages), &have, s, g_plan_ws);
-  check(tq_kv_pages_reserve(t.p, static_cast<int32_t*>(refs.data()), ints(lengths, {t.seqs}, "lengths"),
-                            ints(n_new, {t.seqs}, "n_new"), static_cast<int32_t*>(granted.data()),
-                            t.seqs, t.width, pages, page_size, ws, have, s),
+  check(tq_kv_pages_reserve(t.p, static_cast<int32_t*>(refs.data()), n, ask,
+                            static_cast<int32_t*>(granted.data()), t.seqs, t.width, pages, page_size,
+                            ws, have, s),
         "kv_pages_reserve");
   return granted;
 }
@@ -513,9 +515,11 @@ array kv_pages_advance(const array& block_tables, const array& refs, array& leng
                        const array& n_new, int page_size, StreamOrDevice s) {
   const Tables t = tables_of(block_tables);
   const int pages = page_count(refs);
+  int32_t* n = ints(lengths, {t.seqs}, "lengths");
+  const int32_t* k = ints(n_new, {t.seqs}, "n_new");
   array advanced = array::empty({t.seqs}, Dtype::int32);
-  check(tq_kv_pages_advance(t.p, ints(lengths, {t.seqs}, "lengths"), ints(n_new, {t.seqs}, "n_new"),
-                            static_cast<int32_t*>(advanced.data()), t.seqs, t.width, pages, page_size, s),
+  check(tq_kv_pages_advance(t.p, n, k, static_cast<int32_t*>(advanced.data()), t.seqs, t.width, pages,
+                            page_size, s),
         "kv_pages_advance");
   return advanced;
 }
@@ -524,13 +528,14 @@ array kv_pages_fork(kv_pages& pages, array& block_tables, array& refs, array& le
                     const array& parents, StreamOrDevice s) {
   const PoolDims d = pool_dims(pages, true);
   const Tables t = tables_of(block_tables);
+  int32_t *r = ints(refs, {d.pages}, "refs"), *n = ints(lengths, {t.seqs}, "lengths");
+  const int32_t* from = ints(parents, {t.seqs}, "parents");
   array granted = array::empty({t.seqs}, Dtype::int32);
   size_t have = 0;
   void* ws = workspace(tq_kv_pages_workspace_size(t.seqs, d.pages), &have, s, g_plan_ws);
-  check(tq_kv_pages_fork(SixPages(pages).p, d.sb, d.layers, d.Hkv, d.D, t.p,
-                         ints(refs, {d.pages}, "refs"), ints(lengths, {t.seqs}, "lengths"),
-                         ints(parents, {t.seqs}, "parents"), static_cast<int32_t*>(granted.data()),
-                         t.seqs, t.width, d.pages, d.page, ws, have, s),
+  check(tq_kv_pages_fork(SixPages(pages).p, d.sb, d.layers, d.Hkv, d.D, t.p, r, n, from,
+                         static_cast<int32_t*>(granted.data()), t.seqs, t.width, d.pages, d.page, ws,
+                         have, s),
         "kv_pages_fork");
   return granted;
 }
