@@ -211,3 +211,157 @@ def test_named_arguments_and_a_stream(pg):
     pg.kv_pages_free(block_tables=t, refs=ints([1] * 4), lengths=n, which=ints([1]), stream=s)
     s.synchronize()
     assert host(t).tolist() == [[-1] * 3] and host(n).tolist() == [0]
+
+
+# ---------------------------------------------------------------------------
+# precision
+# ---------------------------------------------------------------------------
+
+# Errors are taken relative to mag = sum_t w_t |v_t|, the attention of the values'
+# magnitudes: a rounding of a weight or of a partial sum is relative to that, while the
+# result itself may be as small as the values cancel.  2-norms over many outputs add
+# roundings as independent ones, each uniform within half a step (rms 0.29 of a step).
+#
+# Weights.  p s_v is held in two parts.  Decode, bf16 (8 bits): the first leaves at
+# most 2^-9, the second 2^-9 of that; 2^-18 at most, 0.23 of it as the rms of a product
+# of two uniform errors over a binade.  It multiplies nibbles 0..15 with s n = 2.7
+# sigma (rms; s = sigma / 3, n = 7.5 +- 3), |v| = 0.8 sigma: 0.23 2^-18 2.7 / 0.8 = 3e-6.
+# The offset of 128 that nibbles carry, 135 / 2.7 times their size, rounds the sums
+# at 2^-24 0.29 50 = 0.9e-6 a step of a wave, a few steps.  Tiles, fp16 (11 bits,
+# truncated, then rounded): 2^-10 and 2^-12 of that, 0.23 2^-22 of n - 8 and biases in
+# the same parts: 2e-7; a group whose V scales are 2^-9 of the largest has weights 19
+# bits above fp16's step: 0.29 2^-19 2.7 / 0.8 = 1.9e-6 where one key has all weight,
+# its root-mean-square over a row's keys otherwise.
+# Scores (scale 1 / sqrt D: |score| below 8 in the log2 domain).  fp32 roundings,
+# 2^-24 8 0.58 of them at most and 8 in a chain: 0.8e-6 of a weight, ln 2 times that;
+# decode's queries of 22 bits (D 512: 21): 4.5 2^-22 0.58 (twice that) sqrt(D) / sqrt(D)
+# = 0.6e-6 (1.2e-6).
+# In all 3.5e-6 for decode and 0.7e-6 for tiles; twice that is allowed.  A part that got
+# lost would be 2^-9 or 2^-11 of a weight, 60 times as much.
+DECODE, TILES = 2.0**-17, 1.5e-6
+
+
+def definition(q, pages, table, n_of, page, gqa, scale, window=0, sinks=0):
+    """Rows q [R, Hq, D] at positions n_of[r] - 1 of one sequence, in 64 bits: results,
+    and the same of the values' magnitudes."""
+    k, v, has = OP.rows(pages, table, page, max(n_of))
+    out = np.zeros((2,) + q.shape)
+    for h in range(q.shape[1]):
+        s = float(np.float32(scale)) * (q[:, h].astype(np.float64) @ k[h // gqa].T)
+        for r, n in enumerate(n_of):
+            s[r, ~(OP.visible(n, max(n_of), window, sinks) & has)] = -np.inf
+        p = np.exp(s - s.max(1, keepdims=True))
+        p /= p.sum(1, keepdims=True)
+        out[0, :, h], out[1, :, h] = p @ v[h // gqa], p @ np.abs(v[h // gqa])
+    return out
+
+
+def within(got, ref_mag, tol, what, dims=None):
+    d = slice(None) if dims is None else dims
+    ref, mag = ref_mag[0][..., d], ref_mag[1][..., d]
+    err = np.linalg.norm(got[..., d] - ref) / np.linalg.norm(mag)
+    assert np.isfinite(err) and err <= tol, f"{what}: {err:.3e} of the magnitudes, {tol:.1e} allowed"
+
+
+PRECISION = [(8, 4, 128, 32), (8, 1, 128, 64), (8, 4, 256, 64), (8, 1, 256, 32), (4, 2, 512, 64), (8, 1, 512, 128)]
+
+
+@pytest.mark.parametrize("sb,qt", [("f16", "bf16"), ("f32", "f32"), ("f16", "f32"), ("f32", "f16")])
+@pytest.mark.parametrize("Hq,Hkv,D,page", PRECISION)
+def test_precision(pg, Hq, Hkv, D, page, sb, qt):
+    """Decode, a shared prefix and a prompt, each to the error that its arithmetic has."""
+    rng = np.random.default_rng(Hq + D)
+    gqa, scale, P = Hq // Hkv, D**-0.5, 4 * 128
+    lens = [P + 1, P + 61, P + 128, 1777]
+    N = P // page + sum(-(-n // page) - P // page for n in lens)
+    tables = random_tables(rng, lens, page, N, -(-max(lens) // page), P // page)
+    pages = make_pool(rng, N, Hkv, page, D, sb)
+    d = [dev(p) for p in pages]
+    q, qf = queries(rng, (len(lens), Hq, D), qt)
+    refs = [definition(qf[b:b + 1], pages, tables[b], [n], page, gqa, scale) for b, n in enumerate(lens)]
+    for shared in (0, P):
+        got = host(pg.sdpa_int4_paged(q, *d, dev(tables), ints(lens), gqa, scale, shared_prefix=shared))
+        for b, n in enumerate(lens):
+            within(got[b:b + 1], refs[b], DECODE, f"decode of {n}, shared {shared}")
+    new, prior = 70, 1777 - 70
+    q, qf = queries(rng, (new, Hq, D), qt)
+    got = host(pg.sdpa_int4_paged_prefill(q, *d, dev(tables[3]), prior, gqa, scale))
+    within(got, definition(qf, pages, tables[3], range(prior + 1, 1778), page, gqa, scale), TILES, "prompt")
+
+
+def uneven_pool(rng, kind, N, Hkv, page, D, sb, table):
+    """A pool whose V scales are not of one size: of groups, of the first rows, of rows
+    in turn (N(0, 1) rows, their scales and biases times powers of two)."""
+    k = O.quantize_int4(O.rms_norm(rng.standard_normal((N, Hkv, page, D)).astype(np.float32)), sb)
+    x = rng.standard_normal((N, Hkv, page, D)).astype(np.float32)
+    first = [(table[t // page], t % page) for t in range(96)]
+    if kind == "first":  # zeros: the quantizer's least scale
+        for e, r in first:
+            x[e, :, r] = 0.0
+    w, *sbs = O.quantize_int4(x, "f32")
+    for y in sbs:
+        if kind.startswith("group"):
+            y[..., -1] *= np.float32(2.0**int(kind[5:]))
+        elif kind.startswith("all"):
+            y *= np.float32(2.0**int(kind[3:]))
+        elif kind == "spread":
+            y[..., 0] *= np.float32(2.0**30)
+            y[..., 1] *= np.float32(2.0**-30)
+        elif kind.startswith("rows"):
+            even, odd = map(int, kind[4:].split("/"))
+            y[:, :, ::2] *= np.float32(2.0**even)
+            y[:, :, 1::2] *= np.float32(2.0**odd)
+        elif kind == "zero":
+            for e, r in first:
+                y[e, :, r] = 0.0
+    return list(k) + [w] + [y.astype({"f16": np.float16, "f32": np.float32}[sb]) for y in sbs]
+
+
+UNEVEN = [("f16", "bf16", k) for k in ("group-8", "group-12", "group-16", "first", "zero", "rows-10/5", "all-14", "all10")] + \
+         [("f32", "f32", k) for k in ("group-8", "group-12", "group-40", "first", "zero", "spread", "rows-30/30", "all-30", "all30")]
+
+
+@pytest.mark.parametrize("sb,qt,kind", UNEVEN)
+@pytest.mark.parametrize("Hq,Hkv,D,page", [(8, 4, 128, 32), (4, 2, 256, 64), (8, 1, 512, 32)])
+def test_unlike_v_scales(pg, Hq, Hkv, D, page, sb, qt, kind):
+    """Each group of 64 values to its own magnitude, also where the scales of a tile or
+    of tiles are far apart."""
+    rng = np.random.default_rng(D + len(kind))
+    gqa, scale, P = Hq // Hkv, D**-0.5, 256
+    lens = [P + 190, P + 5, P + 77]
+    N = P // page + sum(-(-n // page) - P // page for n in lens)
+    tables = random_tables(rng, lens, page, N, -(-max(lens) // page), P // page)
+    pages = uneven_pool(rng, kind, N, Hkv, page, D, sb, tables[0])
+    d = [dev(p) for p in pages]
+    groups = [slice(g, g + 64) for g in range(0, D, 64)]
+    new, prior = 150, lens[0] - 150
+    q, qf = queries(rng, (new, Hq, D), qt)
+    got = host(pg.sdpa_int4_paged_prefill(q, *d, dev(tables[0]), prior, gqa, scale, 200, 70))
+    ref = definition(qf, pages, tables[0], range(prior + 1, lens[0] + 1), page, gqa, scale, 200, 70)
+    for g in groups:
+        within(got, ref, TILES, f"prompt, dims {g.start}", g)
+    q, qf = queries(rng, (len(lens), Hq, D), qt)
+    for shared in (0, P):
+        got = host(pg.sdpa_int4_paged(q, *d, dev(tables), ints(lens), gqa, scale, shared_prefix=shared))
+        for b, n in enumerate(lens):
+            ref = definition(qf[b:b + 1], pages, tables[b], [n], page, gqa, scale)
+            for g in groups:
+                within(got[b:b + 1], ref, DECODE, f"decode of {n}, shared {shared}, dims {g.start}", g)
+
+
+@pytest.mark.parametrize("sb,qt,kind", UNEVEN)
+@pytest.mark.parametrize("Hq,Hkv,D,page", [(66, 33, 128, 32), (66, 33, 256, 32)])
+def test_unlike_v_scales_128_rows(pg, Hq, Hkv, D, page, sb, qt, kind):
+    rng = np.random.default_rng(D + len(kind))
+    gqa, scale, new, prior = Hq // Hkv, D**-0.5, 301, 37
+    n = new + prior
+    N = -(-n // page)
+    table = random_tables(rng, [n], page, N, N)[0]
+    pages = uneven_pool(rng, kind, N, Hkv, page, D, sb, table)
+    q, qf = queries(rng, (new, Hq, D), qt)
+    got = host(pg.sdpa_int4_paged_prefill(q, *map(dev, pages), dev(table), prior, gqa, scale))
+    heads = [0, 1, Hq // 2, Hq - 1]
+    some = [x[:, [h // gqa for h in heads]] for x in pages]
+    ref = definition(qf[:, heads], some, table, range(prior + 1, n + 1), page, 1, scale)
+    for g in range(0, D, 64):
+        within(got[:, heads], ref, TILES, f"dims {g}", slice(g, g + 64))
