@@ -365,3 +365,193 @@ def test_unlike_v_scales_128_rows(pg, Hq, Hkv, D, page, sb, qt, kind):
     ref = definition(qf[:, heads], some, table, range(prior + 1, n + 1), page, 1, scale)
     for g in range(0, D, 64):
         within(got[:, heads], ref, TILES, f"dims {g}", slice(g, g + 64))
+
+
+# ---------------------------------------------------------------------------
+# long sequences: their pages come from a small pool, many times each
+# ---------------------------------------------------------------------------
+
+def keys_of(n, window, sinks):
+    """The keys that the query at n - 1 attends."""
+    if window <= 0 or n <= window:
+        return np.arange(n)
+    return np.concatenate([np.arange(min(sinks, n - window)), np.arange(n - window, n)])
+
+
+def counted(qf, pages, table, n, page, gqa, scale, window=0, sinks=0, heads=None):
+    """One query [Hq, D] in 64 bits by how often each row of the pool occurs."""
+    N = pages[0].shape[0]
+    t = keys_of(n, window, sinks)
+    e = table[t // page].astype(np.int64)
+    has = (e >= 0) & (e < N)
+    count = np.bincount((e * page + t % page)[has], minlength=N * page).astype(np.float64)
+    out = []
+    for h in range(qf.shape[0]) if heads is None else heads:
+        k, v = (O.dequantize(*(x[:, h // gqa].reshape(N * page, -1) for x in pages[i:i + 3])) for i in (0, 3))
+        s = float(np.float32(scale)) * (k @ qf[h].astype(np.float64))
+        p = count * np.exp(s - s[count > 0].max())
+        out.append((p / p.sum()) @ v)
+    return np.array(out)
+
+
+def alias_tables(rng, B, width, N):
+    t = rng.integers(0, N, (B, width)).astype(np.int32)
+    t[:, 1::97] = -1  # some missing
+    return t
+
+
+# (more than 64 blocks a wave: page numbers are loaded again in the loop.  Four waves a
+# workgroup, eight, D 512 without and with heads as columns; chunks of the host and the
+# device)
+@pytest.mark.parametrize("B,Hq,Hkv,D,n,sb", [
+    (1, 2, 1, 128, 3_100_013, "f16"), (1, 2, 1, 256, 3_100_013, "f32"), (1, 8, 1, 512, 3_100_013, "f16"),
+    (1, 2, 2, 512, 2_100_031, "f16"), (70, 8, 4, 256, 90_001, "f16"), (70, 16, 4, 128, 90_017, "f32"),
+    (70, 8, 1, 512, 90_000, "f32"), (70, 2, 1, 512, 60_033, "f32"), (64, 32, 16, 128, 45_000, "f16"),
+    (48, 32, 16, 256, 45_011, "f32"), (64, 64, 8, 512, 45_000, "f16"), (64, 16, 8, 512, 45_007, "f16")])
+def test_decode_of_many_blocks_a_wave(pg, B, Hq, Hkv, D, n, sb):
+    rng = np.random.default_rng(n)
+    page, N, gqa = 32, 500, Hq // Hkv
+    tables = alias_tables(rng, B, -(-n // page) + 1, N)
+    pages = make_pool(rng, N, Hkv, page, D, sb)
+    lens = [n] + [int(x) for x in rng.integers(n // 2, n, B - 1)]
+    q, qf = queries(rng, (B, Hq, D), "bf16")
+    d, t = [dev(p) for p in pages], dev(tables)
+    some = sorted({0, 1, B // 2, B - 1} & set(range(B)))
+    for W, sinks in ((0, 0), (n // 2 + 5, 77)):
+        got = host(pg.sdpa_int4_paged(q, *d, t, ints(lens), gqa, 0.7, W, sinks))
+        for b in some:
+            heads = sorted({0, Hq // 2, Hq - 1})
+            close(got[b, heads], counted(qf[b], pages, tables[b], lens[b], page, gqa, 0.7, W, sinks, heads), f"{b} W {W}")
+
+
+@pytest.mark.parametrize("Hq,Hkv,D,prior,new", [(66, 33, 256, 9000, 301), (66, 33, 128, 9000, 301), (64, 8, 512, 5000, 600),
+                                                (160, 160, 256, 6007, 65)])
+def test_prompts_of_many_tiles_a_workgroup(pg, Hq, Hkv, D, prior, new):
+    rng = np.random.default_rng(D + new)
+    page, N, gqa = 32, 60, Hq // Hkv
+    table = alias_tables(rng, 1, -(-(prior + new) // page), N)[0]
+    pages = make_pool(rng, N, Hkv, page, D, "f16")
+    q, qf = queries(rng, (new, Hq, D), "bf16")
+    d = [dev(p) for p in pages]
+    for W, sinks in ((0, 0), (4500, 130)):
+        got = host(pg.sdpa_int4_paged_prefill(q, *d, dev(table), prior, gqa, 0.7, W, sinks))
+        for i in (0, 31, new - 1):
+            heads = [0, Hq // 2, Hq - 1]
+            close(got[i, heads], counted(qf[i], pages, table, prior + i + 1, page, gqa, 0.7, W, sinks, heads), f"row {i}")
+
+
+@pytest.mark.parametrize("Hq,Hkv,D", [(66, 33, 256), (8, 1, 512), (8, 4, 128)])
+def test_prefixes_of_many_tiles_a_workgroup(pg, Hq, Hkv, D):
+    rng = np.random.default_rng(D)
+    page, N, gqa, B, P = 64, 60, Hq // Hkv, 150, 12800
+    tables = alias_tables(rng, B, P // page + 3, N)
+    tables[1:, :P // page] = tables[0, :P // page]
+    pages = make_pool(rng, N, Hkv, page, D, "f16")
+    lens = [P + int(x) for x in rng.integers(0, 3 * page, B)]
+    lens[4] = 77
+    q, qf = queries(rng, (B, Hq, D), "bf16")
+    got = host(pg.sdpa_int4_paged(q, *map(dev, pages), dev(tables), ints(lens), gqa, 0.7, shared_prefix=P))
+    for b in (0, 4, 149):
+        heads = [0, Hq // 2, Hq - 1]
+        close(got[b, heads], counted(qf[b], pages, tables[b], lens[b], page, gqa, 0.7, heads=heads), f"sequence {b}")
+
+
+@pytest.mark.parametrize("Hq,Hkv,D", [(2, 1, 128), (4, 2, 256), (8, 1, 512)])
+def test_positions_near_the_last(pg, Hq, Hkv, D):
+    """Tables that reach 2^31 - 2^16 rows: every call at their end."""
+    rng = np.random.default_rng(D)
+    page, N, gqa = 32, 40, Hq // Hkv
+    last = 2**31 - 2**16
+    tables = np.full((2, last // page), -1, np.int32)
+    tables[:, :8], tables[:, -64:] = rng.integers(0, 20, (2, 8)), rng.integers(0, 20, (2, 64))
+    tables[:, -2:] = [[20, 21], [22, 23]]
+    pages = make_pool(rng, N, Hkv, page, D, "f16")
+    d, t = [dev(p) for p in pages], dev(tables)
+    k, kf = queries(rng, (2, Hkv, 50, D), "bf16")
+    v, vf = queries(rng, (2, Hkv, 50, D), "bf16")
+    pos = [last - 40, last - 17]  # 10 and 33 rows fall behind the tables
+    pg.kv_append_int4_paged(k, v, *d, t, ints(pos))
+    for b in range(2):
+        m = last - pos[b]
+        OP.append(pages, kf[b:b + 1, :, :m], vf[b:b + 1, :, :m], tables[b:b + 1, -4:], [pos[b] - (last - 4 * page)], page, "f16")
+    for x, y in zip(d, pages):
+        assert np.array_equal(host(x).view(np.uint8), y.view(np.uint8))
+    q, qf = queries(rng, (2, Hq, D), "bf16")
+    lens, W, sinks = [last, last - 9], 1500, 200
+    want = np.array([counted(qf[b], pages, tables[b], lens[b], page, gqa, 0.7, W, sinks) for b in range(2)])
+    close(host(pg.sdpa_int4_paged(q, *d, t, ints(lens), gqa, 0.7, W, sinks)), want)
+    close(host(pg.sdpa_int4_paged(q, *d, t, ints(lens), gqa, 0.7, 0, sinks, windows=ints([W, W]))), want)
+    for b in range(2):
+        one = pg.sdpa_int4_paged(q[b:b + 1], *d, t[b:b + 1], ints(lens[b:b + 1]), gqa, 0.7, W, sinks)
+        close(host(one)[0], want[b])
+    many, mf = queries(rng, (70, Hq, D), "bf16")
+    got = host(pg.sdpa_int4_paged_prefill(many, *d, t[0], last - 70, gqa, 0.7, W, sinks))
+    for i in (0, 69):
+        close(got[i], counted(mf[i], pages, tables[0], last - 69 + i, page, gqa, 0.7, W, sinks))
+    # bookkeeping
+    n, r = ints([last - 40, last - 40]), ints(np.bincount(tables[tables >= 0], minlength=N))
+    t[1, -1] = -1
+    assert host(pg.kv_pages_reserve(t, r, n, ints([41, 40]), page)).tolist() == [0, 1]
+    assert host(pg.kv_pages_advance(t, r, n, ints([41, 40]), page)).tolist() == [0, 1]
+    assert host(n).tolist() == [last - 40, last]
+    before = host(t)
+    pg.kv_pages_evict(t, r, n, page, 100, 33)
+    e = np.arange(last // page, dtype=np.int64)
+    for b, length in enumerate((last - 40, last)):
+        gone = (e * page >= 33) & ((e + 1) * page <= length - 100)
+        assert np.array_equal(host(t[b]), np.where(gone, -1, before[b]))
+
+
+@pytest.mark.parametrize("Hq,Hkv,D,page", [(16, 1, 512, 64), (24, 1, 512, 32), (12, 1, 512, 32), (5, 1, 512, 64), (16, 1, 256, 64),
+                                           (7, 1, 256, 512), (32, 1, 128, 256), (12, 4, 128, 1024), (20, 2, 128, 128)])
+@pytest.mark.parametrize("sb", ["f16", "f32"])
+def test_other_head_ratios_and_page_sizes(pg, Hq, Hkv, D, page, sb):
+    rng = np.random.default_rng(Hq + page)
+    gqa, P = Hq // Hkv, 2 * page
+    lens = [P + 70, P, 33, 0, P + 3 * page - 1]
+    N = P // page + sum(max(-(-n // page) - P // page, 0) for n in lens)
+    tables = random_tables(rng, lens, page, N, P // page + 3, P // page)
+    pages = make_pool(rng, N, Hkv, page, D, sb)
+    spoil(pages, tables, lens, page)
+    d = [dev(p) for p in pages]
+    q, qf = queries(rng, (len(lens), Hq, D), "f16")
+    for W, sinks in ((0, 0), (100, 40)):
+        ref = OP.sdpa_int4_paged(qf, pages, tables, lens, page, gqa, 0.7, W, sinks)
+        for shared in (0, P):
+            close(host(pg.sdpa_int4_paged(q, *d, dev(tables), ints(lens), gqa, 0.7, W, sinks, shared_prefix=shared)), ref)
+        q2, qf2 = queries(rng, (37, Hq, D), "f32")
+        got = host(pg.sdpa_int4_paged_prefill(q2, *d, dev(tables[4]), lens[4] - 37, gqa, 0.7, W, sinks))
+        close(got, OP.sdpa_int4_paged_prefill(qf2, pages, tables[4], lens[4] - 37, page, gqa, 0.7, W, sinks))
+
+
+@pytest.mark.parametrize("Hq,Hkv,D", [(4, 2, 256), (8, 1, 512)])
+def test_shared_prefix_in_a_graph(pg, Hq, Hkv, D):
+    """Tiles and the joining decode, captured with a workspace of their own and replayed
+    between eager calls; the prefix's table, lengths and queries change in place."""
+    from gemma4metal_amd import _lib
+    rng = np.random.default_rng(D)
+    page, P, B, gqa = 64, 1024, 5, Hq // Hkv
+    lens = [P + int(x) for x in rng.integers(1, 200, B)]
+    N = 40 + 2 * P // page
+    tables = random_tables(rng, lens, page, N, P // page + 4, P // page)
+    other = rng.permutation(N)[:P // page].astype(np.int32)
+    pages = make_pool(rng, N, Hkv, page, D, "f16")
+    d, t, n, prefix = [dev(p) for p in pages], dev(tables), ints(lens), dev(tables[0, :P // page])
+    size = _lib.load().tq_sdpa_int4_paged_workspace_size(B, Hq, Hkv, D, tables.shape[1] * page, P)
+    ws = torch.zeros(size, dtype=torch.uint8, device="cuda")
+    q = queries(rng, (B, Hq, D), "bf16")[0]
+    call = lambda w: pg.sdpa_int4_paged(q, *d, t, n, gqa, shared_prefix=P, prefix_table=prefix, workspace=w)  # noqa: E731
+    call(ws)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call(ws)
+    for step in range(4):
+        q.copy_(queries(rng, (B, Hq, D), "bf16")[0])
+        n.copy_(ints([P + int(x) for x in rng.integers(1, 200, B)]))
+        prefix.copy_(dev(other if step % 2 else tables[0, :P // page]))
+        want = call(None).clone()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
