@@ -146,9 +146,8 @@ int set_workspace(PagedParams& p, void* workspace, size_t bytes, const WsLayout&
   return TQ_OK;
 }
 
-// Keys that the rows of a prompt's workgroup attend, about.
-int64_t prompt_keys(int n_prior, int n_new, int window, int sinks) {
-  const int64_t n = static_cast<int64_t>(n_prior) + (n_new + 1) / 2;
+// Keys that a prompt's workgroup attends that ends at position n, about.
+int64_t prompt_keys(int64_t n, int window, int sinks) {
   return window > 0 ? std::min<int64_t>(n, static_cast<int64_t>(window) + sinks + 64) : n;
 }
 
@@ -165,8 +164,8 @@ extern "C" size_t tq_sdpa_int4_paged_workspace_size(int batch, int num_heads, in
   const int gqa = num_heads / num_kv_heads;
   int splits = max_paged_splits(batch, num_heads, num_kv_heads, head_dim, max_kv_len);
   if (shared_prefix > 0)
-    splits += std::max(plan_paged_tiles(static_cast<int64_t>(batch) * gqa, num_kv_heads, head_dim, shared_prefix, false).splits,
-                       plan_paged_tiles(static_cast<int64_t>(batch) * gqa, num_kv_heads, head_dim, shared_prefix, true).splits);
+    splits += std::max(plan_paged_tiles(static_cast<int64_t>(batch) * gqa, num_kv_heads, head_dim, shared_prefix, shared_prefix, false).splits,
+                       plan_paged_tiles(static_cast<int64_t>(batch) * gqa, num_kv_heads, head_dim, shared_prefix, shared_prefix, true).splits);
   return ws_layout(batch, num_heads, head_dim, splits).total + kWsTail;
 }
 
@@ -212,7 +211,7 @@ int paged_decode(const void* q, int q_dtype, const uint32_t* k_quant, const void
   p.cus = pl.slots;
   TilesPlan tiles{0, 0};
   if (shared_prefix > 0)
-    tiles = plan_paged_tiles(static_cast<int64_t>(batch) * gqa_factor, num_kv_heads, head_dim, shared_prefix,
+    tiles = plan_paged_tiles(static_cast<int64_t>(batch) * gqa_factor, num_kv_heads, head_dim, shared_prefix, shared_prefix,
                              q_dtype == TQ_F32 && sb_dtype == TQ_F32);
   p.pre = tiles.splits;
   p.max_splits = pl.max_splits + p.pre;
@@ -283,7 +282,8 @@ extern "C" int tq_sdpa_int4_paged_plan(int batch, int num_heads, int num_kv_head
   if (chunk_keys) *chunk_keys = pl.chunk;
   if (shared_splits)
     *shared_splits = shared_prefix > 0 ? plan_paged_tiles(static_cast<int64_t>(batch) * (num_heads / num_kv_heads),
-                                                          num_kv_heads, head_dim, shared_prefix, false).splits
+                                                          num_kv_heads, head_dim, shared_prefix, shared_prefix,
+                                                          false).splits
                                        : 0;
   if (on_device) *on_device = pl.lpt ? 1 : 0;
   if (kernel && kernel_bytes > 0)
@@ -296,7 +296,7 @@ extern "C" size_t tq_sdpa_int4_paged_prefill_workspace_size(int num_heads, int n
   if (num_kv_heads < 1 || num_heads < num_kv_heads || n_prior < 0 || n_new < 1) return 0;
   // (a window only shortens the splits)
   const int splits = paged_tiles_max_splits(static_cast<int64_t>(n_new) * (num_heads / num_kv_heads), num_kv_heads,
-                                            head_dim, prompt_keys(n_prior, n_new, 0, 0));
+                                            head_dim, static_cast<int64_t>(n_prior) + (n_new + 1) / 2);
   return splits > 1 ? ws_layout(n_new, num_heads, head_dim, splits).total + kWsTail : 0;
 }
 
@@ -324,8 +324,9 @@ extern "C" int tq_sdpa_int4_paged_prefill(const void* q, tq_dtype q_dtype, const
   p.n = n_prior;
   const int64_t rows = static_cast<int64_t>(n_new) * gqa_factor;
   TQ_CHECK_ARG(rows < (int64_t{1} << 31) && (rows + 63) / 64 * num_kv_heads < (int64_t{1} << 31), "%s: grid too large", fn);
-  const TilesPlan tiles = plan_paged_tiles(rows, num_kv_heads, head_dim, prompt_keys(n_prior, n_new, sliding_window, num_sinks),
-                                           q_dtype == TQ_F32 && sb_dtype == TQ_F32);
+  const TilesPlan tiles = plan_paged_tiles(
+      rows, num_kv_heads, head_dim, prompt_keys(static_cast<int64_t>(n_prior) + (n_new + 1) / 2, sliding_window, num_sinks),
+      prompt_keys(static_cast<int64_t>(n_prior) + n_new, sliding_window, num_sinks), q_dtype == TQ_F32 && sb_dtype == TQ_F32);
   p.max_splits = tiles.splits;
   if (tiles.splits > 1)
     if (int r = set_workspace(p, workspace, workspace_bytes, ws_layout(n_new, num_heads, head_dim, tiles.splits), fn)) return r;

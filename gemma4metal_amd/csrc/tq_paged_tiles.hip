@@ -893,21 +893,34 @@ int paged_tiles_max_splits(int64_t rows, int Hkv, int D, int64_t keys) {
   return most_splits(tile_wgs(rows, Hkv, D == 512 ? 4 : 8), (keys + tile_keys(D) - 1) / tile_keys(D));
 }
 
-TilesPlan plan_paged_tiles(int64_t rows, int Hkv, int D, int64_t keys, bool all32) {
-  const int64_t tiles = (keys + tile_keys(D) - 1) / tile_keys(D), cus = target_wgs();
+TilesPlan plan_paged_tiles(int64_t rows, int Hkv, int D, int64_t keys, int64_t longest, bool all32) {
+  const int64_t tiles = (keys + tile_keys(D) - 1) / tile_keys(D), most = (longest + tile_keys(D) - 1) / tile_keys(D);
+  const int64_t cus = target_wgs();
   // A workgroup fills a CU, and costs its prologue, epilogue and part of the merge
-  // beside its tiles, about kFixed of them; a tile of 128 rows costs kTile8 eighths
-  // of one of 64 (5.9 us and 3.3 at D 256): the plan of least estimated time.
-  constexpr int64_t kFixed = 6, kTile8 = 14;
+  // beside its tiles; in eighths of a tile of 64 rows, a tile of 128 rows costs
+  // kTile[1], and the rest kFixed.  The plan of least estimated time: of the rounds of
+  // average workgroups, or of the longest one (a causal prompt's last rows).  64
+  // against 128 rows in us, bf16 queries and fp16 scales, D 128 (Hq 16 Hkv 8) and D 256
+  // (Hq 32 Hkv 16):
+  //   64 sequences over 32,768 shared keys    74 : 68     209 : 184   128 taken
+  //   prompt of 2,048 after 4,096            302 : 280    936 : 758   128
+  //   prompt of 512 after 4,096               78 : 73     211 : 191   128
+  //   prompt of 512 after 4,000, W 1,024      32 : 36      62 : 71     64
+  //   prompt of 1,024                         38 : 45      75 : 91     64
+  //   prompt of 67 after 4,001, W 1,024       19 : 24      34 : 42     64
+  // Of 180 such pairs (other heads, fp32 queries or scales) four take the slower one:
+  // by 3 to 4%, 6% and 10%, the last three of fp32 scales at D 256.
+  constexpr int64_t kTile[2] = {8, 13}, kFixed[2] = {48, 72};
   TilesPlan best{4, 1};
   int64_t least = INT64_MAX;
   // (D 256 with fp32 queries and scales: 100 registers spilled with 128 rows, 331
   // against 240 us over 32,768 shared keys; with one of them in 16 bits, none to 13
   // and 202 to 216 against 226 to 229)
   for (int rs = 4; rs <= (D == 512 || (D == 256 && all32) ? 4 : 8); rs += 4) {
-    const int64_t wgs = tile_wgs(rows, Hkv, rs);
+    const int64_t wgs = tile_wgs(rows, Hkv, rs), tile = kTile[rs / 8], fixed = kFixed[rs / 8];
     for (int s = 1; s <= most_splits(wgs, tiles); ++s) {
-      const int64_t cost = (wgs * s + cus - 1) / cus * ((tiles + s - 1) / s * (rs == 8 ? kTile8 : 8) + 8 * kFixed);
+      const int64_t cost = std::max((wgs * s + cus - 1) / cus * ((tiles + s - 1) / s * tile + fixed),
+                                    (most + s - 1) / s * tile + fixed);
       if (cost < least) {
         least = cost;
         best = {rs, s};

@@ -856,16 +856,16 @@ int launch_prefill_tiles(const SdpaParams& p, int D, int sb_dtype, hipStream_t s
 // The same for fp32 queries, 64 rows (tq_prefill_f32.hip).
 int launch_prefill_tiles_f32(const SdpaParams& p, int D, int sb_dtype, hipStream_t stream);
 // Rows of a paged sequence (prefill) or of a batch's shared prefix on K/V tiles
-// (all32: fp32 queries and scales)
-// (tq_paged_tiles.hip): the most workgroups that share a row's tiles, the plan, and
-// the launch; `partials`: leave (m, l, O) in slots 0 .. splits - 1 of the rows'
-// partials, else write the output.
+// (tq_paged_tiles.hip): the most workgroups that share a row's tiles; the plan for rows
+// that attend `keys` keys on average and `longest` at most (all32: fp32 queries and
+// scales); and the launch (`partials`: leave (m, l, O) in slots 0 .. splits - 1 of the
+// rows' partials, else write the output).
 int paged_tiles_max_splits(int64_t rows, int Hkv, int D, int64_t keys);
 struct TilesPlan {
   int rs;      // 16-row sets of a workgroup
   int splits;  // workgroups along the tiles
 };
-TilesPlan plan_paged_tiles(int64_t rows, int Hkv, int D, int64_t keys, bool all32);
+TilesPlan plan_paged_tiles(int64_t rows, int Hkv, int D, int64_t keys, int64_t longest, bool all32);
 int launch_paged_tiles(const PagedParams& p, int D, int sb_dtype, TilesPlan plan, bool partials, hipStream_t stream);
 // Merge of the split partials of a launch with ext_merge = 1 (batch b of
 // grid.y): tq_sdpa_hc.hip.

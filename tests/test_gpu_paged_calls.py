@@ -353,7 +353,7 @@ def test_unlike_v_scales(pg, Hq, Hkv, D, page, sb, qt, kind):
 @pytest.mark.parametrize("Hq,Hkv,D,page", [(66, 33, 128, 32), (66, 33, 256, 32)])
 def test_unlike_v_scales_128_rows(pg, Hq, Hkv, D, page, sb, qt, kind):
     rng = np.random.default_rng(D + len(kind))
-    gqa, scale, new, prior = Hq // Hkv, D**-0.5, 301, 37
+    gqa, scale, new, prior = Hq // Hkv, D**-0.5, 301, 200  # (more workgroups of 64 rows than compute units)
     n = new + prior
     N = -(-n // page)
     table = random_tables(rng, [n], page, N, N)[0]
@@ -425,7 +425,7 @@ def test_decode_of_many_blocks_a_wave(pg, B, Hq, Hkv, D, n, sb):
 
 
 @pytest.mark.parametrize("Hq,Hkv,D,prior,new", [(66, 33, 256, 9000, 301), (66, 33, 128, 9000, 301), (64, 8, 512, 5000, 600),
-                                                (160, 160, 256, 6007, 65)])
+                                                (160, 160, 256, 6007, 65), (33, 33, 256, 2000, 650)])
 def test_prompts_of_many_tiles_a_workgroup(pg, Hq, Hkv, D, prior, new):
     rng = np.random.default_rng(D + new)
     page, N, gqa = 32, 60, Hq // Hkv
