@@ -181,6 +181,27 @@ __device__ __forceinline__ SplitRange paged_range(const SdpaParams& p, const Pag
   return r;
 }
 
+// Queries of the paged decode kernels in fixed point, X = rint(q 2^-ex up), in steps
+// of 2^ex / pow2 with 2^ex above the row's largest.  Those of 16 bits fit whole: what
+// is rounded is below 2^-12 of the largest.  fp32 ones are stretched to `most`, the
+// largest X that the products take, which is 1 to 4 times as fine.  The score's factor
+// (a * log2 e) stays out of X, where it would round a 16-bit query too: score = X back.
+struct FixedQ {
+  int ex;
+  float up, back;
+  __device__ __forceinline__ int of(float q) const { return static_cast<int>(__builtin_rintf(ldexpf(q, -ex) * up)); }
+};
+
+__device__ __forceinline__ FixedQ fixed_q(float largest, bool q32, float pow2, float most, float scale_log2) {
+  FixedQ r{0, pow2, 0.0f};
+  if (largest > 0.0f) {
+    frexpf(largest, &r.ex);  // largest < 2^ex
+    if (q32) r.up = most / ldexpf(largest, -r.ex);
+  }
+  r.back = ldexpf(scale_log2 / r.up, r.ex);
+  return r;
+}
+
 // Job of a workgroup in a ragged launch with p.lpt set (at most 64
 // sequences).
 // - The chunk is chosen here, from the actual lengths (the host knows only

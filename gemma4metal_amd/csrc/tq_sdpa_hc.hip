@@ -186,7 +186,7 @@ __device__ __forceinline__ float hc_half(uint32_t w, int hi) {
 // block) as 21-bit fixed point per head, scattered into the block-diagonal B
 // images of the K.q products (bq_lds, whose off-diagonal blocks are zeroed
 // here), with the per-(head, group) sums of the fixed-point q (sh_qhat) and
-// the per-head exponent F (sh_F).  Thread t takes the 8-element chunks
+// the per-head factor (sh_sf).  Thread t takes the 8-element chunks
 // t + kNT i: a wave's 64 chunks are the 512 dims of one head, so the head's
 // maximum is a wave reduction, and a chunk is one word (8 dims) of one quant
 // group, whose three base-256 digits fill two whole dwords of one lane's B
@@ -231,10 +231,11 @@ __device__ __forceinline__ int group8_sum_i(int v) {
   return v;
 }
 
+// sh_sf: the factor of a score's sum of products (a power of two; PG: see FixedQ).
 // Ends with a barrier.
-template <int kNT>
+template <int kNT, bool PG = false>
 __device__ __forceinline__ void hc_q_build(const HcQ<kNT>& Q, const SdpaParams& p, uint4 (&bq_lds)[3][kHcNG][64],
-                                           float (&sh_qhat)[kHcG][kHcNG], int (&sh_F)[kHcG], int lane) {
+                                           float (&sh_qhat)[kHcG][kHcNG], float (&sh_sf)[kHcG], int lane) {
   constexpr int NG = kHcNG;
   {
     // the off-diagonal blocks of the B images stay zero: lane 16c + n of an
@@ -271,7 +272,7 @@ __device__ __forceinline__ void hc_q_build(const HcQ<kNT>& Q, const SdpaParams& 
         f = p.q_dtype == TQ_F16 ? __half2float(__ushort_as_half(static_cast<uint16_t>(h16)))
                                 : __uint_as_float(h16 << 16);
       }
-      qv[t] = f * p.scale_log2;
+      qv[t] = PG ? f : f * p.scale_log2;
       mx = fmaxf(mx, fabsf(qv[t]));
     }
     mx = wave_max_dpp(mx);
@@ -282,11 +283,13 @@ __device__ __forceinline__ void hc_q_build(const HcQ<kNT>& Q, const SdpaParams& 
     // 2^21 < 2^31) is exact in int32
     const int F = 21 - ex;
     const float up = ldexpf(1.0f, F);
+    FixedQ fx{};
+    if constexpr (PG) fx = fixed_q(mx, p.q_dtype == TQ_F32, 0x1p21f, 2236000.0f, p.scale_log2);  // (64 * 15 * 2,236,000 < 2^31)
     uint32_t ev[3] = {0u, 0u, 0u}, od[3] = {0u, 0u, 0u};
     int xs = 0;
 #pragma unroll
     for (int t = 0; t < 8; ++t) {
-      const int X = static_cast<int>(__builtin_rintf(qv[t] * up));
+      const int X = PG ? fx.of(qv[t]) : static_cast<int>(__builtin_rintf(qv[t] * up));
       xs += X;
       const int d0 = static_cast<int8_t>(X & 0xFF);
       const int X1 = (X - d0) >> 8;
@@ -306,8 +309,8 @@ __device__ __forceinline__ void hc_q_build(const HcQ<kNT>& Q, const SdpaParams& 
     // per (head, quant group) sum of the fixed-point q over the group's 8
     // lanes, exact: 64 * 2^21 < 2^31
     xs = group8_sum_i(xs);
-    if (w == 0) sh_qhat[head][g] = static_cast<float>(xs) * ldexpf(1.0f, -F);
-    if (lane == 0) sh_F[head] = F;
+    if (w == 0) sh_qhat[head][g] = static_cast<float>(xs);
+    if (lane == 0) sh_sf[head] = PG ? fx.back : ldexpf(1.0f, -F);
   }
   __syncthreads();
 }
@@ -335,7 +338,7 @@ void sdpa_int4_hc_kernel(SdpaParams p) {
   __shared__ uint4 bq_lds[3][NG][64];           // K MFMA B operands [digit][2 pair + half][lane]
   __shared__ uint32_t sc_lds[NW][4][NG][16];    // [wave][array][group][key pair] fp16 x 2
   __shared__ float sh_qhat[G][NG];
-  __shared__ int sh_F[G];
+  __shared__ float sh_sf[G];
 
   const int64_t row0 = (static_cast<int64_t>(cache_batch(p, b)) * p.Hkv + kvh) * p.cap;
   const char* kq_rows = reinterpret_cast<const char*>(p.kq + row0 * (D / 8));
@@ -363,12 +366,12 @@ void sdpa_int4_hc_kernel(SdpaParams p) {
   __builtin_amdgcn_sched_barrier(0);
 
   // ---- prologue: q of the 8 heads as 21-bit fixed point, B images in LDS --
-  hc_q_build<kNT>(Q, p, bq_lds, sh_qhat, sh_F, lane);
-  const float sf = ldexpf(1.0f, -sh_F[hh]);
+  hc_q_build<kNT>(Q, p, bq_lds, sh_qhat, sh_sf, lane);
+  const float sf = sh_sf[hh];
   // q sums of this lane's column: head hh, group 2P + m / 8 of pair P
   float qh[NG / 2];
 #pragma unroll
-  for (int P = 0; P < NG / 2; ++P) qh[P] = sh_qhat[hh][2 * P + (m >> 3)] * ldexpf(1.0f, sh_F[hh]);
+  for (int P = 0; P < NG / 2; ++P) qh[P] = sh_qhat[hh][2 * P + (m >> 3)];
 
   // ---- main loop ----------------------------------------------------------
   float m_run = -INFINITY, l_run = 0.0f;
@@ -636,7 +639,8 @@ void sdpa_int4_hc2_kernel(ParamsOf<PG> p) {
   // the P . V operand slots during the loop; after it, the streams' partial
   // outputs [stream][head][D + 4] (rows padded by 16 bytes, so the 8 heads'
   // rows start in different LDS banks)
-  constexpr int kPvWords = 2 * NS * 4 * 2 * 64 * 4;  // [slot][stream][blk][hi/lo][lane] x uint4
+  constexpr int kParts = PG && F32 ? 3 : 2;  // of a weight
+  constexpr int kPvWords = 2 * NS * 4 * kParts * 64 * 4;  // [slot][stream][blk][part][lane] x uint4
   constexpr int kRow = D + 4;
   constexpr int kOWords = NS * G * kRow;
   constexpr int kArenaWords = kOWords > kPvWords ? kOWords : kPvWords;
@@ -650,7 +654,7 @@ void sdpa_int4_hc2_kernel(ParamsOf<PG> p) {
   __shared__ float f_lds[2][NS][16];          // rescale factor per column, by slot
   __shared__ float off_lds[NS][4][16];        // final offset per (block, column)
   __shared__ float sh_qhat[G][NG];
-  __shared__ int sh_F[G];
+  __shared__ float sh_sf[G];
 
   const int64_t row0 = PG ? 0 : (static_cast<int64_t>(cache_batch(p, b)) * p.Hkv + kvh) * p.cap;
   const char* kq_rows = reinterpret_cast<const char*>(p.kq + row0 * (D / 8));
@@ -724,15 +728,17 @@ void sdpa_int4_hc2_kernel(ParamsOf<PG> p) {
     hc_load_kw(kA, kq_rows, cur.row, cur.lim, m, c);
     hc_load_sc<F32>(sA, sc_rows, cur.row, cur.lim, m);
     __builtin_amdgcn_sched_barrier(0);
-    hc_q_build<kNT>(Q, p, bq_lds, sh_qhat, sh_F, lane);
-    const float sf = ldexpf(1.0f, -sh_F[hh]);
+    hc_q_build<kNT, PG>(Q, p, bq_lds, sh_qhat, sh_sf, lane);
+    const float sf = sh_sf[hh];
     float qh[NG / 2];
 #pragma unroll
-    for (int P = 0; P < NG / 2; ++P) qh[P] = sh_qhat[hh][2 * P + (m >> 3)] * ldexpf(1.0f, sh_F[hh]);
+    for (int P = 0; P < NG / 2; ++P) qh[P] = sh_qhat[hh][2 * P + (m >> 3)];
 
     float m_run = -INFINITY, l_run = 0.0f;
-    // the mean nibble of a weight whole, as in sdpa_int4_mfma_kernel
-    constexpr bool kMean = PG && F32;
+    // the mean nibble of a weight whole (fp32 scales: a third part), and a smaller
+    // offset of the nibbles, as in sdpa_int4_mfma_kernel
+    constexpr bool kMean = PG && !F32;
+    constexpr float kOffset = PG ? 16.0f : 128.0f;
     float wsum[4], bacc[4];
 #pragma unroll
     for (int blk = 0; blk < 4; ++blk) wsum[blk] = bacc[blk] = 0.0f;
@@ -910,7 +916,7 @@ void sdpa_int4_hc2_kernel(ParamsOf<PG> p) {
         // and lo = w - hi, each pair by one packed conversion; the weight
         // sum of the 128 offset takes a word per v_dot2 with (1, 1); the
         // fp16 scales convert inside the multiplies (fma with + 0)
-        uint32_t bh[4], bl[4];
+        uint32_t bh[4], bl[4], bt[4];
         const v2bf ones = __builtin_bit_cast(v2bf, 0x3F803F80u);
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
@@ -924,6 +930,11 @@ void sdpa_int4_hc2_kernel(ParamsOf<PG> p) {
               __builtin_bit_cast(uint32_t, v2bf{static_cast<__bf16>(w0 - h0), static_cast<__bf16>(w1 - h1)});
           bh[k] = hb;
           bl[k] = lb;
+          if constexpr (kParts == 3) {
+            const float l0 = __uint_as_float(lb << 16), l1 = __uint_as_float(lb & 0xFFFF0000u);
+            bt[k] = __builtin_bit_cast(uint32_t, v2bf{static_cast<__bf16>(w0 - h0 - l0), static_cast<__bf16>(w1 - h1 - l1)});
+            wsum[blk] = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(v2bf, bt[k]), ones, wsum[blk], false);
+          }
           wsum[blk] = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(v2bf, hb), ones, wsum[blk], false);
           wsum[blk] = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(v2bf, lb), ones, wsum[blk], false);
           bacc[blk] = fmaf(pw[j], vb[j >> 2][j & 3], bacc[blk]);
@@ -933,9 +944,10 @@ void sdpa_int4_hc2_kernel(ParamsOf<PG> p) {
             bacc[blk] = fmaf(7.5f, w1, bacc[blk]);
           }
         }
-        uint4* dst = pv_lds + (((slot * NS + s) * 4 + blk) * 2) * 64 + lane;
+        uint4* dst = pv_lds + (((slot * NS + s) * 4 + blk) * kParts) * 64 + lane;
         dst[0] = uint4{bh[0], bh[1], bh[2], bh[3]};
         dst[64] = uint4{bl[0], bl[1], bl[2], bl[3]};
+        if constexpr (kParts == 3) dst[128] = uint4{bt[0], bt[1], bt[2], bt[3]};
       }
       cur = nx;
     };
@@ -956,7 +968,7 @@ void sdpa_int4_hc2_kernel(ParamsOf<PG> p) {
       wsum[blk] = xor32_sum(wsum[blk]);
       bacc[blk] = xor16_sum(bacc[blk]);
       bacc[blk] = xor32_sum(bacc[blk]);
-      if (c == 0) off_lds[s][blk][m] = bacc[blk] - (kMean ? 135.5f : 128.0f) * wsum[blk];
+      if (c == 0) off_lds[s][blk][m] = bacc[blk] - (kOffset + (kMean ? 7.5f : 0.0f)) * wsum[blk];
     }
     if (c == 0 && m < 8) {
       ml_lds[0][s][hh] = m_run;
@@ -977,14 +989,15 @@ void sdpa_int4_hc2_kernel(ParamsOf<PG> p) {
       hc_load_v4(vA, vq_rows, b0.row, b0.lim, m, c);
     }
     __builtin_amdgcn_sched_barrier(0);
-    hc_q_build<kNT>(Q, p, bq_lds, sh_qhat, sh_F, lane);
+    hc_q_build<kNT, PG>(Q, p, bq_lds, sh_qhat, sh_sf, lane);
 
     v4f cv[4][8];  // [blk][2 byte + nibble half]
 #pragma unroll
     for (int blk = 0; blk < 4; ++blk)
 #pragma unroll
       for (int ff = 0; ff < 8; ++ff) cv[blk][ff] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-    uint32_t magic = 0x43004300u;  // bf16 of (128 + nibble)
+    // bf16 of (128 + nibble); PG: of (16 + nibble), as in sdpa_int4_mfma_kernel
+    uint32_t magic = PG ? 0x41804180u : 0x43004300u;
     asm volatile("" : "+v"(magic));
 
     // One step: this step's products, with the next step's V loads issued
@@ -1015,9 +1028,11 @@ void sdpa_int4_hc2_kernel(ParamsOf<PG> p) {
           hc_load_v4_blk(nx, vq_rows, bn.row, bn.lim, m, c, blk + 1);
           __builtin_amdgcn_sched_barrier(0);
         }
-        const uint4* src = pv_lds + (((slot * NS + s) * 4 + blk) * 2) * 64 + lane;
+        const uint4* src = pv_lds + (((slot * NS + s) * 4 + blk) * kParts) * 64 + lane;
         const v8bf bhi = __builtin_bit_cast(v8bf, src[0]);
         const v8bf blo = __builtin_bit_cast(v8bf, src[64]);
+        v8bf bthird;
+        if constexpr (kParts == 3) bthird = __builtin_bit_cast(v8bf, src[128]);
 #pragma unroll
         for (int by = 0; by < 4; ++by) {
           const uint32_t sel = static_cast<uint32_t>(by) | (0x0Cu << 8) |
@@ -1026,8 +1041,8 @@ void sdpa_int4_hc2_kernel(ParamsOf<PG> p) {
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
             const uint32_t x = __builtin_amdgcn_perm(vw[2 * r + 1], vw[2 * r], sel);
-            alo[r] = (x & 0x000F000Fu) | magic;
-            ahi[r] = ((x >> 4) & 0x000F000Fu) | magic;
+            alo[r] = PG ? ((x << 3) & 0x00780078u) | magic : (x & 0x000F000Fu) | magic;
+            ahi[r] = PG ? ((x >> 1) & 0x00780078u) | magic : ((x >> 4) & 0x000F000Fu) | magic;
           }
           const v8bf a_lo = __builtin_bit_cast(v8bf, u32x4{alo[0], alo[1], alo[2], alo[3]});
           const v8bf a_hi = __builtin_bit_cast(v8bf, u32x4{ahi[0], ahi[1], ahi[2], ahi[3]});
@@ -1035,6 +1050,10 @@ void sdpa_int4_hc2_kernel(ParamsOf<PG> p) {
           cv[blk][2 * by + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a_hi, bhi, cv[blk][2 * by + 1], 0, 0, 0);
           cv[blk][2 * by] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a_lo, blo, cv[blk][2 * by], 0, 0, 0);
           cv[blk][2 * by + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a_hi, blo, cv[blk][2 * by + 1], 0, 0, 0);
+          if constexpr (kParts == 3) {
+            cv[blk][2 * by] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a_lo, bthird, cv[blk][2 * by], 0, 0, 0);
+            cv[blk][2 * by + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a_hi, bthird, cv[blk][2 * by + 1], 0, 0, 0);
+          }
         }
       }
     };

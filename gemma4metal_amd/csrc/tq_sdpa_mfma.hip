@@ -380,7 +380,8 @@ void sdpa_int4_mfma_kernel(ParamsOf<PG> p) {
     load_iter<D, G, F32, kStreamNT>(bufA, kq_row0, vq_row0, sc_arr, lo, first_row(base0, pbA));
   __builtin_amdgcn_sched_barrier(0);
 
-  // ---- prologue: q as 22-bit fixed point per column set, B image per wave ---
+  // ---- prologue: q as 22-bit fixed point per column set (PG: see FixedQ), B image
+  // per wave ---
   // Each wave builds the whole image it reads, so no barrier orders the
   // prologue: a wave starts its stream as soon as its own q has arrived.
   // The digits equal those of one image shared by the workgroup (the
@@ -395,6 +396,7 @@ void sdpa_int4_mfma_kernel(ParamsOf<PG> p) {
     }
   }
   int Fs[NCH];
+  float backs[PG ? NCH : 1];
   float qhs[NCH];
 #pragma unroll
   for (int s = 0; s < NCH; ++s) {
@@ -422,7 +424,7 @@ void sdpa_int4_mfma_kernel(ParamsOf<PG> p) {
       }
     }
 #pragma unroll
-    for (int e = 0; e < 8; ++e) f[e] = ok ? f[e] * p.scale_log2 : 0.0f;
+    for (int e = 0; e < 8; ++e) f[e] = !ok ? 0.0f : PG ? f[e] : f[e] * p.scale_log2;
     float amax = 0.0f;
 #pragma unroll
     for (int e = 0; e < 8; ++e) amax = fmaxf(amax, fabsf(f[e]));
@@ -432,13 +434,16 @@ void sdpa_int4_mfma_kernel(ParamsOf<PG> p) {
     if (amax > 0.0f) frexpf(amax, &ex);  // amax < 2^ex
     const int F = 22 - ex;               // |round(q * 2^F)| <= 2^22
     const float sF = ldexpf(1.0f, F);
+    // (three signed base-256 digits reach 127 (65536 + 256 + 1) = 8,355,711)
+    FixedQ fx{};
+    if constexpr (PG) fx = fixed_q(amax, q32, 0x1p22f, 8355000.0f, p.scale_log2);
     // three signed base-256 digits per element: the low byte of X, then of
     // X1 = (X - sext(byte)) / 256, then of X2 = (X1 - sext(byte)) / 256
     uint32_t dg[3][8];
     int xs = 0;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const int X = static_cast<int>(__builtin_rintf(f[e] * sF));
+      const int X = PG ? fx.of(f[e]) : static_cast<int>(__builtin_rintf(f[e] * sF));
       xs += X;
       const int X1 = (X - __builtin_amdgcn_sbfe(X, 0, 8)) >> 8;
       const int X2 = (X1 - __builtin_amdgcn_sbfe(X1, 0, 8)) >> 8;
@@ -446,10 +451,11 @@ void sdpa_int4_mfma_kernel(ParamsOf<PG> p) {
       dg[1][e] = static_cast<uint32_t>(X1);
       dg[2][e] = static_cast<uint32_t>(X2);
     }
-    // sum over the quant group's 64 dims (8 lanes), exact: 64 * 2^22 < 2^31
+    // sum over the quant group's 64 dims (8 lanes), exact: 64 * 2^23 < 2^31
     xs = group_sum_i<8>(xs);
     Fs[s] = F;
-    qhs[s] = static_cast<float>(xs) * ldexpf(1.0f, -F);
+    if constexpr (PG) backs[s] = fx.back;
+    qhs[s] = static_cast<float>(xs) * (PG ? fx.back : ldexpf(1.0f, -F));
     // the low bytes of elements 0, 2, 4, 6 (even) and 1, 3, 5, 7 (odd) form
     // two dwords of the 16 k-slots of this chunk's MFMA, lane group and
     // column (three byte permutes per dword)
@@ -481,10 +487,12 @@ void sdpa_int4_mfma_kernel(ParamsOf<PG> p) {
     const int chn = col_used ? (hn * D + 64 * gn) / 8 : 0;
 #pragma unroll
     for (int s = 0; s < NCH; ++s) {
-      const int Fv = __shfl(Fs[s], chn & 63, 64);
+      float sv;
+      if constexpr (PG) sv = __shfl(backs[s], chn & 63, 64);
+      else sv = ldexpf(1.0f, -__shfl(Fs[s], chn & 63, 64));
       const float qv = __shfl(qhs[s], chn & 63, 64);
       if ((chn >> 6) == s && col_used) {
-        sf = ldexpf(1.0f, -Fv);
+        sf = sv;
         qhat = qv;
       }
     }
@@ -511,13 +519,16 @@ void sdpa_int4_mfma_kernel(ParamsOf<PG> p) {
 
   // ---- main loop ----------------------------------------------------------
   float m_run = -INFINITY, l_run = 0.0f, wsum = 0.0f, bacc = 0.0f;
-  constexpr bool kMean = PG && F32;  // see the weights' parts below
+  constexpr bool kMean = PG && !F32, kThird = PG && F32;  // see the weights' parts below
   v4f cv[VM];
 #pragma unroll
   for (int f = 0; f < VM; ++f) cv[f] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
   // bf16 magic of (128 + nibble), kept in a VGPR so each A-operand word is
-  // one v_and_or_b32 (a gfx9 VOP3 instruction takes at most one literal/SGPR)
-  uint32_t magic = 0x43004300u;
+  // one v_and_or_b32 (a gfx9 VOP3 instruction takes at most one literal/SGPR).
+  // PG: 16 + nibble, the nibble in bits 3-6, for a shift more: the sums are rounded at
+  // 24 times the nibbles' spread, not at 136 times.
+  constexpr float kOffset = PG ? 16.0f : 128.0f;
+  uint32_t magic = PG ? 0x41804180u : 0x43004300u;
   asm volatile("" : "+v"(magic));
 
   // The 4 staged scales of array a, group g, keys 16 * tile + 4c + {0..3}.
@@ -744,13 +755,17 @@ void sdpa_int4_mfma_kernel(ParamsOf<PG> p) {
     const v4f vs0 = scale4(2, gn, 0), vs1 = scale4(2, gn, 1);
     // Weights in bf16 pairs (slots 2k, 2k + 1: one B operand word), hi part
     // and lo = w - hi, each pair converted by one packed conversion; the
-    // weight sum of the 128 offset takes a word per v_dot2 with (1, 1).
-    uint32_t bh[4], bl[4];
+    // weight sum of the offset takes a word per v_dot2 with (1, 1).
+    uint32_t bh[4], bl[4], bt[4];
     const v2bf ones = __builtin_bit_cast(v2bf, 0x3F803F80u);
-    // 7.5, the mean nibble, of a weight whole: what its parts leave out (2^-18 of it)
-    // then only counts for nibbles' distances from that.  Paged fp32 scales: a
-    // weight of 1 is not exact in its parts, as it is with an fp16 scale (outputs off
-    // by 8e-6 of themselves without, 4e-6 with it).
+    // Two parts leave up to 2^-17 of a weight out, 2.4e-6 of it on average.  PG, fp16
+    // scales: 7.5, the mean nibble, of a weight whole, so that this counts only for
+    // nibbles' distances from that (results off by 2e-6 of themselves over many alike
+    // weights, 0.4e-6 to 1e-6 under a few large ones, whose parts are exact; 6e-6 and 1e-6
+    // to 5e-6 with neither this, the nibbles' smaller offset nor FixedQ).  A third part
+    // would make it 1e-6 for 3 to 10% of a call's time.  PG, fp32 scales, where no weight
+    // is exact in two: a third part, 0.5e-6 to 1.4e-6 instead of 3e-6 to 5e-6; 64
+    // sequences of 512 to 8,192 keys, Hq 32 Hkv 16 D 256, 259 us against 252.
     const float mean = PACK && T ? 0.0f : 7.5f;
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
@@ -767,6 +782,12 @@ void sdpa_int4_mfma_kernel(ParamsOf<PG> p) {
         bacc = fmaf(mean, w0, bacc);
         bacc = fmaf(mean, w1, bacc);
       }
+      if constexpr (kThird) {
+        const float l0 = __uint_as_float(lb << 16), l1 = __uint_as_float(lb & 0xFFFF0000u);
+        bt[k] = __builtin_bit_cast(uint32_t, v2bf{static_cast<__bf16>(w0 - h0 - l0), static_cast<__bf16>(w1 - h1 - l1)});
+        if (PACK && T) bt[k] = 0;
+        wsum = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(v2bf, bt[k]), ones, wsum, false);
+      }
       if constexpr (PACK) {
         // column n + 8T takes part T of the weight
         bh[k] = T ? lb : hb;
@@ -780,6 +801,7 @@ void sdpa_int4_mfma_kernel(ParamsOf<PG> p) {
     }
     const v8bf bhi = __builtin_bit_cast(v8bf, u32x4{bh[0], bh[1], bh[2], bh[3]});
     const v8bf blo = __builtin_bit_cast(v8bf, u32x4{bl[0], bl[1], bl[2], bl[3]});
+    const v8bf bthird = __builtin_bit_cast(v8bf, u32x4{bt[0], bt[1], bt[2], bt[3]});
 
     __builtin_amdgcn_sched_barrier(0);
     issue(std::integral_constant<int, 2>{});
@@ -795,8 +817,8 @@ void sdpa_int4_mfma_kernel(ParamsOf<PG> p) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const uint32_t x = __builtin_amdgcn_perm(B.vw[2 * r + 1][s], B.vw[2 * r][s], sel);
-          alo[r] = (x & 0x000F000Fu) | magic;
-          ahi[r] = ((x >> 4) & 0x000F000Fu) | magic;
+          alo[r] = PG ? ((x << 3) & 0x00780078u) | magic : (x & 0x000F000Fu) | magic;
+          ahi[r] = PG ? ((x >> 1) & 0x00780078u) | magic : ((x >> 4) & 0x000F000Fu) | magic;
         }
         const v4i ilo = v4i{static_cast<int>(alo[0]), static_cast<int>(alo[1]),
                             static_cast<int>(alo[2]), static_cast<int>(alo[3])};
@@ -810,6 +832,10 @@ void sdpa_int4_mfma_kernel(ParamsOf<PG> p) {
         if constexpr (!PACK) {
           cv[fe] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a_lo, blo, cv[fe], 0, 0, 0);
           cv[fo] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a_hi, blo, cv[fo], 0, 0, 0);
+        }
+        if constexpr (kThird) {
+          cv[fe] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a_lo, bthird, cv[fe], 0, 0, 0);
+          cv[fo] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a_hi, bthird, cv[fo], 0, 0, 0);
         }
       }
     }
@@ -882,7 +908,7 @@ void sdpa_int4_mfma_kernel(ParamsOf<PG> p) {
   }
   // packed: slot 2 * wave + T holds column n's part T (hi / lo)
   const int slot = PACK ? 2 * wave + T : wave;
-  const float corr = bacc - (kMean ? 135.5f : 128.0f) * wsum;  // bias term and the 128 offset
+  const float corr = bacc - (kOffset + (kMean ? 7.5f : 0.0f)) * wsum;  // bias term and the offset
   if (col_used) {
     // Accumulator element (s, j) of C row 4c + i is dim 8 * (VW * (4c + i) +
     // s) + j: for one (c, i) the 8 * VW dims are contiguous and lie in one

@@ -218,27 +218,35 @@ def test_named_arguments_and_a_stream(pg):
 # ---------------------------------------------------------------------------
 
 # Errors are taken relative to mag = sum_t w_t |v_t|, the attention of the values'
-# magnitudes: a rounding of a weight or of a partial sum is relative to that, while the
-# result itself may be as small as the values cancel.  2-norms over many outputs add
-# roundings as independent ones, each uniform within half a step (rms 0.29 of a step).
+# magnitudes (0.8 of sigma): a rounding of a weight or of a partial sum is relative to
+# that, while the result itself may be as small as the values cancel.  2-norms over many
+# outputs add roundings as independent ones, each uniform within half a step (rms 0.58
+# of half a step).
 #
-# Weights.  p s_v is held in two parts.  Decode, bf16 (8 bits): the first leaves at
-# most 2^-9, the second 2^-9 of that; 2^-18 at most, 0.23 of it as the rms of a product
-# of two uniform errors over a binade.  It multiplies nibbles 0..15 with s n = 2.7
-# sigma (rms; s = sigma / 3, n = 7.5 +- 3), |v| = 0.8 sigma: 0.23 2^-18 2.7 / 0.8 = 3e-6.
-# The offset of 128 that nibbles carry, 135 / 2.7 times their size, rounds the sums
-# at 2^-24 0.29 50 = 0.9e-6 a step of a wave, a few steps.  Tiles, fp16 (11 bits,
-# truncated, then rounded): 2^-10 and 2^-12 of that, 0.23 2^-22 of n - 8 and biases in
-# the same parts: 2e-7; a group whose V scales are 2^-9 of the largest has weights 19
-# bits above fp16's step: 0.29 2^-19 2.7 / 0.8 = 1.9e-6 where one key has all weight,
-# its root-mean-square over a row's keys otherwise.
-# Scores (scale 1 / sqrt D: |score| below 8 in the log2 domain).  fp32 roundings,
-# 2^-24 8 0.58 of them at most and 8 in a chain: 0.8e-6 of a weight, ln 2 times that;
-# decode's queries of 22 bits (D 512: 21): 4.5 2^-22 0.58 (twice that) sqrt(D) / sqrt(D)
-# = 0.6e-6 (1.2e-6).
-# In all 3.5e-6 for decode and 0.7e-6 for tiles; twice that is allowed.  A part that got
-# lost would be 2^-9 or 2^-11 of a weight, 60 times as much.
-DECODE, TILES = 2.0**-17, 1.5e-6
+# Weights.  Parts leave a remainder r, uniform within half a step, and the last part
+# rounds that: an error of half of r's own step, which halves with every halving of r.
+# - Decode, fp16 scales: two bf16 parts (8 bits), |r| <= 2^-8, |error| <= 2^-17, rms
+#   sqrt(1/3 1/2 / (1 - 1/8)) = 0.44 of that in the weight's octave, 0.31 of the weight:
+#   2.4e-6 of nibbles' distances from 7.5 (sigma), 3e-6 of mag for one key; but a
+#   weight of 1 is exact, and two of a half are off by 2.1e-6.  Many average out.
+# - Decode, fp32 scales: a third part, 2^-25.
+# - Tiles: two fp16 parts (11 bits, the first truncated), |r| <= 2^-10, |error| <=
+#   2^-22: 1.3e-7.  A group whose V scales are 2^-9 of the largest has weights of 2^-5
+#   there and a last step of 2^-24: 0.58 2^-20 = 5.5e-7, 0.7e-6 of mag for one key.
+# Decode's sums of (16 + n) s: 24 sigma / 3 = 8, 2^-24 8 0.58 = 0.3e-6 a step, 0.5e-6 over
+# the few that count.
+# Scores.  With scale 1 / sqrt D, |score| < 8 (log2 domain): 2^-24 8 0.58 of a rounding, 8
+# of them: 0.8e-6, ln 2 of that in a weight.  With scale 1, < 86: 2.2e-6 each, 4 of them at
+# that size, ln 2: 3e-6, of which p (1 - p) sqrt 2 <= 0.35 remain: 1e-6.
+# Decode's queries: exact of 16 bits but for a few far below the largest.  fp32 in steps
+# of 4.5 / 8.36e6: 0.29 sqrt D of that, 2.5e-6 (D 256), 3.5e-6 (D 512), 0.35 of it with
+# scale 1, 1 / sqrt D of it else; heads as columns (D 512, GQA 8) 4.5 / 2.24e6: 13e-6,
+# 4.6e-6 with scale 1, 0.6e-6 else.
+# In all: scale 1 / sqrt D: fp16 scales 2.3e-6, fp32 0.95e-6, tiles 0.9e-6; scale 1: 2.6e-6
+# (fp16), 1.7e-6 (fp32), heads as columns with fp32 queries 5.2e-6.  About 1.6 times that is
+# allowed.  A part that got lost would be 2^-9 of a weight or more.
+DECODE, DECODE_F32, TILES = 2.0**-18, 2.0**-19, 1.5e-6
+DECODE_ONE, DECODE_ONE_COLUMNS = 2.0**-18, 2.0**-17
 
 
 def definition(q, pages, table, n_of, page, gqa, scale, window=0, sinks=0):
@@ -278,11 +286,13 @@ def test_precision(pg, Hq, Hkv, D, page, sb, qt):
     pages = make_pool(rng, N, Hkv, page, D, sb)
     d = [dev(p) for p in pages]
     q, qf = queries(rng, (len(lens), Hq, D), qt)
-    refs = [definition(qf[b:b + 1], pages, tables[b], [n], page, gqa, scale) for b, n in enumerate(lens)]
-    for shared in (0, P):
-        got = host(pg.sdpa_int4_paged(q, *d, dev(tables), ints(lens), gqa, scale, shared_prefix=shared))
-        for b, n in enumerate(lens):
-            within(got[b:b + 1], refs[b], DECODE, f"decode of {n}, shared {shared}")
+    columns = D == 512 and gqa % 8 == 0 and qt == "f32"
+    for sc, tol in ((scale, DECODE if sb == "f16" else DECODE_F32), (1.0, DECODE_ONE_COLUMNS if columns else DECODE_ONE)):
+        refs = [definition(qf[b:b + 1], pages, tables[b], [n], page, gqa, sc) for b, n in enumerate(lens)]
+        for shared in (0, P):
+            got = host(pg.sdpa_int4_paged(q, *d, dev(tables), ints(lens), gqa, sc, shared_prefix=shared))
+            for b, n in enumerate(lens):
+                within(got[b:b + 1], refs[b], tol, f"decode of {n}, shared {shared}, scale {sc}")
     new, prior = 70, 1777 - 70
     q, qf = queries(rng, (new, Hq, D), qt)
     got = host(pg.sdpa_int4_paged_prefill(q, *d, dev(tables[3]), prior, gqa, scale))
@@ -346,7 +356,8 @@ def test_unlike_v_scales(pg, Hq, Hkv, D, page, sb, qt, kind):
         for b, n in enumerate(lens):
             ref = definition(qf[b:b + 1], pages, tables[b], [n], page, gqa, scale)
             for g in groups:
-                within(got[b:b + 1], ref, DECODE, f"decode of {n}, shared {shared}, dims {g.start}", g)
+                within(got[b:b + 1], ref, DECODE if sb == "f16" else DECODE_F32,
+                       f"decode of {n}, shared {shared}, dims {g.start}", g)
 
 
 @pytest.mark.parametrize("sb,qt,kind", UNEVEN)
@@ -555,3 +566,26 @@ def test_shared_prefix_in_a_graph(pg, Hq, Hkv, D):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("Hq,Hkv,D", [(2, 1, 128), (4, 2, 256), (4, 2, 512), (8, 1, 512)])
+@pytest.mark.parametrize("e", [-110, 100])
+@pytest.mark.parametrize("qt", ["bf16", "f32"])
+def test_queries_far_from_one(pg, Hq, Hkv, D, e, qt):
+    """Queries times 2^e under a scale of 2^-e / sqrt D are the queries themselves; one
+    row is 0, and attends all keys alike."""
+    rng = np.random.default_rng(D)
+    page, gqa, n = 32, Hq // Hkv, 200
+    table = random_tables(rng, [n], page, 9, 9)[0]
+    pages = make_pool(rng, 9, Hkv, page, D, "f32")
+    d, t = [dev(p) for p in pages], dev(table)
+    q, qf = queries(rng, (30, Hq, D), qt)
+    q[0, 0], qf[0, 0] = 0, 0
+    q = (q.float() * 2.0**e).to(q.dtype)  # exact: a power of two
+    scale = float(np.float32(D**-0.5)) * 2.0**-e
+    ref = definition(qf, pages, table, [n - 29 + i for i in range(30)], page, gqa, D**-0.5)
+    within(host(pg.sdpa_int4_paged_prefill(q, *d, t, n - 30, gqa, scale)), ref, TILES, "prompt")
+    lens = ints([n - 29 + i for i in range(30)])
+    for shared in (0, 96):
+        got = host(pg.sdpa_int4_paged(q, *d, t[None].expand(30, -1).contiguous(), lens, gqa, scale, shared_prefix=shared))
+        within(got, ref, DECODE_F32, f"decode, shared {shared}")
