@@ -956,10 +956,11 @@ void sdpa_int4_mfma_kernel(ParamsOf<PG> p) {
 
 template <int D, int G, bool F32>
 int launch_dgs(const PagedParams& p, dim3 grid, hipStream_t s) {
-  if (D == 512 || p.waves == 4)
-    sdpa_int4_mfma_kernel<D, G, 4, false, false, F32, true><<<grid, 4 * 64, 0, s>>>(p);
-  else
-    sdpa_int4_mfma_kernel<D, G, kMfmaWaves, false, false, F32, true><<<grid, kMfmaWaves * 64, 0, s>>>(p);
+  bool four = true;
+  if constexpr (D != 512) four = p.waves == 4;
+  if (four) sdpa_int4_mfma_kernel<D, G, 4, false, false, F32, true><<<grid, 4 * 64, 0, s>>>(p);
+  if constexpr (D != 512)
+    if (!four) sdpa_int4_mfma_kernel<D, G, kMfmaWaves, false, false, F32, true><<<grid, kMfmaWaves * 64, 0, s>>>(p);
   TQ_CHECK_LAUNCH("sdpa_int4_mfma_kernel");
   return TQ_OK;
 }
