@@ -9,6 +9,7 @@
 #include "tq_page_plan.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace tq {
 namespace {
@@ -121,7 +122,8 @@ __device__ __forceinline__ unsigned group_ballot(bool c) {
 template <bool FORK>
 __global__ __launch_bounds__(kPlanThreads) void pages_plan_kernel(PlanParams p) {
   __shared__ int lds[kPlanWaves];
-  __shared__ PlanSum sums[kPlanWaves];
+  using ScanSum = typename std::conditional<FORK, int, PlanSum>::type;  // (a fork needs one page at most)
+  __shared__ ScanSum sums[kPlanWaves];
   constexpr int kGroups = kPlanThreads / kPlanGroup;
   const int lane = threadIdx.x % kPlanGroup, group = threadIdx.x / kPlanGroup;
   const int64_t rows = static_cast<int64_t>(p.max_pages) * p.page_size;
@@ -154,8 +156,8 @@ __global__ __launch_bounds__(kPlanThreads) void pages_plan_kernel(PlanParams p) 
   PlanSum want = 0;
   for (int s0 = 0; s0 < p.seqs; s0 += kPlanThreads) {
     const int s = s0 + threadIdx.x;
-    PlanSum total;
-    const PlanSum b = wg_scan<PlanSum>(s < p.seqs ? max(p.w.need[s], 0) : 0, sums, total);
+    ScanSum total;
+    const ScanSum b = wg_scan<ScanSum>(s < p.seqs ? max(p.w.need[s], 0) : 0, sums, total);
     if (s < p.seqs) p.w.before[s] = plan_before(want + b, p.num_pages);
     want += total;
   }
