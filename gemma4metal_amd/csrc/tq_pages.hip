@@ -111,7 +111,7 @@ __device__ __forceinline__ int free_pages(const int32_t* refs, int num_pages, in
 // before each, the free pages, and the grants.  Chains of dependent loads bound it
 // (request, length, parent, table), so a sequence gets kPlanGroup lanes and 64
 // sequences are in flight: a fork of 56 sequences took 12 us with a wave a sequence,
-// 5.7 us so.
+// 6 us so.
 constexpr int kPlanGroup = 16;
 
 // Of the lanes of one's group, those with a condition.

@@ -186,7 +186,7 @@ __device__ __forceinline__ float half_hi(uint32_t w) {
 // (lane i: iteration i), so that a block's rows cost a v_readlane and scalar
 // arithmetic.  Blocks with masked keys (the sequence's end, the edges of window
 // and sinks, missing pages) lose those keys' scales and biases too.  64 sequences of
-// 512 to 16,384 keys, 16 kv heads of D 256: 425 us (HBM at 5.9 TB/s); 32 with a window
+// 512 to 16,384 keys, 16 kv heads of D 256: 427 us (HBM at 5.9 TB/s); 32 with a window
 // of 1,024 and 4 sinks: 31 us (4.7 TB/s).
 template <int D, int G, int NW, bool kQG, bool kStreamNT, bool F32, bool PG = false>
 __global__ __launch_bounds__(NW * 64)

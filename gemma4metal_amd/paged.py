@@ -13,8 +13,12 @@ device, which need not be the current one.  Every function also takes
 ``stream=`` (a ``torch.cuda.Stream`` of that device; the current one by default).
 
 Workspaces are cached per (device, stream).  Calls captured into HIP graphs
-that may be replayed at the same time need a ``workspace=`` each (uint8,
-zero-filled, at least the ``*_workspace_size`` bytes).
+that may be replayed at the same time, or beside eager calls of the stream that
+they were captured on, need a ``workspace=`` each (uint8, zero-filled, at least
+the ``*_workspace_size`` bytes).
+
+Attention is off by 0.2e-6 to 2e-6 of its result against 64 bits, as far as
+products in 32 bits are.
 """
 from __future__ import annotations
 

@@ -262,6 +262,9 @@ int tq_kv_append_int4_paged(const void* k_new, const void* v_new, tq_dtype x_dty
  * window that shorter sequences (or layers without the window) still attend; the
  * elementwise maximum of the sequences' rows then does.  Given that, it changes no
  * result beyond rounding.
+ * Against 64 bits a result is off by 0.4e-6 to 1.5e-6 of its sequence's 2-norm, with
+ * fp16 scales and many keys of like weight 2e-6 (weights are held in 16 bits there), as
+ * with fp32 queries of head_dim 512 where gqa_factor is a multiple of 8.
  * Workspace as for tq_sdpa_int4_ragged: at least
  * tq_sdpa_int4_paged_workspace_size(...) bytes, zero-filled once, left with its
  * counters zeroed; calls that may overlap (two streams, or two captured graphs
