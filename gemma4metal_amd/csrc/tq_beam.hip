@@ -1,0 +1,501 @@
+// Beam search: choosing the next beams from the logits, and reordering a contiguous
+// int4 cache by the beams chosen (paged caches: tq_pages.hip).
+#include "tq_internal.h"
+
+#include <math.h>
+
+#include <algorithm>
+
+namespace tq {
+namespace {
+
+// ---- choosing the next beams ------------------------------------------------
+// total(w, t) = score[w] + x[w][t] - log sum_t' exp x[w][t'], and of a group's W V
+// totals the K largest, the lowest (w, t) first among equals.
+//
+// One pass over the logits leaves the largest and the sum of exponentials of every
+// segment of kSeg tokens.  An element of the K best lies in one of the K segments
+// whose largest totals come first in the same order (the largest of K segments before
+// its own would all come before it), so that the second kernel reads K segments again
+// and nothing else: the work does not depend on the values, and no candidate list is
+// kept while streaming.  Totals are compared in 64 bits: beams are told apart by
+// scores of any distance, and equal ones have to be equal.
+constexpr int kSeg = 1024;
+constexpr int kMaxBeams = 64;
+
+struct SelectParams {
+  const void* x;
+  int64_t group_stride, beam_stride;  // elements
+  const float* scores;
+  const uint8_t* finished;
+  int groups, beams, vocab, num_out, pad, nseg;
+  float2* seg;  // [groups * beams][nseg]: largest, sum of exp(x - largest)
+  float* scores_out;
+  int32_t* parents_out;
+  int32_t* tokens_out;
+};
+
+template <typename T>
+__device__ __forceinline__ float to_f32(T v);
+template <>
+__device__ __forceinline__ float to_f32<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ float to_f32<_Float16>(_Float16 v) { return static_cast<float>(v); }
+template <>
+__device__ __forceinline__ float to_f32<uint16_t>(uint16_t v) { return bf16_to_f32(v); }
+
+// Whether a beam has candidates of its own (a score of -inf or NaN has none), and
+// whether it is finished: one candidate, the beam itself.
+__device__ __forceinline__ bool beam_alive(float score) { return score > -INFINITY; }
+
+// log2(e) in two parts: the product's constant error would be the same in every term.
+constexpr float kLog2eHi = 1.4426950216293335f, kLog2eLo = 1.925963033500011e-8f;
+
+// A wave a segment.  16-byte loads at the alignment of an element: what a lane sums
+// goes by the place in the row alone, so that equal rows give equal sums.
+template <typename T>
+__global__ __launch_bounds__(256) void beam_scan_kernel(SelectParams p) {
+  constexpr int E = 16 / sizeof(T), NV = kSeg / (64 * E);
+  const int lane = threadIdx.x & 63;
+  const uint32_t id = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);  // (below 2^31)
+  const int rows = p.groups * p.beams;
+  const int row = static_cast<int>(id / static_cast<uint32_t>(p.nseg)), j = static_cast<int>(id) - row * p.nseg;
+  if (row >= rows) return;
+  if (!beam_alive(p.scores[row]) || (p.finished && p.finished[row])) return;  // (nobody reads its segments)
+  const int b = row / p.beams, w = row - b * p.beams;
+  const T* x = static_cast<const T*>(p.x) + b * p.group_stride + w * p.beam_stride + static_cast<int64_t>(j) * kSeg;
+  const int n = min(p.vocab - j * kSeg, kSeg);
+  float v[NV][E];
+  if (n == kSeg) {
+    T raw[NV][E];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) __builtin_memcpy(raw[i], x + (64 * i + lane) * E, 16);
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int e = 0; e < E; ++e) v[i][e] = to_f32(raw[i][e]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const int at = (64 * i + lane) * E + e;
+        v[i][e] = at < n ? to_f32(x[at]) : -INFINITY;
+      }
+  }
+  float m = -INFINITY;  // (fmaxf passes NaN over)
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+#pragma unroll
+    for (int e = 0; e < E; ++e) m = fmaxf(m, v[i][e]);
+  m = wave_max_dpp(m);
+  float s = 0.0f;
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const float d = v[i][e] - m;
+      s += fast_exp2(fmaf(d, kLog2eLo, d * kLog2eHi));
+    }
+  if (__any(!(s < INFINITY))) {
+    // NaN counts as -inf, and of infinities the equal ones are 0 apart
+    s = 0.0f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const float d = v[i][e] - m;
+        s += v[i][e] == m ? (m > -INFINITY ? 1.0f : 0.0f) : d < 0.0f ? fast_exp2(fmaf(d, kLog2eLo, d * kLog2eHi)) : 0.0f;
+      }
+  }
+  s = group_sum<64>(s);
+  if (lane == 0) p.seg[static_cast<int64_t>(row) * p.nseg + j] = make_float2(m, s);
+}
+
+// A candidate: its total in an order of whole numbers (0: none), and its place.
+struct Cand {
+  uint64_t k;
+  uint32_t i;
+};
+__device__ __forceinline__ bool before(const Cand& a, const Cand& b) { return a.k > b.k || (a.k == b.k && a.i < b.i); }
+__device__ __forceinline__ Cand cand(double total, uint32_t i) {
+  const int64_t u = __double_as_longlong(total + 0.0);  // (-0 is 0)
+  const uint64_t k = static_cast<uint64_t>(u) ^ (u < 0 ? ~uint64_t{0} : uint64_t{1} << 63);
+  return total > -INFINITY ? Cand{k, i} : Cand{0, ~0u};
+}
+__device__ __forceinline__ double total_of(uint64_t k) {
+  return __longlong_as_double(static_cast<int64_t>(k >> 63 ? k ^ (uint64_t{1} << 63) : ~k));
+}
+__device__ __forceinline__ Cand shfl_xor_c(const Cand& c, int d) {
+  const uint32_t lo = shfl_xor_u(static_cast<uint32_t>(c.k), d), hi = shfl_xor_u(static_cast<uint32_t>(c.k >> 32), d);
+  return {static_cast<uint64_t>(hi) << 32 | lo, shfl_xor_u(c.i, d)};
+}
+
+constexpr int kPick = 1024;         // threads of the choice, and tokens of a segment
+constexpr int kGroup = 8;           // threads that offer one candidate as a threshold
+constexpr int kGroups = kPick / kGroup;
+constexpr int kSurvivors = 2048;    // (K - 1) * kGroup * items a thread + 1 of them at most: K <= 16 fit with K items
+static_assert(kPick == kSeg && kGroups >= kMaxBeams, "choice");
+
+struct PickLds {
+  Cand group[kGroups];
+  Cand threshold;
+  int count;
+  Cand kept[kSurvivors];
+  Cand out[kMaxBeams];
+};
+
+// The K first of n items into L.out, in order; how many there are.  The K-th of the
+// groups' first ones bounds the K-th of all from below; of the few items not behind it
+// every one counts those before it.
+template <typename F>
+__device__ __forceinline__ int pick(PickLds& L, int n, int K, F item) {
+  const int tid = threadIdx.x;
+  Cand best{0, ~0u};
+#pragma unroll 4
+  for (int i = tid; i < n; i += kPick) {
+    const Cand c = item(i);
+    if (before(c, best)) best = c;
+  }
+#pragma unroll
+  for (int d = 1; d < kGroup; d <<= 1) {
+    const Cand o = shfl_xor_c(best, d);
+    if (before(o, best)) best = o;
+  }
+  if (tid % kGroup == 0) L.group[tid / kGroup] = best;
+  if (tid == 0) {
+    L.threshold = Cand{0, ~0u};
+    L.count = 0;
+  }
+  __syncthreads();
+  int r = 0;
+#pragma unroll
+  for (int j = 0; j < kGroups / kGroup; ++j) r += before(L.group[tid % kGroup + kGroup * j], best);
+  r = group_sum_i<kGroup>(r);
+  if (tid % kGroup == 0 && r == K - 1 && best.k != 0) L.threshold = best;
+  __syncthreads();
+  const Cand least = L.threshold;
+#pragma unroll 4
+  for (int i = tid; i < n; i += kPick) {
+    const Cand c = item(i);
+    if (c.k != 0 && !before(least, c)) {
+      const int at = atomicAdd(&L.count, 1);  // (any order: each one's place is counted below)
+      if (at < kSurvivors) L.kept[at] = c;
+    }
+  }
+  __syncthreads();
+  const int kept = L.count;
+  if (kept <= kSurvivors) {
+    for (int s = tid; s < kept; s += kPick) {
+      const Cand c = L.kept[s];
+      int at = 0;
+      for (int j = 0; j < kept; ++j) at += before(L.kept[j], c);
+      if (at < K) L.out[at] = c;
+    }
+    __syncthreads();
+    return min(kept, K);
+  }
+  // more than K = 16 of candidates that crowd in a few groups: one after the other
+  Cand last{~uint64_t{0}, 0};
+  for (int k = 0; k < K; ++k) {
+    Cand c{0, ~0u};
+    for (int i = tid; i < n; i += kPick) {
+      const Cand x = item(i);
+      if (before(last, x) && before(x, c)) c = x;
+    }
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const Cand o = shfl_xor_c(c, d);
+      if (before(o, c)) c = o;
+    }
+    if ((tid & 63) == 0) L.group[tid >> 6] = c;
+    __syncthreads();
+    for (int j = 0; j < kPick / 64; ++j)
+      if (before(L.group[j], c)) c = L.group[j];
+    if (tid == 0) L.out[k] = c;
+    last = c;
+    __syncthreads();
+  }
+  return K;
+}
+
+// The choice of one group.  What bounds it: latency (a round trip to the segments'
+// statistics, one to the chosen segments, and the barriers of two choices).
+template <typename T>
+__global__ __launch_bounds__(kPick) void beam_pick_kernel(SelectParams p) {
+  __shared__ PickLds L;
+  __shared__ double base[kMaxBeams];  // score - log of the sum of exp(x - most)
+  __shared__ float most[kMaxBeams];   // the beam's largest logit
+  __shared__ int state[kMaxBeams];    // 0: no candidates, 1: alive, 2: finished
+  __shared__ int2 chosen[kMaxBeams];  // segments: beam, first token
+  const int b = blockIdx.x, W = p.beams, V = p.vocab, K = p.num_out, nseg = p.nseg;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const float2* seg = p.seg + static_cast<int64_t>(b) * W * nseg;
+  for (int w = wave; w < W; w += kPick / 64) {
+    const float score = p.scores[b * W + w];
+    const bool done = p.finished && p.finished[b * W + w];
+    const int st = !beam_alive(score) ? 0 : done ? 2 : 1;
+    double c = score;
+    float m = -INFINITY;
+    if (st == 1) {
+      for (int j = lane; j < nseg; j += 64) m = fmaxf(m, seg[w * nseg + j].x);
+      m = wave_max_dpp(m);
+      double s = 0.0;
+      for (int j = lane; j < nseg; j += 64) {
+        const float2 v = seg[w * nseg + j];
+        if (v.y > 0.0f) s += v.y * (v.x == m ? 1.0 : exp(static_cast<double>(v.x) - static_cast<double>(m)));
+      }
+#pragma unroll
+      for (int d = 1; d < 64; d <<= 1) s += __shfl_xor(s, d, 64);
+      c -= log(s);
+    }
+    if (lane == 0) {
+      base[w] = c;
+      most[w] = m;
+      state[w] = st == 1 && !(m > -INFINITY) ? 0 : st;
+    }
+  }
+  __syncthreads();
+  const auto total = [&](int w, float x) {
+    return base[w] + (x == most[w] ? 0.0 : static_cast<double>(x) - static_cast<double>(most[w]));
+  };
+  const int n1 = pick(L, W * nseg, K, [&](int i) {
+    const int w = i / nseg, j = i - w * nseg;
+    if (state[w] == 1) return cand(total(w, seg[i].x), i);
+    return j == 0 && state[w] == 2 ? cand(base[w], i) : Cand{0, ~0u};
+  });
+  if (threadIdx.x < static_cast<unsigned>(n1)) {
+    const int i = L.out[threadIdx.x].i, w = i / nseg;
+    chosen[threadIdx.x] = int2{w, (i - w * nseg) * kSeg};
+  }
+  __syncthreads();
+  const T* x = static_cast<const T*>(p.x) + b * p.group_stride;
+  const int n2 = pick(L, n1 * kSeg, K, [&](int i) {
+    const int2 c = chosen[i / kSeg];
+    const int t = c.y + i % kSeg;
+    if (state[c.x] == 2) return i % kSeg == 0 ? cand(base[c.x], c.x * V + p.pad) : Cand{0, ~0u};
+    if (t >= V) return Cand{0, ~0u};
+    const float v = to_f32(x[c.x * p.beam_stride + t]);
+    return v == v ? cand(total(c.x, v), c.x * V + t) : Cand{0, ~0u};
+  });
+  for (int k = threadIdx.x; k < K; k += kPick) {
+    const int64_t at = static_cast<int64_t>(b) * K + k;
+    const Cand c = k < n2 ? L.out[k] : Cand{0, 0};
+    const int w = static_cast<int>(c.i) / V;
+    p.scores_out[at] = k < n2 ? static_cast<float>(total_of(c.k)) : -INFINITY;
+    p.parents_out[at] = k < n2 ? b * W + w : -1;
+    p.tokens_out[at] = k < n2 ? static_cast<int>(c.i) - w * V : -1;
+  }
+}
+
+template <typename T>
+int launch_select(const SelectParams& p, hipStream_t s) {
+  const int64_t waves = static_cast<int64_t>(p.groups) * p.beams * p.nseg;
+  beam_scan_kernel<T><<<static_cast<unsigned>((waves + 3) / 4), 256, 0, s>>>(p);
+  TQ_CHECK_LAUNCH("beam_scan_kernel");
+  beam_pick_kernel<T><<<static_cast<unsigned>(p.groups), kPick, 0, s>>>(p);
+  TQ_CHECK_LAUNCH("beam_pick_kernel");
+  return TQ_OK;
+}
+
+int segments(int vocab) { return (vocab + kSeg - 1) / kSeg; }
+
+// ---- reordering a contiguous cache ------------------------------------------
+// Rows of sequence b become those of parents[b], in place.  A workgroup takes the same
+// bytes of every sequence: it loads those of all parents into LDS before it stores any,
+// and no other workgroup touches them, so that any map (swaps, cycles, one parent of
+// many) comes out as if all moved at once.
+constexpr int kMaxSeqs = 1024;
+constexpr int kTileUnits = 4096;  // 16-byte units in LDS
+
+struct ReorderParams {
+  char* base[6];
+  int row_bytes[6];
+  int tiles[6];   // of one head
+  int heads, cap, seqs, shift;  // 1 << shift units of a sequence in a tile
+  int32_t* lengths;
+  const int32_t* parents;
+};
+
+__device__ __forceinline__ int parent_of(const int32_t* parents, int s, int seqs) {
+  const int q = parents[s];
+  return static_cast<unsigned>(q) < static_cast<unsigned>(seqs) ? q : -1;
+}
+
+__global__ __launch_bounds__(256) void kv_reorder_kernel(ReorderParams p) {
+  __shared__ uint4 unit[kTileUnits];
+  __shared__ int16_t needed[kMaxSeqs];  // 1 + slot of a parent that is needed, 0 yet without one; else -1
+  __shared__ int2 from[kMaxSeqs];       // sequence, rows
+  __shared__ ushort2 to[kMaxSeqs];      // sequence, slot
+  __shared__ int n_from, n_to;
+  for (int s = threadIdx.x; s < p.seqs; s += 256) needed[s] = -1;
+  if (threadIdx.x == 0) n_from = n_to = 0;
+  __syncthreads();
+  for (int s = threadIdx.x; s < p.seqs; s += 256) {
+    const int q = parent_of(p.parents, s, p.seqs);
+    if (q >= 0 && q != s) needed[q] = 0;
+  }
+  __syncthreads();
+  for (int s = threadIdx.x; s < p.seqs; s += 256) {
+    const int n = min(p.lengths[s], p.cap);
+    if (needed[s] == 0 && n > 0) {  // (any order: it is only where they lie in LDS)
+      const int at = atomicAdd(&n_from, 1);
+      needed[s] = static_cast<int16_t>(at + 1);
+      from[at] = int2{s, n};
+    }
+  }
+  __syncthreads();
+  for (int s = threadIdx.x; s < p.seqs; s += 256) {
+    const int q = parent_of(p.parents, s, p.seqs);
+    if (q >= 0 && q != s && needed[q] > 0) to[atomicAdd(&n_to, 1)] = ushort2{static_cast<uint16_t>(s), static_cast<uint16_t>(needed[q] - 1)};
+  }
+  __syncthreads();
+  const int nf = n_from, nd = n_to, T = 1 << p.shift;
+  int per_head = 0;
+#pragma unroll
+  for (int a = 0; a < 6; ++a) per_head += p.tiles[a];
+  const int64_t total = static_cast<int64_t>(per_head) * p.heads;
+  for (int64_t g = blockIdx.x; g < total; g += gridDim.x) {
+    const int h = static_cast<int>(g / per_head);
+    int u = static_cast<int>(g - static_cast<int64_t>(h) * per_head), a = 0;
+#pragma unroll
+    for (int i = 0; i < 5; ++i)
+      if (a == i && u >= p.tiles[i]) {
+        u -= p.tiles[i];
+        a = i + 1;
+      }
+    char* base = p.base[0];
+    int rb = p.row_bytes[0];
+#pragma unroll
+    for (int i = 1; i < 6; ++i)
+      if (a == i) {
+        base = p.base[i];
+        rb = p.row_bytes[i];
+      }
+    const int64_t first = static_cast<int64_t>(u) << (p.shift + 4);  // bytes into the head's rows
+    const auto place = [&](int s) { return base + (static_cast<int64_t>(s) * p.heads + h) * p.cap * rb + first; };
+#pragma unroll 4
+    for (int i = threadIdx.x; i < nf << p.shift; i += 256) {
+      const int2 f = from[i >> p.shift];
+      const int at = 16 * (i & (T - 1));
+      const int64_t have = static_cast<int64_t>(f.y) * rb - first - at;
+      const char* src = place(f.x) + at;
+      if (have >= 16) {
+        __builtin_memcpy(&unit[i], src, 16);
+      } else {
+        for (int k = 0; k < have; k += 2)
+          reinterpret_cast<uint16_t*>(&unit[i])[k / 2] = *reinterpret_cast<const uint16_t*>(src + k);
+      }
+    }
+    __syncthreads();
+#pragma unroll 4
+    for (int i = threadIdx.x; i < nd << p.shift; i += 256) {
+      const ushort2 d = to[i >> p.shift];
+      const int at = 16 * (i & (T - 1)), in = (d.y << p.shift) + (i & (T - 1));
+      const int64_t have = static_cast<int64_t>(from[d.y].y) * rb - first - at;
+      char* dst = place(d.x) + at;
+      if (have >= 16) {
+        __builtin_memcpy(dst, &unit[in], 16);
+      } else {
+        for (int k = 0; k < have; k += 2)
+          *reinterpret_cast<uint16_t*>(dst + k) = reinterpret_cast<const uint16_t*>(&unit[in])[k / 2];
+      }
+    }
+    __syncthreads();
+  }
+}
+
+__global__ __launch_bounds__(kMaxSeqs) void kv_reorder_lengths_kernel(ReorderParams p) {
+  const int s = threadIdx.x;
+  int n = 0;
+  if (s < p.seqs) {
+    const int q = parent_of(p.parents, s, p.seqs);
+    n = q < 0 ? 0 : p.lengths[q];
+  }
+  __syncthreads();
+  if (s < p.seqs) p.lengths[s] = n;
+}
+
+}  // namespace
+}  // namespace tq
+
+using namespace tq;
+
+extern "C" size_t tq_beam_select_workspace_size(int groups, int beams, int vocab) {
+  if (groups < 1 || beams < 1 || vocab < 1) return 0;
+  return sizeof(float2) * static_cast<size_t>(groups) * beams * segments(vocab);
+}
+
+extern "C" int tq_beam_select(const void* logits, tq_dtype x_dtype, int64_t group_stride, int64_t beam_stride,
+                              const float* scores, const uint8_t* finished, int groups, int beams, int vocab,
+                              int num_out, int pad_token, float* scores_out, int32_t* parents_out,
+                              int32_t* tokens_out, void* workspace, size_t workspace_bytes, void* stream) {
+  clear_error();
+  const char* fn = "tq_beam_select";
+  TQ_CHECK_ARG(valid_dtype(x_dtype), "%s: bad x_dtype %d", fn, x_dtype);
+  TQ_CHECK_ARG(groups >= 0 && groups <= (1 << 20), "%s: groups must be 0 to 2^20", fn);
+  TQ_CHECK_ARG(beams >= 1 && beams <= kMaxBeams, "%s: beams must be 1 to %d (got %d)", fn, kMaxBeams, beams);
+  TQ_CHECK_ARG(num_out >= 1 && num_out <= kMaxBeams, "%s: num_out must be 1 to %d (got %d)", fn, kMaxBeams, num_out);
+  TQ_CHECK_ARG(vocab >= 1 && vocab <= (1 << 24), "%s: vocab must be 1 to 2^24 (got %d)", fn, vocab);
+  TQ_CHECK_ARG(pad_token >= 0 && pad_token < vocab, "%s: pad_token must be a token (got %d)", fn, pad_token);
+  if (groups == 0) return TQ_OK;
+  TQ_CHECK_ARG(group_stride >= 0 && beam_stride >= 0 && group_stride < (int64_t{1} << 40) && beam_stride < (int64_t{1} << 40), "%s: bad strides", fn);
+  TQ_CHECK_ARG(logits && scores && scores_out && parents_out && tokens_out, "%s: null pointer", fn);
+  TQ_CHECK_ARG(reinterpret_cast<uintptr_t>(logits) % dtype_size(x_dtype) == 0, "%s: logits must be aligned to their type", fn);
+  const size_t need = tq_beam_select_workspace_size(groups, beams, vocab);
+  if (!workspace || workspace_bytes < need) {
+    set_error("%s: workspace of %zu bytes needed (got %zu)", fn, need, workspace ? workspace_bytes : size_t{0});
+    return TQ_ERR_WORKSPACE;
+  }
+  TQ_CHECK_ARG(reinterpret_cast<uintptr_t>(workspace) % 16 == 0, "%s: workspace must be 16-byte aligned", fn);
+  const int nseg = segments(vocab);
+  TQ_CHECK_ARG(static_cast<int64_t>(groups) * beams * nseg < (int64_t{1} << 31), "%s: logits too large", fn);
+  SelectParams p{logits, group_stride, beam_stride, scores, finished, groups, beams, vocab, num_out, pad_token, nseg,
+                 static_cast<float2*>(workspace), scores_out, parents_out, tokens_out};
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (x_dtype == TQ_F32) return launch_select<float>(p, s);
+  if (x_dtype == TQ_F16) return launch_select<_Float16>(p, s);
+  return launch_select<uint16_t>(p, s);
+}
+
+extern "C" int tq_kv_reorder_int4(uint32_t* k_quant, void* k_scales, void* k_biases, uint32_t* v_quant,
+                                  void* v_scales, void* v_biases, tq_dtype sb_dtype, int batch, int num_kv_heads,
+                                  int head_dim, int kv_capacity, int32_t* lengths, const int32_t* parents,
+                                  void* stream) {
+  clear_error();
+  const char* fn = "tq_kv_reorder_int4";
+  TQ_CHECK_ARG(sb_dtype == TQ_F16 || sb_dtype == TQ_F32, "%s: sb_dtype must be f16 or f32", fn);
+  TQ_CHECK_ARG(batch >= 0 && batch <= kMaxSeqs, "%s: batch must be 0 to %d (got %d)", fn, kMaxSeqs, batch);
+  TQ_CHECK_ARG(num_kv_heads >= 1 && num_kv_heads <= 65535, "%s: bad num_kv_heads", fn);
+  TQ_CHECK_ARG(head_dim > 0 && head_dim % 64 == 0 && head_dim <= 4096, "%s: head_dim must be a multiple of 64 <= 4096", fn);
+  TQ_CHECK_ARG(kv_capacity >= 1 && kv_capacity <= (1 << 24), "%s: kv_capacity must be 1 to 2^24", fn);
+  if (batch == 0) return TQ_OK;
+  ReorderParams p{};
+  void* const t[6] = {k_quant, k_scales, k_biases, v_quant, v_scales, v_biases};
+  p.shift = 0;
+  while (p.shift < 10 && (batch << (p.shift + 1)) <= kTileUnits) ++p.shift;
+  int64_t tiles = 0;
+  for (int i = 0; i < 6; ++i) {
+    TQ_CHECK_ARG(t[i] != nullptr, "%s: null tensor pointer", fn);
+    TQ_CHECK_ARG(reinterpret_cast<uintptr_t>(t[i]) % 4 == 0, "%s: cache tensors must be 4-byte aligned", fn);
+    p.base[i] = static_cast<char*>(t[i]);
+    p.row_bytes[i] = i % 3 == 0 ? head_dim / 2 : head_dim / 64 * static_cast<int>(dtype_size(sb_dtype));
+    const int64_t bytes = static_cast<int64_t>(kv_capacity) * p.row_bytes[i];
+    const int64_t n = (bytes + (int64_t{16} << p.shift) - 1) / (int64_t{16} << p.shift);
+    TQ_CHECK_ARG(n < (1 << 28), "%s: cache too large", fn);
+    p.tiles[i] = static_cast<int>(n);
+    tiles += n;
+  }
+  TQ_CHECK_ARG(lengths && parents, "%s: null pointer", fn);
+  p.heads = num_kv_heads;
+  p.cap = kv_capacity;
+  p.seqs = batch;
+  p.lengths = lengths;
+  p.parents = parents;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  kv_reorder_kernel<<<static_cast<unsigned>(std::min<int64_t>(tiles * num_kv_heads, 512)), 256, 0, s>>>(p);
+  TQ_CHECK_LAUNCH("kv_reorder_kernel");
+  kv_reorder_lengths_kernel<<<1, kMaxSeqs, 0, s>>>(p);
+  TQ_CHECK_LAUNCH("kv_reorder_lengths_kernel");
+  return TQ_OK;
+}

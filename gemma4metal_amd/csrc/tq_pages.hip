@@ -1,4 +1,4 @@
-// Page management of the paged int4 cache: reserving, forking, freeing,
+// Page management of the paged int4 cache: reserving, forking, reordering, freeing,
 // evicting, compacting and copying pages, all on the device.
 //
 // A call is a plan and an application.  The plan is integer work over the
@@ -198,6 +198,99 @@ __global__ __launch_bounds__(kPlanThreads) void pages_plan_kernel(PlanParams p) 
   }
 }
 
+// Reordering: every sequence becomes the continuation of its parent, all at once.
+enum Role : int { kEnds, kStays, kHeir, kCopy };  // an heir takes its parent's row over
+
+struct RolesParams {
+  PlanParams plan;
+  int* role;
+  int* new_len;
+  int32_t* saved;  // rows of parents, by parent, as they were
+};
+
+__device__ __forceinline__ int parent_of(const int32_t* parents, int s, int seqs) {
+  const int q = parents[s];
+  return static_cast<unsigned>(q) < static_cast<unsigned>(seqs) ? q : -1;
+}
+__device__ __forceinline__ int rows_of(const PlanParams& p, int s) {
+  return static_cast<int>(min(static_cast<int64_t>(max(p.lengths[s], 0)), static_cast<int64_t>(p.max_pages) * p.page_size));
+}
+
+// Roles; rows without a child give up their pages, rows that others need are kept.  A
+// workgroup a sequence reads all parents (of at most kReorderSeqs, from L2).
+constexpr int kReorderSeqs = 65536;
+
+__global__ __launch_bounds__(256) void pages_roles_kernel(RolesParams r) {
+  __shared__ int has_child, has_other, first;
+  const PlanParams& p = r.plan;
+  for (int s = blockIdx.x; s < p.seqs; s += gridDim.x) {
+    if (threadIdx.x == 0) {
+      has_child = has_other = 0;
+      first = p.seqs;
+    }
+    __syncthreads();
+    const int par = parent_of(p.ask, s, p.seqs);
+    for (int t = threadIdx.x; t < p.seqs; t += 256) {
+      const int q = p.ask[t];
+      if (q == s) {
+        has_child = 1;
+        if (t != s) has_other = 1;
+      }
+      if (q == par) atomicMin(&first, t == q ? -1 : t);
+    }
+    __syncthreads();
+    const int32_t* row = p.tables + static_cast<int64_t>(s) * p.max_pages;
+    const bool keeps = has_child != 0, kept = has_other != 0;
+    for (int e = threadIdx.x; e < p.max_pages; e += 256) {
+      const int v = row[e];
+      if (!keeps && is_page(v, p.num_pages)) atomicSub(&p.refs[v], 1);  // whole numbers: any order
+      if (kept) r.saved[static_cast<int64_t>(s) * p.max_pages + e] = v;
+    }
+    if (threadIdx.x == 0) r.role[s] = par < 0 ? kEnds : par == s ? kStays : first == s ? kHeir : kCopy;
+    __syncthreads();
+  }
+}
+
+// Copies of last pages to the lowest free ones, in sequence order.
+__global__ __launch_bounds__(kPlanThreads) void pages_reorder_plan_kernel(RolesParams r) {
+  __shared__ int lds[kPlanWaves], sums[kPlanWaves];
+  const PlanParams& p = r.plan;
+  int want = 0;  // (at most one page a sequence)
+  for (int s0 = 0; s0 < p.seqs; s0 += kPlanThreads) {
+    const int s = s0 + threadIdx.x;
+    int need = -1;
+    if (s < p.seqs) {
+      const int role = r.role[s];
+      if (role != kEnds) {
+        const int par = p.ask[s], n = rows_of(p, par);
+        need = role == kCopy && n % p.page_size != 0 &&
+               is_page(p.tables[static_cast<int64_t>(par) * p.max_pages + n / p.page_size], p.num_pages);
+        r.new_len[s] = n;
+      }
+      p.w.need[s] = need;
+    }
+    int total;
+    const int b = wg_scan(max(need, 0), sums, total);
+    if (s < p.seqs) p.w.before[s] = plan_before(static_cast<PlanSum>(want) + b, p.num_pages);
+    want += total;
+  }
+  const int found = free_pages(p.refs, p.num_pages, min(want, p.num_pages), p.w.list, lds);
+  __syncthreads();
+  for (int s = threadIdx.x; s < p.seqs; s += kPlanThreads) {
+    const int need = p.w.need[s], before = p.w.before[s];
+    const bool ok = plan_grants(need, before, found);
+    p.granted[s] = ok;
+    if (!ok) {
+      r.role[s] = kEnds;
+    } else if (need > 0) {
+      const int par = p.ask[s], dst = p.w.list[before];
+      p.w.jobs[before] = int2{p.tables[static_cast<int64_t>(par) * p.max_pages + r.new_len[s] / p.page_size], dst};
+      p.refs[dst] = 1;
+    }
+  }
+  if (threadIdx.x == 0) *p.w.n_jobs = min(want, found);
+}
+
 struct CompactParams {
   const int32_t* refs;
   int32_t* refs_out;
@@ -279,12 +372,14 @@ struct ApplyParams {
   const int* before;
   const int* list;
   const int* map;
+  const int* role;  // reorder
+  const int* new_len;
   int seqs, max_pages, page_size;
 };
 
 constexpr int kCopyUnit = 16384;  // bytes a workgroup copies at a time
 
-enum class Apply { copy, fork, compact };
+enum class Apply { copy, fork, compact, reorder };
 
 // What bounds it: HBM, as a copy; a workgroup moves 16 KB at a time, four 16-byte
 // loads a lane in flight, and takes units at the grid's stride, so that the
@@ -308,6 +403,29 @@ __global__ __launch_bounds__(256) void pages_apply_kernel(ApplyParams p) {
           v = from[e];
           if (is_page(v, p.num_pages)) atomicAdd(&p.refs[v], 1);  // whole numbers: any order
         } else if (e == full && part) {
+          v = p.list[p.before[s]];
+        }
+        to[e] = v;
+      }
+      if (threadIdx.x == 0) p.lengths[s] = n;
+    }
+  }
+  if constexpr (KIND == Apply::reorder) {
+    for (int s = blockIdx.x; s < p.seqs; s += gridDim.x) {
+      const int role = p.role[s];
+      if (role == kStays) continue;
+      const int n = role == kEnds ? 0 : p.new_len[s], full = n / p.page_size;
+      const bool part = role == kCopy && p.need[s] > 0;
+      const int32_t* from = role == kEnds ? nullptr : p.tables_in + static_cast<int64_t>(p.parents[s]) * p.max_pages;
+      int32_t* to = p.tables + static_cast<int64_t>(s) * p.max_pages;
+      for (int e = threadIdx.x; e < p.max_pages; e += 256) {
+        int v = -1;
+        if (role == kHeir) {
+          v = from[e];
+        } else if (role == kCopy && e < full) {
+          v = from[e];
+          if (is_page(v, p.num_pages)) atomicAdd(&p.refs[v], 1);  // whole numbers: any order
+        } else if (part && e == full) {
           v = p.list[p.before[s]];
         }
         to[e] = v;
@@ -520,6 +638,68 @@ extern "C" int tq_kv_pages_fork(void* const* pages, tq_dtype sb_dtype, int num_l
   a.max_pages = max_pages;
   a.page_size = page_size;
   pages_apply_kernel<Apply::fork><<<apply_grid(a, std::min(num_seqs, num_pages)), 256, 0, s>>>(a);
+  TQ_CHECK_LAUNCH("pages_apply_kernel");
+  return TQ_OK;
+}
+
+namespace {
+// Workspace of a reordering: a plan's, roles and new lengths, and the saved rows.
+size_t reorder_ints(int64_t seqs, int64_t pages, int64_t max_pages) {
+  return plan_ints(seqs, pages) + 2 * seqs + seqs * max_pages;
+}
+}  // namespace
+
+extern "C" size_t tq_kv_pages_reorder_workspace_size(int num_seqs, int num_pages, int max_pages) {
+  if (num_seqs < 0 || num_pages < 1 || max_pages < 1) return 0;
+  return sizeof(int) * ((reorder_ints(num_seqs, num_pages, max_pages) + 3) / 4 * 4);
+}
+
+extern "C" int tq_kv_pages_reorder(void* const* pages, tq_dtype sb_dtype, int num_layers, int num_kv_heads,
+                                   int head_dim, int32_t* block_tables, int32_t* refs, int32_t* lengths,
+                                   const int32_t* parents, int32_t* granted, int num_seqs, int max_pages,
+                                   int num_pages, int page_size, void* workspace, size_t workspace_bytes,
+                                   void* stream) {
+  clear_error();
+  const char* fn = "tq_kv_pages_reorder";
+  if (int r = check_tables(num_seqs, max_pages, num_pages, page_size, fn)) return r;
+  TQ_CHECK_ARG(num_seqs <= kReorderSeqs, "%s: num_seqs must be 0 to %d", fn, kReorderSeqs);
+  ApplyParams a{};
+  if (int r = set_pages(a, pages, sb_dtype, num_layers, num_kv_heads, head_dim, num_pages, page_size, fn)) return r;
+  if (num_seqs == 0) return TQ_OK;
+  TQ_CHECK_ARG(block_tables && refs && lengths && parents && granted, "%s: null pointer", fn);
+  const size_t bytes = tq_kv_pages_reorder_workspace_size(num_seqs, num_pages, max_pages);
+  if (!workspace || workspace_bytes < bytes) {
+    set_error("%s: workspace of %zu bytes needed (got %zu)", fn, bytes, workspace ? workspace_bytes : size_t{0});
+    return TQ_ERR_WORKSPACE;
+  }
+  TQ_CHECK_ARG(reinterpret_cast<uintptr_t>(workspace) % 16 == 0, "%s: workspace must be 16-byte aligned", fn);
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  RolesParams r{};
+  r.plan = PlanParams{block_tables, refs, lengths, parents, granted, num_seqs, max_pages, num_pages, page_size,
+                      plan_ws(workspace, num_seqs, num_pages)};
+  r.role = static_cast<int*>(workspace) + plan_ints(num_seqs, num_pages);
+  r.new_len = r.role + num_seqs;
+  r.saved = r.new_len + num_seqs;
+  pages_roles_kernel<<<static_cast<unsigned>(std::min(num_seqs, 2048)), 256, 0, s>>>(r);
+  TQ_CHECK_LAUNCH("pages_roles_kernel");
+  pages_reorder_plan_kernel<<<1, kPlanThreads, 0, s>>>(r);
+  TQ_CHECK_LAUNCH("pages_reorder_plan_kernel");
+  a.n_jobs = r.plan.w.n_jobs;
+  a.jobs = r.plan.w.jobs;
+  a.tables = block_tables;
+  a.tables_in = r.saved;
+  a.refs = refs;
+  a.lengths = lengths;
+  a.parents = parents;
+  a.need = r.plan.w.need;
+  a.before = r.plan.w.before;
+  a.list = r.plan.w.list;
+  a.role = r.role;
+  a.new_len = r.new_len;
+  a.seqs = num_seqs;
+  a.max_pages = max_pages;
+  a.page_size = page_size;
+  pages_apply_kernel<Apply::reorder><<<apply_grid(a, std::min(num_seqs, num_pages)), 256, 0, s>>>(a);
   TQ_CHECK_LAUNCH("pages_apply_kernel");
   return TQ_OK;
 }

@@ -379,6 +379,33 @@ def kv_pages_fork(pages, block_tables: torch.Tensor, refs: torch.Tensor, lengths
     return granted
 
 
+@functools.lru_cache(maxsize=64)
+def _reorder_ws_size(S: int, N: int, P: int) -> int:
+    return _lib.load().tq_kv_pages_reorder_workspace_size(S, N, P)
+
+
+@_placed
+def kv_pages_reorder(pages, block_tables: torch.Tensor, refs: torch.Tensor, lengths: torch.Tensor,
+                     parents: torch.Tensor, *, workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Makes every sequence s the continuation of sequence parents[s] as it was, all
+    at once (the step of a beam search): the first child of a parent (the parent
+    itself where it is one) takes its row over, the others share its full pages and
+    get a copy of the last one, where partly filled.  Sequences without a child give
+    their pages up first, so that beams of one length never run out.  A parent
+    outside [0, sequences) ends s.  ``pages``: as for :func:`kv_pages_fork`.  Returns
+    int32 (sequences,): 1 where s continues its parent, 0 where it ended, also for
+    want of a page."""
+    S, P, N, dev = _check_state(block_tables, refs, lengths)
+    arr, sbt, L, Hkv, D, _, page = _six(pages, refs, dev)
+    _check_ints("parents", parents, (S,), dev)
+    granted = torch.empty(S, dtype=torch.int32, device=dev)
+    nbytes = _reorder_ws_size(S, N, P)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if workspace is None else _workspace(workspace, nbytes, dev, 0)
+    call("tq_kv_pages_reorder", arr, sbt, L, Hkv, D, _ptr(block_tables), _ptr(refs), _ptr(lengths), _ptr(parents),
+         _ptr(granted), S, P, N, page, _ptr(ws), ws.numel(), _stream(None))
+    return granted
+
+
 @_placed
 def kv_pages_free(block_tables: torch.Tensor, refs: torch.Tensor, lengths: torch.Tensor, which: torch.Tensor) -> None:
     """Ends the sequences with which[s] != 0: pages lose a reference, table rows
@@ -523,6 +550,9 @@ class PagedInt4KVCache:
 
     def fork(self, parents: torch.Tensor) -> torch.Tensor:
         return kv_pages_fork(self.tensors(), self.block_tables, self.refs, self.lengths, parents)
+
+    def reorder(self, parents: torch.Tensor) -> torch.Tensor:
+        return kv_pages_reorder(self.tensors(), self.block_tables, self.refs, self.lengths, parents)
 
     def free(self, which: torch.Tensor) -> None:
         kv_pages_free(self.block_tables, self.refs, self.lengths, which)

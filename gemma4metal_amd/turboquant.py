@@ -367,6 +367,42 @@ class Int4KVCache:
                                 stream=stream)
 
 
+    def reorder(self, parents: torch.Tensor, *, stream=None) -> None:
+        """Makes every sequence the continuation of sequence parents[b] (int32
+        (B,)) as it was: the step of a beam search."""
+        kv_reorder_int4(*self.tensors(), self.lengths, parents, stream=stream)
+
+
+def kv_reorder_int4(k_quant: torch.Tensor, k_scales: torch.Tensor, k_biases: torch.Tensor,
+                    v_quant: torch.Tensor, v_scales: torch.Tensor, v_biases: torch.Tensor,
+                    lengths: torch.Tensor, parents: torch.Tensor, *, stream=None) -> None:
+    """Reorders (B, Hkv, cap, .) caches (linear or ring) in place, all sequences at
+    once: the rows of sequence b become those of sequence parents[b] as they were,
+    lengths[b] its length.  Rows behind the length stay as they were.  A parent
+    outside [0, B) leaves a length of 0."""
+    names = ("k_quant", "k_scales", "k_biases", "v_quant", "v_scales", "v_biases")
+    tensors = (k_quant, k_scales, k_biases, v_quant, v_scales, v_biases)
+    for n, t in zip(names + ("lengths", "parents"), tensors + (lengths, parents)):
+        _check_cuda(n, t)
+        if t.device != k_quant.device:
+            raise ValueError(f"{n} must be on {k_quant.device}")
+    _need(k_quant.dim() == 4, "k_quant must be (B, Hkv, cap, D/8) uint32")
+    B, Hkv, cap, D = *k_quant.shape[:3], k_quant.shape[3] * 8
+    sbt = _sb_dtype("k_scales", k_scales)
+    for i, (n, t) in enumerate(zip(names, tensors)):
+        if i % 3 == 0:
+            if t.shape != k_quant.shape or t.dtype not in _QUANT_DT:
+                raise ValueError(f"{n} must be {tuple(k_quant.shape)} uint32")
+        elif t.shape != (B, Hkv, cap, D // 64) or t.dtype != k_scales.dtype:
+            raise ValueError(f"{n} must be ({B}, {Hkv}, {cap}, {D // 64}) of one scale dtype")
+    for n, t in (("lengths", lengths), ("parents", parents)):
+        if t.dtype != torch.int32 or t.shape != (B,):
+            raise ValueError(f"{n} must be int32 ({B},)")
+    with torch.cuda.device(k_quant.device):
+        call("tq_kv_reorder_int4", *[_ptr(t) for t in tensors], sbt, B, Hkv, D, cap, _ptr(lengths), _ptr(parents),
+             _stream(stream))
+
+
 def kv_append_int4(k_new: torch.Tensor, v_new: torch.Tensor,
                    k_quant: torch.Tensor, k_scales: torch.Tensor, k_biases: torch.Tensor,
                    v_quant: torch.Tensor, v_scales: torch.Tensor, v_biases: torch.Tensor,

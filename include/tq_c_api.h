@@ -369,6 +369,23 @@ int tq_kv_pages_fork(void* const* pages, tq_dtype sb_dtype, int num_layers, int 
                      int num_pages, int page_size, void* workspace, size_t workspace_bytes,
                      void* stream);
 
+/* Makes every sequence s the continuation of sequence parents[s] as it was before the
+ * call, all at once (the step of a beam search): parents[s] == s stays as it is; a
+ * parent outside [0, num_seqs) ends s, as tq_kv_pages_free does.  The first child of a
+ * parent (the parent itself where it is one) takes its row over; every other child
+ * shares its full pages and gets a copy of the last one, where partly filled, in a
+ * page of its own; pages reserved behind it stay with the first child.  A sequence
+ * without a child gives its pages up before copies take theirs, lowest first: beams of
+ * one length never run out.  granted[s] = 1 where s continues its parent; 0 where it
+ * ended, also for want of a page (its old rows are gone then).  num_seqs <= 65536.
+ * workspace: tq_kv_pages_reorder_workspace_size(...) bytes, as above. */
+size_t tq_kv_pages_reorder_workspace_size(int num_seqs, int num_pages, int max_pages);
+int tq_kv_pages_reorder(void* const* pages, tq_dtype sb_dtype, int num_layers, int num_kv_heads,
+                        int head_dim, int32_t* block_tables, int32_t* refs, int32_t* lengths,
+                        const int32_t* parents, int32_t* granted, int num_seqs, int max_pages,
+                        int num_pages, int page_size, void* workspace, size_t workspace_bytes,
+                        void* stream);
+
 /* Ends the sequences with which[s] != 0 (DEVICE int32 [num_seqs]): their pages
  * lose a reference, their table rows become -1 and their lengths 0.  A batch that
  * attends a shared prefix by an ended sequence's row needs another prefix_table
@@ -406,6 +423,43 @@ int tq_kv_pages_compact(void* const* pages, tq_dtype sb_dtype, int num_layers, i
 int tq_kv_pages_copy(void* const* pages, tq_dtype sb_dtype, int num_layers, int num_kv_heads,
                      int head_dim, int num_pages, int page_size, const int32_t* src,
                      const int32_t* dst, int n, void* stream);
+
+/* ---- beam search -------------------------------------------------------------
+ * The engine samples one continuation (engine/gemma4_multilayer.cpp:519-527); these
+ * calls keep several.
+ *
+ * The next beams of `groups` requests with `beams` beams each: of the candidates
+ *   total(w, t) = scores[w] + logits[w][t] - log(sum over t' of exp(logits[w][t']))
+ * of a group the num_out largest, the lowest (w, t) first among equals.  A beam with
+ * finished[w] != 0 (finished == NULL: none) has one candidate, itself: pad_token at
+ * its score; its logits are not read.  Beams with a score of -inf or NaN have none.
+ * A NaN logit counts as -inf; tokens of -inf are no candidates; +inf logits share
+ * their beam's probability.
+ *   logits: element [b][w][t] at b * group_stride + w * beam_stride + t, 16-bit or
+ *   fp32, aligned to an element, strides >= 0; scores f32, finished u8 [groups,
+ *   beams], DEVICE.
+ *   scores_out f32, parents_out, tokens_out int32 [groups, num_out], DEVICE, best
+ *   first: the total, g * beams + w, and t; -inf, -1, -1 where there are fewer
+ *   candidates.  They overlap no input.
+ * 1 <= beams, num_out <= 64; vocab <= 2^24.  Sums of exponentials are held in 32 bits
+ * within 1,024 tokens and in 64 beyond; totals are compared in 64.
+ * workspace: tq_beam_select_workspace_size(...) bytes, 16-byte aligned; need not be
+ * zeroed; calls that may overlap need one each. */
+size_t tq_beam_select_workspace_size(int groups, int beams, int vocab);
+int tq_beam_select(const void* logits, tq_dtype x_dtype, int64_t group_stride, int64_t beam_stride,
+                   const float* scores, const uint8_t* finished, int groups, int beams, int vocab,
+                   int num_out, int pad_token, float* scores_out, int32_t* parents_out,
+                   int32_t* tokens_out, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Reorders a contiguous cache ([batch, num_kv_heads, kv_capacity, .], linear or ring)
+ * in place, all sequences at once: the rows of sequence b become those of sequence
+ * parents[b] as they were, and lengths[b] its length (DEVICE int32 [batch] both).  Rows
+ * behind min(length, kv_capacity) stay as they were.  parents[b] outside [0, batch):
+ * lengths[b] = 0.  batch <= 1024. */
+int tq_kv_reorder_int4(uint32_t* k_quant, void* k_scales, void* k_biases,
+                       uint32_t* v_quant, void* v_scales, void* v_biases, tq_dtype sb_dtype,
+                       int batch, int num_kv_heads, int head_dim, int kv_capacity,
+                       int32_t* lengths, const int32_t* parents, void* stream);
 
 /* Dequantize rows (for the engine's prefill fallback,
  * engine/gemma4_multilayer.cpp:307-308): out[r, d] = s*nibble + b as f32. */
