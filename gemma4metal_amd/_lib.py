@@ -60,6 +60,9 @@ SIGNATURES = {
     "tq_sdpa_int4_paged_prefill_workspace_size": (SZ, [I, I, I, I, I]),
     "tq_sdpa_int4_paged_prefill": (I, [P, I, P, P, P, P, P, P, I, P, I, I, I, I, I, P, I, I, I, I, F,
                                        I, I, P, SZ, P]),
+    "tq_sdpa_int4_paged_chunks_workspace_size": (SZ, [I, I, I, I, I, I, I]),
+    "tq_sdpa_int4_paged_chunks": (I, [P, I, P, P, P, P, P, P, I, P, I, I, I, I, I, I, I, P, I, P, P, I, I, I, F,
+                                      I, I, P, SZ, P]),
     "tq_kv_pages_workspace_size": (SZ, [I, I]),
     "tq_kv_pages_reserve": (I, [P, P, P, P, P, I, I, I, I, P, SZ, P]),
     "tq_kv_pages_advance": (I, [P, P, P, P, I, I, I, I, P]),

@@ -332,3 +332,71 @@ extern "C" int tq_sdpa_int4_paged_prefill(const void* q, tq_dtype q_dtype, const
     if (int r = set_workspace(p, workspace, workspace_bytes, ws_layout(n_new, num_heads, head_dim, tiles.splits), fn)) return r;
   return launch_paged_tiles(p, head_dim, sb_dtype, tiles, false, static_cast<hipStream_t>(stream));
 }
+
+namespace {
+
+// The partials of a batch's split blocks, behind the counters that other calls keep
+// zeroed in the same workspace.
+WsLayout chunks_layout(const ChunksPlan& pl, int D) {
+  WsLayout w = ws_layout(0, 0, D, 0);
+  const size_t rows = static_cast<size_t>(pl.slots) * 16 * pl.rs;
+  w.o_off = w.ml_off + (2 * sizeof(float) * rows + 255) / 256 * 256;
+  w.total = w.o_off + sizeof(float) * rows * D;
+  return w;
+}
+
+}  // namespace
+
+extern "C" size_t tq_sdpa_int4_paged_chunks_workspace_size(int batch, int queries, int num_heads, int num_kv_heads,
+                                                           int head_dim, int max_new, int max_kv_len) {
+  if (batch < 1 || queries < 1 || num_kv_heads < 1 || num_heads < num_kv_heads || num_heads % num_kv_heads != 0 ||
+      (head_dim != 128 && head_dim != 256 && head_dim != 512) || max_new < 0 || max_kv_len < 0)
+    return 0;
+  size_t most = 0;
+  for (bool all32 : {false, true}) {
+    const ChunksPlan pl = plan_chunks(batch, queries, num_heads / num_kv_heads, num_kv_heads, head_dim, max_new, max_kv_len, all32);
+    if (pl.slots > 0) most = std::max(most, chunks_layout(pl, head_dim).total);
+  }
+  return most;
+}
+
+extern "C" int tq_sdpa_int4_paged_chunks(const void* q, tq_dtype q_dtype, const uint32_t* k_quant,
+                                         const void* k_scales, const void* k_biases, const uint32_t* v_quant,
+                                         const void* v_scales, const void* v_biases, tq_dtype sb_dtype, float* out,
+                                         int batch, int queries, int num_heads, int num_kv_heads, int head_dim,
+                                         int page_size, int num_pages, const int32_t* block_tables, int max_pages,
+                                         const int32_t* starts, const int32_t* seq_lens, int max_new, int max_kv_len,
+                                         int gqa_factor, float scale, int sliding_window, int num_sinks,
+                                         void* workspace, size_t workspace_bytes, void* stream) {
+  clear_error();
+  const char* fn = "tq_sdpa_int4_paged_chunks";
+  TQ_CHECK_ARG(batch >= 0 && batch <= 65535, "%s: batch must be 0 to 65535", fn);
+  TQ_CHECK_ARG(queries >= 0, "%s: queries must be >= 0", fn);
+  TQ_CHECK_ARG(max_new >= 0, "%s: max_new must be >= 0", fn);
+  if (batch == 0 || queries == 0) return TQ_OK;
+  PagedParams p{};
+  if (int r = paged_params(p, q, q_dtype, k_quant, k_scales, k_biases, v_quant, v_scales, v_biases, sb_dtype, out,
+                           batch, num_heads, num_kv_heads, head_dim, page_size, num_pages, block_tables, max_pages,
+                           gqa_factor, scale, sliding_window, num_sinks, fn))
+    return r;
+  TQ_CHECK_ARG(starts && seq_lens, "%s: null pointer", fn);
+  TQ_CHECK_ARG(max_kv_len >= 0 && max_kv_len <= max_pages * page_size,
+               "%s: need 0 <= max_kv_len <= max_pages * page_size (got %d, %d)", fn, max_kv_len, max_pages * page_size);
+  TQ_CHECK_ARG(static_cast<int64_t>(queries) * num_heads < (int64_t{1} << 30), "%s: too many queries", fn);
+  p.seq_lens = seq_lens;
+  p.n_clamp = max_kv_len;
+  const ChunksPlan plan = plan_chunks(batch, queries, gqa_factor, num_kv_heads, head_dim, max_new, max_kv_len,
+                                      q_dtype == TQ_F32 && sb_dtype == TQ_F32);
+  TQ_CHECK_ARG(plan.blocks + plan.slots < (int64_t{1} << 30), "%s: grid too large", fn);
+  if (plan.slots > 0) {
+    const WsLayout wl = chunks_layout(plan, head_dim);
+    if (!workspace || workspace_bytes < wl.total) {
+      set_error("%s: workspace of %zu bytes needed (got %zu)", fn, wl.total, workspace ? workspace_bytes : size_t{0});
+      return TQ_ERR_WORKSPACE;
+    }
+    TQ_CHECK_ARG(reinterpret_cast<uintptr_t>(workspace) % 16 == 0, "%s: workspace must be 16-byte aligned", fn);
+    p.ws_ml = reinterpret_cast<float*>(static_cast<char*>(workspace) + wl.ml_off);
+    p.ws_o = reinterpret_cast<float*>(static_cast<char*>(workspace) + wl.o_off);
+  }
+  return launch_chunks(p, head_dim, sb_dtype, plan, starts, queries, static_cast<hipStream_t>(stream));
+}

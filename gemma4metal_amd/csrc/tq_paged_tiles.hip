@@ -1,6 +1,7 @@
 // Multi-query attention over pages with K/V tiles shared by a workgroup's 64 or
 // 128 (query, head) rows of one kv head: prompts (rows of consecutive queries of one
-// sequence), and the shared prefix of a batch (rows of all its sequences).
+// sequence), chunks of prompts of a batch (the same for each of its sequences), and the
+// shared prefix of a batch (rows of all its sequences).
 //
 // The mathematics, operand layouts and staging are those of tq_prefill.hip, and
 // so is what bounds it (VALU).  What differs:
@@ -231,7 +232,146 @@ __device__ __forceinline__ void pg_alike(const PfRaw<Gm>& R, int e0, int* ok) {
 
 struct TileParams : PagedParams {
   int splits;  // workgroups along the tiles (grid y); 1: write p.out
+  // chunks of a batch (nq sequences): their queries are rows starts[b] .. starts[b + 1] - 1
+  // of q and out, of `queries` in all
+  const int* starts;
+  int queries;
 };
+
+// ---- chunks of a batch --------------------------------------------------------
+// A job is (sequence, block of rows, kv head, split of its tiles); the device lays them
+// out from the lengths.  Every workgroup works it out for itself, a sequence a lane: one
+// round trip to the lengths, where a plan of its own would be a launch.
+struct ChunkSeq {
+  int s0, n, len;      // first query, queries, keys
+  int blocks, tiles;   // of rows; of keys (the most that a block of rows attends)
+};
+
+struct ChunkJob {
+  int b, s0, n, len;
+  int blk, kvh, split, splits;
+  int slot;            // of its partials
+};
+
+template <int ROWS, int TK>
+__device__ __forceinline__ ChunkSeq chunk_seq(const TileParams& p, int b) {
+  ChunkSeq c{0, 0, 0, 0, 0};
+  if (b < p.nq) {
+    c.s0 = min(max(p.starts[b], 0), p.queries);
+    c.n = min(max(p.starts[b + 1], c.s0), p.queries) - c.s0;
+    c.len = max(min(p.seq_lens[b], p.n_clamp), 0);
+    c.blocks = (c.n * p.gqa + ROWS - 1) / ROWS;
+    c.tiles = (c.len + TK - 1) / TK;
+    if (p.window > 0) {  // sinks, the rows' windows, and a tile that those begin in
+      const int64_t keys = static_cast<int64_t>(p.window) + ROWS + 2 * TK;
+      c.tiles = static_cast<int>(min(static_cast<int64_t>(c.tiles), keys / TK + p.sinks / TK + 1));
+    }
+  }
+  return c;
+}
+
+__device__ __forceinline__ float sum_of_wave(float v) { return group_sum<64>(v); }
+
+// Tiles of a job at most.  With T >= work / CUs, jobs of split blocks are fewer than 2
+// CUs: a block of t > T tiles makes ceil(t / T) < 2 t / T of them.  Of a few such T, and
+// of no splits, the one with the least estimated time, in the units of plan_paged_tiles:
+// that of a job or of an even share of all.
+constexpr int kMostSplits = 64;
+constexpr int kLeastTiles = 4;
+
+__device__ __forceinline__ int splits_of(const ChunkSeq& c, int T) {
+  return c.tiles <= T ? 1 : min((c.tiles + T - 1) / T, kMostSplits);
+}
+
+template <int ROWS, int TK>
+__device__ __forceinline__ int chunk_tiles(const TileParams& p) {
+  const int lane = threadIdx.x & 63;
+  float work = 0.0f, blocks = 0.0f;
+  int most = 0;
+  for (int b = lane; b - lane < p.nq; b += 64) {
+    const ChunkSeq c = chunk_seq<ROWS, TK>(p, b);
+    const float n = static_cast<float>(c.blocks) * p.Hkv;
+    work += n * c.tiles;
+    blocks += n;
+    if (c.blocks > 0) most = max(most, c.tiles);
+  }
+  work = sum_of_wave(work);
+  blocks = sum_of_wave(blocks);
+  most = max_of_wave(most);
+  constexpr float kTile = ROWS == 64 ? 8.0f : 13.0f, kFixed = ROWS == 64 ? 48.0f : 72.0f;
+  const float cus = static_cast<float>(p.cus), share = work / cus;
+  const auto time = [&](float jobs, int T) {
+    return fmaxf(T * kTile + kFixed, (work * kTile + jobs * kFixed) / cus + (jobs > cus ? 0.5f * T * kTile : 0.0f));
+  };
+  int best = max(most, 1);
+  float least = time(blocks, best);
+#pragma unroll 1
+  for (int k = 2; k <= 8; k += k < 4 ? 1 : 2) {  // shares of 1, 1.5, 2, 3, 4
+    const int T = max(static_cast<int>(fminf(share * (0.5f * k) * 1.0001f, 1e8f)) + 1, kLeastTiles);
+    if (T >= most) break;
+    float jobs = 0.0f;
+    for (int b = lane; b - lane < p.nq; b += 64) {
+      const ChunkSeq c = chunk_seq<ROWS, TK>(p, b);
+      jobs += static_cast<float>(c.blocks) * p.Hkv * splits_of(c, T);
+    }
+    jobs = sum_of_wave(jobs);
+    const float t = time(jobs, T);
+    if (t < least) {
+      least = t;
+      best = T;
+    }
+  }
+  return best;
+}
+
+__device__ __forceinline__ int scan_of_wave(int v) {  // inclusive
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int y = __shfl_up(v, d, 64);
+    if (lane >= d) v += y;
+  }
+  return v;
+}
+
+// Job j (MERGE: the j-th split block of rows and head), or none: splits 0.
+template <int ROWS, int TK, bool MERGE>
+__device__ __forceinline__ ChunkJob chunk_job(const TileParams& p, int j) {
+  const int T = chunk_tiles<ROWS, TK>(p);
+  const int lane = threadIdx.x & 63;
+  int jobs = 0, slots = 0;  // of the sequences before these
+  ChunkJob r{};
+#pragma unroll 1
+  for (int b0 = 0; b0 < p.nq; b0 += 64) {
+    const ChunkSeq c = chunk_seq<ROWS, TK>(p, b0 + lane);
+    const int s = splits_of(c, T), mine = c.blocks * p.Hkv;
+    const int slot = s > 1 ? mine * s : 0;
+    const int n = MERGE ? (s > 1 ? mine : 0) : mine * s;
+    const int upto = jobs + scan_of_wave(n), slot_upto = slots + scan_of_wave(slot);
+    const uint64_t hit = __ballot(upto > j);
+    if (hit != 0) {
+      const int l = __builtin_ctzll(hit);
+      const auto of = [&](int v) { return __builtin_amdgcn_readlane(v, l); };
+      r.b = b0 + l;
+      r.s0 = of(c.s0);
+      r.n = of(c.n);
+      r.len = of(c.len);
+      r.splits = of(s);
+      const int blocks = of(c.blocks);
+      int at = j - (of(upto) - of(n));
+      r.kvh = at % p.Hkv;
+      at /= p.Hkv;
+      r.split = MERGE ? 0 : at % r.splits;
+      if (!MERGE) at /= r.splits;
+      r.blk = blocks - 1 - at;  // the longest key ranges (last queries) start first
+      r.slot = of(slot_upto) - of(slot) + (r.blk * p.Hkv + r.kvh) * r.splits + r.split;
+      return r;
+    }
+    jobs = __builtin_amdgcn_readlane(upto, 63);
+    slots = __builtin_amdgcn_readlane(slot_upto, 63);
+  }
+  return r;
+}
 
 // RS: 16-row sets of a workgroup.  4: a wave takes 32 keys of a tile (of 64 keys, D
 // 512 of 32); 8 (D < 512): all 64, one half after the other, so that twice as many
@@ -240,7 +380,7 @@ struct TileParams : PagedParams {
 // Two waves fill a SIMD (registers).  VALU takes 54% of its cycles and the matrix
 // cores 27% there, 49% and 23% at D 512 (2,048 queries after 6,144 keys: 2.75 ms, 350
 // TFLOP/s); a wave runs the two one after the other.
-template <int D, bool F32, bool Q32, int RS>
+template <int D, bool F32, bool Q32, int RS, bool BATCH>
 __global__ __launch_bounds__(128 * kRs) __attribute__((amdgpu_waves_per_eu(2, 2)))
 void paged_tiles_kernel(TileParams p) {
   using Gm = PfGeom<D, F32, kRs>;
@@ -264,16 +404,27 @@ void paged_tiles_kernel(TileParams p) {
   const int rs = wave % RS, kw = wave / RS % KW, dh = wave / (RS * KW);
   const int m = lane & 15, c = lane >> 4;
   // heads vary fastest, the longest key ranges (last queries) start first
+  ChunkJob job{};
+  if constexpr (BATCH) {
+    job = chunk_job<kRows, TK, false>(p, blockIdx.x);
+    if (job.splits == 0) return;            // (all waves)
+  }
   const int nblk = gridDim.x / p.Hkv;
-  const int kvh = blockIdx.x % p.Hkv, blk = nblk - 1 - static_cast<int>(blockIdx.x / p.Hkv);
-  const int total = p.nq * p.gqa;           // rows of this kv head
+  const int kvh = BATCH ? job.kvh : blockIdx.x % p.Hkv;
+  const int blk = BATCH ? job.blk : nblk - 1 - static_cast<int>(blockIdx.x / p.Hkv);
+  const int total = (BATCH ? job.n : p.nq) * p.gqa;  // rows of this kv head (and sequence)
   const int r0 = blk * kRows;               // first row of this workgroup
+  const int* tables = BATCH ? p.tables + static_cast<int64_t>(job.b) * p.max_pages : p.tables;
+  const int splits = BATCH ? job.splits : p.splits, split = BATCH ? job.split : blockIdx.y;
 
   // ---- the rows' limits, and the workgroup's tiles ----------------------------
   // row r attends key t iff t < hi and (t >= lo or t < sinks)
   const auto limits = [&](int r, int& hi, int& lo) {
     const int q = r / p.gqa;
-    if (p.prefill) {
+    if constexpr (BATCH) {
+      hi = max(job.len - job.n + q + 1, 0);
+      lo = p.window > 0 ? max(0, hi - p.window) : 0;
+    } else if (p.prefill) {
       hi = p.n + q + 1;
       lo = p.window > 0 ? max(0, hi - p.window) : 0;
     } else {
@@ -300,13 +451,13 @@ void paged_tiles_kernel(TileParams p) {
   const int ns = min(p.sinks / TK + (p.sinks % TK != 0), end);  // tiles that hold sinks
   const int skip = max(0, min(lo_w / TK, end) - ns);            // tiles between those and the window's
   const int nt = end - skip;
-  const int per = (nt + p.splits - 1) / p.splits;
-  const int it0 = min(static_cast<int>(blockIdx.y) * per, nt), it1 = min(it0 + per, nt);
+  const int per = (nt + splits - 1) / splits;
+  const int it0 = min(split * per, nt), it1 = min(it0 + per, nt);
   PgRun run;
   const auto load_run = [&](int it) {  // of tiles it ...
     const int v = min(it + lane / KH, nt - 1);
     const int key = max(TK * (v + (v < ns ? 0 : skip)) + 32 * (lane % KH), 0);
-    const int e = nt > 0 ? p.tables[min(key >> p.page_shift, p.max_pages - 1)] : -1;
+    const int e = nt > 0 ? tables[min(key >> p.page_shift, p.max_pages - 1)] : -1;
     const bool has = static_cast<unsigned>(e) < static_cast<unsigned>(p.num_pages);
     const int64_t row = ((static_cast<int64_t>(has ? e : 0) * p.Hkv + kvh) << p.page_shift) + (key & ((1 << p.page_shift) - 1));
     run.lo = static_cast<int>(row);
@@ -347,7 +498,7 @@ void paged_tiles_kernel(TileParams p) {
   // ones over 16; fp32 queries in two fp16 parts.  The sign of a negative scale
   // goes into q.
   v8h qf[2 * NWG], ql[Q32 ? 2 * NWG : 1], qb;
-  const int64_t qrow = static_cast<int64_t>(qi) * p.Hq + kvh * p.gqa + (R - qi * p.gqa);
+  const int64_t qrow = static_cast<int64_t>(qi + job.s0) * p.Hq + kvh * p.gqa + (R - qi * p.gqa);
   float f[2 * NWG][8];
   float mx = 0.0f;
 #pragma unroll
@@ -826,11 +977,11 @@ void paged_tiles_kernel(TileParams p) {
       x1 = fmaf(v.y, fk, x1);
     }
     const int qo = Ro / p.gqa;
-    const int64_t row = static_cast<int64_t>(qo) * p.Hq + kvh * p.gqa + (Ro - qo * p.gqa);
-    if (p.ext_merge == 0) {
+    const int64_t row = static_cast<int64_t>(qo + job.s0) * p.Hq + kvh * p.gqa + (Ro - qo * p.gqa);
+    if (BATCH ? splits == 1 : p.ext_merge == 0) {
       *reinterpret_cast<float2*>(p.out + row * D + d) = make_float2(normalise(x0, l, 0.0f), normalise(x1, l, 0.0f));
     } else {
-      const int64_t slot = row * p.max_splits + blockIdx.y;
+      const int64_t slot = BATCH ? static_cast<int64_t>(job.slot) * kRows + r : row * p.max_splits + blockIdx.y;
       *reinterpret_cast<float2*>(p.ws_o + slot * D + d) = make_float2(x0, x1);
       if (d == 0) *reinterpret_cast<float2*>(p.ws_ml + slot * 2) = make_float2(M, l);
     }
@@ -861,22 +1012,62 @@ __global__ __launch_bounds__(256) void merge_tiles_kernel(const float* ws_ml, co
   reinterpret_cast<v4f*>(out)[i] = r;
 }
 
-template <int D, bool F32, int RS>
+// The outputs of the split blocks of a batch's chunks, a workgroup a quarter of one.
+template <int D, int ROWS>
+__global__ __launch_bounds__(256) void merge_chunks_kernel(TileParams p) {
+  constexpr int TK = D == 512 ? 32 : 64, D4 = D / 4;
+  const ChunkJob job = chunk_job<ROWS, TK, true>(p, blockIdx.x);
+  if (job.splits == 0) return;
+  const int rows = min(job.n * p.gqa - job.blk * ROWS, ROWS);
+  const float2* ml = reinterpret_cast<const float2*>(p.ws_ml) + static_cast<int64_t>(job.slot) * ROWS;
+  const v4f* po = reinterpret_cast<const v4f*>(p.ws_o) + static_cast<int64_t>(job.slot) * ROWS * D4;
+  for (int u = blockIdx.y * 256 + threadIdx.x; u < rows * D4; u += gridDim.y * 256) {
+    const int r = u / D4;
+    float M = -INFINITY, L = 0.0f;
+    for (int k = 0; k < job.splits; ++k) M = fmaxf(M, ml[k * ROWS + r].x);
+    v4f O = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+    for (int k = 0; k < job.splits; ++k) {
+      const float2 x = ml[k * ROWS + r];
+      const float fk = merge_factor(x.x, M);
+      L = fmaf(x.y, fk, L);
+      O += fk * po[static_cast<int64_t>(k) * ROWS * D4 + u];
+    }
+    v4f y;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) y[e] = normalise(O[e], L, 0.0f);
+    const int row = job.blk * ROWS + r, q = row / p.gqa;
+    reinterpret_cast<v4f*>(p.out)[(static_cast<int64_t>(job.s0 + q) * p.Hq + job.kvh * p.gqa + (row - q * p.gqa)) * D4 + u % D4] = y;
+  }
+}
+
+template <int D, bool F32, int RS, bool BATCH>
 void launch_q(const TileParams& p, dim3 grid, hipStream_t s) {
   if constexpr (!(D == 256 && F32 && RS == 8)) {  // (never planned for fp32 queries)
     if (p.q_dtype == TQ_F32) {
-      paged_tiles_kernel<D, F32, true, RS><<<grid, 128 * kRs, 0, s>>>(p);
+      paged_tiles_kernel<D, F32, true, RS, BATCH><<<grid, 128 * kRs, 0, s>>>(p);
       return;
     }
   }
-  paged_tiles_kernel<D, F32, false, RS><<<grid, 128 * kRs, 0, s>>>(p);
+  paged_tiles_kernel<D, F32, false, RS, BATCH><<<grid, 128 * kRs, 0, s>>>(p);
 }
 
-template <bool F32>
+template <bool F32, bool BATCH>
 void launch_dim(const TileParams& p, int D, int rs, dim3 grid, hipStream_t s) {
-  if (D == 512) launch_q<512, F32, 4>(p, grid, s);
-  else if (D == 256) rs == 8 ? launch_q<256, F32, 8>(p, grid, s) : launch_q<256, F32, 4>(p, grid, s);
-  else rs == 8 ? launch_q<128, F32, 8>(p, grid, s) : launch_q<128, F32, 4>(p, grid, s);
+  if (D == 512) launch_q<512, F32, 4, BATCH>(p, grid, s);
+  else if (D == 256) rs == 8 ? launch_q<256, F32, 8, BATCH>(p, grid, s) : launch_q<256, F32, 4, BATCH>(p, grid, s);
+  else rs == 8 ? launch_q<128, F32, 8, BATCH>(p, grid, s) : launch_q<128, F32, 4, BATCH>(p, grid, s);
+}
+
+template <int D>
+void launch_merge(const TileParams& p, int rs, dim3 grid, hipStream_t s) {
+  if constexpr (D < 512) {
+    if (rs == 8) {
+      merge_chunks_kernel<D, 128><<<grid, 256, 0, s>>>(p);
+      return;
+    }
+  }
+  merge_chunks_kernel<D, 64><<<grid, 256, 0, s>>>(p);
 }
 
 int tile_keys(int D) { return D == 512 ? 32 : 64; }
@@ -937,14 +1128,50 @@ int launch_paged_tiles(const PagedParams& p0, int D, int sb_dtype, TilesPlan pla
   p.ext_merge = partials || plan.splits > 1;
   const int64_t rows = static_cast<int64_t>(p.nq) * p.gqa;
   const dim3 grid(static_cast<unsigned>(tile_wgs(rows, p.Hkv, plan.rs)), plan.splits);
-  if (sb_dtype == TQ_F32) launch_dim<true>(p, D, plan.rs, grid, s);
-  else launch_dim<false>(p, D, plan.rs, grid, s);
+  if (sb_dtype == TQ_F32) launch_dim<true, false>(p, D, plan.rs, grid, s);
+  else launch_dim<false, false>(p, D, plan.rs, grid, s);
   TQ_CHECK_LAUNCH("paged_tiles_kernel");
   if (partials || plan.splits == 1) return TQ_OK;
   const int64_t out_rows = static_cast<int64_t>(p.nq) * p.Hq;
   merge_tiles_kernel<<<static_cast<unsigned>((out_rows * (D / 4) + 255) / 256), 256, 0, s>>>(
       p.ws_ml, p.ws_o, p.out, out_rows, plan.splits, p.max_splits, D / 4);
   TQ_CHECK_LAUNCH("merge_tiles_kernel");
+  return TQ_OK;
+}
+
+// ---- chunks of a batch --------------------------------------------------------
+
+ChunksPlan plan_chunks(int batch, int queries, int gqa, int Hkv, int D, int max_new, int64_t max_kv_len, bool all32) {
+  ChunksPlan pl{};
+  const int64_t rows = static_cast<int64_t>(std::min(max_new, queries)) * gqa;
+  pl.rs = D == 512 || (D == 256 && all32) || rows <= 64 ? 4 : 8;
+  const int64_t cus = target_wgs();
+  // blocks of rows of any lengths that add up to `queries`
+  pl.blocks = (static_cast<int64_t>(queries) * gqa / (16 * pl.rs) + std::min(batch, queries)) * Hkv;
+  // (see chunk_tiles)
+  const int64_t most = (max_kv_len + tile_keys(D) - 1) / tile_keys(D);
+  const int64_t splits = std::min<int64_t>((most + kLeastTiles - 1) / kLeastTiles, kMostSplits);
+  pl.slots = splits > 1 ? std::min(2 * cus, pl.blocks * splits) : 0;
+  return pl;
+}
+
+int launch_chunks(const PagedParams& p0, int D, int sb_dtype, const ChunksPlan& plan, const int* starts, int queries,
+                  hipStream_t s) {
+  TileParams p{};
+  static_cast<PagedParams&>(p) = p0;
+  p.splits = 1;
+  p.starts = starts;
+  p.queries = queries;
+  const dim3 grid(static_cast<unsigned>(plan.blocks + plan.slots));
+  if (sb_dtype == TQ_F32) launch_dim<true, true>(p, D, plan.rs, grid, s);
+  else launch_dim<false, true>(p, D, plan.rs, grid, s);
+  TQ_CHECK_LAUNCH("paged_tiles_kernel");
+  if (plan.slots == 0) return TQ_OK;
+  const dim3 merge(static_cast<unsigned>(std::min(plan.blocks, plan.slots / 2)), 4);
+  if (D == 512) launch_merge<512>(p, plan.rs, merge, s);
+  else if (D == 256) launch_merge<256>(p, plan.rs, merge, s);
+  else launch_merge<128>(p, plan.rs, merge, s);
+  TQ_CHECK_LAUNCH("merge_chunks_kernel");
   return TQ_OK;
 }
 

@@ -282,6 +282,66 @@ def sdpa_int4_paged_prefill(queries: torch.Tensor,
     return out
 
 
+@functools.lru_cache(maxsize=256)
+def _chunks_ws_size(*shape) -> int:
+    return _lib.load().tq_sdpa_int4_paged_chunks_workspace_size(*shape)
+
+
+@_placed
+def sdpa_int4_paged_chunks(queries: torch.Tensor,
+                           k_quant: torch.Tensor, k_scales: torch.Tensor, k_biases: torch.Tensor,
+                           v_quant: torch.Tensor, v_scales: torch.Tensor, v_biases: torch.Tensor,
+                           block_tables: torch.Tensor, starts: torch.Tensor, seq_lens: torch.Tensor, gqa_factor: int,
+                           scale: float = 1.0, sliding_window: int = 0, num_sinks: int = 0, *,
+                           max_new: Optional[int] = None, max_kv_len: Optional[int] = None,
+                           out: Optional[torch.Tensor] = None,
+                           workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention of a chunk of new tokens of every sequence of a batch over its pages:
+    prompts in parts, tokens proposed for checking, single tokens among them.
+    queries (N, Hq, D) f32|f16|bf16 hold the sequences' chunks one behind the other:
+    rows starts[b] .. starts[b+1]-1 are sequence b's (starts int32 (B+1,), ascending
+    from 0 to N), block_tables int32 (B, max_pages), seq_lens int32 (B,) with the new
+    rows, which are already appended.  Query i of a chunk of n stands at position
+    seq_lens[b] - n + i and attends key t up to it iff the window W is 0, t is among
+    the last W, or t < num_sinks; none: 0.
+
+    Lengths and chunks are read on the device.  ``max_kv_len`` bounds the lengths
+    (longer ones are cut to it); the table's reach by default.  ``max_new`` is the
+    longest chunk, for the choice of the kernel only; N by default.  Returns (N, Hq, D)
+    float32; rows of ``out`` behind starts[B] stay as they were."""
+    _check_cuda("queries", queries)
+    _need(queries.dim() == 3 and queries.dtype in _DT, "queries must be (N, Hq, D) float32, float16 or bfloat16")
+    N, Hq, D = queries.shape
+    dev = queries.device
+    di = dev.index
+    pages = (k_quant, k_scales, k_biases, v_quant, v_scales, v_biases)
+    if not _pages_fine(pages, D, di):
+        _check_pages(pages, D, dev)
+    num, Hkv, page, _ = k_quant.shape
+    _need(isinstance(block_tables, torch.Tensor) and block_tables.dim() == 2, "block_tables must be (B, max_pages)")
+    B, P = block_tables.shape
+    if not _ints_fine(block_tables, (B, P), di):
+        _check_ints("block_tables", block_tables, (B, P), dev)
+    if not _ints_fine(starts, (B + 1,), di):
+        _check_ints("starts", starts, (B + 1,), dev)
+    if not _ints_fine(seq_lens, (B,), di):
+        _check_ints("seq_lens", seq_lens, (B,), dev)
+    mx = P * page if max_kv_len is None else int(max_kv_len)
+    new = N if max_new is None else int(max_new)
+    if out is None:
+        out = torch.empty((N, Hq, D), dtype=torch.float32, device=dev)
+    else:
+        out = _out(out, (N, Hq, D), dev)
+    sh = _stream(None)
+    nbytes = _chunks_ws_size(B, N, Hq, Hkv, D, new, mx)
+    ws = _workspace(workspace, nbytes, dev, sh) if nbytes else None
+    call("tq_sdpa_int4_paged_chunks", queries.data_ptr(), _DT[queries.dtype], *[t.data_ptr() for t in pages],
+         _DT[k_scales.dtype], out.data_ptr(), B, N, Hq, Hkv, D, page, num, block_tables.data_ptr(), P,
+         starts.data_ptr(), seq_lens.data_ptr(), new, mx, int(gqa_factor), float(scale), int(sliding_window),
+         int(num_sinks), _ptr(ws), nbytes, sh)
+    return out
+
+
 # ---------------------------------------------------------------------------
 # page management
 # ---------------------------------------------------------------------------
@@ -531,6 +591,17 @@ class PagedInt4KVCache:
         return sdpa_int4_paged(queries, *self.layer(layer), self.block_tables, self.lengths + new, gqa_factor, scale,
                                sliding_window, num_sinks, windows=windows, shared_prefix=shared_prefix,
                                prefix_table=prefix_table, max_kv_len=max_kv_len, out=out, workspace=workspace)
+
+    def attend_chunks(self, layer: int, queries: torch.Tensor, starts: torch.Tensor, gqa_factor: int,
+                      scale: float = 1.0, sliding_window: int = 0, num_sinks: int = 0, *,
+                      max_new: Optional[int] = None, max_kv_len: Optional[int] = None,
+                      out: Optional[torch.Tensor] = None, workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """Attention of a chunk of new tokens of every sequence, whose rows are
+        appended and not yet counted: queries (N, Hq, D), those of sequence s in rows
+        starts[s] .. starts[s+1]-1 (:func:`sdpa_int4_paged_chunks`)."""
+        return sdpa_int4_paged_chunks(queries, *self.layer(layer), self.block_tables, starts,
+                                      self.lengths + starts[1:] - starts[:-1], gqa_factor, scale, sliding_window,
+                                      num_sinks, max_new=max_new, max_kv_len=max_kv_len, out=out, workspace=workspace)
 
     def prefix_table(self, shared_prefix: int, sequences: Optional[torch.Tensor] = None) -> torch.Tensor:
         """The pages of the first ``shared_prefix`` rows, which these sequences (an

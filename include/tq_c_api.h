@@ -321,6 +321,34 @@ int tq_sdpa_int4_paged_prefill(const void* q, tq_dtype q_dtype,
                                int sliding_window, int num_sinks,
                                void* workspace, size_t workspace_bytes, void* stream);
 
+/* Attention of a chunk of new tokens of every sequence of a batch over its pages
+ * (prompts in parts, tokens proposed for checking, single tokens among them): the
+ * queries of sequence b are rows starts[b] .. starts[b + 1] - 1 (n of them) of q and
+ * out [queries, num_heads, head_dim]; query i of them stands at position L - n + i, L =
+ * min(seq_lens[b], max_kv_len) with the new rows already appended, and attends key t <=
+ * that position iff sliding_window == 0, t is among the last sliding_window up to it,
+ * or t < num_sinks; none: 0.  starts, DEVICE int32 [batch + 1], ascends from 0 to
+ * queries; rows of out behind starts[batch] stay as they were.  Lengths and chunks are
+ * on the device, so that a captured call serves any of them:
+ * max_new (a sequence's queries) and max_kv_len bound nothing but the plan and the
+ * lengths; a longer chunk is served all the same.
+ * Workspace: tq_sdpa_int4_paged_chunks_workspace_size(...) bytes, 16-byte aligned, of
+ * which the first 256 KiB are left as they are (one workspace serves this call and the
+ * decode calls, in turn); NULL where that is 0; calls that may overlap need one each. */
+size_t tq_sdpa_int4_paged_chunks_workspace_size(int batch, int queries, int num_heads,
+                                                int num_kv_heads, int head_dim, int max_new,
+                                                int max_kv_len);
+int tq_sdpa_int4_paged_chunks(const void* q, tq_dtype q_dtype,
+                              const uint32_t* k_quant, const void* k_scales, const void* k_biases,
+                              const uint32_t* v_quant, const void* v_scales, const void* v_biases,
+                              tq_dtype sb_dtype, float* out,
+                              int batch, int queries, int num_heads, int num_kv_heads,
+                              int head_dim, int page_size, int num_pages,
+                              const int32_t* block_tables, int max_pages, const int32_t* starts,
+                              const int32_t* seq_lens, int max_new, int max_kv_len,
+                              int gqa_factor, float scale, int sliding_window, int num_sinks,
+                              void* workspace, size_t workspace_bytes, void* stream);
+
 /* Page management.  All state is on the device, so that these calls can be
  * captured into a HIP graph: block_tables int32 [num_seqs, max_pages] (-1 = no
  * page), lengths int32 [num_seqs], refs int32 [num_pages] = the number of table

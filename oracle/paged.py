@@ -71,6 +71,22 @@ def sdpa_int4_paged_prefill(q, pages, table, n_prior, page_size, gqa, scale=1.0,
     return out
 
 
+def sdpa_int4_paged_chunks(q, pages, tables, starts, seq_lens, page_size, gqa, scale=1.0, window=0, sinks=0,
+                           max_kv_len=None):
+    """q [N, Hq, D], sequence b's in rows starts[b] .. starts[b + 1] - 1 -> [N, Hq, D] float64."""
+    out = np.zeros(q.shape)
+    for b in range(len(seq_lens)):
+        n = max(int(seq_lens[b]), 0)
+        n = min(n, tables.shape[1] * page_size if max_kv_len is None else max_kv_len)
+        k, v, has = rows(pages, tables[b], page_size, n)
+        new = int(starts[b + 1] - starts[b])
+        for i in range(new):
+            keep = visible(n - new + i + 1, n, window, sinks) & has
+            for h in range(q.shape[1]):
+                out[starts[b] + i, h] = attend(q[starts[b] + i, h], k[h // gqa], v[h // gqa], keep, scale)
+    return out
+
+
 def append(pages, k_new, v_new, tables, positions, page_size, sb, mode="mlx"):
     """Quantized rows into the page arrays, in place."""
     for i, x in ((0, k_new), (3, v_new)):
