@@ -23,7 +23,7 @@ ARCH = "gfx950"
 
 HIP_SOURCES = ["tq_runtime.hip", "tq_quant.hip", "tq_sdpa.hip", "tq_sdpa_mfma.hip", "tq_sdpa_hc.hip",
                "tq_prefill.hip", "tq_prefill_f32.hip", "tq_polar.hip", "tq_paged.hip",
-               "tq_paged_tiles.hip", "tq_pages.hip", "tq_beam.hip"]
+               "tq_paged_tiles.hip", "tq_paged_chunks.hip", "tq_pages.hip", "tq_beam.hip"]
 CXX_SOURCES = ["turboquant.cpp"]
 
 COMMON = ["-O3", "-fPIC", "-std=c++17", f"-I{INCLUDE}", f"-I{CSRC}", "-Wall",

@@ -337,11 +337,23 @@ namespace {
 
 // The partials of a batch's split blocks, behind the counters that other calls keep
 // zeroed in the same workspace.
-WsLayout chunks_layout(const ChunksPlan& pl, int D) {
-  WsLayout w = ws_layout(0, 0, D, 0);
-  const size_t rows = static_cast<size_t>(pl.slots) * 16 * pl.rs;
-  w.o_off = w.ml_off + (2 * sizeof(float) * rows + 255) / 256 * 256;
-  w.total = w.o_off + sizeof(float) * rows * D;
+struct ChunksLayout {
+  size_t ml, o, few_ml, few_o, total;
+};
+
+ChunksLayout chunks_layout(const ChunksPlan& pl, int D) {
+  size_t at = ws_layout(0, 0, D, 0).ml_off;
+  const auto take = [&](int64_t rows, int64_t floats) {
+    const size_t from = at;
+    at += (sizeof(float) * rows * floats + 255) / 256 * 256;
+    return from;
+  };
+  ChunksLayout w;
+  w.ml = take(pl.slots * 16 * pl.rs, 2);
+  w.o = take(pl.slots * 16 * pl.rs, D);
+  w.few_ml = take(pl.few_slots * 16, 2);
+  w.few_o = take(pl.few_slots * 16, D);
+  w.total = at;
   return w;
 }
 
@@ -355,7 +367,7 @@ extern "C" size_t tq_sdpa_int4_paged_chunks_workspace_size(int batch, int querie
   size_t most = 0;
   for (bool all32 : {false, true}) {
     const ChunksPlan pl = plan_chunks(batch, queries, num_heads / num_kv_heads, num_kv_heads, head_dim, max_new, max_kv_len, all32);
-    if (pl.slots > 0) most = std::max(most, chunks_layout(pl, head_dim).total);
+    if (pl.slots + pl.few_slots > 0) most = std::max(most, chunks_layout(pl, head_dim).total);
   }
   return most;
 }
@@ -387,16 +399,20 @@ extern "C" int tq_sdpa_int4_paged_chunks(const void* q, tq_dtype q_dtype, const 
   p.n_clamp = max_kv_len;
   const ChunksPlan plan = plan_chunks(batch, queries, gqa_factor, num_kv_heads, head_dim, max_new, max_kv_len,
                                       q_dtype == TQ_F32 && sb_dtype == TQ_F32);
-  TQ_CHECK_ARG(plan.blocks + plan.slots < (int64_t{1} << 30), "%s: grid too large", fn);
-  if (plan.slots > 0) {
-    const WsLayout wl = chunks_layout(plan, head_dim);
+  TQ_CHECK_ARG(plan.blocks + plan.few_blocks < (int64_t{1} << 29), "%s: grid too large", fn);
+  PagedParams few = p;
+  if (plan.slots + plan.few_slots > 0) {
+    const ChunksLayout wl = chunks_layout(plan, head_dim);
     if (!workspace || workspace_bytes < wl.total) {
       set_error("%s: workspace of %zu bytes needed (got %zu)", fn, wl.total, workspace ? workspace_bytes : size_t{0});
       return TQ_ERR_WORKSPACE;
     }
     TQ_CHECK_ARG(reinterpret_cast<uintptr_t>(workspace) % 16 == 0, "%s: workspace must be 16-byte aligned", fn);
-    p.ws_ml = reinterpret_cast<float*>(static_cast<char*>(workspace) + wl.ml_off);
-    p.ws_o = reinterpret_cast<float*>(static_cast<char*>(workspace) + wl.o_off);
+    const auto at = [&](size_t off) { return reinterpret_cast<float*>(static_cast<char*>(workspace) + off); };
+    p.ws_ml = at(wl.ml);
+    p.ws_o = at(wl.o);
+    few.ws_ml = at(wl.few_ml);
+    few.ws_o = at(wl.few_o);
   }
-  return launch_chunks(p, head_dim, sb_dtype, plan, starts, queries, static_cast<hipStream_t>(stream));
+  return launch_chunks(p, few, head_dim, sb_dtype, plan, starts, queries, static_cast<hipStream_t>(stream));
 }

@@ -16,6 +16,7 @@
 //   then leave partials (m, l, O).
 // - fp32 queries are two fp16 parts, 22 bits, and take two products a k-step.
 //   fp32 biases are applied in fp32.
+#include "tq_chunk_jobs.h"
 #include "tq_prefill_tile.h"
 
 #include <cfloat>
@@ -31,20 +32,6 @@ struct PgRun {
   int lo, hi;
   uint64_t has;
 };
-
-// Largest of 64 lanes, by the steps of wave_max_dpp (wave_max_i goes through the
-// LDS: six of them were 1.5 us of a launch's start).
-__device__ __forceinline__ int max_of_wave(int v) {
-  v = max(v, __builtin_amdgcn_update_dpp(0, v, 0xB1, 0xF, 0xF, false));
-  v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x4E, 0xF, 0xF, false));
-  v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x141, 0xF, 0xF, false));
-  v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x140, 0xF, 0xF, false));
-  const auto a = __builtin_amdgcn_permlane16_swap(static_cast<unsigned>(v), static_cast<unsigned>(v), false, false);
-  v = max(static_cast<int>(a[0]), static_cast<int>(a[1]));
-  const auto b = __builtin_amdgcn_permlane32_swap(static_cast<unsigned>(v), static_cast<unsigned>(v), false, false);
-  return __builtin_amdgcn_readfirstlane(max(static_cast<int>(b[0]), static_cast<int>(b[1])));
-}
-__device__ __forceinline__ int min_of_wave(int v) { return -max_of_wave(-v); }
 
 // Raw loads behind a uniform address: a 32-bit lane offset beside the scalar base,
 // where global loads of this kernel took 64-bit addresses in vector registers.
@@ -230,149 +217,6 @@ __device__ __forceinline__ void pg_alike(const PfRaw<Gm>& R, int e0, int* ok) {
   }
 }
 
-struct TileParams : PagedParams {
-  int splits;  // workgroups along the tiles (grid y); 1: write p.out
-  // chunks of a batch (nq sequences): their queries are rows starts[b] .. starts[b + 1] - 1
-  // of q and out, of `queries` in all
-  const int* starts;
-  int queries;
-};
-
-// ---- chunks of a batch --------------------------------------------------------
-// A job is (sequence, block of rows, kv head, split of its tiles); the device lays them
-// out from the lengths.  Every workgroup works it out for itself, a sequence a lane: one
-// round trip to the lengths, where a plan of its own would be a launch.
-struct ChunkSeq {
-  int s0, n, len;      // first query, queries, keys
-  int blocks, tiles;   // of rows; of keys (the most that a block of rows attends)
-};
-
-struct ChunkJob {
-  int b, s0, n, len;
-  int blk, kvh, split, splits;
-  int slot;            // of its partials
-};
-
-template <int ROWS, int TK>
-__device__ __forceinline__ ChunkSeq chunk_seq(const TileParams& p, int b) {
-  ChunkSeq c{0, 0, 0, 0, 0};
-  if (b < p.nq) {
-    c.s0 = min(max(p.starts[b], 0), p.queries);
-    c.n = min(max(p.starts[b + 1], c.s0), p.queries) - c.s0;
-    c.len = max(min(p.seq_lens[b], p.n_clamp), 0);
-    c.blocks = (c.n * p.gqa + ROWS - 1) / ROWS;
-    c.tiles = (c.len + TK - 1) / TK;
-    if (p.window > 0) {  // sinks, the rows' windows, and a tile that those begin in
-      const int64_t keys = static_cast<int64_t>(p.window) + ROWS + 2 * TK;
-      c.tiles = static_cast<int>(min(static_cast<int64_t>(c.tiles), keys / TK + p.sinks / TK + 1));
-    }
-  }
-  return c;
-}
-
-__device__ __forceinline__ float sum_of_wave(float v) { return group_sum<64>(v); }
-
-// Tiles of a job at most.  With T >= work / CUs, jobs of split blocks are fewer than 2
-// CUs: a block of t > T tiles makes ceil(t / T) < 2 t / T of them.  Of a few such T, and
-// of no splits, the one with the least estimated time, in the units of plan_paged_tiles:
-// that of a job or of an even share of all.
-constexpr int kMostSplits = 64;
-constexpr int kLeastTiles = 4;
-
-__device__ __forceinline__ int splits_of(const ChunkSeq& c, int T) {
-  return c.tiles <= T ? 1 : min((c.tiles + T - 1) / T, kMostSplits);
-}
-
-template <int ROWS, int TK>
-__device__ __forceinline__ int chunk_tiles(const TileParams& p) {
-  const int lane = threadIdx.x & 63;
-  float work = 0.0f, blocks = 0.0f;
-  int most = 0;
-  for (int b = lane; b - lane < p.nq; b += 64) {
-    const ChunkSeq c = chunk_seq<ROWS, TK>(p, b);
-    const float n = static_cast<float>(c.blocks) * p.Hkv;
-    work += n * c.tiles;
-    blocks += n;
-    if (c.blocks > 0) most = max(most, c.tiles);
-  }
-  work = sum_of_wave(work);
-  blocks = sum_of_wave(blocks);
-  most = max_of_wave(most);
-  constexpr float kTile = ROWS == 64 ? 8.0f : 13.0f, kFixed = ROWS == 64 ? 48.0f : 72.0f;
-  const float cus = static_cast<float>(p.cus), share = work / cus;
-  const auto time = [&](float jobs, int T) {
-    return fmaxf(T * kTile + kFixed, (work * kTile + jobs * kFixed) / cus + (jobs > cus ? 0.5f * T * kTile : 0.0f));
-  };
-  int best = max(most, 1);
-  float least = time(blocks, best);
-#pragma unroll 1
-  for (int k = 2; k <= 8; k += k < 4 ? 1 : 2) {  // shares of 1, 1.5, 2, 3, 4
-    const int T = max(static_cast<int>(fminf(share * (0.5f * k) * 1.0001f, 1e8f)) + 1, kLeastTiles);
-    if (T >= most) break;
-    float jobs = 0.0f;
-    for (int b = lane; b - lane < p.nq; b += 64) {
-      const ChunkSeq c = chunk_seq<ROWS, TK>(p, b);
-      jobs += static_cast<float>(c.blocks) * p.Hkv * splits_of(c, T);
-    }
-    jobs = sum_of_wave(jobs);
-    const float t = time(jobs, T);
-    if (t < least) {
-      least = t;
-      best = T;
-    }
-  }
-  return best;
-}
-
-__device__ __forceinline__ int scan_of_wave(int v) {  // inclusive
-  const int lane = threadIdx.x & 63;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const int y = __shfl_up(v, d, 64);
-    if (lane >= d) v += y;
-  }
-  return v;
-}
-
-// Job j (MERGE: the j-th split block of rows and head), or none: splits 0.
-template <int ROWS, int TK, bool MERGE>
-__device__ __forceinline__ ChunkJob chunk_job(const TileParams& p, int j) {
-  const int T = chunk_tiles<ROWS, TK>(p);
-  const int lane = threadIdx.x & 63;
-  int jobs = 0, slots = 0;  // of the sequences before these
-  ChunkJob r{};
-#pragma unroll 1
-  for (int b0 = 0; b0 < p.nq; b0 += 64) {
-    const ChunkSeq c = chunk_seq<ROWS, TK>(p, b0 + lane);
-    const int s = splits_of(c, T), mine = c.blocks * p.Hkv;
-    const int slot = s > 1 ? mine * s : 0;
-    const int n = MERGE ? (s > 1 ? mine : 0) : mine * s;
-    const int upto = jobs + scan_of_wave(n), slot_upto = slots + scan_of_wave(slot);
-    const uint64_t hit = __ballot(upto > j);
-    if (hit != 0) {
-      const int l = __builtin_ctzll(hit);
-      const auto of = [&](int v) { return __builtin_amdgcn_readlane(v, l); };
-      r.b = b0 + l;
-      r.s0 = of(c.s0);
-      r.n = of(c.n);
-      r.len = of(c.len);
-      r.splits = of(s);
-      const int blocks = of(c.blocks);
-      int at = j - (of(upto) - of(n));
-      r.kvh = at % p.Hkv;
-      at /= p.Hkv;
-      r.split = MERGE ? 0 : at % r.splits;
-      if (!MERGE) at /= r.splits;
-      r.blk = blocks - 1 - at;  // the longest key ranges (last queries) start first
-      r.slot = of(slot_upto) - of(slot) + (r.blk * p.Hkv + r.kvh) * r.splits + r.split;
-      return r;
-    }
-    jobs = __builtin_amdgcn_readlane(upto, 63);
-    slots = __builtin_amdgcn_readlane(slot_upto, 63);
-  }
-  return r;
-}
-
 // RS: 16-row sets of a workgroup.  4: a wave takes 32 keys of a tile (of 64 keys, D
 // 512 of 32); 8 (D < 512): all 64, one half after the other, so that twice as many
 // rows share the staging of a tile (64 sequences with 2 query heads a kv head over
@@ -406,7 +250,7 @@ void paged_tiles_kernel(TileParams p) {
   // heads vary fastest, the longest key ranges (last queries) start first
   ChunkJob job{};
   if constexpr (BATCH) {
-    job = chunk_job<kRows, TK, false>(p, blockIdx.x);
+    job = chunk_job<kRows, TK, false, false>(p, blockIdx.x);
     if (job.splits == 0) return;            // (all waves)
   }
   const int nblk = gridDim.x / p.Hkv;
@@ -1012,35 +856,6 @@ __global__ __launch_bounds__(256) void merge_tiles_kernel(const float* ws_ml, co
   reinterpret_cast<v4f*>(out)[i] = r;
 }
 
-// The outputs of the split blocks of a batch's chunks, a workgroup a quarter of one.
-template <int D, int ROWS>
-__global__ __launch_bounds__(256) void merge_chunks_kernel(TileParams p) {
-  constexpr int TK = D == 512 ? 32 : 64, D4 = D / 4;
-  const ChunkJob job = chunk_job<ROWS, TK, true>(p, blockIdx.x);
-  if (job.splits == 0) return;
-  const int rows = min(job.n * p.gqa - job.blk * ROWS, ROWS);
-  const float2* ml = reinterpret_cast<const float2*>(p.ws_ml) + static_cast<int64_t>(job.slot) * ROWS;
-  const v4f* po = reinterpret_cast<const v4f*>(p.ws_o) + static_cast<int64_t>(job.slot) * ROWS * D4;
-  for (int u = blockIdx.y * 256 + threadIdx.x; u < rows * D4; u += gridDim.y * 256) {
-    const int r = u / D4;
-    float M = -INFINITY, L = 0.0f;
-    for (int k = 0; k < job.splits; ++k) M = fmaxf(M, ml[k * ROWS + r].x);
-    v4f O = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll 4
-    for (int k = 0; k < job.splits; ++k) {
-      const float2 x = ml[k * ROWS + r];
-      const float fk = merge_factor(x.x, M);
-      L = fmaf(x.y, fk, L);
-      O += fk * po[static_cast<int64_t>(k) * ROWS * D4 + u];
-    }
-    v4f y;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) y[e] = normalise(O[e], L, 0.0f);
-    const int row = job.blk * ROWS + r, q = row / p.gqa;
-    reinterpret_cast<v4f*>(p.out)[(static_cast<int64_t>(job.s0 + q) * p.Hq + job.kvh * p.gqa + (row - q * p.gqa)) * D4 + u % D4] = y;
-  }
-}
-
 template <int D, bool F32, int RS, bool BATCH>
 void launch_q(const TileParams& p, dim3 grid, hipStream_t s) {
   if constexpr (!(D == 256 && F32 && RS == 8)) {  // (never planned for fp32 queries)
@@ -1057,17 +872,6 @@ void launch_dim(const TileParams& p, int D, int rs, dim3 grid, hipStream_t s) {
   if (D == 512) launch_q<512, F32, 4, BATCH>(p, grid, s);
   else if (D == 256) rs == 8 ? launch_q<256, F32, 8, BATCH>(p, grid, s) : launch_q<256, F32, 4, BATCH>(p, grid, s);
   else rs == 8 ? launch_q<128, F32, 8, BATCH>(p, grid, s) : launch_q<128, F32, 4, BATCH>(p, grid, s);
-}
-
-template <int D>
-void launch_merge(const TileParams& p, int rs, dim3 grid, hipStream_t s) {
-  if constexpr (D < 512) {
-    if (rs == 8) {
-      merge_chunks_kernel<D, 128><<<grid, 256, 0, s>>>(p);
-      return;
-    }
-  }
-  merge_chunks_kernel<D, 64><<<grid, 256, 0, s>>>(p);
 }
 
 int tile_keys(int D) { return D == 512 ? 32 : 64; }
@@ -1139,39 +943,11 @@ int launch_paged_tiles(const PagedParams& p0, int D, int sb_dtype, TilesPlan pla
   return TQ_OK;
 }
 
-// ---- chunks of a batch --------------------------------------------------------
-
-ChunksPlan plan_chunks(int batch, int queries, int gqa, int Hkv, int D, int max_new, int64_t max_kv_len, bool all32) {
-  ChunksPlan pl{};
-  const int64_t rows = static_cast<int64_t>(std::min(max_new, queries)) * gqa;
-  pl.rs = D == 512 || (D == 256 && all32) || rows <= 64 ? 4 : 8;
-  const int64_t cus = target_wgs();
-  // blocks of rows of any lengths that add up to `queries`
-  pl.blocks = (static_cast<int64_t>(queries) * gqa / (16 * pl.rs) + std::min(batch, queries)) * Hkv;
-  // (see chunk_tiles)
-  const int64_t most = (max_kv_len + tile_keys(D) - 1) / tile_keys(D);
-  const int64_t splits = std::min<int64_t>((most + kLeastTiles - 1) / kLeastTiles, kMostSplits);
-  pl.slots = splits > 1 ? std::min(2 * cus, pl.blocks * splits) : 0;
-  return pl;
-}
-
-int launch_chunks(const PagedParams& p0, int D, int sb_dtype, const ChunksPlan& plan, const int* starts, int queries,
-                  hipStream_t s) {
-  TileParams p{};
-  static_cast<PagedParams&>(p) = p0;
-  p.splits = 1;
-  p.starts = starts;
-  p.queries = queries;
-  const dim3 grid(static_cast<unsigned>(plan.blocks + plan.slots));
-  if (sb_dtype == TQ_F32) launch_dim<true, true>(p, D, plan.rs, grid, s);
-  else launch_dim<false, true>(p, D, plan.rs, grid, s);
+int launch_chunk_tiles(const TileParams& p, int D, int sb_dtype, int rs, int64_t jobs, hipStream_t s) {
+  const dim3 grid(static_cast<unsigned>(jobs));
+  if (sb_dtype == TQ_F32) launch_dim<true, true>(p, D, rs, grid, s);
+  else launch_dim<false, true>(p, D, rs, grid, s);
   TQ_CHECK_LAUNCH("paged_tiles_kernel");
-  if (plan.slots == 0) return TQ_OK;
-  const dim3 merge(static_cast<unsigned>(std::min(plan.blocks, plan.slots / 2)), 4);
-  if (D == 512) launch_merge<512>(p, plan.rs, merge, s);
-  else if (D == 256) launch_merge<256>(p, plan.rs, merge, s);
-  else launch_merge<128>(p, plan.rs, merge, s);
-  TQ_CHECK_LAUNCH("merge_chunks_kernel");
   return TQ_OK;
 }
 
