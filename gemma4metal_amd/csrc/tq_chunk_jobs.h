@@ -14,6 +14,7 @@ struct TileParams : PagedParams {
   // a kv head) are the business of paged_few_kernel, the others of paged_tiles_kernel.
   const int* starts;
   int queries, few;
+  int max_new;  // queries of a sequence that are served
 };
 
 int launch_chunk_tiles(const TileParams& p, int D, int sb_dtype, int rs, int64_t jobs, hipStream_t s);
@@ -35,7 +36,7 @@ __device__ __forceinline__ int max_of_wave(int v) {
 __device__ __forceinline__ int min_of_wave(int v) { return -max_of_wave(-v); }
 
 // A job is (sequence, block of rows, kv head, split of its tiles); the device lays them
-// out from the lengths.  Every workgroup works it out for itself, a sequence a lane: one
+// out from the lengths.  A wave of every workgroup works it out, a sequence a lane: one
 // round trip to the lengths, where a plan of its own would be a launch.
 struct ChunkSeq {
   int s0, n, len;      // first query, queries, keys
@@ -47,6 +48,7 @@ struct ChunkJob {
   int blk, kvh, split, splits;
   int slot;            // of its partials
 };
+constexpr int kJobInts = sizeof(ChunkJob) / sizeof(int);
 
 template <int ROWS, int TK, bool FEW>
 __device__ __forceinline__ ChunkSeq chunk_seq(const TileParams& p, int b) {
@@ -55,7 +57,7 @@ __device__ __forceinline__ ChunkSeq chunk_seq(const TileParams& p, int b) {
     c.s0 = min(max(p.starts[b], 0), p.queries);
     c.n = min(max(p.starts[b + 1], c.s0), p.queries) - c.s0;
     c.len = max(min(p.seq_lens[b], p.n_clamp), 0);
-    if ((c.n * p.gqa <= p.few) == FEW) c.blocks = (c.n * p.gqa + ROWS - 1) / ROWS;
+    if ((c.n * p.gqa <= p.few) == FEW) c.blocks = (min(c.n, p.max_new) * p.gqa + ROWS - 1) / ROWS;
     c.tiles = (c.len + TK - 1) / TK;
     if (p.window > 0) {  // sinks, the rows' windows, and a tile that those begin in
       const int64_t keys = static_cast<int64_t>(p.window) + ROWS + 2 * TK;
@@ -67,30 +69,40 @@ __device__ __forceinline__ ChunkSeq chunk_seq(const TileParams& p, int b) {
 
 __device__ __forceinline__ float sum_of_wave(float v) { return group_sum<64>(v); }
 
-// Tiles of a job at most.  With T >= work / CUs, jobs of split blocks are fewer than 2
-// CUs: a block of t > T tiles makes ceil(t / T) < 2 t / T of them.  Of a few such T, and
-// of no splits, the one with the least estimated time, in the units of plan_paged_tiles:
-// that of a job or of an even share of all.
+// Tiles of a job at most.  With T >= work / cus (workgroups that run at once), splits make
+// fewer than cus more jobs of the blocks, and jobs of split blocks are fewer than 2 cus: a
+// block of t > T tiles makes ceil(t / T) < 1 + t / T < 2 t / T of them.  Of a few such T,
+// and of no splits, the one with the least estimated time, in the units of
+// plan_paged_tiles: that of a job or of an even share of all.
 constexpr int kMostSplits = 64;
 template <bool FEW>
 constexpr int kLeastTiles = FEW ? 16 : 4;
 
+// (one function of the lengths for all who ask; one more or less than the quotient rounded
+// up would do: a block's tiles are shared out evenly whatever it is)
 __device__ __forceinline__ int splits_of(const ChunkSeq& c, int T) {
-  return c.tiles <= T ? 1 : min((c.tiles + T - 1) / T, kMostSplits);
+  return c.tiles <= T ? 1 : min(static_cast<int>(ceilf(c.tiles * __builtin_amdgcn_rcpf(static_cast<float>(T)))), kMostSplits);
+}
+
+// f(sequence of this lane) for the sequences of the batch, 64
+// at a time; `first`: the first 64, loaded once.
+template <int ROWS, int TK, bool FEW, typename F>
+__device__ __forceinline__ void each_seq(const TileParams& p, const ChunkSeq& first, F f) {
+  f(first);
+#pragma unroll 1
+  for (int b0 = 64; b0 < p.nq; b0 += 64) f(chunk_seq<ROWS, TK, FEW>(p, b0 + static_cast<int>(threadIdx.x & 63)));
 }
 
 template <int ROWS, int TK, bool FEW>
-__device__ __forceinline__ int chunk_tiles(const TileParams& p) {
-  const int lane = threadIdx.x & 63;
+__device__ __forceinline__ int chunk_tiles(const TileParams& p, const ChunkSeq& first) {
   float work = 0.0f, blocks = 0.0f;
   int most = 0;
-  for (int b = lane; b - lane < p.nq; b += 64) {
-    const ChunkSeq c = chunk_seq<ROWS, TK, FEW>(p, b);
+  each_seq<ROWS, TK, FEW>(p, first, [&](const ChunkSeq& c) {
     const float n = static_cast<float>(c.blocks) * p.Hkv;
     work += n * c.tiles;
     blocks += n;
     if (c.blocks > 0) most = max(most, c.tiles);
-  }
+  });
   work = sum_of_wave(work);
   blocks = sum_of_wave(blocks);
   most = max_of_wave(most);
@@ -106,12 +118,8 @@ __device__ __forceinline__ int chunk_tiles(const TileParams& p) {
     const int T = max(static_cast<int>(fminf(share * (0.5f * k) * 1.0001f, 1e8f)) + 1, kLeastTiles<FEW>);
     if (T >= most) break;
     float jobs = 0.0f;
-    for (int b = lane; b - lane < p.nq; b += 64) {
-      const ChunkSeq c = chunk_seq<ROWS, TK, FEW>(p, b);
-      jobs += static_cast<float>(c.blocks) * p.Hkv * splits_of(c, T);
-    }
-    jobs = sum_of_wave(jobs);
-    const float t = time(jobs, T);
+    each_seq<ROWS, TK, FEW>(p, first, [&](const ChunkSeq& c) { jobs += static_cast<float>(c.blocks) * p.Hkv * splits_of(c, T); });
+    const float t = time(sum_of_wave(jobs), T);
     if (t < least) {
       least = t;
       best = T;
@@ -132,14 +140,15 @@ __device__ __forceinline__ int scan_of_wave(int v) {  // inclusive
 
 // Job j (MERGE: the j-th split block of rows and head), or none: splits 0.
 template <int ROWS, int TK, bool FEW, bool MERGE>
-__device__ __forceinline__ ChunkJob chunk_job(const TileParams& p, int j) {
-  const int T = chunk_tiles<ROWS, TK, FEW>(p);
+__device__ __forceinline__ ChunkJob find_chunk_job(const TileParams& p, int j) {
   const int lane = threadIdx.x & 63;
+  const ChunkSeq first = chunk_seq<ROWS, TK, FEW>(p, lane);
+  const int T = chunk_tiles<ROWS, TK, FEW>(p, first);
   int jobs = 0, slots = 0;  // of the sequences before these
   ChunkJob r{};
 #pragma unroll 1
   for (int b0 = 0; b0 < p.nq; b0 += 64) {
-    const ChunkSeq c = chunk_seq<ROWS, TK, FEW>(p, b0 + lane);
+    const ChunkSeq c = b0 == 0 ? first : chunk_seq<ROWS, TK, FEW>(p, b0 + lane);
     const int s = splits_of(c, T), mine = c.blocks * p.Hkv;
     const int slot = s > 1 ? mine * s : 0;
     const int n = MERGE ? (s > 1 ? mine : 0) : mine * s;
@@ -167,6 +176,26 @@ __device__ __forceinline__ ChunkJob chunk_job(const TileParams& p, int j) {
     slots = __builtin_amdgcn_readlane(slot_upto, 63);
   }
   return r;
+}
+
+// The same, found by the first wave for the whole workgroup (all of its threads ask; a
+// barrier).
+template <int ROWS, int TK, bool FEW, bool MERGE>
+__device__ __forceinline__ ChunkJob chunk_job(const TileParams& p, int j) {
+  __shared__ int told[kJobInts];
+  if (threadIdx.x < 64) {
+    const ChunkJob r = find_chunk_job<ROWS, TK, FEW, MERGE>(p, j);
+    const int v[kJobInts] = {r.b, r.s0, r.n, r.len, r.blk, r.kvh, r.split, r.splits, r.slot};
+    if (threadIdx.x == 0) {
+#pragma unroll
+      for (int i = 0; i < kJobInts; ++i) told[i] = v[i];
+    }
+  }
+  __syncthreads();
+  int v[kJobInts];
+#pragma unroll
+  for (int i = 0; i < kJobInts; ++i) v[i] = __builtin_amdgcn_readfirstlane(told[i]);
+  return {v[0], v[1], v[2], v[3], v[4], v[5], v[6], v[7], v[8]};
 }
 
 }  // namespace

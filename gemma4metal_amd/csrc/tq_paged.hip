@@ -349,10 +349,10 @@ ChunksLayout chunks_layout(const ChunksPlan& pl, int D) {
     return from;
   };
   ChunksLayout w;
-  w.ml = take(pl.slots * 16 * pl.rs, 2);
-  w.o = take(pl.slots * 16 * pl.rs, D);
-  w.few_ml = take(pl.few_slots * 16, 2);
-  w.few_o = take(pl.few_slots * 16, D);
+  w.ml = take(pl.tiles.slots * 16 * pl.rs, 2);
+  w.o = take(pl.tiles.slots * 16 * pl.rs, D);
+  w.few_ml = take(pl.few_rows.slots * 16, 2);
+  w.few_o = take(pl.few_rows.slots * 16, D);
   w.total = at;
   return w;
 }
@@ -367,7 +367,7 @@ extern "C" size_t tq_sdpa_int4_paged_chunks_workspace_size(int batch, int querie
   size_t most = 0;
   for (bool all32 : {false, true}) {
     const ChunksPlan pl = plan_chunks(batch, queries, num_heads / num_kv_heads, num_kv_heads, head_dim, max_new, max_kv_len, all32);
-    if (pl.slots + pl.few_slots > 0) most = std::max(most, chunks_layout(pl, head_dim).total);
+    if (pl.tiles.slots + pl.few_rows.slots > 0) most = std::max(most, chunks_layout(pl, head_dim).total);
   }
   return most;
 }
@@ -399,9 +399,9 @@ extern "C" int tq_sdpa_int4_paged_chunks(const void* q, tq_dtype q_dtype, const 
   p.n_clamp = max_kv_len;
   const ChunksPlan plan = plan_chunks(batch, queries, gqa_factor, num_kv_heads, head_dim, max_new, max_kv_len,
                                       q_dtype == TQ_F32 && sb_dtype == TQ_F32);
-  TQ_CHECK_ARG(plan.blocks + plan.few_blocks < (int64_t{1} << 29), "%s: grid too large", fn);
+  TQ_CHECK_ARG(plan.tiles.jobs < (int64_t{1} << 30) && plan.few_rows.jobs < (int64_t{1} << 30), "%s: grid too large", fn);
   PagedParams few = p;
-  if (plan.slots + plan.few_slots > 0) {
+  if (plan.tiles.slots + plan.few_rows.slots > 0) {
     const ChunksLayout wl = chunks_layout(plan, head_dim);
     if (!workspace || workspace_bytes < wl.total) {
       set_error("%s: workspace of %zu bytes needed (got %zu)", fn, wl.total, workspace ? workspace_bytes : size_t{0});
@@ -414,5 +414,5 @@ extern "C" int tq_sdpa_int4_paged_chunks(const void* q, tq_dtype q_dtype, const 
     few.ws_ml = at(wl.few_ml);
     few.ws_o = at(wl.few_o);
   }
-  return launch_chunks(p, few, head_dim, sb_dtype, plan, starts, queries, static_cast<hipStream_t>(stream));
+  return launch_chunks(p, few, head_dim, sb_dtype, plan, starts, queries, max_new, static_cast<hipStream_t>(stream));
 }

@@ -29,8 +29,9 @@ constexpr int kFewBlock = 16;  // rows of a workgroup
 template <int D, bool F32>
 struct FewGeom {
   using SB = typename std::conditional<F32, float, _Float16>::type;
-  // D 512: one wave a SIMD, for its 128 accumulators and as many words in flight
-  static constexpr int NW = D == 512 ? 4 : 8, NT = 64 * NW;
+  // Four waves a workgroup; two workgroups a CU (one streams under the other's start and
+  // end), at D 512 one, for its 128 accumulators and as many words in flight.
+  static constexpr int NW = 4, NT = 64 * NW;
   static constexpr int W = D / 8, NG = D / 64;
   static constexpr int WP = W + 4;              // row stride in LDS: operand reads reach distinct banks
   static constexpr int NK = W / 8;              // 16-byte pieces of 32 keys' words, per lane
@@ -104,6 +105,25 @@ __device__ __forceinline__ uint32_t few_centre(uint32_t t, uint32_t mask, v2h of
   uint32_t b;
   asm("v_and_or_b32 %0, %1, %2, %3" : "=v"(b) : "v"(t), "v"(mask), "s"(0x64006400u));
   return __builtin_bit_cast(uint32_t, __builtin_bit_cast(v2h, b) + off);
+}
+
+// y0 f, y1 f as a packed fp16 pair, and what that pair leaves of them: mixed-precision
+// fmas, each rounded once (the remainder is of the pair that is stored).
+__device__ __forceinline__ uint32_t few_high(float y0, float y1, float f) {
+  uint32_t r;
+  asm("v_fma_mixlo_f16 %0, %1, %3, 0 op_sel_hi:[0,0,0]\n\t"
+      "v_fma_mixhi_f16 %0, %2, %3, 0 op_sel_hi:[0,0,0]"
+      : "=&v"(r)
+      : "v"(y0), "v"(y1), "v"(f));
+  return r;
+}
+__device__ __forceinline__ uint32_t few_low(uint32_t h, float y0, float y1, float f) {
+  uint32_t r;
+  asm("v_fma_mixlo_f16 %0, %1, %3, -%4 op_sel_hi:[0,0,1]\n\t"
+      "v_fma_mixhi_f16 %0, %2, %3, -%4 op_sel:[0,0,1] op_sel_hi:[0,0,1]"
+      : "=&v"(r)
+      : "v"(y0), "v"(y1), "v"(f), "v"(h));
+  return r;
 }
 
 template <int D, bool F32, bool Q32>
@@ -261,8 +281,12 @@ void paged_few_kernel(TileParams p) {
 #pragma unroll
   for (int b = 0; b < 4 * NG; ++b) o[b] = z;
   float bs[NG];  // sums of p (b_v + 8 s_v)
+  float ef[NG];  // a power of two: what the weights p s_v of a row and group go in times
 #pragma unroll
-  for (int g = 0; g < NG; ++g) bs[g] = 0.0f;
+  for (int g = 0; g < NG; ++g) {
+    bs[g] = 0.0f;
+    ef[g] = 0x1p120f;
+  }
   float m_ref = -INFINITY, l_run = 0.0f;
   // rows m < 8 of a V operand are the low nibbles of a byte of word m, the others the
   // high ones (16 times as large) of word m - 8
@@ -349,6 +373,20 @@ void paged_few_kernel(TileParams p) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) sc[4 * h + e] = s[e];
     }
+    row4 vs[8], vb[8];
+    uint32_t w[8];
+    const auto v_rows = [&](int b) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int key = 16 * (j >> 2) + 4 * c + (j & 3);
+        vs[j] = scale_row(2, key, b);
+        vb[j] = scale_row(3, key, b);
+      }
+    };
+    const auto v_words = [&](int g, uint32_t (&to)[8]) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) to[j] = S.v[16 * (j >> 2) + 4 * c + (j & 3)][8 * g + (m & 7)];
+    };
     // whether all of these keys are attended by all rows; wave-uniform
     const bool inside = t0 <= hi_min - 32 && (t0 >= lo_max || t0 <= p.sinks - 32);
     if (!inside) {
@@ -387,13 +425,7 @@ void paged_few_kernel(TileParams p) {
     // ---- O^T += V^T P^T -----------------------------------------------------------------
 #pragma unroll
     for (int b = 0; b < NG / G4; ++b) {
-      row4 vs[8], vb[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int key = 16 * (j >> 2) + 4 * c + (j & 3);
-        vs[j] = scale_row(2, key, b);
-        vb[j] = scale_row(3, key, b);
-      }
+      v_rows(b);
       if (!inside) {  // a key that this row does not attend may hold anything
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
@@ -408,9 +440,7 @@ void paged_few_kernel(TileParams p) {
 #pragma unroll
       for (int gi = 0; gi < G4; ++gi) {
         const int g = G4 * b + gi;
-        uint32_t w[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) w[j] = S.v[16 * (j >> 2) + 4 * c + (j & 3)][8 * g + (m & 7)];
+        v_words(g, w);
         float y[8], big = 0.0f;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
@@ -419,15 +449,20 @@ void paged_few_kernel(TileParams p) {
           bs[g] = fmaf(pw[j], fmaf(s, 8.0f, static_cast<float>(vb[j][gi])), bs[g]);
           big = fmaxf(big, fabsf(y[j]));
         }
-        // the largest to 2^13 .. 2^14 (an infinity, of exponent 0, stays one)
-        const int k = min(14 - __builtin_amdgcn_frexp_expf(xor32_max(xor16_max(big))), 120);
-        const float un = ldexpf(1.0f, -k);
+        if (__any(big * ef[g] > 0x1p15f)) {
+          // the row's largest to 2^13 .. 2^14 (an infinity, of exponent 0, stays one)
+          const float top = xor32_max(xor16_max(big));
+          const float now = ldexpf(1.0f, min(14 - __builtin_amdgcn_frexp_expf(top), 120));
+          const float fr = top * ef[g] > 0x1p15f && now < ef[g] ? ldexpf(now, 1 - __builtin_amdgcn_frexp_expf(ef[g])) : 1.0f;
+          ef[g] *= fr;
+#pragma unroll
+          for (int x = 0; x < 4; ++x) o[4 * g + x] *= fr;
+        }
         u32x4 hw, lw;
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-          const float y0 = ldexpf(y[2 * q], k), y1 = ldexpf(y[2 * q + 1], k);
-          hw[q] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(y0, y1));
-          lw[q] = pf_rem_pair(hw[q], y0, y1);
+          hw[q] = few_high(y[2 * q], y[2 * q + 1], ef[g]);
+          lw[q] = few_low(hw[q], y[2 * q], y[2 * q + 1], ef[g]);
         }
         const v8h bh = __builtin_bit_cast(v8h, hw), bl = __builtin_bit_cast(v8h, lw);
 #pragma unroll
@@ -436,17 +471,15 @@ void paged_few_kernel(TileParams p) {
 #pragma unroll
           for (int q = 0; q < 4; ++q)  // byte x of two keys' words into the low bytes of the halves
             a[q] = few_centre(__builtin_amdgcn_perm(w[2 * q + 1], w[2 * q], 0x0C040C00u + 0x00010001u * x), vmask, voff);
-          v4f t = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, a), bh, z, 0, 0, 0);
-          t = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, a), bl, t, 0, 0, 0);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) o[4 * g + x][e] = fmaf(t[e], un, o[4 * g + x][e]);
+          v4f& acc = o[4 * g + x];
+          acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, a), bh, acc, 0, 0, 0);
+          acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, a), bl, acc, 0, 0, 0);
         }
       }
     }
   }
 
   // ---- merge of the waves' partials of every row, and the output --------------------
-  const float un = c < 2 ? 1.0f : 0.0625f;  // high nibbles were 16 times as large
   const float lt = xor32_sum(xor16_sum(l_run));
   if (c == 0) {
     ml[wave][m] = m_ref;
@@ -457,6 +490,7 @@ void paged_few_kernel(TileParams p) {
 #pragma unroll
   for (int g = 0; g < NG; ++g) {
     const float bg = xor32_sum(xor16_sum(bs[g]));
+    const float un = ldexpf(c < 2 ? 1.0f : 0.0625f, 1 - __builtin_amdgcn_frexp_expf(ef[g]));  // high nibbles were 16 times as large
 #pragma unroll
     for (int x = 0; x < 4; ++x)
 #pragma unroll
@@ -492,41 +526,60 @@ void paged_few_kernel(TileParams p) {
   }
 }
 
-// The outputs of the split blocks of one kernel's jobs, by workgroups x, y of a grid.
+// The outputs of a split block of one kernel's jobs, by a workgroup.
+constexpr int kMergeThreads = 1024;
+
 template <int D, int ROWS, int TK, bool FEW>
-__device__ __forceinline__ void merge_jobs(const TileParams& p, int y, int ny) {
+__device__ __forceinline__ void merge_job(const TileParams& p) {
   constexpr int D4 = D / 4;
   const ChunkJob job = chunk_job<ROWS, TK, FEW, true>(p, blockIdx.x);
   if (job.splits == 0) return;
   const int rows = min(job.n * p.gqa - job.blk * ROWS, ROWS);
   const float2* ml = reinterpret_cast<const float2*>(p.ws_ml) + static_cast<int64_t>(job.slot) * ROWS;
   const v4f* po = reinterpret_cast<const v4f*>(p.ws_o) + static_cast<int64_t>(job.slot) * ROWS * D4;
-  for (int u = y * 256 + threadIdx.x; u < rows * D4; u += ny * 256) {
+  for (int u = threadIdx.x; u < rows * D4; u += kMergeThreads) {
     const int r = u / D4;
     float M = -INFINITY, L = 0.0f;
-    for (int k = 0; k < job.splits; ++k) M = fmaxf(M, ml[k * ROWS + r].x);
     v4f O = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll 4
-    for (int k = 0; k < job.splits; ++k) {
-      const float2 x = ml[k * ROWS + r];
-      const float fk = merge_factor(x.x, M);
-      L = fmaf(x.y, fk, L);
-      O += fk * po[static_cast<int64_t>(k) * ROWS * D4 + u];
-    }
-    v4f v;
+    for (int k0 = 0; k0 < job.splits; k0 += 4) {  // four in flight (past the end: the last one again, of weight 0)
+      float2 x[4];
+      v4f v[4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = normalise(O[e], L, 0.0f);
+      for (int i = 0; i < 4; ++i) {
+        const int k = min(k0 + i, job.splits - 1);
+        x[i] = ml[k * ROWS + r];
+        v[i] = po[static_cast<int64_t>(k) * ROWS * D4 + u];
+      }
+      float now = M;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (k0 + i >= job.splits) x[i].x = -INFINITY;
+        now = fmaxf(now, x[i].x);
+      }
+      const float f = merge_factor(M, now);
+      L *= f;
+      O *= f;
+      M = now;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float fk = merge_factor(x[i].x, M);
+        L = fmaf(x[i].y, fk, L);
+        O += fk * v[i];
+      }
+    }
+    v4f y;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) y[e] = normalise(O[e], L, 0.0f);
     const int row = job.blk * ROWS + r, q = row / p.gqa;
-    reinterpret_cast<v4f*>(p.out)[(static_cast<int64_t>(job.s0 + q) * p.Hq + job.kvh * p.gqa + (row - q * p.gqa)) * D4 + u % D4] = v;
+    reinterpret_cast<v4f*>(p.out)[(static_cast<int64_t>(job.s0 + q) * p.Hq + job.kvh * p.gqa + (row - q * p.gqa)) * D4 + u % D4] = y;
   }
 }
 
-// few: the parameters of paged_few_kernel, y 0 .. few_y - 1; tiles: the others.
+// few: the parameters of paged_few_kernel's jobs (y 0, if few_y is 1); tiles: the others'.
 template <int D, int ROWS>
-__global__ __launch_bounds__(256) void merge_chunks_kernel(TileParams few, TileParams tiles, int few_y) {
-  const int y = blockIdx.y;
-  if (y < few_y) merge_jobs<D, kFewBlock, 32, true>(few, y, few_y);
-  else merge_jobs<D, ROWS, D == 512 ? 32 : 64, false>(tiles, y - few_y, gridDim.y - few_y);
+__global__ __launch_bounds__(kMergeThreads) void merge_chunks_kernel(TileParams few, TileParams tiles, int few_y) {
+  if (static_cast<int>(blockIdx.y) < few_y) merge_job<D, kFewBlock, 32, true>(few);
+  else merge_job<D, ROWS, D == 512 ? 32 : 64, false>(tiles);
 }
 
 template <bool F32>
@@ -546,18 +599,22 @@ template <int D>
 void launch_merge(const TileParams& few, const TileParams& tiles, int few_y, int rs, dim3 grid, hipStream_t s) {
   if constexpr (D < 512) {
     if (rs == 8) {
-      merge_chunks_kernel<D, 128><<<grid, 256, 0, s>>>(few, tiles, few_y);
+      merge_chunks_kernel<D, 128><<<grid, kMergeThreads, 0, s>>>(few, tiles, few_y);
       return;
     }
   }
-  merge_chunks_kernel<D, 64><<<grid, 256, 0, s>>>(few, tiles, few_y);
+  merge_chunks_kernel<D, 64><<<grid, kMergeThreads, 0, s>>>(few, tiles, few_y);
 }
 
-// Slots for the partials of split jobs: fewer than 2 CUs of them (chunk_tiles).
-int64_t slots_of(int64_t blocks, int64_t tiles, int least) {
+// The jobs of `blocks` blocks of rows of at most `tiles` tiles on `cus` workgroups at
+// once, and the slots for the partials of split ones (chunk_tiles has both bounds).
+ChunkJobs jobs_of(int64_t blocks, int64_t tiles, int least, int64_t cus) {
   const int64_t splits = std::min<int64_t>((tiles + least - 1) / least, kMostSplits);
-  return splits > 1 ? std::min<int64_t>(2 * target_wgs(), blocks * splits) : 0;
+  if (blocks == 0 || splits <= 1) return {blocks, 0};
+  return {blocks + std::min(cus, blocks * (splits - 1)), std::min(2 * cus, blocks * splits)};
 }
+
+int64_t few_cus(int D) { return D == 512 ? target_wgs() : 2 * target_wgs(); }
 
 }  // namespace
 
@@ -570,19 +627,21 @@ ChunksPlan plan_chunks(int batch, int queries, int gqa, int Hkv, int D, int max_
   pl.few = rows <= kFewRows ? INT_MAX : batch > 1 && all / batch < 128 ? kFewRows : 0;
   // blocks of rows of any chunks that add up to `queries`
   if (pl.few != INT_MAX) {
-    pl.blocks = (all / (16 * pl.rs) + std::min(seqs, all / (pl.few + 1))) * Hkv;
+    const int64_t n = std::min(seqs, all / (pl.few + 1)), R = 16 * pl.rs;
     const int tile = D == 512 ? 32 : 64;
-    pl.slots = slots_of(pl.blocks, (max_kv_len + tile - 1) / tile, kLeastTiles<false>);
+    pl.tiles = jobs_of(std::min(all / R + n, n * ((rows + R - 1) / R)) * Hkv, (max_kv_len + tile - 1) / tile,
+                       kLeastTiles<false>, target_wgs());
   }
   if (pl.few != 0) {
-    pl.few_blocks = (pl.few == INT_MAX ? all / kFewBlock + seqs : seqs * (kFewRows / kFewBlock)) * Hkv;
-    pl.few_slots = slots_of(pl.few_blocks, (max_kv_len + 31) / 32, kLeastTiles<true>);
+    const int64_t blocks = (std::min<int64_t>(rows, pl.few) + kFewBlock - 1) / kFewBlock;
+    pl.few_rows = jobs_of(std::min(all / kFewBlock + seqs, seqs * blocks) * Hkv, (max_kv_len + 31) / 32,
+                          kLeastTiles<true>, few_cus(D));
   }
   return pl;
 }
 
 int launch_chunks(const PagedParams& p0, const PagedParams& few0, int D, int sb_dtype, const ChunksPlan& plan,
-                  const int* starts, int queries, hipStream_t s) {
+                  const int* starts, int queries, int max_new, hipStream_t s) {
   TileParams p{}, few{};
   static_cast<PagedParams&>(p) = p0;
   static_cast<PagedParams&>(few) = few0;
@@ -590,18 +649,20 @@ int launch_chunks(const PagedParams& p0, const PagedParams& few0, int D, int sb_
   p.starts = few.starts = starts;
   p.queries = few.queries = queries;
   p.few = few.few = plan.few;
-  if (plan.blocks > 0)
-    if (int r = launch_chunk_tiles(p, D, sb_dtype, plan.rs, plan.blocks + plan.slots, s)) return r;
-  if (plan.few_blocks > 0) {
-    const dim3 grid(static_cast<unsigned>(plan.few_blocks + plan.few_slots));
+  p.max_new = few.max_new = max_new;
+  few.cus = static_cast<int>(few_cus(D));
+  if (plan.tiles.jobs > 0)
+    if (int r = launch_chunk_tiles(p, D, sb_dtype, plan.rs, plan.tiles.jobs, s)) return r;
+  if (plan.few_rows.jobs > 0) {
+    const dim3 grid(static_cast<unsigned>(plan.few_rows.jobs));
     if (sb_dtype == TQ_F32) launch_few<true>(few, D, grid, s);
     else launch_few<false>(few, D, grid, s);
     TQ_CHECK_LAUNCH("paged_few_kernel");
   }
-  const int few_y = plan.few_slots > 0 ? 1 : 0, tiles_y = plan.slots > 0 ? 4 : 0;
+  const int few_y = plan.few_rows.slots > 0 ? 1 : 0, tiles_y = plan.tiles.slots > 0 ? 1 : 0;
   if (few_y + tiles_y == 0) return TQ_OK;
-  const int64_t jobs = std::max(std::min(plan.blocks, plan.slots / 2), std::min(plan.few_blocks, plan.few_slots / 2));
-  const dim3 grid(static_cast<unsigned>(jobs), few_y + tiles_y);
+  // (a split block has two slots at least)
+  const dim3 grid(static_cast<unsigned>(std::max(plan.few_rows.slots, plan.tiles.slots) / 2), few_y + tiles_y);
   if (D == 512) launch_merge<512>(few, p, few_y, plan.rs, grid, s);
   else if (D == 256) launch_merge<256>(few, p, few_y, plan.rs, grid, s);
   else launch_merge<128>(few, p, few_y, plan.rs, grid, s);

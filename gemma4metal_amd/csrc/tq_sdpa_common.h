@@ -888,18 +888,20 @@ struct TilesPlan {
 };
 TilesPlan plan_paged_tiles(int64_t rows, int Hkv, int D, int64_t keys, int64_t longest, bool all32);
 int launch_paged_tiles(const PagedParams& p, int D, int sb_dtype, TilesPlan plan, bool partials, hipStream_t stream);
-// Chunks of a batch (tq_paged_chunks.hip): of paged_tiles_kernel and of paged_few_kernel
-// (sequences of at most `few` rows a kv head) the blocks of rows of every kv head at most,
-// 0 where it has none, and the slots for the partials of blocks that the device splits
-// (of 16 rs and of 16 rows; 0: no splits).  p and few: the same call, with the workspaces
-// of the two.
+// Chunks of a batch (tq_paged_chunks.hip): the jobs of paged_tiles_kernel and of
+// paged_few_kernel (sequences of at most `few` rows a kv head) at most, 0 where it has none,
+// and the slots for the partials of blocks that the device splits (of 16 rs and of 16
+// rows; 0: no splits).  p and few: the same call, with the workspaces of the two.
+struct ChunkJobs {
+  int64_t jobs, slots;
+};
 struct ChunksPlan {
   int rs, few;
-  int64_t blocks, slots, few_blocks, few_slots;
+  ChunkJobs tiles, few_rows;
 };
 ChunksPlan plan_chunks(int batch, int queries, int gqa, int Hkv, int D, int max_new, int64_t max_kv_len, bool all32);
 int launch_chunks(const PagedParams& p, const PagedParams& few, int D, int sb_dtype, const ChunksPlan& plan,
-                  const int* starts, int queries, hipStream_t stream);
+                  const int* starts, int queries, int max_new, hipStream_t stream);
 // Merge of the split partials of a launch with ext_merge = 1 (batch b of
 // grid.y): tq_sdpa_hc.hip.
 int launch_merge_splits(const SdpaParams& p, int D, int batch, hipStream_t stream);

@@ -306,9 +306,9 @@ def sdpa_int4_paged_chunks(queries: torch.Tensor,
     the last W, or t < num_sinks; none: 0.
 
     Lengths and chunks are read on the device.  ``max_kv_len`` bounds the lengths
-    (longer ones are cut to it); the table's reach by default.  ``max_new`` is the
-    longest chunk, for the choice of the kernel only; N by default.  Returns (N, Hq, D)
-    float32; rows of ``out`` behind starts[B] stay as they were."""
+    (longer ones are cut to it); the table's reach by default.  ``max_new`` bounds the
+    chunks (queries behind a chunk's first max_new may be left out); N by default.
+    Returns (N, Hq, D) float32; rows of ``out`` behind starts[B] stay as they were."""
     _check_cuda("queries", queries)
     _need(queries.dim() == 3 and queries.dtype in _DT, "queries must be (N, Hq, D) float32, float16 or bfloat16")
     N, Hq, D = queries.shape

@@ -329,9 +329,9 @@ int tq_sdpa_int4_paged_prefill(const void* q, tq_dtype q_dtype,
  * that position iff sliding_window == 0, t is among the last sliding_window up to it,
  * or t < num_sinks; none: 0.  starts, DEVICE int32 [batch + 1], ascends from 0 to
  * queries; rows of out behind starts[batch] stay as they were.  Lengths and chunks are
- * on the device, so that a captured call serves any of them:
- * max_new (a sequence's queries) and max_kv_len bound nothing but the plan and the
- * lengths; a longer chunk is served all the same.
+ * on the device, so that a captured call serves any of them; max_kv_len and max_new bound
+ * a sequence's keys and its queries (lengths are cut to it; of the queries behind a
+ * chunk's first max_new, which may be served or not, nothing can be said).
  * Workspace: tq_sdpa_int4_paged_chunks_workspace_size(...) bytes, 16-byte aligned, of
  * which the first 256 KiB are left as they are (one workspace serves this call and the
  * decode calls, in turn); NULL where that is 0; calls that may overlap need one each. */
