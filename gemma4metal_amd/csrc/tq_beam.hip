@@ -5,6 +5,7 @@
 #include <math.h>
 
 #include <algorithm>
+#include <cfloat>
 
 namespace tq {
 namespace {
@@ -13,14 +14,15 @@ namespace {
 // total(w, t) = score[w] + x[w][t] - log sum_t' exp x[w][t'], and of a group's W V
 // totals the K largest, the lowest (w, t) first among equals.
 //
-// One pass over the logits leaves the largest and the sum of exponentials of every
-// segment of kSeg tokens.  An element of the K best lies in one of the K segments
+// One pass over the logits leaves the largest of every segment of kSeg tokens and the sum
+// of exponentials of every kScanWaves segments.  An element of the K best lies in one of the K segments
 // whose largest totals come first in the same order (the largest of K segments before
 // its own would all come before it), so that the second kernel reads K segments again
 // and nothing else: the work does not depend on the values, and no candidate list is
 // kept while streaming.  Totals are compared in 64 bits: beams are told apart by
 // scores of any distance, and equal ones have to be equal.
 constexpr int kSeg = 1024;
+constexpr int kScanWaves = 4;  // segments of a workgroup
 constexpr int kMaxBeams = 64;
 
 struct SelectParams {
@@ -28,8 +30,10 @@ struct SelectParams {
   int64_t group_stride, beam_stride;  // elements
   const float* scores;
   const uint8_t* finished;
-  int groups, beams, vocab, num_out, pad, nseg;
-  float2* seg;  // [groups * beams][nseg]: largest, sum of exp(x - largest)
+  int groups, beams, vocab, num_out, pad;
+  int nseg, nsum;  // segments of a row, and sums
+  float2* sum;     // [groups * beams][nsum]: largest, sum of exp(x - largest)
+  float* seg;      // [groups * beams][nseg]: largest
   float* scores_out;
   int32_t* parents_out;
   int32_t* tokens_out;
@@ -51,16 +55,15 @@ __device__ __forceinline__ bool beam_alive(float score) { return score > -INFINI
 // log2(e) in two parts: the product's constant error would be the same in every term.
 constexpr float kLog2eHi = 1.4426950216293335f, kLog2eLo = 1.925963033500011e-8f;
 
-// A wave a segment.  16-byte loads at the alignment of an element: what a lane sums
+// A wave a segment (behind the row's end: an empty one).  16-byte loads at the alignment of an element: what a lane sums
 // goes by the place in the row alone, so that equal rows give equal sums.
 template <typename T>
-__global__ __launch_bounds__(256) void beam_scan_kernel(SelectParams p) {
+__global__ __launch_bounds__(64 * kScanWaves) void beam_scan_kernel(SelectParams p) {
   constexpr int E = 16 / sizeof(T), NV = kSeg / (64 * E);
-  const int lane = threadIdx.x & 63;
-  const uint32_t id = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);  // (below 2^31)
-  const int rows = p.groups * p.beams;
-  const int row = static_cast<int>(id / static_cast<uint32_t>(p.nseg)), j = static_cast<int>(id) - row * p.nseg;
-  if (row >= rows) return;
+  __shared__ float2 part[kScanWaves];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int row = static_cast<int>(blockIdx.x / static_cast<uint32_t>(p.nsum));
+  const int js = static_cast<int>(blockIdx.x) - row * p.nsum, j = js * kScanWaves + wave;
   if (!beam_alive(p.scores[row]) || (p.finished && p.finished[row])) return;  // (nobody reads its segments)
   const int b = row / p.beams, w = row - b * p.beams;
   const T* x = static_cast<const T*>(p.x) + b * p.group_stride + w * p.beam_stride + static_cast<int64_t>(j) * kSeg;
@@ -109,7 +112,22 @@ __global__ __launch_bounds__(256) void beam_scan_kernel(SelectParams p) {
       }
   }
   s = group_sum<64>(s);
-  if (lane == 0) p.seg[static_cast<int64_t>(row) * p.nseg + j] = make_float2(m, s);
+  if (lane == 0) {
+    if (j < p.nseg) p.seg[static_cast<int64_t>(row) * p.nseg + j] = m;
+    part[wave] = make_float2(m, s);
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    float M = -INFINITY, S = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kScanWaves; ++i) M = fmaxf(M, part[i].x);
+#pragma unroll
+    for (int i = 0; i < kScanWaves; ++i) {
+      const float d = part[i].x - M;
+      if (part[i].y > 0.0f) S += part[i].y * (part[i].x == M ? 1.0f : fast_exp2(fmaf(d, kLog2eLo, d * kLog2eHi)));
+    }
+    p.sum[static_cast<int64_t>(row) * p.nsum + js] = make_float2(M, S);
+  }
 }
 
 // A candidate: its total in an order of whole numbers (0: none), and its place.
@@ -130,58 +148,82 @@ __device__ __forceinline__ Cand shfl_xor_c(const Cand& c, int d) {
   const uint32_t lo = shfl_xor_u(static_cast<uint32_t>(c.k), d), hi = shfl_xor_u(static_cast<uint32_t>(c.k >> 32), d);
   return {static_cast<uint64_t>(hi) << 32 | lo, shfl_xor_u(c.i, d)};
 }
-
 constexpr int kPick = 1024;         // threads of the choice, and tokens of a segment
-constexpr int kGroup = 8;           // threads that offer one candidate as a threshold
+constexpr int kGroup = 8;           // threads that offer one total as a bound
 constexpr int kGroups = kPick / kGroup;
-constexpr int kSurvivors = 2048;    // (K - 1) * kGroup * items a thread + 1 of them at most: K <= 16 fit with K items
+constexpr int kSurvivors = 2048;
 static_assert(kPick == kSeg && kGroups >= kMaxBeams, "choice");
 
 struct PickLds {
-  Cand group[kGroups];
-  Cand threshold;
+  float group[kGroups];
+  float bound;
   int count;
+  Cand first[kPick / 64];
   Cand kept[kSurvivors];
   Cand out[kMaxBeams];
 };
 
-// The K first of n items into L.out, in order; how many there are.  The K-th of the
-// groups' first ones bounds the K-th of all from below; of the few items not behind it
-// every one counts those before it.
-template <typename F>
-__device__ __forceinline__ int pick(PickLds& L, int n, int K, F item) {
+__device__ __forceinline__ float max_of_8(float v) {
+  v = fmaxf(v, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0xB1, 0xF, 0xF, false)));
+  v = fmaxf(v, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x4E, 0xF, 0xF, false)));
+  return fmaxf(v, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x141, 0xF, 0xF, false)));
+}
+
+// The K first of n items into L.out, in order; how many there are.  about(i): an item's
+// total in 32 bits, -inf where it is none; exact(i): the candidate.  The K-th largest of
+// the groups' largest bounds the K-th of all from below; the few items that reach it,
+// less what 32 bits can be off, are compared exactly: each counts those before it.
+//
+// 32 bits: a total is base + d, d <= 0, each rounded and the sum too, so off by at most
+// 2^-24 (|base| + |d| + |total|) <= 2^-23 (|base| + |total|), and |total| is at most the
+// larger of |bound| and |base| where it reaches the bound: 2^-22 (2 most + |bound|) for two
+// of them, `most` the largest |base|.  Four times that is allowed for.
+// A thread's first HELD items are looked at once: about(i, number).
+template <int HELD, typename F, typename G>
+__device__ __forceinline__ int pick(PickLds& L, int n, int K, float most, F about, G exact) {
   const int tid = threadIdx.x;
-  Cand best{0, ~0u};
-#pragma unroll 4
-  for (int i = tid; i < n; i += kPick) {
-    const Cand c = item(i);
-    if (before(c, best)) best = c;
-  }
+  float held[HELD], best = -INFINITY;
 #pragma unroll
-  for (int d = 1; d < kGroup; d <<= 1) {
-    const Cand o = shfl_xor_c(best, d);
-    if (before(o, best)) best = o;
-  }
+  for (int i = 0; i < HELD; ++i) held[i] = tid + i * kPick < n ? about(tid + i * kPick, i) : -INFINITY;
+#pragma unroll
+  for (int i = 0; i < HELD; ++i) best = fmaxf(best, held[i]);
+#pragma unroll 4
+  for (int i = tid + HELD * kPick; i < n; i += kPick) best = fmaxf(best, about(i, HELD));
+  best = max_of_8(best);
   if (tid % kGroup == 0) L.group[tid / kGroup] = best;
   if (tid == 0) {
-    L.threshold = Cand{0, ~0u};
+    L.bound = -INFINITY;
     L.count = 0;
   }
   __syncthreads();
-  int r = 0;
+  int r = 0;  // groups above this one's, and (high half) not below it
 #pragma unroll
-  for (int j = 0; j < kGroups / kGroup; ++j) r += before(L.group[tid % kGroup + kGroup * j], best);
+  for (int j = 0; j < kGroups / kGroup; ++j) {
+    const float o = L.group[tid % kGroup + kGroup * j];
+    r += (o > best ? 1 : 0) + (o >= best ? 1 << 16 : 0);
+  }
   r = group_sum_i<kGroup>(r);
-  if (tid % kGroup == 0 && r == K - 1 && best.k != 0) L.threshold = best;
+  if (tid % kGroup == 0 && (r & 0xFFFF) < K && K <= r >> 16) L.bound = best;  // (one value)
   __syncthreads();
-  const Cand least = L.threshold;
-#pragma unroll 4
-  for (int i = tid; i < n; i += kPick) {
-    const Cand c = item(i);
-    if (c.k != 0 && !before(least, c)) {
+  const float bound = L.bound, cut = bound - 0x1p-20f * (2.0f * most + fabsf(bound));
+  const float least = cut == cut ? cut : -INFINITY;
+  const auto keep = [&](int i) {
+    const Cand c = exact(i);
+    if (c.k != 0) {
       const int at = atomicAdd(&L.count, 1);  // (any order: each one's place is counted below)
       if (at < kSurvivors) L.kept[at] = c;
     }
+  };
+  // (few of them: code that runs once is bound by its fetching, so there is one copy)
+  unsigned these = 0;
+#pragma unroll
+  for (int i = 0; i < HELD; ++i) these |= held[i] > -INFINITY && held[i] >= least ? 1u << i : 0u;
+#pragma unroll 1
+  for (; these != 0; these &= these - 1) keep(tid + __builtin_ctz(these) * kPick);
+#pragma unroll 1
+  for (int i = tid + HELD * kPick; i < n; i += kPick) {
+    const float v = about(i, HELD);
+    if (v > -INFINITY && v >= least) keep(i);
   }
   __syncthreads();
   const int kept = L.count;
@@ -195,12 +237,12 @@ __device__ __forceinline__ int pick(PickLds& L, int n, int K, F item) {
     __syncthreads();
     return min(kept, K);
   }
-  // more than K = 16 of candidates that crowd in a few groups: one after the other
+  // many equal ones, or all in a few groups: one after the other
   Cand last{~uint64_t{0}, 0};
   for (int k = 0; k < K; ++k) {
     Cand c{0, ~0u};
     for (int i = tid; i < n; i += kPick) {
-      const Cand x = item(i);
+      const Cand x = exact(i);
       if (before(last, x) && before(x, c)) c = x;
     }
 #pragma unroll
@@ -208,10 +250,10 @@ __device__ __forceinline__ int pick(PickLds& L, int n, int K, F item) {
       const Cand o = shfl_xor_c(c, d);
       if (before(o, c)) c = o;
     }
-    if ((tid & 63) == 0) L.group[tid >> 6] = c;
+    if ((tid & 63) == 0) L.first[tid >> 6] = c;
     __syncthreads();
     for (int j = 0; j < kPick / 64; ++j)
-      if (before(L.group[j], c)) c = L.group[j];
+      if (before(L.first[j], c)) c = L.first[j];
     if (tid == 0) L.out[k] = c;
     last = c;
     __syncthreads();
@@ -221,37 +263,47 @@ __device__ __forceinline__ int pick(PickLds& L, int n, int K, F item) {
 
 // The choice of one group.  What bounds it: latency (a round trip to the segments'
 // statistics, one to the chosen segments, and the barriers of two choices).
-template <typename T>
+// HELD: chosen segments that a thread holds its tokens of.
+template <typename T, int HELD>
 __global__ __launch_bounds__(kPick) void beam_pick_kernel(SelectParams p) {
   __shared__ PickLds L;
   __shared__ double base[kMaxBeams];  // score - log of the sum of exp(x - most)
-  __shared__ float most[kMaxBeams];   // the beam's largest logit
+  __shared__ float most[kMaxBeams];   // the beam's largest logit (finished: 0)
   __shared__ int state[kMaxBeams];    // 0: no candidates, 1: alive, 2: finished
   __shared__ int2 chosen[kMaxBeams];  // segments: beam, first token
   const int b = blockIdx.x, W = p.beams, V = p.vocab, K = p.num_out, nseg = p.nseg;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const float2* seg = p.seg + static_cast<int64_t>(b) * W * nseg;
+  const float* seg = p.seg + static_cast<int64_t>(b) * W * nseg;
+  // (what the first choice looks at, on its way from the start)
+  constexpr int kSegs = 2;
+  float ahead[kSegs];
+#pragma unroll
+  for (int i = 0; i < kSegs; ++i) ahead[i] = seg[min(static_cast<int>(threadIdx.x) + i * kPick, W * nseg - 1)];
+#pragma unroll 1
   for (int w = wave; w < W; w += kPick / 64) {
+    const float2* sum = p.sum + static_cast<int64_t>(b * W + w) * p.nsum;
+    const float2 mine = lane < p.nsum ? sum[lane] : make_float2(-INFINITY, 0.0f);  // (unwritten where nobody needs it)
     const float score = p.scores[b * W + w];
     const bool done = p.finished && p.finished[b * W + w];
     const int st = !beam_alive(score) ? 0 : done ? 2 : 1;
     double c = score;
     float m = -INFINITY;
     if (st == 1) {
-      for (int j = lane; j < nseg; j += 64) m = fmaxf(m, seg[w * nseg + j].x);
+      m = mine.x;
+#pragma unroll 1
+      for (int j = lane + 64; j < p.nsum; j += 64) m = fmaxf(m, sum[j].x);
       m = wave_max_dpp(m);
+      const auto part = [&](float2 v) { return !(v.y > 0.0f) ? 0.0 : v.y * (v.x == m ? 1.0 : exp(static_cast<double>(v.x) - static_cast<double>(m))); };
       double s = 0.0;
-      for (int j = lane; j < nseg; j += 64) {
-        const float2 v = seg[w * nseg + j];
-        if (v.y > 0.0f) s += v.y * (v.x == m ? 1.0 : exp(static_cast<double>(v.x) - static_cast<double>(m)));
-      }
+#pragma unroll 1
+      for (int j = lane; j < p.nsum; j += 64) s += part(j == lane ? mine : sum[j]);
 #pragma unroll
       for (int d = 1; d < 64; d <<= 1) s += __shfl_xor(s, d, 64);
       c -= log(s);
     }
     if (lane == 0) {
       base[w] = c;
-      most[w] = m;
+      most[w] = st == 2 ? 0.0f : m;
       state[w] = st == 1 && !(m > -INFINITY) ? 0 : st;
     }
   }
@@ -259,25 +311,76 @@ __global__ __launch_bounds__(kPick) void beam_pick_kernel(SelectParams p) {
   const auto total = [&](int w, float x) {
     return base[w] + (x == most[w] ? 0.0 : static_cast<double>(x) - static_cast<double>(most[w]));
   };
-  const int n1 = pick(L, W * nseg, K, [&](int i) {
-    const int w = i / nseg, j = i - w * nseg;
-    if (state[w] == 1) return cand(total(w, seg[i].x), i);
-    return j == 0 && state[w] == 2 ? cand(base[w], i) : Cand{0, ~0u};
-  });
+  // (what 32 bits cannot hold is not lost: it counts as their lowest value)
+  const auto about = [&](int w, float x) {
+    const float d = x == most[w] ? 0.0f : fmaxf(x - most[w], -FLT_MAX);
+    return x > -INFINITY ? fmaxf(static_cast<float>(base[w]) + d, -FLT_MAX) : -INFINITY;
+  };
+  // the largest |base| (of at most 64 beams)
+  const float far = wave_max_dpp(lane < W && state[lane] != 0 ? fabsf(static_cast<float>(base[lane])) : 0.0f);
+  // i / nseg: below 64, off by 64 2^-22 at most, and a half is 2^-15 of it at least
+  const float inv = 1.0f / static_cast<float>(nseg);
+  const auto beam_of = [&](int i) { return static_cast<int>((static_cast<float>(i) + 0.5f) * inv); };
+  // a segment's total is its largest token's; a finished beam is the first of its segments
+  const int n1 = pick<kSegs>(
+      L, W * nseg, K, far,
+      [&](int i, int r) {
+        const int w = beam_of(i);
+        const float m = r < kSegs ? ahead[r < kSegs ? r : 0] : seg[i];  // (unwritten where nobody needs it)
+        return state[w] == 1 ? about(w, m) : state[w] == 2 && i == w * nseg ? static_cast<float>(base[w]) : -INFINITY;
+      },
+      [&](int i) {
+        const int w = beam_of(i);
+        return cand(state[w] == 1 ? total(w, seg[i]) : state[w] == 2 && i == w * nseg ? base[w] : -INFINITY, i);
+      });
   if (threadIdx.x < static_cast<unsigned>(n1)) {
-    const int i = L.out[threadIdx.x].i, w = i / nseg;
+    const int i = L.out[threadIdx.x].i, w = beam_of(i);
     chosen[threadIdx.x] = int2{w, (i - w * nseg) * kSeg};
   }
   __syncthreads();
   const T* x = static_cast<const T*>(p.x) + b * p.group_stride;
-  const int n2 = pick(L, n1 * kSeg, K, [&](int i) {
-    const int2 c = chosen[i / kSeg];
-    const int t = c.y + i % kSeg;
-    if (state[c.x] == 2) return i % kSeg == 0 ? cand(base[c.x], c.x * V + p.pad) : Cand{0, ~0u};
-    if (t >= V) return Cand{0, ~0u};
-    const float v = to_f32(x[c.x * p.beam_stride + t]);
-    return v == v ? cand(total(c.x, v), c.x * V + t) : Cand{0, ~0u};
-  });
+  const auto logit = [&](int2 c) {  // this thread's of a chosen segment (behind the row's end: the last one)
+    return to_f32(x[c.x * p.beam_stride + min(c.y + static_cast<int>(threadIdx.x), V - 1)]);
+  };
+  const auto value = [&](int2 c, float v) {  // a finished beam is its first token; NaN is none
+    const bool in = state[c.x] == 2 ? threadIdx.x == 0 : c.y + static_cast<int>(threadIdx.x) < V && v == v;
+    return !in ? -INFINITY : state[c.x] == 2 ? most[c.x] : v;
+  };
+  // The first HELD chosen segments: what concerns segment r in lane r, the loads all on
+  // their way before the first is looked at.
+  float held[HELD];
+  if (n1 > 0) {
+    const int2 c = chosen[min(lane, n1 - 1)];
+    const int64_t off = c.x * p.beam_stride + c.y;
+    const int lo = static_cast<int>(off), hi = static_cast<int>(off >> 32), left = V - 1 - c.y, fin = state[c.x] == 2;
+    const int top = __float_as_int(most[c.x]), from = __float_as_int(static_cast<float>(base[c.x]));
+    const auto of = [](int v, int r) { return __builtin_amdgcn_readlane(v, r); };
+#pragma unroll
+    for (int r = 0; r < HELD; ++r) {
+      const int64_t o = static_cast<int64_t>(static_cast<uint64_t>(static_cast<uint32_t>(of(hi, r))) << 32 | static_cast<uint32_t>(of(lo, r)));
+      held[r] = to_f32(x[o + min(static_cast<int>(threadIdx.x), of(left, r))]);
+    }
+#pragma unroll
+    for (int r = 0; r < HELD; ++r) {
+      const float m = __int_as_float(of(top, r));
+      const bool in = of(fin, r) ? threadIdx.x == 0 : static_cast<int>(threadIdx.x) <= of(left, r);
+      const float v = of(fin, r) ? m : held[r];
+      const float d = v == m ? 0.0f : fmaxf(v - m, -FLT_MAX);
+      held[r] = in && v > -INFINITY ? fmaxf(__int_as_float(of(from, r)) + d, -FLT_MAX) : -INFINITY;
+    }
+  }
+  const int n2 = pick<HELD>(
+      L, n1 * kSeg, K, far,
+      [&](int i, int r) {
+        if (r < HELD) return held[r < HELD ? r : 0];
+        const int2 c = chosen[i / kSeg];
+        return about(c.x, value(c, logit(c)));
+      },
+      [&](int i) {
+        const int2 c = chosen[i / kSeg];
+        const float v = value(c, logit(c));
+        return cand(v > -INFINITY ? total(c.x, v) : -INFINITY, c.x * V + (state[c.x] == 2 ? p.pad : c.y + static_cast<int>(threadIdx.x)));
+      });
   for (int k = threadIdx.x; k < K; k += kPick) {
     const int64_t at = static_cast<int64_t>(b) * K + k;
     const Cand c = k < n2 ? L.out[k] : Cand{0, 0};
@@ -290,15 +393,19 @@ __global__ __launch_bounds__(kPick) void beam_pick_kernel(SelectParams p) {
 
 template <typename T>
 int launch_select(const SelectParams& p, hipStream_t s) {
-  const int64_t waves = static_cast<int64_t>(p.groups) * p.beams * p.nseg;
-  beam_scan_kernel<T><<<static_cast<unsigned>((waves + 3) / 4), 256, 0, s>>>(p);
+  const int64_t sums = static_cast<int64_t>(p.groups) * p.beams * p.nsum;
+  beam_scan_kernel<T><<<static_cast<unsigned>(sums), 64 * kScanWaves, 0, s>>>(p);
   TQ_CHECK_LAUNCH("beam_scan_kernel");
-  beam_pick_kernel<T><<<static_cast<unsigned>(p.groups), kPick, 0, s>>>(p);
+  const unsigned groups = static_cast<unsigned>(p.groups);
+  if (p.num_out <= 4) beam_pick_kernel<T, 4><<<groups, kPick, 0, s>>>(p);
+  else if (p.num_out <= 8) beam_pick_kernel<T, 8><<<groups, kPick, 0, s>>>(p);
+  else beam_pick_kernel<T, 16><<<groups, kPick, 0, s>>>(p);
   TQ_CHECK_LAUNCH("beam_pick_kernel");
   return TQ_OK;
 }
 
 int segments(int vocab) { return (vocab + kSeg - 1) / kSeg; }
+int sums(int vocab) { return (segments(vocab) + kScanWaves - 1) / kScanWaves; }
 
 // ---- reordering a contiguous cache ------------------------------------------
 // Rows of sequence b become those of parents[b], in place.  A workgroup takes the same
@@ -423,7 +530,7 @@ using namespace tq;
 
 extern "C" size_t tq_beam_select_workspace_size(int groups, int beams, int vocab) {
   if (groups < 1 || beams < 1 || vocab < 1) return 0;
-  return sizeof(float2) * static_cast<size_t>(groups) * beams * segments(vocab);
+  return static_cast<size_t>(groups) * beams * (sizeof(float2) * sums(vocab) + sizeof(float) * segments(vocab));
 }
 
 extern "C" int tq_beam_select(const void* logits, tq_dtype x_dtype, int64_t group_stride, int64_t beam_stride,
@@ -450,8 +557,10 @@ extern "C" int tq_beam_select(const void* logits, tq_dtype x_dtype, int64_t grou
   TQ_CHECK_ARG(reinterpret_cast<uintptr_t>(workspace) % 16 == 0, "%s: workspace must be 16-byte aligned", fn);
   const int nseg = segments(vocab);
   TQ_CHECK_ARG(static_cast<int64_t>(groups) * beams * nseg < (int64_t{1} << 31), "%s: logits too large", fn);
+  float2* sum = static_cast<float2*>(workspace);
   SelectParams p{logits, group_stride, beam_stride, scores, finished, groups, beams, vocab, num_out, pad_token, nseg,
-                 static_cast<float2*>(workspace), scores_out, parents_out, tokens_out};
+                 sums(vocab), sum, reinterpret_cast<float*>(sum + static_cast<size_t>(groups) * beams * sums(vocab)),
+                 scores_out, parents_out, tokens_out};
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (x_dtype == TQ_F32) return launch_select<float>(p, s);
   if (x_dtype == TQ_F16) return launch_select<_Float16>(p, s);
