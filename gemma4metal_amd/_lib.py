@@ -69,7 +69,8 @@ SIGNATURES = {
     "tq_kv_pages_fork": (I, [P, I, I, I, I, P, P, P, P, P, I, I, I, I, P, SZ, P]),
     "tq_kv_pages_reorder_workspace_size": (SZ, [I, I, I]),
     "tq_kv_pages_reorder": (I, [P, I, I, I, I, P, P, P, P, P, I, I, I, I, P, SZ, P]),
-    "tq_kv_reorder_int4": (I, [P, P, P, P, P, P, I, I, I, I, I, P, P, P]),
+    "tq_kv_reorder_int4_workspace_size": (SZ, [I]),
+    "tq_kv_reorder_int4": (I, [P, P, P, P, P, P, I, I, I, I, I, P, P, P, SZ, P]),
     "tq_beam_select_workspace_size": (SZ, [I, I, I]),
     "tq_beam_select": (I, [P, I, I64, I64, P, P, I, I, I, I, I, P, P, P, P, SZ, P]),
     "tq_kv_pages_free": (I, [P, P, P, P, I, I, I, P]),

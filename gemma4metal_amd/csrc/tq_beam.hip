@@ -408,20 +408,35 @@ int segments(int vocab) { return (vocab + kSeg - 1) / kSeg; }
 int sums(int vocab) { return (segments(vocab) + kScanWaves - 1) / kScanWaves; }
 
 // ---- reordering a contiguous cache ------------------------------------------
-// Rows of sequence b become those of parents[b], in place.  A workgroup takes the same
-// bytes of every sequence: it loads those of all parents into LDS before it stores any,
-// and no other workgroup touches them, so that any map (swaps, cycles, one parent of
-// many) comes out as if all moved at once.
+// Rows of sequence b become those of parents[b], in place.  Sequences that are joined by
+// the map (a group's beams) are a component; a workgroup takes the same bytes of all
+// sequences of one, loads those of every parent before it stores any, and no other
+// workgroup touches them, so that any map (swaps, cycles, one parent of many) comes out as
+// if all moved at once.  A plan by one workgroup finds the components and the rows each
+// moves, so that nothing behind the lengths is visited.
 constexpr int kMaxSeqs = 1024;
-constexpr int kTileUnits = 4096;  // 16-byte units in LDS
+constexpr int kHeldParents = 8;  // of a component, in a thread's registers; else by way of LDS
+constexpr int kUnits = 2;        // 16-byte units of a thread
+constexpr int kTileUnits = 256 * kUnits;
+constexpr int kLdsUnits = 1024;
+
+struct ReorderComp {
+  int from, nf, rows, tiles;  // parents [from, from + nf), the most rows of one, tiles of the components before
+};
+struct ReorderParent {
+  int seq, rows, to, nd;      // its children [to, to + nd)
+};
 
 struct ReorderParams {
   char* base[6];
   int row_bytes[6];
-  int tiles[6];   // of one head
-  int heads, cap, seqs, shift;  // 1 << shift units of a sequence in a tile
+  int heads, cap, seqs;
   int32_t* lengths;
   const int32_t* parents;
+  int* head;             // components, tiles in all
+  ReorderComp* comps;
+  ReorderParent* from;
+  int* to;
 };
 
 __device__ __forceinline__ int parent_of(const int32_t* parents, int s, int seqs) {
@@ -429,46 +444,152 @@ __device__ __forceinline__ int parent_of(const int32_t* parents, int s, int seqs
   return static_cast<unsigned>(q) < static_cast<unsigned>(seqs) ? q : -1;
 }
 
-__global__ __launch_bounds__(256) void kv_reorder_kernel(ReorderParams p) {
-  __shared__ uint4 unit[kTileUnits];
-  __shared__ int16_t needed[kMaxSeqs];  // 1 + slot of a parent that is needed, 0 yet without one; else -1
-  __shared__ int2 from[kMaxSeqs];       // sequence, rows
-  __shared__ ushort2 to[kMaxSeqs];      // sequence, slot
-  __shared__ int n_from, n_to;
-  for (int s = threadIdx.x; s < p.seqs; s += 256) needed[s] = -1;
-  if (threadIdx.x == 0) n_from = n_to = 0;
-  __syncthreads();
-  for (int s = threadIdx.x; s < p.seqs; s += 256) {
-    const int q = parent_of(p.parents, s, p.seqs);
-    if (q >= 0 && q != s) needed[q] = 0;
-  }
-  __syncthreads();
-  for (int s = threadIdx.x; s < p.seqs; s += 256) {
-    const int n = min(p.lengths[s], p.cap);
-    if (needed[s] == 0 && n > 0) {  // (any order: it is only where they lie in LDS)
-      const int at = atomicAdd(&n_from, 1);
-      needed[s] = static_cast<int16_t>(at + 1);
-      from[at] = int2{s, n};
-    }
-  }
-  __syncthreads();
-  for (int s = threadIdx.x; s < p.seqs; s += 256) {
-    const int q = parent_of(p.parents, s, p.seqs);
-    if (q >= 0 && q != s && needed[q] > 0) to[atomicAdd(&n_to, 1)] = ushort2{static_cast<uint16_t>(s), static_cast<uint16_t>(needed[q] - 1)};
-  }
-  __syncthreads();
-  const int nf = n_from, nd = n_to, T = 1 << p.shift;
-  int per_head = 0;
+// Tiles of one head of n rows, tensor by tensor.
+__device__ __forceinline__ int tiles_of(const ReorderParams& p, int a, int n) {
+  return static_cast<int>((static_cast<int64_t>(n) * p.row_bytes[a] + 16 * kTileUnits - 1) / (16 * kTileUnits));
+}
+
+// Exclusive prefix over the workgroup's threads, and the total.
+__device__ __forceinline__ int plan_scan(int v, int* lds, int& total) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int x = v;
 #pragma unroll
-  for (int a = 0; a < 6; ++a) per_head += p.tiles[a];
-  const int64_t total = static_cast<int64_t>(per_head) * p.heads;
-  for (int64_t g = blockIdx.x; g < total; g += gridDim.x) {
-    const int h = static_cast<int>(g / per_head);
-    int u = static_cast<int>(g - static_cast<int64_t>(h) * per_head), a = 0;
+  for (int d = 1; d < 64; d <<= 1) {
+    const int y = __shfl_up(x, d, 64);
+    if (lane >= d) x += y;
+  }
+  __syncthreads();  // the last call's readers are done
+  if (lane == 63) lds[wave] = x;
+  __syncthreads();
+  int before = 0;
+  total = 0;
+#pragma unroll
+  for (int w = 0; w < kMaxSeqs / 64; ++w) {
+    const int t = lds[w];
+    before += w < wave ? t : 0;
+    total += t;
+  }
+  return before + x - v;
+}
+
+// One thread a sequence; lengths become the parents'.
+__global__ __launch_bounds__(kMaxSeqs) void kv_reorder_plan_kernel(ReorderParams p) {
+  __shared__ int label[kMaxSeqs], kids[kMaxSeqs], nf[kMaxSeqs], most[kMaxSeqs], at[kMaxSeqs], first[kMaxSeqs];
+  __shared__ int lds[kMaxSeqs / 64], changed;
+  const int s = threadIdx.x;
+  const bool in = s < p.seqs;
+  const int q = in ? parent_of(p.parents, s, p.seqs) : -1;
+  const int len = in ? p.lengths[s] : 0;
+  const int length = q < 0 ? 0 : p.lengths[q];
+  const int rows = max(min(len, p.cap), 0);
+  label[s] = s;
+  kids[s] = nf[s] = most[s] = at[s] = 0;
+  __syncthreads();  // (lengths are read)
+  if (in) p.lengths[s] = length;
+  const bool moves = q >= 0 && q != s;
+  if (moves) atomicAdd(&kids[q], 1);
+  __syncthreads();
+  const bool gives = kids[s] > 0 && rows > 0;
+  // components: the lowest number that the map reaches either way
+  for (;;) {
+    if (s == 0) changed = 0;
+    __syncthreads();
+    if (moves) {
+      const int a = label[s], b = label[q];
+      if (a != b) {
+        atomicMin(&label[max(a, b)], min(a, b));
+        atomicMin(&label[s], min(a, b));
+        atomicMin(&label[q], min(a, b));
+        changed = 1;
+      }
+    }
+    __syncthreads();
+    const int l = label[label[s]];
+    __syncthreads();
+    atomicMin(&label[s], l);
+    const bool done = changed == 0;
+    __syncthreads();
+    if (done) break;
+  }
+  const int root = label[s];
+  if (gives) {
+    atomicAdd(&nf[root], 1);
+    atomicMax(&most[root], rows);
+  }
+  __syncthreads();
+  const bool comp = nf[s] > 0;  // of the component's lowest sequence
+  int comps, parents, children, tiles;
+  const int c = plan_scan(comp, lds, comps);
+  const int from0 = plan_scan(nf[s], lds, parents);
+  const int to0 = plan_scan(gives ? kids[s] : 0, lds, children);
+  int n = 0;
+#pragma unroll
+  for (int a = 0; a < 6; ++a) n += comp ? tiles_of(p, a, most[s]) : 0;
+  const int tile0 = plan_scan(n * p.heads, lds, tiles);
+  first[s] = from0;
+  if (comp) p.comps[c] = ReorderComp{from0, nf[s], most[s], tile0};
+  if (s == 0) {
+    p.head[0] = comps;
+    p.head[1] = tiles;
+  }
+  __syncthreads();
+  // (the order of a component's parents is only that of their loads)
+  if (gives) p.from[first[root] + atomicAdd(&at[root], 1)] = ReorderParent{s, rows, to0, kids[s]};
+  kids[s] = gives ? to0 : -1;
+  __syncthreads();
+  if (moves && kids[q] >= 0) p.to[atomicAdd(&kids[q], 1)] = s;
+}
+
+__device__ __forceinline__ uint4 load_unit(const char* src, int64_t left) {
+  uint4 v{};
+  if (left >= 16) {
+    __builtin_memcpy(&v, src, 16);
+  } else if (left > 0) {  // the last rows end inside: whole elements of two bytes
+    uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+    for (int e = 0; e < 7; ++e)
+      if (2 * e < left) w[e / 2] |= static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(src + 2 * e)) << (16 * (e & 1));
+    v = uint4{w[0], w[1], w[2], w[3]};
+  }
+  return v;
+}
+__device__ __forceinline__ void store_unit(char* dst, const uint4& v, int64_t left) {
+  if (left >= 16) {
+    __builtin_memcpy(dst, &v, 16);
+  } else if (left > 0) {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int e = 0; e < 7; ++e)
+      if (2 * e < left) *reinterpret_cast<uint16_t*>(dst + 2 * e) = static_cast<uint16_t>(w[e / 2] >> (16 * (e & 1)));
+  }
+}
+
+// What bounds it: HBM.  Up to kHeldParents parents a component a thread holds its units of
+// all of them, with no barrier; 16-byte accesses at the alignment of an element.
+__global__ __launch_bounds__(256) void kv_reorder_kernel(ReorderParams p) {
+  __shared__ uint4 unit[kLdsUnits];
+  __shared__ int start[kMaxSeqs / 2];  // tiles of the components before (each has two sequences at least)
+  const int comps = p.head[0], total = p.head[1];
+  if (static_cast<int>(blockIdx.x) >= total) return;
+  for (int i = threadIdx.x; i < comps; i += 256) start[i] = p.comps[i].tiles;
+  __syncthreads();
+  for (int g = blockIdx.x; g < total; g += gridDim.x) {
+    int c = 0;
+    for (int end = comps; end - c > 1;) {
+      const int mid = (c + end) / 2;
+      (start[mid] <= g ? c : end) = mid;
+    }
+    c = __builtin_amdgcn_readfirstlane(c);
+    const ReorderComp k = p.comps[c];
+    int tiles[6], per_head = 0;
+#pragma unroll
+    for (int a = 0; a < 6; ++a) per_head += tiles[a] = tiles_of(p, a, k.rows);
+    const int h = (g - k.tiles) / per_head;
+    int u = g - k.tiles - h * per_head, a = 0;
 #pragma unroll
     for (int i = 0; i < 5; ++i)
-      if (a == i && u >= p.tiles[i]) {
-        u -= p.tiles[i];
+      if (a == i && u >= tiles[i]) {
+        u -= tiles[i];
         a = i + 1;
       }
     char* base = p.base[0];
@@ -479,48 +600,56 @@ __global__ __launch_bounds__(256) void kv_reorder_kernel(ReorderParams p) {
         base = p.base[i];
         rb = p.row_bytes[i];
       }
-    const int64_t first = static_cast<int64_t>(u) << (p.shift + 4);  // bytes into the head's rows
-    const auto place = [&](int s) { return base + (static_cast<int64_t>(s) * p.heads + h) * p.cap * rb + first; };
-#pragma unroll 4
-    for (int i = threadIdx.x; i < nf << p.shift; i += 256) {
-      const int2 f = from[i >> p.shift];
-      const int at = 16 * (i & (T - 1));
-      const int64_t have = static_cast<int64_t>(f.y) * rb - first - at;
-      const char* src = place(f.x) + at;
-      if (have >= 16) {
-        __builtin_memcpy(&unit[i], src, 16);
-      } else {
-        for (int k = 0; k < have; k += 2)
-          reinterpret_cast<uint16_t*>(&unit[i])[k / 2] = *reinterpret_cast<const uint16_t*>(src + k);
-      }
+    const int64_t first = static_cast<int64_t>(u) * (16 * kTileUnits);  // bytes into the head's rows
+    const int64_t head = static_cast<int64_t>(p.cap) * rb, stride = p.heads * head;
+    base += h * head + first;
+    const ReorderParent* from = p.from + k.from;
+    const auto left = [&](int rows, int at) { return static_cast<int64_t>(rows) * rb - first - at; };
+    if (k.nf <= kHeldParents) {
+      uint4 v[kHeldParents][kUnits];
+#pragma unroll
+      for (int i = 0; i < kHeldParents; ++i)
+        if (i < k.nf) {
+          const ReorderParent f = from[i];
+#pragma unroll
+          for (int j = 0; j < kUnits; ++j) {
+            const int at = 16 * (threadIdx.x + 256 * j);
+            v[i][j] = load_unit(base + f.seq * stride + at, left(f.rows, at));
+          }
+        }
+#pragma unroll
+      for (int i = 0; i < kHeldParents; ++i)
+        if (i < k.nf) {
+          const ReorderParent f = from[i];
+          for (int d = 0; d < f.nd; ++d) {
+            char* dst = base + p.to[f.to + d] * stride;
+#pragma unroll
+            for (int j = 0; j < kUnits; ++j) {
+              const int at = 16 * (threadIdx.x + 256 * j);
+              store_unit(dst + at, v[i][j], left(f.rows, at));
+            }
+          }
+        }
+      continue;
     }
-    __syncthreads();
-#pragma unroll 4
-    for (int i = threadIdx.x; i < nd << p.shift; i += 256) {
-      const ushort2 d = to[i >> p.shift];
-      const int at = 16 * (i & (T - 1)), in = (d.y << p.shift) + (i & (T - 1));
-      const int64_t have = static_cast<int64_t>(from[d.y].y) * rb - first - at;
-      char* dst = place(d.x) + at;
-      if (have >= 16) {
-        __builtin_memcpy(dst, &unit[in], 16);
-      } else {
-        for (int k = 0; k < have; k += 2)
-          *reinterpret_cast<uint16_t*>(dst + k) = reinterpret_cast<const uint16_t*>(&unit[in])[k / 2];
+    // as many units at a time as the LDS holds of every parent
+    const int T = max(kLdsUnits / k.nf, 1);
+    for (int u0 = 0; u0 < kTileUnits; u0 += T) {
+      for (int i = threadIdx.x; i < T * k.nf; i += 256) {
+        const ReorderParent f = from[i / T];
+        const int at = 16 * (u0 + i % T);
+        if (u0 + i % T < kTileUnits) unit[i] = load_unit(base + f.seq * stride + at, left(f.rows, at));
       }
+      __syncthreads();
+      for (int i = threadIdx.x; i < T * k.nf; i += 256) {
+        const ReorderParent f = from[i / T];
+        const int at = 16 * (u0 + i % T);
+        if (u0 + i % T < kTileUnits)
+          for (int d = 0; d < f.nd; ++d) store_unit(base + p.to[f.to + d] * stride + at, unit[i], left(f.rows, at));
+      }
+      __syncthreads();
     }
-    __syncthreads();
   }
-}
-
-__global__ __launch_bounds__(kMaxSeqs) void kv_reorder_lengths_kernel(ReorderParams p) {
-  const int s = threadIdx.x;
-  int n = 0;
-  if (s < p.seqs) {
-    const int q = parent_of(p.parents, s, p.seqs);
-    n = q < 0 ? 0 : p.lengths[q];
-  }
-  __syncthreads();
-  if (s < p.seqs) p.lengths[s] = n;
 }
 
 }  // namespace
@@ -567,10 +696,15 @@ extern "C" int tq_beam_select(const void* logits, tq_dtype x_dtype, int64_t grou
   return launch_select<uint16_t>(p, s);
 }
 
+extern "C" size_t tq_kv_reorder_int4_workspace_size(int batch) {
+  if (batch < 1 || batch > kMaxSeqs) return 0;
+  return 16 + static_cast<size_t>(batch) * (sizeof(ReorderComp) + sizeof(ReorderParent) + sizeof(int));
+}
+
 extern "C" int tq_kv_reorder_int4(uint32_t* k_quant, void* k_scales, void* k_biases, uint32_t* v_quant,
                                   void* v_scales, void* v_biases, tq_dtype sb_dtype, int batch, int num_kv_heads,
                                   int head_dim, int kv_capacity, int32_t* lengths, const int32_t* parents,
-                                  void* stream) {
+                                  void* workspace, size_t workspace_bytes, void* stream) {
   clear_error();
   const char* fn = "tq_kv_reorder_int4";
   TQ_CHECK_ARG(sb_dtype == TQ_F16 || sb_dtype == TQ_F32, "%s: sb_dtype must be f16 or f32", fn);
@@ -581,30 +715,36 @@ extern "C" int tq_kv_reorder_int4(uint32_t* k_quant, void* k_scales, void* k_bia
   if (batch == 0) return TQ_OK;
   ReorderParams p{};
   void* const t[6] = {k_quant, k_scales, k_biases, v_quant, v_scales, v_biases};
-  p.shift = 0;
-  while (p.shift < 10 && (batch << (p.shift + 1)) <= kTileUnits) ++p.shift;
   int64_t tiles = 0;
   for (int i = 0; i < 6; ++i) {
     TQ_CHECK_ARG(t[i] != nullptr, "%s: null tensor pointer", fn);
     TQ_CHECK_ARG(reinterpret_cast<uintptr_t>(t[i]) % 4 == 0, "%s: cache tensors must be 4-byte aligned", fn);
     p.base[i] = static_cast<char*>(t[i]);
     p.row_bytes[i] = i % 3 == 0 ? head_dim / 2 : head_dim / 64 * static_cast<int>(dtype_size(sb_dtype));
-    const int64_t bytes = static_cast<int64_t>(kv_capacity) * p.row_bytes[i];
-    const int64_t n = (bytes + (int64_t{16} << p.shift) - 1) / (int64_t{16} << p.shift);
-    TQ_CHECK_ARG(n < (1 << 28), "%s: cache too large", fn);
-    p.tiles[i] = static_cast<int>(n);
-    tiles += n;
+    tiles += (static_cast<int64_t>(kv_capacity) * p.row_bytes[i] + 16 * kTileUnits - 1) / (16 * kTileUnits);
   }
+  tiles *= static_cast<int64_t>(num_kv_heads) * ((batch + 1) / 2);  // (a component has two sequences at least)
+  TQ_CHECK_ARG(tiles < (int64_t{1} << 30), "%s: cache too large", fn);
   TQ_CHECK_ARG(lengths && parents, "%s: null pointer", fn);
+  const size_t need = tq_kv_reorder_int4_workspace_size(batch);
+  if (!workspace || workspace_bytes < need) {
+    set_error("%s: workspace of %zu bytes needed (got %zu)", fn, need, workspace ? workspace_bytes : size_t{0});
+    return TQ_ERR_WORKSPACE;
+  }
+  TQ_CHECK_ARG(reinterpret_cast<uintptr_t>(workspace) % 16 == 0, "%s: workspace must be 16-byte aligned", fn);
   p.heads = num_kv_heads;
   p.cap = kv_capacity;
   p.seqs = batch;
   p.lengths = lengths;
   p.parents = parents;
+  p.head = static_cast<int*>(workspace);
+  p.comps = reinterpret_cast<ReorderComp*>(p.head + 4);
+  p.from = reinterpret_cast<ReorderParent*>(p.comps + batch);
+  p.to = reinterpret_cast<int*>(p.from + batch);
   hipStream_t s = static_cast<hipStream_t>(stream);
-  kv_reorder_kernel<<<static_cast<unsigned>(std::min<int64_t>(tiles * num_kv_heads, 512)), 256, 0, s>>>(p);
+  kv_reorder_plan_kernel<<<1, kMaxSeqs, 0, s>>>(p);
+  TQ_CHECK_LAUNCH("kv_reorder_plan_kernel");
+  kv_reorder_kernel<<<static_cast<unsigned>(std::min<int64_t>(tiles, 2048)), 256, 0, s>>>(p);
   TQ_CHECK_LAUNCH("kv_reorder_kernel");
-  kv_reorder_lengths_kernel<<<1, kMaxSeqs, 0, s>>>(p);
-  TQ_CHECK_LAUNCH("kv_reorder_lengths_kernel");
   return TQ_OK;
 }

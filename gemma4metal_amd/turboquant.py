@@ -375,7 +375,8 @@ class Int4KVCache:
 
 def kv_reorder_int4(k_quant: torch.Tensor, k_scales: torch.Tensor, k_biases: torch.Tensor,
                     v_quant: torch.Tensor, v_scales: torch.Tensor, v_biases: torch.Tensor,
-                    lengths: torch.Tensor, parents: torch.Tensor, *, stream=None) -> None:
+                    lengths: torch.Tensor, parents: torch.Tensor, *, workspace: Optional[torch.Tensor] = None,
+                    stream=None) -> None:
     """Reorders (B, Hkv, cap, .) caches (linear or ring) in place, all sequences at
     once: the rows of sequence b become those of sequence parents[b] as they were,
     lengths[b] its length.  Rows behind the length stay as they were.  A parent
@@ -398,9 +399,22 @@ def kv_reorder_int4(k_quant: torch.Tensor, k_scales: torch.Tensor, k_biases: tor
     for n, t in (("lengths", lengths), ("parents", parents)):
         if t.dtype != torch.int32 or t.shape != (B,):
             raise ValueError(f"{n} must be int32 ({B},)")
-    with torch.cuda.device(k_quant.device):
+    nbytes = _lib.load().tq_kv_reorder_int4_workspace_size(B)
+    if workspace is not None:
+        _check_cuda("workspace", workspace)
+        if workspace.dtype != torch.uint8 or workspace.numel() < nbytes or workspace.device != k_quant.device:
+            raise ValueError(f"workspace must be uint8 of at least {nbytes} bytes on {k_quant.device}")
+
+    def run():
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=k_quant.device) if workspace is None else workspace
         call("tq_kv_reorder_int4", *[_ptr(t) for t in tensors], sbt, B, Hkv, D, cap, _ptr(lengths), _ptr(parents),
-             _stream(stream))
+             _ptr(ws), nbytes, _stream(None))
+
+    if stream is None and k_quant.device.index == torch.cuda.current_device():
+        run()
+    else:  # launches, allocations and the capture state go by the current device and stream
+        with torch.cuda.device(k_quant.device), torch.cuda.stream(stream):
+            run()
 
 
 def kv_append_int4(k_new: torch.Tensor, v_new: torch.Tensor,

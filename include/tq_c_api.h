@@ -483,11 +483,15 @@ int tq_beam_select(const void* logits, tq_dtype x_dtype, int64_t group_stride, i
  * in place, all sequences at once: the rows of sequence b become those of sequence
  * parents[b] as they were, and lengths[b] its length (DEVICE int32 [batch] both).  Rows
  * behind min(length, kv_capacity) stay as they were.  parents[b] outside [0, batch):
- * lengths[b] = 0.  batch <= 1024. */
+ * lengths[b] = 0.  batch <= 1024.
+ * workspace: tq_kv_reorder_int4_workspace_size(...) bytes, 16-byte aligned; need not be
+ * zeroed; calls that may overlap need one each. */
+size_t tq_kv_reorder_int4_workspace_size(int batch);
 int tq_kv_reorder_int4(uint32_t* k_quant, void* k_scales, void* k_biases,
                        uint32_t* v_quant, void* v_scales, void* v_biases, tq_dtype sb_dtype,
                        int batch, int num_kv_heads, int head_dim, int kv_capacity,
-                       int32_t* lengths, const int32_t* parents, void* stream);
+                       int32_t* lengths, const int32_t* parents, void* workspace,
+                       size_t workspace_bytes, void* stream);
 
 /* Dequantize rows (for the engine's prefill fallback,
  * engine/gemma4_multilayer.cpp:307-308): out[r, d] = s*nibble + b as f32. */
