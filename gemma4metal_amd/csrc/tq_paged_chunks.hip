@@ -22,8 +22,12 @@
 namespace tq {
 namespace {
 
-// Rows of a sequence up to which it is one of few.
-constexpr int kFewRows = 16;
+// Rows of a sequence up to which it is one of few.  In us, this kernel against the tile
+// kernel, 32 sequences of 300 to 6,000 keys, bf16 queries: D 256 (Hkv 16, window 1,024) of
+// 24 rows 99 : 132, 48 rows 139 : 146, 64 rows 176 : 165; D 128 (Hkv 8) of 32 rows 90 :
+// 162, 64 rows 141 : 184, 128 rows 252 : 263; D 512 (Hkv 4) of 16 rows 158 : 209, 32 rows
+// 302 : 221.
+constexpr int few_rows(int D) { return D == 512 ? 16 : D == 256 ? 48 : 128; }
 constexpr int kFewBlock = 16;  // rows of a workgroup
 
 template <int D, bool F32>
@@ -526,18 +530,18 @@ void paged_few_kernel(TileParams p) {
   }
 }
 
-// The outputs of a split block of one kernel's jobs, by a workgroup.
+// The outputs of a split block of one kernel's jobs, by workgroup y of ny.
 constexpr int kMergeThreads = 1024;
 
 template <int D, int ROWS, int TK, bool FEW>
-__device__ __forceinline__ void merge_job(const TileParams& p) {
+__device__ __forceinline__ void merge_job(const TileParams& p, int y, int ny) {
   constexpr int D4 = D / 4;
   const ChunkJob job = chunk_job<ROWS, TK, FEW, true>(p, blockIdx.x);
   if (job.splits == 0) return;
   const int rows = min(job.n * p.gqa - job.blk * ROWS, ROWS);
   const float2* ml = reinterpret_cast<const float2*>(p.ws_ml) + static_cast<int64_t>(job.slot) * ROWS;
   const v4f* po = reinterpret_cast<const v4f*>(p.ws_o) + static_cast<int64_t>(job.slot) * ROWS * D4;
-  for (int u = threadIdx.x; u < rows * D4; u += kMergeThreads) {
+  for (int u = y * kMergeThreads + threadIdx.x; u < rows * D4; u += ny * kMergeThreads) {
     const int r = u / D4;
     float M = -INFINITY, L = 0.0f;
     v4f O = v4f{0.0f, 0.0f, 0.0f, 0.0f};
@@ -575,11 +579,13 @@ __device__ __forceinline__ void merge_job(const TileParams& p) {
   }
 }
 
-// few: the parameters of paged_few_kernel's jobs (y 0, if few_y is 1); tiles: the others'.
+// few: the parameters of paged_few_kernel's jobs (the first few_y workgroups of a block);
+// tiles: the others'.
 template <int D, int ROWS>
 __global__ __launch_bounds__(kMergeThreads) void merge_chunks_kernel(TileParams few, TileParams tiles, int few_y) {
-  if (static_cast<int>(blockIdx.y) < few_y) merge_job<D, kFewBlock, 32, true>(few);
-  else merge_job<D, ROWS, D == 512 ? 32 : 64, false>(tiles);
+  const int y = blockIdx.y;
+  if (y < few_y) merge_job<D, kFewBlock, 32, true>(few, y, few_y);
+  else merge_job<D, ROWS, D == 512 ? 32 : 64, false>(tiles, y - few_y, gridDim.y - few_y);
 }
 
 template <bool F32>
@@ -623,8 +629,9 @@ ChunksPlan plan_chunks(int batch, int queries, int gqa, int Hkv, int D, int max_
   const int64_t rows = static_cast<int64_t>(std::min(max_new, queries)) * gqa, all = static_cast<int64_t>(queries) * gqa;
   const int64_t seqs = std::min(batch, queries);
   pl.rs = D == 512 || (D == 256 && all32) || rows <= 64 ? 4 : 8;
-  // sequences of few rows alone, some of them, or none
-  pl.few = rows <= kFewRows ? INT_MAX : batch > 1 && all / batch < 128 ? kFewRows : 0;
+  // sequences of few rows alone, or a batch that may hold some (a launch without work
+  // takes up to 10 us), or none
+  pl.few = rows <= few_rows(D) ? INT_MAX : batch > 1 && all / batch < 4 * few_rows(D) ? few_rows(D) : 0;
   // blocks of rows of any chunks that add up to `queries`
   if (pl.few != INT_MAX) {
     const int64_t n = std::min(seqs, all / (pl.few + 1)), R = 16 * pl.rs;
@@ -659,7 +666,7 @@ int launch_chunks(const PagedParams& p0, const PagedParams& few0, int D, int sb_
     else launch_few<false>(few, D, grid, s);
     TQ_CHECK_LAUNCH("paged_few_kernel");
   }
-  const int few_y = plan.few_rows.slots > 0 ? 1 : 0, tiles_y = plan.tiles.slots > 0 ? 1 : 0;
+  const int few_y = plan.few_rows.slots > 0 ? 1 : 0, tiles_y = plan.tiles.slots > 0 ? 4 : 0;
   if (few_y + tiles_y == 0) return TQ_OK;
   // (a split block has two slots at least)
   const dim3 grid(static_cast<unsigned>(std::max(plan.few_rows.slots, plan.tiles.slots) / 2), few_y + tiles_y);

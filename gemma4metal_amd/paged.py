@@ -122,6 +122,25 @@ def _pages_fine(pages, D: int, di: int) -> bool:
         return False
 
 
+def _pool_fine(pages, di: int) -> bool:
+    """The same of pages with or without a leading axis of layers."""
+    try:
+        kq, ks, kb, vq, vs, vb = pages
+        shape, dt = kq.shape, ks.dtype
+        rows = shape[:-1] + (shape[-1] // 8,)
+        return (4 <= len(shape) <= 5 and shape[-1] % 8 == 0 and vq.shape == shape
+                and ks.shape == rows and kb.shape == rows and vs.shape == rows and vb.shape == rows
+                and dt is kb.dtype and dt is vs.dtype and dt is vb.dtype
+                and (dt is torch.float16 or dt is torch.float32)
+                and kq.dtype in _QUANT_DT and vq.dtype in _QUANT_DT
+                and kq.get_device() == di and ks.get_device() == di and kb.get_device() == di
+                and vq.get_device() == di and vs.get_device() == di and vb.get_device() == di
+                and kq.is_contiguous() and ks.is_contiguous() and kb.is_contiguous()
+                and vq.is_contiguous() and vs.is_contiguous() and vb.is_contiguous())
+    except (AttributeError, IndexError, TypeError, ValueError):
+        return False
+
+
 def _ints_fine(t, shape, di: int) -> bool:
     return (isinstance(t, torch.Tensor) and t.dtype is torch.int32 and t.shape == shape and t.get_device() == di
             and t.is_contiguous())
@@ -351,10 +370,13 @@ def _check_state(block_tables, refs, lengths=None):
     _need(block_tables.dim() == 2, "block_tables must be (sequences, max_pages)")
     dev = block_tables.device
     S, P = block_tables.shape
-    _check_ints("block_tables", block_tables, (S, P), dev)
+    di = dev.index
+    if not _ints_fine(block_tables, (S, P), di):
+        _check_ints("block_tables", block_tables, (S, P), dev)
     _need(isinstance(refs, torch.Tensor) and refs.dim() == 1, "refs must be int32 (num_pages,)")
-    _check_ints("refs", refs, refs.shape, dev)
-    if lengths is not None:
+    if not _ints_fine(refs, refs.shape, di):
+        _check_ints("refs", refs, refs.shape, dev)
+    if lengths is not None and not _ints_fine(lengths, (S,), di):
         _check_ints("lengths", lengths, (S,), dev)
     return S, P, refs.shape[0], dev
 
@@ -367,7 +389,10 @@ def _six(pages, refs, device):
     _check_cuda("k_quant", kq)
     _need(kq.dim() in (4, 5), "page tensors must be ([layers,] num_pages, Hkv, page_size, .)")
     lead = kq.dim() - 4
-    N, Hkv, page, sbt = _check_pages(pages, kq.shape[-1] * 8, device, lead)
+    if _pool_fine(pages, device.index):
+        N, Hkv, page, sbt = *kq.shape[lead:-1], _DT[pages[1].dtype]
+    else:
+        N, Hkv, page, sbt = _check_pages(pages, kq.shape[-1] * 8, device, lead)
     _need(refs is None or N == refs.shape[0], "refs must have one count a page")
     arr = (ctypes.c_void_p * 6)(*[t.data_ptr() for t in pages])
     return arr, sbt, (kq.shape[0] if lead else 1), Hkv, kq.shape[-1] * 8, N, page
@@ -457,12 +482,13 @@ def kv_pages_reorder(pages, block_tables: torch.Tensor, refs: torch.Tensor, leng
     want of a page."""
     S, P, N, dev = _check_state(block_tables, refs, lengths)
     arr, sbt, L, Hkv, D, _, page = _six(pages, refs, dev)
-    _check_ints("parents", parents, (S,), dev)
+    if not _ints_fine(parents, (S,), dev.index):
+        _check_ints("parents", parents, (S,), dev)
     granted = torch.empty(S, dtype=torch.int32, device=dev)
     nbytes = _reorder_ws_size(S, N, P)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if workspace is None else _workspace(workspace, nbytes, dev, 0)
-    call("tq_kv_pages_reorder", arr, sbt, L, Hkv, D, _ptr(block_tables), _ptr(refs), _ptr(lengths), _ptr(parents),
-         _ptr(granted), S, P, N, page, _ptr(ws), ws.numel(), _stream(None))
+    call("tq_kv_pages_reorder", arr, sbt, L, Hkv, D, block_tables.data_ptr(), refs.data_ptr(), lengths.data_ptr(),
+         parents.data_ptr(), granted.data_ptr(), S, P, N, page, ws.data_ptr(), nbytes, _stream(None))
     return granted
 
 

@@ -373,6 +373,54 @@ class Int4KVCache:
         kv_reorder_int4(*self.tensors(), self.lengths, parents, stream=stream)
 
 
+@functools.lru_cache(maxsize=64)
+def _reorder_ws_size(B: int) -> int:
+    return _lib.load().tq_kv_reorder_int4_workspace_size(B)
+
+
+def _reorder_fine(kq, ks, kb, vq, vs, vb, lengths, parents) -> bool:
+    """What _check_reorder checks, as one expression (a small reorder is bound by it)."""
+    try:
+        shape, dt, di = kq.shape, ks.dtype, kq.get_device()
+        rows, seqs = shape[:3] + (shape[3] // 8,), shape[:1]
+        return (di >= 0 and len(shape) == 4 and shape[3] % 8 == 0 and vq.shape == shape
+                and ks.shape == rows and kb.shape == rows and vs.shape == rows and vb.shape == rows
+                and dt is kb.dtype and dt is vs.dtype and dt is vb.dtype
+                and (dt is torch.float16 or dt is torch.float32)
+                and kq.dtype in _QUANT_DT and vq.dtype in _QUANT_DT
+                and lengths.dtype is torch.int32 and parents.dtype is torch.int32
+                and lengths.shape == seqs and parents.shape == seqs
+                and ks.get_device() == di and kb.get_device() == di and vq.get_device() == di
+                and vs.get_device() == di and vb.get_device() == di and lengths.get_device() == di
+                and parents.get_device() == di
+                and kq.is_contiguous() and ks.is_contiguous() and kb.is_contiguous() and vq.is_contiguous()
+                and vs.is_contiguous() and vb.is_contiguous() and lengths.is_contiguous()
+                and parents.is_contiguous())
+    except (AttributeError, IndexError):
+        return False
+
+
+def _check_reorder(*tensors) -> None:
+    names = ("k_quant", "k_scales", "k_biases", "v_quant", "v_scales", "v_biases", "lengths", "parents")
+    kq = tensors[0]
+    for n, t in zip(names, tensors):
+        _check_cuda(n, t)
+        if t.device != kq.device:
+            raise ValueError(f"{n} must be on {kq.device}")
+    _need(kq.dim() == 4 and kq.shape[3] % 8 == 0, "k_quant must be (B, Hkv, cap, D/8) uint32")
+    _sb_dtype("k_scales", tensors[1])
+    rows = tuple(kq.shape[:3]) + (kq.shape[3] // 8,)
+    for i, (n, t) in enumerate(zip(names[:6], tensors)):
+        if i % 3 == 0:
+            if t.shape != kq.shape or t.dtype not in _QUANT_DT:
+                raise ValueError(f"{n} must be {tuple(kq.shape)} uint32")
+        elif t.shape != rows or t.dtype != tensors[1].dtype:
+            raise ValueError(f"{n} must be {rows} of one scale dtype")
+    for n, t in zip(names[6:], tensors[6:]):
+        if t.dtype != torch.int32 or t.shape != kq.shape[:1]:
+            raise ValueError(f"{n} must be int32 ({kq.shape[0]},)")
+
+
 def kv_reorder_int4(k_quant: torch.Tensor, k_scales: torch.Tensor, k_biases: torch.Tensor,
                     v_quant: torch.Tensor, v_scales: torch.Tensor, v_biases: torch.Tensor,
                     lengths: torch.Tensor, parents: torch.Tensor, *, workspace: Optional[torch.Tensor] = None,
@@ -381,25 +429,11 @@ def kv_reorder_int4(k_quant: torch.Tensor, k_scales: torch.Tensor, k_biases: tor
     once: the rows of sequence b become those of sequence parents[b] as they were,
     lengths[b] its length.  Rows behind the length stay as they were.  A parent
     outside [0, B) leaves a length of 0."""
-    names = ("k_quant", "k_scales", "k_biases", "v_quant", "v_scales", "v_biases")
     tensors = (k_quant, k_scales, k_biases, v_quant, v_scales, v_biases)
-    for n, t in zip(names + ("lengths", "parents"), tensors + (lengths, parents)):
-        _check_cuda(n, t)
-        if t.device != k_quant.device:
-            raise ValueError(f"{n} must be on {k_quant.device}")
-    _need(k_quant.dim() == 4, "k_quant must be (B, Hkv, cap, D/8) uint32")
-    B, Hkv, cap, D = *k_quant.shape[:3], k_quant.shape[3] * 8
-    sbt = _sb_dtype("k_scales", k_scales)
-    for i, (n, t) in enumerate(zip(names, tensors)):
-        if i % 3 == 0:
-            if t.shape != k_quant.shape or t.dtype not in _QUANT_DT:
-                raise ValueError(f"{n} must be {tuple(k_quant.shape)} uint32")
-        elif t.shape != (B, Hkv, cap, D // 64) or t.dtype != k_scales.dtype:
-            raise ValueError(f"{n} must be ({B}, {Hkv}, {cap}, {D // 64}) of one scale dtype")
-    for n, t in (("lengths", lengths), ("parents", parents)):
-        if t.dtype != torch.int32 or t.shape != (B,):
-            raise ValueError(f"{n} must be int32 ({B},)")
-    nbytes = _lib.load().tq_kv_reorder_int4_workspace_size(B)
+    if not _reorder_fine(*tensors, lengths, parents):
+        _check_reorder(*tensors, lengths, parents)
+    (B, Hkv, cap, W), sbt = k_quant.shape, _DT[k_scales.dtype]
+    nbytes = _reorder_ws_size(B)
     if workspace is not None:
         _check_cuda("workspace", workspace)
         if workspace.dtype != torch.uint8 or workspace.numel() < nbytes or workspace.device != k_quant.device:
@@ -407,8 +441,8 @@ def kv_reorder_int4(k_quant: torch.Tensor, k_scales: torch.Tensor, k_biases: tor
 
     def run():
         ws = torch.empty(nbytes, dtype=torch.uint8, device=k_quant.device) if workspace is None else workspace
-        call("tq_kv_reorder_int4", *[_ptr(t) for t in tensors], sbt, B, Hkv, D, cap, _ptr(lengths), _ptr(parents),
-             _ptr(ws), nbytes, _stream(None))
+        call("tq_kv_reorder_int4", *[t.data_ptr() for t in tensors], sbt, B, Hkv, 8 * W, cap, lengths.data_ptr(),
+             parents.data_ptr(), ws.data_ptr(), nbytes, _stream(None))
 
     if stream is None and k_quant.device.index == torch.cuda.current_device():
         run()
