@@ -530,13 +530,14 @@ void paged_few_kernel(TileParams p) {
   }
 }
 
-// The outputs of a split block of one kernel's jobs, by workgroup y of ny.
-constexpr int kMergeThreads = 1024;
+// The outputs of split block j of one kernel's jobs, by workgroup y of ny.
+constexpr int kMergeThreads = 256;
+constexpr int kMergeParts = 4;  // workgroups of a block of paged_tiles_kernel
 
 template <int D, int ROWS, int TK, bool FEW>
-__device__ __forceinline__ void merge_job(const TileParams& p, int y, int ny) {
+__device__ __forceinline__ void merge_job(const TileParams& p, int j, int y, int ny) {
   constexpr int D4 = D / 4;
-  const ChunkJob job = chunk_job<ROWS, TK, FEW, true>(p, blockIdx.x);
+  const ChunkJob job = chunk_job<ROWS, TK, FEW, true>(p, j);
   if (job.splits == 0) return;
   const int rows = min(job.n * p.gqa - job.blk * ROWS, ROWS);
   const float2* ml = reinterpret_cast<const float2*>(p.ws_ml) + static_cast<int64_t>(job.slot) * ROWS;
@@ -579,13 +580,13 @@ __device__ __forceinline__ void merge_job(const TileParams& p, int y, int ny) {
   }
 }
 
-// few: the parameters of paged_few_kernel's jobs (the first few_y workgroups of a block);
-// tiles: the others'.
+// few: the parameters of paged_few_kernel's jobs (the first few_n workgroups); tiles: the
+// others'.  (Most workgroups find no split block: as many as the chip runs at once.)
 template <int D, int ROWS>
-__global__ __launch_bounds__(kMergeThreads) void merge_chunks_kernel(TileParams few, TileParams tiles, int few_y) {
-  const int y = blockIdx.y;
-  if (y < few_y) merge_job<D, kFewBlock, 32, true>(few, y, few_y);
-  else merge_job<D, ROWS, D == 512 ? 32 : 64, false>(tiles, y - few_y, gridDim.y - few_y);
+__global__ __launch_bounds__(kMergeThreads) void merge_chunks_kernel(TileParams few, TileParams tiles, int few_n) {
+  const int i = blockIdx.x;
+  if (i < few_n) merge_job<D, kFewBlock, 32, true>(few, i, 0, 1);
+  else merge_job<D, ROWS, D == 512 ? 32 : 64, false>(tiles, (i - few_n) / kMergeParts, (i - few_n) % kMergeParts, kMergeParts);
 }
 
 template <bool F32>
@@ -602,14 +603,14 @@ void launch_few(const TileParams& p, int D, dim3 grid, hipStream_t s) {
 }
 
 template <int D>
-void launch_merge(const TileParams& few, const TileParams& tiles, int few_y, int rs, dim3 grid, hipStream_t s) {
+void launch_merge(const TileParams& few, const TileParams& tiles, int few_n, int rs, unsigned grid, hipStream_t s) {
   if constexpr (D < 512) {
     if (rs == 8) {
-      merge_chunks_kernel<D, 128><<<grid, kMergeThreads, 0, s>>>(few, tiles, few_y);
+      merge_chunks_kernel<D, 128><<<grid, kMergeThreads, 0, s>>>(few, tiles, few_n);
       return;
     }
   }
-  merge_chunks_kernel<D, 64><<<grid, kMergeThreads, 0, s>>>(few, tiles, few_y);
+  merge_chunks_kernel<D, 64><<<grid, kMergeThreads, 0, s>>>(few, tiles, few_n);
 }
 
 // The jobs of `blocks` blocks of rows of at most `tiles` tiles on `cus` workgroups at
@@ -666,13 +667,13 @@ int launch_chunks(const PagedParams& p0, const PagedParams& few0, int D, int sb_
     else launch_few<false>(few, D, grid, s);
     TQ_CHECK_LAUNCH("paged_few_kernel");
   }
-  const int few_y = plan.few_rows.slots > 0 ? 1 : 0, tiles_y = plan.tiles.slots > 0 ? 4 : 0;
-  if (few_y + tiles_y == 0) return TQ_OK;
+  if (plan.few_rows.slots + plan.tiles.slots == 0) return TQ_OK;
   // (a split block has two slots at least)
-  const dim3 grid(static_cast<unsigned>(std::max(plan.few_rows.slots, plan.tiles.slots) / 2), few_y + tiles_y);
-  if (D == 512) launch_merge<512>(few, p, few_y, plan.rs, grid, s);
-  else if (D == 256) launch_merge<256>(few, p, few_y, plan.rs, grid, s);
-  else launch_merge<128>(few, p, few_y, plan.rs, grid, s);
+  const int few_n = static_cast<int>(plan.few_rows.slots / 2);
+  const unsigned grid = static_cast<unsigned>(few_n + plan.tiles.slots / 2 * kMergeParts);
+  if (D == 512) launch_merge<512>(few, p, few_n, plan.rs, grid, s);
+  else if (D == 256) launch_merge<256>(few, p, few_n, plan.rs, grid, s);
+  else launch_merge<128>(few, p, few_n, plan.rs, grid, s);
   TQ_CHECK_LAUNCH("merge_chunks_kernel");
   return TQ_OK;
 }
