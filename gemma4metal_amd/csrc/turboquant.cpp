@@ -496,6 +496,34 @@ array sdpa_int4_paged_prefill(const array& queries, const kv_pages& pages,
   return out;
 }
 
+array sdpa_int4_paged_chunks(const array& queries, const kv_pages& pages, const array& block_tables,
+                             const array& starts, const array& seq_lens, int gqa_factor, float scale,
+                             int sliding_window, int num_sinks, int max_new, int max_kv_len,
+                             StreamOrDevice s) {
+  const PoolDims d = pool_dims(pages, false);
+  const Tables t = tables_of(block_tables);
+  need(queries.ndim() == 3 && queries.shape(2) == d.D && queries.shape(0) <= INT32_MAX &&
+           queries.shape(1) <= INT32_MAX,
+       "queries must be (N, num_heads, head_dim) for these pages");
+  const int N = static_cast<int>(queries.shape(0)), Hq = static_cast<int>(queries.shape(1));
+  const int64_t reach = static_cast<int64_t>(t.width) * d.page;
+  need(max_kv_len >= 0 || reach <= INT32_MAX, "block_tables reach past 32 bits");
+  const int n = max_kv_len < 0 ? static_cast<int>(reach) : max_kv_len, most = max_new < 0 ? N : max_new;
+  const int32_t *from = ints(starts, {static_cast<int64_t>(t.seqs) + 1}, "starts"), *lens = ints(seq_lens, {t.seqs}, "seq_lens");
+  array out = array::empty({N, Hq, d.D}, Dtype::float32);
+  size_t have = 0;
+  void* ws = workspace(tq_sdpa_int4_paged_chunks_workspace_size(t.seqs, N, Hq, d.Hkv, d.D, most, n), &have, s);
+  check(tq_sdpa_int4_paged_chunks(queries.data(), c_dtype(queries.dtype()), words(pages.k_quant),
+                                  pages.k_scales.data(), pages.k_biases.data(),
+                                  words(pages.v_quant), pages.v_scales.data(),
+                                  pages.v_biases.data(), d.sb, static_cast<float*>(out.data()),
+                                  t.seqs, N, Hq, d.Hkv, d.D, d.page, d.pages, t.p, t.width, from,
+                                  lens, most, n, gqa_factor, scale, sliding_window, num_sinks, ws,
+                                  have, s),
+        "sdpa_int4_paged_chunks");
+  return out;
+}
+
 array kv_pages_reserve(array& block_tables, array& refs, const array& lengths, const array& n_new,
                        int page_size, StreamOrDevice s) {
   const Tables t = tables_of(block_tables);
@@ -540,6 +568,22 @@ array kv_pages_fork(kv_pages& pages, array& block_tables, array& refs, array& le
   return granted;
 }
 
+array kv_pages_reorder(kv_pages& pages, array& block_tables, array& refs, array& lengths,
+                       const array& parents, StreamOrDevice s) {
+  const PoolDims d = pool_dims(pages, true);
+  const Tables t = tables_of(block_tables);
+  int32_t *r = ints(refs, {d.pages}, "refs"), *n = ints(lengths, {t.seqs}, "lengths");
+  const int32_t* from = ints(parents, {t.seqs}, "parents");
+  array granted = array::empty({t.seqs}, Dtype::int32);
+  size_t have = 0;
+  void* ws = workspace(tq_kv_pages_reorder_workspace_size(t.seqs, d.pages, t.width), &have, s, g_plan_ws);
+  check(tq_kv_pages_reorder(SixPages(pages).p, d.sb, d.layers, d.Hkv, d.D, t.p, r, n, from,
+                            static_cast<int32_t*>(granted.data()), t.seqs, t.width, d.pages, d.page,
+                            ws, have, s),
+        "kv_pages_reorder");
+  return granted;
+}
+
 void kv_pages_free(array& block_tables, array& refs, array& lengths, const array& which,
                    StreamOrDevice s) {
   const Tables t = tables_of(block_tables);
@@ -580,6 +624,49 @@ void kv_pages_copy(kv_pages& pages, const array& src, const array& dst, StreamOr
                          ints(src, {src.shape(0)}, "src"), ints(dst, {src.shape(0)}, "dst"),
                          static_cast<int>(src.shape(0)), s),
         "kv_pages_copy");
+}
+
+// ---------------------------------------------------------------------------
+// Beam search
+
+beams beam_select(const array& logits, const array& scores, int num_out, const array& finished,
+                  int pad_token, StreamOrDevice s) {
+  need(logits.ndim() == 3, "logits must be (groups, beams, vocab)");
+  for (int i = 0; i < 3; ++i) need(logits.shape(i) <= INT32_MAX, "logits: a size does not fit 32 bits");
+  const int G = static_cast<int>(logits.shape(0)), W = static_cast<int>(logits.shape(1));
+  const int V = static_cast<int>(logits.shape(2)), K = num_out == 0 ? W : num_out;
+  need(scores.dtype() == Dtype::float32 && scores.shape() == std::vector<int64_t>{G, W},
+       "scores must be float32 (groups, beams)");
+  need(finished.ndim() == 0 || (finished.dtype() == Dtype::uint8 && finished.shape() == scores.shape()),
+       "finished must be uint8 (groups, beams)");
+  need(K >= 1, "num_out must be >= 1");
+  beams out{array::empty({G, K}, Dtype::float32), array::empty({G, K}, Dtype::int32),
+            array::empty({G, K}, Dtype::int32)};
+  size_t have = 0;
+  void* ws = workspace(tq_beam_select_workspace_size(G, W, V), &have, s, g_plan_ws);
+  check(tq_beam_select(logits.data(), c_dtype(logits.dtype()), static_cast<int64_t>(W) * V, V,
+                       static_cast<const float*>(scores.data()),
+                       finished.ndim() > 0 ? static_cast<const uint8_t*>(finished.data()) : nullptr, G,
+                       W, V, K, pad_token, static_cast<float*>(out.scores.data()),
+                       static_cast<int32_t*>(out.parents.data()),
+                       static_cast<int32_t*>(out.tokens.data()), ws, have, s),
+        "beam_select");
+  return out;
+}
+
+void kv_reorder_int4(array& k_quant, array& k_scales, array& k_biases, array& v_quant,
+                     array& v_scales, array& v_biases, array& lengths, const array& parents,
+                     StreamOrDevice s) {
+  // (the same tensors as a pool's, sequences in place of pages)
+  const PoolDims d = pool_dims(kv_pages{k_quant, k_scales, k_biases, v_quant, v_scales, v_biases}, false);
+  int32_t* n = ints(lengths, {d.pages}, "lengths");
+  const int32_t* from = ints(parents, {d.pages}, "parents");
+  size_t have = 0;
+  void* ws = workspace(tq_kv_reorder_int4_workspace_size(d.pages), &have, s, g_plan_ws);
+  check(tq_kv_reorder_int4(static_cast<uint32_t*>(k_quant.data()), k_scales.data(), k_biases.data(),
+                           static_cast<uint32_t*>(v_quant.data()), v_scales.data(), v_biases.data(),
+                           d.sb, d.pages, d.Hkv, d.D, d.page, n, from, ws, have, s),
+        "kv_reorder_int4");
 }
 
 // ---------------------------------------------------------------------------

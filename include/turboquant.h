@@ -176,6 +176,16 @@ array sdpa_int4_paged_prefill(const array& queries, const kv_pages& pages,
                               float scale = 1.0f, int sliding_window = 0, int num_sinks = 0,
                               StreamOrDevice s = {});
 
+// Chunks of new tokens of a batch: queries (N, num_heads, head_dim), those of sequence b
+// in rows starts[b] .. starts[b + 1] - 1 (starts int32 (B + 1)), at the end of its first
+// seq_lens[b] rows, which hold the new ones already.  max_new < 0: N; max_kv_len < 0: what
+// the tables reach.  Returns (N, num_heads, head_dim) f32, unwritten behind starts[B].
+array sdpa_int4_paged_chunks(const array& queries, const kv_pages& pages,
+                             const array& block_tables, const array& starts,
+                             const array& seq_lens, int gqa_factor, float scale = 1.0f,
+                             int sliding_window = 0, int num_sinks = 0, int max_new = -1,
+                             int max_kv_len = -1, StreamOrDevice s = {});
+
 // Pages for rows lengths[s] .. lengths[s] + n_new[s] - 1.  Returns int32
 // (num_seqs): 1 where the request was granted (as kv_pages_fork does).
 array kv_pages_reserve(array& block_tables, array& refs, const array& lengths, const array& n_new,
@@ -187,6 +197,10 @@ array kv_pages_advance(const array& block_tables, const array& refs, array& leng
 // Sequence s continues parents[s] (negative: none).
 array kv_pages_fork(kv_pages& pages, array& block_tables, array& refs, array& lengths,
                     const array& parents, StreamOrDevice s = {});
+// Every sequence becomes the continuation of parents[s] as it was, all at once (outside
+// [0, num_seqs): ends).  Returns int32 (num_seqs): 1 where it continues one.
+array kv_pages_reorder(kv_pages& pages, array& block_tables, array& refs, array& lengths,
+                       const array& parents, StreamOrDevice s = {});
 // Ends the sequences with which[s] != 0.
 void kv_pages_free(array& block_tables, array& refs, array& lengths, const array& which,
                    StreamOrDevice s = {});
@@ -198,6 +212,22 @@ void kv_pages_evict(array& block_tables, array& refs, const array& lengths, int 
 array kv_pages_compact(kv_pages& pages, array& block_tables, array& refs, StreamOrDevice s = {});
 // Copies page src[i] to page dst[i].
 void kv_pages_copy(kv_pages& pages, const array& src, const array& dst, StreamOrDevice s = {});
+
+// ---- beam search (no counterpart in the reference) ---------------------------
+// tq_beam_select and tq_kv_reorder_int4 of tq_c_api.h; workspaces and outputs as above.
+struct beams {
+  array scores, parents, tokens;  // (groups, num_out) f32, int32, int32
+};
+// The num_out (0: as many as there are) best continuations of every group of beams:
+// logits (groups, beams, vocab) f32|f16|bf16, scores (groups, beams) f32, finished uint8
+// (groups, beams) or empty: those continue as themselves, with pad_token.
+beams beam_select(const array& logits, const array& scores, int num_out = 0,
+                  const array& finished = {}, int pad_token = 0, StreamOrDevice s = {});
+// Rows and lengths of sequence b of (B, Hkv, capacity, .) caches become those of
+// parents[b] as they were, in place; lengths, parents int32 (B).
+void kv_reorder_int4(array& k_quant, array& k_scales, array& k_biases, array& v_quant,
+                     array& v_scales, array& v_biases, array& lengths, const array& parents,
+                     StreamOrDevice s = {});
 
 // ---- PolarQuant (lib/turboquant.h:52-165) -----------------------------------
 // Reference layouts: 16-value blocks, 4 levels, codebooks per level.
