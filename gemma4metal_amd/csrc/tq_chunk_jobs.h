@@ -15,6 +15,7 @@ struct TileParams : PagedParams {
   const int* starts;
   int queries, few;
   int max_new;  // queries of a sequence that are served
+  int slots;    // of the workspace
 };
 
 int launch_chunk_tiles(const TileParams& p, int D, int sb_dtype, int rs, int64_t jobs, hipStream_t s);
@@ -34,6 +35,9 @@ __device__ __forceinline__ int max_of_wave(int v) {
   return __builtin_amdgcn_readfirstlane(max(static_cast<int>(b[0]), static_cast<int>(b[1])));
 }
 __device__ __forceinline__ int min_of_wave(int v) { return -max_of_wave(-v); }
+
+// A row's result: 0 where it attends nothing (weights of NaN stay NaN).
+__device__ __forceinline__ float chunk_result(float O, float L) { return L == 0.0f ? 0.0f : O / L; }
 
 // A job is (sequence, block of rows, kv head, split of its tiles); the device lays them
 // out from the lengths.  A wave of every workgroup works it out, a sequence a lane: one
@@ -128,12 +132,16 @@ __device__ __forceinline__ int chunk_tiles(const TileParams& p, const ChunkSeq& 
   return best;
 }
 
-__device__ __forceinline__ int scan_of_wave(int v) {  // inclusive
+// Inclusive prefix, of counts up to kMostJobs, where it stays: starts that do not ascend may
+// add up to anything, and what lies past the grid or the slots is left out.
+constexpr int kMostJobs = 1 << 29;
+
+__device__ __forceinline__ int scan_of_wave(int v) {
   const int lane = threadIdx.x & 63;
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) {
     const int y = __shfl_up(v, d, 64);
-    if (lane >= d) v += y;
+    if (lane >= d) v = min(v + y, kMostJobs);
   }
   return v;
 }
@@ -150,26 +158,30 @@ __device__ __forceinline__ ChunkJob find_chunk_job(const TileParams& p, int j) {
   for (int b0 = 0; b0 < p.nq; b0 += 64) {
     const ChunkSeq c = b0 == 0 ? first : chunk_seq<ROWS, TK, FEW>(p, b0 + lane);
     const int s = splits_of(c, T), mine = c.blocks * p.Hkv;
-    const int slot = s > 1 ? mine * s : 0;
-    const int n = MERGE ? (s > 1 ? mine : 0) : mine * s;
-    const int upto = jobs + scan_of_wave(n), slot_upto = slots + scan_of_wave(slot);
+    const int slot = s > 1 ? min(mine * s, kMostJobs) : 0;
+    const int n = MERGE ? (s > 1 ? mine : 0) : s > 1 ? slot : mine;
+    const int upto = min(jobs + scan_of_wave(n), kMostJobs), slot_upto = min(slots + scan_of_wave(slot), kMostJobs);
     const uint64_t hit = __ballot(upto > j);
     if (hit != 0) {
       const int l = __builtin_ctzll(hit);
       const auto of = [&](int v) { return __builtin_amdgcn_readlane(v, l); };
+      // (of the lanes before: not past j)
+      const int before = l > 0 ? __builtin_amdgcn_readlane(upto, l - 1) : jobs;
+      const int slot0 = l > 0 ? __builtin_amdgcn_readlane(slot_upto, l - 1) : slots;
       r.b = b0 + l;
       r.s0 = of(c.s0);
       r.n = of(c.n);
       r.len = of(c.len);
       r.splits = of(s);
       const int blocks = of(c.blocks);
-      int at = j - (of(upto) - of(n));
+      int at = j - before;
       r.kvh = at % p.Hkv;
       at /= p.Hkv;
       r.split = MERGE ? 0 : at % r.splits;
       if (!MERGE) at /= r.splits;
       r.blk = blocks - 1 - at;  // the longest key ranges (last queries) start first
-      r.slot = of(slot_upto) - of(slot) + (r.blk * p.Hkv + r.kvh) * r.splits + r.split;
+      r.slot = slot0 + (r.blk * p.Hkv + r.kvh) * r.splits + r.split;
+      if (r.splits > 1 && r.slot > p.slots - (MERGE ? r.splits : 1)) r.splits = 0;
       return r;
     }
     jobs = __builtin_amdgcn_readlane(upto, 63);

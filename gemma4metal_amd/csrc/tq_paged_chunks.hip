@@ -457,8 +457,9 @@ void paged_few_kernel(TileParams p) {
           // the row's largest to 2^13 .. 2^14 (an infinity, of exponent 0, stays one)
           const float top = xor32_max(xor16_max(big));
           const float now = ldexpf(1.0f, min(14 - __builtin_amdgcn_frexp_expf(top), 120));
-          const float fr = top * ef[g] > 0x1p15f && now < ef[g] ? ldexpf(now, 1 - __builtin_amdgcn_frexp_expf(ef[g])) : 1.0f;
-          ef[g] *= fr;
+          const bool down = top * ef[g] > 0x1p15f && now < ef[g];
+          const float fr = down ? ldexpf(now, 1 - __builtin_amdgcn_frexp_expf(ef[g])) : 1.0f;  // (may be 0: nothing is left)
+          ef[g] = down ? now : ef[g];
 #pragma unroll
           for (int x = 0; x < 4; ++x) o[4 * g + x] *= fr;
         }
@@ -521,7 +522,7 @@ void paged_few_kernel(TileParams p) {
     if (job.splits == 1) {
       const int qo = Ro / p.gqa;
       const int64_t row = static_cast<int64_t>(qo + job.s0) * p.Hq + job.kvh * p.gqa + (Ro - qo * p.gqa);
-      *reinterpret_cast<float2*>(p.out + row * D + d) = make_float2(normalise(x0, l, 0.0f), normalise(x1, l, 0.0f));
+      *reinterpret_cast<float2*>(p.out + row * D + d) = make_float2(chunk_result(x0, l), chunk_result(x1, l));
     } else {
       const int64_t slot = static_cast<int64_t>(job.slot) * kFewBlock + r;
       *reinterpret_cast<float2*>(p.ws_o + slot * D + d) = make_float2(x0, x1);
@@ -574,7 +575,7 @@ __device__ __forceinline__ void merge_job(const TileParams& p, int j, int y, int
     }
     v4f y;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) y[e] = normalise(O[e], L, 0.0f);
+    for (int e = 0; e < 4; ++e) y[e] = chunk_result(O[e], L);
     const int row = job.blk * ROWS + r, q = row / p.gqa;
     reinterpret_cast<v4f*>(p.out)[(static_cast<int64_t>(job.s0 + q) * p.Hq + job.kvh * p.gqa + (row - q * p.gqa)) * D4 + u % D4] = y;
   }
@@ -658,6 +659,8 @@ int launch_chunks(const PagedParams& p0, const PagedParams& few0, int D, int sb_
   p.queries = few.queries = queries;
   p.few = few.few = plan.few;
   p.max_new = few.max_new = max_new;
+  p.slots = static_cast<int>(plan.tiles.slots);
+  few.slots = static_cast<int>(plan.few_rows.slots);
   few.cus = static_cast<int>(few_cus(D));
   if (plan.tiles.jobs > 0)
     if (int r = launch_chunk_tiles(p, D, sb_dtype, plan.rs, plan.tiles.jobs, s)) return r;

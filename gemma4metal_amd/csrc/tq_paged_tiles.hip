@@ -823,7 +823,9 @@ void paged_tiles_kernel(TileParams p) {
     const int qo = Ro / p.gqa;
     const int64_t row = static_cast<int64_t>(qo + job.s0) * p.Hq + kvh * p.gqa + (Ro - qo * p.gqa);
     if (BATCH ? splits == 1 : p.ext_merge == 0) {
-      *reinterpret_cast<float2*>(p.out + row * D + d) = make_float2(normalise(x0, l, 0.0f), normalise(x1, l, 0.0f));
+      *reinterpret_cast<float2*>(p.out + row * D + d) =
+          BATCH ? make_float2(chunk_result(x0, l), chunk_result(x1, l))
+                : make_float2(normalise(x0, l, 0.0f), normalise(x1, l, 0.0f));
     } else {
       const int64_t slot = BATCH ? static_cast<int64_t>(job.slot) * kRows + r : row * p.max_splits + blockIdx.y;
       *reinterpret_cast<float2*>(p.ws_o + slot * D + d) = make_float2(x0, x1);

@@ -88,6 +88,13 @@ def test_select(bm, dtype, B, W, V, K):
     check(bm.beam_select(x, dev(scores), K), xf, scores, K)
 
 
+def test_a_vocabulary_of_more_sums_than_lanes(bm):
+    rng = np.random.default_rng(13)
+    x, xf = logits(rng, (1, 2, 300001), "bf16")
+    scores = np.array([[-1.0, -1.25]], np.float32)
+    check(bm.beam_select(x, dev(scores), 5), xf, scores, 5)
+
+
 def test_ties_go_to_the_lowest(bm):
     """Equal rows at unlike alignments, equal logits, and rows of one value."""
     rng = np.random.default_rng(3)

@@ -110,6 +110,72 @@ def test_missing_pages_short_lengths_and_rows_behind(pg):
     assert run(pg, q[:0], pages, tables, [0] * 6, lens, 2).shape == (0, Hq, D)
 
 
+@pytest.mark.parametrize("big", [1e-30, 1e25, 1e36])
+@pytest.mark.parametrize("D,new", [(128, 3), (256, 3), (256, 60), (512, 1), (512, 30)])
+def test_any_range_of_v_scales(pg, D, new, big):
+    """V scales and biases of fp32 caches near the ends of fp32, one key far above the
+    others (some rows attend it, some do not), and groups far apart."""
+    rng = np.random.default_rng(D)
+    Hq, Hkv, page, lens = 4, 2, 32, [new + 70, new]
+    q, qf, pages, tables, starts = batch(rng, [new, new], lens, Hq, Hkv, D, page, "f32", "f32")
+    for i in (4, 5):
+        pages[i] *= np.float32(big)
+        pages[i][..., 0] *= np.float32(1e-7)
+    for t in (40, lens[0] - 1):          # keys of sequence 0
+        e = tables[0, t // page]
+        for i in (4, 5):
+            pages[i][e, :, t % page] *= np.float32(100)
+    ref = OP.sdpa_int4_paged_chunks(qf, pages, tables, starts, lens, page, 2, 0.05)
+    got = run(pg, q, pages, tables, starts, lens, 2, 0.05).astype(np.float64)
+    # By group of 64 dims: a group's precision is its own.  Weights are at most 2^8 and are
+    # summed before they are divided by their sum: values of more than 2^128 / (2^8 keys)
+    # may overflow (at 1e36 all do, and infinities come of times 100), to infinity or NaN.
+    most = np.abs(pages[4]).max(axis=(0, 1, 2)) * 15 + np.abs(pages[5]).max(axis=(0, 1, 2))
+    for g in range(D // 64):
+        a, b = got[..., 64 * g:64 * g + 64], ref[..., 64 * g:64 * g + 64]
+        fine = np.isfinite(a).all(-1)
+        assert fine.all() or not most[g] < 2.0**128 / (2.0**8 * lens[0]), g
+        a, b = a[fine] / big, b[fine] / big
+        err = np.linalg.norm(a - b, axis=-1) / np.linalg.norm(b, axis=-1)
+        assert fine.sum() == 0 or err.max() <= 1e-4, (g, err.max())
+
+
+def test_infinite_values_stay_with_who_attends_them(pg):
+    """A key with infinite V scales or biases, or NaN ones: only the queries that see it
+    have them in their results."""
+    rng = np.random.default_rng(8)
+    for D, new in ((128, 5), (256, 60), (512, 2), (512, 30)):
+        Hq, Hkv, page, lens = 4, 2, 32, [new + 100]
+        q, qf, pages, tables, starts = batch(rng, [new], lens, Hq, Hkv, D, page)
+        t = lens[0] - 1                   # the last query's own key
+        for i, bad in ((4, np.inf), (5, np.nan), (1, np.nan)):
+            p = [x.copy() for x in pages]
+            p[i][tables[0, t // page], :, t % page] = bad
+            got = run(pg, q, p, tables, starts, lens, 2)
+            with np.errstate(invalid="ignore"):
+                ref = OP.sdpa_int4_paged_chunks(qf, pages, tables, starts, lens, page, 2)
+            close(got[:-1], ref[:-1])
+            assert not np.isfinite(got[-1]).all()
+
+
+def test_starts_that_do_not_ascend(pg):
+    """Nothing can be said of the result, but nothing else is touched either."""
+    rng = np.random.default_rng(12)
+    new, lens = [2, 3, 1], [700, 900, 300]
+    q, qf, pages, tables, starts = batch(rng, new, lens, 4, 2, 128, 32)
+    d, t, n = [dev(p) for p in pages], dev(tables), ints(lens)
+    ws = torch.zeros(1 << 26, dtype=torch.uint8, device="cuda")
+    big = torch.full((40, 4, 128), 5.0, device="cuda")
+    call = lambda st: pg.sdpa_int4_paged_chunks(q, *d, t, ints(st), n, 2, out=big[16:22], max_kv_len=900, workspace=ws)  # noqa: E731
+    need = pg._chunks_ws_size(3, 6, 4, 2, 128, 6, 900)
+    ws[need:] = 77
+    for bad in ([0, 6, 0, 6], [6, 0, 6, 0], [-9, 100, -9, 100], [2**31 - 1, -2**31, 2**31 - 1, 5]):
+        call(bad)
+        torch.cuda.synchronize()
+        assert (big[:16] == 5).all() and (big[22:] == 5).all() and (ws[need:] == 77).all() and not ws[:1 << 18].any()
+    close(host(call(starts)), OP.sdpa_int4_paged_chunks(qf, pages, tables, starts, lens, 32, 2))
+
+
 def test_equal_to_the_calls_it_stands_for(pg):
     """A prompt's chunks one after the other, and single tokens, as the calls of one
     sequence and of one token have them."""
