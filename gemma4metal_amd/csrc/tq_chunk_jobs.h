@@ -15,7 +15,7 @@ struct TileParams : PagedParams {
   const int* starts;
   int queries, few;
   int max_new;  // queries of a sequence that are served
-  int slots;    // of the workspace
+  int slots;    // of the workspace; 0: no splits
 };
 
 int launch_chunk_tiles(const TileParams& p, int D, int sb_dtype, int rs, int64_t jobs, hipStream_t s);
@@ -151,7 +151,7 @@ template <int ROWS, int TK, bool FEW, bool MERGE>
 __device__ __forceinline__ ChunkJob find_chunk_job(const TileParams& p, int j) {
   const int lane = threadIdx.x & 63;
   const ChunkSeq first = chunk_seq<ROWS, TK, FEW>(p, lane);
-  const int T = chunk_tiles<ROWS, TK, FEW>(p, first);
+  const int T = p.slots > 0 ? chunk_tiles<ROWS, TK, FEW>(p, first) : 1 << 30;
   int jobs = 0, slots = 0;  // of the sequences before these
   ChunkJob r{};
 #pragma unroll 1

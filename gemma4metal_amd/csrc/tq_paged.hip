@@ -364,9 +364,10 @@ extern "C" size_t tq_sdpa_int4_paged_chunks_workspace_size(int batch, int querie
   if (batch < 1 || queries < 1 || num_kv_heads < 1 || num_heads < num_kv_heads || num_heads % num_kv_heads != 0 ||
       (head_dim != 128 && head_dim != 256 && head_dim != 512) || max_new < 0 || max_kv_len < 0)
     return 0;
+  // (a window only takes keys away; where it leaves so few that nothing is split, none)
   size_t most = 0;
   for (bool all32 : {false, true}) {
-    const ChunksPlan pl = plan_chunks(batch, queries, num_heads / num_kv_heads, num_kv_heads, head_dim, max_new, max_kv_len, all32);
+    const ChunksPlan pl = plan_chunks(batch, queries, num_heads / num_kv_heads, num_kv_heads, head_dim, max_new, max_kv_len, 0, 0, all32);
     if (pl.tiles.slots + pl.few_rows.slots > 0) most = std::max(most, chunks_layout(pl, head_dim).total);
   }
   return most;
@@ -398,7 +399,7 @@ extern "C" int tq_sdpa_int4_paged_chunks(const void* q, tq_dtype q_dtype, const 
   p.seq_lens = seq_lens;
   p.n_clamp = max_kv_len;
   const ChunksPlan plan = plan_chunks(batch, queries, gqa_factor, num_kv_heads, head_dim, max_new, max_kv_len,
-                                      q_dtype == TQ_F32 && sb_dtype == TQ_F32);
+                                      sliding_window, num_sinks, q_dtype == TQ_F32 && sb_dtype == TQ_F32);
   TQ_CHECK_ARG(plan.tiles.jobs < (int64_t{1} << 29) && plan.few_rows.jobs < (int64_t{1} << 29), "%s: grid too large", fn);
   PagedParams few = p;
   if (plan.tiles.slots + plan.few_rows.slots > 0) {

@@ -9,8 +9,12 @@
 // fp16 high part and remainder), with one difference: the weights p s_v of every (row,
 // group) of a block go in under a power of two of their own and the products are added
 // to the sums in fp32, so that no range of V scales needs a path beside this one.
-// What bounds it: HBM, while VALU (about 700 instructions a wave and block at D 256)
-// keeps up.
+// What bounds it: VALU (about 700 instructions a wave and block at D 256, 58% of a SIMD's
+// cycles with two waves) and the start and end of a workgroup (about 9 us).  5 new tokens
+// of 32 sequences behind a window of 1,024 (Hq 32 Hkv 16 D 256): 50 us, 3.0 TB/s of what
+// has to be read, where the tile kernel takes 121.  Measured, not kept: workgroups of eight
+// waves, one a CU, 69; V's operands read ahead of the softmax 60 (spills); nibbles as fp16
+// subnormals, uncentred, for K 51 against 55, but errors of 3e-6 to 5e-6 in place of 0.5e-6.
 #include "tq_chunk_jobs.h"
 #include "tq_prefill_tile.h"
 
@@ -615,10 +619,15 @@ void launch_merge(const TileParams& few, const TileParams& tiles, int few_n, int
 }
 
 // The jobs of `blocks` blocks of rows of at most `tiles` tiles on `cus` workgroups at
-// once, and the slots for the partials of split ones (chunk_tiles has both bounds).
-ChunkJobs jobs_of(int64_t blocks, int64_t tiles, int least, int64_t cus) {
+// once, and the slots for the partials of split ones (chunk_tiles has both bounds).  Where
+// the blocks fill the chip and none is longer than kEven keys, none is split: the merge's
+// launch is 4 us (5 tokens of 32 sequences behind a window of 1,024 53 us with it, 50 without).
+constexpr int kEven = 2048;
+
+ChunkJobs jobs_of(int64_t blocks, int64_t keys, int tile, int least, int64_t cus) {
+  const int64_t tiles = (keys + tile - 1) / tile;
   const int64_t splits = std::min<int64_t>((tiles + least - 1) / least, kMostSplits);
-  if (blocks == 0 || splits <= 1) return {blocks, 0};
+  if (blocks == 0 || splits <= 1 || (blocks >= cus && keys <= kEven)) return {blocks, 0};
   return {blocks + std::min(cus, blocks * (splits - 1)), std::min(2 * cus, blocks * splits)};
 }
 
@@ -626,10 +635,15 @@ int64_t few_cus(int D) { return D == 512 ? target_wgs() : 2 * target_wgs(); }
 
 }  // namespace
 
-ChunksPlan plan_chunks(int batch, int queries, int gqa, int Hkv, int D, int max_new, int64_t max_kv_len, bool all32) {
+ChunksPlan plan_chunks(int batch, int queries, int gqa, int Hkv, int D, int max_new, int64_t max_kv_len, int64_t window,
+                       int64_t sinks, bool all32) {
   ChunksPlan pl{};
   const int64_t rows = static_cast<int64_t>(std::min(max_new, queries)) * gqa, all = static_cast<int64_t>(queries) * gqa;
   const int64_t seqs = std::min(batch, queries);
+  // keys of a block of R rows at most, in whole tiles of either kernel (no fewer than chunk_seq counts)
+  const auto keys = [&](int64_t R) {
+    return window > 0 ? std::min<int64_t>(max_kv_len, window + R + 256 + (sinks + 63) / 64 * 64) : max_kv_len;
+  };
   pl.rs = D == 512 || (D == 256 && all32) || rows <= 64 ? 4 : 8;
   // sequences of few rows alone, or a batch that may hold some (a launch without work
   // takes up to 10 us), or none
@@ -637,13 +651,12 @@ ChunksPlan plan_chunks(int batch, int queries, int gqa, int Hkv, int D, int max_
   // blocks of rows of any chunks that add up to `queries`
   if (pl.few != INT_MAX) {
     const int64_t n = std::min(seqs, all / (pl.few + 1)), R = 16 * pl.rs;
-    const int tile = D == 512 ? 32 : 64;
-    pl.tiles = jobs_of(std::min(all / R + n, n * ((rows + R - 1) / R)) * Hkv, (max_kv_len + tile - 1) / tile,
+    pl.tiles = jobs_of(std::min(all / R + n, n * ((rows + R - 1) / R)) * Hkv, keys(R), D == 512 ? 32 : 64,
                        kLeastTiles<false>, target_wgs());
   }
   if (pl.few != 0) {
     const int64_t blocks = (std::min<int64_t>(rows, pl.few) + kFewBlock - 1) / kFewBlock;
-    pl.few_rows = jobs_of(std::min(all / kFewBlock + seqs, seqs * blocks) * Hkv, (max_kv_len + 31) / 32,
+    pl.few_rows = jobs_of(std::min(all / kFewBlock + seqs, seqs * blocks) * Hkv, keys(kFewBlock), 32,
                           kLeastTiles<true>, few_cus(D));
   }
   return pl;

@@ -899,7 +899,8 @@ struct ChunksPlan {
   int rs, few;
   ChunkJobs tiles, few_rows;
 };
-ChunksPlan plan_chunks(int batch, int queries, int gqa, int Hkv, int D, int max_new, int64_t max_kv_len, bool all32);
+ChunksPlan plan_chunks(int batch, int queries, int gqa, int Hkv, int D, int max_new, int64_t max_kv_len, int64_t window,
+                       int64_t sinks, bool all32);
 int launch_chunks(const PagedParams& p, const PagedParams& few, int D, int sb_dtype, const ChunksPlan& plan,
                   const int* starts, int queries, int max_new, hipStream_t stream);
 // Merge of the split partials of a launch with ext_merge = 1 (batch b of
