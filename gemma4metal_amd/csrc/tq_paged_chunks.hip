@@ -9,7 +9,7 @@
 // fp16 high part and remainder), with one difference: the weights p s_v of every (row,
 // group) of a block go in under a power of two of their own and the products are added
 // to the sums in fp32, so that no range of V scales needs a path beside this one.
-// What bounds it: VALU (about 700 instructions a wave and block at D 256, 58% of a SIMD's
+// What bounds it: VALU (about 700 instructions a wave and block at D 256, 61% of a SIMD's
 // cycles with two waves) and the start and end of a workgroup (about 9 us).  5 new tokens
 // of 32 sequences behind a window of 1,024 (Hq 32 Hkv 16 D 256): 50 us, 3.0 TB/s of what
 // has to be read, where the tile kernel takes 121.  Measured, not kept: workgroups of eight

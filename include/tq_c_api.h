@@ -470,7 +470,8 @@ int tq_kv_pages_copy(void* const* pages, tq_dtype sb_dtype, int num_layers, int 
  *   first: the total, g * beams + w, and t; -inf, -1, -1 where there are fewer
  *   candidates.  They overlap no input.
  * 1 <= beams, num_out <= 64; vocab <= 2^24.  Sums of exponentials are held in 32 bits
- * within 1,024 tokens and in 64 beyond; totals are compared in 64.
+ * within 4,096 tokens and in 64 beyond; totals are compared in 64.  A beam's tokens are in
+ * exact order; totals of two beams that differ by less than about 1e-7 may change places.
  * workspace: tq_beam_select_workspace_size(...) bytes, 16-byte aligned; need not be
  * zeroed; calls that may overlap need one each. */
 size_t tq_beam_select_workspace_size(int groups, int beams, int vocab);
