@@ -18,7 +18,9 @@ struct TileParams : PagedParams {
   int slots;    // of the workspace; 0: no splits
 };
 
-int launch_chunk_tiles(const TileParams& p, int D, int sb_dtype, int rs, int64_t jobs, hipStream_t s);
+// few_jobs > 0: both kernels' jobs in one launch (D < 512).
+int launch_chunk_tiles(const TileParams& p, int D, int sb_dtype, int rs, int64_t jobs, const TileParams& few,
+                       int64_t few_jobs, hipStream_t s);
 
 namespace {
 
@@ -190,15 +192,14 @@ __device__ __forceinline__ ChunkJob find_chunk_job(const TileParams& p, int j) {
   return r;
 }
 
-// The same, found by the first wave for the whole workgroup (all of its threads ask; a
-// barrier).
+// The same, found by the first of the waves that ask (tid: a thread's number among theirs)
+// and told by way of the LDS.  A barrier of the workgroup.
 template <int ROWS, int TK, bool FEW, bool MERGE>
-__device__ __forceinline__ ChunkJob chunk_job(const TileParams& p, int j) {
-  __shared__ int told[kJobInts];
-  if (threadIdx.x < 64) {
+__device__ __forceinline__ ChunkJob chunk_job(const TileParams& p, int j, int tid, int (&told)[kJobInts]) {
+  if (tid < 64) {
     const ChunkJob r = find_chunk_job<ROWS, TK, FEW, MERGE>(p, j);
     const int v[kJobInts] = {r.b, r.s0, r.n, r.len, r.blk, r.kvh, r.split, r.splits, r.slot};
-    if (threadIdx.x == 0) {
+    if (tid == 0) {
 #pragma unroll
       for (int i = 0; i < kJobInts; ++i) told[i] = v[i];
     }

@@ -16,8 +16,7 @@
 //   then leave partials (m, l, O).
 // - fp32 queries are two fp16 parts, 22 bits, and take two products a k-step.
 //   fp32 biases are applied in fp32.
-#include "tq_chunk_jobs.h"
-#include "tq_prefill_tile.h"
+#include "tq_paged_few.h"
 
 #include <cfloat>
 
@@ -217,6 +216,21 @@ __device__ __forceinline__ void pg_alike(const PfRaw<Gm>& R, int e0, int* ok) {
   }
 }
 
+template <int D, bool F32>
+struct TilesLds {
+  using Gm = PfGeom<D, F32, kRs>;
+  union Shared {
+    PgStage<D, F32> st;
+    float o[Gm::NW][16 * Gm::OSTR];
+    __device__ Shared() {}
+  } u;
+  uint32_t vmx;               // bits of the first tile's largest |V scale|
+  int alike[2][2 * Gm::NSW];  // see pg_alike (all of them set)
+  float ml[Gm::NW][16], ll[Gm::NW][16];
+  int told[kJobInts];
+  __device__ TilesLds() {}
+};
+
 // RS: 16-row sets of a workgroup.  4: a wave takes 32 keys of a tile (of 64 keys, D
 // 512 of 32); 8 (D < 512): all 64, one half after the other, so that twice as many
 // rows share the staging of a tile (64 sequences with 2 query heads a kv head over
@@ -225,8 +239,7 @@ __device__ __forceinline__ void pg_alike(const PfRaw<Gm>& R, int e0, int* ok) {
 // cores 27% there, 49% and 23% at D 512 (2,048 queries after 6,144 keys: 2.75 ms, 350
 // TFLOP/s); a wave runs the two one after the other.
 template <int D, bool F32, bool Q32, int RS, bool BATCH>
-__global__ __launch_bounds__(128 * kRs) __attribute__((amdgpu_waves_per_eu(2, 2)))
-void paged_tiles_kernel(TileParams p) {
+__device__ __forceinline__ void tiles_job(const TileParams& p, TilesLds<D, F32>& lds) {
   using Gm = PfGeom<D, F32, kRs>;
   using SB = typename Gm::SB;
   constexpr int NG = Gm::NG, NWG = Gm::NW_, TK = Gm::TK, KH = Gm::KH, DH = Gm::DH;
@@ -234,14 +247,10 @@ void paged_tiles_kernel(TileParams p) {
   constexpr int kRows = 16 * RS;
   static_assert(KW >= 1 && HB >= 1, "waves");
   using St = PgStage<D, F32>;
-  __shared__ __attribute__((aligned(16))) union Lds {
-    St st;
-    float o[Gm::NW][16 * Gm::OSTR];
-    __device__ Lds() {}
-  } L;
-  __shared__ uint32_t vmx;                  // bits of the first tile's largest |V scale|
-  __shared__ int alike[2][2 * Gm::NSW];     // see pg_alike (all of them set)
-  __shared__ float ml[Gm::NW][16], ll[Gm::NW][16];
+  auto& L = lds.u;
+  auto& vmx = lds.vmx;
+  auto& alike = lds.alike;
+  auto &ml = lds.ml, &ll = lds.ll;
 
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
@@ -250,7 +259,7 @@ void paged_tiles_kernel(TileParams p) {
   // heads vary fastest, the longest key ranges (last queries) start first
   ChunkJob job{};
   if constexpr (BATCH) {
-    job = chunk_job<kRows, TK, false, false>(p, blockIdx.x);
+    job = chunk_job<kRows, TK, false, false>(p, blockIdx.x, threadIdx.x, lds.told);
     if (job.splits == 0) return;            // (all waves)
   }
   const int nblk = gridDim.x / p.Hkv;
@@ -834,6 +843,34 @@ void paged_tiles_kernel(TileParams p) {
   }
 }
 
+template <int D, bool F32, bool Q32, int RS, bool BATCH>
+__global__ __launch_bounds__(128 * kRs) __attribute__((amdgpu_waves_per_eu(2, 2)))
+void paged_tiles_kernel(TileParams p) {
+  __shared__ __attribute__((aligned(16))) TilesLds<D, F32> lds;
+  tiles_job<D, F32, Q32, RS, BATCH>(p, lds);
+}
+
+// The jobs of a batch of both kinds: `tiles` workgroups, then pairs of jobs of few rows, a
+// half of a workgroup each, which start where the tiles' workgroups leave CUs idle.
+template <int D, bool F32, bool Q32, int RS>
+__global__ __launch_bounds__(128 * kRs) __attribute__((amdgpu_waves_per_eu(2, 2)))
+void paged_mixed_kernel(TileParams p, TileParams few, int tiles) {
+  using Few = FewGeom<D, F32>;
+  static_assert(2 * Few::NT == 128 * kRs, "halves");
+  __shared__ __attribute__((aligned(16))) union Lds {
+    TilesLds<D, F32> tiles;
+    typename Few::Lds few[2];
+    __device__ Lds() {}
+  } lds;
+  const int i = static_cast<int>(blockIdx.x) - tiles;
+  if (i < 0) {
+    tiles_job<D, F32, Q32, RS, true>(p, lds.tiles);
+  } else {
+    const int half = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / Few::NT);
+    few_job<D, F32, Q32>(few, 2 * i + half, threadIdx.x % Few::NT, lds.few[half]);
+  }
+}
+
 // The output of a row from its S partials: a thread takes four dims.
 __global__ __launch_bounds__(256) void merge_tiles_kernel(const float* ws_ml, const float* ws_o, float* out,
                                                           int64_t rows, int S, int stride, int D4) {
@@ -874,6 +911,27 @@ void launch_dim(const TileParams& p, int D, int rs, dim3 grid, hipStream_t s) {
   if (D == 512) launch_q<512, F32, 4, BATCH>(p, grid, s);
   else if (D == 256) rs == 8 ? launch_q<256, F32, 8, BATCH>(p, grid, s) : launch_q<256, F32, 4, BATCH>(p, grid, s);
   else rs == 8 ? launch_q<128, F32, 8, BATCH>(p, grid, s) : launch_q<128, F32, 4, BATCH>(p, grid, s);
+}
+
+template <bool F32>
+void launch_mixed(const TileParams& p, int D, int rs, int jobs, const TileParams& few, int64_t few_jobs, hipStream_t s) {
+  const unsigned grid = static_cast<unsigned>(jobs + (few_jobs + 1) / 2);
+  const auto run = [&](auto d, auto r) {
+    constexpr int kD = decltype(d)::value, kR = decltype(r)::value;
+    if constexpr (!(kD == 256 && F32 && kR == 8)) {
+      if (p.q_dtype == TQ_F32) {
+        paged_mixed_kernel<kD, F32, true, kR><<<grid, 128 * kRs, 0, s>>>(p, few, jobs);
+        return;
+      }
+    }
+    paged_mixed_kernel<kD, F32, false, kR><<<grid, 128 * kRs, 0, s>>>(p, few, jobs);
+  };
+  const std::integral_constant<int, 128> d128;
+  const std::integral_constant<int, 256> d256;
+  const std::integral_constant<int, 4> r4;
+  const std::integral_constant<int, 8> r8;
+  if (D == 256) rs == 8 ? run(d256, r8) : run(d256, r4);
+  else rs == 8 ? run(d128, r8) : run(d128, r4);
 }
 
 int tile_keys(int D) { return D == 512 ? 32 : 64; }
@@ -945,7 +1003,14 @@ int launch_paged_tiles(const PagedParams& p0, int D, int sb_dtype, TilesPlan pla
   return TQ_OK;
 }
 
-int launch_chunk_tiles(const TileParams& p, int D, int sb_dtype, int rs, int64_t jobs, hipStream_t s) {
+int launch_chunk_tiles(const TileParams& p, int D, int sb_dtype, int rs, int64_t jobs, const TileParams& few,
+                       int64_t few_jobs, hipStream_t s) {
+  if (few_jobs > 0) {
+    if (sb_dtype == TQ_F32) launch_mixed<true>(p, D, rs, static_cast<int>(jobs), few, few_jobs, s);
+    else launch_mixed<false>(p, D, rs, static_cast<int>(jobs), few, few_jobs, s);
+    TQ_CHECK_LAUNCH("paged_mixed_kernel");
+    return TQ_OK;
+  }
   const dim3 grid(static_cast<unsigned>(jobs));
   if (sb_dtype == TQ_F32) launch_dim<true, true>(p, D, rs, grid, s);
   else launch_dim<false, true>(p, D, rs, grid, s);
