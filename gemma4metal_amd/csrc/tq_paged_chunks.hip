@@ -107,16 +107,19 @@ void launch_merge(const TileParams& few, const TileParams& tiles, int few_n, int
   merge_chunks_kernel<D, 64><<<grid, kMergeThreads, 0, s>>>(few, tiles, few_n);
 }
 
-// The jobs of `blocks` blocks of rows of at most `tiles` tiles on `cus` workgroups at
-// once, and the slots for the partials of split ones (chunk_tiles has both bounds).  Where
-// the blocks fill the chip and none is longer than kEven keys, none is split: the merge's
-// launch is 4 us (5 tokens of 32 sequences behind a window of 1,024 53 us with it, 50 without).
+// The jobs of `blocks` blocks of rows of at most `keys` keys on `cus` workgroups at once,
+// and the slots for the partials of split ones (chunk_tiles has both bounds).  Where the
+// blocks, or those of the other kernel beside them (filled), fill the chip and none is
+// longer than kEven keys, none is split: the merge's launch is 4 us (5 tokens of 32
+// sequences behind a window of 1,024 53 us with it, 50 without), and jobs that there might
+// be and are not, 11 ns each (2 chunks of 700 and 6 of 300, D 256, 214 us with splits of
+// few rows in the grid, 209 without).
 constexpr int kEven = 2048;
 
-ChunkJobs jobs_of(int64_t blocks, int64_t keys, int tile, int least, int64_t cus) {
+ChunkJobs jobs_of(int64_t blocks, int64_t keys, int tile, int least, int64_t cus, bool filled) {
   const int64_t tiles = (keys + tile - 1) / tile;
   const int64_t splits = std::min<int64_t>((tiles + least - 1) / least, kMostSplits);
-  if (blocks == 0 || splits <= 1 || (blocks >= cus && keys <= kEven)) return {blocks, 0};
+  if (blocks == 0 || splits <= 1 || ((filled || blocks >= cus) && keys <= kEven)) return {blocks, 0};
   return {blocks + std::min(cus, blocks * (splits - 1)), std::min(2 * cus, blocks * splits)};
 }
 
@@ -134,19 +137,21 @@ ChunksPlan plan_chunks(int batch, int queries, int gqa, int Hkv, int D, int max_
     return window > 0 ? std::min<int64_t>(max_kv_len, window + R + 256 + (sinks + 63) / 64 * 64) : max_kv_len;
   };
   pl.rs = D == 512 || (D == 256 && all32) || rows <= 64 ? 4 : 8;
-  // sequences of few rows alone, or a batch that may hold some (a launch without work
-  // takes up to 10 us), or none
-  pl.few = rows <= few_rows(D) ? INT_MAX : batch > 1 && all / batch < 4 * few_rows(D) ? few_rows(D) : 0;
+  // sequences of few rows alone, or a batch that may hold some, or none.  (Us without and
+  // with them apart, D 256: 3 chunks of 1,000 among 24 sequences 686, 549; 2 of 700 and 6 of
+  // 300, none of them few, 207, 209.  At D 512, where a launch of its own without work takes
+  // up to 10, only where chunks are short on average.)
+  pl.few = rows <= few_rows(D) ? INT_MAX : batch > 1 && (D < 512 || all / batch < 4 * few_rows(D)) ? few_rows(D) : 0;
   // blocks of rows of any chunks that add up to `queries`
   if (pl.few != INT_MAX) {
     const int64_t n = std::min(seqs, all / (pl.few + 1)), R = 16 * pl.rs;
     pl.tiles = jobs_of(std::min(all / R + n, n * ((rows + R - 1) / R)) * Hkv, keys(R), D == 512 ? 32 : 64,
-                       kLeastTiles<false>, target_wgs());
+                       kLeastTiles<false>, target_wgs(), false);
   }
   if (pl.few != 0) {
     const int64_t blocks = (std::min<int64_t>(rows, pl.few) + kFewBlock - 1) / kFewBlock;
     pl.few_rows = jobs_of(std::min(all / kFewBlock + seqs, seqs * blocks) * Hkv, keys(kFewBlock), 32,
-                          kLeastTiles<true>, few_cus(D));
+                          kLeastTiles<true>, few_cus(D), D < 512 && pl.tiles.jobs > 0);
   }
   return pl;
 }

@@ -64,6 +64,25 @@ def test_types_and_many_rows(pg, Hq, Hkv, D, sb, qt):
         close(run(pg, q, pages, tables, starts, lens, Hq // Hkv, 0.3, max_new=most, max_kv_len=2100), ref)
 
 
+@pytest.mark.parametrize("sb,qt", [("f16", "bf16"), ("f32", "f32"), ("f16", "f32"), ("f32", "f16")])
+@pytest.mark.parametrize("Hq,Hkv,D", [(6, 3, 128), (12, 3, 256), (8, 1, 512)])
+@pytest.mark.parametrize("new,prior,window,sinks", [([1, 70, 3, 1, 2, 90, 1], [900, 10, 2100, 0, 33, 700, 64], 0, 0),
+                                                    ([129, 1, 0, 1], [0, 5, 9, 2600], 300, 4),
+                                                    ([1, 65], [3000, 0], 0, 0), ([64, 1, 64], [40, 1, 3000], 0, 0)])
+def test_long_chunks_and_few_rows_in_one_call(pg, Hq, Hkv, D, sb, qt, new, prior, window, sinks):
+    """Jobs of both kinds, odd numbers of either, split and whole; again after a call
+    that left other partials, bit by bit."""
+    rng = np.random.default_rng(len(new) + D)
+    lens = [n + m for n, m in zip(new, prior)]
+    q, qf, pages, tables, starts = batch(rng, new, lens, Hq, Hkv, D, 64, sb, qt)
+    ref = OP.sdpa_int4_paged_chunks(qf, pages, tables, starts, lens, 64, Hq // Hkv, 0.4, window, sinks)
+    kw = dict(max_new=max(new), max_kv_len=max(lens))
+    got = run(pg, q, pages, tables, starts, lens, Hq // Hkv, 0.4, window, sinks, **kw)
+    close(got, ref)
+    run(pg, q, pages, tables, starts, lens, Hq // Hkv, 3.0)
+    assert np.array_equal(got, run(pg, q, pages, tables, starts, lens, Hq // Hkv, 0.4, window, sinks, **kw))
+
+
 @pytest.mark.parametrize("B", [63, 64, 65, 200])
 def test_more_sequences_than_a_wave(pg, B):
     rng = np.random.default_rng(B)
