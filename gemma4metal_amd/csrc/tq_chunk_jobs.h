@@ -11,7 +11,7 @@ struct TileParams : PagedParams {
   int splits;  // workgroups along the tiles (grid y); 1: write p.out
   // chunks of a batch (nq sequences): their queries are rows starts[b] .. starts[b + 1] - 1
   // of q and out, of `queries` in all.  Sequences of at most `few` rows (queries x heads of
-  // a kv head) are the business of paged_few_kernel, the others of paged_tiles_kernel.
+  // a kv head) are the business of few_job, the others of tiles_job.
   const int* starts;
   int queries, few;
   int max_new;  // queries of a sequence that are served
@@ -90,8 +90,8 @@ __device__ __forceinline__ int splits_of(const ChunkSeq& c, int T) {
   return c.tiles <= T ? 1 : min(static_cast<int>(ceilf(c.tiles * __builtin_amdgcn_rcpf(static_cast<float>(T)))), kMostSplits);
 }
 
-// f(sequence of this lane) for the sequences of the batch, 64
-// at a time; `first`: the first 64, loaded once.
+// f(sequence of this lane) for the sequences of the batch, 64 at a time; `first`: the
+// first 64, loaded once.
 template <int ROWS, int TK, bool FEW, typename F>
 __device__ __forceinline__ void each_seq(const TileParams& p, const ChunkSeq& first, F f) {
   f(first);

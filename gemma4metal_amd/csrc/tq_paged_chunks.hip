@@ -1,6 +1,7 @@
 // Chunks of new tokens of a batch's sequences over pages: the kernel for sequences of
 // few rows (queries x heads of a kv head), the merge of split jobs, and the plan.
-// Sequences of more rows run paged_tiles_kernel (tq_paged_tiles.hip).
+// Sequences of more rows run paged_tiles_kernel, or both kinds paged_mixed_kernel
+// (tq_paged_tiles.hip).
 #include "tq_paged_few.h"
 
 #include <climits>

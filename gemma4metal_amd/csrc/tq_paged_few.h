@@ -1,14 +1,14 @@
 // Chunks of a batch: a job of few rows (queries x heads of a kv head) over pages.
 //
-// Four waves take 16 rows of one kv head and split their keys,
-// where tiles staged for 64 or 128 rows would leave most of a workgroup idle: each wave
-// streams 32-key blocks of its own, with no barrier until the end.  The mathematics is
-// that of tq_paged_tiles.hip (centred fp16 nibbles; S^T = K q^T by quant group, P V as
-// fp16 high part and remainder), with one difference: the weights p s_v of every (row,
-// group) of a block go in under a power of two of their own and the products are added
-// to the sums in fp32, so that no range of V scales needs a path beside this one.
+// Four waves take 16 rows of one kv head and split their keys, where tiles staged for 64
+// or 128 rows would leave most of a workgroup idle: each wave streams 32-key blocks of its
+// own, with no barrier until the end.  The mathematics is that of tq_paged_tiles.hip
+// (centred fp16 nibbles; S^T = K q^T by quant group, P V as fp16 high part and remainder),
+// with one difference: the weights p s_v of a (row, group) go in times a power of two that
+// its sums carry too, and which falls where a weight would pass fp16, so that no range of
+// V scales needs a path beside this one.
 // What bounds it: VALU (about 700 instructions a wave and block at D 256, 61% of a SIMD's
-// cycles with two waves) and the start and end of a workgroup (about 9 us).  5 new tokens
+// cycles with two waves) and the start and end of a job (about 9 us).  5 new tokens
 // of 32 sequences behind a window of 1,024 (Hq 32 Hkv 16 D 256): 50 us, 3.0 TB/s of what
 // has to be read, where the tile kernel takes 121.  Measured, not kept: workgroups of eight
 // waves, one a CU, 69; V's operands read ahead of the softmax 60 (spills); nibbles as fp16
