@@ -257,6 +257,20 @@ def test_reorder_pages(pg, S, page, lo, hi):
             assert np.array_equal(counted(pool), pool.refs)
 
 
+@pytest.mark.parametrize("S,width", [(256, 16), (256, 17), (257, 3), (64, 64), (8, 512), (8, 513), (1, 4096), (1, 5000)])
+def test_reorder_pages_of_many_entries(pg, S, width):
+    """Few and many sequences and table entries, on both sides of where the plan takes
+    the roles too."""
+    rng = np.random.default_rng(S + width)
+    lens = rng.integers(1, 32 * min(width, 40), S).tolist()
+    pool = pool_of(rng, S, width, S * min(width, 40) + 2, 32, lens, 1, layers=1)
+    for _ in range(2):
+        parents = rng.integers(0, S, S)
+        parents[rng.random(S) < 0.1] = -1
+        run_reorder(pg, pool, parents)
+        assert np.array_equal(counted(pool), pool.refs)
+
+
 @pytest.mark.parametrize("parents", [[0, 1, 2, 3], [1, 0, 3, 2], [1, 2, 3, 0], [0, 0, 0, 0], [3, 3, 3, 3],
                                      [-1, -1, -1, -1], [2, 2, 9, -5], [1, 1, 0, 0]])
 def test_reorder_pages_maps(pg, parents):
