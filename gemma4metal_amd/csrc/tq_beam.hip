@@ -452,7 +452,8 @@ __device__ __forceinline__ int tiles_of(const ReorderParams& p, int a, int n) {
   return static_cast<int>((static_cast<int64_t>(n) * p.row_bytes[a] + 16 * kTileUnits - 1) / (16 * kTileUnits));
 }
 
-// Exclusive prefix over the workgroup's threads, and the total.
+// Exclusive prefix over the workgroup's N threads, and the total.
+template <int N>
 __device__ __forceinline__ int plan_scan(int v, int* lds, int& total) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   int x = v;
@@ -467,7 +468,7 @@ __device__ __forceinline__ int plan_scan(int v, int* lds, int& total) {
   int before = 0;
   total = 0;
 #pragma unroll
-  for (int w = 0; w < kMaxSeqs / 64; ++w) {
+  for (int w = 0; w < N / 64; ++w) {
     const int t = lds[w];
     before += w < wave ? t : 0;
     total += t;
@@ -475,10 +476,13 @@ __device__ __forceinline__ int plan_scan(int v, int* lds, int& total) {
   return before + x - v;
 }
 
-// One thread a sequence; lengths become the parents'.
-__global__ __launch_bounds__(kMaxSeqs) void kv_reorder_plan_kernel(ReorderParams p) {
-  __shared__ int label[kMaxSeqs], kids[kMaxSeqs], nf[kMaxSeqs], most[kMaxSeqs], at[kMaxSeqs], first[kMaxSeqs];
-  __shared__ int lds[kMaxSeqs / 64], changed;
+// One thread a sequence, of N at most; lengths become the parents'.  What bounds it: a
+// chain of loads, shared counts and scans; 4 sequences 3.9 us with a wave, 5.7 with sixteen,
+// 32 sequences 5.0 and 7.1.
+template <int N>
+__global__ __launch_bounds__(N) void kv_reorder_plan_kernel(ReorderParams p) {
+  __shared__ int label[N], kids[N], nf[N], most[N], at[N], first[N];
+  __shared__ int lds[N / 64], changed;
   const int s = threadIdx.x;
   const bool in = s < p.seqs;
   const int q = in ? parent_of(p.parents, s, p.seqs) : -1;
@@ -522,13 +526,13 @@ __global__ __launch_bounds__(kMaxSeqs) void kv_reorder_plan_kernel(ReorderParams
   __syncthreads();
   const bool comp = nf[s] > 0;  // of the component's lowest sequence
   int comps, parents, children, tiles;
-  const int c = plan_scan(comp, lds, comps);
-  const int from0 = plan_scan(nf[s], lds, parents);
-  const int to0 = plan_scan(gives ? kids[s] : 0, lds, children);
+  const int c = plan_scan<N>(comp, lds, comps);
+  const int from0 = plan_scan<N>(nf[s], lds, parents);
+  const int to0 = plan_scan<N>(gives ? kids[s] : 0, lds, children);
   int n = 0;
 #pragma unroll
   for (int a = 0; a < 6; ++a) n += comp ? tiles_of(p, a, most[s]) : 0;
-  const int tile0 = plan_scan(n * p.heads, lds, tiles);
+  const int tile0 = plan_scan<N>(n * p.heads, lds, tiles);
   first[s] = from0;
   if (comp) p.comps[c] = ReorderComp{from0, nf[s], most[s], tile0};
   if (s == 0) {
@@ -748,7 +752,8 @@ extern "C" int tq_kv_reorder_int4(uint32_t* k_quant, void* k_scales, void* k_bia
   p.from = reinterpret_cast<ReorderParent*>(p.comps + batch);
   p.to = reinterpret_cast<int*>(p.from + batch);
   hipStream_t s = static_cast<hipStream_t>(stream);
-  kv_reorder_plan_kernel<<<1, kMaxSeqs, 0, s>>>(p);
+  if (batch <= 64) kv_reorder_plan_kernel<64><<<1, 64, 0, s>>>(p);
+  else kv_reorder_plan_kernel<kMaxSeqs><<<1, kMaxSeqs, 0, s>>>(p);
   TQ_CHECK_LAUNCH("kv_reorder_plan_kernel");
   kv_reorder_kernel<<<static_cast<unsigned>(std::min<int64_t>(tiles, 8192)), 256, 0, s>>>(p);
   TQ_CHECK_LAUNCH("kv_reorder_kernel");

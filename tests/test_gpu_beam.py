@@ -356,6 +356,28 @@ def test_reorder_cache(gpu, B, Hkv, cap, D, sb):
             assert np.array_equal(host(a), b)
 
 
+@pytest.mark.parametrize("B", [63, 64, 65])
+def test_reorder_cache_of_a_waves_sequences(gpu, B):
+    """Both sizes of the plan: a ring of all sequences, one parent of all, and none."""
+    from gemma4metal_amd import turboquant as tq
+    rng = np.random.default_rng(B)
+    Hkv, cap, D = 1, 37, 64
+    lens = rng.integers(0, cap + 1, B).astype(np.int32)
+    x = [rng.integers(0, 2**32, (B, Hkv, cap, D // 8), dtype=np.uint32) if i % 3 == 0
+         else rng.standard_normal((B, Hkv, cap, D // 64)).astype(np.float16) for i in range(6)]
+    for parents in (np.roll(np.arange(B), 1), np.full(B, B - 1), np.full(B, -1), np.arange(B) // 2):
+        d, n = [dev(t) for t in x], dev(lens)
+        tq.kv_reorder_int4(*d, n, ints(parents))
+        par = np.where((parents >= 0) & (parents < B), parents, -1)
+        assert np.array_equal(host(n), np.where(par >= 0, lens[par], 0))
+        for t, got in zip(x, d):
+            want = t.copy()
+            for b in range(B):
+                if par[b] >= 0:
+                    want[b, :, :lens[par[b]]] = t[par[b], :, :lens[par[b]]]
+            assert np.array_equal(host(got), want)
+
+
 def test_reorder_cache_class_and_graph(gpu):
     rng = np.random.default_rng(1)
     c = gpu.Int4KVCache(4, 2, 40, 128, "cuda", ring=True)
