@@ -78,6 +78,10 @@ def beam_step(caches, logits: torch.Tensor, scores: torch.Tensor, *, finished: O
     the rows of its new beam, whose token comes next.  Returns beam_select's results."""
     out = beam_select(logits, scores, finished=finished, pad_token=pad_token)
     parents = out[1].flatten()
-    for cache in caches if isinstance(caches, (list, tuple)) else (caches,):
+    caches = caches if isinstance(caches, (list, tuple)) else (caches,)
+    for cache in caches:  # (before any of them is reordered)
+        _need(cache.lengths.shape == parents.shape and cache.lengths.device == parents.device,
+              "every cache must hold a sequence for each beam, on the logits' device")
+    for cache in caches:
         cache.reorder(parents)
     return out

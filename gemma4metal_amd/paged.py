@@ -625,6 +625,9 @@ class PagedInt4KVCache:
         """Attention of a chunk of new tokens of every sequence, whose rows are
         appended and not yet counted: queries (N, Hq, D), those of sequence s in rows
         starts[s] .. starts[s+1]-1 (:func:`sdpa_int4_paged_chunks`)."""
+        dev, ends = self.lengths.device, (self.lengths.shape[0] + 1,)
+        if not _ints_fine(starts, ends, dev.index):
+            _check_ints("starts", starts, ends, dev)
         return sdpa_int4_paged_chunks(queries, *self.layer(layer), self.block_tables, starts,
                                       self.lengths + starts[1:] - starts[:-1], gqa_factor, scale, sliding_window,
                                       num_sinks, max_new=max_new, max_kv_len=max_kv_len, out=out, workspace=workspace)

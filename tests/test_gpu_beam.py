@@ -488,3 +488,15 @@ def test_other_device_or_stream_arguments(bm, pg):
     for bad, word in ((dict(num_out=65), "num_out"), (dict(pad_token=8), "pad_token"), (dict(pad_token=-1), "pad_token")):
         with pytest.raises(TQError, match=word):
             bm.beam_select(x, sc, **bad)
+
+
+def test_a_step_is_refused_before_any_cache_moves(gpu, bm):
+    a, b = gpu.Int4KVCache(2, 1, 8, 128, "cuda"), gpu.Int4KVCache(3, 1, 8, 128, "cuda")
+    a.lengths.copy_(ints([5, 3]))
+    x = torch.zeros(1, 2, 8, device="cuda")
+    x[0, 1, 3] = 9.0
+    with pytest.raises(ValueError, match="every cache"):
+        bm.beam_step([a, b], x, torch.zeros(1, 2, device="cuda"))
+    assert host(a.lengths).tolist() == [5, 3]
+    parents = bm.beam_step((a,), x, torch.zeros(1, 2, device="cuda"))[1]
+    assert host(parents)[0, 0] == 1 and host(a.lengths)[0] == 3

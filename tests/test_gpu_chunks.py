@@ -295,3 +295,8 @@ def test_refusals(pg):
     with pytest.raises(ValueError, match="workspace"):
         wide = torch.full((2, 64), -1, dtype=torch.int32, device="cuda")
         ok(t=wide, st=big, workspace=torch.zeros(64, dtype=torch.uint8, device="cuda"))
+    c = pg.PagedInt4KVCache(4, 32, 2, 2, 2, 128, "cuda")
+    for bad in (ints([0, 3]), st.long(), st.cpu()):
+        with pytest.raises(ValueError, match="starts"):
+            c.attend_chunks(0, q, bad, 2)
+    assert not host(c.attend_chunks(0, q, ints([0, 0, 0]), 2, out=torch.zeros(3, 4, 128, device="cuda"))).any()
