@@ -475,6 +475,7 @@ __device__ __forceinline__ void few_job(const TileParams& p, int j, int tid, typ
           hw[q] = few_high(y[2 * q], y[2 * q + 1], ef[g]);
           lw[q] = few_low(hw[q], y[2 * q], y[2 * q + 1], ef[g]);
         }
+        pf_settle(hw, lw);
         const v8h bh = __builtin_bit_cast(v8h, hw), bl = __builtin_bit_cast(v8h, lw);
 #pragma unroll
         for (int x = 0; x < 4; ++x) {

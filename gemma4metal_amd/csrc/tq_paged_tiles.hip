@@ -689,6 +689,7 @@ __device__ __forceinline__ void tiles_job(const TileParams& p, TilesLds<D, F32>&
             hw[q] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(y[2 * q], y[2 * q + 1]));
             lw[q] = pf_rem_pair(hw[q], y[2 * q], y[2 * q + 1]);
           }
+          pf_settle(lw);
           bh = __builtin_bit_cast(v8h, hw);
           bl = __builtin_bit_cast(v8h, lw);
         };

@@ -326,6 +326,7 @@ __device__ __forceinline__ void prefill_rows(const SdpaParams& p) {
           hi[q] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(y[2 * q], y[2 * q + 1]));
           lw[q] = pf_rem_pair(hi[q], y[2 * q], y[2 * q + 1]);
         }
+        pf_settle(lw);
         bh = __builtin_bit_cast(v8h, hi);
         bl = __builtin_bit_cast(v8h, lw);
       };

@@ -141,6 +141,9 @@ __device__ __forceinline__ void pf_split_q(const float* q, float scale, v8h& qh,
     h[i] = __builtin_bit_cast(uint32_t, v2h{static_cast<_Float16>(x[2 * i]), static_cast<_Float16>(x[2 * i + 1])});
     l[i] = pf_rem_pair(h[i], x[2 * i], x[2 * i + 1]);
   }
+  // a matrix operand two wait states behind its writing, which the compiler sees to
+  // only where that is no inline assembly
+  asm("s_nop 1" : "+v"(l));
   qh = __builtin_bit_cast(v8h, h);
   ql = __builtin_bit_cast(v8h, l);
 }

@@ -191,5 +191,13 @@ __device__ __forceinline__ uint32_t pf_rem_pair(uint32_t hp, float x0, float x1)
   return r;
 }
 
+// Operands of matrix instructions that inline assembly has written go through this.  A
+// matrix instruction may read what a vector instruction writes two wait states later at
+// the earliest; the compiler sees to that for its own instructions and does not look into
+// assembly.  (With one state less a kernel of D 512 multiplied V by what half of a
+// register had held before.)
+__device__ __forceinline__ void pf_settle(u32x4& a) { asm("s_nop 1" : "+v"(a)); }
+__device__ __forceinline__ void pf_settle(u32x4& a, u32x4& b) { asm("s_nop 1" : "+v"(a), "+v"(b)); }
+
 }  // namespace
 }  // namespace tq
