@@ -5,8 +5,12 @@
 // own, with no barrier until the end.  The mathematics is that of tq_paged_tiles.hip
 // (centred fp16 nibbles; S^T = K q^T by quant group, P V as fp16 high part and remainder),
 // with one difference: the weights p s_v of a (row, group) go in times a power of two that
-// its sums carry too, and which falls where a weight would pass fp16, so that no range of
-// V scales needs a path beside this one.
+// its sums carry too.  It falls where a weight would pass fp16 and rises where a row with a
+// p of about 1 (its largest is that or more) has no weight of 1 or more, so that no range of
+// V scales needs a path beside this one: fp16's last step is 2^-24, and what is rounded off a
+// weight is 2^-25 of the row's sums at most.  Both in branches that equal scales hardly take
+// (with the rise's part inside the other's: 49.4 -> 50.2 us of the 5 tokens below; a rise
+// with every new reference 54).
 // What bounds it: VALU (about 700 instructions a wave and block at D 256, 61% of a SIMD's
 // cycles with two waves) and the start and end of a job (about 9 us).  5 new tokens
 // of 32 sequences behind a window of 1,024 (Hq 32 Hkv 16 D 256): 50 us, 3.0 TB/s of what
@@ -433,6 +437,10 @@ __device__ __forceinline__ void few_job(const TileParams& p, int j, int tid, typ
     }
 
     // ---- O^T += V^T P^T -----------------------------------------------------------------
+    float pm = pw[0];
+#pragma unroll
+    for (int j = 1; j < 8; ++j) pm = fmaxf(pm, pw[j]);
+    const uint64_t heavy = __ballot(pm >= 0.5f);
 #pragma unroll
     for (int b = 0; b < NG / G4; ++b) {
       v_rows(b);
@@ -459,15 +467,30 @@ __device__ __forceinline__ void few_job(const TileParams& p, int j, int tid, typ
           bs[g] = fmaf(pw[j], fmaf(s, 8.0f, static_cast<float>(vb[j][gi])), bs[g]);
           big = fmaxf(big, fabsf(y[j]));
         }
-        if (__any(big * ef[g] > 0x1p15f)) {
+        const float in = big * ef[g];
+        const uint64_t under = __ballot(in < 1.0f) & heavy;
+        if ((__ballot(in > 0x1p15f) | under) != 0) {
           // the row's largest to 2^13 .. 2^14 (an infinity, of exponent 0, stays one)
           const float top = xor32_max(xor16_max(big));
-          const float now = ldexpf(1.0f, min(14 - __builtin_amdgcn_frexp_expf(top), 120));
-          const bool down = top * ef[g] > 0x1p15f && now < ef[g];
-          const float fr = down ? ldexpf(now, 1 - __builtin_amdgcn_frexp_expf(ef[g])) : 1.0f;  // (may be 0: nothing is left)
-          ef[g] = down ? now : ef[g];
+          const float row = top * ef[g];
+          const int want = min(14 - __builtin_amdgcn_frexp_expf(top), 120) + 1 - __builtin_amdgcn_frexp_expf(ef[g]);
+          int by = row > 0x1p15f ? min(want, 0) : 0;
+          if (under != 0) {
+            // up as far as the sums stay below 2^100 (weights that much smaller are nothing)
+            float most = 0.0f;
 #pragma unroll
-          for (int x = 0; x < 4; ++x) o[4 * g + x] *= fr;
+            for (int x = 0; x < 4; ++x)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) most = fmaxf(most, fabsf(o[4 * g + x][e]));
+            most = xor32_max(xor16_max(most));
+            const int room = most > 0.0f ? 100 - __builtin_amdgcn_frexp_expf(most) : want;
+            if (top > 0.0f && row < 1.0f) by = max(min(want, room), 0);
+          }
+          ef[g] = ldexpf(ef[g], by);
+#pragma unroll
+          for (int x = 0; x < 4; ++x)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[4 * g + x][e] = ldexpf(o[4 * g + x][e], by);
         }
         u32x4 hw, lw;
 #pragma unroll

@@ -33,3 +33,52 @@ def test_every_form(pg, Hq, Hkv, new, lens, D, sb, qt):
         ref = definition(qf[mine], pages, tables[b], range(L - new[b] + 1, L + 1), 32, Hq // Hkv, D**-0.5)
         for g in range(0, D, 64):
             within(got[mine], ref, TILES, f"sequence {b}, dims from {g}", slice(g, g + 64))
+
+
+LOG2E = 1.4426950408889634
+
+# (score in powers of two below the last keys', factor of the V scales and biases) of 128
+# keys each, so that a wave that takes every fourth block of 32 meets all of them
+FADES = {
+    "f16": [[(-60, 1e4), (0, 1e-3)], [(-60, 1e4), (0, 1e-4)], [(-60, 1e4), (-40, 10.0), (-20, 1e-2), (0, 1e-4)],
+            [(-60, 1e-4), (0, 1e4)]],
+    "f32": [[(-60, 1e10), (0, 0.1)], [(-120, 1e25), (-80, 1e10), (0, 1e-5)], [(-110, 1e-20), (-90, 1e10), (0, 1e-10)],
+            [(-60, 1e3), (-30, 1.0), (0, 1e-3)], [(-126, 1e20), (0, 1e-30)],
+            [(-160, 1e20), (0, 1e-20)]],
+}
+
+
+@pytest.mark.parametrize("sb,qt,fade", [(sb, qt, i) for sb, qt in (("f16", "bf16"), ("f16", "f32"), ("f32", "f32"), ("f32", "f16"))
+                                        for i in range(len(FADES[sb]))])
+@pytest.mark.parametrize("D,new", [(128, 3), (128, 60), (128, 100), (256, 3), (256, 40), (512, 3), (512, 30)])
+def test_keys_that_fade_leave_no_rounding(pg, D, new, sb, qt, fade):
+    """What a row adds up is rounded against what is left of its sums, not against what
+    they held before a larger score came.  What the first keys leave is at most 1e-4 of the
+    result, so that their scores' rounding is no part of the error -- but in the case of 126,
+    whose result they are as far as fp32 holds their weights (2^-126 and more: rows that are
+    120 below at most): 2^-24 of 126 in each of four roundings (the sum, the factor, the
+    product with it less the reference, fp32 queries), ln 2 of that in every weight."""
+    rng = np.random.default_rng(D + new + fade)
+    Hq, Hkv, page, lens = 4, 2, 32, [500]
+    q, qf, pages, tables, starts = batch(rng, [new], lens, Hq, Hkv, D, page, sb, qt)
+    q, qf = q.abs(), np.abs(qf)
+    steps, scale = FADES[sb][fade], 1 / 128
+    sums = qf.sum(-1)
+    for t in range(lens[0]):
+        e, r = tables[0, t // page], t % page
+        far, factor = steps[min(t // 128, len(steps) - 1)]
+        # (q . k) scale = far ln 2, but for the last keys' own spread
+        if far:
+            pages[1][e, :, r] = 0
+            pages[2][e, :, r] = far / LOG2E / (scale * sums.mean())
+        for i in (4, 5):
+            pages[i][e, :, r] *= pages[i].dtype.type(factor)
+    assert all(np.isfinite(p[tables[0, 0]].astype(np.float64)).all() for p in pages[1:3] + pages[4:])
+    got = run(pg, q, pages, tables, starts, lens, Hq // Hkv, scale)
+    ref = definition(qf, pages, tables[0], range(lens[0] - new + 1, lens[0] + 1), page, Hq // Hkv, scale)
+    tol, rows = TILES, np.ones(sums.shape, bool)
+    if steps[0][0] == -126:
+        tol, rows = TILES + 4 * 126 * 2.0**-24 / LOG2E, 126 * sums / sums.mean() <= 120
+    assert np.isfinite(got).all()
+    if rows.any():
+        within(got[rows], [ref[0][rows], ref[1][rows]], tol, f"{steps}")
