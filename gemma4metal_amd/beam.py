@@ -71,17 +71,40 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, num_out: Optional[in
     return out
 
 
+def _check_caches(caches, sequences: int, device) -> dict:
+    """What a step needs of its caches, before any of them moves.  Returns the number
+    of the last cache with each lengths tensor."""
+    last, held = {}, {}
+    for i, cache in enumerate(caches):
+        n = cache.lengths
+        _need(n.shape == (sequences,) and n.device == device and n.dtype is torch.int32 and n.is_contiguous(),
+              "every cache must hold a sequence for each beam, on the logits' device, in contiguous int32 lengths")
+        paged = hasattr(cache, "block_tables")
+        for t in (cache.tensors()[0], cache.block_tables) if paged else cache.tensors()[:1]:
+            _need(t.data_ptr() not in held, "a cache (its rows, or its block_tables) is given twice")
+            held[t.data_ptr()] = True
+        at = n.data_ptr()
+        for other, j in last.items():
+            _need(abs(other - at) >= 4 * sequences
+                  or other == at and not paged and not hasattr(caches[j], "block_tables"),
+                  "lengths may be shared by Int4KVCaches only, and whole")
+        last[at] = i
+    return last
+
+
 def beam_step(caches, logits: torch.Tensor, scores: torch.Tensor, *, finished: Optional[torch.Tensor] = None,
               pad_token: int = 0):
     """:func:`beam_select` of as many beams, and ``reorder`` of the cache (or each of a
     list of caches), whose sequences are the B * W beams: sequence b * W + w then holds
-    the rows of its new beam, whose token comes next.  Returns beam_select's results."""
+    the rows of its new beam, whose token comes next.  Int4KVCaches may share one
+    ``lengths`` tensor.  Returns beam_select's results."""
+    caches = caches if isinstance(caches, (list, tuple)) else (caches,)
     out = beam_select(logits, scores, finished=finished, pad_token=pad_token)
     parents = out[1].flatten()
-    caches = caches if isinstance(caches, (list, tuple)) else (caches,)
-    for cache in caches:  # (before any of them is reordered)
-        _need(cache.lengths.shape == parents.shape and cache.lengths.device == parents.device,
-              "every cache must hold a sequence for each beam, on the logits' device")
-    for cache in caches:
-        cache.reorder(parents)
+    last = _check_caches(caches, parents.shape[0], parents.device)
+    for i, cache in enumerate(caches):
+        if last[cache.lengths.data_ptr()] == i:
+            cache.reorder(parents)
+        else:
+            cache.reorder(parents, set_lengths=False)
     return out

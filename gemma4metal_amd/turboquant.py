@@ -367,10 +367,11 @@ class Int4KVCache:
                                 stream=stream)
 
 
-    def reorder(self, parents: torch.Tensor, *, stream=None) -> None:
+    def reorder(self, parents: torch.Tensor, *, set_lengths: bool = True, stream=None) -> None:
         """Makes every sequence the continuation of sequence parents[b] (int32
-        (B,)) as it was: the step of a beam search."""
-        kv_reorder_int4(*self.tensors(), self.lengths, parents, stream=stream)
+        (B,)) as it was: the step of a beam search.  Of caches that share one
+        ``lengths`` tensor only the last to be reordered sets it."""
+        kv_reorder_int4(*self.tensors(), self.lengths, parents, set_lengths=set_lengths, stream=stream)
 
 
 @functools.lru_cache(maxsize=64)
@@ -423,12 +424,16 @@ def _check_reorder(*tensors) -> None:
 
 def kv_reorder_int4(k_quant: torch.Tensor, k_scales: torch.Tensor, k_biases: torch.Tensor,
                     v_quant: torch.Tensor, v_scales: torch.Tensor, v_biases: torch.Tensor,
-                    lengths: torch.Tensor, parents: torch.Tensor, *, workspace: Optional[torch.Tensor] = None,
-                    stream=None) -> None:
+                    lengths: torch.Tensor, parents: torch.Tensor, *, set_lengths: bool = True,
+                    workspace: Optional[torch.Tensor] = None, stream=None) -> None:
     """Reorders (B, Hkv, cap, .) caches (linear or ring) in place, all sequences at
     once: the rows of sequence b become those of sequence parents[b] as they were,
     lengths[b] its length.  Rows behind the length stay as they were.  A parent
-    outside [0, B) leaves a length of 0."""
+    outside [0, B) leaves a length of 0.
+
+    The lengths are those before the step.  Layers that share them are reordered with
+    ``set_lengths=False``, all but the last: lengths that are set already would be
+    taken for those of other rows."""
     tensors = (k_quant, k_scales, k_biases, v_quant, v_scales, v_biases)
     if not _reorder_fine(*tensors, lengths, parents):
         _check_reorder(*tensors, lengths, parents)
@@ -441,7 +446,8 @@ def kv_reorder_int4(k_quant: torch.Tensor, k_scales: torch.Tensor, k_biases: tor
 
     def run():
         ws = torch.empty(nbytes, dtype=torch.uint8, device=k_quant.device) if workspace is None else workspace
-        call("tq_kv_reorder_int4", *[t.data_ptr() for t in tensors], sbt, B, Hkv, 8 * W, cap, lengths.data_ptr(),
+        n = lengths if set_lengths else lengths.clone()
+        call("tq_kv_reorder_int4", *[t.data_ptr() for t in tensors], sbt, B, Hkv, 8 * W, cap, n.data_ptr(),
              parents.data_ptr(), ws.data_ptr(), nbytes, _stream(None))
 
     if stream is None and k_quant.device.index == torch.cuda.current_device():

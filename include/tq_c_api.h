@@ -484,7 +484,8 @@ int tq_beam_select(const void* logits, tq_dtype x_dtype, int64_t group_stride, i
  * in place, all sequences at once: the rows of sequence b become those of sequence
  * parents[b] as they were, and lengths[b] its length (DEVICE int32 [batch] both).  Rows
  * behind min(length, kv_capacity) stay as they were.  parents[b] outside [0, batch):
- * lengths[b] = 0.  batch <= 1024.
+ * lengths[b] = 0.  batch <= 1024.  A call reads the lengths before the step and replaces
+ * them: layers that share one array each need a copy of it, made before the first call.
  * workspace: tq_kv_reorder_int4_workspace_size(...) bytes, 16-byte aligned; need not be
  * zeroed; calls that may overlap need one each. */
 size_t tq_kv_reorder_int4_workspace_size(int batch);

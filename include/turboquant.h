@@ -224,7 +224,8 @@ struct beams {
 beams beam_select(const array& logits, const array& scores, int num_out = 0,
                   const array& finished = {}, int pad_token = 0, StreamOrDevice s = {});
 // Rows and lengths of sequence b of (B, Hkv, capacity, .) caches become those of
-// parents[b] as they were, in place; lengths, parents int32 (B).
+// parents[b] as they were, in place; lengths, parents int32 (B).  The lengths are replaced:
+// layers that share them each need a copy, made before the first call.
 void kv_reorder_int4(array& k_quant, array& k_scales, array& k_biases, array& v_quant,
                      array& v_scales, array& v_biases, array& lengths, const array& parents,
                      StreamOrDevice s = {});
