@@ -97,14 +97,15 @@ def beam_step(caches, logits: torch.Tensor, scores: torch.Tensor, *, finished: O
     """:func:`beam_select` of as many beams, and ``reorder`` of the cache (or each of a
     list of caches), whose sequences are the B * W beams: sequence b * W + w then holds
     the rows of its new beam, whose token comes next.  Int4KVCaches may share one
-    ``lengths`` tensor.  Returns beam_select's results."""
+    ``lengths`` tensor.  Returns beam_select's results; a beam for which a paged cache had
+    no page has ended and has a score of -inf."""
     caches = caches if isinstance(caches, (list, tuple)) else (caches,)
     out = beam_select(logits, scores, finished=finished, pad_token=pad_token)
     parents = out[1].flatten()
     last = _check_caches(caches, parents.shape[0], parents.device)
     for i, cache in enumerate(caches):
-        if last[cache.lengths.data_ptr()] == i:
-            cache.reorder(parents)
+        if hasattr(cache, "block_tables"):
+            out[0].masked_fill_(cache.reorder(parents).view(out[0].shape) == 0, float("-inf"))
         else:
-            cache.reorder(parents, set_lengths=False)
+            cache.reorder(parents, set_lengths=last[cache.lengths.data_ptr()] == i)
     return out

@@ -125,3 +125,27 @@ def test_caches_that_a_step_cannot_move(gpu, bm, pg):
     r.block_tables = p.block_tables
     with pytest.raises(ValueError, match="tables|twice"):
         bm.beam_step([p, r], x, scores)
+
+
+def test_a_beam_without_a_page_has_no_score(gpu, bm, pg):
+    """A request's first step in a full pool: one beam goes on, the other finds no page
+    for its copy of the last one.  It is no beam of the next step either."""
+    rng = np.random.default_rng(9)
+    c = pg.PagedInt4KVCache(2, 32, 2, 2, 1, 64, "cuda")
+    other = gpu.Int4KVCache(2, 1, 64, 64, "cuda")
+    n = ints([40, 0])
+    assert host(c.reserve(n)).tolist() == [1, 0]
+    k = torch.from_numpy(rng.standard_normal((2, 1, 40, 64)).astype(np.float32)).cuda()
+    c.append(0, k, k)
+    c.advance(n)
+    other.append(k, k, advance=False)
+    other.lengths.copy_(c.lengths)
+    x, scores = choice([0, 0])
+    for caches in ([c, other], [c]):
+        got = bm.beam_step(caches, x, scores)
+        assert host(got[1]).tolist() == [[0, 0]]
+        assert host(c.lengths).tolist() == [40, 0]
+        s = host(got[0])
+        assert np.isfinite(s[0, 0]) and s[0, 1] == -np.inf
+    x, _ = choice([0, 1])
+    assert host(bm.beam_step(c, x, got[0])[1]).tolist() == [[0, 0]]  # both of the one that is left
