@@ -20,7 +20,7 @@ import torch
 
 from . import _lib
 from ._lib import call
-from .paged import _placed, _workspace
+from .paged import _fits_int, _placed, _workspace
 from .turboquant import _DT, _need, _ptr, _stream
 
 
@@ -59,14 +59,15 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, num_out: Optional[in
                                      and finished.shape == (B, W) and finished.device == dev
                                      and finished.is_contiguous()):
         raise ValueError(f"finished must be contiguous bool or uint8 ({B}, {W}) on {dev}")
-    K = W if num_out is None else int(num_out)
+    K, pad = W if num_out is None else int(num_out), int(pad_token)
     _need(K >= 1, "num_out must be at least 1")
+    _fits_int(num_out=K, pad_token=pad)
     out = (torch.empty((B, K), dtype=torch.float32, device=dev), torch.empty((B, K), dtype=torch.int32, device=dev),
            torch.empty((B, K), dtype=torch.int32, device=dev))
     nbytes = _select_ws_size(B, W, V)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if workspace is None else _workspace(workspace, nbytes, dev, 0)
     call("tq_beam_select", logits.data_ptr(), _DT[logits.dtype], logits.stride(0), logits.stride(1), scores.data_ptr(),
-         _ptr(finished), B, W, V, K, int(pad_token), *[t.data_ptr() for t in out], ws.data_ptr(), ws.numel(),
+         _ptr(finished), B, W, V, K, pad, *[t.data_ptr() for t in out], ws.data_ptr(), ws.numel(),
          _stream(None))
     return out
 

@@ -44,6 +44,12 @@ def _need(cond: bool, msg: str):
         raise ValueError(msg)
 
 
+def _fits_int(**numbers):
+    """Refuses what a C int would cut off to another number."""
+    if max(numbers.values()) >= 2**31 or min(numbers.values()) < -2**31:
+        raise ValueError(f"{', '.join(n for n, v in numbers.items() if not -2**31 <= v < 2**31)}: more than 32 bits")
+
+
 def _workspace(ws: Optional[torch.Tensor], nbytes: int, device: torch.device, stream: int) -> torch.Tensor:
     if ws is None:
         ws = _cached_workspace(nbytes, device, stream)
@@ -347,6 +353,8 @@ def sdpa_int4_paged_chunks(queries: torch.Tensor,
         _check_ints("seq_lens", seq_lens, (B,), dev)
     mx = P * page if max_kv_len is None else int(max_kv_len)
     new = N if max_new is None else int(max_new)
+    gqa, window, sinks = int(gqa_factor), int(sliding_window), int(num_sinks)
+    _fits_int(max_new=new, max_kv_len=mx, gqa_factor=gqa, sliding_window=window, num_sinks=sinks)
     if out is None:
         out = torch.empty((N, Hq, D), dtype=torch.float32, device=dev)
     else:
@@ -356,8 +364,7 @@ def sdpa_int4_paged_chunks(queries: torch.Tensor,
     ws = _workspace(workspace, nbytes, dev, sh) if nbytes else None
     call("tq_sdpa_int4_paged_chunks", queries.data_ptr(), _DT[queries.dtype], *[t.data_ptr() for t in pages],
          _DT[k_scales.dtype], out.data_ptr(), B, N, Hq, Hkv, D, page, num, block_tables.data_ptr(), P,
-         starts.data_ptr(), seq_lens.data_ptr(), new, mx, int(gqa_factor), float(scale), int(sliding_window),
-         int(num_sinks), _ptr(ws), nbytes, sh)
+         starts.data_ptr(), seq_lens.data_ptr(), new, mx, gqa, float(scale), window, sinks, _ptr(ws), nbytes, sh)
     return out
 
 

@@ -149,3 +149,20 @@ def test_a_beam_without_a_page_has_no_score(gpu, bm, pg):
         assert np.isfinite(s[0, 0]) and s[0, 1] == -np.inf
     x, _ = choice([0, 1])
     assert host(bm.beam_step(c, x, got[0])[1]).tolist() == [[0, 0]]  # both of the one that is left
+
+
+def test_numbers_past_32_bits(bm, pg):
+    """They are refused, not cut off to others."""
+    x, scores = choice([0, 1])
+    for name in ("pad_token", "num_out"):
+        with pytest.raises(ValueError, match=name):
+            bm.beam_select(x, scores, **{name: 2**32 + 1})
+    pages = [torch.zeros((2, 1, 32, n), dtype=t, device="cuda") for n, t in
+             ((16, torch.uint32), (2, torch.float16), (2, torch.float16)) * 2]
+    q = torch.zeros((2, 1, 128), device="cuda")
+    t, st, n = ints([[0], [1]]), ints([0, 1, 2]), ints([5, 7])
+    ok = dict(gqa_factor=1, sliding_window=0, num_sinks=0, max_new=1, max_kv_len=32)
+    pg.sdpa_int4_paged_chunks(q, *pages, t, st, n, **ok)
+    for name, value in ok.items():
+        with pytest.raises(ValueError, match=name):
+            pg.sdpa_int4_paged_chunks(q, *pages, t, st, n, **(ok | {name: 2**32 + value}))
