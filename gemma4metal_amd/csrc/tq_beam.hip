@@ -695,7 +695,8 @@ extern "C" int tq_beam_select(const void* logits, tq_dtype x_dtype, int64_t grou
   }
   TQ_CHECK_ARG(reinterpret_cast<uintptr_t>(workspace) % 16 == 0, "%s: workspace must be 16-byte aligned", fn);
   const int nseg = segments(vocab);
-  TQ_CHECK_ARG(static_cast<int64_t>(groups) * beams * nseg < (int64_t{1} << 31), "%s: logits too large", fn);
+  // (a launch has fewer than 2^32 threads)
+  TQ_CHECK_ARG(static_cast<int64_t>(groups) * beams * sums(vocab) < (int64_t{1} << 32) / (64 * kScanWaves), "%s: logits too large", fn);
   float2* sum = static_cast<float2*>(workspace);
   SelectParams p{logits, group_stride, beam_stride, scores, finished, groups, beams, vocab, num_out, pad_token, nseg,
                  sums(vocab), sum, reinterpret_cast<float*>(sum + static_cast<size_t>(groups) * beams * sums(vocab)),

@@ -18,6 +18,8 @@ struct TileParams : PagedParams {
   int slots;    // of the workspace; 0: no splits
 };
 
+constexpr int kTileThreads = 512;  // of paged_tiles_kernel and paged_mixed_kernel
+
 // few_jobs > 0: both kernels' jobs in one launch (D < 512).
 int launch_chunk_tiles(const TileParams& p, int D, int sb_dtype, int rs, int64_t jobs, const TileParams& few,
                        int64_t few_jobs, hipStream_t s);

@@ -400,7 +400,7 @@ extern "C" int tq_sdpa_int4_paged_chunks(const void* q, tq_dtype q_dtype, const 
   p.n_clamp = max_kv_len;
   const ChunksPlan plan = plan_chunks(batch, queries, gqa_factor, num_kv_heads, head_dim, max_new, max_kv_len,
                                       sliding_window, num_sinks, q_dtype == TQ_F32 && sb_dtype == TQ_F32);
-  TQ_CHECK_ARG(plan.tiles.jobs < (int64_t{1} << 29) && plan.few_rows.jobs < (int64_t{1} << 29), "%s: grid too large", fn);
+  TQ_CHECK_ARG(chunk_threads(plan, head_dim) < (int64_t{1} << 32), "%s: grid too large", fn);
   PagedParams few = p;
   if (plan.tiles.slots + plan.few_rows.slots > 0) {
     const ChunksLayout wl = chunks_layout(plan, head_dim);

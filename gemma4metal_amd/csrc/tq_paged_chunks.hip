@@ -157,6 +157,12 @@ ChunksPlan plan_chunks(int batch, int queries, int gqa, int Hkv, int D, int max_
   return pl;
 }
 
+int64_t chunk_threads(const ChunksPlan& plan, int D) {
+  constexpr int64_t kTiles = kTileThreads, kFew = FewGeom<128, false>::NT;
+  const bool one = D < 512 && plan.tiles.jobs > 0;  // (launch_chunks)
+  return one ? kTiles * plan.tiles.jobs + kFew * (plan.few_rows.jobs + 1) : std::max(kTiles * plan.tiles.jobs, kFew * plan.few_rows.jobs);
+}
+
 int launch_chunks(const PagedParams& p0, const PagedParams& few0, int D, int sb_dtype, const ChunksPlan& plan,
                   const int* starts, int queries, int max_new, hipStream_t s) {
   TileParams p{}, few{};

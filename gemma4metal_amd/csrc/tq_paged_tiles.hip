@@ -24,6 +24,7 @@ namespace tq {
 namespace {
 
 constexpr int kRs = 4;  // 16-row sets of a tile's geometry (PfGeom): 8 waves
+static_assert(128 * kRs == kTileThreads, "launches");
 
 // Pool rows at which the 32-row parts of a run of tiles begin: part h of the run's
 // tile i in lane KH i + h, and whether its page exists in that bit of has.

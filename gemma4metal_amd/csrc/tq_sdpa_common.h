@@ -901,6 +901,8 @@ struct ChunksPlan {
 };
 ChunksPlan plan_chunks(int batch, int queries, int gqa, int Hkv, int D, int max_new, int64_t max_kv_len, int64_t window,
                        int64_t sinks, bool all32);
+// Threads of its largest launch (one has fewer than 2^32).
+int64_t chunk_threads(const ChunksPlan& plan, int D);
 int launch_chunks(const PagedParams& p, const PagedParams& few, int D, int sb_dtype, const ChunksPlan& plan,
                   const int* starts, int queries, int max_new, hipStream_t stream);
 // Merge of the split partials of a launch with ext_merge = 1 (batch b of
