@@ -37,7 +37,7 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, num_out: Optional[in
     but the last's, which is 1; scores (B, W) f32, the beams' sums of log-probabilities
     so far.  Of a group's totals ``scores[w] + log_softmax(logits[w])[t]`` the
     ``num_out`` (W by default) largest, the lowest (w, t) first among equals; totals of
-    two beams that differ by less than about 1e-7 may change places.
+    two beams that differ by less than 7.2e-7 may change places (6e-8 as a rule).
     A beam with finished[b, w] (bool or uint8) has one candidate: itself, with
     ``pad_token``.  A score of -inf or NaN gives its beam none (the first step of a
     request: all beams but one), nor does a logit of -inf or NaN.

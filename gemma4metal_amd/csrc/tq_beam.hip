@@ -25,6 +25,17 @@ constexpr int kSeg = 1024;
 constexpr int kScanWaves = 4;  // segments of a workgroup
 constexpr int kMaxBeams = 64;
 
+// Of kScanWaves segments: their largest logit, and their exponentials as sum exp(ref).
+struct ScanSum {
+  float most, ref;
+  double sum;
+};
+
+// v's exponentials less a logit m, which none of the row's is above.
+__device__ __forceinline__ double exp_from(const ScanSum& v, float m) {
+  return v.sum == 0.0 ? 0.0 : v.sum * (v.ref == m ? 1.0 : exp(static_cast<double>(v.ref) - static_cast<double>(m)));
+}
+
 struct SelectParams {
   const void* x;
   int64_t group_stride, beam_stride;  // elements
@@ -32,7 +43,7 @@ struct SelectParams {
   const uint8_t* finished;
   int groups, beams, vocab, num_out, pad;
   int nseg, nsum;  // segments of a row, and sums
-  float2* sum;     // [groups * beams][nsum]: largest, sum of exp(x - largest)
+  ScanSum* sum;    // [groups * beams][nsum]
   float* seg;      // [groups * beams][nseg]: largest
   float* scores_out;
   int32_t* parents_out;
@@ -52,17 +63,65 @@ __device__ __forceinline__ float to_f32<uint16_t>(uint16_t v) { return bf16_to_f
 // whether it is finished: one candidate, the beam itself.
 __device__ __forceinline__ bool beam_alive(float score) { return score > -INFINITY; }
 
-// log2(e) in two parts: the product's constant error would be the same in every term.
+// log2(e) in two parts, 2^-49 of it apart.
 constexpr float kLog2eHi = 1.4426950216293335f, kLog2eLo = 1.925963033500011e-8f;
+
+template <int CTRL>
+__device__ __forceinline__ double dpp_add(double v) {
+  const uint64_t u = static_cast<uint64_t>(__double_as_longlong(v));
+  const uint32_t lo = __builtin_amdgcn_update_dpp(0, static_cast<int>(u), CTRL, 0xF, 0xF, false);
+  const uint32_t hi = __builtin_amdgcn_update_dpp(0, static_cast<int>(u >> 32), CTRL, 0xF, 0xF, false);
+  return v + __longlong_as_double(static_cast<int64_t>(static_cast<uint64_t>(hi) << 32 | lo));
+}
+// group_sum<64> in 64 bits.
+__device__ __forceinline__ double sum_of_wave(double v) {
+  v = dpp_add<0xB1>(v);
+  v = dpp_add<0x4E>(v);
+  v = dpp_add<0x141>(v);
+  v = dpp_add<0x140>(v);
+  const auto pair = [](uint32_t hi, uint32_t lo) { return __longlong_as_double(static_cast<int64_t>(static_cast<uint64_t>(hi) << 32 | lo)); };
+  uint64_t u = static_cast<uint64_t>(__double_as_longlong(v));
+  const auto l16 = __builtin_amdgcn_permlane16_swap(static_cast<uint32_t>(u), static_cast<uint32_t>(u), false, false);
+  const auto h16 = __builtin_amdgcn_permlane16_swap(static_cast<uint32_t>(u >> 32), static_cast<uint32_t>(u >> 32), false, false);
+  v = pair(h16[0], l16[0]) + pair(h16[1], l16[1]);
+  u = static_cast<uint64_t>(__double_as_longlong(v));
+  const auto l32 = __builtin_amdgcn_permlane32_swap(static_cast<uint32_t>(u), static_cast<uint32_t>(u), false, false);
+  const auto h32 = __builtin_amdgcn_permlane32_swap(static_cast<uint32_t>(u >> 32), static_cast<uint32_t>(u >> 32), false, false);
+  return pair(h32[0], l32[0]) + pair(h32[1], l32[1]);
+}
+
+// The sum of N exponentials: exp x = 2^a (1 + r ln 2), a = x log2 e rounded, r what is left of
+// it, which two fmas find; the corrections are summed by themselves.  (With a alone all equal
+// logits err alike, by 2^-21 or 2^-20: sums were off by up to 0.9e-6.)  Terms are added in
+// pairs, so that equal ones add up exactly.  Off by 2^-23 (the power, an ulp) + 4 2^-24 =
+// 3.6e-7 of itself at most.
+template <int N>
+__device__ __forceinline__ double sum_of_exps(const float (&x)[N]) {
+  float e[N], c = 0.0f;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const float a = x[i] * kLog2eHi, r = fmaf(x[i], kLog2eLo, fmaf(x[i], kLog2eHi, -a));
+    e[i] = fast_exp2(a);
+    c = fmaf(e[i], r, c);
+  }
+#pragma unroll
+  for (int d = 1; d < N; d *= 2)
+#pragma unroll
+    for (int i = 0; i < N; i += 2 * d) e[i] += e[i + d];
+  return fma(static_cast<double>(c), 0.69314718055994531, static_cast<double>(e[0]));
+}
 
 // A wave a segment (behind the row's end: an empty one).  16-byte loads at the alignment
 // of an element: what a lane sums goes by the place in the row alone, so that equal rows
-// give equal sums.  What bounds it: HBM (248 rows of 262,144 bf16 tokens 28 us, 4.6 TB/s,
-// where a large copy reaches 5.1; VALU 75%).
+// give equal sums.  Logits of ordinary size are taken as they are (ref 0), so that segments
+// add up without a common reference.  More than a lane's 16 terms are added in 64 bits.
+//
+// What bounds it: HBM (248 rows of 262,144 bf16 tokens 28 us, 4.6 TB/s, where a large copy
+// reaches 5.1; VALU 75%).
 template <typename T>
 __global__ __launch_bounds__(64 * kScanWaves) void beam_scan_kernel(SelectParams p) {
   constexpr int E = 16 / sizeof(T), NV = kSeg / (64 * E);
-  __shared__ float2 part[kScanWaves];
+  __shared__ ScanSum part[kScanWaves];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int row = static_cast<int>(blockIdx.x / static_cast<uint32_t>(p.nsum));
   const int js = static_cast<int>(blockIdx.x) - row * p.nsum, j = js * kScanWaves + wave;
@@ -70,65 +129,57 @@ __global__ __launch_bounds__(64 * kScanWaves) void beam_scan_kernel(SelectParams
   const int b = row / p.beams, w = row - b * p.beams;
   const T* x = static_cast<const T*>(p.x) + b * p.group_stride + w * p.beam_stride + static_cast<int64_t>(j) * kSeg;
   const int n = min(p.vocab - j * kSeg, kSeg);
-  float v[NV][E];
+  float v[NV * E];
   if (n == kSeg) {
     T raw[NV][E];
 #pragma unroll
     for (int i = 0; i < NV; ++i) __builtin_memcpy(raw[i], x + (64 * i + lane) * E, 16);
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
-#pragma unroll
-      for (int e = 0; e < E; ++e) v[i][e] = to_f32(raw[i][e]);
+    for (int i = 0; i < NV * E; ++i) v[i] = to_f32(raw[i / E][i % E]);
   } else {
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
-#pragma unroll
-      for (int e = 0; e < E; ++e) {
-        const int at = (64 * i + lane) * E + e;
-        v[i][e] = at < n ? to_f32(x[at]) : -INFINITY;
-      }
+    for (int i = 0; i < NV * E; ++i) {
+      const int at = (64 * (i / E) + lane) * E + i % E;
+      v[i] = at < n ? to_f32(x[at]) : -INFINITY;
+    }
   }
   float m = -INFINITY;  // (fmaxf passes NaN over)
 #pragma unroll
-  for (int i = 0; i < NV; ++i)
+  for (int i = 0; i < NV * E; ++i) m = fmaxf(m, v[i]);
+  m = __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(wave_max_dpp(m))));
+  const bool plain = m > -40.0f && m < 80.0f;
+  double s = 0.0;
+  if (plain) s = sum_of_exps(v);
+  if (!plain || __any(!(s < INFINITY))) {  // -inf, the lowest values and NaN leave NaN
+    // from the largest (exact where it counts: no logit within 40 of it is nearer to 0 than
+    // to it), what is lower by 85 and NaN as 85 lower: nothing; infinities are 0 apart
+    const float from = plain ? 0.0f : m;
 #pragma unroll
-    for (int e = 0; e < E; ++e) m = fmaxf(m, v[i][e]);
-  m = wave_max_dpp(m);
-  float s = 0.0f;
-#pragma unroll
-  for (int i = 0; i < NV; ++i)
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const float d = v[i][e] - m;
-      s += fast_exp2(fmaf(d, kLog2eLo, d * kLog2eHi));
-    }
-  if (__any(!(s < INFINITY))) {
-    // NaN counts as -inf, and of infinities the equal ones are 0 apart
-    s = 0.0f;
-#pragma unroll
-    for (int i = 0; i < NV; ++i)
-#pragma unroll
-      for (int e = 0; e < E; ++e) {
-        const float d = v[i][e] - m;
-        s += v[i][e] == m ? (m > -INFINITY ? 1.0f : 0.0f) : d < 0.0f ? fast_exp2(fmaf(d, kLog2eLo, d * kLog2eHi)) : 0.0f;
-      }
+    for (int i = 0; i < NV * E; ++i) v[i] = fmaxf(v[i] == from ? 0.0f : v[i] - from, -85.0f);
+    s = m > -INFINITY ? sum_of_exps(v) : 0.0;
   }
-  s = group_sum<64>(s);
+  s = sum_of_wave(s);
   if (lane == 0) {
     if (j < p.nseg) p.seg[static_cast<int64_t>(row) * p.nseg + j] = m;
-    part[wave] = make_float2(m, s);
+    part[wave] = ScanSum{m, plain || s == 0.0 ? 0.0f : m, s};
   }
   __syncthreads();
   if (threadIdx.x == 0) {
-    float M = -INFINITY, S = 0.0f;
+    ScanSum all = part[0];
+    bool alike = all.ref == 0.0f;
 #pragma unroll
-    for (int i = 0; i < kScanWaves; ++i) M = fmaxf(M, part[i].x);
-#pragma unroll
-    for (int i = 0; i < kScanWaves; ++i) {
-      const float d = part[i].x - M;
-      if (part[i].y > 0.0f) S += part[i].y * (part[i].x == M ? 1.0f : fast_exp2(fmaf(d, kLog2eLo, d * kLog2eHi)));
+    for (int i = 1; i < kScanWaves; ++i) {
+      all.most = fmaxf(all.most, part[i].most);
+      all.sum += part[i].sum;
+      alike &= part[i].ref == 0.0f;
     }
-    p.sum[static_cast<int64_t>(row) * p.nsum + js] = make_float2(M, S);
+    if (!alike) {
+      all.ref = all.most;
+      all.sum = 0.0;
+#pragma unroll 1
+      for (int i = 0; i < kScanWaves; ++i) all.sum += exp_from(part[i], all.most);
+    }
+    p.sum[static_cast<int64_t>(row) * p.nsum + js] = all;
   }
 }
 
@@ -284,22 +335,21 @@ __global__ __launch_bounds__(kPick) void beam_pick_kernel(SelectParams p) {
   for (int i = 0; i < kSegs; ++i) ahead[i] = seg[min(static_cast<int>(threadIdx.x) + i * kPick, W * nseg - 1)];
 #pragma unroll 1
   for (int w = wave; w < W; w += kPick / 64) {
-    const float2* sum = p.sum + static_cast<int64_t>(b * W + w) * p.nsum;
-    const float2 mine = lane < p.nsum ? sum[lane] : make_float2(-INFINITY, 0.0f);  // (unwritten where nobody needs it)
+    const ScanSum* sum = p.sum + static_cast<int64_t>(b * W + w) * p.nsum;
+    const ScanSum mine = lane < p.nsum ? sum[lane] : ScanSum{-INFINITY, 0.0f, 0.0};  // (unwritten where nobody needs it)
     const float score = p.scores[b * W + w];
     const bool done = p.finished && p.finished[b * W + w];
     const int st = !beam_alive(score) ? 0 : done ? 2 : 1;
     double c = score;
     float m = -INFINITY;
     if (st == 1) {
-      m = mine.x;
+      m = mine.most;
 #pragma unroll 1
-      for (int j = lane + 64; j < p.nsum; j += 64) m = fmaxf(m, sum[j].x);
+      for (int j = lane + 64; j < p.nsum; j += 64) m = fmaxf(m, sum[j].most);
       m = wave_max_dpp(m);
-      const auto part = [&](float2 v) { return !(v.y > 0.0f) ? 0.0 : v.y * (v.x == m ? 1.0 : exp(static_cast<double>(v.x) - static_cast<double>(m))); };
       double s = 0.0;
 #pragma unroll 1
-      for (int j = lane; j < p.nsum; j += 64) s += part(j == lane ? mine : sum[j]);
+      for (int j = lane; j < p.nsum; j += 64) s += exp_from(j == lane ? mine : sum[j], m);
 #pragma unroll
       for (int d = 1; d < 64; d <<= 1) s += __shfl_xor(s, d, 64);
       c -= log(s);
@@ -669,7 +719,7 @@ using namespace tq;
 
 extern "C" size_t tq_beam_select_workspace_size(int groups, int beams, int vocab) {
   if (groups < 1 || beams < 1 || vocab < 1) return 0;
-  return static_cast<size_t>(groups) * beams * (sizeof(float2) * sums(vocab) + sizeof(float) * segments(vocab));
+  return static_cast<size_t>(groups) * beams * (sizeof(ScanSum) * sums(vocab) + sizeof(float) * segments(vocab));
 }
 
 extern "C" int tq_beam_select(const void* logits, tq_dtype x_dtype, int64_t group_stride, int64_t beam_stride,
@@ -697,7 +747,7 @@ extern "C" int tq_beam_select(const void* logits, tq_dtype x_dtype, int64_t grou
   const int nseg = segments(vocab);
   // (a launch has fewer than 2^32 threads)
   TQ_CHECK_ARG(static_cast<int64_t>(groups) * beams * sums(vocab) < (int64_t{1} << 32) / (64 * kScanWaves), "%s: logits too large", fn);
-  float2* sum = static_cast<float2*>(workspace);
+  ScanSum* sum = static_cast<ScanSum*>(workspace);
   SelectParams p{logits, group_stride, beam_stride, scores, finished, groups, beams, vocab, num_out, pad_token, nseg,
                  sums(vocab), sum, reinterpret_cast<float*>(sum + static_cast<size_t>(groups) * beams * sums(vocab)),
                  scores_out, parents_out, tokens_out};

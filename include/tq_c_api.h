@@ -469,9 +469,10 @@ int tq_kv_pages_copy(void* const* pages, tq_dtype sb_dtype, int num_layers, int 
  *   scores_out f32, parents_out, tokens_out int32 [groups, num_out], DEVICE, best
  *   first: the total, g * beams + w, and t; -inf, -1, -1 where there are fewer
  *   candidates.  They overlap no input.
- * 1 <= beams, num_out <= 64; vocab <= 2^24.  Sums of exponentials are held in 32 bits
- * within 4,096 tokens and in 64 beyond; totals are compared in 64.  A beam's tokens are in
- * exact order; totals of two beams that differ by less than about 1e-7 may change places.
+ * 1 <= beams, num_out <= 64; vocab <= 2^24.  Exponentials and sums of 16 of them are held
+ * in 32 bits, longer sums and totals in 64: a beam's totals are off by 3.6e-7 at most (3e-8
+ * as a rule), all alike.  Its tokens are in exact order; totals of two beams that differ
+ * by less than twice that may change places.
  * workspace: tq_beam_select_workspace_size(...) bytes, 16-byte aligned; need not be
  * zeroed; calls that may overlap need one each. */
 size_t tq_beam_select_workspace_size(int groups, int beams, int vocab);
