@@ -366,8 +366,9 @@ extern "C" size_t tq_sdpa_int4_paged_chunks_workspace_size(int batch, int querie
     return 0;
   // (a window only takes keys away; where it leaves so few that nothing is split, none)
   size_t most = 0;
-  for (bool all32 : {false, true}) {
-    const ChunksPlan pl = plan_chunks(batch, queries, num_heads / num_kv_heads, num_kv_heads, head_dim, max_new, max_kv_len, 0, 0, all32);
+  for (int wide : {0, 1, 3}) {  // of the queries (1), and the scales
+    const ChunksPlan pl = plan_chunks(batch, queries, num_heads / num_kv_heads, num_kv_heads, head_dim, max_new, max_kv_len,
+                                      0, 0, (wide & 1) != 0, (wide & 2) != 0);
     if (pl.tiles.slots + pl.few_rows.slots > 0) most = std::max(most, chunks_layout(pl, head_dim).total);
   }
   return most;
@@ -399,7 +400,7 @@ extern "C" int tq_sdpa_int4_paged_chunks(const void* q, tq_dtype q_dtype, const 
   p.seq_lens = seq_lens;
   p.n_clamp = max_kv_len;
   const ChunksPlan plan = plan_chunks(batch, queries, gqa_factor, num_kv_heads, head_dim, max_new, max_kv_len,
-                                      sliding_window, num_sinks, q_dtype == TQ_F32 && sb_dtype == TQ_F32);
+                                      sliding_window, num_sinks, q_dtype == TQ_F32, sb_dtype == TQ_F32);
   TQ_CHECK_ARG(chunk_threads(plan, head_dim) < (int64_t{1} << 32), "%s: grid too large", fn);
   PagedParams few = p;
   if (plan.tiles.slots + plan.few_rows.slots > 0) {

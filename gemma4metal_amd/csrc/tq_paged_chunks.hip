@@ -12,11 +12,19 @@ namespace tq {
 namespace {
 
 // Rows of a sequence up to which it is one of few.  In us, this kernel against the tile
-// kernel, 32 sequences of 300 to 6,000 keys, bf16 queries: D 256 (Hkv 16, window 1,024) of
-// 24 rows 99 : 132, 48 rows 139 : 146, 64 rows 176 : 165; D 128 (Hkv 8) of 32 rows 90 :
-// 162, 64 rows 141 : 184, 128 rows 252 : 263; D 512 (Hkv 4) of 16 rows 158 : 209, 32 rows
-// 302 : 221.
-constexpr int few_rows(int D) { return D == 512 ? 16 : D == 256 ? 48 : 128; }
+// kernel, 32 sequences of 300 to 6,000 keys, bf16 queries and fp16 scales / fp32 queries /
+// fp32 scales / both:
+// D 128 (Hkv 8)  64 rows 144 : 169 / 150 : 181 / 148 : 187 / 157 : 194
+//               128 rows 257 : 259 / 264 : 280 / 258 : 285 / 267 : 299
+// D 256 (Hkv 16, window 1,024)
+//                32 rows  93 : 124 / 123 : 133 / 109 : 129 / 146 : 154
+//                48 rows 129 : 132 / 176 : 142 / 155 : 138 / 208 : 163
+//                64 rows 167 : 137
+// D 512 (Hkv 4)  16 rows 144 : 209 / 209 : 230 / 186 : 225 / 239 : 256
+//                24 rows 284 : 216 / 403 : 237 / 353 : 232 / 456 : 263
+// (fp32 queries are twice the operands, and fp32 scales twice the words, of registers that
+// D 256 and 512 do not have: 19 to 79 and 95 to 208 of them are spilled.)
+constexpr int few_rows(int D, bool wide) { return D == 512 ? 16 : D == 256 ? (wide ? 32 : 48) : 128; }
 template <int D, bool F32, bool Q32>
 __global__ __launch_bounds__((FewGeom<D, F32>::NT)) __attribute__((amdgpu_waves_per_eu(D == 512 ? 1 : 2, D == 512 ? 1 : 2)))
 void paged_few_kernel(TileParams p) {
@@ -129,20 +137,21 @@ int64_t few_cus(int D) { return D == 512 ? target_wgs() : 2 * target_wgs(); }
 }  // namespace
 
 ChunksPlan plan_chunks(int batch, int queries, int gqa, int Hkv, int D, int max_new, int64_t max_kv_len, int64_t window,
-                       int64_t sinks, bool all32) {
+                       int64_t sinks, bool q32, bool s32) {
   ChunksPlan pl{};
+  const int few = few_rows(D, q32 || s32);
   const int64_t rows = static_cast<int64_t>(std::min(max_new, queries)) * gqa, all = static_cast<int64_t>(queries) * gqa;
   const int64_t seqs = std::min(batch, queries);
   // keys of a block of R rows at most, in whole tiles of either kernel (no fewer than chunk_seq counts)
   const auto keys = [&](int64_t R) {
     return window > 0 ? std::min<int64_t>(max_kv_len, window + R + 256 + (sinks + 63) / 64 * 64) : max_kv_len;
   };
-  pl.rs = D == 512 || (D == 256 && all32) || rows <= 64 ? 4 : 8;
+  pl.rs = D == 512 || (D == 256 && q32 && s32) || rows <= 64 ? 4 : 8;
   // sequences of few rows alone, or a batch that may hold some, or none.  (Us without and
   // with them apart, D 256: 3 chunks of 1,000 among 24 sequences 686, 549; 2 of 700 and 6 of
   // 300, none of them few, 207, 209.  At D 512, where a launch of its own without work takes
   // up to 10, only where chunks are short on average.)
-  pl.few = rows <= few_rows(D) ? INT_MAX : batch > 1 && (D < 512 || all / batch < 4 * few_rows(D)) ? few_rows(D) : 0;
+  pl.few = rows <= few ? INT_MAX : batch > 1 && (D < 512 || all / batch < 4 * few) ? few : 0;
   // blocks of rows of any chunks that add up to `queries`
   if (pl.few != INT_MAX) {
     const int64_t n = std::min(seqs, all / (pl.few + 1)), R = 16 * pl.rs;

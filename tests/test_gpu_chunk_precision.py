@@ -35,6 +35,23 @@ def test_every_form(pg, Hq, Hkv, new, lens, D, sb, qt):
             within(got[mine], ref, TILES, f"sequence {b}, dims from {g}", slice(g, g + 64))
 
 
+@pytest.mark.parametrize("sb,qt", [("f16", "bf16"), ("f16", "f32"), ("f32", "bf16"), ("f32", "f32")])
+@pytest.mark.parametrize("D,rows", [(128, 128), (256, 32), (256, 48), (512, 16)])
+def test_around_the_limits_of_few_rows(pg, D, rows, sb, qt):
+    """Sequences of as many rows as the kernels part at, two more and two less, alone and
+    side by side, with keys to be split and without."""
+    rng = np.random.default_rng(D + rows)
+    Hq, Hkv, page = 4, 2, 32
+    at = rows // 2
+    for new, lens in (([at - 1], [700]), ([at], [2600]), ([at + 1], [2600]), ([at - 1, at, at + 1, 1], [90, 1500, 2600, 400])):
+        q, qf, pages, tables, starts = batch(rng, new, lens, Hq, Hkv, D, page, sb, qt)
+        got = run(pg, q, pages, tables, starts, lens, 2, D**-0.5, max_new=max(new), max_kv_len=max(lens))
+        for b, L in enumerate(lens):
+            mine = slice(starts[b], starts[b + 1])
+            ref = definition(qf[mine], pages, tables[b], range(L - new[b] + 1, L + 1), page, 2, D**-0.5)
+            within(got[mine], ref, TILES, f"{new}: sequence {b}")
+
+
 LOG2E = 1.4426950408889634
 
 # (score in powers of two below the last keys', factor of the V scales and biases) of 128
