@@ -335,6 +335,12 @@ extern "C" int tq_sdpa_int4_paged_prefill(const void* q, tq_dtype q_dtype, const
 
 namespace {
 
+// Sequences of a launch.  A job is found by a pass over them all, a wave's 64 at a time, and
+// splits by up to six more: us a sequence of calls of 64, 1,024, 2,048 and 4,096 sequences
+// (Hkv 8 D 128, up to 6,000 keys), one token 1.5, 1.0, 1.1, 1.3, 40 tokens 11.9, 11.5, 13.6,
+// 17.6; it would be the square of them.
+constexpr int kChunkSeqs = 1024;
+
 // The partials of a batch's split blocks, behind the counters that other calls keep
 // zeroed in the same workspace.
 struct ChunksLayout {
@@ -366,11 +372,13 @@ extern "C" size_t tq_sdpa_int4_paged_chunks_workspace_size(int batch, int querie
     return 0;
   // (a window only takes keys away; where it leaves so few that nothing is split, none)
   size_t most = 0;
-  for (int wide : {0, 1, 3}) {  // of the queries (1), and the scales
-    const ChunksPlan pl = plan_chunks(batch, queries, num_heads / num_kv_heads, num_kv_heads, head_dim, max_new, max_kv_len,
-                                      0, 0, (wide & 1) != 0, (wide & 2) != 0);
-    if (pl.tiles.slots + pl.few_rows.slots > 0) most = std::max(most, chunks_layout(pl, head_dim).total);
-  }
+  for (int seqs : {std::min(batch, kChunkSeqs), batch % kChunkSeqs})
+    for (int wide : {0, 1, 3}) {  // of the queries (1), and the scales
+      if (seqs == 0) continue;
+      const ChunksPlan pl = plan_chunks(seqs, batch, queries, num_heads / num_kv_heads, num_kv_heads, head_dim, max_new,
+                                        max_kv_len, 0, 0, (wide & 1) != 0, (wide & 2) != 0);
+      if (pl.tiles.slots + pl.few_rows.slots > 0) most = std::max(most, chunks_layout(pl, head_dim).total);
+    }
   return most;
 }
 
@@ -397,24 +405,40 @@ extern "C" int tq_sdpa_int4_paged_chunks(const void* q, tq_dtype q_dtype, const 
   TQ_CHECK_ARG(max_kv_len >= 0 && max_kv_len <= max_pages * page_size,
                "%s: need 0 <= max_kv_len <= max_pages * page_size (got %d, %d)", fn, max_kv_len, max_pages * page_size);
   TQ_CHECK_ARG(static_cast<int64_t>(queries) * num_heads < (int64_t{1} << 30), "%s: too many queries", fn);
-  p.seq_lens = seq_lens;
   p.n_clamp = max_kv_len;
-  const ChunksPlan plan = plan_chunks(batch, queries, gqa_factor, num_kv_heads, head_dim, max_new, max_kv_len,
-                                      sliding_window, num_sinks, q_dtype == TQ_F32, sb_dtype == TQ_F32);
-  TQ_CHECK_ARG(chunk_threads(plan, head_dim) < (int64_t{1} << 32), "%s: grid too large", fn);
-  PagedParams few = p;
-  if (plan.tiles.slots + plan.few_rows.slots > 0) {
-    const ChunksLayout wl = chunks_layout(plan, head_dim);
-    if (!workspace || workspace_bytes < wl.total) {
-      set_error("%s: workspace of %zu bytes needed (got %zu)", fn, wl.total, workspace ? workspace_bytes : size_t{0});
+  const auto plan_of = [&](int seqs) {
+    return plan_chunks(seqs, batch, queries, gqa_factor, num_kv_heads, head_dim, max_new, max_kv_len, sliding_window,
+                       num_sinks, q_dtype == TQ_F32, sb_dtype == TQ_F32);
+  };
+  // (all checks before the first launch)
+  for (int seqs : {std::min(batch, kChunkSeqs), batch % kChunkSeqs}) {
+    if (seqs == 0) continue;
+    const ChunksPlan plan = plan_of(seqs);
+    TQ_CHECK_ARG(chunk_threads(plan, head_dim) < (int64_t{1} << 32), "%s: grid too large", fn);
+    if (plan.tiles.slots + plan.few_rows.slots == 0) continue;
+    const size_t need = chunks_layout(plan, head_dim).total;
+    if (!workspace || workspace_bytes < need) {
+      set_error("%s: workspace of %zu bytes needed (got %zu)", fn, need, workspace ? workspace_bytes : size_t{0});
       return TQ_ERR_WORKSPACE;
     }
     TQ_CHECK_ARG(reinterpret_cast<uintptr_t>(workspace) % 16 == 0, "%s: workspace must be 16-byte aligned", fn);
-    const auto at = [&](size_t off) { return reinterpret_cast<float*>(static_cast<char*>(workspace) + off); };
-    p.ws_ml = at(wl.ml);
-    p.ws_o = at(wl.o);
-    few.ws_ml = at(wl.few_ml);
-    few.ws_o = at(wl.few_o);
   }
-  return launch_chunks(p, few, head_dim, sb_dtype, plan, starts, queries, max_new, static_cast<hipStream_t>(stream));
+  for (int b0 = 0; b0 < batch; b0 += kChunkSeqs) {  // (one after the other on the stream: one workspace)
+    const ChunksPlan plan = plan_of(std::min(batch - b0, kChunkSeqs));
+    const ChunksLayout wl = chunks_layout(plan, head_dim);
+    const auto at = [&](size_t off) { return reinterpret_cast<float*>(static_cast<char*>(workspace) + off); };
+    PagedParams part = p;
+    part.nq = std::min(batch - b0, kChunkSeqs);
+    part.tables = block_tables + static_cast<int64_t>(b0) * max_pages;
+    part.seq_lens = seq_lens + b0;
+    PagedParams few = part;
+    if (plan.tiles.slots + plan.few_rows.slots > 0) {
+      part.ws_ml = at(wl.ml);
+      part.ws_o = at(wl.o);
+      few.ws_ml = at(wl.few_ml);
+      few.ws_o = at(wl.few_o);
+    }
+    if (int r = launch_chunks(part, few, head_dim, sb_dtype, plan, starts + b0, queries, max_new, static_cast<hipStream_t>(stream))) return r;
+  }
+  return TQ_OK;
 }

@@ -136,7 +136,7 @@ int64_t few_cus(int D) { return D == 512 ? target_wgs() : 2 * target_wgs(); }
 
 }  // namespace
 
-ChunksPlan plan_chunks(int batch, int queries, int gqa, int Hkv, int D, int max_new, int64_t max_kv_len, int64_t window,
+ChunksPlan plan_chunks(int batch, int of, int queries, int gqa, int Hkv, int D, int max_new, int64_t max_kv_len, int64_t window,
                        int64_t sinks, bool q32, bool s32) {
   ChunksPlan pl{};
   const int few = few_rows(D, q32 || s32);
@@ -151,7 +151,7 @@ ChunksPlan plan_chunks(int batch, int queries, int gqa, int Hkv, int D, int max_
   // with them apart, D 256: 3 chunks of 1,000 among 24 sequences 686, 549; 2 of 700 and 6 of
   // 300, none of them few, 207, 209.  At D 512, where a launch of its own without work takes
   // up to 10, only where chunks are short on average.)
-  pl.few = rows <= few ? INT_MAX : batch > 1 && (D < 512 || all / batch < 4 * few) ? few : 0;
+  pl.few = rows <= few ? INT_MAX : batch > 1 && (D < 512 || all / of < 4 * few) ? few : 0;
   // blocks of rows of any chunks that add up to `queries`
   if (pl.few != INT_MAX) {
     const int64_t n = std::min(seqs, all / (pl.few + 1)), R = 16 * pl.rs;

@@ -899,7 +899,8 @@ struct ChunksPlan {
   int rs, few;
   ChunkJobs tiles, few_rows;
 };
-ChunksPlan plan_chunks(int batch, int queries, int gqa, int Hkv, int D, int max_new, int64_t max_kv_len, int64_t window,
+// The jobs of `batch` sequences of `of` that bring `queries` together.
+ChunksPlan plan_chunks(int batch, int of, int queries, int gqa, int Hkv, int D, int max_new, int64_t max_kv_len, int64_t window,
                        int64_t sinks, bool q32, bool s32);
 // Threads of its largest launch (one has fewer than 2^32).
 int64_t chunk_threads(const ChunksPlan& plan, int D);

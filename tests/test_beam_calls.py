@@ -12,8 +12,8 @@ BIG = dict(wb=1 << 60)
     (select(G=1 << 18, W=64, V=100, **BIG), 1, "logits too large"),
     (select(G=1 << 18, W=32, V=4097, **BIG), 1, "logits too large"),
     # few rows alone (256 threads), both kinds (pairs of them behind the tiles' 512)
-    (chunks(B=65535, N=65535 * 16, Hq=257, Hkv=257, gqa=1, new=16), 1, "grid too large"),
-    (chunks(B=65535, N=65535 * 100, Hq=64, Hkv=64, gqa=1, new=300), 1, "grid too large"),
+    (chunks(B=1024, N=1 << 17, Hq=2049, Hkv=2049, gqa=1, new=128), 1, "grid too large"),
+    (chunks(B=1024, N=300 * 1024, Hq=1171, Hkv=1171, gqa=1, new=300), 1, "grid too large"),
     (chunks(B=1, N=(1 << 22) - 1, Hq=255, Hkv=255, gqa=1, new=(1 << 22) - 1, D=512), 1, "grid too large"),
 ])
 def test_grids_that_cannot_be_launched(call, status, needle):

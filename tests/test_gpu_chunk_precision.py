@@ -4,7 +4,10 @@ import numpy as np
 import pytest
 import torch
 
+from oracle import paged as OP
+from tests.gpu_util import dev, host
 from tests.test_gpu_chunks import batch, run
+from tests.test_gpu_paged import close, ints
 from tests.test_gpu_paged_calls import TILES, definition, within
 
 pytestmark = pytest.mark.gpu
@@ -99,3 +102,37 @@ def test_keys_that_fade_leave_no_rounding(pg, D, new, sb, qt, fade):
     assert np.isfinite(got).all()
     if rows.any():
         within(got[rows], [ref[0][rows], ref[1][rows]], tol, f"{steps}")
+
+
+@pytest.mark.parametrize("D,B", [(128, 1024), (128, 1025), (512, 2100), (256, 3000)])
+def test_batches_of_several_launches(pg, D, B):
+    """More sequences than a launch takes: chunks of either kind in all of them, a last
+    launch whose keys are split, empty sequences, rows behind the last chunk; in a graph."""
+    rng = np.random.default_rng(B)
+    Hq, Hkv, page = 2, 1, 32
+    new = rng.integers(0, 3, B)
+    new[[3, B // 2, B - 1]] = [70, 140, 5]
+    prior = rng.integers(0, 60, B)
+    prior[[3, B - 1]] = [2500, 2600]
+    lens = (new + prior).tolist()
+    q, qf, pages, tables, starts = batch(rng, new.tolist(), lens, Hq, Hkv, D, page)
+    extra = torch.cat([q, q[:3]])
+    args = [extra, *[dev(p) for p in pages], dev(tables), ints(starts), ints(lens), 2, D**-0.5]
+    out = torch.full(extra.shape, 7.0, device="cuda")
+    kw = dict(max_new=140, max_kv_len=max(lens), out=out)
+    s = torch.cuda.Stream()
+    with torch.cuda.stream(s):
+        pg.sdpa_int4_paged_chunks(*args, **kw)
+    s.synchronize()
+    first = host(out)
+    ref = OP.sdpa_int4_paged_chunks(qf, pages, tables, starts, lens, page, 2, D**-0.5)
+    close(first[:starts[-1]], ref)
+    assert (first[starts[-1]:] == 7).all()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=s):
+        pg.sdpa_int4_paged_chunks(*args, **kw)
+    for _ in range(3):
+        out.fill_(7.0)
+        g.replay()
+        torch.cuda.synchronize()
+        assert np.array_equal(host(out), first)
