@@ -492,38 +492,9 @@ struct ReorderParams {
   int* to;
 };
 
-__device__ __forceinline__ int parent_of(const int32_t* parents, int s, int seqs) {
-  const int q = parents[s];
-  return static_cast<unsigned>(q) < static_cast<unsigned>(seqs) ? q : -1;
-}
-
 // Tiles of one head of n rows, tensor by tensor.
 __device__ __forceinline__ int tiles_of(const ReorderParams& p, int a, int n) {
   return static_cast<int>((static_cast<int64_t>(n) * p.row_bytes[a] + 16 * kTileUnits - 1) / (16 * kTileUnits));
-}
-
-// Exclusive prefix over the workgroup's N threads, and the total.
-template <int N>
-__device__ __forceinline__ int plan_scan(int v, int* lds, int& total) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  int x = v;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const int y = __shfl_up(x, d, 64);
-    if (lane >= d) x += y;
-  }
-  __syncthreads();  // the last call's readers are done
-  if (lane == 63) lds[wave] = x;
-  __syncthreads();
-  int before = 0;
-  total = 0;
-#pragma unroll
-  for (int w = 0; w < N / 64; ++w) {
-    const int t = lds[w];
-    before += w < wave ? t : 0;
-    total += t;
-  }
-  return before + x - v;
 }
 
 // One thread a sequence, of N at most; lengths become the parents'.  What bounds it: a
@@ -576,13 +547,13 @@ __global__ __launch_bounds__(N) void kv_reorder_plan_kernel(ReorderParams p) {
   __syncthreads();
   const bool comp = nf[s] > 0;  // of the component's lowest sequence
   int comps, parents, children, tiles;
-  const int c = plan_scan<N>(comp, lds, comps);
-  const int from0 = plan_scan<N>(nf[s], lds, parents);
-  const int to0 = plan_scan<N>(gives ? kids[s] : 0, lds, children);
+  const int c = wg_scan<N, int>(comp, lds, comps);
+  const int from0 = wg_scan<N>(nf[s], lds, parents);
+  const int to0 = wg_scan<N>(gives ? kids[s] : 0, lds, children);
   int n = 0;
 #pragma unroll
   for (int a = 0; a < 6; ++a) n += comp ? tiles_of(p, a, most[s]) : 0;
-  const int tile0 = plan_scan<N>(n * p.heads, lds, tiles);
+  const int tile0 = wg_scan<N>(n * p.heads, lds, tiles);
   first[s] = from0;
   if (comp) p.comps[c] = ReorderComp{from0, nf[s], most[s], tile0};
   if (s == 0) {

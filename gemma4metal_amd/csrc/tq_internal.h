@@ -198,6 +198,36 @@ __device__ __forceinline__ int wave_sum_dpp(int v) {
   return xor32_sum(xor16_sum(v));
 }
 
+// Exclusive prefix of v over the N threads of a workgroup, and their total; lds: N / 64 of T.
+template <int N, typename T>
+__device__ __forceinline__ T wg_scan(T v, T* lds, T& total) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  T x = v;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const T y = __shfl_up(x, d, 64);
+    if (lane >= d) x += y;
+  }
+  __syncthreads();  // the last call's readers are done
+  if (lane == 63) lds[wave] = x;
+  __syncthreads();
+  T before = 0;
+  total = 0;
+#pragma unroll
+  for (int w = 0; w < N / 64; ++w) {
+    const T t = lds[w];
+    before += w < wave ? t : 0;
+    total += t;
+  }
+  return before + x - v;
+}
+
+// The sequence that s continues in a reordering of `seqs`, -1: none.
+__device__ __forceinline__ int parent_of(const int32_t* parents, int s, int seqs) {
+  const int q = parents[s];
+  return static_cast<unsigned>(q) < static_cast<unsigned>(seqs) ? q : -1;
+}
+
 // exp2 with -inf handled (v_exp_f32 returns 0 for -inf already; kept explicit).
 __device__ __forceinline__ float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 

@@ -49,30 +49,6 @@ PlanWs plan_ws(void* ws, int64_t seqs, int64_t pages) {
   return w;
 }
 
-// Exclusive prefix of v over the workgroup's threads, and their total.
-template <typename T>
-__device__ __forceinline__ T wg_scan(T v, T* lds, T& total) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  T x = v;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const T y = __shfl_up(x, d, 64);
-    if (lane >= d) x += y;
-  }
-  __syncthreads();  // the last call's readers are done
-  if (lane == 63) lds[wave] = x;
-  __syncthreads();
-  T before = 0;
-  total = 0;
-#pragma unroll
-  for (int w = 0; w < kPlanWaves; ++w) {
-    const T t = lds[w];
-    before += w < wave ? t : 0;
-    total += t;
-  }
-  return before + x - v;
-}
-
 struct PlanParams {
   int32_t* tables;
   int32_t* refs;
@@ -98,7 +74,7 @@ __device__ __forceinline__ int free_pages(const int32_t* refs, int num_pages, in
       n += f[i];
     }
     int total;
-    int at = found + wg_scan(n, lds, total);
+    int at = found + wg_scan<kPlanThreads>(n, lds, total);
 #pragma unroll
     for (int i = 0; i < kScanPer; ++i)
       if (f[i]) list[at++] = p + i;
@@ -157,7 +133,7 @@ __global__ __launch_bounds__(kPlanThreads) void pages_plan_kernel(PlanParams p) 
   for (int s0 = 0; s0 < p.seqs; s0 += kPlanThreads) {
     const int s = s0 + threadIdx.x;
     ScanSum total;
-    const ScanSum b = wg_scan<ScanSum>(s < p.seqs ? max(p.w.need[s], 0) : 0, sums, total);
+    const ScanSum b = wg_scan<kPlanThreads, ScanSum>(s < p.seqs ? max(p.w.need[s], 0) : 0, sums, total);
     if (s < p.seqs) p.w.before[s] = plan_before(want + b, p.num_pages);
     want += total;
   }
@@ -208,10 +184,6 @@ struct RolesParams {
   int32_t* saved;  // rows of parents, by parent, as they were
 };
 
-__device__ __forceinline__ int parent_of(const int32_t* parents, int s, int seqs) {
-  const int q = parents[s];
-  return static_cast<unsigned>(q) < static_cast<unsigned>(seqs) ? q : -1;
-}
 __device__ __forceinline__ int rows_of(const PlanParams& p, int s) {
   return static_cast<int>(min(static_cast<int64_t>(max(p.lengths[s], 0)), static_cast<int64_t>(p.max_pages) * p.page_size));
 }
@@ -302,7 +274,7 @@ __global__ __launch_bounds__(kPlanThreads) void pages_reorder_plan_kernel(RolesP
       p.w.need[s] = need;
     }
     int total;
-    const int b = wg_scan(max(need, 0), sums, total);
+    const int b = wg_scan<kPlanThreads>(max(need, 0), sums, total);
     if (s < p.seqs) p.w.before[s] = plan_before(static_cast<PlanSum>(want) + b, p.num_pages);
     want += total;
   }
@@ -335,7 +307,7 @@ __global__ __launch_bounds__(kPlanThreads) void pages_compact_plan_kernel(Compac
   __shared__ int lds[kPlanWaves];
   int mine = 0, live;
   for (int i = threadIdx.x; i < p.num_pages; i += kPlanThreads) mine += p.refs[i] > 0;
-  wg_scan(mine, lds, live);
+  wg_scan<kPlanThreads>(mine, lds, live);
   int* hole = p.w.list;
   int n_hole = 0, n_move = 0;
   for (int p0 = 0; p0 < p.num_pages; p0 += kScanTile) {  // uniform
@@ -351,7 +323,7 @@ __global__ __launch_bounds__(kPlanThreads) void pages_compact_plan_kernel(Compac
       n += kind[i];
     }
     int total;
-    const int b = wg_scan(n, lds, total);
+    const int b = wg_scan<kPlanThreads>(n, lds, total);
     int h = n_hole + (b & 0xFFFF), m = n_move + (b >> 16);
 #pragma unroll
     for (int i = 0; i < kScanPer; ++i) {
