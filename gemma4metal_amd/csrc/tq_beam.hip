@@ -116,8 +116,9 @@ __device__ __forceinline__ double sum_of_exps(const float (&x)[N]) {
 // give equal sums.  Logits of ordinary size are taken as they are (ref 0), so that segments
 // add up without a common reference.  More than a lane's 16 terms are added in 64 bits.
 //
-// What bounds it: HBM (248 rows of 262,144 bf16 tokens 28 us, 4.6 TB/s, where a large copy
-// reaches 5.1; VALU 75%).
+// What bounds it: VALU (87%) beside HBM (248 rows of 262,144 bf16 tokens 30 us, 4.3 TB/s, where
+// a large copy reaches 5.1; 28 without the corrections, 35 with the exponent split off by
+// adding 1.5 2^23 and one reference for four segments).
 template <typename T>
 __global__ __launch_bounds__(64 * kScanWaves) void beam_scan_kernel(SelectParams p) {
   constexpr int E = 16 / sizeof(T), NV = kSeg / (64 * E);
@@ -316,7 +317,7 @@ __device__ __forceinline__ int pick(PickLds& L, int n, int K, float most, F abou
 
 // The choice of one group.  What bounds it: latency (a round trip to the segments'
 // statistics, one to the chosen segments, and the barriers of two choices): 8 us of 4
-// beams of 32,000 tokens, 10.5 of 32 groups of 8 beams of 262,144, 13.6 with 10 places.
+// beams of 32,000 tokens, 10.7 of 32 groups of 8 beams of 262,144, 13.7 with 10 places.
 // HELD: chosen segments that a thread holds its tokens of.
 template <typename T, int HELD>
 __global__ __launch_bounds__(kPick) void beam_pick_kernel(SelectParams p) {

@@ -13,8 +13,8 @@
 // with every new reference 54).
 // What bounds it: VALU (about 700 instructions a wave and block at D 256, 61% of a SIMD's
 // cycles with two waves) and the start and end of a job (about 9 us).  5 new tokens
-// of 32 sequences behind a window of 1,024 (Hq 32 Hkv 16 D 256): 50 us, 3.0 TB/s of what
-// has to be read, where the tile kernel takes 121.  Measured, not kept: workgroups of eight
+// of 32 sequences behind a window of 1,024 (Hq 32 Hkv 16 D 256): 52 us, 2.9 TB/s of what
+// has to be read, where the tile kernel takes 114.  Measured, not kept: workgroups of eight
 // waves, one a CU, 69; V's operands read ahead of the softmax 60 (spills); nibbles as fp16
 // subnormals, uncentred, for K 51 against 55, but errors of 3e-6 to 5e-6 in place of 0.5e-6.
 #pragma once
