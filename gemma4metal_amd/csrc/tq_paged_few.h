@@ -8,9 +8,8 @@
 // its sums carry too.  It falls where a weight would pass fp16 and rises where a row with a
 // p of about 1 (its largest is that or more) has no weight of 1 or more, so that no range of
 // V scales needs a path beside this one: fp16's last step is 2^-24, and what is rounded off a
-// weight is 2^-25 of the row's sums at most.  Both in branches that equal scales hardly take
-// (with the rise's part inside the other's: 49.4 -> 50.2 us of the 5 tokens below; a rise
-// with every new reference 54).
+// weight is 2^-25 of the row's sums at most.  (5 tokens as below: 49.4 us without the rise,
+// 50.2 with it in a branch of the other's, 54 with a rise at every new reference.)
 // What bounds it: VALU (about 700 instructions a wave and block at D 256, 61% of a SIMD's
 // cycles with two waves) and the start and end of a job (about 9 us).  5 new tokens
 // of 32 sequences behind a window of 1,024 (Hq 32 Hkv 16 D 256): 52 us, 2.9 TB/s of what
